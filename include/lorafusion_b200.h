@@ -459,9 +459,129 @@ LF_API int lf_assign_rows(const int32_t* bin_start, const int32_t* entry_adapter
                           int32_t n_bins, int32_t world_size, int32_t granule_rows, int32_t max_ranges,
                           int64_t* range_start, int64_t* range_end, int32_t* range_rank, int32_t* n_ranges);
 
+/* ------------------------------------------------------------------------------------------------
+ * Serving: rows in any order, each with the adapter a device-side index names.
+ * No counterpart in the reference (its batches are packed into contiguous routes on the host).
+ */
+
+/* Largest padded rank of an adapter bank. */
+#define LF_BANK_MAX_RANK 128
+
+/* One projection and a bank of resident adapters.  `slot_rank_dev` holds each slot's rank (0: empty
+ * slot, its rows get the shared projection alone), at most r_pad; bank entries past it must be zero. */
+typedef struct lf_rows_problem {
+  int32_t dtype;             /* lf_dtype of x, W, y and the bank */
+  int32_t T, K, N;           /* rows, in_features, out_features */
+  int32_t n_slots, r_pad;    /* slots of the bank; its padded rank: 16, 32, 64 or 128 */
+  int32_t row_slot_bytes;    /* bytes of one row_slot entry: 4 or 8 (signed) */
+  int32_t reserved;
+  int64_t ldx;               /* elements from one row of x to the next, at least K */
+  const void* x_dev;         /* [T] rows of K */
+  const void* w_dev;         /* [N,K] */
+  const void* a_bank_dev;    /* [n_slots, r_pad, K] */
+  const void* b_bank_dev;    /* [n_slots, N, r_pad] */
+  const int32_t* slot_rank_dev;  /* [n_slots] */
+  const float* slot_scale_dev;   /* [n_slots] s_i */
+  const void* row_slot_dev;  /* [T] slot of each row; negative: no adapter */
+} lf_rows_problem;
+
+/* Workspace bytes of lf_rows_forward (256-byte aligned buffer). */
+LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t r_pad, int32_t dtype);
+
+/*
+ * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense.  row_slot is read on
+ * the device, so a captured call follows later changes of it and of the bank's contents.  A
+ * slot at or above n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
+ * bf16/f16 with K, N and ldx multiples of 8 and 16-byte aligned buffers run on the tensor cores, other
+ * problems on CUDA cores.  Enqueued on `stream` (2 launches); never synchronizes.
+ */
+LF_API int lf_rows_forward(const lf_rows_problem* prob, void* y_dev, void* workspace_dev, size_t workspace_bytes,
+                           lf_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------------
+ * Training: gradient norms, clipping and AdamW of many adapters.  No counterpart in the reference
+ * (it has no optimizer).
+ */
+
+/* One gradient tensor (dense). */
+typedef struct lf_grad_tensor {
+  uint64_t ptr;    /* device address */
+  uint64_t numel;  /* below 2^32 - 8192 */
+  int32_t dtype;   /* lf_dtype */
+  int32_t group;   /* the adapter it belongs to, 0 .. n_groups - 1 */
+} lf_grad_tensor;
+
+/* Workspace bytes of lf_grad_clip (0 on bad arguments). */
+LF_API size_t lf_grad_clip_workspace_bytes(const lf_grad_tensor* tensors, int32_t n_tensors, int32_t n_groups);
+
+/*
+ * norms[g] = sqrt(sum g^2) over every tensor of group g (inf_norm: the largest |g|), float32, summed
+ * in float64 in a fixed order; then, with `scale`, every gradient of the group times
+ * min(1, max_norm / (norm + 1e-6)), in place, rounded once.  A group without tensors has norm 0.
+ * `tensors` is host memory, read before the call returns (its addresses travel in the launches'
+ * parameters, so a captured call needs nothing else).  Tensors that share memory are refused when
+ * scaling.  3 launches for up to 1500 tensors, never synchronizes.
+ */
+LF_API int lf_grad_clip(const lf_grad_tensor* tensors, int32_t n_tensors, int32_t n_groups, int32_t inf_norm,
+                        int32_t scale, double max_norm, float* norms_dev, void* workspace_dev,
+                        size_t workspace_bytes, lf_stream_t stream);
+
+/* One weight tensor of an AdamW plan; the caller fills param, numel and group, lf_adamw_plan the rest. */
+typedef struct lf_adamw_tensor {
+  uint64_t param;     /* device address of the weight, dense */
+  int64_t state_off;  /* its first element in the state arrays (a multiple of 8) */
+  uint32_t numel;     /* below 2^32 - 8192 */
+  int32_t group;
+  int32_t chunk0;     /* first chunk */
+  int32_t n_chunks;
+} lf_adamw_tensor;
+
+/*
+ * Lay out the state of n_tensors weights (host only): fills every record, *n_chunks and
+ * *state_elems (elements of exp_avg, exp_avg_sq and master each).  chunk_tensor (host, may be null to
+ * learn the sizes) receives the tensor of each chunk; LF_ERR_CAPACITY when max_chunks is too small.
+ * The caller copies records and chunk_tensor to device memory once.
+ */
+LF_API int lf_adamw_plan(lf_adamw_tensor* tensors, int32_t n_tensors, int32_t n_groups, int32_t* chunk_tensor,
+                         int64_t max_chunks, int64_t* n_chunks, int64_t* state_elems);
+
+typedef struct lf_adamw_args {
+  const lf_adamw_tensor* tensors;      /* host records of the plan */
+  const lf_adamw_tensor* tensors_dev;  /* the same on the device */
+  const int32_t* chunk_tensor_dev;
+  const uint64_t* grads;     /* host [n_tensors]: device address of this step's gradient, 0: none */
+  const double* hyper_dev;   /* [n_groups][2] learning rate, weight decay */
+  int32_t* steps_dev;        /* [n_groups] updates made so far */
+  float* exp_avg_dev;
+  float* exp_avg_sq_dev;
+  float* master_dev;         /* float32 weights; null when the weights are float32 themselves */
+  float* norms_dev;          /* [n_groups], or null: no norms */
+  void* workspace_dev;
+  size_t workspace_bytes;    /* lf_adamw_workspace_bytes */
+  int64_t n_chunks;
+  double beta1, beta2, eps;
+  double max_norm;           /* below 0: no clipping */
+  int32_t n_tensors, n_groups;
+  int32_t param_dtype;       /* lf_dtype of every weight */
+  int32_t grad_dtype;        /* LF_F32 or param_dtype */
+  int32_t skip_nonfinite;    /* leave a group whose norm is not finite as it is */
+  int32_t reserved;
+} lf_adamw_args;
+
+LF_API size_t lf_adamw_workspace_bytes(int64_t n_chunks, int32_t n_groups);
+
+/*
+ * One AdamW step of every group that has a gradient: t = ++steps[group], g' = c g with the group's clip
+ * factor c, m = b1 m + (1 - b1) g', v = b2 v + (1 - b2) g'^2,
+ * p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps), in float32 on the master (or
+ * float32) weight; a 16-bit weight is the master rounded.  Tensors without a gradient keep weight and
+ * state.  2 or 3 launches for up to 3840 tensors; never synchronizes.
+ */
+LF_API int lf_adamw_step(const lf_adamw_args* args, lf_stream_t stream);
+
 /*
  * Read and clear the device-side error word (bounded-wait timeouts inside kernels: codes 0x101 ..
- * 0x105).  Synchronizes the current device.  *code = 0 when no kernel reported a problem; after a
+ * 0x105; a row slot out of range: 0x106).  Synchronizes the current device.  *code = 0 when no kernel reported a problem; after a
  * nonzero code the outputs of the calls since the previous read are undefined.
  */
 LF_API int lf_device_error(int32_t* code);

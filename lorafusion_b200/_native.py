@@ -72,6 +72,30 @@ class HostChunk(ctypes.Structure):
                 ("table_dev", ctypes.c_void_p)]
 
 
+class RowsProblem(ctypes.Structure):
+    _fields_ = [("dtype", _c_i32), ("T", _c_i32), ("K", _c_i32), ("N", _c_i32), ("n_slots", _c_i32),
+                ("r_pad", _c_i32), ("row_slot_bytes", _c_i32), ("reserved", _c_i32), ("ldx", ctypes.c_int64),
+                ("x_dev", _c_p), ("w_dev", _c_p), ("a_bank_dev", _c_p), ("b_bank_dev", _c_p),
+                ("slot_rank_dev", _c_p), ("slot_scale_dev", _c_p), ("row_slot_dev", _c_p)]
+
+
+class AdamWArgs(ctypes.Structure):
+    _fields_ = [("tensors", _c_p), ("tensors_dev", _c_p), ("chunk_tensor_dev", _c_p), ("grads", _c_p),
+                ("hyper_dev", _c_p), ("steps_dev", _c_p), ("exp_avg_dev", _c_p), ("exp_avg_sq_dev", _c_p),
+                ("master_dev", _c_p), ("norms_dev", _c_p), ("workspace_dev", _c_p),
+                ("workspace_bytes", ctypes.c_size_t), ("n_chunks", ctypes.c_int64), ("beta1", ctypes.c_double),
+                ("beta2", ctypes.c_double), ("eps", ctypes.c_double), ("max_norm", ctypes.c_double),
+                ("n_tensors", _c_i32), ("n_groups", _c_i32), ("param_dtype", _c_i32), ("grad_dtype", _c_i32),
+                ("skip_nonfinite", _c_i32), ("reserved", _c_i32)]
+
+
+# numpy layouts of lf_grad_tensor and lf_adamw_tensor (arrays of records passed by pointer)
+GRAD_TENSOR = [("ptr", "<u8"), ("numel", "<u8"), ("dtype", "<i4"), ("group", "<i4")]
+ADAMW_TENSOR = [("param", "<u8"), ("state_off", "<i8"), ("numel", "<u4"), ("group", "<i4"), ("chunk0", "<i4"),
+                ("n_chunks", "<i4")]
+BANK_MAX_RANK = 128
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -148,6 +172,21 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_backward_sf.restype = ctypes.c_int
     L.lf_forward_noalloc.argtypes = [P(Problem), P(PlanInfo), _c_p, _c_p, _c_p]
     L.lf_forward_noalloc.restype = ctypes.c_int
+    L.lf_rows_workspace_bytes.argtypes = [_c_i32, _c_i32, _c_i32]
+    L.lf_rows_workspace_bytes.restype = ctypes.c_size_t
+    L.lf_rows_forward.argtypes = [P(RowsProblem), _c_p, _c_p, ctypes.c_size_t, _c_p]
+    L.lf_rows_forward.restype = ctypes.c_int
+    L.lf_grad_clip_workspace_bytes.argtypes = [_c_p, _c_i32, _c_i32]
+    L.lf_grad_clip_workspace_bytes.restype = ctypes.c_size_t
+    L.lf_grad_clip.argtypes = [_c_p, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_double, _c_p, _c_p, ctypes.c_size_t,
+                               _c_p]
+    L.lf_grad_clip.restype = ctypes.c_int
+    L.lf_adamw_plan.argtypes = [_c_p, _c_i32, _c_i32, _c_p, ctypes.c_int64, P(ctypes.c_int64), P(ctypes.c_int64)]
+    L.lf_adamw_plan.restype = ctypes.c_int
+    L.lf_adamw_workspace_bytes.argtypes = [ctypes.c_int64, _c_i32]
+    L.lf_adamw_workspace_bytes.restype = ctypes.c_size_t
+    L.lf_adamw_step.argtypes = [P(AdamWArgs), _c_p]
+    L.lf_adamw_step.restype = ctypes.c_int
     L.lf_set_wait_limit.argtypes = [ctypes.c_uint64]
     L.lf_set_wait_limit.restype = ctypes.c_int
     L.lf_inject_stale_ready.argtypes = [_c_i32]
@@ -205,6 +244,7 @@ def co_scheduling() -> tuple[int, int]:
     return int(mode.value), int(refused.value)
 
 
+ERR_ROW_SLOT = 0x106  # a row of fused_lora_forward_rows named a slot its bank does not have
 # device status codes of bounded waits that ran out (lf_ptx.cuh DeviceErr)
 ERR_TIMEOUT_FULL, ERR_TIMEOUT_EMPTY, ERR_TIMEOUT_ACC, ERR_TIMEOUT_DRAIN, ERR_TIMEOUT_FLAG = 0x101, 0x102, 0x103, 0x104, 0x105
 

@@ -836,6 +836,67 @@ extern "C" int lf_ipc_close(void* dev_ptr) {
   return cudaIpcCloseMemHandle(dev_ptr) == cudaSuccess ? LF_OK : LF_ERR_CUDA;
 }
 
+// Workspace of lf_rows_forward: each row's adapter and factor, then S (two 16-bit halves, or one
+// float32 array on the CUDA-core path: the same bytes).
+extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t r_pad, int32_t dtype) {
+  (void)dtype;
+  if (T < 0 || r_pad < 0) return 0;
+  return 2 * align256(static_cast<size_t>(T) * 4) + 2 * align256(static_cast<size_t>(T) * r_pad * 2);
+}
+
+extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* workspace_dev, size_t workspace_bytes,
+                               lf_stream_t stream) {
+  if (!p || p->T < 0 || p->K < 0 || p->N < 0 || p->n_slots < 0) return LF_ERR_INVALID_ARG;
+  if (p->dtype != LF_F32 && p->dtype != LF_BF16 && p->dtype != LF_F16) return LF_ERR_INVALID_ARG;
+  if (p->r_pad != 16 && p->r_pad != 32 && p->r_pad != 64 && p->r_pad != LF_BANK_MAX_RANK) return LF_ERR_INVALID_ARG;
+  if (p->row_slot_bytes != 4 && p->row_slot_bytes != 8) return LF_ERR_INVALID_ARG;
+  if (p->n_slots >= (1 << 24)) return LF_ERR_UNSUPPORTED;
+  if (p->T == 0 || p->N == 0) return LF_OK;
+  if (p->ldx < p->K || !p->x_dev || !p->w_dev || !p->row_slot_dev || !y_dev) return LF_ERR_INVALID_ARG;
+  if (p->n_slots > 0 && (!p->a_bank_dev || !p->b_bank_dev || !p->slot_rank_dev || !p->slot_scale_dev))
+    return LF_ERR_INVALID_ARG;
+  if (!workspace_dev || workspace_bytes < lf_rows_workspace_bytes(p->T, p->r_pad, p->dtype)) return LF_ERR_CAPACITY;
+  if (!aligned16(workspace_dev)) return LF_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
+  RowsArgs a{};
+  a.x = p->x_dev;
+  a.w = p->w_dev;
+  a.a_bank = p->a_bank_dev;
+  a.b_bank = p->b_bank_dev;
+  a.slot_rank = p->slot_rank_dev;
+  a.slot_scale = p->slot_scale_dev;
+  a.row_slot = p->row_slot_dev;
+  a.y = y_dev;
+  a.ldx = p->ldx;
+  a.T = p->T;
+  a.K = p->K;
+  a.N = p->N;
+  a.n_slots = p->n_slots;
+  a.r_pad = p->r_pad;
+  a.wide = p->row_slot_bytes == 8;
+  a.err = ds->status;
+  char* ws = static_cast<char*>(workspace_dev);
+  const size_t words = align256(static_cast<size_t>(p->T) * 4), s_bytes = align256(static_cast<size_t>(p->T) * p->r_pad * 2);
+  a.eff = reinterpret_cast<uint32_t*>(ws);
+  a.factor = reinterpret_cast<float*>(ws + words);
+  a.s_hi = ws + 2 * words;
+  a.s_lo = ws + 2 * words + s_bytes;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool tc = p->dtype != LF_F32 && p->K > 0 && p->K % 8 == 0 && p->N % 8 == 0 && p->ldx % 8 == 0 &&
+                  aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) &&
+                  aligned16(p->b_bank_dev) && aligned16(y_dev);
+  if (!tc) {
+    if ((p->T + 31) / 32 > 65535) return LF_ERR_UNSUPPORTED;
+    return to_status(rows_forward_simt(a, p->dtype, st));
+  }
+  CUtensorMap w_map, x_map;
+  if (!make_map(&w_map, p->dtype, p->w_dev, p->K, p->N, static_cast<uint64_t>(p->K) * 2, 64, 128) ||
+      !make_map(&x_map, p->dtype, p->x_dev, p->K, p->T, static_cast<uint64_t>(p->ldx) * 2, 64, rows_tile(p->T)))
+    return LF_ERR_UNSUPPORTED;
+  return to_status(rows_forward_tc(a, p->dtype, w_map, x_map, ds->num_sms, st));
+}
+
 extern "C" int lf_device_error(int32_t* code) {
   if (!code) return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;

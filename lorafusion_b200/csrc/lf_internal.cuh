@@ -160,6 +160,32 @@ __host__ __device__ inline size_t peer_half_bytes(int world, int n_blocks, int r
 cudaError_t tc_gram(int dtype, const GramJobDesc* jobs, int n_jobs, const Tables& tb, int num_sms, cudaStream_t st,
                     int planes = 1, void* scratch = nullptr, uint64_t gen = 0, const GramPeer* peer = nullptr);
 
+// --------------------------------------------------------------- rows with an adapter each
+// lf_rows_problem plus the workspace the two launches share.
+struct RowsArgs {
+  const void* x;
+  const void* w;
+  const void* a_bank;
+  const void* b_bank;
+  const int32_t* slot_rank;
+  const float* slot_scale;
+  const void* row_slot;
+  void* y;
+  int64_t ldx;
+  int T, K, N, n_slots, r_pad;
+  int wide;          // row_slot entries are 64-bit
+  uint32_t* eff;     // [T] rank << 24 | slot of each row, all ones without an adapter
+  float* factor;     // [T] s_i times the power of two S was divided by (tensor-core path)
+  void* s_hi;        // [T][r_pad] high halves of S (float32 S itself on the CUDA-core path)
+  void* s_lo;        // [T][r_pad] low halves
+  int* err;          // device status word
+};
+int rows_tile(int T);  // rows of one tensor-core tile
+// w: [N, K] box (64, 128), x: [T, K] box (64, rows_tile(T)), both with the 128-byte swizzle
+cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int num_sms,
+                            cudaStream_t st);
+cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
+
 // --------------------------------------------------------------- packing
 cudaError_t pack_adapters(int src_dtype, int dst_dtype, const uint64_t* src_ptrs, const int32_t* ranks,
                           int n_slots, int rank_dim, int other_dim, int transpose, int d0, int d1, void* dst,

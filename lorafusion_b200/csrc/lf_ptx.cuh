@@ -18,6 +18,7 @@ enum DeviceErr : int {
   kErrTimeoutAcc = 0x103,     // waits on the accumulator hand-off
   kErrTimeoutDrain = 0x104,
   kErrTimeoutFlag = 0x105,    // waited too long for another CTA's ready flag
+  kErrRowSlot = 0x106,        // a row named a slot its adapter bank does not have
 };
 
 // ~1 s of wall time: far above any legitimate wait in these kernels.
@@ -107,6 +108,27 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
       return false;
     }
   }
+}
+
+// Time-bounded wait used only while unwinding after an abort: ignores the abort flag.
+__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, int* err) {
+  const uint64_t t0 = globaltimer_ns();
+  const uint64_t limit = wait_limit(err);
+  while (!mbar_try_wait_sleep(bar, parity, kWaitSleepNs)) {
+    if (globaltimer_ns() - t0 > limit) {
+      record_error(err, kErrTimeoutDrain);
+      return;
+    }
+  }
+}
+
+// Bounded wait done by lane 0 and broadcast, so the warp stays converged for tcgen05.ld.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                          int code) {
+  int ok = 0;
+  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, err, code) ? 1 : 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  return ok != 0;
 }
 
 // ---------------------------------------------------------------- inter-CTA flags

@@ -78,33 +78,12 @@ __device__ __forceinline__ void pack8_hi_lo(const float* v, uint4& pk_hi, uint4&
   }
 }
 
-// Time-bounded wait used only while unwinding after an abort: ignores the abort flag.
-__device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, int* err) {
-  const uint64_t t0 = globaltimer_ns();
-  const uint64_t limit = wait_limit(err);
-  while (!mbar_try_wait_sleep(bar, parity, kWaitSleepNs)) {
-    if (globaltimer_ns() - t0 > limit) {
-      record_error(err, kErrTimeoutDrain);
-      return;
-    }
-  }
-}
-
 // Global load issued at this point in program order (an asm volatile is never moved past the
 // other asm statements), so a value needed only after a k-loop is fetched before the loop.
 __device__ __forceinline__ int ld_early(const int32_t* p) {
   int v;
   asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(v) : "l"(p));
   return v;
-}
-
-// Bounded wait done by lane 0 and broadcast, so the warp stays converged for tcgen05.ld.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
-                                          int code) {
-  int ok = 0;
-  if ((threadIdx.x & 31) == 0) ok = mbar_wait(bar, parity, abort_flag, err, code) ? 1 : 0;
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  return ok != 0;
 }
 
 // ========================================================================== GEMM

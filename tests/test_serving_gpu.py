@@ -1,0 +1,266 @@
+"""Rows with an adapter each (serving.fused_lora_forward_rows) against the formula in 64 bits.
+
+Error bound per element, from the arithmetic: the result is rounded once (half a step of the output
+type); sums run in float32 over K products of the base and r products of the adapter, each addition
+off by at most 2^-23 of the magnitudes summed (a truncating accumulator); S enters the expand as two
+halves of the input type after scaling by its row's largest magnitude, off by 2^-16 (bf16) or
+2^-21 (f16) of that magnitude, and is itself a float32 sum over K.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from lorafusion_b200 import _native as nat
+from lorafusion_b200 import b200_ops
+from lorafusion_b200.serving import AdapterBank, fused_lora_forward_rows
+
+pytestmark = pytest.mark.gpu
+
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+S_HALVES = {BF16: 2.0 ** -16, F16: 2.0 ** -21, F32: 2.0 ** -24}
+
+
+def make(dtype, T, K, N, ranks, max_rank, seed=0, slots=None):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=gen, device="cuda")  # noqa: E731
+    x = rnd(T, K).to(dtype)
+    w = (rnd(N, K) / K ** 0.5).to(dtype)
+    bank = AdapterBank(len(ranks), max_rank, K, N, dtype, "cuda")
+    adapters = []
+    for i, r in enumerate(ranks):
+        a, b, s = (rnd(r, K) / K ** 0.5).to(dtype), (0.1 * rnd(N, r)).to(dtype), 0.5 + 0.25 * i % 3
+        if r:
+            bank.load(i, a, b, s)
+        adapters.append((a, b, s))
+    if slots is None:
+        slots = torch.randint(-1, len(ranks), (T,), generator=gen, device="cuda", dtype=torch.int32)
+    return x, w, bank, adapters, slots
+
+
+def reference(x, w, adapters, slots):
+    """(y, bound on the error) in 64 bits."""
+    xd, wd = x.double(), w.double()
+    K = x.shape[1]
+    y = xd @ wd.T
+    size = xd.abs() @ wd.abs().T
+    slack = torch.zeros_like(y)
+    for i in range(len(adapters)):
+        at = (slots == i).nonzero().view(-1)
+        if not len(at) or adapters[i][0].shape[0] == 0:
+            continue
+        a, b, s = adapters[i][0].double(), adapters[i][1].double(), adapters[i][2]
+        S = xd[at] @ a.T
+        y[at] += s * S @ b.T
+        size[at] += abs(s) * S.abs() @ b.T.abs()
+        off = S_HALVES[x.dtype] * S.abs().amax(1, keepdim=True) + (K + 32) * 2.0 ** -23 * (xd[at].abs() @ a.T.abs())
+        slack[at] += abs(s) * off @ b.T.abs()
+    half = torch.finfo(x.dtype).eps / 2
+    tiny = torch.finfo(x.dtype).smallest_normal * torch.finfo(x.dtype).eps
+    return y, half * y.abs() + (K + 200) * 2.0 ** -23 * size + 1.01 * slack + tiny
+
+
+def check(y, x, w, adapters, slots):
+    ref, bound = reference(x, w, adapters, slots)
+    over = (y.double() - ref).abs() - bound
+    assert y.shape == ref.shape and y.dtype == x.dtype
+    assert torch.isfinite(y).all()
+    assert over.max() <= 0, f"{int((over > 0).sum())} of {over.numel()} over the bound, worst by {over.max():.3g}"
+
+
+CASES = [  # dtype, T, K, N, ranks, max_rank
+    (BF16, 1, 64, 128, [16], 16),
+    (BF16, 1, 4096, 4096, [16, 8], 16),
+    (F16, 2, 8, 8, [1], 1),
+    (BF16, 7, 72, 136, [3, 16, 0, 1], 16),
+    (F16, 16, 1000, 520, [16, 5], 20),
+    (BF16, 17, 264, 2048, [32] * 5, 32),
+    (BF16, 33, 4096, 1024, [64, 8, 33, 17], 64),
+    (F16, 64, 520, 776, [128, 100, 1], 128),
+    (BF16, 65, 1024, 14336, [16] * 80, 16),
+    (BF16, 130, 2048, 264, [8, 16, 32, 64] * 10, 64),
+    (F16, 256, 512, 512, [16] * 300, 16),
+    (BF16, 257, 328, 392, [48, 20], 48),
+    (BF16, 1031, 640, 1288, [16, 40, 64], 64),
+    (F32, 1, 37, 53, [4], 4),
+    (F32, 128, 256, 256, [8] * 4, 8),
+    (F32, 45, 300, 129, [16, 1, 70], 70),
+    (BF16, 19, 37, 61, [5, 2], 8),   # K, N no multiples of 8: CUDA cores
+    (F16, 40, 64, 30, [5, 2], 8),
+]
+
+
+@pytest.mark.filterwarnings("ignore::lorafusion_b200.b200_ops.CudaCorePathWarning")
+@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{str(c[0])[6:]}-{c[1]}x{c[2]}x{c[3]}-r{c[5]}")
+def test_rows_against_64_bits(case):
+    dtype, T, K, N, ranks, max_rank = case
+    x, w, bank, adapters, slots = make(dtype, T, K, N, ranks, max_rank)
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    assert b200_ops.last_launch_count() == 2
+    check(y, x, w, adapters, slots)
+    again = fused_lora_forward_rows(x, w, bank, slots.to(torch.int64))
+    assert torch.equal(y, again)  # the same bits on every run, for either index type
+    assert nat.device_error() == 0
+
+
+def test_orders_and_absent_adapters():
+    T, K, N = 300, 512, 640
+    x, w, bank, adapters, _ = make(BF16, T, K, N, [16, 8, 12], 16)
+    sorted_slots = torch.arange(T, device="cuda", dtype=torch.int32) // 100
+    y_sorted = fused_lora_forward_rows(x, w, bank, sorted_slots)
+    check(y_sorted, x, w, adapters, sorted_slots)
+    none = torch.full((T,), -7, device="cuda", dtype=torch.int32)
+    base = fused_lora_forward_rows(x, w, bank, none)
+    check(base, x, w, adapters, none)
+    one = torch.zeros(T, device="cuda", dtype=torch.int32)
+    check(fused_lora_forward_rows(x, w, bank, one), x, w, adapters, one)
+    bank.unload(1)
+    y = fused_lora_forward_rows(x, w, bank, sorted_slots)
+    assert torch.equal(y[100:200], base[100:200]) and torch.equal(y[:100], y_sorted[:100])
+
+
+def test_agrees_with_the_packed_forward():
+    from lorafusion_b200.config import AdapterSpec, TileRoute, TileRoutingConfig
+    T, K, N = 200, 256, 384
+    x, w, bank, adapters, _ = make(BF16, T, K, N, [16, 8], 16)
+    slots = (torch.arange(T, device="cuda") >= 90).to(torch.int32)
+    specs = {i: AdapterSpec(i, a.shape[0], s * a.shape[0], K, N) for i, (a, _, s) in enumerate(adapters)}
+    routing = TileRoutingConfig(128, [TileRoute(0, 90, 0), TileRoute(90, T, 1)])
+    packed = b200_ops.fused_lora_forward(x, w, {i: a for i, (a, _, _) in enumerate(adapters)},
+                                         {i: b for i, (_, b, _) in enumerate(adapters)}, specs, routing)
+    rows = fused_lora_forward_rows(x, w, bank, slots)
+    check(rows, x, w, adapters, slots)
+    torch.testing.assert_close(rows.float(), packed.float(), rtol=2e-2, atol=2e-2)
+
+
+def test_empty_batch_out_and_strided_rows():
+    x, w, bank, adapters, slots = make(BF16, 40, 256, 264, [16, 4], 16)
+    assert fused_lora_forward_rows(x[:0], w, bank, slots[:0]).shape == (0, 264)
+    out = torch.full((42, 264), 3.0, dtype=BF16, device="cuda")
+    y = fused_lora_forward_rows(x, w, bank, slots, out=out[:40])
+    assert y.data_ptr() == out.data_ptr() and bool((out[40:] == 3.0).all())  # rows behind the last stay
+    check(y, x, w, adapters, slots)
+    wide = torch.zeros(40, 264, dtype=BF16, device="cuda")
+    for x2 in (wide[:, :256], wide[:, 8:], wide[:, 3:259], torch.zeros(256, 40, dtype=BF16, device="cuda").T,
+               torch.zeros(40, 2 * 256, dtype=BF16, device="cuda")[:, ::2], wide.new_zeros(80, 256)[::2]):
+        x2.copy_(x)
+        assert torch.equal(fused_lora_forward_rows(x2, w, bank, slots), y)
+    odd = torch.zeros(40 * 259, dtype=BF16, device="cuda").view(40, 259)[:, :256]  # row pitch no multiple of 8
+    odd.copy_(x)
+    assert torch.equal(fused_lora_forward_rows(odd, w, bank, slots), y)
+    one_row = x[5].expand(40, 256)  # stride 0
+    y1 = fused_lora_forward_rows(one_row, w, bank, slots)
+    check(y1, one_row.contiguous(), w, adapters, slots)
+
+
+def test_slots_out_of_range_are_reported():
+    x, w, bank, adapters, slots = make(BF16, 24, 128, 128, [16, 16], 16)
+    bad = slots.to(torch.int64)
+    bad[3], bad[20] = 2, (1 << 32) + 1
+    nat.device_error()
+    y = fused_lora_forward_rows(x, w, bank, bad)
+    assert nat.device_error() == nat.ERR_ROW_SLOT
+    as_none = slots.clone()
+    as_none[3] = as_none[20] = -1
+    check(y, x, w, adapters, as_none)
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_values_that_are_not_finite_stay_with_their_rows(dtype):
+    T, K, N = 24, 256, 256
+    x, w, bank, adapters, _ = make(dtype, T, K, N, [16, 9, 16], 16)
+    slots = torch.arange(T, device="cuda", dtype=torch.int32) % 3
+    good = fused_lora_forward_rows(x, w, bank, slots)
+    bank.load(1, torch.full((9, K), float("nan"), device="cuda"), torch.full((N, 9), float("inf"), device="cuda"), 1.0)
+    x[2, 5] = float("inf")
+    x[4, 7] = float("nan")
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    bad = (slots == 1)
+    bad[2] = bad[4] = True
+    assert torch.equal(y[~bad], good[~bad])
+    assert not torch.isfinite(y[bad]).any()
+
+
+def test_float16_rank_products_beyond_its_range():
+    """S far above 65504 and far below float16's smallest value, with results inside the range."""
+    T, K, N = 9, 512, 128
+    x, w, bank, adapters, _ = make(F16, T, K, N, [16, 16], 16)
+    x *= 100
+    slots = torch.arange(T, device="cuda", dtype=torch.int32) % 2
+    big = (adapters[0][0] * 400, (adapters[0][1] * 1e-3).to(F16), 1.0)
+    small = ((adapters[1][0] * 1e-4).to(F16), adapters[1][1], 300.0)
+    for i, (a, b, s) in enumerate((big, small)):
+        bank.load(i, a, b, s)
+    S = x.double() @ big[0].double().T
+    assert S.abs().max() > 65504
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    check(y, x, w, [big, small], slots)
+
+
+def test_captured_call_follows_slots_and_bank():
+    T, K, N = 12, 512, 512
+    x, w, bank, adapters, slots = make(BF16, T, K, N, [16, 8], 16)
+    out = torch.empty(T, N, dtype=BF16, device="cuda")
+    fused_lora_forward_rows(x, w, bank, slots, out=out)
+    graph, other = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    out2 = torch.empty_like(out)
+    with torch.cuda.graph(graph):
+        fused_lora_forward_rows(x, w, bank, slots, out=out)
+    with torch.cuda.graph(other, pool=graph.pool()):
+        fused_lora_forward_rows(x, w, bank, slots, out=out2)
+    for k in range(3):
+        slots.copy_(torch.randint(-1, 2, (T,), dtype=torch.int32))
+        a, b, _ = adapters[1]
+        adapters[1] = (a * 0.5, b, 1.0 + k)
+        bank.load(1, *adapters[1])
+        x.copy_(torch.randn(T, K))
+        graph.replay()
+        other.replay()
+        check(out, x, w, adapters, slots)
+        assert torch.equal(out, out2)
+
+
+def test_two_streams_at_once():
+    x, w, bank, adapters, slots = make(BF16, 64, 2048, 2048, [16] * 64, 16)
+    alone = fused_lora_forward_rows(x, w, bank, slots)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for _ in range(20):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k].append(fused_lora_forward_rows(x, w, bank, slots))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, alone) for ys in got for y in ys)
+
+
+def test_refusals():
+    x, w, bank, _, slots = make(BF16, 8, 64, 64, [16], 16)
+    bad = [
+        dict(x=x[0]), dict(x=x.cpu()), dict(x=x.half()), dict(x=x[:, :56]), dict(w=w[:56]), dict(w=w.float()),
+        dict(w=w.T.contiguous().T), dict(w=w.cpu()), dict(slots=slots[:7]), dict(slots=slots.cpu()),
+        dict(slots=slots.to(torch.int16)), dict(slots=slots.float()), dict(out=torch.empty(8, 65, device="cuda")),
+        dict(out=torch.empty(8, 64, device="cuda")), dict(out=torch.empty(64, 8, dtype=BF16, device="cuda").T),
+        dict(out=torch.empty(8, 64, dtype=BF16)),
+    ]
+    for b in bad:
+        with pytest.raises(ValueError):
+            fused_lora_forward_rows(b.get("x", x), b.get("w", w), bank, b.get("slots", slots), out=b.get("out"))
+    a, b = torch.zeros(4, 64, device="cuda"), torch.zeros(64, 4, device="cuda")
+    for args in ((1, a, b, 1.0), (-1, a, b, 1.0), (0, a[:, :60], b, 1.0), (0, a, b[:60], 1.0), (0, a, b[:, :3], 1.0),
+                 (0, a[:0], b[:, :0], 1.0), (0, a[0], b, 1.0), (0, a.repeat(5, 1), b.repeat(1, 5), 1.0)):
+        with pytest.raises(ValueError):
+            bank.load(*args)
+    with pytest.raises(ValueError):
+        bank.unload(1)
+
+
+def test_load_converts_and_clears_past_the_rank():
+    _, _, bank, _, _ = make(BF16, 8, 64, 72, [16], 16)
+    a, b = torch.randn(5, 64, device="cuda"), torch.randn(72, 5, device="cuda")
+    bank.load(0, a, b, 2.0)
+    assert torch.equal(bank.lora_a[0, :5], a.to(BF16)) and torch.equal(bank.lora_b[0, :, :5], b.to(BF16))
+    assert not bank.lora_a[0, 5:].any() and not bank.lora_b[0, :, 5:].any()
+    assert bank.ranks.tolist() == [5] and bank.scales.tolist() == [2.0]
+    assert np.isclose(bank.lora_a.element_size(), 2)
