@@ -468,7 +468,8 @@ LF_API int lf_assign_rows(const int32_t* bin_start, const int32_t* entry_adapter
 #define LF_BANK_MAX_RANK 128
 
 /* One projection and a bank of resident adapters.  `slot_rank_dev` holds each slot's rank (0: empty
- * slot, its rows get the shared projection alone), at most r_pad; bank entries past it must be zero. */
+ * slot, its rows get the shared projection alone), at most r_pad; bank entries past it must be zero.
+ * A block of the B bank holds feature f, rank r of its 16 x 16 at 8 (4 (f % 8) + r / 4) + 4 (f / 8) + r % 4. */
 typedef struct lf_rows_problem {
   int32_t dtype;             /* lf_dtype of x, W, y and the bank */
   int32_t T, K, N;           /* rows, in_features, out_features */
@@ -479,14 +480,14 @@ typedef struct lf_rows_problem {
   const void* x_dev;         /* [T] rows of K */
   const void* w_dev;         /* [N,K] */
   const void* a_bank_dev;    /* [n_slots, r_pad, K] */
-  const void* b_bank_dev;    /* [n_slots, N, r_pad] */
+  const void* b_bank_dev;    /* [n_slots, r_pad/16, ceil(N/16), 256]: blocks of 16 ranks x 16 features */
   const int32_t* slot_rank_dev;  /* [n_slots] */
   const float* slot_scale_dev;   /* [n_slots] s_i */
   const void* row_slot_dev;  /* [T] slot of each row; negative: no adapter */
 } lf_rows_problem;
 
 /* Workspace bytes of lf_rows_forward (256-byte aligned buffer). */
-LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t r_pad, int32_t dtype);
+LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype);
 
 /*
  * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense.  row_slot is read on

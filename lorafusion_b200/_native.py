@@ -8,9 +8,13 @@ and raises ``RuntimeError`` when it is missing: the operator has no fallback.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import re
 import threading
+from contextlib import nullcontext
+
+import torch
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "liblorafusion_b200.so")
@@ -98,6 +102,7 @@ BANK_MAX_RANK = 128
 
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
+_glue = None
 
 
 def _declare(L: ctypes.CDLL) -> None:
@@ -172,7 +177,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_backward_sf.restype = ctypes.c_int
     L.lf_forward_noalloc.argtypes = [P(Problem), P(PlanInfo), _c_p, _c_p, _c_p]
     L.lf_forward_noalloc.restype = ctypes.c_int
-    L.lf_rows_workspace_bytes.argtypes = [_c_i32, _c_i32, _c_i32]
+    L.lf_rows_workspace_bytes.argtypes = [_c_i32, _c_i32, _c_i32, _c_i32]
     L.lf_rows_workspace_bytes.restype = ctypes.c_size_t
     L.lf_rows_forward.argtypes = [P(RowsProblem), _c_p, _c_p, ctypes.c_size_t, _c_p]
     L.lf_rows_forward.restype = ctypes.c_int
@@ -216,6 +221,25 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def glue():
+    """The Python module of ``csrc/lf_pyglue.cpp`` (tensor checks and calls without a Python step per
+    tensor); ``RuntimeError`` if it has not been built."""
+    global _glue
+    if _glue is None:
+        L = lib()
+        with _lock:
+            if _glue is None:
+                path = os.path.join(_HERE, "_lib", "lf_pyglue.so")
+                if not os.path.exists(path):
+                    raise RuntimeError(f"{path} not found; build it with `python -m lorafusion_b200.csrc.build`")
+                spec = importlib.util.spec_from_file_location("lf_pyglue", path)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                _glue = module
+        assert L is not None
+    return _glue
+
+
 def header_symbols() -> list[str]:
     """Names of every entry point the public header declares."""
     text = open(HEADER_PATH).read()
@@ -234,6 +258,16 @@ def check(code: int, what: str) -> None:
     if code in (LF_ERR_CUDA, LF_ERR_DEVICE):
         raise RuntimeError(msg)
     raise ValueError(msg)
+
+
+def raw_stream(device_index: int) -> int:
+    """cudaStream_t of the device's current stream (without building a Stream object: 0.1 us, not 2)."""
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
+def on_device(device_index: int):
+    """Context that makes a device current; nothing to do where it already is."""
+    return nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
 
 
 def co_scheduling() -> tuple[int, int]:

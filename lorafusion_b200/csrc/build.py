@@ -5,7 +5,8 @@
 Every translation unit is compiled by nvcc for ``compute_100a``/``sm_100a`` only
 (with ``-lineinfo``), in parallel, then linked into one position-independent
 shared library with a static CUDA runtime.  Objects are rebuilt when a source
-or header is newer than the object.
+or header is newer than the object.  ``_lib/lf_pyglue.so``, a Python module that
+links PyTorch and that library, is built beside it.
 """
 
 from __future__ import annotations
@@ -23,6 +24,7 @@ REPO = os.path.dirname(PKG)
 OBJ_DIR = os.path.join(PKG, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_NAME = "liblorafusion_b200.so"
+GLUE_SOURCE, GLUE_NAME = "lf_pyglue.cpp", "lf_pyglue.so"  # Python module: tensor checks and calls for PyTorch
 SOURCES = ["lf_tables.cpp", "lf_sched.cpp", "lf_simt.cu", "lf_tc.cu", "lf_rows.cu", "lf_lora_rows.cu", "lf_train.cu",
            "lf_capi.cu", "lf_noalloc.cu"]
 HEADERS = ["lf_ptx.cuh", "lf_internal.cuh", "lf_launch.cuh", os.path.join("..", "..", "include", "lorafusion_b200.h")]
@@ -65,6 +67,30 @@ def _compile(src: str, force: bool, verbose: bool, extra: list[str]) -> str:
     return obj
 
 
+def _build_glue(force: bool, verbose: bool) -> None:
+    """The Python module of csrc/lf_pyglue.cpp, beside the library it calls."""
+    import sysconfig
+
+    import torch
+    src, out = os.path.join(HERE, GLUE_SOURCE), os.path.join(LIB_DIR, GLUE_NAME)
+    header = os.path.join(REPO, "include", "lorafusion_b200.h")
+    if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(header)):
+        return
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}", "-I" + os.path.join(REPO, "include"),
+           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + os.path.join(cuda, "include"), "-I" + sysconfig.get_paths()["include"], "-o", out, src,
+           "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu", "-ltorch_cuda", "-lc10", "-lc10_cuda",
+           "-L" + LIB_DIR, "-llorafusion_b200", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"compiling {GLUE_SOURCE} failed:\n{res.stdout}\n{res.stderr}")
+
+
 def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) -> str:
     os.makedirs(OBJ_DIR, exist_ok=True)
     os.makedirs(LIB_DIR, exist_ok=True)
@@ -79,6 +105,7 @@ def build(force: bool = False, verbose: bool = False, ptxas_info: bool = False) 
         res = subprocess.run(cmd, capture_output=True, text=True)
         if res.returncode != 0:
             raise RuntimeError(f"link failed:\n{res.stdout}\n{res.stderr}")
+    _build_glue(force, verbose)
     return out
 
 

@@ -837,11 +837,11 @@ extern "C" int lf_ipc_close(void* dev_ptr) {
 }
 
 // Workspace of lf_rows_forward: each row's adapter and factor, then S (two 16-bit halves, or one
-// float32 array on the CUDA-core path: the same bytes).
-extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t r_pad, int32_t dtype) {
-  (void)dtype;
-  if (T < 0 || r_pad < 0) return 0;
-  return 2 * align256(static_cast<size_t>(T) * 4) + 2 * align256(static_cast<size_t>(T) * r_pad * 2);
+// float32 array on the CUDA-core path: the same bytes), then the adapters' part of the result.
+extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype) {
+  if (T < 0 || N < 0 || r_pad < 0) return 0;
+  const size_t delta = dtype == LF_F32 ? 0 : static_cast<size_t>(T) * ((N + 15) / 16 * 16) * 4;
+  return 2 * align256(static_cast<size_t>(T) * 4) + 2 * align256(static_cast<size_t>(T) * r_pad * 2) + align256(delta);
 }
 
 extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* workspace_dev, size_t workspace_bytes,
@@ -855,7 +855,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   if (p->ldx < p->K || !p->x_dev || !p->w_dev || !p->row_slot_dev || !y_dev) return LF_ERR_INVALID_ARG;
   if (p->n_slots > 0 && (!p->a_bank_dev || !p->b_bank_dev || !p->slot_rank_dev || !p->slot_scale_dev))
     return LF_ERR_INVALID_ARG;
-  if (!workspace_dev || workspace_bytes < lf_rows_workspace_bytes(p->T, p->r_pad, p->dtype)) return LF_ERR_CAPACITY;
+  if (!workspace_dev || workspace_bytes < lf_rows_workspace_bytes(p->T, p->N, p->r_pad, p->dtype)) return LF_ERR_CAPACITY;
   if (!aligned16(workspace_dev)) return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
@@ -882,6 +882,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   a.factor = reinterpret_cast<float*>(ws + words);
   a.s_hi = ws + 2 * words;
   a.s_lo = ws + 2 * words + s_bytes;
+  a.delta = reinterpret_cast<float*>(ws + 2 * words + 2 * s_bytes);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = p->dtype != LF_F32 && p->K > 0 && p->K % 8 == 0 && p->N % 8 == 0 && p->ldx % 8 == 0 &&
                   aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) &&
@@ -890,11 +891,12 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     if ((p->T + 31) / 32 > 65535) return LF_ERR_UNSUPPORTED;
     return to_status(rows_forward_simt(a, p->dtype, st));
   }
+  const RowsTiles tiles = rows_tiles(p->T, p->K, p->N, ds->num_sms);
   CUtensorMap w_map, x_map;
   if (!make_map(&w_map, p->dtype, p->w_dev, p->K, p->N, static_cast<uint64_t>(p->K) * 2, 64, 128) ||
-      !make_map(&x_map, p->dtype, p->x_dev, p->K, p->T, static_cast<uint64_t>(p->ldx) * 2, 64, rows_tile(p->T)))
+      !make_map(&x_map, p->dtype, p->x_dev, p->K, p->T, static_cast<uint64_t>(p->ldx) * 2, 64, tiles.rows))
     return LF_ERR_UNSUPPORTED;
-  return to_status(rows_forward_tc(a, p->dtype, w_map, x_map, ds->num_sms, st));
+  return to_status(rows_forward_tc(a, p->dtype, w_map, x_map, tiles, ds->num_sms, st));
 }
 
 extern "C" int lf_device_error(int32_t* code) {

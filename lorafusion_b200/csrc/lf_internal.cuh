@@ -178,12 +178,17 @@ struct RowsArgs {
   float* factor;     // [T] s_i times the power of two S was divided by (tensor-core path)
   void* s_hi;        // [T][r_pad] high halves of S (float32 S itself on the CUDA-core path)
   void* s_lo;        // [T][r_pad] low halves
+  float* delta;      // [T][N rounded up to 16] the adapters' part of rows that have one
   int* err;          // device status word
 };
-int rows_tile(int T);  // rows of one tensor-core tile
-// w: [N, K] box (64, 128), x: [T, K] box (64, rows_tile(T)), both with the 128-byte swizzle
-cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int num_sms,
-                            cudaStream_t st);
+struct RowsTiles {
+  int rows;    // of x a tile
+  int ksplit;  // CTAs that share a tile, each with a part of K
+};
+RowsTiles rows_tiles(int T, int K, int N, int num_sms);
+// w: [N, K] box (64, 128), x: [T, K] box (64, tiles.rows), both with the 128-byte swizzle
+cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
+                            int num_sms, cudaStream_t st);
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
 
 // --------------------------------------------------------------- packing

@@ -2,20 +2,19 @@
 //   y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T,   i = row_slot[t]  (negative: no adapter).
 //
 // Two launches, the second started while the first runs:
-//   rows_shrink  S[t] = x[t] A_i^T.  Rows are grouped by adapter inside tiles of 128 rows, on the
-//                device, so any order of rows works and no host plan is needed.  A group's A_i is
-//                read once per tile.  Few rows bring one adapter each, so the product is a stream
-//                of A_i through warp-level MMAs whose 8 columns are rows of one adapter: bound by the
-//                bytes of A_i, and by x for long batches, never by the MMA rate.
+//   rows_lora    the adapters' part, float32: S = x[t] A_i^T, then s_i S B_i^T.  Rows are grouped by adapter on
+//                the device, so any order of rows works and no host plan is needed.  A cluster takes a
+//                few groups: its CTAs cut K for S, exchange their sums through distributed shared
+//                memory, then cut the output features, so no grid-wide step lies between A_i and B_i.
+//                Few rows bring one adapter each: both products are streams of weights through
+//                warp-level MMAs whose 8 columns are rows of one adapter, bound by bytes.
 //   rows_gemm    y^T tiles of 128 output features x up to 256 rows with tcgen05 (the weight is the
 //                M operand, so a decode step of a few rows wastes no tensor-memory lanes and streams
 //                W once), K split over a cluster when the tiles alone would leave SMs idle.  The
-//                epilogue waits for the shrink, adds s_i S[t] B_i^T per 8 rows with warp-level MMAs on
-//                the accumulator fragments, and writes y once.  B_i is prefetched into L2 while the
-//                weight streams.
+//                epilogue waits for the first launch, adds its part and writes y once.
 //
-// S is kept as hi + lo halves of the input type after a per-row power-of-two scaling (the row's
-// largest magnitude becomes 1..2), so it enters the expand to about 2^-16 (bf16) or 2^-22 (f16)
+// S enters the second product as hi + lo halves of the input type after a per-row power-of-two scaling (the
+// row's largest magnitude becomes 1..2), so it is exact to about 2^-16 (bf16) or 2^-22 (f16)
 // relative and a float16 S cannot overflow.  All sums are float32.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -71,318 +70,479 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 // and B agree, so a lane takes consecutive elements of its rows with one wide load.
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, __nv_bfloat16*) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1, __half*) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// ============================================================================ shrink
-// Grid: (row tile, slice of its groups, K part); the K parts of one (tile, slice) form a cluster.
-// Every warp takes its own K range of every group of 8 rows; partial products meet in shared memory,
-// then across the cluster, in a fixed order.
-template <typename T, int kMT>
-__global__ void __launch_bounds__(kShrinkThreads) rows_shrink_kernel(const RowsArgs p, int slices, int kparts) {
-  constexpr int kRP = kMT * 16;                                         // padded rank
-  constexpr int kBatch = kPartBytes / (kShrinkWarps * kRP * 8 * 4);     // groups of 8 rows per batch
-  __shared__ float part[kShrinkWarps][kBatch][kRP * 8];
-  __shared__ uint32_t s_eff[kTileRows];
-  __shared__ int16_t s_pos[kTileRows];
-  __shared__ int16_t s_start[kTileRows];     // first row of each group
-  __shared__ int16_t s_rows[kTileRows][8];   // rows of each group, -1: none
-  __shared__ int s_warp_groups[4];
-  pdl_launch_dependents();
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int crank = blockIdx.x % kparts;
-  const int slice = blockIdx.x / kparts % slices;
-  const int t0 = blockIdx.x / (kparts * slices) * kTileRows;
-  const int rows = min(kTileRows, p.T - t0);
+__device__ __forceinline__ void st_cluster_f32(uint32_t addr, uint32_t v) {
+  asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
+}
 
-  uint32_t eff = kNoSlot;
-  if (tid < kTileRows) {
-    if (tid < rows) {
-      eff = row_adapter(p, t0 + tid, true);
-      if (crank == 0 && slice == 0) p.eff[t0 + tid] = eff;
+// One warp's K steps k0 .. k1 - 1 (32 elements each) of up to kNB groups of one adapter (rank up to 16 kMT) into its
+// slots of `part`.  Few instructions a step count more here than anything else (with the bounds of K and
+// of the rows tested on every load a step took 90): whole steps run without a test, and a row that a group
+// does not have points at one that exists, for columns nobody reads.
+template <typename T, int kMT, int kNB, int kUnroll>
+__device__ __forceinline__ void shrink_steps(float (&acc)[kMT][kNB][4], const T* const (&xr)[kNB], const T* ar, int K,
+                                             int k, bool in) {
+  const uint4 zero = make_uint4(0, 0, 0, 0);
+  uint4 xv[kUnroll][kNB], lo[kUnroll][kMT], hi[kUnroll][kMT];
+#pragma unroll
+  for (int i = 0; i < kUnroll; ++i) {
+#pragma unroll
+    for (int m = 0; m < kMT; ++m) {
+      lo[i][m] = in ? *reinterpret_cast<const uint4*>(ar + m * 16 * K + (k + i) * 32) : zero;
+      hi[i][m] = in ? *reinterpret_cast<const uint4*>(ar + (m * 16 + 8) * K + (k + i) * 32) : zero;
     }
-    s_eff[tid] = eff;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s_rows[tid][i] = -1;
+    for (int b = 0; b < kNB; ++b) xv[i][b] = in ? *reinterpret_cast<const uint4*>(xr[b] + (k + i) * 32) : zero;
   }
-  __syncthreads();
-  // position of each row among its adapter's rows of the tile; every eighth starts a group
-  int pos = 0;
-  if (tid < rows && eff != kNoSlot)
-    for (int j = 0; j < tid; ++j) pos += s_eff[j] == eff;
-  const bool starts = tid < rows && eff != kNoSlot && (pos & 7) == 0;
-  uint32_t vote = 0;
-  if (tid < kTileRows) {
-    s_pos[tid] = static_cast<int16_t>(pos);
-    vote = __ballot_sync(0xffffffffu, starts);
-    if (lane == 0) s_warp_groups[warp] = __popc(vote);
-  }
-  __syncthreads();
-  int n_groups = 0, before = 0;
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    if (w < warp) before += s_warp_groups[w];
-    n_groups += s_warp_groups[w];
-  }
-  if (starts) s_start[before + __popc(vote & ((1u << lane) - 1))] = static_cast<int16_t>(tid);
-  __syncthreads();
-  if (tid < rows && eff != kNoSlot) {
-    const int want = pos & ~7;
-    for (int u = 0; u < n_groups; ++u) {
-      const int st = s_start[u];
-      if (s_eff[st] == eff && s_pos[st] == want) {
-        s_rows[u][pos & 7] = static_cast<int16_t>(tid);
-        break;
+  for (int i = 0; i < kUnroll; ++i)
+#pragma unroll
+    for (int m = 0; m < kMT; ++m)
+#pragma unroll
+      for (int b = 0; b < kNB; ++b) {
+        mma16816(acc[m][b], lo[i][m].x, hi[i][m].x, lo[i][m].y, hi[i][m].y, xv[i][b].x, xv[i][b].y,
+                 static_cast<T*>(nullptr));
+        mma16816(acc[m][b], lo[i][m].z, hi[i][m].z, lo[i][m].w, hi[i][m].w, xv[i][b].z, xv[i][b].w,
+                 static_cast<T*>(nullptr));
+      }
+}
+template <typename T, int kMT, int kNB, int kUnroll, int kStride>
+__device__ __forceinline__ void shrink_groups(const T* const (&xr)[kNB], const T* ar, int K, int k0, int k1, int nb,
+                                              float* dst) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  float acc[kMT][kNB][4];
+#pragma unroll
+  for (int m = 0; m < kMT; ++m)
+#pragma unroll
+    for (int b = 0; b < kNB; ++b) acc[m][b][0] = acc[m][b][1] = acc[m][b][2] = acc[m][b][3] = 0.f;
+  const int whole = min(k1, K / 32);
+  int k = k0;
+#pragma unroll 1
+  for (; k + kUnroll <= whole; k += kUnroll) shrink_steps<T, kMT, kNB, kUnroll>(acc, xr, ar, K, k, true);
+#pragma unroll 1
+  for (; k < k1; ++k) shrink_steps<T, kMT, kNB, 1>(acc, xr, ar, K, k, k * 32 + 8 * q < K);
+#pragma unroll
+  for (int b = 0; b < kNB; ++b) {
+    if (b < nb) {
+#pragma unroll
+      for (int m = 0; m < kMT; ++m) {
+        float* at = dst + b * kStride + (m * 16 + g) * 8 + 2 * q;
+        *reinterpret_cast<float2*>(at) = make_float2(acc[m][b][0], acc[m][b][1]);
+        *reinterpret_cast<float2*>(at + 64) = make_float2(acc[m][b][2], acc[m][b][3]);
       }
     }
   }
-  __syncthreads();
+}
 
+// ============================================================================ adapters' part
+// Rows of a tile grouped by adapter, at most 8 a group; groups of one adapter follow one another.
+struct Groups {
+  uint32_t eff[kTileRows];      // adapter of each row
+  int16_t base[kTileRows];      // first group of the adapter whose first row this is
+  int16_t start[kTileRows];     // first row of each group
+  int16_t rows[kTileRows][8];   // rows of each group, -1: none
+  int warp_groups[4];
+  int cost[kTileRows];          // what the groups up to each one (this one not) cost, and all of them
+  int total;
+};
+
+// Number of groups of rows t0 .. t0 + rows - 1 (at most kTileRows).  All threads of the CTA call it; ends with a barrier.
+__device__ __forceinline__ int group_rows(const RowsArgs& p, int t0, int rows, bool report, Groups& s) {
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t eff = kNoSlot;
+  if (tid < kTileRows) {
+    if (tid < rows) eff = row_adapter(p, t0 + tid, report);
+    s.eff[tid] = eff;
+    *reinterpret_cast<uint4*>(s.rows[tid]) = make_uint4(~0u, ~0u, ~0u, ~0u);
+  }
+  __syncthreads();
+  // rows of the same adapter as a bit mask: the row's place among them, and its adapter's first row
+  const bool on = tid < rows && eff != kNoSlot;
+  int pos = 0, first_row = -1, groups = 0, before = 0;
+  if (tid < kTileRows) {
+    uint32_t m[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      m[w] = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint4 u = *reinterpret_cast<const uint4*>(s.eff + w * 32 + i * 4);
+        m[w] |= (static_cast<uint32_t>(u.x == eff) | static_cast<uint32_t>(u.y == eff) << 1 |
+                 static_cast<uint32_t>(u.z == eff) << 2 | static_cast<uint32_t>(u.w == eff) << 3) << (4 * i);
+      }
+    }
+    int total = 0;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      if (w < warp) pos += __popc(m[w]);
+      if (w == warp) pos += __popc(m[w] & ((1u << lane) - 1));
+      total += __popc(m[w]);
+      if (first_row < 0 && m[w]) first_row = w * 32 + __ffs(m[w]) - 1;
+    }
+    groups = on && pos == 0 ? (total + 7) / 8 : 0;
+    int sum = groups;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffffu, sum, o);
+      if (lane >= o) sum += up;
+    }
+    if (lane == 31) s.warp_groups[warp] = sum;
+    before = sum - groups;
+  }
+  __syncthreads();
+  int n_groups = 0;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    if (w < warp) before += s.warp_groups[w];
+    n_groups += s.warp_groups[w];
+  }
+  if (groups > 0) s.base[tid] = static_cast<int16_t>(before);
+  __syncthreads();
+  if (on) {
+    const int grp = s.base[first_row] + (pos >> 3);
+    s.rows[grp][pos & 7] = static_cast<int16_t>(tid);
+    if ((pos & 7) == 0) s.start[grp] = static_cast<int16_t>(tid);
+  }
+  __syncthreads();
+  // a group's cost: its rank steps, and about one step for the rest
+  if (warp == 0) {
+    int sum = 0;
+    for (int c = 0; c < n_groups; c += 32) {
+      const int mine = c + lane < n_groups ? 1 + ((rank_of(s.eff[s.start[c + lane]]) + 15) >> 4) : 0;
+      int up = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, up, o);
+        if (lane >= o) up += v;
+      }
+      if (c + lane < n_groups) s.cost[c + lane] = sum + up - mine;
+      sum += __shfl_sync(0xffffffffu, up, 31);
+    }
+    if (lane == 0) s.total = sum;
+  }
+  __syncthreads();
+  return n_groups;
+}
+
+// First group of a slice: groups go to the slice that their cost's middle falls into.
+__device__ __forceinline__ int slice_start(const Groups& s, int n_groups, int slice, int slices) {
+  int lo = 0, hi = n_groups;  // the first group whose middle is at or past the slice's share
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    const int next = mid + 1 < n_groups ? s.cost[mid + 1] : s.total;
+    if (static_cast<int64_t>(s.cost[mid] + next) * slices < 2ll * s.total * slice) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// 2^ex with the largest of a row's values over 1..2; 0 for a row that is all zero or not finite.
+__device__ __forceinline__ int row_exponent(float top) {
+  return top > 0.f && top <= 3.402823466e38f ? max(-126, min(126, ilogbf(top))) : 0;
+}
+// v scaled, as high and low halves; the high half of a value that is not finite says it all
+template <typename T>
+__device__ __forceinline__ void halves(float w, T& hi, T& lo) {
+  hi = from_f32<T>(w);
+  lo = from_f32<T>(fabsf(w) <= 4.f ? w - to_f32(hi) : 0.f);
+}
+
+// The second product of one group of 8 rows for output blocks b0 .. b1 - 1 (16 features each): kNM rank steps
+// of 16, kPer blocks loaded together.  B_i is stored in the order of the MMA's operand: one 16-byte load a
+// lane and step.  hi, lo: S of row g, null without one.  A row that the group does not have is -1; `second`:
+// whether any of the odd rows exists.
+template <typename T, int kNM, int kPer>
+__device__ __forceinline__ void expand_blocks(const uint4* w, int pitch, const uint2 (&sh)[kNM], const uint2 (&sl)[kNM],
+                                              float f0, float f1, float* o0, float* o1, bool on0, bool on1,
+                                              bool second) {
+  T* const tag = nullptr;
+  uint4 v[kPer][kNM];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+#pragma unroll
+    for (int k = 0; k < kNM; ++k) v[i][k] = w[k * pitch + i * 32];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < kNM; ++k) {
+      mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sh[k].x, sh[k].y, tag);
+      mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sl[k].x, sl[k].y, tag);
+    }
+    if (on0) o0[i * 16] = f0 * d[0], o0[i * 16 + 8] = f0 * d[2];
+    if (second && on1) o1[i * 16] = f1 * d[1], o1[i * 16 + 8] = f1 * d[3];
+  }
+}
+template <typename T, int kNM, int kPer>
+__device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int b0, int b1, const T* hi, const T* lo,
+                                             float f0, float f1, int row0, int row1) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int blocks = (p.N + 15) >> 4, steps = p.r_pad >> 4;
+  uint2 sh[kNM], sl[kNM];
+#pragma unroll
+  for (int k = 0; k < kNM; ++k) {
+    const bool on = hi != nullptr && 16 * k < rank_of(e);
+    sh[k] = on ? *reinterpret_cast<const uint2*>(hi + 16 * k + 4 * q) : make_uint2(0, 0);
+    sl[k] = on ? *reinterpret_cast<const uint2*>(lo + 16 * k + 4 * q) : make_uint2(0, 0);
+  }
+  const bool on0 = row0 >= 0, on1 = row1 >= 0, second = __any_sync(0xffffffffu, on1);
+  const uint4* w = static_cast<const uint4*>(p.b_bank) +
+                   (static_cast<size_t>(slot_of(e)) * steps * blocks + b0) * 32 + lane;
+  float* o0 = p.delta + (static_cast<size_t>(max(row0, 0)) * blocks + b0) * 16 + g;
+  float* o1 = p.delta + (static_cast<size_t>(max(row1, 0)) * blocks + b0) * 16 + g;
+  int n = b1 - b0;
+#pragma unroll 1
+  for (; n >= kPer; n -= kPer, w += kPer * 32, o0 += kPer * 16, o1 += kPer * 16)
+    expand_blocks<T, kNM, kPer>(w, blocks * 32, sh, sl, f0, f1, o0, o1, on0, on1, second);
+#pragma unroll 1
+  for (; n > 0; --n, w += 32, o0 += 16, o1 += 16)
+    expand_blocks<T, kNM, 1>(w, blocks * 32, sh, sl, f0, f1, o0, o1, on0, on1, second);
+}
+
+// Groups from `grp` on, at most kNB and `most`, that belong to one adapter.
+template <int kNB>
+__device__ __forceinline__ int unit_size(const Groups& s, int grp, int most) {
+  int nb = 1;
+  if (kNB > 1) {
+    const uint32_t e = s.eff[s.start[grp]];
+    while (nb < kNB && nb < most && s.eff[s.start[grp + nb]] == e) ++nb;
+  }
+  return nb;
+}
+
+// Work items: (row tile, slice of its groups), each taken by a cluster of `kparts` CTAs that cut K for the
+// first product and the output features for the second.  Partial products
+// meet in shared memory, then across the cluster, in a fixed order.  The grid fits the GPU at once, so
+// the dependent GEMM streams its weight while this kernel runs.
+// kToGlobal: write S (halves and factor) to global memory instead, for a GEMM that does the second product.
+template <typename T, int kMT, int kNB, bool kToGlobal>
+__global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts) {
+  constexpr int kRP = kMT * 16;                                         // padded rank
+  constexpr int kBatch = kPartBytes / (kShrinkWarps * kRP * 8 * 4);     // groups of 8 rows per batch
+  constexpr int kPitch = kRP + 8;                                       // of S rows: no bank conflicts
+  __shared__ float part[kShrinkWarps][kBatch][kRP * 8];
+  __shared__ __align__(16) Groups s;
+  __shared__ __align__(16) T s_hi[kBatch][8][kPitch], s_lo[kBatch][8][kPitch];
+  __shared__ float s_fac[kBatch][8];
+  __shared__ float s_in[kBatch * kRP * 8 + 8];  // the cluster's sums of this CTA's share (see below)
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, q = lane & 3;
+  const int crank = blockIdx.x % kparts;
   const T* x = static_cast<const T*>(p.x);
   const T* bank = static_cast<const T*>(p.a_bank);
   const int K = p.K;
   const int n_blocks = (K + 31) / 32;  // 32 elements of K a step: 8 a lane
-  const int ranges = kparts * kShrinkWarps, me = crank * kShrinkWarps + warp;
-  const int b0 = static_cast<int>(static_cast<int64_t>(me) * n_blocks / ranges);
-  const int b1 = static_cast<int>(static_cast<int64_t>(me + 1) * n_blocks / ranges);
-  const uint4 zero = make_uint4(0, 0, 0, 0);
+  const int out_blocks = (p.N + 15) >> 4;  // of 16 features; this CTA's: [nb0, nb1)
+  const int nb0 = out_blocks * crank / kparts, nb1 = out_blocks * (crank + 1) / kparts;
+  const int n_items = (p.T + kTileRows - 1) / kTileRows * slices;
 
-  const int mine = n_groups > slice ? (n_groups - slice + slices - 1) / slices : 0;  // groups slice, slice + slices, ..
-  for (int first = 0; first < mine; first += kBatch) {
-    const int batch = min(kBatch, mine - first);
-    for (int u = 0; u < batch; ++u) {
-      const int grp = slice + (first + u) * slices;
-      const uint32_t e = s_eff[s_start[grp]];
-      const int row = s_rows[grp][g];
-      const int nm = (rank_of(e) + 15) >> 4;
-      const T* xr = x + static_cast<int64_t>(t0 + max(row, 0)) * p.ldx + 8 * q;
-      const T* ar = bank + (static_cast<size_t>(slot_of(e)) * p.r_pad + g) * K + 8 * q;
-      float acc[kMT][4];
+  for (int item = blockIdx.x / kparts; item < n_items; item += gridDim.x / kparts) {
+    const int slice = item % slices, t0 = item / slices * kTileRows;
+    const int rows = min(kTileRows, p.T - t0);
+    const int n_groups = group_rows(p, t0, rows, true, s);
+    if (kToGlobal && crank == 0 && slice == 0 && tid < rows) p.eff[t0 + tid] = s.eff[tid];
+    const int g_lo = slice_start(s, n_groups, slice, slices);
+    const int g_hi = slice + 1 < slices ? slice_start(s, n_groups, slice + 1, slices) : n_groups;
+    for (int first = g_lo; first < g_hi; first += kBatch) {
+      const int batch = min(kBatch, g_hi - first);
+      // Up to kNB groups of one adapter are a unit.  The warps divide the units first, so that as many streams
+      // of A_i as there are warps are in flight, and K where there are fewer units than warps.
+      int n_units = 0;
+      for (int u = 0; u < batch; u += unit_size<kNB>(s, first + u, batch - u)) ++n_units;
+      const int lanes = n_units >= 8 ? 8 : n_units >= 4 ? 4 : n_units >= 2 ? 2 : 1;  // units at a time
+      const int subs = kShrinkWarps / lanes, sub = warp / lanes;
+      const int ranges = kparts * subs, me = crank * subs + sub;
+      const int b0 = static_cast<int>(static_cast<int64_t>(me) * n_blocks / ranges);
+      const int b1 = static_cast<int>(static_cast<int64_t>(me + 1) * n_blocks / ranges);
+      for (int u = 0, index = 0, nb; u < batch; u += nb, ++index) {
+        nb = unit_size<kNB>(s, first + u, batch - u);
+        if (index % lanes != warp % lanes) continue;
+        const uint32_t e = s.eff[s.start[first + u]];
+        const int nm = (rank_of(e) + 15) >> 4;
+        const T* xr[kNB];
 #pragma unroll
-      for (int m = 0; m < kMT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-#pragma unroll(kMT == 1 ? 4 : kMT == 2 ? 2 : 1)
-      for (int b = b0; b < b1; ++b) {
-        const bool in = b * 32 + 8 * q < K;
-        const uint4 xv = in && row >= 0 ? *reinterpret_cast<const uint4*>(xr + b * 32) : zero;
-        uint4 lo[kMT], hi[kMT];
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          const bool on = in && m < nm;
-          lo[m] = on ? *reinterpret_cast<const uint4*>(ar + static_cast<size_t>(m * 16) * K + b * 32) : zero;
-          hi[m] = on ? *reinterpret_cast<const uint4*>(ar + static_cast<size_t>(m * 16 + 8) * K + b * 32) : zero;
+        for (int b = 0; b < kNB; ++b) {
+          const int row = b < nb ? s.rows[first + u + b][g] : 0;
+          xr[b] = x + static_cast<int64_t>(t0 + max(row, 0)) * p.ldx + 8 * q;
         }
-#pragma unroll
-        for (int m = 0; m < kMT; ++m) {
-          if (m < nm) {
-            mma16816(acc[m], lo[m].x, hi[m].x, lo[m].y, hi[m].y, xv.x, xv.y, static_cast<T*>(nullptr));
-            mma16816(acc[m], lo[m].z, hi[m].z, lo[m].w, hi[m].w, xv.z, xv.w, static_cast<T*>(nullptr));
+        const T* ar = bank + (static_cast<size_t>(slot_of(e)) * p.r_pad + g) * K + 8 * q;
+        float* dst = part[sub][u];
+        const T* const one_x[1] = {xr[0]};
+        constexpr int kS = kRP * 8;
+        // the smallest kernel that covers the adapter's rank and the groups at hand
+        if (nm == 1) {
+          if (kNB == 1 || nb == 1) shrink_groups<T, 1, 1, 8, kS>(one_x, ar, K, b0, b1, 1, dst);
+          else shrink_groups<T, 1, kNB, 2, kS>(xr, ar, K, b0, b1, nb, dst);
+        } else if (nm == 2) {
+          if constexpr (kMT >= 2) {
+            if (kNB == 1 || nb == 1) shrink_groups<T, 2, 1, 4, kS>(one_x, ar, K, b0, b1, 1, dst);
+            else shrink_groups<T, 2, kNB, 2, kS>(xr, ar, K, b0, b1, nb, dst);
           }
+        } else if (nm <= 4) {
+          if constexpr (kMT >= 4) {
+            if (kNB == 1 || nb == 1) shrink_groups<T, 4, 1, 2, kS>(one_x, ar, K, b0, b1, 1, dst);
+            else shrink_groups<T, 4, kNB, 1, kS>(xr, ar, K, b0, b1, nb, dst);
+          }
+        } else if constexpr (kMT >= 8) {
+          shrink_groups<T, 8, 1, 1, kS>(one_x, ar, K, b0, b1, 1, dst);
         }
       }
-#pragma unroll
-      for (int m = 0; m < kMT; ++m) {
-        float* dst = part[warp][u] + (m * 16 + g) * 8 + 2 * q;
-        *reinterpret_cast<float2*>(dst) = make_float2(acc[m][0], acc[m][1]);
-        *reinterpret_cast<float2*>(dst + 64) = make_float2(acc[m][2], acc[m][3]);
+      __syncthreads();
+      // The warps' sums, and with a cluster the CTAs': value i (of the batch's kRP x 8 a group) is summed by CTA
+      // i / segment, which the others send theirs and which sends the sum to all.
+      // The finished sums take the place of the first warp's.
+      float* const s_sum = &part[0][0][0];
+      const int values = batch * kRP * 8, segment = (values + kparts - 1) / kparts;
+      for (int i = tid; i < values; i += kShrinkThreads) {
+        float v = part[0][0][i];
+        for (int w = 1; w < subs; ++w) v += part[w][0][i];
+        if (kparts == 1) {
+          s_sum[i] = v;
+        } else {
+          const int owner = i / segment;
+          st_cluster_f32(map_to_cta(smem_u32(&s_in[crank * segment + i - owner * segment]), owner), __float_as_uint(v));
+        }
       }
-    }
-    __syncthreads();
-    for (int i = tid; i < batch * kRP * 8; i += kShrinkThreads) {
-      const int u = i / (kRP * 8), j = i % (kRP * 8);
-      float v = part[0][u][j];
+      if (kparts > 1) {
+        cluster_sync_all();
+        for (int i = tid; i < min(segment, values - crank * segment); i += kShrinkThreads) {
+          float v = s_in[i];
+          for (int c = 1; c < kparts; ++c) v += s_in[c * segment + i];
+          const uint32_t at = smem_u32(&s_sum[crank * segment + i]);
+          for (int c = 0; c < kparts; ++c) st_cluster_f32(map_to_cta(at, c), __float_as_uint(v));
+        }
+        cluster_sync_all();
+      } else {
+        __syncthreads();
+      }
+      // S of each group, one warp a group; every CTA needs all of them for the second product
+      const int u_step = kToGlobal ? kShrinkWarps * kparts : kShrinkWarps;
+      for (int u = kToGlobal ? warp * kparts + crank : warp; u < batch; u += u_step) {
+        const uint32_t e = s.eff[s.start[first + u]];
+        const int rank = rank_of(e), row = s.rows[first + u][lane & 7];
+        float v[kRP / 4];
+        float top = 0.f;
 #pragma unroll
-      for (int w = 1; w < kShrinkWarps; ++w) v += part[w][u][j];
-      part[0][u][j] = v;
-    }
-    if (kparts > 1) cluster_sync_all();
-    else __syncthreads();
-    // group u of the batch is finished by CTA u % kparts of the cluster, one warp a group
-    for (int u = warp * kparts + crank; u < batch; u += kShrinkWarps * kparts) {
-      const int grp = slice + (first + u) * slices;
-      const uint32_t e = s_eff[s_start[grp]];
-      const int rank = rank_of(e), row = s_rows[grp][lane & 7];
-      float v[kRP / 4];
-      float top = 0.f;
+        for (int i = 0; i < kRP / 4; ++i) v[i] = (lane >> 3) + 4 * i < rank ? s_sum[u * kRP * 8 + lane + 32 * i] : 0.f;
 #pragma unroll
-      for (int i = 0; i < kRP / 4; ++i) {
-        const int j = (lane >> 3) + 4 * i;
-        v[i] = 0.f;
-        if (j < rank) {
-          const uint32_t at = smem_u32(&part[0][u][j * 8 + (lane & 7)]);
-          if (kparts > 1) {
-            for (int c = 0; c < kparts; ++c) v[i] += ld_cluster_f32(map_to_cta(at, c));
-          } else {
-            v[i] = part[0][u][j * 8 + (lane & 7)];
-          }
+        for (int i = 0; i < kRP / 4; ++i) {
           top = fmaxf(top, fabsf(v[i]));
           if (!(fabsf(v[i]) <= 3.402823466e38f)) top = __int_as_float(0x7f800000);
         }
-      }
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-      // 2^exp: the largest magnitude over 1..2; a row that is all zero or not finite stays as it is
-      int ex = 0;
-      if (top > 0.f && top <= 3.402823466e38f) ex = max(-126, min(126, ilogbf(top)));
-      const float down = scalbnf(1.f, -ex);
-      if (row >= 0) {
-        const size_t at = static_cast<size_t>(t0 + row) * p.r_pad;
-        T* hi = static_cast<T*>(p.s_hi) + at;
-        T* lo = static_cast<T*>(p.s_lo) + at;
-        if (lane < 8) p.factor[t0 + row] = p.slot_scale[slot_of(e)] * scalbnf(1.f, ex);
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        const int ex = row_exponent(top);
+        const float down = scalbnf(1.f, -ex), fac = p.slot_scale[slot_of(e)] * scalbnf(1.f, ex);
+        if (kToGlobal && row < 0) continue;  // (no warp-wide step follows in this branch)
+        const size_t at = kToGlobal ? static_cast<size_t>(t0 + row) * p.r_pad : 0;
+        T* hi = kToGlobal ? static_cast<T*>(p.s_hi) + at : s_hi[u][lane & 7];
+        T* lo = kToGlobal ? static_cast<T*>(p.s_lo) + at : s_lo[u][lane & 7];
+        if (lane < 8) *(kToGlobal ? p.factor + t0 + row : &s_fac[u][lane]) = fac;
 #pragma unroll
         for (int i = 0; i < kRP / 4; ++i) {
           const int j = (lane >> 3) + 4 * i;
-          if (j < ((rank + 15) & ~15)) {
-            const float w = v[i] * down;
-            const T h = from_f32<T>(w);
-            const float rest = w - to_f32(h);
-            hi[j] = h;
-            lo[j] = from_f32<T>(fabsf(w) <= 4.f ? rest : 0.f);  // not finite: the high half says it all
-          }
+          if (j < ((rank + 15) & ~15)) halves<T>(v[i] * down, hi[j], lo[j]);
         }
       }
+      __syncthreads();
+      if constexpr (!kToGlobal) {
+        // the warps divide the groups first here too
+        const int at_once = batch >= 8 ? 8 : batch >= 4 ? 4 : batch >= 2 ? 2 : 1;
+        const int pieces = kShrinkWarps / at_once, piece = warp / at_once;
+        const int f0_ = nb0 + (nb1 - nb0) * piece / pieces, f1_ = nb0 + (nb1 - nb0) * (piece + 1) / pieces;
+        for (int u = warp % at_once; u < batch; u += at_once) {
+          const uint32_t e = s.eff[s.start[first + u]];
+          const int nm = (rank_of(e) + 15) >> 4;
+          int row0 = s.rows[first + u][2 * q], row1 = s.rows[first + u][2 * q + 1];
+          row0 = row0 < 0 ? -1 : t0 + row0;
+          row1 = row1 < 0 ? -1 : t0 + row1;
+          const float f0 = s_fac[u][2 * q], f1 = s_fac[u][2 * q + 1];
+          const T* hi = s_hi[u][g];
+          const T* lo = s_lo[u][g];
+          if (nm == 1) expand_group<T, 1, 8>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
+          else if (nm == 2) {
+            if constexpr (kMT >= 2) expand_group<T, 2, 4>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
+          } else if (nm <= 4) {
+            if constexpr (kMT >= 4) expand_group<T, 4, 2>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
+          } else if constexpr (kMT >= 8) {
+            expand_group<T, 8, 1>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
+          }
+        }
+        __syncthreads();
+      }
     }
-    if (kparts > 1) cluster_sync_all();  // peers have read this CTA's sums
-    else __syncthreads();
+    __syncthreads();
   }
 }
 
 // ============================================================================ GEMM + expand
-constexpr int kGemmThreads = 256;
+constexpr int kEpiWarps = 8;
+constexpr int kGemmThreads = 64 + 32 * kEpiWarps;
 constexpr int kWRows = 128;  // output features a tile: the M of the MMA
 constexpr int kBK = 64;      // K elements of a stage: one 128-byte swizzle row
 constexpr int kWBytes = kWRows * kBK * 2;
+constexpr int kMaxStages = 28;
 
 struct RowsGemm {
   RowsArgs a;
   int ksplit, stages;
+  int sub;  // 64-element K blocks of a stage
   uint32_t idesc;
 };
 
-__device__ __forceinline__ void tmem_ld_16x256(uint32_t taddr, float (&v)[4]) {
-  uint32_t r[4];
-  asm volatile("tcgen05.ld.sync.aligned.16x256b.x1.b32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(taddr));
-  tmem_wait_ld();
-#pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(r[i]);
+// 32 tensor-memory lanes x kN columns, a lane's row in its registers.
+template <int kN>
+__device__ __forceinline__ void tmem_ld_rows(uint32_t taddr, uint32_t (&v)[kN]) {
+  static_assert(kN == 8 || kN == 32, "instruction shapes in use");
+  if constexpr (kN == 32) {
+    tmem_ld32(taddr, v);
+  } else {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7])
+                 : "r"(taddr));
+  }
 }
-__device__ __forceinline__ void st_cluster_v4(uint32_t addr, const float (&v)[4]) {
-  asm volatile("st.shared::cluster.v4.f32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "f"(v[0]), "f"(v[1]), "f"(v[2]),
-               "f"(v[3])
-               : "memory");
-}
-
-// c (16 output features x 8 rows, fragment layout) += s_i S B_i^T for the rows' adapters.  eff: adapter of
-// row g of the 8; f0, f1: factors of rows 2q, 2q + 1.  Each distinct adapter of the 8 rows takes its
-// own MMAs, and its result only reaches its own rows: values of another adapter that are not finite
-// stay with their rows.
 template <typename T>
-__device__ __forceinline__ void expand8(const RowsArgs& p, float (&c)[4], int n_base, int tok0, uint32_t eff, float f0,
-                                        float f1) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  if (__ballot_sync(0xffffffffu, eff != kNoSlot) == 0) return;
-  uint32_t e[8];
-  uint32_t lead = 0;
-  int steps = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    e[i] = __shfl_sync(0xffffffffu, eff, 4 * i);
-    bool first = e[i] != kNoSlot;
-#pragma unroll
-    for (int j = 0; j < i; ++j) first = first && e[j] != e[i];
-    if (first) {
-      lead |= 1u << i;
-      steps = max(steps, (rank_of(e[i]) + 15) >> 4);
-    }
-  }
-  const uint32_t col0 = __shfl_sync(0xffffffffu, eff, 8 * q), col1 = __shfl_sync(0xffffffffu, eff, 8 * q + 4);
-  const T* bank = static_cast<const T*>(p.b_bank);
-  const bool ok0 = n_base + g < p.N, ok1 = n_base + g + 8 < p.N;
-  const size_t srow = static_cast<size_t>(eff != kNoSlot ? tok0 + g : 0) * p.r_pad + 4 * q;
-  const T* hi = static_cast<const T*>(p.s_hi) + srow;
-  const T* lo = static_cast<const T*>(p.s_lo) + srow;
-  const uint2 zero = make_uint2(0, 0);
-  float d[4] = {0.f, 0.f, 0.f, 0.f};
-  for (int k = 0; k < steps; ++k) {
-    const bool live = eff != kNoSlot && 16 * k < rank_of(eff);
-    const uint2 sh = live ? *reinterpret_cast<const uint2*>(hi + 16 * k) : zero;
-    const uint2 sl = live ? *reinterpret_cast<const uint2*>(lo + 16 * k) : zero;
-    uint2 u[8], v[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      u[i] = v[i] = zero;
-      if ((lead >> i & 1u) && 16 * k < rank_of(e[i])) {
-        const T* b = bank + (static_cast<size_t>(slot_of(e[i])) * p.N + n_base + g) * p.r_pad + 16 * k + 4 * q;
-        if (ok0) u[i] = *reinterpret_cast<const uint2*>(b);
-        if (ok1) v[i] = *reinterpret_cast<const uint2*>(b + static_cast<size_t>(8) * p.r_pad);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if ((lead >> i & 1u) && 16 * k < rank_of(e[i])) {
-        const bool m = eff == e[i];
-        float t[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(t, u[i].x, v[i].x, u[i].y, v[i].y, m ? sh.x : 0u, m ? sh.y : 0u, static_cast<T*>(nullptr));
-        mma16816(t, u[i].x, v[i].x, u[i].y, v[i].y, m ? sl.x : 0u, m ? sl.y : 0u, static_cast<T*>(nullptr));
-        if (col0 == e[i]) d[0] += t[0], d[2] += t[2];
-        if (col1 == e[i]) d[1] += t[1], d[3] += t[3];
-      }
-    }
-  }
-  if (col0 != kNoSlot) c[0] += f0 * d[0], c[2] += f0 * d[2];
-  if (col1 != kNoSlot) c[1] += f1 * d[1], c[3] += f1 * d[3];
-}
+__device__ __forceinline__ uint32_t pack_pair(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) { return pack_bf16x2(a, b); }
+template <>
+__device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) { return pack_f16x2(a, b); }
 
-// Writes a fragment (16 features x 8 rows) to y through 256 bytes of the warp's shared memory, 16 bytes
-// a store (N is a multiple of 8).
-template <typename T>
-__device__ __forceinline__ void store8rows(const RowsArgs& p, const float (&c)[4], int n_base, int tok0, T* stage) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  __syncwarp();
-  stage[(2 * q) * 16 + g] = from_f32<T>(c[0]);
-  stage[(2 * q + 1) * 16 + g] = from_f32<T>(c[1]);
-  stage[(2 * q) * 16 + g + 8] = from_f32<T>(c[2]);
-  stage[(2 * q + 1) * 16 + g + 8] = from_f32<T>(c[3]);
-  __syncwarp();
-  if (lane < 16) {
-    const int t = tok0 + (lane >> 1), n = n_base + 8 * (lane & 1);
-    if (t < p.T && n < p.N)
-      *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + static_cast<size_t>(t) * p.N + n) =
-          *reinterpret_cast<const uint4*>(stage + (lane >> 1) * 16 + 8 * (lane & 1));
-  }
-}
-
-// kTN: rows (tokens) of a tile, the N of the MMA.
+// kTN: rows (tokens) of a tile, the N of the MMA.  Warp 0 loads, warp 1 issues the MMAs, eight epilogue warps
+// finish the tile.
 template <typename T, int kTN>
-__global__ void __launch_bounds__(kGemmThreads)
+__global__ void __maxnreg__(80)
     rows_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ RowsGemm prm) {
   constexpr int kXBytes = kTN * kBK * 2;
-  constexpr int kStageBytes = kWBytes + kXBytes;
   constexpr int kCols = kTN < 32 ? 32 : kTN;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ uint64_t full[16], empty[16], acc_bar, drain_bar;
+  __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_bar, drain_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
-  __shared__ uint32_t s_eff[kTN];
-  __shared__ float s_fac[kTN];
-  __shared__ __align__(16) T s_stage[8][128];
+  __shared__ uint8_t s_on[kTN];  // whether the row has an adapter
   const RowsArgs& p = prm.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int w_bytes = kWBytes, block_bytes = w_bytes + kXBytes;
+  // A stage holds `sub` blocks of 64 elements of K.  A block costs the loading thread two copies and the MMA
+  // thread four MMAs, but each wait costs both about 0.1 us: with one block a stage, a tile of few rows took 0.35 us
+  // a block however small its bytes.
+  const int sub = prm.sub, stage_bytes = sub * block_bytes;
   const int ks = prm.ksplit, stages = prm.stages;
   const int part = blockIdx.x % ks;  // rank in the cluster
   const int n0 = blockIdx.x / ks * kWRows;
@@ -417,15 +577,18 @@ __global__ void __launch_bounds__(kGemmThreads)
       int stage = 0;
       uint32_t phase = 0, issued = 0, parity = 0;
       bool ok = true;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
+      for (int kb = kb0; kb < kb1; kb += sub) {
+        if (!mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
           ok = false;
           break;
         }
-        uint8_t* w = ring + stage * kStageBytes;
-        mbar_arrive_expect_tx(&full[stage], kStageBytes);
-        tma_load_2d(w, &map_w, &full[stage], kb * kBK, n0);
-        tma_load_2d(w + kWBytes, &map_x, &full[stage], kb * kBK, t0);
+        uint8_t* w = ring + stage * stage_bytes;
+        const int n = min(sub, kb1 - kb);
+        mbar_arrive_expect_tx(&full[stage], n * block_bytes);
+        for (int i = 0; i < n; ++i, w += block_bytes) {
+          tma_load_2d(w, &map_w, &full[stage], (kb + i) * kBK, n0);
+          tma_load_2d(w + w_bytes, &map_x, &full[stage], (kb + i) * kBK, t0);
+        }
         issued |= 1u << stage;
         parity = (parity & ~(1u << stage)) | (phase << stage);
         if (++stage == stages) {
@@ -443,18 +606,23 @@ __global__ void __launch_bounds__(kGemmThreads)
       int stage = 0;
       uint32_t phase = 0, acc = 0;
       bool ok = true;
-      const uint32_t base = smem_u32(ring);
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
+      // descriptors of the first block; addresses are in 16-byte units in their low bits
+      const uint64_t w0 = umma_sdesc(smem_u32(ring), 16, 1024, 2);
+      for (int kb = kb0; kb < kb1; kb += sub) {
+        if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t w = base + stage * kStageBytes, x = w + kWBytes;
+        const int n = min(sub, kb1 - kb);
+        uint64_t w = w0 + ((stage * stage_bytes) >> 4);
+        for (int i = 0; i < n; ++i, w += block_bytes >> 4) {
+          const uint64_t x = w + (w_bytes >> 4);
 #pragma unroll
-        for (int k = 0; k < kBK / 16; ++k) {
-          umma_f16(tmem, umma_sdesc(w + k * 32, 16, 1024, 2), umma_sdesc(x + k * 32, 16, 1024, 2), prm.idesc, acc);
-          acc = 1;
+          for (int k = 0; k < kBK / 16; ++k) {
+            umma_f16(tmem, w + 2 * k, x + 2 * k, prm.idesc, acc);
+            acc = 1;
+          }
         }
         umma_commit(&empty[stage]);
         if (++stage == stages) {
@@ -471,84 +639,62 @@ __global__ void __launch_bounds__(kGemmThreads)
     }
     __syncwarp();
   } else {
-    // B_i of the rows this CTA will expand, into L2
-    const int own = kWRows / ks;  // output features this CTA finishes
-    const int nb = n0 + part * own;
-    const int feats = min(own, p.N - nb);
-    if (feats > 0) {
-      const uint32_t bytes = static_cast<uint32_t>(feats) * p.r_pad * 2, lines = (bytes + 127) / 128;
-      const int n_rows = min(kTN, p.T - t0);
-      for (int r = warp - 2; r < n_rows; r += 6) {
-        const uint32_t e = row_adapter(p, t0 + r, false);
-        if (e == kNoSlot || (r > 0 && row_adapter(p, t0 + r - 1, false) == e)) continue;
-        const char* b = static_cast<const char*>(p.b_bank) +
-                        (static_cast<size_t>(slot_of(e)) * p.N + nb) * p.r_pad * 2;
-        for (uint32_t l = lane; l < lines; l += 32)
-          asm volatile("prefetch.global.L2 [%0];" ::"l"(b + static_cast<size_t>(l) * 128));
-      }
-    }
+    for (int i = tid - 64; i < kTN; i += kEpiWarps * 32)
+      s_on[i] = t0 + i < p.T && row_adapter(p, t0 + i, false) != kNoSlot;
+    named_barrier(1, kEpiWarps * 32);
   }
-  bool ok = warp_wait(&acc_bar, 0, &abort_flag, p.err, kErrTimeoutAcc);
+  const bool ok = warp_wait(&acc_bar, 0, &abort_flag, p.err, kErrTimeoutAcc);
   tc_fence_after();
-  pdl_wait();  // the shrink's results
-  for (int i = tid; i < kTN; i += kGemmThreads) {
-    const bool in = t0 + i < p.T;
-    const uint32_t e = in ? p.eff[t0 + i] : kNoSlot;
-    s_eff[i] = e;
-    s_fac[i] = e != kNoSlot ? p.factor[t0 + i] : 0.f;
-  }
-  __syncthreads();
 
-  const int g = lane >> 2, q = lane & 3;
-  const int quad = warp & 3, half = warp >> 2;  // tensor-memory lanes of the warp; which row groups it takes
-  constexpr int kGroups = kTN / 8;
-  const int n_groups = min(kGroups, (p.T - t0 + 7) / 8);
-  T* stage_out = s_stage[warp];
-  if (ks == 1) {
-    if (ok) {
-      for (int c = half; c < n_groups; c += 2) {
+  // The accumulator goes through the idle ring as [source CTA][row][feature], float32, so that a thread then
+  // holds 8 features of a row.  Every CTA of the cluster finishes its own share of the features and gets
+  // the others' partial sums of it.
+  const int ew = warp - 2, quad = warp & 3;
+  const int own = kWRows / ks, rows = min(kTN, p.T - t0);
+  if (ks > 1) cluster_sync_all();  // every ring is idle
+  if (ok && ew >= 0) {
+    constexpr int kN = kTN >= 64 ? 32 : 8;  // rows a load
+    constexpr int kHalf = kTN / 2;          // the two warps of a lane quarter take half the rows each
+    const int f = quad * 32 + lane, first = (ew >> 2) * kHalf;
+    uint32_t at = smem_u32(ring) + static_cast<uint32_t>((part * kTN * own + (f & (own - 1))) * 4);
+    if (ks > 1) at = map_to_cta(at, f / own);
+#pragma unroll 1
+    for (int r = first; r < min(first + kHalf, rows); r += kN) {
+      uint32_t v[kN];
+      tmem_ld_rows<kN>(tmem + (static_cast<uint32_t>(quad * 32) << 16) + r, v);
+      tmem_wait_ld();
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int n_base = n0 + quad * 32 + h * 16;
-          float v[4];
-          tmem_ld_16x256(tmem + (static_cast<uint32_t>(quad * 32 + h * 16) << 16) + c * 8, v);
-          if (n_base < p.N) {
-            expand8<T>(p, v, n_base, t0 + c * 8, s_eff[c * 8 + g], s_fac[c * 8 + 2 * q], s_fac[c * 8 + 2 * q + 1]);
-            store8rows<T>(p, v, n_base, t0 + c * 8, stage_out);
-          }
-        }
-      }
+      for (int i = 0; i < kN; ++i) st_cluster_f32(at + static_cast<uint32_t>((r + i) * own * 4), v[i]);
     }
-  } else {
-    // every CTA of the cluster finishes kWRows / ks features: the others send it their partial sums
-    const int per = 8 / ks;      // 16-feature blocks a CTA finishes
-    cluster_sync_all();          // every ring is idle
-    if (ok) {
-      for (int c = half; c < n_groups; c += 2) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int mt = quad * 2 + h;
-          float v[4];
-          tmem_ld_16x256(tmem + (static_cast<uint32_t>(mt * 16) << 16) + c * 8, v);
-          const uint32_t at = smem_u32(ring) + static_cast<uint32_t>(((part * per + mt % per) * kGroups + c) * 512 + lane * 16);
-          st_cluster_v4(map_to_cta(at, mt / per), v);
-        }
+  }
+  if (ks > 1) cluster_sync_all();
+  else __syncthreads();
+  pdl_wait();  // the adapters' part
+  if (ok) {
+    const int nb = n0 + part * own;                       // this CTA's features
+    const int shift = 4 - (31 - __clz(ks));               // log2 of 8-feature pieces a row
+    const float* sums = reinterpret_cast<const float*>(ring);
+    const int pitch = (p.N + 15) & ~15;
+    for (int i = tid; i < rows << shift; i += kGemmThreads) {
+      const int r = i >> shift, f = (i & ((1 << shift) - 1)) * 8, n = nb + f;
+      if (n >= p.N) continue;  // N is a multiple of 8
+      float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
+      if (s_on[r]) {
+        const float4* d = reinterpret_cast<const float4*>(p.delta + static_cast<size_t>(t0 + r) * pitch + n);
+        lo = d[0], hi = d[1];
       }
-    }
-    cluster_sync_all();
-    if (ok) {
-      for (int u = warp; u < per * n_groups; u += 8) {
-        const int m = u / n_groups, c = u % n_groups;
-        const int n_base = n0 + (part * per + m) * 16;
-        if (n_base >= p.N) continue;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < ks; ++s) {  // fixed order
-          const float4 w = *reinterpret_cast<const float4*>(ring + ((s * per + m) * kGroups + c) * 512 + lane * 16);
-          v[0] += w.x, v[1] += w.y, v[2] += w.z, v[3] += w.w;
-        }
-        expand8<T>(p, v, n_base, t0 + c * 8, s_eff[c * 8 + g], s_fac[c * 8 + 2 * q], s_fac[c * 8 + 2 * q + 1]);
-        store8rows<T>(p, v, n_base, t0 + c * 8, stage_out);
+      float4 a0 = make_float4(0.f, 0.f, 0.f, 0.f), a1 = a0;
+      for (int c = 0; c < ks; ++c) {  // fixed order
+        const float4* w = reinterpret_cast<const float4*>(sums + (c * kTN + r) * own + f);
+        a0.x += w[0].x, a0.y += w[0].y, a0.z += w[0].z, a0.w += w[0].w;
+        a1.x += w[1].x, a1.y += w[1].y, a1.z += w[1].z, a1.w += w[1].w;
       }
+      uint4 y;
+      y.x = pack_pair<T>(a0.x + lo.x, a0.y + lo.y);
+      y.y = pack_pair<T>(a0.z + lo.z, a0.w + lo.w);
+      y.z = pack_pair<T>(a1.x + hi.x, a1.y + hi.y);
+      y.w = pack_pair<T>(a1.z + hi.z, a1.w + hi.w);
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.y) + static_cast<size_t>(t0 + r) * p.N + n) = y;
     }
   }
   tc_fence_before();
@@ -641,9 +787,13 @@ __global__ void __launch_bounds__(256) rows_gemm_simt_kernel(const RowsArgs p) {
       if (n >= p.N) continue;
       float v = acc[i][j];
       if (e != kNoSlot) {
-        const T* b = static_cast<const T*>(p.b_bank) + (static_cast<size_t>(slot_of(e)) * p.N + n) * p.r_pad;
+        // feature n of its block of 16, rank r of its step of 16: place 8 (4 (n % 8) + r / 4) + 4 (n / 8) + r % 4
+        const int blocks = (p.N + 15) >> 4, f = n & 15;
+        const T* b = static_cast<const T*>(p.b_bank) +
+                     (static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) * blocks + (n >> 4)) * 256 + (f & 7) * 32 + (f >> 3) * 4;
         float add = 0.f;
-        for (int r = 0; r < rank_of(e); ++r) add = fmaf(s[r], to_f32(b[r]), add);
+        for (int r = 0; r < rank_of(e); ++r)
+          add = fmaf(s[r], to_f32(b[static_cast<size_t>(r >> 4) * blocks * 256 + (r >> 2 & 3) * 8 + (r & 3)]), add);
         v += add;
       }
       static_cast<T*>(p.y)[static_cast<size_t>(t) * p.N + n] = from_f32<T>(v);
@@ -651,7 +801,8 @@ __global__ void __launch_bounds__(256) rows_gemm_simt_kernel(const RowsArgs p) {
   }
 }
 
-// Opts a kernel into its dynamic shared memory once per device.
+// Opts a kernel into its dynamic shared memory once per device, and into the SM's largest shared-memory
+// split (a kernel with a smaller one would keep the dependent GEMM's CTAs off its SMs).
 cudaError_t allow_smem(const void* kernel, int bytes) {
   struct Done {
     const void* fn;
@@ -667,54 +818,62 @@ cudaError_t allow_smem(const void* kernel, int bytes) {
   for (int i = 0; i < n; ++i)
     if (done[i].fn == kernel && done[i].dev == dev) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
   if (e == cudaSuccess && n < 256) done[n++] = Done{kernel, dev};
   return e;
 }
 
-constexpr int kRingBytes = 160 * 1024;  // largest ring: leaves room for a shrink CTA beside it
+// Shared memory of the stages.  Enough to keep HBM busy, little enough to leave room for a CTA of the
+// adapters' kernel beside it, and more than a third of an SM, so that CTAs that share one always find
+// tensor memory.  The epilogue passes kTN * 512 bytes of sums through it.
+constexpr int ring_bytes(int tn) { return tn > 256 ? 0 : 160 * 1024; }
+static_assert(ring_bytes(256) >= 256 * 512, "the sums fit the ring");
 
 template <typename T, int kTN>
 cudaError_t launch_gemm(const RowsGemm& g, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t st) {
-  const int stage = kWBytes + kTN * kBK * 2;
-  const int smem = g.stages * stage + 1024;
   auto* k = rows_gemm_kernel<T, kTN>;
-  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), kRingBytes + 1024);
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), ring_bytes(kTN) + 1024);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>((g.a.N + kWRows - 1) / kWRows * g.ksplit),
                   static_cast<unsigned>((g.a.T + kTN - 1) / kTN));
-  return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), smem, st, true, w, x, g);
+  return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), ring_bytes(kTN) + 1024, st, true, w, x, g);
 }
 
 template <typename T>
-cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int tn, int num_sms,
-                    cudaStream_t st) {
-  // shrink: enough CTAs to fill the GPU once, K cut first (a cluster of up to 8), then the groups
+cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int tn, int ksplit,
+                    int num_sms, cudaStream_t st) {
+  // the adapters' part: one CTA an SM, beside the GEMM's; few rows are cut over a larger cluster
   const int tiles = (a.T + kTileRows - 1) / kTileRows;
-  int kparts = a.T <= 16 ? 8 : 4;
+  int kparts = tiles == 1 ? 8 : tiles <= 16 ? 4 : 1;
   while (kparts > 1 && (a.K + 31) / 32 < kparts * kShrinkWarps) kparts /= 2;
-  int slices = 2 * num_sms / (tiles * kparts);
+  const int clusters = num_sms / kparts;
+  int slices = clusters / tiles;
   slices = slices < 1 ? 1 : slices > kTileRows ? kTileRows : slices;
   if (slices > a.T) slices = a.T;
-  const dim3 grid(static_cast<unsigned>(tiles) * slices * kparts);
+  const dim3 grid(static_cast<unsigned>((tiles * slices < clusters ? tiles * slices : clusters) * kparts));
   cudaError_t e;
-#define LF_SHRINK(MT) \
-  e = launch_cluster(rows_shrink_kernel<T, MT>, grid, kparts, dim3(kShrinkThreads), 0, st, false, a, slices, kparts)
-  if (a.r_pad == 16) LF_SHRINK(1);
-  else if (a.r_pad == 32) LF_SHRINK(2);
-  else if (a.r_pad == 64) LF_SHRINK(4);
-  else LF_SHRINK(8);
-#undef LF_SHRINK
+#define LF_LORA(MT, NB)                                                                                             \
+  {                                                                                                                 \
+    e = allow_smem(reinterpret_cast<const void*>(rows_lora_kernel<T, MT, NB, false>), 0);                            \
+    if (e != cudaSuccess) return e;                                                                                 \
+    e = launch_cluster(rows_lora_kernel<T, MT, NB, false>, grid, kparts, dim3(kShrinkThreads), 0, st, false, a, slices, \
+                       kparts);                                                                                     \
+  }
+  if (a.r_pad == 16) LF_LORA(1, 4)
+  else if (a.r_pad == 32) LF_LORA(2, 4)
+  else if (a.r_pad == 64) LF_LORA(4, 2)
+  else LF_LORA(8, 1)
+#undef LF_LORA
   if (e != cudaSuccess) return e;
 
   RowsGemm g{};
   g.a = a;
   g.idesc = umma_idesc_f16(kWRows, tn, dtype == LF_BF16 ? 1 : 0, 0, 0);
-  const int64_t out_tiles = static_cast<int64_t>((a.N + kWRows - 1) / kWRows) * ((a.T + tn - 1) / tn);
-  const int nkb = (a.K + kBK - 1) / kBK;
-  g.ksplit = 1;
-  while (g.ksplit < 8 && out_tiles * g.ksplit * 2 <= num_sms && nkb >= g.ksplit * 2 * 4) g.ksplit *= 2;
-  const int stage = kWBytes + tn * kBK * 2;
-  g.stages = kRingBytes / stage < 12 ? kRingBytes / stage : 12;
+  g.ksplit = ksplit;
+  const int room = ring_bytes(tn), block = (kWRows + tn) * kBK * 2;
+  g.sub = room / (2 * block) >= 3 ? 2 : 1;
+  g.stages = room / (g.sub * block);
   if (tn == 16) return launch_gemm<T, 16>(g, w, x, st);
   if (tn == 32) return launch_gemm<T, 32>(g, w, x, st);
   if (tn == 64) return launch_gemm<T, 64>(g, w, x, st);
@@ -732,13 +891,24 @@ cudaError_t rows_simt_t(const RowsArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-int rows_tile(int T) { return T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256; }
+RowsTiles rows_tiles(int T, int K, int N, int num_sms) {
+  RowsTiles t{};
+  t.rows = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
+  // K is split while the tiles leave more than half of the SMs without one and a part has 256 elements.
+  // (Smaller tiles that cover every SM were slower: 32 features a tile and no split took 20 us where
+  // 128 features and a split in four takes 12.6, at 1 x 4096 -> 4096, and a GPU without free SMs cannot place the
+  // adapters' CTAs beside the GEMM's.)
+  const int64_t tiles = static_cast<int64_t>((N + kWRows - 1) / kWRows) * ((T + t.rows - 1) / t.rows);
+  const int nkb = (K + kBK - 1) / kBK;
+  t.ksplit = 1;
+  while (t.ksplit < 8 && tiles * t.ksplit * 2 <= num_sms && nkb >= t.ksplit * 2 * 4) t.ksplit *= 2;
+  return t;
+}
 
-cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int num_sms,
-                            cudaStream_t st) {
-  const int tn = rows_tile(a.T);
-  return dtype == LF_BF16 ? rows_tc<__nv_bfloat16>(a, dtype, w, x, tn, num_sms, st)
-                          : rows_tc<__half>(a, dtype, w, x, tn, num_sms, st);
+cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
+                            int num_sms, cudaStream_t st) {
+  return dtype == LF_BF16 ? rows_tc<__nv_bfloat16>(a, dtype, w, x, t.rows, t.ksplit, num_sms, st)
+                          : rows_tc<__half>(a, dtype, w, x, t.rows, t.ksplit, num_sms, st);
 }
 
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st) {

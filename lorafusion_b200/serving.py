@@ -54,7 +54,11 @@ class AdapterBank:
         self.dtype, self.device = dtype, device
         self.r_pad = next(r for r in (16, 32, 64, nat.BANK_MAX_RANK) if max_rank <= r)
         self.lora_a = torch.zeros(n_slots, self.r_pad, in_features, dtype=dtype, device=device)
-        self.lora_b = torch.zeros(n_slots, out_features, self.r_pad, dtype=dtype, device=device)
+        # B_i in blocks of 16 ranks x 16 features, each in the order of the matrix instruction's operand
+        # ([feature % 8, rank // 4, feature // 8, rank % 4]): a lane's part of a block is one 16-byte load, and
+        # what is read of an adapter is contiguous whatever its rank
+        self.lora_b = torch.zeros(n_slots, self.r_pad // 16, -(-out_features // 16), 8, 4, 2, 4, dtype=dtype,
+                                  device=device)
         self.ranks = torch.zeros(n_slots, dtype=torch.int32, device=device)
         self.scales = torch.zeros(n_slots, dtype=torch.float32, device=device)
 
@@ -72,10 +76,11 @@ class AdapterBank:
         if not 0 < r <= self.max_rank:
             raise ValueError(f"slot {slot}: rank {r} is outside 1 .. {self.max_rank}")
         self.lora_a[slot, :r] = lora_a
-        self.lora_b[slot, :, :r] = lora_b
         if r < self.r_pad:  # the kernels read zeros past the rank
             self.lora_a[slot, r:] = 0
-            self.lora_b[slot, :, r:] = 0
+        blocks = self.lora_b.shape[2]
+        lora_b = torch.nn.functional.pad(lora_b, (0, self.r_pad - r, 0, 16 * blocks - self.out_features))
+        self.lora_b[slot] = lora_b.view(blocks, 2, 8, self.r_pad // 16, 4, 4).permute(3, 0, 2, 4, 1, 5)
         self.scales[slot] = float(scaling)
         self.ranks[slot] = r
 
@@ -100,6 +105,13 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     out_features is not a multiple of 8, or whose buffers are not 16-byte aligned, run on CUDA cores
     with a ``CudaCorePathWarning``.
     """
+    y = nat.glue().rows_forward(
+        x, base_weight, bank.lora_a, bank.lora_b, bank.ranks, bank.scales, row_slot, out, bank.r_pad,
+        bank.out_features) if bank is not None else None
+    if y is not None:
+        b200_ops._last_launches = 2
+        return y
+    # anything that needs a copy, a warning or an error
     if x.dim() != 2:
         raise ValueError(f"x must be 2-D, got shape {tuple(x.shape)}")
     device, dtype = x.device, x.dtype
@@ -146,13 +158,9 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
             p.x_dev, p.ldx = x.data_ptr(), K
         b200_ops._warn_if_cuda_core(dtype, K, N, (x, base_weight, bank.lora_a, bank.lora_b, out))
     L = nat.lib()
-    ws = torch.empty(L.lf_rows_workspace_bytes(T, bank.r_pad, p.dtype), dtype=torch.uint8, device=device)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        rc = L.lf_rows_forward(p, out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
-    else:
-        with torch.cuda.device(device):
-            rc = L.lf_rows_forward(p, out.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    ws = torch.empty(L.lf_rows_workspace_bytes(T, N, bank.r_pad, p.dtype), dtype=torch.uint8, device=device)
+    with nat.on_device(device.index):
+        rc = L.lf_rows_forward(p, out.data_ptr(), ws.data_ptr(), ws.numel(), nat.raw_stream(device.index))
     nat.check(rc, "lf_rows_forward")
     b200_ops._last_launches = 2
     return out

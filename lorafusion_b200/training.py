@@ -47,10 +47,6 @@ def _one_device(tensors, what: str) -> int:
     return devices.pop()
 
 
-def _on(device: int):
-    return torch.cuda.device(device)
-
-
 def clip_adapter_grads(grads: Sequence[Mapping], max_norm: float | None, *, norm_type: float = 2.0,
                        per_adapter: bool = True) -> torch.Tensor:
     """Norm of each adapter's gradients over all dicts of ``grads``, and the gradients clipped in place.
@@ -70,6 +66,11 @@ def clip_adapter_grads(grads: Sequence[Mapping], max_norm: float | None, *, norm
         raise ValueError(f"max_norm must be non-negative, got {max_norm}")
     if norm_type not in (2.0, math.inf):
         raise ValueError(f"norm_type must be 2 or inf, got {norm_type}")
+    grads = list(grads)
+    norms = nat.glue().clip(grads, per_adapter, norm_type != 2.0, None if max_norm is None else float(max_norm))
+    if norms is not None:
+        return norms
+    # anything that is an error, or a mapping that is not a dict
     tensors: list[torch.Tensor] = []
     ids: list = []
     for d in grads:
@@ -104,10 +105,10 @@ def clip_adapter_grads(grads: Sequence[Mapping], max_norm: float | None, *, norm
     at = rec.ctypes.data
     ws = torch.empty(max(16, L.lf_grad_clip_workspace_bytes(at, n, n_groups)), dtype=torch.uint8, device=device)
     norms = torch.empty(n_groups, dtype=torch.float32, device=device)
-    with _on(index):
+    with nat.on_device(index):
         rc = L.lf_grad_clip(at, n, n_groups, int(norm_type != 2.0), int(max_norm is not None),
                             0.0 if max_norm is None else float(max_norm), norms.data_ptr(), ws.data_ptr(), ws.numel(),
-                            torch.cuda.current_stream(device).cuda_stream)
+                            nat.raw_stream(index))
     if rc == nat.LF_ERR_INVALID_ARG:
         raise ValueError("gradients share memory: each may be named once")
     nat.check(rc, "lf_grad_clip")
@@ -185,6 +186,8 @@ class AdapterAdamW:
         nat.check(L.lf_adamw_plan(rec.ctypes.data, n, len(self.ids), chunk_tensor.ctypes.data, n_chunks.value,
                                   ctypes.byref(n_chunks), ctypes.byref(elems)), "lf_adamw_plan")
         self._rec, self._n_chunks = rec, n_chunks.value
+        self._addresses = np.ascontiguousarray(rec["param"])
+        self._ws_bytes = int(L.lf_adamw_workspace_bytes(self._n_chunks, len(self.ids)))
         self._rec_dev = torch.from_numpy(rec.view(np.uint8).copy()).to(self.device)
         self._chunk_dev = torch.from_numpy(chunk_tensor).to(self.device)
         self._hyper_dev = torch.from_numpy(self._hyper.copy()).to(self.device)
@@ -270,47 +273,52 @@ class AdapterAdamW:
         """
         if len(grads) != len(self.params):
             raise ValueError(f"expected {len(self.params)} dicts of gradients, got {len(grads)}")
-        found: list = []
-        for d, keys in zip(grads, self._keys):
-            row = list(map(d.get, keys))
-            if len(d) != len(keys) - row.count(None):
-                raise ValueError(f"gradients of unknown adapters: {[a for a in d if a not in set(keys)]}")
-            found += row
-        full = None not in found
-        present = found if full else [g for g in found if g is not None]
-        if not present:
+        ptrs = np.empty(len(self._tensors), dtype=np.uint64)
+        code = nat.glue().gather_step(grads, self._keys, self._tensors, self._addresses, ptrs)
+        if code is None:
+            code = self._gather(grads, ptrs)
+        if code < 0:
             return self._no_gradients()
-        if _one_device(present, "gradients") != self.device.index:
-            raise ValueError(f"gradients must live on {self.device}")
-        dtypes = set(map(_DTYPE, present))
+        norms = self._launch(ptrs, code)
+        nat.glue().changed(self._tensors, ptrs)
+        return norms
+
+    def _gather(self, grads, ptrs: np.ndarray) -> int:
+        """``gather_step`` with every check on its own, for its error; dicts may be other mappings here."""
+        dtypes, at = set(), 0
+        for d, keys in zip(grads, self._keys):
+            unknown = set(d) - set(keys)
+            if unknown:
+                raise ValueError(f"gradients of unknown adapters: {sorted(unknown, key=str)}")
+            for aid in keys:
+                w, g = self._tensors[at], d.get(aid)
+                if w.data_ptr() != self._addresses[at]:
+                    raise RuntimeError("a weight's storage was replaced: build a new AdapterAdamW")
+                if g is not None:
+                    if g.device != self.device:
+                        raise ValueError(f"gradients must live on {self.device}, got {g.device}")
+                    if not g.is_contiguous():
+                        raise ValueError("gradients must be contiguous")
+                    if g.shape != w.shape:
+                        raise ValueError(f"gradient of adapter {aid} (dict {self._names[at][0]}) has shape "
+                                         f"{tuple(g.shape)}, its weight {tuple(w.shape)}")
+                    dtypes.add(g.dtype)
+                ptrs[at] = 0 if g is None else g.data_ptr()
+                at += 1
+        if not dtypes:
+            return -1
         gdt = dtypes.pop()
         if dtypes or (gdt != torch.float32 and gdt != self.dtype):
             raise ValueError(f"gradients must all be float32 or all {self.dtype}, got {dtypes | {gdt}}")
-        if not all(map(_CONTIGUOUS, present)):
-            raise ValueError("gradients must be contiguous")
-        shapes = self._shapes if full else [s for s, g in zip(self._shapes, found) if g is not None]
-        if list(map(_SHAPE, present)) != shapes:
-            k = next(k for k, (s, g) in enumerate(zip(self._shapes, found)) if g is not None and g.shape != s)
-            raise ValueError(f"gradient of adapter {self._names[k][1]} (dict {self._names[k][0]}) has shape "
-                             f"{tuple(found[k].shape)}, its weight {tuple(self._shapes[k])}")
-        tensors = self._tensors if full else [t for t, g in zip(self._tensors, found) if g is not None]
-        if list(map(_DATA_PTR, self._tensors)) != self._rec["param"].tolist():
-            raise RuntimeError("a weight's storage was replaced: build a new AdapterAdamW")
-        if full:
-            ptrs = np.array(list(map(_DATA_PTR, found)), dtype=np.uint64)
-        else:
-            ptrs = np.array([0 if g is None else g.data_ptr() for g in found], dtype=np.uint64)
-        norms = self._launch(ptrs, gdt)
-        torch.autograd.graph.increment_version(tensors)
-        return norms
+        return _CODE[gdt]
 
     def _no_gradients(self):
         if self.max_norm is None and not self.skip_nonfinite:
             return None
         return torch.zeros(len(self.ids), dtype=torch.float32, device=self.device)
 
-    def _launch(self, ptrs: np.ndarray, gdt: torch.dtype) -> torch.Tensor | None:
-        with _on(self.device.index):
+    def _launch(self, ptrs: np.ndarray, grad_code: int) -> torch.Tensor | None:
+        with nat.on_device(self.device.index):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("AdapterAdamW.step cannot be captured into a CUDA graph: replays would change "
                                    "weights whose packed copies b200_ops keeps")
@@ -321,15 +329,14 @@ class AdapterAdamW:
             L = nat.lib()
             want = self.max_norm is not None or self.skip_nonfinite
             norms = torch.empty(n_groups, dtype=torch.float32, device=self.device) if want else None
-            ws = torch.empty(L.lf_adamw_workspace_bytes(self._n_chunks, n_groups), dtype=torch.uint8,
-                             device=self.device)
+            ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
             args = nat.AdamWArgs(
                 self._rec.ctypes.data, self._rec_dev.data_ptr(), self._chunk_dev.data_ptr(), ptrs.ctypes.data,
                 self._hyper_dev.data_ptr(), self.steps.data_ptr(), self.exp_avg.data_ptr(),
                 self.exp_avg_sq.data_ptr(), None if self.master is None else self.master.data_ptr(),
                 None if norms is None else norms.data_ptr(), ws.data_ptr(), ws.numel(), self._n_chunks, *self.betas,
                 self.eps, -1.0 if self.max_norm is None else float(self.max_norm), len(ptrs), n_groups,
-                _CODE[self.dtype], _CODE[gdt], int(self.skip_nonfinite), 0)
-            nat.check(L.lf_adamw_step(ctypes.byref(args), torch.cuda.current_stream(self.device).cuda_stream),
+                _CODE[self.dtype], grad_code, int(self.skip_nonfinite), 0)
+            nat.check(L.lf_adamw_step(ctypes.byref(args), nat.raw_stream(self.device.index)),
                       "lf_adamw_step")
         return norms

@@ -260,7 +260,9 @@ def test_load_converts_and_clears_past_the_rank():
     _, _, bank, _, _ = make(BF16, 8, 64, 72, [16], 16)
     a, b = torch.randn(5, 64, device="cuda"), torch.randn(72, 5, device="cuda")
     bank.load(0, a, b, 2.0)
-    assert torch.equal(bank.lora_a[0, :5], a.to(BF16)) and torch.equal(bank.lora_b[0, :, :5], b.to(BF16))
-    assert not bank.lora_a[0, 5:].any() and not bank.lora_b[0, :, 5:].any()
+    assert torch.equal(bank.lora_a[0, :5], a.to(BF16)) and not bank.lora_a[0, 5:].any()
+    # blocks of 16 features x 16 ranks as [feature % 8, rank // 4, feature // 8, rank % 4]
+    back = bank.lora_b[0].permute(1, 4, 2, 0, 3, 5).reshape(80, 16)
+    assert torch.equal(back[:72, :5], b.to(BF16)) and not back[72:].any() and not back[:, 5:].any()
     assert bank.ranks.tolist() == [5] and bank.scales.tolist() == [2.0]
     assert np.isclose(bank.lora_a.element_size(), 2)

@@ -68,8 +68,8 @@ def _rows(**kw):
 
 def test_rows_entry_refuses_before_any_launch():
     L = nat.lib()
-    ws = L.lf_rows_workspace_bytes(4, 16, nat.LF_BF16)
-    assert ws == 2 * 256 + 2 * 256
+    ws = L.lf_rows_workspace_bytes(4, 16, 16, nat.LF_BF16)
+    assert ws == 2 * 256 + 2 * 256 + 256 and L.lf_rows_workspace_bytes(4, 16, 16, nat.LF_F32) == 4 * 256
     call = lambda p, y=256, w=256, n=ws: L.lf_rows_forward(p, y, w, n, None)  # noqa: E731
     for kw in (dict(dtype=3), dict(dtype=-1), dict(T=-1), dict(K=-1), dict(N=-1), dict(n_slots=-1), dict(r_pad=8),
                dict(r_pad=256), dict(row_slot_bytes=2), dict(ldx=15), dict(x_dev=None), dict(w_dev=None),
