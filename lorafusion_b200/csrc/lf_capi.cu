@@ -840,7 +840,8 @@ extern "C" int lf_ipc_close(void* dev_ptr) {
 // float32 array on the CUDA-core path: the same bytes), then the adapters' part of the result.
 extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype) {
   if (T < 0 || N < 0 || r_pad < 0) return 0;
-  const size_t delta = dtype == LF_F32 ? 0 : static_cast<size_t>(T) * ((N + 15) / 16 * 16) * 4;
+  const size_t rows = T < kRowsChunk ? T : kRowsChunk;  // long batches run in chunks of rows
+  const size_t delta = dtype == LF_F32 ? 0 : rows * ((N + 15) / 16 * 16) * 4;
   return 2 * align256(static_cast<size_t>(T) * 4) + 2 * align256(static_cast<size_t>(T) * r_pad * 2) + align256(delta);
 }
 
@@ -891,12 +892,43 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     if ((p->T + 31) / 32 > 65535) return LF_ERR_UNSUPPORTED;
     return to_status(rows_forward_simt(a, p->dtype, st));
   }
-  const RowsTiles tiles = rows_tiles(p->T, p->K, p->N, ds->num_sms);
-  CUtensorMap w_map, x_map;
-  if (!make_map(&w_map, p->dtype, p->w_dev, p->K, p->N, static_cast<uint64_t>(p->K) * 2, 64, 128) ||
-      !make_map(&x_map, p->dtype, p->x_dev, p->K, p->T, static_cast<uint64_t>(p->ldx) * 2, 64, tiles.rows))
-    return LF_ERR_UNSUPPORTED;
-  return to_status(rows_forward_tc(a, p->dtype, w_map, x_map, tiles, ds->num_sms, st));
+  // chunks of kRowsChunk rows share the adapters' part, one after another on the stream
+  const char* x = static_cast<const char*>(p->x_dev);
+  const char* slots = static_cast<const char*>(p->row_slot_dev);
+  char* y = static_cast<char*>(y_dev);
+  for (int t0 = 0; t0 < p->T; t0 += kRowsChunk) {
+    a.T = p->T - t0 < kRowsChunk ? p->T - t0 : kRowsChunk;
+    a.x = x + static_cast<size_t>(t0) * p->ldx * 2;
+    a.row_slot = slots + static_cast<size_t>(t0) * p->row_slot_bytes;
+    a.y = y + static_cast<size_t>(t0) * p->N * 2;
+    const uint64_t x_pitch = static_cast<uint64_t>(p->ldx) * 2, w_pitch = static_cast<uint64_t>(p->K) * 2;
+    cudaError_t e;
+    if (rows_use_pairs(a.T, a.K, a.N, ds->num_sms)) {
+      TcMaps maps;
+      if (!make_map(&maps.p, p->dtype, a.x, a.K, a.T, x_pitch, 64, 128) ||
+          !make_map(&maps.q, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128) ||
+          !make_map(&maps.o, p->dtype, a.y, a.N, a.T, static_cast<uint64_t>(a.N) * 2, 64, 32))
+        return LF_ERR_UNSUPPORTED;
+      maps.s = maps.l = maps.p;
+      Tables tb{};
+      tb.r_pad = 16;
+      tb.err = ds->status;
+      const PairDelta delta{a.delta, a.eff, (a.N + 15) / 16 * 16};
+      e = rows_lora_part(a, p->dtype, ds->num_sms, st);
+      if (e == cudaSuccess)
+        e = tc_gemm_pair(p->dtype, false, maps, a.T, a.N, a.K, false, tb, a.y, a.N, ds->num_sms, st, nullptr, nullptr,
+                         &delta);
+    } else {
+      const RowsTiles tiles = rows_tiles(a.T, a.K, a.N, ds->num_sms);
+      CUtensorMap w_map, x_map;
+      if (!make_map(&w_map, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128) ||
+          !make_map(&x_map, p->dtype, a.x, a.K, a.T, x_pitch, 64, tiles.rows))
+        return LF_ERR_UNSUPPORTED;
+      e = rows_forward_tc(a, p->dtype, w_map, x_map, tiles, ds->num_sms, st);
+    }
+    if (e != cudaSuccess) return LF_ERR_CUDA;
+  }
+  return LF_OK;
 }
 
 extern "C" int lf_device_error(int32_t* code) {

@@ -101,12 +101,20 @@ struct PairTail {
   int slots;
   uint64_t gen;
 };
+// Float32 [T][ld] added to the product of rows whose word in `eff` is not all ones, written by the launch
+// ahead on the stream (this one starts before it has finished).
+struct PairDelta {
+  const float* delta;
+  const uint32_t* eff;
+  int64_t ld;  // a multiple of 4
+};
 // CTA pairs the pair GEMM can leave to a co-scheduled shrink without adding a round (0: none).
 int pair_spare_pairs(int T, int Nout, int num_sms, int n_units);
 // `tail` (optional) enables the K-split tail; the launch is then cooperative.
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
-                         const PairShrink* shrink = nullptr, const PairTail* tail = nullptr);
+                         const PairShrink* shrink = nullptr, const PairTail* tail = nullptr,
+                         const PairDelta* delta = nullptr);
 // Forward workspace without the tail scratch (the least lf_forward accepts).
 size_t forward_min_workspace_bytes(const lf_plan_info* info);
 // Gram load balance: slots (slot_order positions) the kernel can split into parts, and the
@@ -189,6 +197,10 @@ RowsTiles rows_tiles(int T, int K, int N, int num_sms);
 // w: [N, K] box (64, 128), x: [T, K] box (64, tiles.rows), both with the 128-byte swizzle
 cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
                             int num_sms, cudaStream_t st);
+// The adapters' part alone (a.delta, a.eff), for a GEMM that adds it: tc_gemm_pair's `delta`.
+cudaError_t rows_lora_part(const RowsArgs& a, int dtype, int num_sms, cudaStream_t st);
+bool rows_use_pairs(int T, int K, int N, int num_sms);
+constexpr int kRowsChunk = 8192;  // rows whose adapters' part is held at a time
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
 
 // --------------------------------------------------------------- packing

@@ -259,56 +259,77 @@ __device__ __forceinline__ void halves(float w, T& hi, T& lo) {
   lo = from_f32<T>(fabsf(w) <= 4.f ? w - to_f32(hi) : 0.f);
 }
 
-// The second product of one group of 8 rows for output blocks b0 .. b1 - 1 (16 features each): kNM rank steps
-// of 16, kPer blocks loaded together.  B_i is stored in the order of the MMA's operand: one 16-byte load a
-// lane and step.  hi, lo: S of row g, null without one.  A row that the group does not have is -1; `second`:
-// whether any of the odd rows exists.
-template <typename T, int kNM, int kPer>
-__device__ __forceinline__ void expand_blocks(const uint4* w, int pitch, const uint2 (&sh)[kNM], const uint2 (&sl)[kNM],
-                                              float f0, float f1, float* o0, float* o1, bool on0, bool on1,
+// One group of 8 rows as the second product sees it: S halves of row g, rows and factors of columns 2q, 2q + 1 (-1:
+// the group has no such row).
+template <typename T>
+struct GroupRows {
+  const T* hi;
+  const T* lo;
+  int row0, row1;
+  float f0, f1;
+};
+
+// The second product of up to kNB groups of one adapter for output blocks b0 .. b1 - 1 (16 features each): kNM rank
+// steps of 16, kPer blocks loaded together.  B_i is stored in the order of the MMA's operand: one 16-byte load a
+// lane and step.
+template <typename T, int kNM, int kNB, int kPer>
+__device__ __forceinline__ void expand_blocks(const uint4* w, int pitch, const uint2 (&sh)[kNB][kNM],
+                                              const uint2 (&sl)[kNB][kNM], const GroupRows<T> (&rows)[kNB],
+                                              float* const (&o0)[kNB], float* const (&o1)[kNB], int at, int nb,
                                               bool second) {
   T* const tag = nullptr;
   uint4 v[kPer][kNM];
 #pragma unroll
   for (int i = 0; i < kPer; ++i)
 #pragma unroll
-    for (int k = 0; k < kNM; ++k) v[i][k] = w[k * pitch + i * 32];
+    for (int k = 0; k < kNM; ++k) v[i][k] = w[k * pitch + (at + i) * 32];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int k = 0; k < kNM; ++k) {
-      mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sh[k].x, sh[k].y, tag);
-      mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sl[k].x, sl[k].y, tag);
+    for (int b = 0; b < kNB; ++b) {
+      if (b < nb) {
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int k = 0; k < kNM; ++k) {
+          mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sh[b][k].x, sh[b][k].y, tag);
+          mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sl[b][k].x, sl[b][k].y, tag);
+        }
+        float* p0 = o0[b] + (at + i) * 16;
+        float* p1 = o1[b] + (at + i) * 16;
+        if (rows[b].row0 >= 0) p0[0] = rows[b].f0 * d[0], p0[8] = rows[b].f0 * d[2];
+        if (second && rows[b].row1 >= 0) p1[0] = rows[b].f1 * d[1], p1[8] = rows[b].f1 * d[3];
+      }
     }
-    if (on0) o0[i * 16] = f0 * d[0], o0[i * 16 + 8] = f0 * d[2];
-    if (second && on1) o1[i * 16] = f1 * d[1], o1[i * 16 + 8] = f1 * d[3];
   }
 }
-template <typename T, int kNM, int kPer>
-__device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int b0, int b1, const T* hi, const T* lo,
-                                             float f0, float f1, int row0, int row1) {
+template <typename T, int kNM, int kNB, int kPer>
+__device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int b0, int b1,
+                                             const GroupRows<T> (&rows)[kNB], int nb) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int blocks = (p.N + 15) >> 4, steps = p.r_pad >> 4;
-  uint2 sh[kNM], sl[kNM];
+  uint2 sh[kNB][kNM], sl[kNB][kNM];
+  float *o0[kNB], *o1[kNB];
+  bool odd = false;
 #pragma unroll
-  for (int k = 0; k < kNM; ++k) {
-    const bool on = hi != nullptr && 16 * k < rank_of(e);
-    sh[k] = on ? *reinterpret_cast<const uint2*>(hi + 16 * k + 4 * q) : make_uint2(0, 0);
-    sl[k] = on ? *reinterpret_cast<const uint2*>(lo + 16 * k + 4 * q) : make_uint2(0, 0);
+  for (int b = 0; b < kNB; ++b) {
+#pragma unroll
+    for (int k = 0; k < kNM; ++k) {
+      const bool on = 16 * k < rank_of(e);
+      sh[b][k] = on ? *reinterpret_cast<const uint2*>(rows[b].hi + 16 * k + 4 * q) : make_uint2(0, 0);
+      sl[b][k] = on ? *reinterpret_cast<const uint2*>(rows[b].lo + 16 * k + 4 * q) : make_uint2(0, 0);
+    }
+    o0[b] = p.delta + static_cast<size_t>(max(rows[b].row0, 0)) * blocks * 16 + g;
+    o1[b] = p.delta + static_cast<size_t>(max(rows[b].row1, 0)) * blocks * 16 + g;
+    odd = odd || rows[b].row1 >= 0;
   }
-  const bool on0 = row0 >= 0, on1 = row1 >= 0, second = __any_sync(0xffffffffu, on1);
-  const uint4* w = static_cast<const uint4*>(p.b_bank) +
-                   (static_cast<size_t>(slot_of(e)) * steps * blocks + b0) * 32 + lane;
-  float* o0 = p.delta + (static_cast<size_t>(max(row0, 0)) * blocks + b0) * 16 + g;
-  float* o1 = p.delta + (static_cast<size_t>(max(row1, 0)) * blocks + b0) * 16 + g;
-  int n = b1 - b0;
+  const bool second = __any_sync(0xffffffffu, odd);
+  const uint4* w = static_cast<const uint4*>(p.b_bank) + static_cast<size_t>(slot_of(e)) * steps * blocks * 32 + lane;
+  int b = b0;
 #pragma unroll 1
-  for (; n >= kPer; n -= kPer, w += kPer * 32, o0 += kPer * 16, o1 += kPer * 16)
-    expand_blocks<T, kNM, kPer>(w, blocks * 32, sh, sl, f0, f1, o0, o1, on0, on1, second);
+  for (; b + kPer <= b1; b += kPer)
+    expand_blocks<T, kNM, kNB, kPer>(w, blocks * 32, sh, sl, rows, o0, o1, b, nb, second);
 #pragma unroll 1
-  for (; n > 0; --n, w += 32, o0 += 16, o1 += 16)
-    expand_blocks<T, kNM, 1>(w, blocks * 32, sh, sl, f0, f1, o0, o1, on0, on1, second);
+  for (; b < b1; ++b) expand_blocks<T, kNM, kNB, 1>(w, blocks * 32, sh, sl, rows, o0, o1, b, nb, second);
 }
 
 // Groups from `grp` on, at most kNB and `most`, that belong to one adapter.
@@ -326,9 +347,11 @@ __device__ __forceinline__ int unit_size(const Groups& s, int grp, int most) {
 // first product and the output features for the second.  Partial products
 // meet in shared memory, then across the cluster, in a fixed order.  The grid fits the GPU at once, so
 // the dependent GEMM streams its weight while this kernel runs.
-// kToGlobal: write S (halves and factor) to global memory instead, for a GEMM that does the second product.
-template <typename T, int kMT, int kNB, bool kToGlobal>
-__global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts) {
+// kNB = 1: a few rows, clusters.  kNB > 1: many rows (prompts), no cluster; up to kNB groups of one adapter share
+// what is read of it.
+template <typename T, int kMT, int kNB>
+__global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts_) {
+  const int kparts = kNB > 1 ? 1 : kparts_;
   constexpr int kRP = kMT * 16;                                         // padded rank
   constexpr int kBatch = kPartBytes / (kShrinkWarps * kRP * 8 * 4);     // groups of 8 rows per batch
   constexpr int kPitch = kRP + 8;                                       // of S rows: no bank conflicts
@@ -353,7 +376,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
     const int slice = item % slices, t0 = item / slices * kTileRows;
     const int rows = min(kTileRows, p.T - t0);
     const int n_groups = group_rows(p, t0, rows, true, s);
-    if (kToGlobal && crank == 0 && slice == 0 && tid < rows) p.eff[t0 + tid] = s.eff[tid];
+    if (crank == 0 && slice == 0 && tid < rows) p.eff[t0 + tid] = s.eff[tid];
     const int g_lo = slice_start(s, n_groups, slice, slices);
     const int g_hi = slice + 1 < slices ? slice_start(s, n_groups, slice + 1, slices) : n_groups;
     for (int first = g_lo; first < g_hi; first += kBatch) {
@@ -429,10 +452,9 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
         __syncthreads();
       }
       // S of each group, one warp a group; every CTA needs all of them for the second product
-      const int u_step = kToGlobal ? kShrinkWarps * kparts : kShrinkWarps;
-      for (int u = kToGlobal ? warp * kparts + crank : warp; u < batch; u += u_step) {
+      for (int u = warp; u < batch; u += kShrinkWarps) {
         const uint32_t e = s.eff[s.start[first + u]];
-        const int rank = rank_of(e), row = s.rows[first + u][lane & 7];
+        const int rank = rank_of(e);
         float v[kRP / 4];
         float top = 0.f;
 #pragma unroll
@@ -446,43 +468,44 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
         const int ex = row_exponent(top);
         const float down = scalbnf(1.f, -ex), fac = p.slot_scale[slot_of(e)] * scalbnf(1.f, ex);
-        if (kToGlobal && row < 0) continue;  // (no warp-wide step follows in this branch)
-        const size_t at = kToGlobal ? static_cast<size_t>(t0 + row) * p.r_pad : 0;
-        T* hi = kToGlobal ? static_cast<T*>(p.s_hi) + at : s_hi[u][lane & 7];
-        T* lo = kToGlobal ? static_cast<T*>(p.s_lo) + at : s_lo[u][lane & 7];
-        if (lane < 8) *(kToGlobal ? p.factor + t0 + row : &s_fac[u][lane]) = fac;
+        if (lane < 8) s_fac[u][lane] = fac;
 #pragma unroll
         for (int i = 0; i < kRP / 4; ++i) {
           const int j = (lane >> 3) + 4 * i;
-          if (j < ((rank + 15) & ~15)) halves<T>(v[i] * down, hi[j], lo[j]);
+          if (j < ((rank + 15) & ~15)) halves<T>(v[i] * down, s_hi[u][lane & 7][j], s_lo[u][lane & 7][j]);
         }
       }
       __syncthreads();
-      if constexpr (!kToGlobal) {
-        // the warps divide the groups first here too
-        const int at_once = batch >= 8 ? 8 : batch >= 4 ? 4 : batch >= 2 ? 2 : 1;
-        const int pieces = kShrinkWarps / at_once, piece = warp / at_once;
-        const int f0_ = nb0 + (nb1 - nb0) * piece / pieces, f1_ = nb0 + (nb1 - nb0) * (piece + 1) / pieces;
-        for (int u = warp % at_once; u < batch; u += at_once) {
-          const uint32_t e = s.eff[s.start[first + u]];
-          const int nm = (rank_of(e) + 15) >> 4;
-          int row0 = s.rows[first + u][2 * q], row1 = s.rows[first + u][2 * q + 1];
-          row0 = row0 < 0 ? -1 : t0 + row0;
-          row1 = row1 < 0 ? -1 : t0 + row1;
-          const float f0 = s_fac[u][2 * q], f1 = s_fac[u][2 * q + 1];
-          const T* hi = s_hi[u][g];
-          const T* lo = s_lo[u][g];
-          if (nm == 1) expand_group<T, 1, 8>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
-          else if (nm == 2) {
-            if constexpr (kMT >= 2) expand_group<T, 2, 4>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
-          } else if (nm <= 4) {
-            if constexpr (kMT >= 4) expand_group<T, 4, 2>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
-          } else if constexpr (kMT >= 8) {
-            expand_group<T, 8, 1>(p, e, f0_, f1_, hi, lo, f0, f1, row0, row1);
-          }
+      // the warps divide the units, then the features, here too
+      const int f0 = nb0 + (nb1 - nb0) * sub / subs, f1 = nb0 + (nb1 - nb0) * (sub + 1) / subs;
+      for (int u = 0, index = 0, nb; u < batch; u += nb, ++index) {
+        nb = unit_size<kNB>(s, first + u, batch - u);
+        if (index % lanes != warp % lanes) continue;
+        const uint32_t e = s.eff[s.start[first + u]];
+        const int nm = (rank_of(e) + 15) >> 4;
+        GroupRows<T> rows_of[kNB];
+#pragma unroll
+        for (int b = 0; b < kNB; ++b) {
+          const int v = u + min(b, nb - 1);
+          rows_of[b].hi = s_hi[v][g];
+          rows_of[b].lo = s_lo[v][g];
+          const int r0 = b < nb ? s.rows[first + v][2 * q] : -1, r1 = b < nb ? s.rows[first + v][2 * q + 1] : -1;
+          rows_of[b].row0 = r0 < 0 ? -1 : t0 + r0;
+          rows_of[b].row1 = r1 < 0 ? -1 : t0 + r1;
+          rows_of[b].f0 = s_fac[v][2 * q];
+          rows_of[b].f1 = s_fac[v][2 * q + 1];
         }
-        __syncthreads();
+        constexpr int kPer = kNB > 1 ? 4 : 8;  // 16-byte loads in flight a lane
+        if (nm == 1) expand_group<T, 1, kNB, kPer>(p, e, f0, f1, rows_of, nb);
+        else if (nm == 2) {
+          if constexpr (kMT >= 2) expand_group<T, 2, kNB, kPer / 2>(p, e, f0, f1, rows_of, nb);
+        } else if (nm <= 4) {
+          if constexpr (kMT >= 4) expand_group<T, 4, kNB, kPer / 4>(p, e, f0, f1, rows_of, nb);
+        } else if constexpr (kMT >= 8) {
+          expand_group<T, 8, kNB, 1>(p, e, f0, f1, rows_of, nb);
+        }
       }
+      __syncthreads();
     }
     __syncthreads();
   }
@@ -840,33 +863,39 @@ cudaError_t launch_gemm(const RowsGemm& g, const CUtensorMap& w, const CUtensorM
   return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), ring_bytes(kTN) + 1024, st, true, w, x, g);
 }
 
+// The adapters' part of rows with `a`.  Up to 256 rows: one CTA an SM, beside the GEMM's; few rows are cut over a larger
+// cluster.  More rows: two CTAs an SM and no cluster (the GEMM that follows needs whole SMs).
 template <typename T>
-cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int tn, int ksplit,
-                    int num_sms, cudaStream_t st) {
-  // the adapters' part: one CTA an SM, beside the GEMM's; few rows are cut over a larger cluster
+cudaError_t lora_part(const RowsArgs& a, int num_sms, cudaStream_t st) {
   const int tiles = (a.T + kTileRows - 1) / kTileRows;
-  int kparts = tiles == 1 ? 8 : tiles <= 16 ? 4 : 1;
+  const bool many = tiles > 2;
+  int kparts = many ? 1 : tiles == 1 ? 8 : 4;
   while (kparts > 1 && (a.K + 31) / 32 < kparts * kShrinkWarps) kparts /= 2;
-  const int clusters = num_sms / kparts;
+  const int clusters = (many ? 2 : 1) * num_sms / kparts;
   int slices = clusters / tiles;
   slices = slices < 1 ? 1 : slices > kTileRows ? kTileRows : slices;
   if (slices > a.T) slices = a.T;
   const dim3 grid(static_cast<unsigned>((tiles * slices < clusters ? tiles * slices : clusters) * kparts));
   cudaError_t e;
-#define LF_LORA(MT, NB)                                                                                             \
-  {                                                                                                                 \
-    e = allow_smem(reinterpret_cast<const void*>(rows_lora_kernel<T, MT, NB, false>), 0);                            \
-    if (e != cudaSuccess) return e;                                                                                 \
-    e = launch_cluster(rows_lora_kernel<T, MT, NB, false>, grid, kparts, dim3(kShrinkThreads), 0, st, false, a, slices, \
-                       kparts);                                                                                     \
+#define LF_LORA(MT, NB)                                                                                       \
+  {                                                                                                           \
+    auto* k = many ? rows_lora_kernel<T, MT, NB> : rows_lora_kernel<T, MT, 1>;                                \
+    e = allow_smem(reinterpret_cast<const void*>(k), 0);                                                      \
+    if (e == cudaSuccess) e = launch_cluster(k, grid, kparts, dim3(kShrinkThreads), 0, st, false, a, slices, kparts); \
   }
   if (a.r_pad == 16) LF_LORA(1, 4)
   else if (a.r_pad == 32) LF_LORA(2, 4)
   else if (a.r_pad == 64) LF_LORA(4, 2)
   else LF_LORA(8, 1)
 #undef LF_LORA
-  if (e != cudaSuccess) return e;
+  return e;
+}
 
+template <typename T>
+cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int tn, int ksplit,
+                    int num_sms, cudaStream_t st) {
+  const cudaError_t e = lora_part<T>(a, num_sms, st);
+  if (e != cudaSuccess) return e;
   RowsGemm g{};
   g.a = a;
   g.idesc = umma_idesc_f16(kWRows, tn, dtype == LF_BF16 ? 1 : 0, 0, 0);
@@ -909,6 +938,22 @@ cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, 
                             int num_sms, cudaStream_t st) {
   return dtype == LF_BF16 ? rows_tc<__nv_bfloat16>(a, dtype, w, x, t.rows, t.ksplit, num_sms, st)
                           : rows_tc<__half>(a, dtype, w, x, t.rows, t.ksplit, num_sms, st);
+}
+
+cudaError_t rows_lora_part(const RowsArgs& a, int dtype, int num_sms, cudaStream_t st) {
+  return dtype == LF_BF16 ? lora_part<__nv_bfloat16>(a, num_sms, st) : lora_part<__half>(a, num_sms, st);
+}
+
+// Rounds of full tiles times the time of one (measured at K = 4096: 23 us for a 256 x 256 tile of a CTA pair, 32 us for
+// a 128 x 256 tile of one CTA when every SM has one, a K part taking its share and the split about 5 us more).
+bool rows_use_pairs(int T, int K, int N, int num_sms) {
+  if (T <= 256) return false;
+  const int64_t pair_tiles = static_cast<int64_t>((T + 255) / 256) * ((N + 255) / 256);
+  const int64_t tiles = static_cast<int64_t>((T + 255) / 256) * ((N + kWRows - 1) / kWRows);
+  const int ks = rows_tiles(T, K, N, num_sms).ksplit;
+  const double pair = 23.0 * ((pair_tiles + num_sms / 2 - 1) / (num_sms / 2)) * K / 4096;
+  const double one = 32.0 * ((tiles * ks + num_sms - 1) / num_sms) * K / 4096 / ks + 5.0;
+  return pair < one;
 }
 
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st) {

@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 
 #include "lf_internal.cuh"
+#include "lf_launch.cuh"
 #include "lf_ptx.cuh"
 
 namespace lf {
@@ -424,6 +425,7 @@ struct PairParams {
   // optional second shrink job (own activations/slab/K), items after the first job's
   int job2, Kred2;
   void* s_ext2;
+  PairDelta delta;  // kDelta kernels
   Tables tb;
 };
 
@@ -749,7 +751,8 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
   if (kPrologue) __syncthreads();
 }
 
-template <bool kQMN, typename OutT>
+// kDelta: a float32 matrix is added to the product (prm.delta).
+template <bool kQMN, typename OutT, bool kDelta>
 __global__ void __launch_bounds__(kThreads, 1)
     tc_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_l,
@@ -1041,6 +1044,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int n_stores = 0;
     const int wslot = static_cast<int>(crank) * 4 + q;  // this warp's 32 rows of a partial tile
     uint32_t tail_pending = 0, tail_par = 0;  // lane 0: partial-tile copies in flight per buffer, their parity
+    if constexpr (kDelta) pdl_wait();
     for (int k = 0; k < n_units; ++k, ++it) {
       const PairUnit un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
       const int mp = un.mp, n = un.n;
@@ -1150,6 +1154,22 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const int col0 = n * 256 + c * 64;
         if (row0 >= prm.T || col0 >= prm.Nout) continue;
+        if constexpr (kDelta) {
+          const int row = row0 + lane;
+          if (row < prm.T && prm.delta.eff[row] != 0xffffffffu) {
+            const float4* d = reinterpret_cast<const float4*>(prm.delta.delta + row * prm.delta.ld + col0);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (col0 + 4 * i < prm.Nout) {
+                const float4 f = d[i];
+                v[4 * i] = __float_as_uint(__uint_as_float(v[4 * i]) + f.x);
+                v[4 * i + 1] = __float_as_uint(__uint_as_float(v[4 * i + 1]) + f.y);
+                v[4 * i + 2] = __float_as_uint(__uint_as_float(v[4 * i + 2]) + f.z);
+                v[4 * i + 3] = __float_as_uint(__uint_as_float(v[4 * i + 3]) + f.w);
+              }
+            }
+          }
+        }
         uint8_t* sbuf = ring_stage ? ring_w + c * (32 * 64 * 2) : stage_w + (n_stores & 1) * (32 * 64 * 2);
         if (!ring_stage && lane == 0) bulk_wait_read<1>();  // the store that used this buffer has read it
         __syncwarp();
@@ -2175,7 +2195,7 @@ int pair_spare_pairs(int T, int Nout, int num_sms, int n_units) {
 
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
-                         const PairShrink* shrink, const PairTail* tail) {
+                         const PairShrink* shrink, const PairTail* tail, const PairDelta* delta) {
   PairParams p{};
   p.out = out;
   p.ldo = ldo;
@@ -2270,22 +2290,35 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cfg.attrs = attr;
   cfg.numAttrs = p.n_shrink_pairs > 0 || p.shrink_prologue || p.tail_parts > 1 ? 2 : 1;
   cudaError_t e;
-#define LF_LAUNCH_PAIR(QMN, OT)                                                                  \
-  e = ensure_smem(tc_gemm_pair_kernel<QMN, OT>, kPairSmem);                                     \
+#define LF_LAUNCH_PAIR(QMN, OT, DELTA)                                                          \
+  e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA>, kPairSmem);                              \
   if (e != cudaSuccess) return e;                                                               \
-  e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT>, maps.p, maps.q, maps.s, maps.l, maps.o, *a_map, *p2_map, \
+  e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT, DELTA>, maps.p, maps.q, maps.s, maps.l, maps.o, *a_map, *p2_map, \
                          *a2_map, p);
+  if (delta != nullptr) {
+    if (q_mn_major || shrink != nullptr || tail != nullptr) return cudaErrorInvalidValue;
+    p.delta = *delta;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+    if (dtype == LF_BF16) {
+      LF_LAUNCH_PAIR(false, __nv_bfloat16, true)
+    } else {
+      LF_LAUNCH_PAIR(false, __half, true)
+    }
+    return e;
+  }
   if (dtype == LF_BF16) {
     if (q_mn_major) {
-      LF_LAUNCH_PAIR(true, __nv_bfloat16)
+      LF_LAUNCH_PAIR(true, __nv_bfloat16, false)
     } else {
-      LF_LAUNCH_PAIR(false, __nv_bfloat16)
+      LF_LAUNCH_PAIR(false, __nv_bfloat16, false)
     }
   } else {
     if (q_mn_major) {
-      LF_LAUNCH_PAIR(true, __half)
+      LF_LAUNCH_PAIR(true, __half, false)
     } else {
-      LF_LAUNCH_PAIR(false, __half)
+      LF_LAUNCH_PAIR(false, __half, false)
     }
   }
 #undef LF_LAUNCH_PAIR

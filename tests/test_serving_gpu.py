@@ -82,6 +82,10 @@ CASES = [  # dtype, T, K, N, ranks, max_rank
     (F16, 256, 512, 512, [16] * 300, 16),
     (BF16, 257, 328, 392, [48, 20], 48),
     (BF16, 1031, 640, 1288, [16, 40, 64], 64),
+    (F16, 300, 1032, 2056, [16, 3, 33, 64, 0], 64),
+    (BF16, 700, 520, 1032, [128, 90, 16], 128),
+    (F16, 2000, 264, 4104, [16] * 200, 16),
+    (BF16, 8500, 72, 264, [8, 24, 16], 32),  # more rows than one chunk
     (F32, 1, 37, 53, [4], 4),
     (F32, 128, 256, 256, [8] * 4, 8),
     (F32, 45, 300, 129, [16, 1, 70], 70),
@@ -117,6 +121,20 @@ def test_orders_and_absent_adapters():
     bank.unload(1)
     y = fused_lora_forward_rows(x, w, bank, sorted_slots)
     assert torch.equal(y[100:200], base[100:200]) and torch.equal(y[:100], y_sorted[:100])
+
+
+@pytest.mark.parametrize("dtype, r", [(BF16, 16), (F16, 32), (BF16, 64), (BF16, 128)])
+def test_prompts(dtype, r):
+    """Long runs of one adapter, short ones and rows without any, across the tiles of a long batch."""
+    lengths = [1, 300, 7, 8, 9, 511, 64, 33, 128, 40, 2, 900]
+    slots = torch.cat([torch.full((n,), i % 4 - 1, dtype=torch.int32) for i, n in enumerate(lengths)]).cuda()
+    x, w, bank, adapters, slots = make(dtype, len(slots), 776, 1544, [r, r - 3, r // 2], r, slots=slots)
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    check(y, x, w, adapters, slots)
+    order = torch.randperm(len(slots), device="cuda")
+    shuffled = fused_lora_forward_rows(x[order].contiguous(), w, bank, slots[order].contiguous())
+    check(shuffled, x[order], w, adapters, slots[order])
+    assert nat.device_error() == 0
 
 
 def test_agrees_with_the_packed_forward():
@@ -167,8 +185,9 @@ def test_slots_out_of_range_are_reported():
 
 
 @pytest.mark.parametrize("dtype", [BF16, F16])
-def test_values_that_are_not_finite_stay_with_their_rows(dtype):
-    T, K, N = 24, 256, 256
+@pytest.mark.parametrize("T", [24, 1500])
+def test_values_that_are_not_finite_stay_with_their_rows(dtype, T):
+    K, N = 256, 256
     x, w, bank, adapters, _ = make(dtype, T, K, N, [16, 9, 16], 16)
     slots = torch.arange(T, device="cuda", dtype=torch.int32) % 3
     good = fused_lora_forward_rows(x, w, bank, slots)
@@ -198,8 +217,9 @@ def test_float16_rank_products_beyond_its_range():
     check(y, x, w, [big, small], slots)
 
 
-def test_captured_call_follows_slots_and_bank():
-    T, K, N = 12, 512, 512
+@pytest.mark.parametrize("T", [12, 200, 1100])
+def test_captured_call_follows_slots_and_bank(T):
+    K, N = 512, 512
     x, w, bank, adapters, slots = make(BF16, T, K, N, [16, 8], 16)
     out = torch.empty(T, N, dtype=BF16, device="cuda")
     fused_lora_forward_rows(x, w, bank, slots, out=out)
