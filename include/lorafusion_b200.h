@@ -469,7 +469,7 @@ LF_API int lf_assign_rows(const int32_t* bin_start, const int32_t* entry_adapter
 
 /* One projection and a bank of resident adapters.  `slot_rank_dev` holds each slot's rank (0: empty
  * slot, its rows get the shared projection alone), at most r_pad; bank entries past it must be zero.
- * A block of the B bank holds feature f, rank r of its 16 x 16 at 8 (4 (f % 8) + r / 4) + 4 (f / 8) + r % 4. */
+ * n_slots * r_pad / 16 * max(N, 16) must fit in 31 bits. */
 typedef struct lf_rows_problem {
   int32_t dtype;             /* lf_dtype of x, W, y and the bank */
   int32_t T, K, N;           /* rows, in_features, out_features */
@@ -480,7 +480,7 @@ typedef struct lf_rows_problem {
   const void* x_dev;         /* [T] rows of K */
   const void* w_dev;         /* [N,K] */
   const void* a_bank_dev;    /* [n_slots, r_pad, K] */
-  const void* b_bank_dev;    /* [n_slots, r_pad/16, ceil(N/16), 256]: blocks of 16 ranks x 16 features */
+  const void* b_bank_dev;    /* [n_slots, r_pad/16, N, 16]: B_i in steps of 16 ranks */
   const int32_t* slot_rank_dev;  /* [n_slots] */
   const float* slot_scale_dev;   /* [n_slots] s_i */
   const void* row_slot_dev;  /* [T] slot of each row; negative: no adapter */
@@ -494,10 +494,14 @@ LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32
  * the device, so a captured call follows later changes of it and of the bank's contents.  A
  * slot at or above n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
  * bf16/f16 with K, N and ldx multiples of 8 and 16-byte aligned buffers run on the tensor cores, other
- * problems on CUDA cores.  Enqueued on `stream` (2 launches); never synchronizes.
+ * problems on CUDA cores.  Long batches run in chunks of 8192 rows, of 4
+ * launches (2 up to 256 rows).  Enqueued on `stream`; never synchronizes.
  */
 LF_API int lf_rows_forward(const lf_rows_problem* prob, void* y_dev, void* workspace_dev, size_t workspace_bytes,
                            lf_stream_t stream);
+
+/* Launches of lf_rows_forward of T rows on the tensor cores (on CUDA cores there are 2). */
+LF_API int lf_rows_launch_count(int32_t T);
 
 /* ------------------------------------------------------------------------------------------------
  * Training: gradient norms, clipping and AdamW of many adapters.  No counterpart in the reference

@@ -836,13 +836,40 @@ extern "C" int lf_ipc_close(void* dev_ptr) {
   return cudaIpcCloseMemHandle(dev_ptr) == cudaSuccess ? LF_OK : LF_ERR_CUDA;
 }
 
-// Workspace of lf_rows_forward: each row's adapter and factor, then S (two 16-bit halves, or one
-// float32 array on the CUDA-core path: the same bytes), then the adapters' part of the result.
+// Workspace of lf_rows_forward: each row's adapter, S (two 16-bit halves, or one float32 array on the CUDA-core
+// path: the same bytes), what the tensor-core path knows of the sorted rows, the adapters' part of the
+// result.  Long batches run in chunks of rows, one after another in the same place.
+struct RowsSpace {
+  size_t eff, s_hi, s_lo, factor, perm, tiles, n_tiles, delta, bytes;
+};
+static RowsSpace rows_space(int32_t T, int32_t N, int32_t r_pad, int32_t dtype) {
+  const size_t all = static_cast<size_t>(T), rows = T < kRowsChunk ? all : kRowsChunk;
+  const bool tc = dtype != LF_F32;
+  RowsSpace s{};
+  size_t at = 0;
+  auto take = [&](size_t& place, size_t bytes) {
+    place = at;
+    at += align256(bytes);
+  };
+  take(s.eff, all * 4);
+  take(s.s_hi, all * r_pad * 2);
+  take(s.s_lo, all * r_pad * 2);
+  take(s.factor, tc ? rows * 4 : 0);
+  take(s.perm, tc ? rows * 4 : 0);
+  take(s.tiles, tc ? rows * 16 : 0);
+  take(s.n_tiles, tc ? 4 : 0);
+  take(s.delta, tc ? rows * ((static_cast<size_t>(N) + 15) / 16 * 16) * 4 : 0);
+  s.bytes = at;
+  return s;
+}
 extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype) {
-  if (T < 0 || N < 0 || r_pad < 0) return 0;
-  const size_t rows = T < kRowsChunk ? T : kRowsChunk;  // long batches run in chunks of rows
-  const size_t delta = dtype == LF_F32 ? 0 : rows * ((N + 15) / 16 * 16) * 4;
-  return 2 * align256(static_cast<size_t>(T) * 4) + 2 * align256(static_cast<size_t>(T) * r_pad * 2) + align256(delta);
+  return T < 0 || N < 0 || r_pad < 0 ? 0 : rows_space(T, N, r_pad, dtype).bytes;
+}
+
+extern "C" int lf_rows_launch_count(int32_t T) {
+  int n = 0;
+  for (int t0 = 0; t0 < T; t0 += kRowsChunk) n += T - t0 > kFewRows ? 4 : 2;
+  return n;
 }
 
 extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* workspace_dev, size_t workspace_bytes,
@@ -851,7 +878,9 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   if (p->dtype != LF_F32 && p->dtype != LF_BF16 && p->dtype != LF_F16) return LF_ERR_INVALID_ARG;
   if (p->r_pad != 16 && p->r_pad != 32 && p->r_pad != 64 && p->r_pad != LF_BANK_MAX_RANK) return LF_ERR_INVALID_ARG;
   if (p->row_slot_bytes != 4 && p->row_slot_bytes != 8) return LF_ERR_INVALID_ARG;
-  if (p->n_slots >= (1 << 24)) return LF_ERR_UNSUPPORTED;
+  if (p->n_slots >= (1 << 24) || 
+      static_cast<int64_t>(p->n_slots) * (p->r_pad / 16) * (p->N > 16 ? p->N : 16) > INT32_MAX)
+    return LF_ERR_UNSUPPORTED;
   if (p->T == 0 || p->N == 0) return LF_OK;
   if (p->ldx < p->K || !p->x_dev || !p->w_dev || !p->row_slot_dev || !y_dev) return LF_ERR_INVALID_ARG;
   if (p->n_slots > 0 && (!p->a_bank_dev || !p->b_bank_dev || !p->slot_rank_dev || !p->slot_scale_dev))
@@ -878,12 +907,15 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   a.wide = p->row_slot_bytes == 8;
   a.err = ds->status;
   char* ws = static_cast<char*>(workspace_dev);
-  const size_t words = align256(static_cast<size_t>(p->T) * 4), s_bytes = align256(static_cast<size_t>(p->T) * p->r_pad * 2);
-  a.eff = reinterpret_cast<uint32_t*>(ws);
-  a.factor = reinterpret_cast<float*>(ws + words);
-  a.s_hi = ws + 2 * words;
-  a.s_lo = ws + 2 * words + s_bytes;
-  a.delta = reinterpret_cast<float*>(ws + 2 * words + 2 * s_bytes);
+  const RowsSpace space = rows_space(p->T, p->N, p->r_pad, p->dtype);
+  a.eff = reinterpret_cast<uint32_t*>(ws + space.eff);
+  a.s_hi = ws + space.s_hi;
+  a.s_lo = ws + space.s_lo;
+  a.factor = reinterpret_cast<float*>(ws + space.factor);
+  a.perm = reinterpret_cast<int*>(ws + space.perm);
+  a.tiles = ws + space.tiles;
+  a.n_tiles = reinterpret_cast<int*>(ws + space.n_tiles);
+  a.delta = reinterpret_cast<float*>(ws + space.delta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = p->dtype != LF_F32 && p->K > 0 && p->K % 8 == 0 && p->N % 8 == 0 && p->ldx % 8 == 0 &&
                   aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) &&
@@ -903,6 +935,19 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     a.y = y + static_cast<size_t>(t0) * p->N * 2;
     const uint64_t x_pitch = static_cast<uint64_t>(p->ldx) * 2, w_pitch = static_cast<uint64_t>(p->K) * 2;
     cudaError_t e;
+    ManyMaps many;
+    if (a.T > kFewRows) {
+      const uint64_t bank_rows = static_cast<uint64_t>(a.n_slots > 0 ? a.n_slots : 1) * a.r_pad;
+      const uint64_t s_pitch = static_cast<uint64_t>(a.r_pad) * 2;
+      const void* a_bank = a.n_slots > 0 ? a.a_bank : a.w;  // an empty bank: a map that nothing uses
+      const void* b_bank = a.n_slots > 0 ? a.b_bank : a.w;
+      if (!make_map(&many.x, p->dtype, a.x, a.K, a.T, x_pitch, 64, 1) ||
+          !make_map(&many.a, p->dtype, a_bank, a.K, bank_rows, w_pitch, 64, 16) ||
+          !make_map(&many.s_hi, p->dtype, a.s_hi, a.r_pad, a.T, s_pitch, 16, 128) ||
+          !make_map(&many.s_lo, p->dtype, a.s_lo, a.r_pad, a.T, s_pitch, 16, 128) ||
+          !make_map(&many.b, p->dtype, b_bank, 16, bank_rows / 16 * a.N, 32, 16, 256))
+        return LF_ERR_UNSUPPORTED;
+    }
     if (rows_use_pairs(a.T, a.K, a.N, ds->num_sms)) {
       TcMaps maps;
       if (!make_map(&maps.p, p->dtype, a.x, a.K, a.T, x_pitch, 64, 128) ||
@@ -914,7 +959,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
       tb.r_pad = 16;
       tb.err = ds->status;
       const PairDelta delta{a.delta, a.eff, (a.N + 15) / 16 * 16};
-      e = rows_lora_part(a, p->dtype, ds->num_sms, st);
+      e = rows_many_part(a, p->dtype, many, ds->num_sms, st);
       if (e == cudaSuccess)
         e = tc_gemm_pair(p->dtype, false, maps, a.T, a.N, a.K, false, tb, a.y, a.N, ds->num_sms, st, nullptr, nullptr,
                          &delta);
@@ -924,7 +969,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
       if (!make_map(&w_map, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128) ||
           !make_map(&x_map, p->dtype, a.x, a.K, a.T, x_pitch, 64, tiles.rows))
         return LF_ERR_UNSUPPORTED;
-      e = rows_forward_tc(a, p->dtype, w_map, x_map, tiles, ds->num_sms, st);
+      e = rows_forward_tc(a, p->dtype, w_map, x_map, tiles, a.T > kFewRows ? &many : nullptr, ds->num_sms, st);
     }
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }

@@ -169,7 +169,7 @@ cudaError_t tc_gram(int dtype, const GramJobDesc* jobs, int n_jobs, const Tables
                     int planes = 1, void* scratch = nullptr, uint64_t gen = 0, const GramPeer* peer = nullptr);
 
 // --------------------------------------------------------------- rows with an adapter each
-// lf_rows_problem plus the workspace the two launches share.
+// lf_rows_problem plus the workspace the launches share.
 struct RowsArgs {
   const void* x;
   const void* w;
@@ -183,9 +183,13 @@ struct RowsArgs {
   int T, K, N, n_slots, r_pad;
   int wide;          // row_slot entries are 64-bit
   uint32_t* eff;     // [T] rank << 24 | slot of each row, all ones without an adapter
-  float* factor;     // [T] s_i times the power of two S was divided by (tensor-core path)
   void* s_hi;        // [T][r_pad] high halves of S (float32 S itself on the CUDA-core path)
   void* s_lo;        // [T][r_pad] low halves
+  // long batches: S, its factors and `perm` are in the order of the rows sorted by adapter
+  float* factor;     // [T] s_i times the power of two S was divided by
+  int* perm;         // [T] row of each sorted row
+  void* tiles;       // [T] runs of sorted rows of one adapter, 16 bytes each
+  int* n_tiles;
   float* delta;      // [T][N rounded up to 16] the adapters' part of rows that have one
   int* err;          // device status word
 };
@@ -194,13 +198,21 @@ struct RowsTiles {
   int ksplit;  // CTAs that share a tile, each with a part of K
 };
 RowsTiles rows_tiles(int T, int K, int N, int num_sms);
-// w: [N, K] box (64, 128), x: [T, K] box (64, tiles.rows), both with the 128-byte swizzle
-cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
-                            int num_sms, cudaStream_t st);
-// The adapters' part alone (a.delta, a.eff), for a GEMM that adds it: tc_gemm_pair's `delta`.
-cudaError_t rows_lora_part(const RowsArgs& a, int dtype, int num_sms, cudaStream_t st);
-bool rows_use_pairs(int T, int K, int N, int num_sms);
+// What the adapters' part of many rows is read through.
+struct ManyMaps {
+  CUtensorMap x;           // [T, K] box (64, 1), 128-byte swizzle: rows are gathered
+  CUtensorMap a;           // bank A [n_slots r_pad, K] box (64, 16), 128-byte swizzle
+  CUtensorMap s_hi, s_lo;  // S [T, r_pad] box (16, 128), 32-byte swizzle
+  CUtensorMap b;           // bank B [n_slots r_pad/16 N, 16] box (16, 256), 32-byte swizzle
+};
 constexpr int kRowsChunk = 8192;  // rows whose adapters' part is held at a time
+constexpr int kFewRows = 256;  // rows from which the adapters' part takes the launches for many rows
+// w: [N, K] box (64, 128), x: [T, K] box (64, tiles.rows), both with the 128-byte swizzle; m: null up to kFewRows rows
+cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
+                            const ManyMaps* m, int num_sms, cudaStream_t st);
+// The adapters' part alone (a.delta, a.eff), for a GEMM that adds it: tc_gemm_pair's `delta`.
+cudaError_t rows_many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_sms, cudaStream_t st);
+bool rows_use_pairs(int T, int K, int N, int num_sms);
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
 
 // --------------------------------------------------------------- packing

@@ -87,15 +87,14 @@ __device__ __forceinline__ void st_cluster_f32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
 
-// One warp's K steps k0 .. k1 - 1 (32 elements each) of up to kNB groups of one adapter (rank up to 16 kMT) into its
-// slots of `part`.  Few instructions a step count more here than anything else (with the bounds of K and
-// of the rows tested on every load a step took 90): whole steps run without a test, and a row that a group
-// does not have points at one that exists, for columns nobody reads.
-template <typename T, int kMT, int kNB, int kUnroll>
-__device__ __forceinline__ void shrink_steps(float (&acc)[kMT][kNB][4], const T* const (&xr)[kNB], const T* ar, int K,
-                                             int k, bool in) {
+// One warp's K steps k0 .. k1 - 1 (32 elements each) of a group's rows with A_i (rank up to 16 kMT), into its slot of
+// `part`.  Few instructions a step count more here than anything else (with the bounds of K and of the rows
+// tested on every load a step took 90): whole steps run without a test, and a row that the group does not
+// have points at one that exists, for a column nobody reads.
+template <typename T, int kMT, int kUnroll>
+__device__ __forceinline__ void shrink_steps(float (&acc)[kMT][4], const T* xr, const T* ar, int K, int k, bool in) {
   const uint4 zero = make_uint4(0, 0, 0, 0);
-  uint4 xv[kUnroll][kNB], lo[kUnroll][kMT], hi[kUnroll][kMT];
+  uint4 xv[kUnroll], lo[kUnroll][kMT], hi[kUnroll][kMT];
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i) {
 #pragma unroll
@@ -103,46 +102,33 @@ __device__ __forceinline__ void shrink_steps(float (&acc)[kMT][kNB][4], const T*
       lo[i][m] = in ? *reinterpret_cast<const uint4*>(ar + m * 16 * K + (k + i) * 32) : zero;
       hi[i][m] = in ? *reinterpret_cast<const uint4*>(ar + (m * 16 + 8) * K + (k + i) * 32) : zero;
     }
-#pragma unroll
-    for (int b = 0; b < kNB; ++b) xv[i][b] = in ? *reinterpret_cast<const uint4*>(xr[b] + (k + i) * 32) : zero;
+    xv[i] = in ? *reinterpret_cast<const uint4*>(xr + (k + i) * 32) : zero;
   }
 #pragma unroll
   for (int i = 0; i < kUnroll; ++i)
 #pragma unroll
-    for (int m = 0; m < kMT; ++m)
-#pragma unroll
-      for (int b = 0; b < kNB; ++b) {
-        mma16816(acc[m][b], lo[i][m].x, hi[i][m].x, lo[i][m].y, hi[i][m].y, xv[i][b].x, xv[i][b].y,
-                 static_cast<T*>(nullptr));
-        mma16816(acc[m][b], lo[i][m].z, hi[i][m].z, lo[i][m].w, hi[i][m].w, xv[i][b].z, xv[i][b].w,
-                 static_cast<T*>(nullptr));
-      }
+    for (int m = 0; m < kMT; ++m) {
+      mma16816(acc[m], lo[i][m].x, hi[i][m].x, lo[i][m].y, hi[i][m].y, xv[i].x, xv[i].y, static_cast<T*>(nullptr));
+      mma16816(acc[m], lo[i][m].z, hi[i][m].z, lo[i][m].w, hi[i][m].w, xv[i].z, xv[i].w, static_cast<T*>(nullptr));
+    }
 }
-template <typename T, int kMT, int kNB, int kUnroll, int kStride>
-__device__ __forceinline__ void shrink_groups(const T* const (&xr)[kNB], const T* ar, int K, int k0, int k1, int nb,
-                                              float* dst) {
+template <typename T, int kMT, int kUnroll>
+__device__ __forceinline__ void shrink_groups(const T* xr, const T* ar, int K, int k0, int k1, float* dst) {
   const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  float acc[kMT][kNB][4];
+  float acc[kMT][4];
 #pragma unroll
-  for (int m = 0; m < kMT; ++m)
-#pragma unroll
-    for (int b = 0; b < kNB; ++b) acc[m][b][0] = acc[m][b][1] = acc[m][b][2] = acc[m][b][3] = 0.f;
+  for (int m = 0; m < kMT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
   const int whole = min(k1, K / 32);
   int k = k0;
 #pragma unroll 1
-  for (; k + kUnroll <= whole; k += kUnroll) shrink_steps<T, kMT, kNB, kUnroll>(acc, xr, ar, K, k, true);
+  for (; k + kUnroll <= whole; k += kUnroll) shrink_steps<T, kMT, kUnroll>(acc, xr, ar, K, k, true);
 #pragma unroll 1
-  for (; k < k1; ++k) shrink_steps<T, kMT, kNB, 1>(acc, xr, ar, K, k, k * 32 + 8 * q < K);
+  for (; k < k1; ++k) shrink_steps<T, kMT, 1>(acc, xr, ar, K, k, k * 32 + 8 * q < K);
 #pragma unroll
-  for (int b = 0; b < kNB; ++b) {
-    if (b < nb) {
-#pragma unroll
-      for (int m = 0; m < kMT; ++m) {
-        float* at = dst + b * kStride + (m * 16 + g) * 8 + 2 * q;
-        *reinterpret_cast<float2*>(at) = make_float2(acc[m][b][0], acc[m][b][1]);
-        *reinterpret_cast<float2*>(at + 64) = make_float2(acc[m][b][2], acc[m][b][3]);
-      }
-    }
+  for (int m = 0; m < kMT; ++m) {
+    float* at = dst + (m * 16 + g) * 8 + 2 * q;
+    *reinterpret_cast<float2*>(at) = make_float2(acc[m][0], acc[m][1]);
+    *reinterpret_cast<float2*>(at + 64) = make_float2(acc[m][2], acc[m][3]);
   }
 }
 
@@ -269,89 +255,82 @@ struct GroupRows {
   float f0, f1;
 };
 
-// The second product of up to kNB groups of one adapter for output blocks b0 .. b1 - 1 (16 features each): kNM rank
-// steps of 16, kPer blocks loaded together.  B_i is stored in the order of the MMA's operand: one 16-byte load a
-// lane and step.
-template <typename T, int kNM, int kNB, int kPer>
-__device__ __forceinline__ void expand_blocks(const uint4* w, int pitch, const uint2 (&sh)[kNB][kNM],
-                                              const uint2 (&sl)[kNB][kNM], const GroupRows<T> (&rows)[kNB],
-                                              float* const (&o0)[kNB], float* const (&o1)[kNB], int at, int nb,
+// The second product of one group for output blocks b0 .. b1 - 1 (16 features each): kNM rank steps of 16, kPer blocks
+// loaded together.  A block of a step is 512 contiguous bytes of B_i.  The order of K inside an MMA is free, so
+// over two steps a lane takes 16 bytes: 8 ranks of one step, of which the first MMA multiplies 4 and the second the
+// others.  The second half of a last, half block repeats the first, for results that land in the padding of
+// `delta`.
+template <typename T, int kNM, int kPer>
+__device__ __forceinline__ void expand_blocks(const uint2* w, int N, int n, const uint2 (&sh)[kNM],
+                                              const uint2 (&sl)[kNM], const GroupRows<T>& rows, float* o0, float* o1,
                                               bool second) {
   T* const tag = nullptr;
-  uint4 v[kPer][kNM];
-#pragma unroll
-  for (int i = 0; i < kPer; ++i)
-#pragma unroll
-    for (int k = 0; k < kNM; ++k) v[i][k] = w[k * pitch + (at + i) * 32];
+  uint2 u[kPer][kNM], v[kPer][kNM];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
+    const int half = n + i * 16 + 8 < N ? 32 : 0;
+    if constexpr (kNM == 1) {
+      u[i][0] = w[i * 64];
+      v[i][0] = w[i * 64 + half];
+    } else {
 #pragma unroll
-    for (int b = 0; b < kNB; ++b) {
-      if (b < nb) {
-        float d[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < kNM; ++k) {
-          mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sh[b][k].x, sh[b][k].y, tag);
-          mma16816(d, v[i][k].x, v[i][k].z, v[i][k].y, v[i][k].w, sl[b][k].x, sl[b][k].y, tag);
-        }
-        float* p0 = o0[b] + (at + i) * 16;
-        float* p1 = o1[b] + (at + i) * 16;
-        if (rows[b].row0 >= 0) p0[0] = rows[b].f0 * d[0], p0[8] = rows[b].f0 * d[2];
-        if (second && rows[b].row1 >= 0) p1[0] = rows[b].f1 * d[1], p1[8] = rows[b].f1 * d[3];
+      for (int k = 0; k < kNM; k += 2) {
+        const uint2* at = w + static_cast<size_t>(k) * N * 4 + i * 64;
+        const uint4 a = *reinterpret_cast<const uint4*>(at), b = *reinterpret_cast<const uint4*>(at + half);
+        u[i][k] = make_uint2(a.x, a.y), u[i][k + 1] = make_uint2(a.z, a.w);
+        v[i][k] = make_uint2(b.x, b.y), v[i][k + 1] = make_uint2(b.z, b.w);
       }
     }
   }
-}
-template <typename T, int kNM, int kNB, int kPer>
-__device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int b0, int b1,
-                                             const GroupRows<T> (&rows)[kNB], int nb) {
-  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int blocks = (p.N + 15) >> 4, steps = p.r_pad >> 4;
-  uint2 sh[kNB][kNM], sl[kNB][kNM];
-  float *o0[kNB], *o1[kNB];
-  bool odd = false;
 #pragma unroll
-  for (int b = 0; b < kNB; ++b) {
+  for (int i = 0; i < kPer; ++i) {
+    float d[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < kNM; ++k) {
-      const bool on = 16 * k < rank_of(e);
-      sh[b][k] = on ? *reinterpret_cast<const uint2*>(rows[b].hi + 16 * k + 4 * q) : make_uint2(0, 0);
-      sl[b][k] = on ? *reinterpret_cast<const uint2*>(rows[b].lo + 16 * k + 4 * q) : make_uint2(0, 0);
+      mma16816(d, u[i][k].x, v[i][k].x, u[i][k].y, v[i][k].y, sh[k].x, sh[k].y, tag);
+      mma16816(d, u[i][k].x, v[i][k].x, u[i][k].y, v[i][k].y, sl[k].x, sl[k].y, tag);
     }
-    o0[b] = p.delta + static_cast<size_t>(max(rows[b].row0, 0)) * blocks * 16 + g;
-    o1[b] = p.delta + static_cast<size_t>(max(rows[b].row1, 0)) * blocks * 16 + g;
-    odd = odd || rows[b].row1 >= 0;
+    if (rows.row0 >= 0) o0[i * 16] = rows.f0 * d[0], o0[i * 16 + 8] = rows.f0 * d[2];
+    if (second && rows.row1 >= 0) o1[i * 16] = rows.f1 * d[1], o1[i * 16 + 8] = rows.f1 * d[3];
   }
-  const bool second = __any_sync(0xffffffffu, odd);
-  const uint4* w = static_cast<const uint4*>(p.b_bank) + static_cast<size_t>(slot_of(e)) * steps * blocks * 32 + lane;
-  int b = b0;
-#pragma unroll 1
-  for (; b + kPer <= b1; b += kPer)
-    expand_blocks<T, kNM, kNB, kPer>(w, blocks * 32, sh, sl, rows, o0, o1, b, nb, second);
-#pragma unroll 1
-  for (; b < b1; ++b) expand_blocks<T, kNM, kNB, 1>(w, blocks * 32, sh, sl, rows, o0, o1, b, nb, second);
 }
-
-// Groups from `grp` on, at most kNB and `most`, that belong to one adapter.
-template <int kNB>
-__device__ __forceinline__ int unit_size(const Groups& s, int grp, int most) {
-  int nb = 1;
-  if (kNB > 1) {
-    const uint32_t e = s.eff[s.start[grp]];
-    while (nb < kNB && nb < most && s.eff[s.start[grp + nb]] == e) ++nb;
+template <typename T, int kNM, int kPer>
+__device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int b0, int b1, const GroupRows<T>& rows) {
+  const int lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int pitch = (p.N + 15) & ~15;
+  uint2 sh[kNM], sl[kNM];
+  const uint2 zero = make_uint2(0, 0);
+  // the lane's step and first rank of a pair of steps (of the only step)
+  const int step = kNM == 1 ? 0 : q >> 1, rank0 = kNM == 1 ? 4 * q : 8 * (q & 1);
+#pragma unroll
+  for (int k = 0; k < kNM; ++k) {
+    const int at = 16 * ((k & ~1) + step);  // beyond the rank nothing was written
+    const bool on = at < rank_of(e);
+    const int r = at + rank0 + 4 * (k & 1);
+    sh[k] = on ? *reinterpret_cast<const uint2*>(rows.hi + r) : zero;
+    sl[k] = on ? *reinterpret_cast<const uint2*>(rows.lo + r) : zero;
   }
-  return nb;
+  const bool second = __any_sync(0xffffffffu, rows.row1 >= 0);
+  float* o0 = p.delta + static_cast<size_t>(max(rows.row0, 0)) * pitch + b0 * 16 + g;
+  float* o1 = p.delta + static_cast<size_t>(max(rows.row1, 0)) * pitch + b0 * 16 + g;
+  const uint2* w = static_cast<const uint2*>(p.b_bank) + rank0 / 4 +
+                   ((static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) + step) * p.N + b0 * 16 + g) * 4;
+  int n = b0 * 16;
+  const int end = b1 * 16;
+#pragma unroll 1
+  for (; n + kPer * 16 <= end; n += kPer * 16, w += kPer * 64, o0 += kPer * 16, o1 += kPer * 16)
+    expand_blocks<T, kNM, kPer>(w, p.N, n, sh, sl, rows, o0, o1, second);
+#pragma unroll 1
+  for (; n < end; n += 16, w += 64, o0 += 16, o1 += 16)
+    expand_blocks<T, kNM, 1>(w, p.N, n, sh, sl, rows, o0, o1, second);
 }
 
 // Work items: (row tile, slice of its groups), each taken by a cluster of `kparts` CTAs that cut K for the
 // first product and the output features for the second.  Partial products
 // meet in shared memory, then across the cluster, in a fixed order.  The grid fits the GPU at once, so
 // the dependent GEMM streams its weight while this kernel runs.
-// kNB = 1: a few rows, clusters.  kNB > 1: many rows (prompts), no cluster; up to kNB groups of one adapter share
-// what is read of it.
-template <typename T, int kMT, int kNB>
-__global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts_) {
-  const int kparts = kNB > 1 ? 1 : kparts_;
+template <typename T, int kMT>
+__global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts) {
   constexpr int kRP = kMT * 16;                                         // padded rank
   constexpr int kBatch = kPartBytes / (kShrinkWarps * kRP * 8 * 4);     // groups of 8 rows per batch
   constexpr int kPitch = kRP + 8;                                       // of S rows: no bank conflicts
@@ -381,46 +360,27 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
     const int g_hi = slice + 1 < slices ? slice_start(s, n_groups, slice + 1, slices) : n_groups;
     for (int first = g_lo; first < g_hi; first += kBatch) {
       const int batch = min(kBatch, g_hi - first);
-      // Up to kNB groups of one adapter are a unit.  The warps divide the units first, so that as many streams
-      // of A_i as there are warps are in flight, and K where there are fewer units than warps.
-      int n_units = 0;
-      for (int u = 0; u < batch; u += unit_size<kNB>(s, first + u, batch - u)) ++n_units;
-      const int lanes = n_units >= 8 ? 8 : n_units >= 4 ? 4 : n_units >= 2 ? 2 : 1;  // units at a time
+      // The warps divide the groups first, so that as many streams of A_i as there are warps are in flight, and K
+      // where there are fewer groups than warps.
+      const int lanes = batch >= 8 ? 8 : batch >= 4 ? 4 : batch >= 2 ? 2 : 1;  // groups at a time
       const int subs = kShrinkWarps / lanes, sub = warp / lanes;
       const int ranges = kparts * subs, me = crank * subs + sub;
       const int b0 = static_cast<int>(static_cast<int64_t>(me) * n_blocks / ranges);
       const int b1 = static_cast<int>(static_cast<int64_t>(me + 1) * n_blocks / ranges);
-      for (int u = 0, index = 0, nb; u < batch; u += nb, ++index) {
-        nb = unit_size<kNB>(s, first + u, batch - u);
-        if (index % lanes != warp % lanes) continue;
+      for (int u = warp % lanes; u < batch; u += lanes) {
         const uint32_t e = s.eff[s.start[first + u]];
         const int nm = (rank_of(e) + 15) >> 4;
-        const T* xr[kNB];
-#pragma unroll
-        for (int b = 0; b < kNB; ++b) {
-          const int row = b < nb ? s.rows[first + u + b][g] : 0;
-          xr[b] = x + static_cast<int64_t>(t0 + max(row, 0)) * p.ldx + 8 * q;
-        }
+        const T* xr = x + static_cast<int64_t>(t0 + max(static_cast<int>(s.rows[first + u][g]), 0)) * p.ldx + 8 * q;
         const T* ar = bank + (static_cast<size_t>(slot_of(e)) * p.r_pad + g) * K + 8 * q;
         float* dst = part[sub][u];
-        const T* const one_x[1] = {xr[0]};
-        constexpr int kS = kRP * 8;
-        // the smallest kernel that covers the adapter's rank and the groups at hand
-        if (nm == 1) {
-          if (kNB == 1 || nb == 1) shrink_groups<T, 1, 1, 8, kS>(one_x, ar, K, b0, b1, 1, dst);
-          else shrink_groups<T, 1, kNB, 2, kS>(xr, ar, K, b0, b1, nb, dst);
-        } else if (nm == 2) {
-          if constexpr (kMT >= 2) {
-            if (kNB == 1 || nb == 1) shrink_groups<T, 2, 1, 4, kS>(one_x, ar, K, b0, b1, 1, dst);
-            else shrink_groups<T, 2, kNB, 2, kS>(xr, ar, K, b0, b1, nb, dst);
-          }
+        // the smallest kernel that covers the adapter's rank
+        if (nm == 1) shrink_groups<T, 1, 8>(xr, ar, K, b0, b1, dst);
+        else if (nm == 2) {
+          if constexpr (kMT >= 2) shrink_groups<T, 2, 4>(xr, ar, K, b0, b1, dst);
         } else if (nm <= 4) {
-          if constexpr (kMT >= 4) {
-            if (kNB == 1 || nb == 1) shrink_groups<T, 4, 1, 2, kS>(one_x, ar, K, b0, b1, 1, dst);
-            else shrink_groups<T, 4, kNB, 1, kS>(xr, ar, K, b0, b1, nb, dst);
-          }
+          if constexpr (kMT >= 4) shrink_groups<T, 4, 2>(xr, ar, K, b0, b1, dst);
         } else if constexpr (kMT >= 8) {
-          shrink_groups<T, 8, 1, 1, kS>(one_x, ar, K, b0, b1, 1, dst);
+          shrink_groups<T, 8, 1>(xr, ar, K, b0, b1, dst);
         }
       }
       __syncthreads();
@@ -476,33 +436,26 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
         }
       }
       __syncthreads();
-      // the warps divide the units, then the features, here too
+      // the warps divide the groups, then the features, here too
       const int f0 = nb0 + (nb1 - nb0) * sub / subs, f1 = nb0 + (nb1 - nb0) * (sub + 1) / subs;
-      for (int u = 0, index = 0, nb; u < batch; u += nb, ++index) {
-        nb = unit_size<kNB>(s, first + u, batch - u);
-        if (index % lanes != warp % lanes) continue;
+      for (int u = warp % lanes; u < batch; u += lanes) {
         const uint32_t e = s.eff[s.start[first + u]];
         const int nm = (rank_of(e) + 15) >> 4;
-        GroupRows<T> rows_of[kNB];
-#pragma unroll
-        for (int b = 0; b < kNB; ++b) {
-          const int v = u + min(b, nb - 1);
-          rows_of[b].hi = s_hi[v][g];
-          rows_of[b].lo = s_lo[v][g];
-          const int r0 = b < nb ? s.rows[first + v][2 * q] : -1, r1 = b < nb ? s.rows[first + v][2 * q + 1] : -1;
-          rows_of[b].row0 = r0 < 0 ? -1 : t0 + r0;
-          rows_of[b].row1 = r1 < 0 ? -1 : t0 + r1;
-          rows_of[b].f0 = s_fac[v][2 * q];
-          rows_of[b].f1 = s_fac[v][2 * q + 1];
-        }
-        constexpr int kPer = kNB > 1 ? 4 : 8;  // 16-byte loads in flight a lane
-        if (nm == 1) expand_group<T, 1, kNB, kPer>(p, e, f0, f1, rows_of, nb);
+        GroupRows<T> rows_of;
+        const int r0 = s.rows[first + u][2 * q], r1 = s.rows[first + u][2 * q + 1];
+        rows_of.hi = s_hi[u][g];
+        rows_of.lo = s_lo[u][g];
+        rows_of.row0 = r0 < 0 ? -1 : t0 + r0;
+        rows_of.row1 = r1 < 0 ? -1 : t0 + r1;
+        rows_of.f0 = s_fac[u][2 * q];
+        rows_of.f1 = s_fac[u][2 * q + 1];
+        if (nm == 1) expand_group<T, 1, 8>(p, e, f0, f1, rows_of);
         else if (nm == 2) {
-          if constexpr (kMT >= 2) expand_group<T, 2, kNB, kPer / 2>(p, e, f0, f1, rows_of, nb);
+          if constexpr (kMT >= 2) expand_group<T, 2, 4>(p, e, f0, f1, rows_of);
         } else if (nm <= 4) {
-          if constexpr (kMT >= 4) expand_group<T, 4, kNB, kPer / 4>(p, e, f0, f1, rows_of, nb);
+          if constexpr (kMT >= 4) expand_group<T, 4, 2>(p, e, f0, f1, rows_of);
         } else if constexpr (kMT >= 8) {
-          expand_group<T, 8, kNB, 1>(p, e, f0, f1, rows_of, nb);
+          expand_group<T, 8, 1>(p, e, f0, f1, rows_of);
         }
       }
       __syncthreads();
@@ -725,6 +678,465 @@ __global__ void __maxnreg__(80)
   if (warp == 1) tmem_dealloc(tmem, kCols);
 }
 
+// ============================================================================ many rows
+// The adapters' part of long batches (prompts).  The rows are sorted by adapter on the device into tiles of up to 128
+// rows of one adapter, and both products run on tcgen05 with the tile's rows as M: x is gathered row by row for the
+// first, S kept in sorted order, and the second product's rows are written to their own places in `delta`.
+// Which tile a row falls into, and where, depends on the order of atomics; a row's result does not, since
+// no row of an MMA sees another.  (Other ways, 8192 x 4096 -> 4096, 64 adapters of rank up to 64, prompts / shuffled
+// tokens, the part that is not hidden by the GEMM: groups of 8 rows with warp-level MMAs 154 / 373 us, every group
+// fetching its A_i and B_i again; 128 rows as they come, multiplied by every adapter among them, 112 / 1110 us.)
+struct ManyTile {
+  uint32_t e;  // adapter
+  int first;   // of the sorted rows
+  int rows;
+  int pad;
+};
+
+// Sorts at most kRowsChunk rows: a hash table of adapters in shared memory counts them, a scan places them.
+constexpr int kPlanThreads = 1024;
+constexpr int kPlanSlots = 2 * kRowsChunk;  // of the table: never more than half full
+constexpr int kPlanRows = kRowsChunk / kPlanThreads, kPlanPer = kPlanSlots / kPlanThreads;
+constexpr int kPlanSmem = kPlanSlots * 8;
+__global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsArgs p) {
+  extern __shared__ uint32_t plan_smem[];
+  uint32_t* key = plan_smem;
+  uint32_t* count = plan_smem + kPlanSlots;  // then the first sorted row
+  __shared__ int warp_rows[32], warp_tiles[32];
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint32_t e[kPlanRows];  // loads of one kind together: two latencies, not sixteen
+  int64_t slot[kPlanRows];
+#pragma unroll
+  for (int i = 0; i < kPlanRows; ++i) {
+    const int t = tid + i * kPlanThreads;
+    slot[i] = t >= p.T ? -1 : p.wide ? static_cast<const int64_t*>(p.row_slot)[t] : static_cast<const int32_t*>(p.row_slot)[t];
+  }
+#pragma unroll
+  for (int i = 0; i < kPlanRows; ++i) {
+    const bool in = slot[i] >= 0 && slot[i] < p.n_slots;
+    if (slot[i] >= p.n_slots) record_error(p.err, kErrRowSlot);
+    const int r = in ? min(p.slot_rank[slot[i]], p.r_pad) : 0;
+    e[i] = r <= 0 ? kNoSlot : static_cast<uint32_t>(r) << 24 | static_cast<uint32_t>(slot[i]);
+    if (tid + i * kPlanThreads < p.T) p.eff[tid + i * kPlanThreads] = e[i];
+  }
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    key[tid + i * kPlanThreads] = kNoSlot;
+    count[tid + i * kPlanThreads] = 0;
+  }
+  __syncthreads();
+  uint32_t at[kPlanRows], pos[kPlanRows];
+#pragma unroll
+  for (int i = 0; i < kPlanRows; ++i) {
+    at[i] = pos[i] = 0;
+    const uint32_t same = __match_any_sync(0xffffffffu, e[i]);
+    const int lead = __ffs(same) - 1;
+    if (e[i] != kNoSlot && lane == lead) {
+      uint32_t h = (e[i] * 0x9e3779b1u) >> 18;
+      static_assert(kPlanSlots == 1 << 14, "the hash's bits");
+      for (;;) {
+        const uint32_t was = atomicCAS(&key[h], kNoSlot, e[i]);
+        if (was == kNoSlot || was == e[i]) break;
+        h = (h + 1) & (kPlanSlots - 1);
+      }
+      at[i] = h;
+      pos[i] = atomicAdd(&count[h], __popc(same));
+    }
+    at[i] = __shfl_sync(0xffffffffu, at[i], lead);
+    pos[i] = __shfl_sync(0xffffffffu, pos[i], lead) + __popc(same & ((1u << lane) - 1));
+  }
+  __syncthreads();
+  int rows = 0, tiles = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int c = static_cast<int>(count[tid + i * kPlanThreads]);
+    rows += c;
+    tiles += (c + kTileRows - 1) / kTileRows;
+  }
+  int row0 = rows, tile0 = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int r = __shfl_up_sync(0xffffffffu, row0, o), t = __shfl_up_sync(0xffffffffu, tile0, o);
+    if (lane >= o) row0 += r, tile0 += t;
+  }
+  if (lane == 31) warp_rows[warp] = row0, warp_tiles[warp] = tile0;
+  __syncthreads();
+  row0 -= rows, tile0 -= tiles;
+  for (int w = 0; w < warp; ++w) row0 += warp_rows[w], tile0 += warp_tiles[w];
+  if (tid == kPlanThreads - 1) *p.n_tiles = tile0 + tiles;
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int h = tid + i * kPlanThreads, c = static_cast<int>(count[h]);
+    count[h] = row0;
+    for (int r = 0; r < c; r += kTileRows)
+      static_cast<ManyTile*>(p.tiles)[tile0++] = ManyTile{key[h], row0 + r, min(kTileRows, c - r), 0};
+    row0 += c;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPlanRows; ++i)
+    if (e[i] != kNoSlot) p.perm[count[at[i]] + pos[i]] = tid + i * kPlanThreads;
+}
+
+// S = x A_i^T of a tile, in sorted order.  K is cut over a cluster when there cannot be many tiles.
+constexpr int kShrinkStages = 4;
+constexpr int kShrinkStageBytes = kWBytes + LF_BANK_MAX_RANK * kBK * 2;  // 128 rows of x, up to 128 of A_i
+struct ManyShrink {
+  RowsArgs a;
+  int ksplit, pitch;  // floats from one row's S to the next in shared memory
+  int ab_fmt;
+};
+template <typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    many_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a,
+                       const __grid_constant__ ManyShrink prm) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* s_part = reinterpret_cast<float*>(ring + kShrinkStages * kShrinkStageBytes);  // [128][pitch]
+  __shared__ uint64_t full[kShrinkStages], empty[kShrinkStages], acc_full, drain_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const RowsArgs& p = prm.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int ks = prm.ksplit, part = blockIdx.x % ks;
+  const int nkb = (p.K + kBK - 1) / kBK;
+  const int kb0 = static_cast<int>(static_cast<int64_t>(part) * nkb / ks);
+  const int kb1 = static_cast<int>(static_cast<int64_t>(part + 1) * nkb / ks);
+  if (tid == 0) {
+    for (int s = 0; s < kShrinkStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(&acc_full, 1);
+    mbar_init(&drain_bar, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, LF_BANK_MAX_RANK);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();  // not before this CTA has its tensor memory: the next kernel's could take it and wait for us
+  pdl_wait();
+  const uint32_t tmem = tmem_slot;
+  const int n_tiles = *p.n_tiles;
+  const uint64_t x0 = umma_sdesc(smem_u32(ring), 16, 1024, 2);
+  int stage = 0;  // of the loading warp, of the MMA thread
+  uint32_t phase = 0, issued = 0, parity = 0, done = 0, drained = 0;
+  for (int i = blockIdx.x / ks; i < n_tiles; i += gridDim.x / ks, done ^= 1) {
+    const ManyTile tile = static_cast<const ManyTile*>(p.tiles)[i];
+    const int slot = slot_of(tile.e), rank = rank_of(tile.e), steps = (rank + 15) >> 4;
+    bool ok = true;
+    if (warp == 0) {
+      // a lane gathers four rows of x: 128 bytes of each a stage; rows past the last one repeat it
+      const int loads = (tile.rows + 3) >> 2;
+      int r[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) r[j] = p.perm[tile.first + min(4 * lane + j, tile.rows - 1)];
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (lane == 0) {
+          ok = mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
+          if (ok) mbar_arrive_expect_tx(&full[stage], loads * 512 + steps * 16 * kBK * 2);
+        }
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        uint8_t* d = ring + stage * kShrinkStageBytes;
+        if (lane < loads) tma_gather4(d + lane * 512, &map_x, &full[stage], kb * kBK, r[0], r[1], r[2], r[3]);
+        if (lane < steps)
+          tma_load_2d(d + kWBytes + lane * 16 * kBK * 2, &map_a, &full[stage], kb * kBK, slot * p.r_pad + 16 * lane);
+        issued |= 1u << stage;
+        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == kShrinkStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    } else if (warp == 1) {
+      if (lane == 0) {
+        const uint32_t idesc = umma_idesc_f16(kTileRows, steps * 16, prm.ab_fmt, 0, 0);
+        uint32_t acc = 0;
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t x = x0 + ((stage * kShrinkStageBytes) >> 4), w = x + (kWBytes >> 4);
+#pragma unroll
+          for (int k = 0; k < kBK / 16; ++k) {
+            umma_f16(tmem, x + 2 * k, w + 2 * k, idesc, acc);
+            acc = 1;
+          }
+          umma_commit(&empty[stage]);
+          if (++stage == kShrinkStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok) umma_commit(&acc_full);
+        else if (acc) {
+          umma_commit(&drain_bar);
+          drain_wait(&drain_bar, drained, p.err);
+          drained ^= 1;
+        }
+      }
+      __syncwarp();
+    } else if (warp_wait(&acc_full, done, &abort_flag, p.err, kErrTimeoutAcc)) {
+      // the two warps of a lane quarter take alternate steps
+      tc_fence_after();
+      const int quad = warp & 3, row = quad * 32 + lane;
+      if (quad * 32 < tile.rows) {
+        for (int k = (warp - 2) >> 2; k < steps; k += 2) {
+          uint32_t v[16];
+          tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + 16 * k, v);
+          tmem_wait_ld();
+          uint4* to = reinterpret_cast<uint4*>(s_part + row * prm.pitch + 16 * k);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) to[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+        }
+      }
+      tc_fence_before();
+    }
+    if (ks > 1) cluster_sync_all();
+    else __syncthreads();
+    tc_fence_after();
+    // this CTA's rows of the tile: sum over the cluster in a fixed order, scale, split
+    const float scale = p.slot_scale[slot];
+    for (int row = part + ks * warp; row < tile.rows; row += ks * (kGemmThreads / 32)) {
+      const size_t to = static_cast<size_t>(tile.first + row);
+      float v[LF_BANK_MAX_RANK / 32];
+      float top = 0.f;
+#pragma unroll
+      for (int k = 0; k < LF_BANK_MAX_RANK / 32; ++k) {
+        const int j = lane + 32 * k;
+        v[k] = 0.f;
+        if (j < rank) {
+          const float* at = s_part + row * prm.pitch + j;
+          if (ks == 1) v[k] = *at;
+          else
+            for (int c = 0; c < ks; ++c) v[k] += ld_cluster_f32(map_to_cta(smem_u32(at), c));
+        }
+        top = fmaxf(top, fabsf(v[k]));
+        if (!(fabsf(v[k]) <= 3.402823466e38f)) top = __int_as_float(0x7f800000);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      const int ex = row_exponent(top);
+      const float down = scalbnf(1.f, -ex);
+      if (lane == 0) p.factor[to] = scale * scalbnf(1.f, ex);
+#pragma unroll
+      for (int k = 0; k < LF_BANK_MAX_RANK / 32; ++k) {
+        const int j = lane + 32 * k;
+        if (j < steps * 16) {
+          T hi, lo;
+          halves<T>(v[k] * down, hi, lo);
+          static_cast<T*>(p.s_hi)[to * p.r_pad + j] = hi;
+          static_cast<T*>(p.s_lo)[to * p.r_pad + j] = lo;
+        }
+      }
+    }
+    if (ks > 1) cluster_sync_all();  // peers have read this CTA's sums
+    else __syncthreads();
+  }  // when a wait has run out the remaining tiles' waits end at once: the cluster's CTAs stay in step
+  if (warp == 0 && lane == 0 && abort_flag)  // let every copy that was started land before the memory is used again
+    for (int s = 0; s < kShrinkStages; ++s)
+      if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
+  __syncthreads();
+  if (warp == 1) tmem_dealloc(tmem, LF_BANK_MAX_RANK);
+}
+
+// delta = s_i S B_i^T.  A unit is a tile x 256 features, and a CTA takes a run of them; the rank steps of S (high, then low
+// halves) times those of B_i go into one of two accumulators.
+constexpr int kSStepBytes = kTileRows * 32;  // 16 ranks of 128 rows
+constexpr int kBStepBytes = 256 * 32;        // 16 ranks of 256 features
+constexpr int kExpandStages = 5, kExpandChunk = 2;  // rank steps of a stage, at most
+constexpr int kExpandStepBytes = 2 * kSStepBytes + kBStepBytes;
+constexpr int kExpandStageBytes = kExpandChunk * kExpandStepBytes;
+constexpr int kDeltaStageBytes = 32 * 36 * 4;  // a warp's 32 rows x 32 columns, padded
+struct ManyExpand {
+  RowsArgs a;
+  uint32_t idesc;
+};
+template <typename T>
+__global__ void __launch_bounds__(kGemmThreads, 1)
+    many_expand_kernel(const __grid_constant__ CUtensorMap map_hi, const __grid_constant__ CUtensorMap map_lo,
+                       const __grid_constant__ CUtensorMap map_b, const __grid_constant__ ManyExpand prm) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* out = ring + kExpandStages * kExpandStageBytes;
+  __shared__ uint64_t full[kExpandStages], empty[kExpandStages], tfull[2], tempty[2], drain_bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
+  const RowsArgs& p = prm.a;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid == 0) {
+    for (int s = 0; s < kExpandStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], kEpiWarps);
+    }
+    mbar_init(&drain_bar, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  pdl_launch_dependents();  // after the allocation, as above
+  pdl_wait();
+  const uint32_t tmem = tmem_slot;
+  const ManyTile* tiles = static_cast<const ManyTile*>(p.tiles);
+  const int blocks = (p.N + 255) / 256;
+  const int64_t units = static_cast<int64_t>(*p.n_tiles) * blocks;
+  const int u0 = static_cast<int>(units * blockIdx.x / gridDim.x), u1 = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x);
+  if (warp == 0) {
+    if (lane == 0) {
+      fence_proxy_async_global();  // S was written by plain stores
+      int stage = 0;
+      uint32_t phase = 0, issued = 0, parity = 0;
+      bool ok = true;
+      for (int u = u0; u < u1 && ok; ++u) {
+        const ManyTile tile = tiles[u / blocks];
+        const int n0 = u % blocks * 256, steps = (rank_of(tile.e) + 15) >> 4;
+        const int row_b = slot_of(tile.e) * (p.r_pad >> 4) * p.N + n0;
+        for (int k0 = 0; k0 < steps; k0 += kExpandChunk) {
+          if (!mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
+            ok = false;
+            break;
+          }
+          const int ns = min(kExpandChunk, steps - k0);
+          mbar_arrive_expect_tx(&full[stage], ns * kExpandStepBytes);
+          uint8_t* d = ring + stage * kExpandStageBytes;
+          for (int k = k0; k < k0 + ns; ++k, d += kExpandStepBytes) {
+            tma_load_2d(d, &map_hi, &full[stage], 16 * k, tile.first);
+            tma_load_2d(d + kSStepBytes, &map_lo, &full[stage], 16 * k, tile.first);
+            tma_load_2d(d + 2 * kSStepBytes, &map_b, &full[stage], 0, row_b + k * p.N);
+          }
+          issued |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == kExpandStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok)
+        for (int s = 0; s < kExpandStages; ++s)
+          if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool any = false, ok = true;
+      const uint64_t s0 = umma_sdesc(smem_u32(ring), 16, 256, 6);
+      for (int u = u0; u < u1 && ok; ++u) {
+        const int steps = (rank_of(tiles[u / blocks].e) + 15) >> 4, buf = (u - u0) & 1;
+        if (!mbar_wait_stage(&tempty[buf], (((u - u0) >> 1) & 1) ^ 1, &abort_flag, p.err, kErrTimeoutAcc)) {
+          ok = false;
+          break;
+        }
+        const uint32_t d = tmem + buf * 256;
+        for (int k0 = 0; k0 < steps; k0 += kExpandChunk) {
+          if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          uint64_t s = s0 + ((stage * kExpandStageBytes) >> 4);
+          for (int k = k0; k < min(steps, k0 + kExpandChunk); ++k, s += kExpandStepBytes >> 4) {
+            const uint64_t w = s + ((2 * kSStepBytes) >> 4);
+            umma_f16(d, s, w, prm.idesc, k > 0);
+            umma_f16(d, s + (kSStepBytes >> 4), w, prm.idesc, 1);
+          }
+          any = true;
+          umma_commit(&empty[stage]);
+          if (++stage == kExpandStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (ok) umma_commit(&tfull[buf]);
+      }
+      if (!ok && any) {
+        umma_commit(&drain_bar);
+        drain_wait(&drain_bar, 0, p.err);
+      }
+    }
+    __syncwarp();
+  } else {
+    // rows 32 quad .. + 31, columns 128 half .. + 127 of every unit
+    const int ew = warp - 2, quad = warp & 3, half = ew >> 2;
+    const int pitch = (p.N + 15) & ~15;
+    float* stage_out = reinterpret_cast<float*>(out + ew * kDeltaStageBytes);
+    int at = -1, rows = 0;
+    float fac = 0.f;
+    float* to[8];  // a lane writes 16 bytes of rows 4 i + lane / 8
+    for (int u = u0; u < u1; ++u) {
+      if (u / blocks != at) {
+        at = u / blocks;
+        const ManyTile tile = tiles[at];
+        rows = tile.rows - quad * 32;
+        const int first = tile.first + quad * 32;
+        if (rows > 0) {
+          fac = p.factor[first + min(lane, rows - 1)];
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            to[i] = p.delta + static_cast<size_t>(p.perm[first + min(4 * i + (lane >> 3), rows - 1)]) * pitch + 4 * (lane & 7);
+        }
+      }
+      const int buf = (u - u0) & 1, n0 = u % blocks * 256 + half * 128;
+      if (!warp_wait(&tfull[buf], ((u - u0) >> 1) & 1, &abort_flag, p.err, kErrTimeoutAcc)) break;
+      tc_fence_after();
+      if (rows > 0) {
+#pragma unroll 1
+        for (int c = 0; c < 128 && n0 + c < p.N; c += 32) {
+          uint32_t v[32];
+          tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256 + half * 128 + c, v);
+          tmem_wait_ld();
+          float4* st = reinterpret_cast<float4*>(stage_out + lane * 36);
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            st[i] = make_float4(fac * __uint_as_float(v[4 * i]), fac * __uint_as_float(v[4 * i + 1]),
+                                fac * __uint_as_float(v[4 * i + 2]), fac * __uint_as_float(v[4 * i + 3]));
+          __syncwarp();
+          // 128 contiguous bytes a row, four rows an access
+          if (n0 + c + 4 * (lane & 7) < p.N) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int r = 4 * i + (lane >> 3);
+              if (r < rows)
+                *reinterpret_cast<float4*>(to[i] + n0 + c) =
+                    *reinterpret_cast<const float4*>(stage_out + r * 36 + 4 * (lane & 7));
+            }
+          }
+          __syncwarp();
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty[buf]);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
 // ============================================================================ CUDA cores
 // Float32 problems and shapes TMA cannot address.  One CTA a row for S; then 32 x 32 output tiles.
 constexpr int kSimtShrink = 128;
@@ -810,13 +1222,11 @@ __global__ void __launch_bounds__(256) rows_gemm_simt_kernel(const RowsArgs p) {
       if (n >= p.N) continue;
       float v = acc[i][j];
       if (e != kNoSlot) {
-        // feature n of its block of 16, rank r of its step of 16: place 8 (4 (n % 8) + r / 4) + 4 (n / 8) + r % 4
-        const int blocks = (p.N + 15) >> 4, f = n & 15;
         const T* b = static_cast<const T*>(p.b_bank) +
-                     (static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) * blocks + (n >> 4)) * 256 + (f & 7) * 32 + (f >> 3) * 4;
+                     (static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) * p.N + n) * 16;  // steps of 16 ranks
         float add = 0.f;
         for (int r = 0; r < rank_of(e); ++r)
-          add = fmaf(s[r], to_f32(b[static_cast<size_t>(r >> 4) * blocks * 256 + (r >> 2 & 3) * 8 + (r & 3)]), add);
+          add = fmaf(s[r], to_f32(b[static_cast<size_t>(r >> 4) * p.N * 16 + (r & 15)]), add);
         v += add;
       }
       static_cast<T*>(p.y)[static_cast<size_t>(t) * p.N + n] = from_f32<T>(v);
@@ -863,38 +1273,69 @@ cudaError_t launch_gemm(const RowsGemm& g, const CUtensorMap& w, const CUtensorM
   return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), ring_bytes(kTN) + 1024, st, true, w, x, g);
 }
 
-// The adapters' part of rows with `a`.  Up to 256 rows: one CTA an SM, beside the GEMM's; few rows are cut over a larger
-// cluster.  More rows: two CTAs an SM and no cluster (the GEMM that follows needs whole SMs).
+// The adapters' part of up to 256 rows: one CTA an SM, beside the GEMM's; few rows are cut over a larger cluster.
 template <typename T>
 cudaError_t lora_part(const RowsArgs& a, int num_sms, cudaStream_t st) {
   const int tiles = (a.T + kTileRows - 1) / kTileRows;
-  const bool many = tiles > 2;
-  int kparts = many ? 1 : tiles == 1 ? 8 : 4;
+  int kparts = tiles == 1 ? 8 : 4;
   while (kparts > 1 && (a.K + 31) / 32 < kparts * kShrinkWarps) kparts /= 2;
-  const int clusters = (many ? 2 : 1) * num_sms / kparts;
+  const int clusters = num_sms / kparts;
   int slices = clusters / tiles;
   slices = slices < 1 ? 1 : slices > kTileRows ? kTileRows : slices;
   if (slices > a.T) slices = a.T;
   const dim3 grid(static_cast<unsigned>((tiles * slices < clusters ? tiles * slices : clusters) * kparts));
-  cudaError_t e;
-#define LF_LORA(MT, NB)                                                                                       \
-  {                                                                                                           \
-    auto* k = many ? rows_lora_kernel<T, MT, NB> : rows_lora_kernel<T, MT, 1>;                                \
-    e = allow_smem(reinterpret_cast<const void*>(k), 0);                                                      \
-    if (e == cudaSuccess) e = launch_cluster(k, grid, kparts, dim3(kShrinkThreads), 0, st, false, a, slices, kparts); \
-  }
-  if (a.r_pad == 16) LF_LORA(1, 4)
-  else if (a.r_pad == 32) LF_LORA(2, 4)
-  else if (a.r_pad == 64) LF_LORA(4, 2)
-  else LF_LORA(8, 1)
-#undef LF_LORA
-  return e;
+  auto* k = a.r_pad == 16   ? rows_lora_kernel<T, 1>
+            : a.r_pad == 32 ? rows_lora_kernel<T, 2>
+            : a.r_pad == 64 ? rows_lora_kernel<T, 4>
+                            : rows_lora_kernel<T, 8>;
+  const cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), 0);
+  if (e != cudaSuccess) return e;
+  return launch_cluster(k, grid, kparts, dim3(kShrinkThreads), 0, st, false, a, slices, kparts);
+}
+
+// The adapters' part of many rows, in three launches.
+template <typename T>
+cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_sms, cudaStream_t st) {
+  cudaError_t e = allow_smem(reinterpret_cast<const void*>(many_plan_kernel), kPlanSmem);
+  if (e == cudaSuccess) e = launch(many_plan_kernel, 1, kPlanThreads, kPlanSmem, st, false, a);
+  if (e != cudaSuccess) return e;
+  const int64_t most = static_cast<int64_t>(a.T / kTileRows) + a.n_slots;  // a slot has one tile that is not full
+  const int tiles = static_cast<int>(most < a.T ? most : a.T);
+  ManyShrink s{};
+  s.a = a;
+  s.ab_fmt = dtype == LF_BF16 ? 1 : 0;
+  s.ksplit = 1;
+  const int nkb = (a.K + kBK - 1) / kBK;
+  while (s.ksplit < 8 && tiles * s.ksplit * 2 <= num_sms && nkb >= s.ksplit * 8) s.ksplit *= 2;
+  s.pitch = a.r_pad + 4;
+  // one limit for every rank: a kernel is opted into its shared memory once
+  constexpr int kRing = kShrinkStages * kShrinkStageBytes + 1024;
+  constexpr int kMost = kRing + kTileRows * (LF_BANK_MAX_RANK + 4) * 4;
+  constexpr int kExpandSmem = kExpandStages * kExpandStageBytes + kEpiWarps * kDeltaStageBytes + 1024;
+  static_assert(kMost <= 224 * 1024 && kExpandSmem <= 224 * 1024, "shared memory of an SM");
+  auto* k = many_shrink_kernel<T>;
+  int clusters = num_sms / s.ksplit;
+  if (clusters > tiles) clusters = tiles;
+  e = allow_smem(reinterpret_cast<const void*>(k), kMost);
+  if (e == cudaSuccess)
+    e = launch_cluster(k, dim3(static_cast<unsigned>(clusters * s.ksplit)), s.ksplit, dim3(kGemmThreads),
+                       kRing + kTileRows * s.pitch * 4, st, true, m.x, m.a, s);
+  if (e != cudaSuccess) return e;
+  ManyExpand x{};
+  x.a = a;
+  x.idesc = umma_idesc_f16(kTileRows, 256, s.ab_fmt, 0, 0);
+  const int64_t units = static_cast<int64_t>(tiles) * ((a.N + 255) / 256);
+  auto* kx = many_expand_kernel<T>;
+  e = allow_smem(reinterpret_cast<const void*>(kx), kExpandSmem);
+  if (e != cudaSuccess) return e;
+  return launch_cluster(kx, dim3(static_cast<unsigned>(units < num_sms ? units : num_sms)), 1, dim3(kGemmThreads),
+                        kExpandSmem, st, true, m.s_hi, m.s_lo, m.b, x);
 }
 
 template <typename T>
-cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, int tn, int ksplit,
-                    int num_sms, cudaStream_t st) {
-  const cudaError_t e = lora_part<T>(a, num_sms, st);
+cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const ManyMaps* m, int tn,
+                    int ksplit, int num_sms, cudaStream_t st) {
+  const cudaError_t e = m ? many_part<T>(a, dtype, *m, num_sms, st) : lora_part<T>(a, num_sms, st);
   if (e != cudaSuccess) return e;
   RowsGemm g{};
   g.a = a;
@@ -935,13 +1376,14 @@ RowsTiles rows_tiles(int T, int K, int N, int num_sms) {
 }
 
 cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
-                            int num_sms, cudaStream_t st) {
-  return dtype == LF_BF16 ? rows_tc<__nv_bfloat16>(a, dtype, w, x, t.rows, t.ksplit, num_sms, st)
-                          : rows_tc<__half>(a, dtype, w, x, t.rows, t.ksplit, num_sms, st);
+                            const ManyMaps* m, int num_sms, cudaStream_t st) {
+  return dtype == LF_BF16 ? rows_tc<__nv_bfloat16>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st)
+                          : rows_tc<__half>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st);
 }
 
-cudaError_t rows_lora_part(const RowsArgs& a, int dtype, int num_sms, cudaStream_t st) {
-  return dtype == LF_BF16 ? lora_part<__nv_bfloat16>(a, num_sms, st) : lora_part<__half>(a, num_sms, st);
+cudaError_t rows_many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_sms, cudaStream_t st) {
+  return dtype == LF_BF16 ? many_part<__nv_bfloat16>(a, dtype, m, num_sms, st)
+                          : many_part<__half>(a, dtype, m, num_sms, st);
 }
 
 // Rounds of full tiles times the time of one (measured at K = 4096: 23 us for a 256 x 256 tile of a CTA pair, 32 us for

@@ -24,6 +24,10 @@ __all__ = ["AdapterBank", "fused_lora_forward_rows"]
 _DTYPE_CODE = b200_ops._DTYPE_CODE
 
 
+def _launches(rows: int, tensor_cores: bool = True) -> int:
+    return 2 if rows <= 256 or not tensor_cores else nat.lib().lf_rows_launch_count(rows)
+
+
 class AdapterBank:
     """Resident low-rank adapters of one projection, in ``n_slots`` slots of rank up to ``max_rank``.
 
@@ -54,11 +58,8 @@ class AdapterBank:
         self.dtype, self.device = dtype, device
         self.r_pad = next(r for r in (16, 32, 64, nat.BANK_MAX_RANK) if max_rank <= r)
         self.lora_a = torch.zeros(n_slots, self.r_pad, in_features, dtype=dtype, device=device)
-        # B_i in blocks of 16 ranks x 16 features, each in the order of the matrix instruction's operand
-        # ([feature % 8, rank // 4, feature // 8, rank % 4]): a lane's part of a block is one 16-byte load, and
-        # what is read of an adapter is contiguous whatever its rank
-        self.lora_b = torch.zeros(n_slots, self.r_pad // 16, -(-out_features // 16), 8, 4, 2, 4, dtype=dtype,
-                                  device=device)
+        # B_i in steps of 16 ranks: what a kernel reads of an adapter is contiguous whatever its rank
+        self.lora_b = torch.zeros(n_slots, self.r_pad // 16, out_features, 16, dtype=dtype, device=device)
         self.ranks = torch.zeros(n_slots, dtype=torch.int32, device=device)
         self.scales = torch.zeros(n_slots, dtype=torch.float32, device=device)
 
@@ -78,9 +79,8 @@ class AdapterBank:
         self.lora_a[slot, :r] = lora_a
         if r < self.r_pad:  # the kernels read zeros past the rank
             self.lora_a[slot, r:] = 0
-        blocks = self.lora_b.shape[2]
-        lora_b = torch.nn.functional.pad(lora_b, (0, self.r_pad - r, 0, 16 * blocks - self.out_features))
-        self.lora_b[slot] = lora_b.view(blocks, 2, 8, self.r_pad // 16, 4, 4).permute(3, 0, 2, 4, 1, 5)
+            lora_b = torch.nn.functional.pad(lora_b, (0, self.r_pad - r))
+        self.lora_b[slot] = lora_b.view(self.out_features, -1, 16).transpose(0, 1)
         self.scales[slot] = float(scaling)
         self.ranks[slot] = r
 
@@ -101,7 +101,8 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor.
 
-    Two launches on the current stream of ``x``'s device.  bf16/f16 problems whose in_features or
+    Two launches on the current stream of ``x``'s device, long batches in chunks of
+    8192 rows of four launches each.  bf16/f16 problems whose in_features or
     out_features is not a multiple of 8, or whose buffers are not 16-byte aligned, run on CUDA cores
     with a ``CudaCorePathWarning``.
     """
@@ -109,7 +110,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
         x, base_weight, bank.lora_a, bank.lora_b, bank.ranks, bank.scales, row_slot, out, bank.r_pad,
         bank.out_features) if bank is not None else None
     if y is not None:
-        b200_ops._last_launches = 2
+        b200_ops._last_launches = _launches(x.shape[0], x.dtype is not torch.float32)
         return y
     # anything that needs a copy, a warning or an error
     if x.dim() != 2:
@@ -151,16 +152,18 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     p = nat.RowsProblem(_DTYPE_CODE[dtype], T, K, N, bank.n_slots, bank.r_pad, 4 if slot_dtype is torch.int32 else 8,
                         0, ldx, x.data_ptr(), base_weight.data_ptr(), bank.lora_a.data_ptr(), bank.lora_b.data_ptr(),
                         bank.ranks.data_ptr(), bank.scales.data_ptr(), row_slot.data_ptr())
-    if dtype is not torch.float32 and (K % 8 or N % 8 or ldx % 8 or
+    tensor_cores = dtype is not torch.float32
+    if tensor_cores and (K % 8 or N % 8 or ldx % 8 or
                                        (p.x_dev | p.w_dev | p.a_bank_dev | p.b_bank_dev | out.data_ptr()) % 16):
         if ldx % 8 or p.x_dev % 16:  # only x's rows: a dense copy of x is far cheaper than CUDA cores
             x = x.clone(memory_format=torch.contiguous_format)
             p.x_dev, p.ldx = x.data_ptr(), K
+        tensor_cores = not (K % 8 or N % 8 or (p.w_dev | p.a_bank_dev | p.b_bank_dev | out.data_ptr()) % 16)
         b200_ops._warn_if_cuda_core(dtype, K, N, (x, base_weight, bank.lora_a, bank.lora_b, out))
     L = nat.lib()
     ws = torch.empty(L.lf_rows_workspace_bytes(T, N, bank.r_pad, p.dtype), dtype=torch.uint8, device=device)
     with nat.on_device(device.index):
         rc = L.lf_rows_forward(p, out.data_ptr(), ws.data_ptr(), ws.numel(), nat.raw_stream(device.index))
     nat.check(rc, "lf_rows_forward")
-    b200_ops._last_launches = 2
+    b200_ops._last_launches = _launches(T, tensor_cores)
     return out

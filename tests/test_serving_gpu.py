@@ -100,7 +100,8 @@ def test_rows_against_64_bits(case):
     dtype, T, K, N, ranks, max_rank = case
     x, w, bank, adapters, slots = make(dtype, T, K, N, ranks, max_rank)
     y = fused_lora_forward_rows(x, w, bank, slots)
-    assert b200_ops.last_launch_count() == 2
+    few = T <= 256 or dtype is torch.float32 or K % 8 or N % 8
+    assert b200_ops.last_launch_count() == (2 if few else 4 * -(-T // 8192))
     check(y, x, w, adapters, slots)
     again = fused_lora_forward_rows(x, w, bank, slots.to(torch.int64))
     assert torch.equal(y, again)  # the same bits on every run, for either index type
@@ -281,8 +282,6 @@ def test_load_converts_and_clears_past_the_rank():
     a, b = torch.randn(5, 64, device="cuda"), torch.randn(72, 5, device="cuda")
     bank.load(0, a, b, 2.0)
     assert torch.equal(bank.lora_a[0, :5], a.to(BF16)) and not bank.lora_a[0, 5:].any()
-    # blocks of 16 features x 16 ranks as [feature % 8, rank // 4, feature // 8, rank % 4]
-    back = bank.lora_b[0].permute(1, 4, 2, 0, 3, 5).reshape(80, 16)
-    assert torch.equal(back[:72, :5], b.to(BF16)) and not back[72:].any() and not back[:, 5:].any()
+    assert torch.equal(bank.lora_b[0, 0, :, :5], b.to(BF16)) and not bank.lora_b[0, :, :, 5:].any()
     assert bank.ranks.tolist() == [5] and bank.scales.tolist() == [2.0]
     assert np.isclose(bank.lora_a.element_size(), 2)
