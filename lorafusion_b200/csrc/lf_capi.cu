@@ -941,8 +941,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
       const uint64_t s_pitch = static_cast<uint64_t>(a.r_pad) * 2;
       const void* a_bank = a.n_slots > 0 ? a.a_bank : a.w;  // an empty bank: a map that nothing uses
       const void* b_bank = a.n_slots > 0 ? a.b_bank : a.w;
-      if (!make_map(&many.x, p->dtype, a.x, a.K, a.T, x_pitch, 64, 1) ||
-          !make_map(&many.a, p->dtype, a_bank, a.K, bank_rows, w_pitch, 64, 16) ||
+      if (!make_map(&many.a, p->dtype, a_bank, a.K, bank_rows, w_pitch, 64, 16) ||
           !make_map(&many.s_hi, p->dtype, a.s_hi, a.r_pad, a.T, s_pitch, 16, 128) ||
           !make_map(&many.s_lo, p->dtype, a.s_lo, a.r_pad, a.T, s_pitch, 16, 128) ||
           !make_map(&many.b, p->dtype, b_bank, 16, bank_rows / 16 * a.N, 32, 16, 256))

@@ -200,7 +200,6 @@ struct RowsTiles {
 RowsTiles rows_tiles(int T, int K, int N, int num_sms);
 // What the adapters' part of many rows is read through.
 struct ManyMaps {
-  CUtensorMap x;           // [T, K] box (64, 1), 128-byte swizzle: rows are gathered
   CUtensorMap a;           // bank A [n_slots r_pad, K] box (64, 16), 128-byte swizzle
   CUtensorMap s_hi, s_lo;  // S [T, r_pad] box (16, 128), 32-byte swizzle
   CUtensorMap b;           // bank B [n_slots r_pad/16 N, 16] box (16, 256), 32-byte swizzle

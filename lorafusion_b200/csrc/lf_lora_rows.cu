@@ -696,12 +696,13 @@ struct ManyTile {
 // Sorts at most kRowsChunk rows: a hash table of adapters in shared memory counts them, a scan places them.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSlots = 2 * kRowsChunk;  // of the table: never more than half full
-constexpr int kPlanRows = kRowsChunk / kPlanThreads, kPlanPer = kPlanSlots / kPlanThreads;
+constexpr int kPlanRows = kRowsChunk / kPlanThreads;
 constexpr int kPlanSmem = kPlanSlots * 8;
-__global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsArgs p) {
+__global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsArgs p, int log2_slots) {
   extern __shared__ uint32_t plan_smem[];
   uint32_t* key = plan_smem;
-  uint32_t* count = plan_smem + kPlanSlots;  // then the first sorted row
+  const int slots = 1 << log2_slots;
+  uint32_t* count = plan_smem + slots;  // then the first sorted row
   __shared__ int warp_rows[32], warp_tiles[32];
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -720,10 +721,9 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
     e[i] = r <= 0 ? kNoSlot : static_cast<uint32_t>(r) << 24 | static_cast<uint32_t>(slot[i]);
     if (tid + i * kPlanThreads < p.T) p.eff[tid + i * kPlanThreads] = e[i];
   }
-#pragma unroll
-  for (int i = 0; i < kPlanPer; ++i) {
-    key[tid + i * kPlanThreads] = kNoSlot;
-    count[tid + i * kPlanThreads] = 0;
+  for (int h = tid; h < slots; h += kPlanThreads) {
+    key[h] = kNoSlot;
+    count[h] = 0;
   }
   __syncthreads();
   uint32_t at[kPlanRows], pos[kPlanRows];
@@ -733,12 +733,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
     const uint32_t same = __match_any_sync(0xffffffffu, e[i]);
     const int lead = __ffs(same) - 1;
     if (e[i] != kNoSlot && lane == lead) {
-      uint32_t h = (e[i] * 0x9e3779b1u) >> 18;
-      static_assert(kPlanSlots == 1 << 14, "the hash's bits");
+      uint32_t h = (e[i] * 0x9e3779b1u) >> (32 - log2_slots);
       for (;;) {
         const uint32_t was = atomicCAS(&key[h], kNoSlot, e[i]);
         if (was == kNoSlot || was == e[i]) break;
-        h = (h + 1) & (kPlanSlots - 1);
+        h = (h + 1) & (slots - 1);
       }
       at[i] = h;
       pos[i] = atomicAdd(&count[h], __popc(same));
@@ -748,9 +747,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
   }
   __syncthreads();
   int rows = 0, tiles = 0;
-#pragma unroll
-  for (int i = 0; i < kPlanPer; ++i) {
-    const int c = static_cast<int>(count[tid + i * kPlanThreads]);
+  for (int h = tid; h < slots; h += kPlanThreads) {
+    const int c = static_cast<int>(count[h]);
     rows += c;
     tiles += (c + kTileRows - 1) / kTileRows;
   }
@@ -765,9 +763,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
   row0 -= rows, tile0 -= tiles;
   for (int w = 0; w < warp; ++w) row0 += warp_rows[w], tile0 += warp_tiles[w];
   if (tid == kPlanThreads - 1) *p.n_tiles = tile0 + tiles;
-#pragma unroll
-  for (int i = 0; i < kPlanPer; ++i) {
-    const int h = tid + i * kPlanThreads, c = static_cast<int>(count[h]);
+  for (int h = tid; h < slots; h += kPlanThreads) {
+    const int c = static_cast<int>(count[h]);
     count[h] = row0;
     for (int r = 0; r < c; r += kTileRows)
       static_cast<ManyTile*>(p.tiles)[tile0++] = ManyTile{key[h], row0 + r, min(kTileRows, c - r), 0};
@@ -779,33 +776,43 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
     if (e[i] != kNoSlot) p.perm[count[at[i]] + pos[i]] = tid + i * kPlanThreads;
 }
 
-// S = x A_i^T of a tile, in sorted order.  K is cut over a cluster when there cannot be many tiles.
-constexpr int kShrinkStages = 4;
-constexpr int kShrinkStageBytes = kWBytes + LF_BANK_MAX_RANK * kBK * 2;  // 128 rows of x, up to 128 of A_i
+// S = x A_i^T of a tile, in sorted order.  K is cut over a cluster when there cannot be many tiles.  Eight warps gather x
+// with 16-byte copies, 8 lanes to the 128 bytes of a row and block of 64 elements, placed as the 128-byte swizzle
+// would (a TMA gather of four rows takes about 50 ns however many are in flight: 99 us for 8192 rows); TMA
+// loads A_i.
+constexpr int kXBytes = kTileRows * kBK * 2;
+constexpr int kShrinkMaxStages = 8;
 struct ManyShrink {
   RowsArgs a;
   int ksplit, pitch;  // floats from one row's S to the next in shared memory
+  int stages, sub;    // blocks of 64 elements a stage: a wait costs as much as a block's MMAs
   int ab_fmt;
 };
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 template <typename T>
 __global__ void __launch_bounds__(kGemmThreads, 1)
-    many_shrink_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_a,
-                       const __grid_constant__ ManyShrink prm) {
+    many_shrink_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ ManyShrink prm) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* s_part = reinterpret_cast<float*>(ring + kShrinkStages * kShrinkStageBytes);  // [128][pitch]
-  __shared__ uint64_t full[kShrinkStages], empty[kShrinkStages], acc_full, drain_bar;
+  __shared__ uint64_t full[kShrinkMaxStages], empty[kShrinkMaxStages], acc_full, drain_bar;
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const RowsArgs& p = prm.a;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int ks = prm.ksplit, part = blockIdx.x % ks;
+  const int ks = prm.ksplit, part = blockIdx.x % ks, stages = prm.stages, sub = prm.sub;
+  const int block_bytes = kXBytes + p.r_pad * kBK * 2, stage_bytes = sub * block_bytes;
+  float* s_part = reinterpret_cast<float*>(ring);  // [128][pitch], while the ring is idle
   const int nkb = (p.K + kBK - 1) / kBK;
   const int kb0 = static_cast<int>(static_cast<int64_t>(part) * nkb / ks);
   const int kb1 = static_cast<int>(static_cast<int64_t>(part + 1) * nkb / ks);
   if (tid == 0) {
-    for (int s = 0; s < kShrinkStages; ++s) {
-      mbar_init(&full[s], 1);
+    for (int s = 0; s < stages; ++s) {
+      mbar_init(&full[s], 1 + 32 * kEpiWarps);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_full, 1);
@@ -825,53 +832,53 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const uint32_t tmem = tmem_slot;
   const int n_tiles = *p.n_tiles;
   const uint64_t x0 = umma_sdesc(smem_u32(ring), 16, 1024, 2);
-  int stage = 0;  // of the loading warp, of the MMA thread
+  int stage = 0;  // of every loading warp and of the MMA thread
   uint32_t phase = 0, issued = 0, parity = 0, done = 0, drained = 0;
   for (int i = blockIdx.x / ks; i < n_tiles; i += gridDim.x / ks, done ^= 1) {
     const ManyTile tile = static_cast<const ManyTile*>(p.tiles)[i];
     const int slot = slot_of(tile.e), rank = rank_of(tile.e), steps = (rank + 15) >> 4;
-    bool ok = true;
     if (warp == 0) {
-      // a lane gathers four rows of x: 128 bytes of each a stage; rows past the last one repeat it
-      const int loads = (tile.rows + 3) >> 2;
-      int r[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) r[j] = p.perm[tile.first + min(4 * lane + j, tile.rows - 1)];
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (lane == 0) {
-          ok = mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
-          if (ok) mbar_arrive_expect_tx(&full[stage], loads * 512 + steps * 16 * kBK * 2);
-        }
-        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        uint8_t* d = ring + stage * kShrinkStageBytes;
-        if (lane < loads) tma_gather4(d + lane * 512, &map_x, &full[stage], kb * kBK, r[0], r[1], r[2], r[3]);
-        if (lane < steps)
-          tma_load_2d(d + kWBytes + lane * 16 * kBK * 2, &map_a, &full[stage], kb * kBK, slot * p.r_pad + 16 * lane);
-        issued |= 1u << stage;
-        parity = (parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == kShrinkStages) {
-          stage = 0;
-          phase ^= 1;
+      if (lane == 0) {
+        for (int kb = kb0; kb < kb1; kb += sub) {
+          if (!mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) break;
+          const int n = min(sub, kb1 - kb);
+          mbar_arrive_expect_tx(&full[stage], n * steps * 16 * kBK * 2);
+          uint8_t* d = ring + stage * stage_bytes + kXBytes;
+          for (int b = 0; b < n; ++b, d += block_bytes)
+            for (int k = 0; k < steps; ++k)
+              tma_load_2d(d + k * 16 * kBK * 2, &map_a, &full[stage], (kb + b) * kBK, slot * p.r_pad + 16 * k);
+          issued |= 1u << stage;
+          parity = (parity & ~(1u << stage)) | (phase << stage);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
         }
       }
+      __syncwarp();
     } else if (warp == 1) {
       if (lane == 0) {
         const uint32_t idesc = umma_idesc_f16(kTileRows, steps * 16, prm.ab_fmt, 0, 0);
         uint32_t acc = 0;
-        for (int kb = kb0; kb < kb1; ++kb) {
+        bool ok = true;
+        for (int kb = kb0; kb < kb1; kb += sub) {
           if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t x = x0 + ((stage * kShrinkStageBytes) >> 4), w = x + (kWBytes >> 4);
+          fence_proxy_async_smem();  // x came by ordinary copies
+          const int n = min(sub, kb1 - kb);
+          uint64_t x = x0 + ((stage * stage_bytes) >> 4);
+          for (int b = 0; b < n; ++b, x += block_bytes >> 4) {
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            umma_f16(tmem, x + 2 * k, w + 2 * k, idesc, acc);
-            acc = 1;
+            for (int k = 0; k < kBK / 16; ++k) {
+              umma_f16(tmem, x + 2 * k, x + (kXBytes >> 4) + 2 * k, idesc, acc);
+              acc = 1;
+            }
           }
           umma_commit(&empty[stage]);
-          if (++stage == kShrinkStages) {
+          if (++stage == stages) {
             stage = 0;
             phase ^= 1;
           }
@@ -884,21 +891,50 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
       __syncwarp();
-    } else if (warp_wait(&acc_full, done, &abort_flag, p.err, kErrTimeoutAcc)) {
-      // the two warps of a lane quarter take alternate steps
-      tc_fence_after();
-      const int quad = warp & 3, row = quad * 32 + lane;
-      if (quad * 32 < tile.rows) {
-        for (int k = (warp - 2) >> 2; k < steps; k += 2) {
-          uint32_t v[16];
-          tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + 16 * k, v);
-          tmem_wait_ld();
-          uint4* to = reinterpret_cast<uint4*>(s_part + row * prm.pitch + 16 * k);
+    } else {
+      // rows (tid - 64) / 8 + 32 j, 16 bytes of each
+      const int r0 = (tid - 64) >> 3, piece = tid & 7;
+      const T* from[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) to[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+      for (int j = 0; j < 4; ++j)
+        from[j] = static_cast<const T*>(p.x) + piece * 8 +
+                  static_cast<int64_t>(p.perm[tile.first + min(r0 + 32 * j, tile.rows - 1)]) * p.ldx;
+      const uint32_t to = smem_u32(ring) + static_cast<uint32_t>(r0 * 128 + ((piece ^ (r0 & 7)) << 4));
+      for (int kb = kb0; kb < kb1; kb += sub) {
+        bool ok = true;
+        if (lane == 0) ok = mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
+        if (!__shfl_sync(0xffffffffu, ok, 0)) break;
+        const int n = min(sub, kb1 - kb);
+        for (int b = 0; b < n; ++b) {
+          const int col = (kb + b) * kBK;
+          const uint32_t bytes = col + piece * 8 < p.K ? 16 : 0;  // zeros behind K
+          const uint32_t d = to + stage * stage_bytes + b * block_bytes;
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (r0 + 32 * j < tile.rows) cp_async16(d + j * 32 * 128, from[j] + (bytes ? col : 0), bytes);
+        }
+        cp_async_arrive(&full[stage]);  // once this thread's copies have landed
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      tc_fence_before();
+      // the two warps of a lane quarter take alternate steps
+      if (warp_wait(&acc_full, done, &abort_flag, p.err, kErrTimeoutAcc)) {
+        tc_fence_after();
+        const int quad = warp & 3, row = quad * 32 + lane;
+        if (quad * 32 < tile.rows) {
+          for (int k = (warp - 2) >> 2; k < steps; k += 2) {
+            uint32_t v[16];
+            tmem_ld16(tmem + (static_cast<uint32_t>(quad * 32) << 16) + 16 * k, v);
+            tmem_wait_ld();
+            uint4* to_s = reinterpret_cast<uint4*>(s_part + row * prm.pitch + 16 * k);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) to_s[j] = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+          }
+        }
+        tc_fence_before();
+      }
     }
     if (ks > 1) cluster_sync_all();
     else __syncthreads();
@@ -938,11 +974,13 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
     }
+    fence_proxy_async_smem();  // TMA writes here next
     if (ks > 1) cluster_sync_all();  // peers have read this CTA's sums
     else __syncthreads();
   }  // when a wait has run out the remaining tiles' waits end at once: the cluster's CTAs stay in step
+  asm volatile("cp.async.wait_all;" ::: "memory");
   if (warp == 0 && lane == 0 && abort_flag)  // let every copy that was started land before the memory is used again
-    for (int s = 0; s < kShrinkStages; ++s)
+    for (int s = 0; s < stages; ++s)
       if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
   __syncthreads();
   if (warp == 1) tmem_dealloc(tmem, LF_BANK_MAX_RANK);
@@ -1101,27 +1139,32 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
       tc_fence_after();
       if (rows > 0) {
 #pragma unroll 1
-        for (int c = 0; c < 128 && n0 + c < p.N; c += 32) {
-          uint32_t v[32];
-          tmem_ld32(tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256 + half * 128 + c, v);
+        for (int c0 = 0; c0 < 128 && n0 + c0 < p.N; c0 += 64) {
+          uint32_t v[2][32];
+          const uint32_t from = tmem + (static_cast<uint32_t>(quad * 32) << 16) + buf * 256 + half * 128 + c0;
+          tmem_ld32(from, v[0]);
+          tmem_ld32(from + 32, v[1]);
           tmem_wait_ld();
-          float4* st = reinterpret_cast<float4*>(stage_out + lane * 36);
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            st[i] = make_float4(fac * __uint_as_float(v[4 * i]), fac * __uint_as_float(v[4 * i + 1]),
-                                fac * __uint_as_float(v[4 * i + 2]), fac * __uint_as_float(v[4 * i + 3]));
-          __syncwarp();
-          // 128 contiguous bytes a row, four rows an access
-          if (n0 + c + 4 * (lane & 7) < p.N) {
+          for (int h = 0; h < 2; ++h) {
+            const int n = n0 + c0 + 32 * h;
+            float4* st = reinterpret_cast<float4*>(stage_out + lane * 36);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const int r = 4 * i + (lane >> 3);
-              if (r < rows)
-                *reinterpret_cast<float4*>(to[i] + n0 + c) =
-                    *reinterpret_cast<const float4*>(stage_out + r * 36 + 4 * (lane & 7));
+            for (int i = 0; i < 8; ++i)
+              st[i] = make_float4(fac * __uint_as_float(v[h][4 * i]), fac * __uint_as_float(v[h][4 * i + 1]),
+                                  fac * __uint_as_float(v[h][4 * i + 2]), fac * __uint_as_float(v[h][4 * i + 3]));
+            __syncwarp();
+            // 128 contiguous bytes a row, four rows an access
+            if (n + 4 * (lane & 7) < p.N) {
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const int r = 4 * i + (lane >> 3);
+                if (r < rows)
+                  *reinterpret_cast<float4*>(to[i] + n) = *reinterpret_cast<const float4*>(stage_out + r * 36 + 4 * (lane & 7));
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
       tc_fence_before();
@@ -1297,7 +1340,9 @@ cudaError_t lora_part(const RowsArgs& a, int num_sms, cudaStream_t st) {
 template <typename T>
 cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_sms, cudaStream_t st) {
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(many_plan_kernel), kPlanSmem);
-  if (e == cudaSuccess) e = launch(many_plan_kernel, 1, kPlanThreads, kPlanSmem, st, false, a);
+  int log2_slots = 10;  // of the sort's table: at most half full
+  while ((1 << log2_slots) < 2 * a.T) ++log2_slots;
+  if (e == cudaSuccess) e = launch(many_plan_kernel, 1, kPlanThreads, 8u << log2_slots, st, false, a, log2_slots);
   if (e != cudaSuccess) return e;
   const int64_t most = static_cast<int64_t>(a.T / kTileRows) + a.n_slots;  // a slot has one tile that is not full
   const int tiles = static_cast<int>(most < a.T ? most : a.T);
@@ -1308,18 +1353,21 @@ cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_s
   const int nkb = (a.K + kBK - 1) / kBK;
   while (s.ksplit < 8 && tiles * s.ksplit * 2 <= num_sms && nkb >= s.ksplit * 8) s.ksplit *= 2;
   s.pitch = a.r_pad + 4;
-  // one limit for every rank: a kernel is opted into its shared memory once
-  constexpr int kRing = kShrinkStages * kShrinkStageBytes + 1024;
-  constexpr int kMost = kRing + kTileRows * (LF_BANK_MAX_RANK + 4) * 4;
+  constexpr int kMost = 224 * 1024;  // one limit for every rank: a kernel is opted into its shared memory once
   constexpr int kExpandSmem = kExpandStages * kExpandStageBytes + kEpiWarps * kDeltaStageBytes + 1024;
-  static_assert(kMost <= 224 * 1024 && kExpandSmem <= 224 * 1024, "shared memory of an SM");
+  static_assert(kExpandSmem <= kMost, "shared memory of an SM");
+  static_assert(2 * 2 * (kXBytes + 16 * kBK * 2) >= kTileRows * (LF_BANK_MAX_RANK + 4) * 4, "the sums fit the ring");
+  const int block = kXBytes + a.r_pad * kBK * 2;
+  s.sub = 2;
+  s.stages = (kMost - 1024) / (s.sub * block);
+  if (s.stages > kShrinkMaxStages) s.stages = kShrinkMaxStages;
   auto* k = many_shrink_kernel<T>;
   int clusters = num_sms / s.ksplit;
   if (clusters > tiles) clusters = tiles;
   e = allow_smem(reinterpret_cast<const void*>(k), kMost);
   if (e == cudaSuccess)
     e = launch_cluster(k, dim3(static_cast<unsigned>(clusters * s.ksplit)), s.ksplit, dim3(kGemmThreads),
-                       kRing + kTileRows * s.pitch * 4, st, true, m.x, m.a, s);
+                       s.stages * s.sub * block + 1024, st, true, m.a, s);
   if (e != cudaSuccess) return e;
   ManyExpand x{};
   x.a = a;
