@@ -513,7 +513,7 @@ __global__ void __maxnreg__(80)
   __shared__ volatile int abort_flag;
   __shared__ uint8_t s_on[kTN];  // whether the row has an adapter
   const RowsArgs& p = prm.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   constexpr int w_bytes = kWBytes, block_bytes = w_bytes + kXBytes;
   // A stage holds `sub` blocks of 64 elements of K.  A block costs the loading thread two copies and the MMA
   // thread four MMAs, but each wait costs both about 0.1 us: with one block a stage, a tile of few rows took 0.35 us
@@ -549,15 +549,15 @@ __global__ void __maxnreg__(80)
   const uint32_t tmem = tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, issued = 0, parity = 0;
-      bool ok = true;
-      for (int kb = kb0; kb < kb1; kb += sub) {
-        if (!mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
-          ok = false;
-          break;
-        }
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, parity = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; kb += sub) {
+      if (!warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
+        ok = false;
+        break;
+      }
+      if (elect_one()) {
         uint8_t* w = ring + stage * stage_bytes;
         const int n = min(sub, kb1 - kb);
         mbar_arrive_expect_tx(&full[stage], n * block_bytes);
@@ -565,47 +565,48 @@ __global__ void __maxnreg__(80)
           tma_load_2d(w, &map_w, &full[stage], (kb + i) * kBK, n0);
           tma_load_2d(w + w_bytes, &map_x, &full[stage], (kb + i) * kBK, t0);
         }
-        issued |= 1u << stage;
-        parity = (parity & ~(1u << stage)) | (phase << stage);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
-      if (!ok)  // let every copy this thread started land before the memory is used again
-        for (int s = 0; s < stages; ++s)
-          if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
+      issued |= 1u << stage;
+      parity = (parity & ~(1u << stage)) | (phase << stage);
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1;
+      }
     }
+    if (!ok && lane == 0)  // let every copy that was started land before the memory is used again
+      for (int s = 0; s < stages; ++s)
+        if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0, acc = 0;
-      bool ok = true;
-      // descriptors of the first block; addresses are in 16-byte units in their low bits
-      const uint64_t w0 = umma_sdesc(smem_u32(ring), 16, 1024, 2);
-      for (int kb = kb0; kb < kb1; kb += sub) {
-        if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const int n = min(sub, kb1 - kb);
+    int stage = 0;
+    uint32_t phase = 0, acc = 0;
+    bool ok = true;
+    // descriptors of the first block; addresses are in 16-byte units in their low bits
+    const uint64_t w0 = umma_sdesc(smem_u32(ring), 16, 1024, 2);
+    for (int kb = kb0; kb < kb1; kb += sub) {
+      if (!warp_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int n = min(sub, kb1 - kb);
+      if (elect_one()) {
         uint64_t w = w0 + ((stage * stage_bytes) >> 4);
         for (int i = 0; i < n; ++i, w += block_bytes >> 4) {
           const uint64_t x = w + (w_bytes >> 4);
 #pragma unroll
-          for (int k = 0; k < kBK / 16; ++k) {
-            umma_f16(tmem, w + 2 * k, x + 2 * k, prm.idesc, acc);
-            acc = 1;
-          }
+          for (int k = 0; k < kBK / 16; ++k) umma_f16(tmem, w + 2 * k, x + 2 * k, prm.idesc, acc | i | k);
         }
         umma_commit(&empty[stage]);
-        if (++stage == stages) {
-          stage = 0;
-          phase ^= 1;
-        }
       }
+      __syncwarp();
+      acc = 1;
+      if (++stage == stages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
+    if (elect_one()) {
       if (ok) {
         umma_commit(&acc_bar);
       } else if (acc) {
@@ -782,10 +783,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
 // loads A_i.
 constexpr int kXBytes = kTileRows * kBK * 2;
 constexpr int kShrinkMaxStages = 8;
+constexpr int kLoadWarps = 4;
 struct ManyShrink {
   RowsArgs a;
   int ksplit, pitch;  // floats from one row's S to the next in shared memory
-  int stages, sub;    // blocks of 64 elements a stage: a wait costs as much as a block's MMAs
+  int stages;
   int ab_fmt;
 };
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -803,16 +805,17 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const RowsArgs& p = prm.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int ks = prm.ksplit, part = blockIdx.x % ks, stages = prm.stages, sub = prm.sub;
-  const int block_bytes = kXBytes + p.r_pad * kBK * 2, stage_bytes = sub * block_bytes;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int ks = prm.ksplit, part = blockIdx.x % ks, stages = prm.stages;
+  // two blocks of 64 elements a stage: a wait costs as much as a block's MMAs
+  const int block_bytes = kXBytes + p.r_pad * kBK * 2, stage_bytes = 2 * block_bytes;
   float* s_part = reinterpret_cast<float*>(ring);  // [128][pitch], while the ring is idle
   const int nkb = (p.K + kBK - 1) / kBK;
   const int kb0 = static_cast<int>(static_cast<int64_t>(part) * nkb / ks);
   const int kb1 = static_cast<int>(static_cast<int64_t>(part + 1) * nkb / ks);
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1 + 32 * kEpiWarps);
+      mbar_init(&full[s], 1 + 32 * kLoadWarps);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_full, 1);
@@ -838,80 +841,95 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     const ManyTile tile = static_cast<const ManyTile*>(p.tiles)[i];
     const int slot = slot_of(tile.e), rank = rank_of(tile.e), steps = (rank + 15) >> 4;
     if (warp == 0) {
-      if (lane == 0) {
-        for (int kb = kb0; kb < kb1; kb += sub) {
-          if (!mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) break;
-          const int n = min(sub, kb1 - kb);
+      for (int kb = kb0; kb < kb1; kb += 2) {
+        if (!warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) break;
+        if (elect_one()) {
+          const int n = min(2, kb1 - kb);
           mbar_arrive_expect_tx(&full[stage], n * steps * 16 * kBK * 2);
           uint8_t* d = ring + stage * stage_bytes + kXBytes;
           for (int b = 0; b < n; ++b, d += block_bytes)
             for (int k = 0; k < steps; ++k)
               tma_load_2d(d + k * 16 * kBK * 2, &map_a, &full[stage], (kb + b) * kBK, slot * p.r_pad + 16 * k);
-          issued |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-          }
+        }
+        issued |= 1u << stage;
+        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
       __syncwarp();
     } else if (warp == 1) {
-      if (lane == 0) {
-        const uint32_t idesc = umma_idesc_f16(kTileRows, steps * 16, prm.ab_fmt, 0, 0);
-        uint32_t acc = 0;
-        bool ok = true;
-        for (int kb = kb0; kb < kb1; kb += sub) {
-          if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          fence_proxy_async_smem();  // x came by ordinary copies
-          const int n = min(sub, kb1 - kb);
+      const uint32_t idesc = umma_idesc_f16(kTileRows, steps * 16, prm.ab_fmt, 0, 0);
+      uint32_t acc = 0;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; kb += 2) {
+        if (!warp_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        fence_proxy_async_smem();  // x came by ordinary copies
+        const int n = min(2, kb1 - kb);
+        if (elect_one()) {
           uint64_t x = x0 + ((stage * stage_bytes) >> 4);
           for (int b = 0; b < n; ++b, x += block_bytes >> 4) {
 #pragma unroll
-            for (int k = 0; k < kBK / 16; ++k) {
-              umma_f16(tmem, x + 2 * k, x + (kXBytes >> 4) + 2 * k, idesc, acc);
-              acc = 1;
-            }
+            for (int k = 0; k < kBK / 16; ++k) umma_f16(tmem, x + 2 * k, x + (kXBytes >> 4) + 2 * k, idesc, acc | b | k);
           }
           umma_commit(&empty[stage]);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-          }
         }
+        __syncwarp();
+        acc = 1;
+        if (++stage == stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (elect_one()) {
         if (ok) umma_commit(&acc_full);
         else if (acc) {
           umma_commit(&drain_bar);
           drain_wait(&drain_bar, drained, p.err);
-          drained ^= 1;
         }
       }
       __syncwarp();
+      if (!ok && acc) drained ^= 1;
     } else {
-      // rows (tid - 64) / 8 + 32 j, 16 bytes of each
+      // rows (tid - 64) / 8 + kStep j, 16 bytes of each; a row that is not there reads nothing and becomes zeros
+      constexpr int kStep = 4 * kLoadWarps, kPer = kTileRows / kStep;
       const int r0 = (tid - 64) >> 3, piece = tid & 7;
-      const T* from[4];
+      const T* from[kPer];
+      uint32_t bytes[kPer];
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        from[j] = static_cast<const T*>(p.x) + piece * 8 +
-                  static_cast<int64_t>(p.perm[tile.first + min(r0 + 32 * j, tile.rows - 1)]) * p.ldx;
+      for (int j = 0; j < kPer; ++j) {
+        const int row = r0 + kStep * j;
+        from[j] = static_cast<const T*>(p.x) + piece * 8 + kb0 * kBK +
+                  static_cast<int64_t>(p.perm[tile.first + min(row, tile.rows - 1)]) * p.ldx;
+        bytes[j] = row < tile.rows ? 16 : 0;
+      }
       const uint32_t to = smem_u32(ring) + static_cast<uint32_t>(r0 * 128 + ((piece ^ (r0 & 7)) << 4));
-      for (int kb = kb0; kb < kb1; kb += sub) {
+      for (int kb = warp < 2 + kLoadWarps ? kb0 : kb1; kb < kb1; kb += 2) {
         bool ok = true;
         if (lane == 0) ok = mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
         if (!__shfl_sync(0xffffffffu, ok, 0)) break;
-        const int n = min(sub, kb1 - kb);
-        for (int b = 0; b < n; ++b) {
-          const int col = (kb + b) * kBK;
-          const uint32_t bytes = col + piece * 8 < p.K ? 16 : 0;  // zeros behind K
-          const uint32_t d = to + stage * stage_bytes + b * block_bytes;
+        const uint32_t d = to + stage * stage_bytes;
+        if (kb + 2 <= kb1 && (kb + 2) * kBK <= p.K) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j)
-            if (r0 + 32 * j < tile.rows) cp_async16(d + j * 32 * 128, from[j] + (bytes ? col : 0), bytes);
+          for (int j = 0; j < kPer; ++j) {
+            cp_async16(d + j * kStep * 128, from[j], bytes[j]);
+            cp_async16(d + block_bytes + j * kStep * 128, from[j] + kBK, bytes[j]);
+            from[j] += 2 * kBK;
+          }
+        } else {
+          for (int b = 0; b < min(2, kb1 - kb); ++b) {
+            const bool in = (kb + b) * kBK + piece * 8 < p.K;  // zeros behind K
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+              cp_async16(d + b * block_bytes + j * kStep * 128, in ? from[j] : static_cast<const T*>(p.x), in ? bytes[j] : 0);
+              from[j] += kBK;
+            }
+          }
         }
         cp_async_arrive(&full[stage]);  // once this thread's copies have landed
         if (++stage == stages) {
@@ -1009,7 +1027,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   const RowsArgs& p = prm.a;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   if (tid == 0) {
     for (int s = 0; s < kExpandStages; ++s) {
       mbar_init(&full[s], 1);
@@ -1038,20 +1056,20 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
   const int64_t units = static_cast<int64_t>(*p.n_tiles) * blocks;
   const int u0 = static_cast<int>(units * blockIdx.x / gridDim.x), u1 = static_cast<int>(units * (blockIdx.x + 1) / gridDim.x);
   if (warp == 0) {
-    if (lane == 0) {
-      fence_proxy_async_global();  // S was written by plain stores
-      int stage = 0;
-      uint32_t phase = 0, issued = 0, parity = 0;
-      bool ok = true;
-      for (int u = u0; u < u1 && ok; ++u) {
-        const ManyTile tile = tiles[u / blocks];
-        const int n0 = u % blocks * 256, steps = (rank_of(tile.e) + 15) >> 4;
-        const int row_b = slot_of(tile.e) * (p.r_pad >> 4) * p.N + n0;
-        for (int k0 = 0; k0 < steps; k0 += kExpandChunk) {
-          if (!mbar_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
-            ok = false;
-            break;
-          }
+    fence_proxy_async_global();  // S was written by plain stores
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, parity = 0;
+    bool ok = true;
+    for (int u = u0; u < u1 && ok; ++u) {
+      const ManyTile tile = tiles[u / blocks];
+      const int n0 = u % blocks * 256, steps = (rank_of(tile.e) + 15) >> 4;
+      const int row_b = slot_of(tile.e) * (p.r_pad >> 4) * p.N + n0;
+      for (int k0 = 0; k0 < steps; k0 += kExpandChunk) {
+        if (!warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
+          ok = false;
+          break;
+        }
+        if (elect_one()) {
           const int ns = min(kExpandChunk, steps - k0);
           mbar_arrive_expect_tx(&full[stage], ns * kExpandStepBytes);
           uint8_t* d = ring + stage * kExpandStageBytes;
@@ -1060,57 +1078,58 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             tma_load_2d(d + kSStepBytes, &map_lo, &full[stage], 16 * k, tile.first);
             tma_load_2d(d + 2 * kSStepBytes, &map_b, &full[stage], 0, row_b + k * p.N);
           }
-          issued |= 1u << stage;
-          parity = (parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == kExpandStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+        }
+        issued |= 1u << stage;
+        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == kExpandStages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
-      if (!ok)
-        for (int s = 0; s < kExpandStages; ++s)
-          if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
     }
+    if (!ok && lane == 0)
+      for (int s = 0; s < kExpandStages; ++s)
+        if (issued & (1u << s)) drain_wait(&full[s], (parity >> s) & 1u, p.err);
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool any = false, ok = true;
-      const uint64_t s0 = umma_sdesc(smem_u32(ring), 16, 256, 6);
-      for (int u = u0; u < u1 && ok; ++u) {
-        const int steps = (rank_of(tiles[u / blocks].e) + 15) >> 4, buf = (u - u0) & 1;
-        if (!mbar_wait_stage(&tempty[buf], (((u - u0) >> 1) & 1) ^ 1, &abort_flag, p.err, kErrTimeoutAcc)) {
+    int stage = 0;
+    uint32_t phase = 0;
+    bool any = false, ok = true;
+    const uint64_t s0 = umma_sdesc(smem_u32(ring), 16, 256, 6);
+    for (int u = u0; u < u1 && ok; ++u) {
+      const int steps = (rank_of(tiles[u / blocks].e) + 15) >> 4, buf = (u - u0) & 1;
+      if (!warp_wait_stage(&tempty[buf], (((u - u0) >> 1) & 1) ^ 1, &abort_flag, p.err, kErrTimeoutAcc)) {
+        ok = false;
+        break;
+      }
+      const uint32_t d = tmem + buf * 256;
+      for (int k0 = 0; k0 < steps; k0 += kExpandChunk) {
+        if (!warp_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
           ok = false;
           break;
         }
-        const uint32_t d = tmem + buf * 256;
-        for (int k0 = 0; k0 < steps; k0 += kExpandChunk) {
-          if (!mbar_wait_stage(&full[stage], phase, &abort_flag, p.err, kErrTimeoutFull)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        tc_fence_after();
+        if (elect_one()) {
           uint64_t s = s0 + ((stage * kExpandStageBytes) >> 4);
           for (int k = k0; k < min(steps, k0 + kExpandChunk); ++k, s += kExpandStepBytes >> 4) {
             const uint64_t w = s + ((2 * kSStepBytes) >> 4);
             umma_f16(d, s, w, prm.idesc, k > 0);
             umma_f16(d, s + (kSStepBytes >> 4), w, prm.idesc, 1);
           }
-          any = true;
           umma_commit(&empty[stage]);
-          if (++stage == kExpandStages) {
-            stage = 0;
-            phase ^= 1;
-          }
+          if (k0 + kExpandChunk >= steps) umma_commit(&tfull[buf]);
         }
-        if (ok) umma_commit(&tfull[buf]);
+        __syncwarp();
+        any = true;
+        if (++stage == kExpandStages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
-      if (!ok && any) {
-        umma_commit(&drain_bar);
-        drain_wait(&drain_bar, 0, p.err);
-      }
+    }
+    if (!ok && any && elect_one()) {
+      umma_commit(&drain_bar);
+      drain_wait(&drain_bar, 0, p.err);
     }
     __syncwarp();
   } else {
@@ -1358,8 +1377,7 @@ cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_s
   static_assert(kExpandSmem <= kMost, "shared memory of an SM");
   static_assert(2 * 2 * (kXBytes + 16 * kBK * 2) >= kTileRows * (LF_BANK_MAX_RANK + 4) * 4, "the sums fit the ring");
   const int block = kXBytes + a.r_pad * kBK * 2;
-  s.sub = 2;
-  s.stages = (kMost - 1024) / (s.sub * block);
+  s.stages = (kMost - 1024) / (2 * block);
   if (s.stages > kShrinkMaxStages) s.stages = kShrinkMaxStages;
   auto* k = many_shrink_kernel<T>;
   int clusters = num_sms / s.ksplit;
@@ -1367,7 +1385,7 @@ cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_s
   e = allow_smem(reinterpret_cast<const void*>(k), kMost);
   if (e == cudaSuccess)
     e = launch_cluster(k, dim3(static_cast<unsigned>(clusters * s.ksplit)), s.ksplit, dim3(kGemmThreads),
-                       s.stages * s.sub * block + 1024, st, true, m.a, s);
+                       s.stages * 2 * block + 1024, st, true, m.a, s);
   if (e != cudaSuccess) return e;
   ManyExpand x{};
   x.a = a;

@@ -130,6 +130,24 @@ __device__ __forceinline__ void drain_wait(uint64_t* bar, uint32_t parity, int* 
   }
 }
 
+// The same from all lanes of a warp, for a loop that the whole warp runs.
+__device__ __forceinline__ bool warp_wait_stage(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
+                                                int err_code) {
+  return __all_sync(0xffffffffu, mbar_wait_stage(bar, parity, abort_flag, err, err_code));
+}
+// True in one lane of a converged warp, always the same one.  A loop that the whole warp runs keeps its counters and
+// descriptors in uniform registers, from which tensor-core and TMA instructions take them; in a loop
+// that only one lane runs, each of those instructions first moves its operands there.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t on;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(on));
+  return on != 0;
+}
+
 // Bounded wait done by lane 0 and broadcast, so the warp stays converged for tcgen05.ld.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err,
                                           int code) {
