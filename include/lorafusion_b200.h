@@ -495,13 +495,13 @@ LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32
  * slot at or above n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
  * bf16/f16 with K, N and ldx multiples of 8 and 16-byte aligned buffers run on the tensor cores, other
  * problems on CUDA cores.  Long batches run in chunks of 8192 rows, of 4
- * launches (2 up to 256 rows).  Enqueued on `stream`; never synchronizes.
+ * launches each (2 up to 256 rows, or 512 where r_pad is at most 32).  Enqueued on `stream`; never synchronizes.
  */
 LF_API int lf_rows_forward(const lf_rows_problem* prob, void* y_dev, void* workspace_dev, size_t workspace_bytes,
                            lf_stream_t stream);
 
 /* Launches of lf_rows_forward of T rows on the tensor cores (on CUDA cores there are 2). */
-LF_API int lf_rows_launch_count(int32_t T);
+LF_API int lf_rows_launch_count(int32_t T, int32_t r_pad);
 
 /* ------------------------------------------------------------------------------------------------
  * Training: gradient norms, clipping and AdamW of many adapters.  No counterpart in the reference

@@ -181,7 +181,7 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_rows_workspace_bytes.restype = ctypes.c_size_t
     L.lf_rows_forward.argtypes = [P(RowsProblem), _c_p, _c_p, ctypes.c_size_t, _c_p]
     L.lf_rows_forward.restype = ctypes.c_int
-    L.lf_rows_launch_count.argtypes = [_c_i32]
+    L.lf_rows_launch_count.argtypes = [_c_i32, _c_i32]
     L.lf_rows_launch_count.restype = ctypes.c_int
     L.lf_grad_clip_workspace_bytes.argtypes = [_c_p, _c_i32, _c_i32]
     L.lf_grad_clip_workspace_bytes.restype = ctypes.c_size_t

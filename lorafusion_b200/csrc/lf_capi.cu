@@ -866,9 +866,9 @@ extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, i
   return T < 0 || N < 0 || r_pad < 0 ? 0 : rows_space(T, N, r_pad, dtype).bytes;
 }
 
-extern "C" int lf_rows_launch_count(int32_t T) {
+extern "C" int lf_rows_launch_count(int32_t T, int32_t r_pad) {
   int n = 0;
-  for (int t0 = 0; t0 < T; t0 += kRowsChunk) n += T - t0 > kFewRows ? 4 : 2;
+  for (int t0 = 0; t0 < T; t0 += kRowsChunk) n += T - t0 > few_rows(r_pad) ? 4 : 2;
   return n;
 }
 
@@ -935,16 +935,17 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     a.y = y + static_cast<size_t>(t0) * p->N * 2;
     const uint64_t x_pitch = static_cast<uint64_t>(p->ldx) * 2, w_pitch = static_cast<uint64_t>(p->K) * 2;
     cudaError_t e;
-    ManyMaps many;
-    if (a.T > kFewRows) {
+    ManyMaps maps_of_many;
+    ManyMaps* many = a.T > few_rows(a.r_pad) ? &maps_of_many : nullptr;
+    if (many) {
       const uint64_t bank_rows = static_cast<uint64_t>(a.n_slots > 0 ? a.n_slots : 1) * a.r_pad;
       const uint64_t s_pitch = static_cast<uint64_t>(a.r_pad) * 2;
       const void* a_bank = a.n_slots > 0 ? a.a_bank : a.w;  // an empty bank: a map that nothing uses
       const void* b_bank = a.n_slots > 0 ? a.b_bank : a.w;
-      if (!make_map(&many.a, p->dtype, a_bank, a.K, bank_rows, w_pitch, 64, 16) ||
-          !make_map(&many.s_hi, p->dtype, a.s_hi, a.r_pad, a.T, s_pitch, 16, 128) ||
-          !make_map(&many.s_lo, p->dtype, a.s_lo, a.r_pad, a.T, s_pitch, 16, 128) ||
-          !make_map(&many.b, p->dtype, b_bank, 16, bank_rows / 16 * a.N, 32, 16, 256))
+      if (!make_map(&many->a, p->dtype, a_bank, a.K, bank_rows, w_pitch, 64, 16) ||
+          !make_map(&many->s_hi, p->dtype, a.s_hi, a.r_pad, a.T, s_pitch, 16, 128) ||
+          !make_map(&many->s_lo, p->dtype, a.s_lo, a.r_pad, a.T, s_pitch, 16, 128) ||
+          !make_map(&many->b, p->dtype, b_bank, 16, bank_rows / 16 * a.N, 32, 16, 256))
         return LF_ERR_UNSUPPORTED;
     }
     if (rows_use_pairs(a.T, a.K, a.N, ds->num_sms)) {
@@ -958,7 +959,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
       tb.r_pad = 16;
       tb.err = ds->status;
       const PairDelta delta{a.delta, a.eff, (a.N + 15) / 16 * 16};
-      e = rows_many_part(a, p->dtype, many, ds->num_sms, st);
+      e = rows_lora_part(a, p->dtype, many, ds->num_sms, st);
       if (e == cudaSuccess)
         e = tc_gemm_pair(p->dtype, false, maps, a.T, a.N, a.K, false, tb, a.y, a.N, ds->num_sms, st, nullptr, nullptr,
                          &delta);
@@ -968,7 +969,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
       if (!make_map(&w_map, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128) ||
           !make_map(&x_map, p->dtype, a.x, a.K, a.T, x_pitch, 64, tiles.rows))
         return LF_ERR_UNSUPPORTED;
-      e = rows_forward_tc(a, p->dtype, w_map, x_map, tiles, a.T > kFewRows ? &many : nullptr, ds->num_sms, st);
+      e = rows_forward_tc(a, p->dtype, w_map, x_map, tiles, many, ds->num_sms, st);
     }
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }

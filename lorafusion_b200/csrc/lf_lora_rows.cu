@@ -698,13 +698,14 @@ struct ManyTile {
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSlots = 2 * kRowsChunk;  // of the table: never more than half full
 constexpr int kPlanRows = kRowsChunk / kPlanThreads;
-constexpr int kPlanSmem = kPlanSlots * 8;
+constexpr int kPlanSmem = kPlanSlots * 8 + kRowsChunk * 2;
 __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsArgs p, int log2_slots) {
   extern __shared__ uint32_t plan_smem[];
   uint32_t* key = plan_smem;
   const int slots = 1 << log2_slots;
   uint32_t* count = plan_smem + slots;  // then the first sorted row
-  __shared__ int warp_rows[32], warp_tiles[32];
+  uint16_t* list = reinterpret_cast<uint16_t*>(count + slots);  // the table's slots in use
+  __shared__ int warp_rows[32], warp_tiles[32], n_list;
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   uint32_t e[kPlanRows];  // loads of one kind together: two latencies, not sixteen
@@ -726,6 +727,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
     key[h] = kNoSlot;
     count[h] = 0;
   }
+  if (tid == 0) n_list = 0;
   __syncthreads();
   uint32_t at[kPlanRows], pos[kPlanRows];
 #pragma unroll
@@ -737,6 +739,7 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
       uint32_t h = (e[i] * 0x9e3779b1u) >> (32 - log2_slots);
       for (;;) {
         const uint32_t was = atomicCAS(&key[h], kNoSlot, e[i]);
+        if (was == kNoSlot) list[atomicAdd(&n_list, 1)] = static_cast<uint16_t>(h);
         if (was == kNoSlot || was == e[i]) break;
         h = (h + 1) & (slots - 1);
       }
@@ -747,31 +750,30 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
     pos[i] = __shfl_sync(0xffffffffu, pos[i], lead) + __popc(same & ((1u << lane) - 1));
   }
   __syncthreads();
-  int rows = 0, tiles = 0;
-  for (int h = tid; h < slots; h += kPlanThreads) {
-    const int c = static_cast<int>(count[h]);
-    rows += c;
-    tiles += (c + kTileRows - 1) / kTileRows;
-  }
-  int row0 = rows, tile0 = tiles;
+  const int n = n_list;
+  int row_base = 0, tile_base = 0;
+  for (int i0 = 0; i0 < n; i0 += kPlanThreads) {
+    const int h = i0 + tid < n ? list[i0 + tid] : 0, rows = i0 + tid < n ? static_cast<int>(count[h]) : 0;
+    const int tiles = (rows + kTileRows - 1) / kTileRows;
+    int row0 = rows, tile0 = tiles;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int r = __shfl_up_sync(0xffffffffu, row0, o), t = __shfl_up_sync(0xffffffffu, tile0, o);
-    if (lane >= o) row0 += r, tile0 += t;
+    for (int o = 1; o < 32; o <<= 1) {
+      const int r = __shfl_up_sync(0xffffffffu, row0, o), t = __shfl_up_sync(0xffffffffu, tile0, o);
+      if (lane >= o) row0 += r, tile0 += t;
+    }
+    if (lane == 31) warp_rows[warp] = row0, warp_tiles[warp] = tile0;
+    __syncthreads();
+    row0 += row_base - rows, tile0 += tile_base - tiles;
+    for (int w = 0; w < kPlanThreads / 32; ++w) {
+      if (w < warp) row0 += warp_rows[w], tile0 += warp_tiles[w];
+      row_base += warp_rows[w], tile_base += warp_tiles[w];
+    }
+    if (rows > 0) count[h] = row0;
+    for (int r = 0; r < rows; r += kTileRows)
+      static_cast<ManyTile*>(p.tiles)[tile0++] = ManyTile{key[h], row0 + r, min(kTileRows, rows - r), 0};
+    __syncthreads();
   }
-  if (lane == 31) warp_rows[warp] = row0, warp_tiles[warp] = tile0;
-  __syncthreads();
-  row0 -= rows, tile0 -= tiles;
-  for (int w = 0; w < warp; ++w) row0 += warp_rows[w], tile0 += warp_tiles[w];
-  if (tid == kPlanThreads - 1) *p.n_tiles = tile0 + tiles;
-  for (int h = tid; h < slots; h += kPlanThreads) {
-    const int c = static_cast<int>(count[h]);
-    count[h] = row0;
-    for (int r = 0; r < c; r += kTileRows)
-      static_cast<ManyTile*>(p.tiles)[tile0++] = ManyTile{key[h], row0 + r, min(kTileRows, c - r), 0};
-    row0 += c;
-  }
-  __syncthreads();
+  if (tid == 0) *p.n_tiles = tile_base;
 #pragma unroll
   for (int i = 0; i < kPlanRows; ++i)
     if (e[i] != kNoSlot) p.perm[count[at[i]] + pos[i]] = tid + i * kPlanThreads;
@@ -938,7 +940,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
       // the two warps of a lane quarter take alternate steps
-      if (warp_wait(&acc_full, done, &abort_flag, p.err, kErrTimeoutAcc)) {
+      if (warp_wait_stage(&acc_full, done, &abort_flag, p.err, kErrTimeoutAcc)) {
         tc_fence_after();
         const int quad = warp & 3, row = quad * 32 + lane;
         if (quad * 32 < tile.rows) {
@@ -957,38 +959,48 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     if (ks > 1) cluster_sync_all();
     else __syncthreads();
     tc_fence_after();
-    // this CTA's rows of the tile: sum over the cluster in a fixed order, scale, split
-    const float scale = p.slot_scale[slot];
-    for (int row = part + ks * warp; row < tile.rows; row += ks * (kGemmThreads / 32)) {
+    // this CTA's rows of the tile: sum over the cluster in a fixed order, scale, split; 2 ks lanes a row, 8 values a time
+    const int row = part + ks * (tid / (2 * ks)), sub = tid & (2 * ks - 1);
+    if (tid < kEpiWarps * 32) {
       const size_t to = static_cast<size_t>(tile.first + row);
-      float v[LF_BANK_MAX_RANK / 32];
+      float v[LF_BANK_MAX_RANK / 16][8];
       float top = 0.f;
 #pragma unroll
-      for (int k = 0; k < LF_BANK_MAX_RANK / 32; ++k) {
-        const int j = lane + 32 * k;
-        v[k] = 0.f;
-        if (j < rank) {
-          const float* at = s_part + row * prm.pitch + j;
-          if (ks == 1) v[k] = *at;
-          else
-            for (int c = 0; c < ks; ++c) v[k] += ld_cluster_f32(map_to_cta(smem_u32(at), c));
-        }
-        top = fmaxf(top, fabsf(v[k]));
-        if (!(fabsf(v[k]) <= 3.402823466e38f)) top = __int_as_float(0x7f800000);
-      }
+      for (int c = 0; c < LF_BANK_MAX_RANK / 16; ++c) {
+        const int j0 = 8 * (sub + 2 * ks * c);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        for (int j = 0; j < 8; ++j) v[c][j] = 0.f;
+        if (j0 < rank && row < tile.rows) {
+          const uint32_t at = smem_u32(s_part + row * prm.pitch + j0);
+          for (int peer = 0; peer < ks; ++peer) {
+            const uint32_t from = ks == 1 ? at : map_to_cta(at, peer);
+            const float4 lo = ld_cluster_f32x4(from), hi = ld_cluster_f32x4(from + 16);
+            v[c][0] += lo.x, v[c][1] += lo.y, v[c][2] += lo.z, v[c][3] += lo.w;
+            v[c][4] += hi.x, v[c][5] += hi.y, v[c][6] += hi.z, v[c][7] += hi.w;
+          }
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            if (j0 + j >= rank) v[c][j] = 0.f;  // columns past the rank: zero times x, which may not be finite
+            top = fmaxf(top, fabsf(v[c][j]));
+            if (!(fabsf(v[c][j]) <= 3.402823466e38f)) top = __int_as_float(0x7f800000);
+          }
+        }
+      }
+      for (int o = 1; o < 2 * ks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       const int ex = row_exponent(top);
       const float down = scalbnf(1.f, -ex);
-      if (lane == 0) p.factor[to] = scale * scalbnf(1.f, ex);
+      if (row < tile.rows) {
+        if (sub == 0) p.factor[to] = p.slot_scale[slot] * scalbnf(1.f, ex);
 #pragma unroll
-      for (int k = 0; k < LF_BANK_MAX_RANK / 32; ++k) {
-        const int j = lane + 32 * k;
-        if (j < steps * 16) {
-          T hi, lo;
-          halves<T>(v[k] * down, hi, lo);
-          static_cast<T*>(p.s_hi)[to * p.r_pad + j] = hi;
-          static_cast<T*>(p.s_lo)[to * p.r_pad + j] = lo;
+        for (int c = 0; c < LF_BANK_MAX_RANK / 16; ++c) {
+          const int j0 = 8 * (sub + 2 * ks * c);
+          if (j0 < steps * 16) {
+            __align__(16) T hi[8], lo[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) halves<T>(v[c][j] * down, hi[j], lo[j]);
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.s_hi) + to * p.r_pad + j0) = *reinterpret_cast<const uint4*>(hi);
+            *reinterpret_cast<uint4*>(static_cast<T*>(p.s_lo) + to * p.r_pad + j0) = *reinterpret_cast<const uint4*>(lo);
+          }
         }
       }
     }
@@ -1096,9 +1108,9 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     uint32_t phase = 0;
     bool any = false, ok = true;
     const uint64_t s0 = umma_sdesc(smem_u32(ring), 16, 256, 6);
-    for (int u = u0; u < u1 && ok; ++u) {
-      const int steps = (rank_of(tiles[u / blocks].e) + 15) >> 4, buf = (u - u0) & 1;
-      if (!warp_wait_stage(&tempty[buf], (((u - u0) >> 1) & 1) ^ 1, &abort_flag, p.err, kErrTimeoutAcc)) {
+    for (int u = u0, i = 0; u < u1 && ok; ++u, ++i) {
+      const int steps = (rank_of(tiles[u / blocks].e) + 15) >> 4, buf = i & 1;
+      if (!warp_wait_stage(&tempty[buf], ((i >> 1) & 1) ^ 1, &abort_flag, p.err, kErrTimeoutAcc)) {
         ok = false;
         break;
       }
@@ -1140,7 +1152,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
     int at = -1, rows = 0;
     float fac = 0.f;
     float* to[8];  // a lane writes 16 bytes of rows 4 i + lane / 8
-    for (int u = u0; u < u1; ++u) {
+    for (int u = u0, i = 0; u < u1; ++u, ++i) {
       if (u / blocks != at) {
         at = u / blocks;
         const ManyTile tile = tiles[at];
@@ -1149,12 +1161,12 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         if (rows > 0) {
           fac = p.factor[first + min(lane, rows - 1)];
 #pragma unroll
-          for (int i = 0; i < 8; ++i)
-            to[i] = p.delta + static_cast<size_t>(p.perm[first + min(4 * i + (lane >> 3), rows - 1)]) * pitch + 4 * (lane & 7);
+          for (int j = 0; j < 8; ++j)
+            to[j] = p.delta + static_cast<size_t>(p.perm[first + min(4 * j + (lane >> 3), rows - 1)]) * pitch + 4 * (lane & 7);
         }
       }
-      const int buf = (u - u0) & 1, n0 = u % blocks * 256 + half * 128;
-      if (!warp_wait(&tfull[buf], ((u - u0) >> 1) & 1, &abort_flag, p.err, kErrTimeoutAcc)) break;
+      const int buf = i & 1, n0 = u % blocks * 256 + half * 128;
+      if (!warp_wait_stage(&tfull[buf], (i >> 1) & 1, &abort_flag, p.err, kErrTimeoutAcc)) break;
       tc_fence_after();
       if (rows > 0) {
 #pragma unroll 1
@@ -1176,10 +1188,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
             // 128 contiguous bytes a row, four rows an access
             if (n + 4 * (lane & 7) < p.N) {
 #pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const int r = 4 * i + (lane >> 3);
+              for (int j = 0; j < 8; ++j) {
+                if (4 * j >= rows) break;
+                const int r = 4 * j + (lane >> 3);
                 if (r < rows)
-                  *reinterpret_cast<float4*>(to[i] + n) = *reinterpret_cast<const float4*>(stage_out + r * 36 + 4 * (lane & 7));
+                  *reinterpret_cast<float4*>(to[j] + n) = *reinterpret_cast<const float4*>(stage_out + r * 36 + 4 * (lane & 7));
               }
             }
             __syncwarp();
@@ -1361,7 +1374,7 @@ cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_s
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(many_plan_kernel), kPlanSmem);
   int log2_slots = 10;  // of the sort's table: at most half full
   while ((1 << log2_slots) < 2 * a.T) ++log2_slots;
-  if (e == cudaSuccess) e = launch(many_plan_kernel, 1, kPlanThreads, 8u << log2_slots, st, false, a, log2_slots);
+  if (e == cudaSuccess) e = launch(many_plan_kernel, 1, kPlanThreads, (8u << log2_slots) + a.T * 2, st, false, a, log2_slots);
   if (e != cudaSuccess) return e;
   const int64_t most = static_cast<int64_t>(a.T / kTileRows) + a.n_slots;  // a slot has one tile that is not full
   const int tiles = static_cast<int>(most < a.T ? most : a.T);
@@ -1399,9 +1412,14 @@ cudaError_t many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_s
 }
 
 template <typename T>
+cudaError_t adapters_part(const RowsArgs& a, int dtype, const ManyMaps* m, int num_sms, cudaStream_t st) {
+  return m ? many_part<T>(a, dtype, *m, num_sms, st) : lora_part<T>(a, num_sms, st);
+}
+
+template <typename T>
 cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const ManyMaps* m, int tn,
                     int ksplit, int num_sms, cudaStream_t st) {
-  const cudaError_t e = m ? many_part<T>(a, dtype, *m, num_sms, st) : lora_part<T>(a, num_sms, st);
+  const cudaError_t e = adapters_part<T>(a, dtype, m, num_sms, st);
   if (e != cudaSuccess) return e;
   RowsGemm g{};
   g.a = a;
@@ -1447,9 +1465,9 @@ cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, 
                           : rows_tc<__half>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st);
 }
 
-cudaError_t rows_many_part(const RowsArgs& a, int dtype, const ManyMaps& m, int num_sms, cudaStream_t st) {
-  return dtype == LF_BF16 ? many_part<__nv_bfloat16>(a, dtype, m, num_sms, st)
-                          : many_part<__half>(a, dtype, m, num_sms, st);
+cudaError_t rows_lora_part(const RowsArgs& a, int dtype, const ManyMaps* m, int num_sms, cudaStream_t st) {
+  return dtype == LF_BF16 ? adapters_part<__nv_bfloat16>(a, dtype, m, num_sms, st)
+                          : adapters_part<__half>(a, dtype, m, num_sms, st);
 }
 
 // Rounds of full tiles times the time of one (measured at K = 4096: 23 us for a 256 x 256 tile of a CTA pair, 32 us for

@@ -24,8 +24,8 @@ __all__ = ["AdapterBank", "fused_lora_forward_rows"]
 _DTYPE_CODE = b200_ops._DTYPE_CODE
 
 
-def _launches(rows: int, tensor_cores: bool = True) -> int:
-    return 2 if rows <= 256 or not tensor_cores else nat.lib().lf_rows_launch_count(rows)
+def _launches(rows: int, r_pad: int, tensor_cores: bool) -> int:
+    return 2 if rows <= 256 or not tensor_cores else nat.lib().lf_rows_launch_count(rows, r_pad)
 
 
 class AdapterBank:
@@ -101,8 +101,8 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor.
 
-    Two launches on the current stream of ``x``'s device, long batches in chunks of
-    8192 rows of four launches each.  bf16/f16 problems whose in_features or
+    Two launches on the current stream of ``x``'s device, long batches (above 256 rows,
+    or 512 where the bank's padded rank is at most 32) in chunks of 8192 rows of four launches each.  bf16/f16 problems whose in_features or
     out_features is not a multiple of 8, or whose buffers are not 16-byte aligned, run on CUDA cores
     with a ``CudaCorePathWarning``.
     """
@@ -110,7 +110,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
         x, base_weight, bank.lora_a, bank.lora_b, bank.ranks, bank.scales, row_slot, out, bank.r_pad,
         bank.out_features) if bank is not None else None
     if y is not None:
-        b200_ops._last_launches = _launches(x.shape[0], x.dtype is not torch.float32)
+        b200_ops._last_launches = _launches(x.shape[0], bank.r_pad, x.dtype is not torch.float32)
         return y
     # anything that needs a copy, a warning or an error
     if x.dim() != 2:
@@ -165,5 +165,5 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     with nat.on_device(device.index):
         rc = L.lf_rows_forward(p, out.data_ptr(), ws.data_ptr(), ws.numel(), nat.raw_stream(device.index))
     nat.check(rc, "lf_rows_forward")
-    b200_ops._last_launches = _launches(T, tensor_cores)
+    b200_ops._last_launches = _launches(T, bank.r_pad, tensor_cores)
     return out
