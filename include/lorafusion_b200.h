@@ -480,7 +480,7 @@ typedef struct lf_rows_problem {
   const void* x_dev;         /* [T] rows of K */
   const void* w_dev;         /* [N,K] */
   const void* a_bank_dev;    /* [n_slots, r_pad, K] */
-  const void* b_bank_dev;    /* [n_slots, r_pad/16, N, 16]: B_i in steps of 16 ranks */
+  const void* b_bank_dev;    /* [n_slots, r_pad/16, N, 16]: B_i in steps of 16 ranks, 16-byte aligned */
   const int32_t* slot_rank_dev;  /* [n_slots] */
   const float* slot_scale_dev;   /* [n_slots] s_i */
   const void* row_slot_dev;  /* [T] slot of each row; negative: no adapter */

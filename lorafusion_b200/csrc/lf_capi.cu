@@ -886,7 +886,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   if (p->n_slots > 0 && (!p->a_bank_dev || !p->b_bank_dev || !p->slot_rank_dev || !p->slot_scale_dev))
     return LF_ERR_INVALID_ARG;
   if (!workspace_dev || workspace_bytes < lf_rows_workspace_bytes(p->T, p->N, p->r_pad, p->dtype)) return LF_ERR_CAPACITY;
-  if (!aligned16(workspace_dev)) return LF_ERR_INVALID_ARG;
+  if (!aligned16(workspace_dev) || !aligned16(p->b_bank_dev)) return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
   RowsArgs a{};
@@ -918,8 +918,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   a.delta = reinterpret_cast<float*>(ws + space.delta);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = p->dtype != LF_F32 && p->K > 0 && p->K % 8 == 0 && p->N % 8 == 0 && p->ldx % 8 == 0 &&
-                  aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) &&
-                  aligned16(p->b_bank_dev) && aligned16(y_dev);
+                  aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) && aligned16(y_dev);
   if (!tc) {
     if ((p->T + 31) / 32 > 65535) return LF_ERR_UNSUPPORTED;
     return to_status(rows_forward_simt(a, p->dtype, st));

@@ -1230,6 +1230,7 @@ __global__ void __launch_bounds__(kSimtShrink) rows_shrink_simt_kernel(const Row
   const float scale = p.slot_scale[slot_of(e)];
   for (int j0 = 0; j0 < rank; j0 += 8) {
     float acc[8] = {};
+#pragma unroll 4
     for (int k = tid; k < K; k += kSimtShrink) {
       const float xv = to_f32(x[k]);
 #pragma unroll
@@ -1243,14 +1244,20 @@ __global__ void __launch_bounds__(kSimtShrink) rows_shrink_simt_kernel(const Row
       if ((tid & 31) == 0) part[tid >> 5][j] = acc[j];
     }
     __syncthreads();
-    if (tid < 8 && j0 + tid < rank) {
+    if (tid < 8) {  // zeros behind the rank: the second product reads whole groups of four
       float v = part[0][tid];
 #pragma unroll
       for (int w = 1; w < kSimtShrink / 32; ++w) v += part[w][tid];
-      s[j0 + tid] = scale * v;
+      s[j0 + tid] = j0 + tid < rank ? scale * v : 0.f;
     }
     __syncthreads();
   }
+}
+
+__device__ __forceinline__ float4 load4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <typename T>
+__device__ __forceinline__ float4 load4(const T* p) {  // 16-bit values at an address of any alignment they allow
+  return make_float4(to_f32(p[0]), to_f32(p[1]), to_f32(p[2]), to_f32(p[3]));
 }
 
 constexpr int kST = 32, kSK = 32;  // tile edge, K elements a step
@@ -1284,29 +1291,41 @@ __global__ void __launch_bounds__(256) rows_gemm_simt_kernel(const RowsArgs p) {
       for (int j = 0; j < 2; ++j) acc[i][j] += sum[i][j];
     __syncthreads();
   }
-  pdl_wait();
+  // The adapters' part of both rows and both features together, four ranks a load; which adapters they are does not
+  // depend on the first launch.
+  const T* b[2][2];
+  int rank[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    const int t = t0 + tr + i;
-    if (t >= p.T) continue;
-    const uint32_t e = p.eff[t];
-    const float* s = static_cast<const float*>(p.s_hi) + static_cast<size_t>(t) * p.r_pad;
+    const uint32_t e = t0 + tr + i < p.T ? row_adapter(p, t0 + tr + i, false) : kNoSlot;
+    rank[i] = e == kNoSlot ? 0 : rank_of(e);
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int n = n0 + tc + j;
-      if (n >= p.N) continue;
-      float v = acc[i][j];
-      if (e != kNoSlot) {
-        const T* b = static_cast<const T*>(p.b_bank) +
-                     (static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) * p.N + n) * 16;  // steps of 16 ranks
-        float add = 0.f;
-        for (int r = 0; r < rank_of(e); ++r)
-          add = fmaf(s[r], to_f32(b[static_cast<size_t>(r >> 4) * p.N * 16 + (r & 15)]), add);
-        v += add;
+    for (int j = 0; j < 2; ++j)
+      b[i][j] = static_cast<const T*>(p.b_bank) +
+                (rank[i] ? (static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) * p.N + min(n0 + tc + j, p.N - 1)) * 16 : 0);
+  }
+  pdl_wait();
+  float add[2][2] = {};
+#pragma unroll 2
+  for (int r = 0; r < max(rank[0], rank[1]); r += 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      if (r >= rank[i]) continue;
+      const float4 sv = *reinterpret_cast<const float4*>(static_cast<const float*>(p.s_hi) +
+                                                         static_cast<size_t>(t0 + tr + i) * p.r_pad + r);
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 bv = load4(b[i][j] + static_cast<size_t>(r >> 4) * p.N * 16 + (r & 15));
+        add[i][j] = fmaf(sv.x, bv.x, fmaf(sv.y, bv.y, fmaf(sv.z, bv.z, fmaf(sv.w, bv.w, add[i][j]))));
       }
-      static_cast<T*>(p.y)[static_cast<size_t>(t) * p.N + n] = from_f32<T>(v);
     }
   }
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      if (t0 + tr + i < p.T && n0 + tc + j < p.N)
+        static_cast<T*>(p.y)[static_cast<size_t>(t0 + tr + i) * p.N + n0 + tc + j] = from_f32<T>(acc[i][j] + add[i][j]);
 }
 
 // Opts a kernel into its dynamic shared memory once per device, and into the SM's largest shared-memory
