@@ -236,22 +236,86 @@ PyObject* gather_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromLong(dtype);
 }
 
-// changed(weights, addresses): advances the version counter of every weight whose gradient address is not 0.
-PyObject* changed(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 2 || !PyList_CheckExact(a[0])) {
-    PyErr_SetString(PyExc_TypeError, "changed takes a list of weights and a buffer");
+struct Buffer {  // a contiguous buffer for the length of a call
+  Py_buffer b{};
+  bool ok;
+  explicit Buffer(PyObject* o) : ok(PyObject_GetBuffer(o, &b, PyBUF_SIMPLE) == 0) {}
+  ~Buffer() {
+    if (ok) PyBuffer_Release(&b);
+  }
+};
+
+// adamw_step(weights, addresses, records, device records, chunks, hyper, steps, exp_avg, exp_avg_sq, master or None,
+// n_chunks, n_groups, workspace bytes, (beta1, beta2), eps, max_norm or None, skip_nonfinite, dtype codes of the
+// weights and the gradients): lf_adamw_step, and the version counter of every weight that has a gradient.
+// Returns the norms, or None when neither clipping nor skip_nonfinite asks for them.
+PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 19 || !PyList_CheckExact(a[0]) || !PyTuple_CheckExact(a[13]) || PyTuple_GET_SIZE(a[13]) != 2) {
+    PyErr_SetString(PyExc_TypeError, "adamw_step takes a list of weights and 18 more arguments");
     return nullptr;
   }
-  Py_buffer b;
-  if (PyObject_GetBuffer(a[1], &b, PyBUF_SIMPLE) < 0) return nullptr;
-  const Py_ssize_t count = PyList_GET_SIZE(a[0]);
-  const uint64_t* ptrs = static_cast<const uint64_t*>(b.buf);
-  for (Py_ssize_t i = 0; i < count && (i + 1) * 8 <= b.len; ++i) {
-    PyObject* o = PyList_GET_ITEM(a[0], i);
-    if (ptrs[i] && THPVariable_Check(o)) bump(THPVariable_Unpack(o));
+  const at::Tensor* t[7];
+  for (int i = 0; i < 7; ++i) {
+    t[i] = a[3 + i] == Py_None && i == 6 ? nullptr : cuda_tensor(a[3 + i]);
+    if (!t[i] && !(i == 6 && a[9] == Py_None)) {
+      PyErr_SetString(PyExc_TypeError, "the optimizer's state must be CUDA tensors");
+      return nullptr;
+    }
   }
-  PyBuffer_Release(&b);
-  Py_RETURN_NONE;
+  const Buffer grads(a[1]), records(a[2]);
+  if (!grads.ok || !records.ok) return nullptr;
+  const Py_ssize_t count = PyList_GET_SIZE(a[0]);
+  if (grads.b.len != count * 8 || records.b.len != count * static_cast<Py_ssize_t>(sizeof(lf_adamw_tensor))) {
+    PyErr_SetString(PyExc_ValueError, "one address and one record a weight");
+    return nullptr;
+  }
+  lf_adamw_args p{};
+  p.tensors = static_cast<const lf_adamw_tensor*>(records.b.buf);
+  p.tensors_dev = static_cast<const lf_adamw_tensor*>(t[0]->const_data_ptr());
+  p.chunk_tensor_dev = static_cast<const int32_t*>(t[1]->const_data_ptr());
+  p.grads = static_cast<const uint64_t*>(grads.b.buf);
+  p.hyper_dev = static_cast<const double*>(t[2]->const_data_ptr());
+  p.steps_dev = static_cast<int32_t*>(t[3]->data_ptr());
+  p.exp_avg_dev = static_cast<float*>(t[4]->data_ptr());
+  p.exp_avg_sq_dev = static_cast<float*>(t[5]->data_ptr());
+  p.master_dev = t[6] ? static_cast<float*>(t[6]->data_ptr()) : nullptr;
+  p.n_chunks = PyLong_AsLongLong(a[10]);
+  p.n_groups = static_cast<int32_t>(PyLong_AsLong(a[11]));
+  p.workspace_bytes = PyLong_AsSize_t(a[12]);
+  p.beta1 = PyFloat_AsDouble(PyTuple_GET_ITEM(a[13], 0));
+  p.beta2 = PyFloat_AsDouble(PyTuple_GET_ITEM(a[13], 1));
+  p.eps = PyFloat_AsDouble(a[14]);
+  p.max_norm = a[15] == Py_None ? -1.0 : PyFloat_AsDouble(a[15]);
+  p.skip_nonfinite = PyObject_IsTrue(a[16]);
+  p.param_dtype = static_cast<int32_t>(PyLong_AsLong(a[17]));
+  p.grad_dtype = static_cast<int32_t>(PyLong_AsLong(a[18]));
+  p.n_tensors = static_cast<int32_t>(count);
+  if (PyErr_Occurred()) return nullptr;
+  const auto dev = t[3]->device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+    PyErr_SetString(PyExc_RuntimeError,
+                    "AdapterAdamW.step cannot be captured into a CUDA graph: replays would change weights whose packed "
+                    "copies b200_ops keeps");
+    return nullptr;
+  }
+  at::Tensor norms;
+  if (p.max_norm >= 0.0 || p.skip_nonfinite) {
+    norms = at::detail::empty_cuda({p.n_groups}, at::kFloat, dev, std::nullopt);
+    p.norms_dev = static_cast<float*>(norms.data_ptr());
+  }
+  at::Tensor ws = at::detail::empty_cuda({static_cast<int64_t>(p.workspace_bytes)}, at::kByte, dev, std::nullopt);
+  p.workspace_dev = ws.data_ptr();
+  const int rc = lf_adamw_step(&p, stream);
+  if (rc != LF_OK) return fail(rc, "lf_adamw_step");
+  for (Py_ssize_t i = 0; i < count; ++i) {
+    PyObject* o = PyList_GET_ITEM(a[0], i);
+    if (p.grads[i] && THPVariable_Check(o)) bump(THPVariable_Unpack(o));
+  }
+  if (!norms.defined()) Py_RETURN_NONE;
+  return THPVariable_Wrap(std::move(norms));
 }
 
 // C++ exceptions (an allocation that fails, a CUDA error in the allocator) as Python ones.
@@ -277,7 +341,7 @@ PyMethodDef methods[] = {
     {"rows_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<rows_forward>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},
     {"gather_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<gather_step>)), METH_FASTCALL, nullptr},
-    {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<changed>)), METH_FASTCALL, nullptr},
+    {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<adamw_step>)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "lf_pyglue", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -279,9 +279,15 @@ class AdapterAdamW:
             code = self._gather(grads, ptrs)
         if code < 0:
             return self._no_gradients()
-        norms = self._launch(ptrs, code)
-        nat.glue().changed(self._tensors, ptrs)
-        return norms
+        if self._hyper_changed:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdapterAdamW.step cannot be captured into a CUDA graph")
+            self._hyper_dev.copy_(torch.from_numpy(self._hyper))
+            self._hyper_changed = False
+        return nat.glue().adamw_step(
+            self._tensors, ptrs, self._rec, self._rec_dev, self._chunk_dev, self._hyper_dev, self.steps, self.exp_avg,
+            self.exp_avg_sq, self.master, self._n_chunks, len(self.ids), self._ws_bytes, self.betas, self.eps,
+            self.max_norm, self.skip_nonfinite, _CODE[self.dtype], code)
 
     def _gather(self, grads, ptrs: np.ndarray) -> int:
         """``gather_step`` with every check on its own, for its error; dicts may be other mappings here."""
@@ -316,27 +322,3 @@ class AdapterAdamW:
         if self.max_norm is None and not self.skip_nonfinite:
             return None
         return torch.zeros(len(self.ids), dtype=torch.float32, device=self.device)
-
-    def _launch(self, ptrs: np.ndarray, grad_code: int) -> torch.Tensor | None:
-        with nat.on_device(self.device.index):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdapterAdamW.step cannot be captured into a CUDA graph: replays would change "
-                                   "weights whose packed copies b200_ops keeps")
-            if self._hyper_changed:
-                self._hyper_dev.copy_(torch.from_numpy(self._hyper))
-                self._hyper_changed = False
-            n_groups = len(self.ids)
-            L = nat.lib()
-            want = self.max_norm is not None or self.skip_nonfinite
-            norms = torch.empty(n_groups, dtype=torch.float32, device=self.device) if want else None
-            ws = torch.empty(self._ws_bytes, dtype=torch.uint8, device=self.device)
-            args = nat.AdamWArgs(
-                self._rec.ctypes.data, self._rec_dev.data_ptr(), self._chunk_dev.data_ptr(), ptrs.ctypes.data,
-                self._hyper_dev.data_ptr(), self.steps.data_ptr(), self.exp_avg.data_ptr(),
-                self.exp_avg_sq.data_ptr(), None if self.master is None else self.master.data_ptr(),
-                None if norms is None else norms.data_ptr(), ws.data_ptr(), ws.numel(), self._n_chunks, *self.betas,
-                self.eps, -1.0 if self.max_norm is None else float(self.max_norm), len(ptrs), n_groups,
-                _CODE[self.dtype], grad_code, int(self.skip_nonfinite), 0)
-            nat.check(L.lf_adamw_step(ctypes.byref(args), nat.raw_stream(self.device.index)),
-                      "lf_adamw_step")
-        return norms

@@ -69,14 +69,17 @@ def _rows(**kw):
 def test_rows_entry_refuses_before_any_launch():
     L = nat.lib()
     ws = L.lf_rows_workspace_bytes(4, 16, 16, nat.LF_BF16)
-    assert ws == 2 * 256 + 2 * 256 + 256 and L.lf_rows_workspace_bytes(4, 16, 16, nat.LF_F32) == 4 * 256
+    assert ws == 8 * 256 and L.lf_rows_workspace_bytes(4, 16, 16, nat.LF_F32) == 3 * 256
+    assert [L.lf_rows_launch_count(T, 64) for T in (0, 1, 256, 257, 8192, 8193, 16384)] == [0, 2, 2, 4, 4, 6, 8]
+    assert [L.lf_rows_launch_count(T, 32) for T in (257, 512, 513)] == [2, 2, 4]
     call = lambda p, y=256, w=256, n=ws: L.lf_rows_forward(p, y, w, n, None)  # noqa: E731
     for kw in (dict(dtype=3), dict(dtype=-1), dict(T=-1), dict(K=-1), dict(N=-1), dict(n_slots=-1), dict(r_pad=8),
                dict(r_pad=256), dict(row_slot_bytes=2), dict(ldx=15), dict(x_dev=None), dict(w_dev=None),
                dict(row_slot_dev=None), dict(a_bank_dev=None), dict(b_bank_dev=None), dict(slot_rank_dev=None),
-               dict(slot_scale_dev=None)):
+               dict(slot_scale_dev=None), dict(b_bank_dev=264)):
         assert call(_rows(**kw)) == nat.LF_ERR_INVALID_ARG, kw
     assert call(_rows(n_slots=1 << 24)) == nat.LF_ERR_UNSUPPORTED
+    assert call(_rows(n_slots=(1 << 24) - 1, N=136), n=1 << 40) == nat.LF_ERR_UNSUPPORTED  # more than 31 bits of bank rows
     assert call(_rows(), y=None) == nat.LF_ERR_INVALID_ARG
     assert call(_rows(), w=264) == nat.LF_ERR_INVALID_ARG
     assert call(_rows(), w=None) == nat.LF_ERR_CAPACITY and call(_rows(), n=ws - 1) == nat.LF_ERR_CAPACITY
