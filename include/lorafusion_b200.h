@@ -486,6 +486,23 @@ typedef struct lf_rows_problem {
   const void* row_slot_dev;  /* [T] slot of each row; negative: no adapter */
 } lf_rows_problem;
 
+/* An adapter and the places of its slot in a bank. */
+typedef struct lf_bank_adapter {
+  int32_t dtype;             /* lf_dtype of the adapter and the bank */
+  int32_t K, N, r_pad, rank; /* 0 < rank <= r_pad */
+  float scale;               /* s_i */
+  int64_t lda, ldb;          /* elements between rows */
+  const void* a_dev;         /* A_i: rank rows of K */
+  const void* b_dev;         /* B_i: N rows of rank */
+  void* slot_a_dev;          /* [r_pad, K] */
+  void* slot_b_dev;          /* [r_pad/16, N, 16] */
+  int32_t* slot_rank_dev;
+  float* slot_scale_dev;
+} lf_bank_adapter;
+
+/* Copies an adapter into its slot in one launch, zeros past its rank; `stream` orders it with the forwards. */
+LF_API int lf_bank_load(const lf_bank_adapter* adapter, lf_stream_t stream);
+
 /* Workspace bytes of lf_rows_forward (256-byte aligned buffer). */
 LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype);
 

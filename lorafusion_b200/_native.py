@@ -83,6 +83,13 @@ class RowsProblem(ctypes.Structure):
                 ("slot_rank_dev", _c_p), ("slot_scale_dev", _c_p), ("row_slot_dev", _c_p)]
 
 
+class BankAdapter(ctypes.Structure):
+    _fields_ = [("dtype", _c_i32), ("K", _c_i32), ("N", _c_i32), ("r_pad", _c_i32), ("rank", _c_i32),
+                ("scale", ctypes.c_float), ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64), ("a_dev", _c_p),
+                ("b_dev", _c_p), ("slot_a_dev", _c_p), ("slot_b_dev", _c_p), ("slot_rank_dev", _c_p),
+                ("slot_scale_dev", _c_p)]
+
+
 class AdamWArgs(ctypes.Structure):
     _fields_ = [("tensors", _c_p), ("tensors_dev", _c_p), ("chunk_tensor_dev", _c_p), ("grads", _c_p),
                 ("hyper_dev", _c_p), ("steps_dev", _c_p), ("exp_avg_dev", _c_p), ("exp_avg_sq_dev", _c_p),
@@ -181,6 +188,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_rows_workspace_bytes.restype = ctypes.c_size_t
     L.lf_rows_forward.argtypes = [P(RowsProblem), _c_p, _c_p, ctypes.c_size_t, _c_p]
     L.lf_rows_forward.restype = ctypes.c_int
+    L.lf_bank_load.argtypes = [P(BankAdapter), _c_p]
+    L.lf_bank_load.restype = ctypes.c_int
     L.lf_rows_launch_count.argtypes = [_c_i32, _c_i32]
     L.lf_rows_launch_count.restype = ctypes.c_int
     L.lf_grad_clip_workspace_bytes.argtypes = [_c_p, _c_i32, _c_i32]

@@ -866,6 +866,20 @@ extern "C" size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, i
   return T < 0 || N < 0 || r_pad < 0 ? 0 : rows_space(T, N, r_pad, dtype).bytes;
 }
 
+extern "C" int lf_bank_load(const lf_bank_adapter* p, lf_stream_t stream) {
+  if (!p || (p->dtype != LF_F32 && p->dtype != LF_BF16 && p->dtype != LF_F16)) return LF_ERR_INVALID_ARG;
+  if (p->r_pad != 16 && p->r_pad != 32 && p->r_pad != 64 && p->r_pad != LF_BANK_MAX_RANK) return LF_ERR_INVALID_ARG;
+  if (p->K <= 0 || p->N <= 0 || p->rank <= 0 || p->rank > p->r_pad) return LF_ERR_INVALID_ARG;
+  if ((p->rank > 1 && p->lda < p->K) || (p->N > 1 && p->ldb < p->rank)) return LF_ERR_INVALID_ARG;
+  if (!p->a_dev || !p->b_dev || !p->slot_a_dev || !p->slot_b_dev || !p->slot_rank_dev || !p->slot_scale_dev)
+    return LF_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
+  const BankLoad b{p->a_dev, p->b_dev,  p->slot_a_dev, p->slot_b_dev, p->slot_rank_dev, p->slot_scale_dev, p->lda,
+                   p->ldb,   p->K,      p->N,          p->r_pad,      p->rank,          p->scale};
+  return to_status(bank_load(b, p->dtype, ds->num_sms, static_cast<cudaStream_t>(stream)));
+}
+
 extern "C" int lf_rows_launch_count(int32_t T, int32_t r_pad) {
   int n = 0;
   for (int t0 = 0; t0 < T; t0 += kRowsChunk) n += T - t0 > few_rows(r_pad) ? 4 : 2;

@@ -215,6 +215,16 @@ cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, 
 // The adapters' part alone (a.delta, a.eff), for a GEMM that adds it: tc_gemm_pair's `delta`.
 cudaError_t rows_lora_part(const RowsArgs& a, int dtype, const ManyMaps* m, int num_sms, cudaStream_t st);
 bool rows_use_pairs(int T, int K, int N, int num_sms);
+struct BankLoad {
+  const void *a, *b;  // [rank][lda], [N][ldb]
+  void *a_out, *b_out;
+  int32_t* rank_out;
+  float* scale_out;
+  int64_t lda, ldb;
+  int K, N, r_pad, rank;
+  float scale;
+};
+cudaError_t bank_load(const BankLoad& p, int dtype, int num_sms, cudaStream_t st);
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
 
 // --------------------------------------------------------------- packing

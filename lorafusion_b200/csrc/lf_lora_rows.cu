@@ -1328,6 +1328,28 @@ __global__ void __launch_bounds__(256) rows_gemm_simt_kernel(const RowsArgs p) {
         static_cast<T*>(p.y)[static_cast<size_t>(t0 + tr + i) * p.N + n0 + tc + j] = from_f32<T>(acc[i][j] + add[i][j]);
 }
 
+// One adapter into its slot: A_i as it is, B_i in steps of 16 ranks, zeros past the rank.  One launch of a few
+// microseconds whatever the rank (the same with tensor operations was seven, 43 us of host time).
+template <typename T>
+__global__ void __launch_bounds__(256) bank_load_kernel(const BankLoad p) {
+  const T zero = from_f32<T>(0.f);
+  const int64_t in_a = static_cast<int64_t>(p.r_pad) * p.K, all = in_a + static_cast<int64_t>(p.r_pad) * p.N;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < all; i += gridDim.x * 256ll) {
+    if (i < in_a) {
+      const int64_t r = i / p.K;
+      static_cast<T*>(p.a_out)[i] = r < p.rank ? static_cast<const T*>(p.a)[r * p.lda + (i - r * p.K)] : zero;
+    } else {
+      const int64_t o = i - in_a, q = o >> 4, step = q / p.N;
+      const int r = static_cast<int>(step) * 16 + static_cast<int>(o & 15);
+      static_cast<T*>(p.b_out)[o] = r < p.rank ? static_cast<const T*>(p.b)[(q - step * p.N) * p.ldb + r] : zero;
+    }
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    *p.rank_out = p.rank;
+    *p.scale_out = p.scale;
+  }
+}
+
 // Opts a kernel into its dynamic shared memory once per device, and into the SM's largest shared-memory
 // split (a kernel with a smaller one would keep the dependent GEMM's CTAs off its SMs).
 cudaError_t allow_smem(const void* kernel, int bytes) {
@@ -1499,6 +1521,13 @@ bool rows_use_pairs(int T, int K, int N, int num_sms) {
   const double pair = 23.0 * ((pair_tiles + num_sms / 2 - 1) / (num_sms / 2)) * K / 4096;
   const double one = 32.0 * ((tiles * ks + num_sms - 1) / num_sms) * K / 4096 / ks + 5.0;
   return pair < one;
+}
+
+cudaError_t bank_load(const BankLoad& p, int dtype, int num_sms, cudaStream_t st) {
+  const int64_t blocks = (static_cast<int64_t>(p.r_pad) * (static_cast<int64_t>(p.K) + p.N) + 255) / 256;
+  const unsigned grid = static_cast<unsigned>(blocks < 16 * num_sms ? blocks : 16 * num_sms);
+  auto* k = dtype == LF_F32 ? bank_load_kernel<float> : dtype == LF_BF16 ? bank_load_kernel<__nv_bfloat16> : bank_load_kernel<__half>;
+  return launch(k, grid, 256, 0, st, false, p);
 }
 
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st) {

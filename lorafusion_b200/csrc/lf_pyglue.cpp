@@ -108,6 +108,47 @@ PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(y));
 }
 
+// bank_load(bank_a, bank_b, ranks, scales, slot, lora_a, lora_b, scaling): an adapter into its slot.  None unless its
+// tensors have the bank's dtype and device and dense rows; shapes were checked by the caller.
+PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 8) {
+    PyErr_SetString(PyExc_TypeError, "bank_load takes 8 arguments");
+    return nullptr;
+  }
+  const at::Tensor* t[6];
+  for (int i = 0; i < 6; ++i)
+    if (!(t[i] = cuda_tensor(a[i < 4 ? i : i + 1]))) Py_RETURN_NONE;
+  const at::Tensor &ba = *t[0], &bb = *t[1], &la = *t[4], &lb = *t[5];
+  const int64_t slot = PyLong_AsLongLong(a[4]);
+  lf_bank_adapter p{};
+  p.scale = static_cast<float>(PyFloat_AsDouble(a[7]));
+  if (PyErr_Occurred()) return nullptr;
+  p.dtype = dtype_code(ba.scalar_type());
+  if (p.dtype < 0 || la.scalar_type() != ba.scalar_type() || lb.scalar_type() != ba.scalar_type() ||
+      la.device() != ba.device() || lb.device() != ba.device() || la.dim() != 2 || lb.dim() != 2 ||
+      (la.size(1) > 1 && la.stride(1) != 1) || (lb.size(1) > 1 && lb.stride(1) != 1) || la.size(0) > ba.size(1) || la.size(1) != ba.size(2) || lb.size(0) != bb.size(2) ||
+      lb.size(1) != la.size(0) || slot < 0 || slot >= ba.size(0))
+    Py_RETURN_NONE;
+  p.K = static_cast<int32_t>(ba.size(2));
+  p.N = static_cast<int32_t>(bb.size(2));
+  p.r_pad = static_cast<int32_t>(ba.size(1));
+  p.rank = static_cast<int32_t>(la.size(0));
+  p.lda = la.stride(0);
+  p.ldb = lb.stride(0);
+  if ((p.rank > 1 && p.lda < p.K) || (p.N > 1 && p.ldb < p.rank)) Py_RETURN_NONE;  // rows that overlap
+  const size_t es = ba.element_size();
+  p.a_dev = la.const_data_ptr();
+  p.b_dev = lb.const_data_ptr();
+  p.slot_a_dev = static_cast<char*>(ba.data_ptr()) + static_cast<size_t>(slot) * p.r_pad * p.K * es;
+  p.slot_b_dev = static_cast<char*>(bb.data_ptr()) + static_cast<size_t>(slot) * p.r_pad * p.N * es;
+  p.slot_rank_dev = static_cast<int32_t*>(t[2]->data_ptr()) + slot;
+  p.slot_scale_dev = static_cast<float*>(t[3]->data_ptr()) + slot;
+  const c10::cuda::OptionalCUDAGuard guard(ba.device());
+  const int rc = lf_bank_load(&p, c10::cuda::getCurrentCUDAStream(ba.device().index()).stream());
+  if (rc != LF_OK) return fail(rc, "lf_bank_load");
+  Py_RETURN_TRUE;
+}
+
 void bump(const at::Tensor& t) {
   if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
@@ -339,6 +380,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"rows_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<rows_forward>)), METH_FASTCALL, nullptr},
+    {"bank_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<bank_load>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},
     {"gather_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<gather_step>)), METH_FASTCALL, nullptr},
     {"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<adamw_step>)), METH_FASTCALL, nullptr},

@@ -76,13 +76,13 @@ class AdapterBank:
                              f"in_features={self.in_features}, out_features={self.out_features}")
         if not 0 < r <= self.max_rank:
             raise ValueError(f"slot {slot}: rank {r} is outside 1 .. {self.max_rank}")
-        self.lora_a[slot, :r] = lora_a
-        if r < self.r_pad:  # the kernels read zeros past the rank
-            self.lora_a[slot, r:] = 0
-            lora_b = torch.nn.functional.pad(lora_b, (0, self.r_pad - r))
-        self.lora_b[slot] = lora_b.view(self.out_features, -1, 16).transpose(0, 1)
-        self.scales[slot] = float(scaling)
-        self.ranks[slot] = r
+        scaling = float(scaling)
+        if nat.glue().bank_load(self.lora_a, self.lora_b, self.ranks, self.scales, slot, lora_a, lora_b, scaling):
+            return
+        # another dtype or device, or rows that are not dense: as the bank has them, then the same call
+        lora_a, lora_b = (t.to(self.device, self.dtype).contiguous() for t in (lora_a, lora_b))
+        if not nat.glue().bank_load(self.lora_a, self.lora_b, self.ranks, self.scales, slot, lora_a, lora_b, scaling):
+            raise ValueError(f"slot {slot}: the adapter cannot be copied into the bank's tensors")
 
     def unload(self, slot: int) -> None:
         """Empty ``slot``: its rows get the shared projection alone."""

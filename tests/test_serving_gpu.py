@@ -303,3 +303,25 @@ def test_load_converts_and_clears_past_the_rank():
     assert torch.equal(bank.lora_b[0, 0, :, :5], b.to(BF16)) and not bank.lora_b[0, :, :, 5:].any()
     assert bank.ranks.tolist() == [5] and bank.scales.tolist() == [2.0]
     assert np.isclose(bank.lora_a.element_size(), 2)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("r, max_rank", [(1, 16), (16, 16), (17, 32), (33, 64), (64, 64), (100, 128)])
+def test_load_of_dense_strided_and_foreign_tensors(dtype, r, max_rank):
+    K, N = 75, 41
+    bank = AdapterBank(3, max_rank, K, N, dtype, "cuda")
+    bank.lora_a.fill_(float("nan"))
+    bank.lora_b.fill_(float("nan"))
+    a, b = torch.randn(2 * r, K + 3, device="cuda"), torch.randn(N, 2 * r, device="cuda")
+    sources = [(a[:r, :K].to(dtype).contiguous(), b[:, :r].to(dtype).contiguous()),  # dense
+               (a.to(dtype)[:r, 1:K + 1], b.to(dtype)[:, :r]),  # rows apart
+               (a[::2, :K], b[:, ::2]),  # float32 and no dense rows
+               (a[:r, :K].cpu().double(), b[:, :r].cpu().double()),  # another device
+               (a[:r, :K].to(dtype).t().contiguous().t(), b[:, :r].to(dtype).t().contiguous().t())]
+    for i, (sa, sb) in enumerate(sources):
+        bank.load(1, sa, sb, 0.5 + i)
+        assert torch.equal(bank.lora_a[1, :r], sa.to("cuda", dtype)) and not bank.lora_a[1, r:].any()
+        ranks = bank.lora_b[1].transpose(0, 1).reshape(N, -1)
+        assert torch.equal(ranks[:, :r], sb.to("cuda", dtype)) and not ranks[:, r:].any()
+        assert bank.ranks.tolist() == [0, r, 0] and bank.scales.tolist() == [0.0, 0.5 + i, 0.0]
+    assert bank.lora_a[::2].isnan().all() and bank.lora_b[::2].isnan().all()  # the neighbours

@@ -10,7 +10,7 @@ from lorafusion_b200 import _native as nat
 from lorafusion_b200.serving import AdapterBank, fused_lora_forward_rows
 from lorafusion_b200.training import AdapterAdamW, clip_adapter_grads
 
-C_TYPES = {"int32_t": 4, "uint32_t": 4, "int64_t": 8, "uint64_t": 8, "size_t": 8, "double": 8}
+C_TYPES = {"int32_t": 4, "uint32_t": 4, "float": 4, "int64_t": 8, "uint64_t": 8, "size_t": 8, "double": 8}
 
 
 def _fields(name):
@@ -29,7 +29,8 @@ def _fields(name):
     return out
 
 
-@pytest.mark.parametrize("name, cls", [("lf_rows_problem", nat.RowsProblem), ("lf_adamw_args", nat.AdamWArgs)])
+@pytest.mark.parametrize("name, cls", [("lf_rows_problem", nat.RowsProblem), ("lf_adamw_args", nat.AdamWArgs),
+                                       ("lf_bank_adapter", nat.BankAdapter)])
 def test_structs_match_the_header(name, cls):
     assert _fields(name) == [(f, getattr(cls, f).size) for f, _ in cls._fields_]
 
@@ -85,6 +86,19 @@ def test_rows_entry_refuses_before_any_launch():
     assert call(_rows(), w=None) == nat.LF_ERR_CAPACITY and call(_rows(), n=ws - 1) == nat.LF_ERR_CAPACITY
     assert L.lf_rows_forward(None, 256, 256, ws, None) == nat.LF_ERR_INVALID_ARG
     assert call(_rows(T=0, x_dev=None)) == nat.LF_OK and call(_rows(N=0)) == nat.LF_OK
+
+
+def test_bank_load_refuses_before_any_launch():
+    def call(**kw):
+        d = dict(dtype=nat.LF_BF16, K=32, N=24, r_pad=16, rank=4, scale=1.0, lda=32, ldb=4, a_dev=256, b_dev=256,
+                 slot_a_dev=256, slot_b_dev=256, slot_rank_dev=256, slot_scale_dev=256)
+        return nat.lib().lf_bank_load(nat.BankAdapter(**{**d, **kw}), None)
+
+    for kw in (dict(dtype=3), dict(K=0), dict(N=-1), dict(r_pad=8), dict(r_pad=256), dict(rank=0), dict(rank=17),
+               dict(lda=31), dict(ldb=3), dict(a_dev=None), dict(b_dev=None), dict(slot_a_dev=None),
+               dict(slot_b_dev=None), dict(slot_rank_dev=None), dict(slot_scale_dev=None)):
+        assert call(**kw) == nat.LF_ERR_INVALID_ARG, kw
+    assert nat.lib().lf_bank_load(None, None) == nat.LF_ERR_INVALID_ARG
 
 
 def _grads(*rows):
