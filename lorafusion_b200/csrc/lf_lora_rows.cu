@@ -32,7 +32,12 @@ constexpr uint32_t kNoSlot = 0xffffffffu;
 constexpr int kTileRows = 128;  // rows grouped by adapter together
 constexpr int kShrinkThreads = 256;
 constexpr int kShrinkWarps = kShrinkThreads / 32;
-constexpr int kPartBytes = 32 * 1024;  // per-warp partial products of one batch of groups
+constexpr int kSteps = 8;  // rank steps of 16 that the groups of one batch have at most
+// Lines of 128 bytes that a thread may ask of L2 ahead of its loads.  One row 4096 -> 4096: 15.0 -> 13.8 us, 250 rows of 219
+// adapters 37.3 -> 35.2; with 14 (64 rows to 14336 features) or 24 lines a thread the requests hold up the
+// loads behind them, 47 -> 50 and 94 -> 109 us.
+constexpr int kPrefetchLines = 8;
+constexpr int kSPitch = 24;  // elements from one row of a step of S to the next: no bank conflicts
 
 // Slot and rank of row t as rank << 24 | slot, or kNoSlot.
 __device__ __forceinline__ uint32_t row_adapter(const RowsArgs& p, int t, bool report) {
@@ -47,6 +52,11 @@ __device__ __forceinline__ uint32_t row_adapter(const RowsArgs& p, int t, bool r
 }
 __device__ __forceinline__ int slot_of(uint32_t e) { return static_cast<int>(e & 0xffffffu); }
 __device__ __forceinline__ int rank_of(uint32_t e) { return static_cast<int>(e >> 24); }
+// Rank steps of 16 of the smallest kernel that covers the adapter.
+__device__ __forceinline__ int width_of(uint32_t e) {
+  const int n = (rank_of(e) + 15) >> 4;
+  return n <= 2 ? n : n <= 4 ? 4 : 8;
+}
 
 template <typename T>
 __device__ __forceinline__ float to_f32(T v);
@@ -83,6 +93,7 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ void st_cluster_f32(uint32_t addr, uint32_t v) {
   asm volatile("st.shared::cluster.b32 [%0], %1;" ::"r"(addr), "r"(v) : "memory");
 }
@@ -140,8 +151,8 @@ struct Groups {
   int16_t start[kTileRows];     // first row of each group
   int16_t rows[kTileRows][8];   // rows of each group, -1: none
   int warp_groups[4];
-  int cost[kTileRows];          // what the groups up to each one (this one not) cost, and all of them
-  int total;
+  uint8_t order[kTileRows];     // the groups, widest adapters first
+  uint32_t wide[4][4];          // groups 32 w .. + 31 of width 8, 4, 2, 1
 };
 
 // Number of groups of rows t0 .. t0 + rows - 1 (at most kTileRows).  All threads of the CTA call it; ends with a barrier.
@@ -202,36 +213,30 @@ __device__ __forceinline__ int group_rows(const RowsArgs& p, int t0, int rows, b
     if ((pos & 7) == 0) s.start[grp] = static_cast<int16_t>(tid);
   }
   __syncthreads();
-  // a group's cost: its rank steps, and about one step for the rest
-  if (warp == 0) {
-    int sum = 0;
-    for (int c = 0; c < n_groups; c += 32) {
-      const int mine = c + lane < n_groups ? 1 + ((rank_of(s.eff[s.start[c + lane]]) + 15) >> 4) : 0;
-      int up = mine;
+  // Order by width: a cluster then takes every slices-th group, there and back, and all get about the same.
+  const int width = tid < n_groups ? width_of(s.eff[s.start[tid]]) : 0;
+  if (tid < kTileRows) {
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, up, o);
-        if (lane >= o) up += v;
-      }
-      if (c + lane < n_groups) s.cost[c + lane] = sum + up - mine;
-      sum += __shfl_sync(0xffffffffu, up, 31);
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t m = __ballot_sync(0xffffffffu, width == 8 >> c);
+      if (lane == 0) s.wide[c][warp] = m;
     }
-    if (lane == 0) s.total = sum;
+  }
+  __syncthreads();
+  if (tid < n_groups) {
+    int at = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t m = s.wide[c][w];
+        if (width < 8 >> c || (width == 8 >> c && w < warp)) at += __popc(m);
+        else if (width == 8 >> c && w == warp) at += __popc(m & ((1u << lane) - 1));
+      }
+    s.order[at] = static_cast<uint8_t>(tid);
   }
   __syncthreads();
   return n_groups;
-}
-
-// First group of a slice: groups go to the slice that their cost's middle falls into.
-__device__ __forceinline__ int slice_start(const Groups& s, int n_groups, int slice, int slices) {
-  int lo = 0, hi = n_groups;  // the first group whose middle is at or past the slice's share
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    const int next = mid + 1 < n_groups ? s.cost[mid + 1] : s.total;
-    if (static_cast<int64_t>(s.cost[mid] + next) * slices < 2ll * s.total * slice) lo = mid + 1;
-    else hi = mid;
-  }
-  return lo;
 }
 
 // 2^ex with the largest of a row's values over 1..2; 0 for a row that is all zero or not finite.
@@ -245,7 +250,7 @@ __device__ __forceinline__ void halves(float w, T& hi, T& lo) {
   lo = from_f32<T>(fabsf(w) <= 4.f ? w - to_f32(hi) : 0.f);
 }
 
-// One group of 8 rows as the second product sees it: S halves of row g, rows and factors of columns 2q, 2q + 1 (-1:
+// One group of 8 rows as the second product sees it: S halves of row g (8 kSPitch from step to step), rows and factors of columns 2q, 2q + 1 (-1:
 // the group has no such row).
 template <typename T>
 struct GroupRows {
@@ -304,9 +309,9 @@ __device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int 
   const int step = kNM == 1 ? 0 : q >> 1, rank0 = kNM == 1 ? 4 * q : 8 * (q & 1);
 #pragma unroll
   for (int k = 0; k < kNM; ++k) {
-    const int at = 16 * ((k & ~1) + step);  // beyond the rank nothing was written
-    const bool on = at < rank_of(e);
-    const int r = at + rank0 + 4 * (k & 1);
+    const int at = (k & ~1) + step;  // beyond the rank nothing was written
+    const bool on = 16 * at < rank_of(e);
+    const int r = at * 8 * kSPitch + rank0 + 4 * (k & 1);
     sh[k] = on ? *reinterpret_cast<const uint2*>(rows.hi + r) : zero;
     sl[k] = on ? *reinterpret_cast<const uint2*>(rows.lo + r) : zero;
   }
@@ -331,14 +336,12 @@ __device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int 
 // the dependent GEMM streams its weight while this kernel runs.
 template <typename T, int kMT>
 __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts) {
-  constexpr int kRP = kMT * 16;                                         // padded rank
-  constexpr int kBatch = kPartBytes / (kShrinkWarps * kRP * 8 * 4);     // groups of 8 rows per batch
-  constexpr int kPitch = kRP + 8;                                       // of S rows: no bank conflicts
-  __shared__ float part[kShrinkWarps][kBatch][kRP * 8];
+  constexpr int kRP = kMT * 16;  // padded rank
+  __shared__ __align__(16) float part[kShrinkWarps][kSteps][16 * 8];
   __shared__ __align__(16) Groups s;
-  __shared__ __align__(16) T s_hi[kBatch][8][kPitch], s_lo[kBatch][8][kPitch];
-  __shared__ float s_fac[kBatch][8];
-  __shared__ float s_in[kBatch * kRP * 8 + 8];  // the cluster's sums of this CTA's share (see below)
+  __shared__ __align__(16) T s_hi[kSteps][8][kSPitch], s_lo[kSteps][8][kSPitch];
+  __shared__ float s_fac[kSteps][8];
+  __shared__ __align__(16) float s_sum[kSteps][16 * 8];
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, q = lane & 3;
@@ -356,10 +359,29 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
     const int rows = min(kTileRows, p.T - t0);
     const int n_groups = group_rows(p, t0, rows, true, s);
     if (crank == 0 && slice == 0 && tid < rows) p.eff[t0 + tid] = s.eff[tid];
-    const int g_lo = slice_start(s, n_groups, slice, slices);
-    const int g_hi = slice + 1 < slices ? slice_start(s, n_groups, slice + 1, slices) : n_groups;
-    for (int first = g_lo; first < g_hi; first += kBatch) {
-      const int batch = min(kBatch, g_hi - first);
+    // this cluster's groups: places slice, 2 slices - 1 - slice, 2 slices + slice, ... of the order
+    auto group_at = [&](int j) { return static_cast<int>(s.order[j * slices + (j & 1 ? slices - 1 - slice : slice)]); };
+    const int rest = n_groups % slices, rounds = n_groups / slices;
+    const int mine = rounds + ((rounds & 1 ? slices - 1 - slice : slice) < rest);
+    for (int first = 0, batch; first < mine; first += batch) {
+      int steps = 0, ranks = 0;  // as many groups as there is room for
+      for (batch = 0; first + batch < mine; ++batch) {
+        const uint32_t e = s.eff[s.start[group_at(first + batch)]];
+        if (steps + width_of(e) > kSteps) break;
+        steps += width_of(e);
+        ranks += rank_of(e);
+      }
+      // This CTA's part of every A_i on its way to L2 at once: what the warps load at a time is too little to cover the
+      // latency of HBM that the GEMM's stream of W keeps busy.
+      const int k_lo = static_cast<int>(static_cast<int64_t>(crank) * n_blocks / kparts) * 32;
+      const int k_hi = min(K, static_cast<int>(static_cast<int64_t>(crank + 1) * n_blocks / kparts) * 32);
+      const int lines = (k_hi - k_lo + 63) >> 6;
+      for (int u = 0; u < batch && ranks * lines <= kPrefetchLines * kShrinkThreads; ++u) {
+        const uint32_t e = s.eff[s.start[group_at(first + u)]];
+        const T* a = bank + static_cast<size_t>(slot_of(e)) * p.r_pad * K + k_lo;
+        for (int l = tid; l < rank_of(e) * lines; l += kShrinkThreads)
+          prefetch_l2(a + static_cast<size_t>(l / lines) * K + (l % lines) * 64);
+      }
       // The warps divide the groups first, so that as many streams of A_i as there are warps are in flight, and K
       // where there are fewer groups than warps.
       const int lanes = batch >= 8 ? 8 : batch >= 4 ? 4 : batch >= 2 ? 2 : 1;  // groups at a time
@@ -367,12 +389,15 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
       const int ranges = kparts * subs, me = crank * subs + sub;
       const int b0 = static_cast<int>(static_cast<int64_t>(me) * n_blocks / ranges);
       const int b1 = static_cast<int>(static_cast<int64_t>(me + 1) * n_blocks / ranges);
-      for (int u = warp % lanes; u < batch; u += lanes) {
-        const uint32_t e = s.eff[s.start[first + u]];
-        const int nm = (rank_of(e) + 15) >> 4;
-        const T* xr = x + static_cast<int64_t>(t0 + max(static_cast<int>(s.rows[first + u][g]), 0)) * p.ldx + 8 * q;
+      for (int u = 0, at = 0; u < batch; ++u) {
+        const int grp = group_at(first + u);
+        const uint32_t e = s.eff[s.start[grp]];
+        const int nm = width_of(e), slot_at = at;
+        at += nm;
+        if (u % lanes != warp % lanes) continue;
+        const T* xr = x + static_cast<int64_t>(t0 + max(static_cast<int>(s.rows[grp][g]), 0)) * p.ldx + 8 * q;
         const T* ar = bank + (static_cast<size_t>(slot_of(e)) * p.r_pad + g) * K + 8 * q;
-        float* dst = part[sub][u];
+        float* dst = part[sub][slot_at];
         // the smallest kernel that covers the adapter's rank
         if (nm == 1) shrink_groups<T, 1, 8>(xr, ar, K, b0, b1, dst);
         else if (nm == 2) {
@@ -383,42 +408,55 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
           shrink_groups<T, 8, 1>(xr, ar, K, b0, b1, dst);
         }
       }
+      // and its part of every B_i, which takes the time that the exchange below does
+      const int b_lines = (nb1 - nb0) * 4;
+      for (int u = 0; u < batch && steps * b_lines <= kPrefetchLines * kShrinkThreads; ++u) {
+        const uint32_t e = s.eff[s.start[group_at(first + u)]];
+        const char* b = static_cast<const char*>(p.b_bank) +
+                        (static_cast<size_t>(slot_of(e)) * (p.r_pad >> 4) * p.N + nb0 * 16) * 32;
+        const int bytes = (min(nb1 * 16, p.N) - nb0 * 16) * 32;
+        for (int k = 0; 16 * k < rank_of(e); ++k)
+          for (int l = tid * 128; l < bytes; l += kShrinkThreads * 128)
+            prefetch_l2(b + static_cast<size_t>(k) * p.N * 32 + l);
+      }
       __syncthreads();
-      // The warps' sums, and with a cluster the CTAs': value i (of the batch's kRP x 8 a group) is summed by CTA
-      // i / segment, which the others send theirs and which sends the sum to all.
-      // The finished sums take the place of the first warp's.
-      float* const s_sum = &part[0][0][0];
-      const int values = batch * kRP * 8, segment = (values + kparts - 1) / kparts;
-      for (int i = tid; i < values; i += kShrinkThreads) {
+      // The warps' sums, in the place of the first warp's; with a cluster every CTA reads the others' and adds them up
+      // in the same order.  (Passing the sums on by remote stores, to the CTA that adds them and back, took two
+      // cluster barriers and 5 us; this takes one.)
+      for (int i = tid; i < steps * 128; i += kShrinkThreads) {
         float v = part[0][0][i];
         for (int w = 1; w < subs; ++w) v += part[w][0][i];
-        if (kparts == 1) {
-          s_sum[i] = v;
-        } else {
-          const int owner = i / segment;
-          st_cluster_f32(map_to_cta(smem_u32(&s_in[crank * segment + i - owner * segment]), owner), __float_as_uint(v));
-        }
+        if (kparts == 1) s_sum[0][i] = v;
+        else part[0][0][i] = v;
       }
       if (kparts > 1) {
         cluster_sync_all();
-        for (int i = tid; i < min(segment, values - crank * segment); i += kShrinkThreads) {
-          float v = s_in[i];
-          for (int c = 1; c < kparts; ++c) v += s_in[c * segment + i];
-          const uint32_t at = smem_u32(&s_sum[crank * segment + i]);
-          for (int c = 0; c < kparts; ++c) st_cluster_f32(map_to_cta(at, c), __float_as_uint(v));
+        for (int i = 4 * tid; i < steps * 128; i += 4 * kShrinkThreads) {
+          const uint32_t at = smem_u32(&part[0][0][i]);
+          float4 v[8];
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (c < kparts) v[c] = ld_cluster_f32x4(map_to_cta(at, c));
+#pragma unroll
+          for (int c = 1; c < 8; ++c)
+            if (c < kparts) v[0].x += v[c].x, v[0].y += v[c].y, v[0].z += v[c].z, v[0].w += v[c].w;
+          *reinterpret_cast<float4*>(&s_sum[0][i]) = v[0];
         }
-        cluster_sync_all();
-      } else {
-        __syncthreads();
+        __syncwarp();
+        cluster_arrive();  // the others may write their sums again once all have come here
       }
+      __syncthreads();
       // S of each group, one warp a group; every CTA needs all of them for the second product
-      for (int u = warp; u < batch; u += kShrinkWarps) {
-        const uint32_t e = s.eff[s.start[first + u]];
-        const int rank = rank_of(e);
+      for (int u = 0, at = 0; u < batch; ++u) {
+        const int grp = group_at(first + u);
+        const uint32_t e = s.eff[s.start[grp]];
+        const int rank = rank_of(e), slot_at = at;
+        at += width_of(e);
+        if (u != warp) continue;
         float v[kRP / 4];
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < kRP / 4; ++i) v[i] = (lane >> 3) + 4 * i < rank ? s_sum[u * kRP * 8 + lane + 32 * i] : 0.f;
+        for (int i = 0; i < kRP / 4; ++i) v[i] = (lane >> 3) + 4 * i < rank ? s_sum[slot_at][lane + 32 * i] : 0.f;
 #pragma unroll
         for (int i = 0; i < kRP / 4; ++i) {
           top = fmaxf(top, fabsf(v[i]));
@@ -432,19 +470,23 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
 #pragma unroll
         for (int i = 0; i < kRP / 4; ++i) {
           const int j = (lane >> 3) + 4 * i;
-          if (j < ((rank + 15) & ~15)) halves<T>(v[i] * down, s_hi[u][lane & 7][j], s_lo[u][lane & 7][j]);
+          if (j < ((rank + 15) & ~15))
+            halves<T>(v[i] * down, s_hi[slot_at + (j >> 4)][lane & 7][j & 15], s_lo[slot_at + (j >> 4)][lane & 7][j & 15]);
         }
       }
       __syncthreads();
       // the warps divide the groups, then the features, here too
       const int f0 = nb0 + (nb1 - nb0) * sub / subs, f1 = nb0 + (nb1 - nb0) * (sub + 1) / subs;
-      for (int u = warp % lanes; u < batch; u += lanes) {
-        const uint32_t e = s.eff[s.start[first + u]];
-        const int nm = (rank_of(e) + 15) >> 4;
+      for (int u = 0, at = 0; u < batch; ++u) {
+        const int grp = group_at(first + u);
+        const uint32_t e = s.eff[s.start[grp]];
+        const int nm = width_of(e), slot_at = at;
+        at += nm;
+        if (u % lanes != warp % lanes) continue;
         GroupRows<T> rows_of;
-        const int r0 = s.rows[first + u][2 * q], r1 = s.rows[first + u][2 * q + 1];
-        rows_of.hi = s_hi[u][g];
-        rows_of.lo = s_lo[u][g];
+        const int r0 = s.rows[grp][2 * q], r1 = s.rows[grp][2 * q + 1];
+        rows_of.hi = s_hi[slot_at][g];
+        rows_of.lo = s_lo[slot_at][g];
         rows_of.row0 = r0 < 0 ? -1 : t0 + r0;
         rows_of.row1 = r1 < 0 ? -1 : t0 + r1;
         rows_of.f0 = s_fac[u][2 * q];
@@ -458,6 +500,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
           expand_group<T, 8, 1>(p, e, f0, f1, rows_of);
         }
       }
+      if (kparts > 1) cluster_wait();
       __syncthreads();
     }
     __syncthreads();
