@@ -469,7 +469,7 @@ LF_API int lf_assign_rows(const int32_t* bin_start, const int32_t* entry_adapter
 
 /* One projection and a bank of resident adapters.  `slot_rank_dev` holds each slot's rank (0: empty
  * slot, its rows get the shared projection alone), at most r_pad; bank entries past it must be zero.
- * n_slots * r_pad / 16 * max(N, 16) must fit in 31 bits. */
+ * n_slots * r_pad / 16 * max(N, 16) must fit in 31 bits, K and N are at most 2^24. */
 typedef struct lf_rows_problem {
   int32_t dtype;             /* lf_dtype of x, W, y and the bank */
   int32_t T, K, N;           /* rows, in_features, out_features */
@@ -507,7 +507,8 @@ LF_API int lf_bank_load(const lf_bank_adapter* adapter, lf_stream_t stream);
 LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype);
 
 /*
- * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense.  row_slot is read on
+ * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense, shares no memory with x, W or
+ * the bank.  row_slot is read on
  * the device, so a captured call follows later changes of it and of the bank's contents.  A
  * slot at or above n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
  * bf16/f16 with K, N and ldx multiples of 8 and 16-byte aligned buffers run on the tensor cores, other

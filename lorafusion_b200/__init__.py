@@ -5,6 +5,10 @@
 * :mod:`lorafusion_b200.config` — ``AdapterSpec``, ``TileRoute``, ``TileRoutingConfig``.
 * :mod:`lorafusion_b200.scheduler` — grouping, bin packing and fused-batch assembly.
 * :mod:`lorafusion_b200.coordinator` — ``Coordinator`` (request batch in, results out).
+* :mod:`lorafusion_b200.training` — what follows the backward: ``clip_adapter_grads`` and ``AdapterAdamW``, each
+  adapter with its own norm, step count and rates.
+* :mod:`lorafusion_b200.serving` — trained adapters resident in an ``AdapterBank`` and
+  ``fused_lora_forward_rows``, one projection for rows of many requests, an adapter index per row.
 * :mod:`lorafusion_b200.sharding` — row sharding of packed bins across GPUs and the
   gradient all-reduce of adapters that span ranks.
 """

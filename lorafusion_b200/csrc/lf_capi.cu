@@ -892,7 +892,8 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   if (p->dtype != LF_F32 && p->dtype != LF_BF16 && p->dtype != LF_F16) return LF_ERR_INVALID_ARG;
   if (p->r_pad != 16 && p->r_pad != 32 && p->r_pad != 64 && p->r_pad != LF_BANK_MAX_RANK) return LF_ERR_INVALID_ARG;
   if (p->row_slot_bytes != 4 && p->row_slot_bytes != 8) return LF_ERR_INVALID_ARG;
-  if (p->n_slots >= (1 << 24) || 
+  // what 32-bit indices of elements and of bank rows hold
+  if (p->K > (1 << 24) || p->N > (1 << 24) || p->n_slots >= (1 << 24) ||
       static_cast<int64_t>(p->n_slots) * (p->r_pad / 16) * (p->N > 16 ? p->N : 16) > INT32_MAX)
     return LF_ERR_UNSUPPORTED;
   if (p->T == 0 || p->N == 0) return LF_OK;
@@ -901,6 +902,15 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     return LF_ERR_INVALID_ARG;
   if (!workspace_dev || workspace_bytes < lf_rows_workspace_bytes(p->T, p->N, p->r_pad, p->dtype)) return LF_ERR_CAPACITY;
   if (!aligned16(workspace_dev) || !aligned16(p->b_bank_dev)) return LF_ERR_INVALID_ARG;
+  const uint64_t es = static_cast<uint64_t>(elem_bytes(p->dtype)), T = p->T, K = p->K, N = p->N;
+  const uint64_t ranks = static_cast<uint64_t>(p->n_slots) * p->r_pad, y0 = reinterpret_cast<uint64_t>(y_dev);
+  auto meets_y = [&](const void* base, uint64_t elems) {
+    const uint64_t b = reinterpret_cast<uint64_t>(base);
+    return elems > 0 && b < y0 + T * N * es && y0 < b + elems * es;
+  };
+  if (meets_y(p->x_dev, (T - 1) * p->ldx + K) || meets_y(p->w_dev, N * K) || meets_y(p->a_bank_dev, ranks * K) ||
+      meets_y(p->b_bank_dev, ranks * N))
+    return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
   RowsArgs a{};

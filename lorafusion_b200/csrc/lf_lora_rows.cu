@@ -1,21 +1,28 @@
 // One shared projection with an adapter per row, the adapter's index read on the device:
 //   y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T,   i = row_slot[t]  (negative: no adapter).
 //
-// Two launches, the second started while the first runs:
-//   rows_lora    the adapters' part, float32: S = x[t] A_i^T, then s_i S B_i^T.  Rows are grouped by adapter on
-//                the device, so any order of rows works and no host plan is needed.  A cluster takes a
-//                few groups: its CTAs cut K for S, exchange their sums through distributed shared
-//                memory, then cut the output features, so no grid-wide step lies between A_i and B_i.
-//                Few rows bring one adapter each: both products are streams of weights through
-//                warp-level MMAs whose 8 columns are rows of one adapter, bound by bytes.
-//   rows_gemm    y^T tiles of 128 output features x up to 256 rows with tcgen05 (the weight is the
-//                M operand, so a decode step of a few rows wastes no tensor-memory lanes and streams
-//                W once), K split over a cluster when the tiles alone would leave SMs idle.  The
-//                epilogue waits for the first launch, adds its part and writes y once.
+// The adapters' part goes to a float32 buffer, and a GEMM whose last launch starts while that is still written adds it in
+// its epilogue:
+//   few rows     (decode) rows_lora: one launch.  A tile's rows are grouped by adapter, 8 at a time; a cluster takes
+//                a few groups, its CTAs cut K for S = x A_i^T, exchange their sums through distributed
+//                shared memory, then cut the output features for s_i S B_i^T, so that no grid-wide step lies
+//                between A_i and B_i.  Few rows bring one adapter each: both products are streams of weights
+//                through warp-level MMAs whose 8 columns are rows of one adapter, bound by bytes and latency.
+//   many rows    (prompts) many_plan, many_shrink, many_expand: rows sorted by adapter, both products on tcgen05.
+//   rows_gemm    y^T tiles of 128 output features x up to 256 rows with tcgen05 (the weight is the M operand, so a
+//                decode step of a few rows wastes no tensor-memory lanes and streams W once), K split
+//                over a cluster when the tiles alone would leave SMs idle.  Long batches go through
+//                the CTA-pair GEMM of lf_tc.cu where its tiles fit better.
+// Any order of rows works and no host plan is needed: the adapters are read on the device.
 //
 // S enters the second product as hi + lo halves of the input type after a per-row power-of-two scaling (the
 // row's largest magnitude becomes 1..2), so it is exact to about 2^-16 (bf16) or 2^-22 (f16)
 // relative and a float16 S cannot overflow.  All sums are float32.
+//
+// Measured (replayed graph, weights from HBM; the shared projection alone by cuBLAS in brackets): 1 row 4096 -> 4096, rank 16
+// 13.6 us (13.0); 64 rows of 56 adapters, ranks 8 to 64, 4096 -> 14336 47 us (23); 250 rows of 219 adapters
+// of rank 16, 4096 -> 4096 35 us (11); 8192 rows of prompts, 64 adapters of ranks 8 to 64, 4096 -> 4096
+// 252 us (178).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -330,10 +337,14 @@ __device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int 
     expand_blocks<T, kNM, 1>(w, p.N, n, sh, sl, rows, o0, o1, second);
 }
 
-// Work items: (row tile, slice of its groups), each taken by a cluster of `kparts` CTAs that cut K for the
-// first product and the output features for the second.  Partial products
-// meet in shared memory, then across the cluster, in a fixed order.  The grid fits the GPU at once, so
-// the dependent GEMM streams its weight while this kernel runs.
+// Few rows.  Work items: (row tile, slice of its groups), each taken by a cluster of `kparts` CTAs that cut K for the first
+// product and the output features for the second.  Partial products meet in shared memory, then across the
+// cluster, in a fixed order.  The grid fits the GPU at once with one CTA an SM and leaves room for a CTA of the
+// GEMM, which streams W meanwhile.
+// Bound by latency: at 64 rows of 56 adapters, 4096 -> 14336, a CTA needs 4 us to sort its tile, 6 to 10 for its part of
+// A_i, 8 for the exchange and S, and 8 to 19 for its part of B_i with 32 KB of loads in flight, while the
+// GEMM is through after 28 us of the 47.  Tried without gain: 16 loads a lane instead of 8 for B_i (registers), bulk
+// copies into a ring in the GEMM's epilogue, a third launch for the second product.
 template <typename T, int kMT>
 __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts) {
   constexpr int kRP = kMT * 16;  // padded rank
@@ -558,9 +569,9 @@ __global__ void __maxnreg__(80)
   const RowsArgs& p = prm.a;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   constexpr int w_bytes = kWBytes, block_bytes = w_bytes + kXBytes;
-  // A stage holds `sub` blocks of 64 elements of K.  A block costs the loading thread two copies and the MMA
-  // thread four MMAs, but each wait costs both about 0.1 us: with one block a stage, a tile of few rows took 0.35 us
-  // a block however small its bytes.
+  // A stage holds `sub` blocks of 64 elements of K.  A block costs the loading warp two copies and the MMA warp four
+  // MMAs, but each wait costs both about 0.1 us: with one block a stage, and with loops that only one lane ran, a
+  // tile of few rows took 0.35 us a block however small its bytes; 1 row 4096 -> 4096 then took 12.1 us, now 11.0.
   const int sub = prm.sub, stage_bytes = sub * block_bytes;
   const int ks = prm.ksplit, stages = prm.stages;
   const int part = blockIdx.x % ks;  // rank in the cluster
@@ -737,7 +748,8 @@ struct ManyTile {
   int pad;
 };
 
-// Sorts at most kRowsChunk rows: a hash table of adapters in shared memory counts them, a scan places them.
+// Sorts at most kRowsChunk rows: a hash table of adapters in shared memory counts them, a scan places them.  One CTA,
+// latency: 10 us for 8192 rows, 7 for 1000.
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanSlots = 2 * kRowsChunk;  // of the table: never more than half full
 constexpr int kPlanRows = kRowsChunk / kPlanThreads;
@@ -822,10 +834,11 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
     if (e[i] != kNoSlot) p.perm[count[at[i]] + pos[i]] = tid + i * kPlanThreads;
 }
 
-// S = x A_i^T of a tile, in sorted order.  K is cut over a cluster when there cannot be many tiles.  Eight warps gather x
+// S = x A_i^T of a tile, in sorted order.  K is cut over a cluster when there cannot be many tiles.  Four warps gather x
 // with 16-byte copies, 8 lanes to the 128 bytes of a row and block of 64 elements, placed as the 128-byte swizzle
 // would (a TMA gather of four rows takes about 50 ns however many are in flight: 99 us for 8192 rows); TMA
-// loads A_i.
+// loads A_i.  24 us for 8192 x 4096 and 64 adapters of ranks 8 to 64: a round of 87 tiles, half a microsecond for 128
+// elements of K, where the MMA warp's eight small MMAs and their waits take what the copies do.
 constexpr int kXBytes = kTileRows * kBK * 2;
 constexpr int kShrinkMaxStages = 8;
 constexpr int kLoadWarps = 4;
@@ -1060,7 +1073,8 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 }
 
 // delta = s_i S B_i^T.  A unit is a tile x 256 features, and a CTA takes a run of them; the rank steps of S (high, then low
-// halves) times those of B_i go into one of two accumulators.
+// halves) times those of B_i go into one of two accumulators.  38 us for 8192 x 4096 (117 MB written): bound by
+// the epilogue's way through shared memory, 128 KB in, out and to L2 a unit, about 4000 clocks.
 constexpr int kSStepBytes = kTileRows * 32;  // 16 ranks of 128 rows
 constexpr int kBStepBytes = 256 * 32;        // 16 ranks of 256 features
 constexpr int kExpandStages = 5, kExpandChunk = 2;  // rank steps of a stage, at most
@@ -1534,7 +1548,7 @@ RowsTiles rows_tiles(int T, int K, int N, int num_sms) {
   t.rows = T <= 16 ? 16 : T <= 32 ? 32 : T <= 64 ? 64 : T <= 128 ? 128 : 256;
   // K is split while the tiles leave more than half of the SMs without one and a part has 256 elements.
   // (Smaller tiles that cover every SM were slower: 32 features a tile and no split took 20 us where
-  // 128 features and a split in four takes 12.6, at 1 x 4096 -> 4096, and a GPU without free SMs cannot place the
+  // 128 features and a split in four took 12.6, at 1 x 4096 -> 4096, and a GPU without free SMs cannot place the
   // adapters' CTAs beside the GEMM's.)
   const int64_t tiles = static_cast<int64_t>((N + kWRows - 1) / kWRows) * ((T + t.rows - 1) / t.rows);
   const int nkb = (K + kBK - 1) / kBK;

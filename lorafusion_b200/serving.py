@@ -49,14 +49,17 @@ class AdapterBank:
             raise ValueError(f"n_slots must be 1 .. {(1 << 24) - 1}, got {n_slots}")
         if not 0 < max_rank <= nat.BANK_MAX_RANK:
             raise ValueError(f"max_rank must be 1 .. {nat.BANK_MAX_RANK}, got {max_rank}")
-        if in_features <= 0 or out_features <= 0:
-            raise ValueError("in_features and out_features must be positive")
+        if not (0 < in_features <= 1 << 24 and 0 < out_features <= 1 << 24):
+            raise ValueError(f"in_features and out_features must be 1 .. {1 << 24}, got {in_features}, {out_features}")
+        self.r_pad = next(r for r in (16, 32, 64, nat.BANK_MAX_RANK) if max_rank <= r)
+        if n_slots * (self.r_pad // 16) * max(out_features, 16) >= 1 << 31:
+            raise ValueError(f"{n_slots} slots of rank {self.r_pad} and {out_features} features are too many for one bank: "
+                             "n_slots * padded rank / 16 * out_features must stay below 2**31")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.n_slots, self.max_rank = n_slots, max_rank
         self.in_features, self.out_features = in_features, out_features
         self.dtype, self.device = dtype, device
-        self.r_pad = next(r for r in (16, 32, 64, nat.BANK_MAX_RANK) if max_rank <= r)
         self.lora_a = torch.zeros(n_slots, self.r_pad, in_features, dtype=dtype, device=device)
         # B_i in steps of 16 ranks: what a kernel reads of an adapter is contiguous whatever its rank
         self.lora_b = torch.zeros(n_slots, self.r_pad // 16, out_features, 16, dtype=dtype, device=device)
@@ -99,7 +102,8 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     tensor on that device, in any order; a negative entry means no adapter, and so does an
     empty slot.  An entry at or above ``bank.n_slots`` also gets the shared projection alone and is
     reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.
-    ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor.
+    ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor; it must not
+    overlap ``x``, ``base_weight`` or the bank.
 
     Two launches on the current stream of ``x``'s device, long batches (above 256 rows,
     or 512 where the bank's padded rank is at most 32) in chunks of 8192 rows of four launches each.  bf16/f16 problems whose in_features or

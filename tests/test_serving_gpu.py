@@ -281,7 +281,7 @@ def test_refusals():
         dict(w=w.T.contiguous().T), dict(w=w.cpu()), dict(slots=slots[:7]), dict(slots=slots.cpu()),
         dict(slots=slots.to(torch.int16)), dict(slots=slots.float()), dict(out=torch.empty(8, 65, device="cuda")),
         dict(out=torch.empty(8, 64, device="cuda")), dict(out=torch.empty(64, 8, dtype=BF16, device="cuda").T),
-        dict(out=torch.empty(8, 64, dtype=BF16)),
+        dict(out=torch.empty(8, 64, dtype=BF16)), dict(out=x), dict(out=w[8:16]), dict(out=bank.lora_a[0, :8]), dict(out=bank.lora_b.view(-1, 64)[4:12]),
     ]
     for b in bad:
         with pytest.raises(ValueError):

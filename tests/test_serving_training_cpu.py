@@ -54,7 +54,8 @@ def test_host_tensors_are_refused():
 
 
 @pytest.mark.parametrize("args", [(0, 8, 16, 16), (1 << 24, 8, 16, 16), (2, 0, 16, 16), (2, 129, 16, 16),
-                                  (2, 8, 0, 16), (2, 8, 16, 0), (2, 8, 16, 16, torch.int8)])
+                                  (2, 8, 0, 16), (2, 8, 16, 0), (2, 8, 16, 16, torch.int8), (2, 8, (1 << 24) + 1, 16),
+                                  (2, 8, 16, (1 << 24) + 1), (1 << 23, 128, 16, 64)])
 def test_bank_sizes(args):
     with pytest.raises(ValueError):
         AdapterBank(*args, device="cuda:0")
@@ -80,6 +81,7 @@ def test_rows_entry_refuses_before_any_launch():
                dict(slot_scale_dev=None), dict(b_bank_dev=264)):
         assert call(_rows(**kw)) == nat.LF_ERR_INVALID_ARG, kw
     assert call(_rows(n_slots=1 << 24)) == nat.LF_ERR_UNSUPPORTED
+    assert call(_rows(K=(1 << 24) + 1, ldx=1 << 25)) == call(_rows(N=(1 << 24) + 1), n=1 << 60) == nat.LF_ERR_UNSUPPORTED
     assert call(_rows(n_slots=(1 << 24) - 1, N=136), n=1 << 40) == nat.LF_ERR_UNSUPPORTED  # more than 31 bits of bank rows
     assert call(_rows(), y=None) == nat.LF_ERR_INVALID_ARG
     assert call(_rows(), w=264) == nat.LF_ERR_INVALID_ARG
