@@ -281,7 +281,8 @@ def test_refusals():
         dict(w=w.T.contiguous().T), dict(w=w.cpu()), dict(slots=slots[:7]), dict(slots=slots.cpu()),
         dict(slots=slots.to(torch.int16)), dict(slots=slots.float()), dict(out=torch.empty(8, 65, device="cuda")),
         dict(out=torch.empty(8, 64, device="cuda")), dict(out=torch.empty(64, 8, dtype=BF16, device="cuda").T),
-        dict(out=torch.empty(8, 64, dtype=BF16)), dict(out=x), dict(out=w[8:16]), dict(out=bank.lora_a[0, :8]), dict(out=bank.lora_b.view(-1, 64)[4:12]),
+        dict(out=torch.empty(8, 64, dtype=BF16)), dict(out=x), dict(out=w[8:16]),
+        dict(out=bank.lora_a[0, :8]), dict(out=bank.lora_b.view(-1, 64)[4:12]),
     ]
     for b in bad:
         with pytest.raises(ValueError):
@@ -325,3 +326,46 @@ def test_load_of_dense_strided_and_foreign_tensors(dtype, r, max_rank):
         assert torch.equal(ranks[:, :r], sb.to("cuda", dtype)) and not ranks[:, r:].any()
         assert bank.ranks.tolist() == [0, r, 0] and bank.scales.tolist() == [0.0, 0.5 + i, 0.0]
     assert bank.lora_a[::2].isnan().all() and bank.lora_b[::2].isnan().all()  # the neighbours
+
+
+@pytest.mark.parametrize("T", [40, 1100])
+def test_rows_apart_without_adapters_and_out_of_range(T):
+    K, N = 136, 264
+    x, w, bank, adapters, slots = make(BF16, T, K, N, [64, 8, 0], 64)
+    wide = torch.full((T, K + 24), float("nan"), dtype=BF16, device="cuda")
+    wide[:, 8:K + 8] = x
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    assert torch.equal(fused_lora_forward_rows(wide[:, 8:K + 8], w, bank, slots), y)
+    off = torch.full((T, K + 3), float("nan"), dtype=BF16, device="cuda")  # rows that are not 16-byte aligned
+    off[:, 1:K + 1] = x
+    assert torch.equal(fused_lora_forward_rows(off[:, 1:K + 1], w, bank, slots), y)
+    none = fused_lora_forward_rows(x, w, bank, torch.full((T,), -1, device="cuda"))
+    check(none, x, w, adapters, torch.full((T,), -1, device="cuda"))
+    assert torch.equal(fused_lora_forward_rows(x, w, bank, torch.full((T,), 2, device="cuda")), none)  # an empty slot
+    assert nat.device_error() == 0
+    assert torch.equal(fused_lora_forward_rows(x, w, bank, torch.full((T,), 3, device="cuda")), none)
+    assert nat.device_error() == nat.ERR_ROW_SLOT and nat.device_error() == 0
+
+
+def test_long_batches_on_two_streams():
+    first = make(BF16, 1300, 512, 1024, [16, 64, 33], 64, seed=1)
+    second = make(BF16, 900, 1024, 512, [100, 16], 128, seed=2)
+    want = [fused_lora_forward_rows(x, w, bank, slots) for x, w, bank, _, slots in (first, second)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (x, w, bank, _, slots) in enumerate((first, second)):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(fused_lora_forward_rows(x, w, bank, slots))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[i]) for i in range(2) for y in got[i])
+    assert nat.device_error() == 0
+
+
+def test_a_single_slot_and_a_single_feature_block():
+    """One adapter on every row of a long batch, eight output features, K below one block."""
+    T, K, N = 1025, 8, 8
+    x, w, bank, adapters, _ = make(F16, T, K, N, [7], 8)
+    slots = torch.zeros(T, dtype=torch.int32, device="cuda")
+    check(fused_lora_forward_rows(x, w, bank, slots), x, w, adapters, slots)
