@@ -20,8 +20,8 @@
 // relative and a float16 S cannot overflow.  All sums are float32.
 //
 // Measured (replayed graph, weights from HBM; the shared projection alone by cuBLAS in brackets): 1 row 4096 -> 4096, rank 16
-// 13.6 us (13.0); 64 rows of 56 adapters, ranks 8 to 64, 4096 -> 14336 47 us (23); 250 rows of 219 adapters
-// of rank 16, 4096 -> 4096 35 us (11); 8192 rows of prompts, 64 adapters of ranks 8 to 64, 4096 -> 4096
+// 12.7 us (12.9); 64 rows of 56 adapters, ranks 8 to 64, 4096 -> 14336 42 us (23); 250 rows of 219 adapters
+// of rank 16, 4096 -> 4096 37 us (11); 8192 rows of prompts, 64 adapters of ranks 8 to 64, 4096 -> 4096
 // 252 us (178).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -358,7 +358,7 @@ __device__ __forceinline__ void expand_group(const RowsArgs& p, uint32_t e, int 
 // GEMM, which streams W meanwhile.
 // Bound by latency: at 64 rows of 56 adapters, 4096 -> 14336, a CTA needs 4 us to sort its tile, 6 to 10 for its part of
 // A_i, 8 for the exchange and S, and 8 to 19 for its part of B_i with 32 KB of loads in flight, while the
-// GEMM is through after 28 us of the 47.  Tried without gain: 16 loads a lane instead of 8 for B_i (registers), bulk
+// GEMM is through after 28 us of the 42.  Tried without gain: 16 loads a lane instead of 8 for B_i (registers), bulk
 // copies into a ring in the GEMM's epilogue, a third launch for the second product.
 template <typename T, int kMT>
 __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const RowsArgs p, int slices, int kparts) {
@@ -502,8 +502,8 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
       }
       __syncthreads();
       // The warps divide the groups, then the features, here too; but the features alone where the groups' widths differ:
-      // one warp would have four times another's work (64 rows of ranks 8 to 64 to 14336 features 47 -> 42 us; with
-      // equal widths 250 rows of rank 16 are 35 against 37).
+      // one warp would have four times another's work (64 rows of ranks 8 to 64 to 14336 features 46 -> 42 us; with equal
+      // widths the other way was slower, 250 rows of rank 16 37.1 against 36.5).
       int lanes_b = lanes;
       if (width_of(s.eff[s.start[group_at(first)]]) != width_of(s.eff[s.start[group_at(first + batch - 1)]]))
         for (lanes_b = 1; lanes_b < lanes && (nb1 - nb0) * lanes_b < 4 * kShrinkWarps;) lanes_b *= 2;

@@ -12,6 +12,12 @@
 // the rounded weight.  They are bound by HBM; passes that follow a norm pass walk the chunks
 // backwards, so they start on what the norm pass left in the 126 MB L2.
 //
+// Measured, the seven projections of a Llama-3-8B block (896 tensors of 64 adapters, ranks 8 to 64): clipping 315 MB of
+// bf16 gradients by adapter 110 us (one read, and a write of the 231 MB beyond the limit: 83 us at the rate
+// of a copy), the AdamW step, 4.4 GB, 735 us (673); 256 adapters of rank 64 on 8192 x 28672, 16.9 GB
+// 2530 us (2586).  Chunks of 8192 elements, all loads of a thread before the first use; small
+// calls (11 us) are the launches and their host side.
+//
 // Sums of squares are held in float64 from the first product on: a float32 square overflows above
 // 1.8e19 and vanishes below 1e-23, and the sums run over up to 10^9 elements.  Partial sums are
 // added in a fixed order, so the norms are the same bits on every run.
