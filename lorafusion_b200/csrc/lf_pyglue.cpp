@@ -336,7 +336,9 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::cuda::OptionalCUDAGuard guard(dev);
   const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
   cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
-  if (cudaStreamIsCapturing(stream, &capture) != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+  const cudaError_t asked = cudaStreamIsCapturing(stream, &capture);
+  if (asked != cudaSuccess || capture != cudaStreamCaptureStatusNone) {
+    if (asked != cudaSuccess) cudaGetLastError();  // the answer to the question, not an error of a later call
     PyErr_SetString(PyExc_RuntimeError,
                     "AdapterAdamW.step cannot be captured into a CUDA graph: replays would change weights whose packed "
                     "copies b200_ops keeps");

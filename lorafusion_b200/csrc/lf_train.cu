@@ -14,7 +14,7 @@
 //
 // Measured, the seven projections of a Llama-3-8B block (896 tensors of 64 adapters, ranks 8 to 64): clipping 315 MB of
 // bf16 gradients by adapter 110 us (one read, and a write of the 231 MB beyond the limit: 83 us at the rate
-// of a copy), the AdamW step, 4.4 GB, 735 us (673); 256 adapters of rank 64 on 8192 x 28672, 16.9 GB
+// of a copy), the AdamW step, 4.4 GB, 725 us (673); 256 adapters of rank 64 on 8192 x 28672, 16.9 GB
 // 2530 us (2586).  Chunks of 8192 elements, all loads of a thread before the first use; small
 // calls (11 us) are the launches and their host side.
 //
@@ -39,6 +39,9 @@ namespace {
 constexpr int kChunk = 8192;      // elements a CTA handles: 4 to 8 16-byte loads a thread
 constexpr int kThreads = 256;
 constexpr int kFinalThreads = 512;
+// CTAs that share a chunk's update (1 / 2 / 4: 16 adapters of rank 16, 4096 -> 4096 22.4 / 20.8 / 20.5 us, the 896 tensors
+// named above 721 / 711 / 738).
+constexpr int kUpdateParts = 2;
 constexpr int kGroupsPerLaunch = 4096;  // groups whose presence bits fit one launch's parameters
 
 // ------------------------------------------------------------------- element access
@@ -436,8 +439,18 @@ struct AdamFinal {
 __global__ void __launch_bounds__(kThreads)
     adam_final_kernel(const __grid_constant__ Presence pr, AdamTables tb, AdamFinal a) {
   pdl_launch_dependents();
-  pdl_wait();
   const int g = pr.group0 + blockIdx.x;
+  const bool present = (pr.bits[blockIdx.x >> 5] >> (blockIdx.x & 31)) & 1u;
+  AdamCoef c{1.0f, 1.0f, 0.0f, -1.0f};  // root < 0: leave the group as it is
+  int t = 0;
+  if (threadIdx.x == 0 && present) {  // all but the factor, while the norms are still summed
+    t = a.steps[g] + 1;
+    const double2 h = a.hyper[g];
+    c.shrink = static_cast<float>(1.0 - h.x * h.y);
+    c.size = static_cast<float>(h.x / (1.0 - pow(a.beta1, static_cast<double>(t))));
+    c.root = static_cast<float>(sqrt(1.0 - pow(a.beta2, static_cast<double>(t))));
+  }
+  pdl_wait();
   double acc = 0.0;
   if (a.part != nullptr) {
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -461,17 +474,12 @@ __global__ void __launch_bounds__(kThreads)
   if (threadIdx.x != 0) return;
   const double norm = sqrt(acc);
   if (a.part != nullptr) a.norms[g] = static_cast<float>(norm);
-  AdamCoef c{1.0f, 1.0f, 0.0f, -1.0f};  // root < 0: leave the group as it is
-  const bool present = (pr.bits[blockIdx.x >> 5] >> (blockIdx.x & 31)) & 1u;
   const bool bad = a.skip_nonfinite && !(norm <= 1.7976931348623157e308);
   if (present && !bad) {
-    const int t = a.steps[g] + 1;
     a.steps[g] = t;
-    const double2 h = a.hyper[g];
-    c.factor = a.max_norm >= 0.0 ? static_cast<float>(clip_factor(norm, a.max_norm)) : 1.0f;
-    c.shrink = static_cast<float>(1.0 - h.x * h.y);
-    c.size = static_cast<float>(h.x / (1.0 - pow(a.beta1, static_cast<double>(t))));
-    c.root = static_cast<float>(sqrt(1.0 - pow(a.beta2, static_cast<double>(t))));
+    if (a.max_norm >= 0.0) c.factor = static_cast<float>(clip_factor(norm, a.max_norm));
+  } else {
+    c.root = -1.0f;
   }
   a.coef[g] = c;
 }
@@ -513,24 +521,25 @@ template <typename P, typename G, int kN>
 __global__ void __launch_bounds__(kThreads)
     adam_update_kernel(const __grid_constant__ PtrPack<kN> pk, AdamTables tb, AdamState s, int chunk0) {
   constexpr bool kMaster = sizeof(P) == 2;
-  const int chunk = chunk0 + (gridDim.x - 1 - blockIdx.x);
+  const int part = blockIdx.x % kUpdateParts;  // of the chunk
+  const int chunk = chunk0 + (gridDim.x - 1 - blockIdx.x) / kUpdateParts;
   const int t = tb.chunk_tensor[chunk];
   const lf_adamw_tensor rec = tb.rec[t];
   const G* grad = reinterpret_cast<const G*>(pk.ptr[t - pk.tensor0]);
-  pdl_wait();
-  if (grad == nullptr) return;
-  const AdamCoef c = s.coef[rec.group];
-  if (c.root < 0.0f) return;
   const uint32_t first = static_cast<uint32_t>(chunk - rec.chunk0) * kChunk;
   const int n = min(static_cast<uint32_t>(kChunk), rec.numel - first);
-  grad += first;
   P* w = reinterpret_cast<P*>(rec.param) + first;
   float* m = s.exp_avg + rec.state_off + first;
   float* v = s.exp_avg_sq + rec.state_off + first;
   float* q = kMaster ? s.master + rec.state_off + first : reinterpret_cast<float*>(w);
+  pdl_wait();
+  if (grad == nullptr) return;
+  const AdamCoef c = s.coef[rec.group];
+  if (c.root < 0.0f) return;
+  grad += first;
   int done = 0;
   if (aligned16(grad) && aligned16(w)) {  // states start at multiples of 8 elements
-    for (int at = threadIdx.x * 8; at + 8 <= n; at += kThreads * 8) {
+    for (int at = (part * kThreads + threadIdx.x) * 8; at + 8 <= n; at += kUpdateParts * kThreads * 8) {
       float fg[8], fq[8], fm[8], fv[8];
       load8(grad + at, fg);
       load8(q + at, fq);
@@ -545,7 +554,7 @@ __global__ void __launch_bounds__(kThreads)
     }
     done = n / 8 * 8;
   }
-  for (int at = done + threadIdx.x; at < n; at += kThreads) {
+  for (int at = done + part * kThreads + threadIdx.x; at < n; at += kUpdateParts * kThreads) {
     float fq = q[at], fm = m[at], fv = v[at];
     adam_one(load1(grad + at), fq, fm, fv, c, s);
     q[at] = fq, m[at] = fm, v[at] = fv;
@@ -564,15 +573,16 @@ cudaError_t adam_pass_n(const lf_adamw_args* a, int t0, int t1, int pass, const 
   if (nc == 0) return cudaSuccess;
   if (pass == 0) return launch(adam_norm_kernel<kN>, nc, kThreads, 0, st, false, pk, tb, a->grad_dtype, c0, part);
   const bool pdl = t0 == 0;
+  const int ctas = nc * kUpdateParts;
   const int pd = a->param_dtype, gd = a->grad_dtype;
-  if (pd == LF_F32) return launch(adam_update_kernel<float, float, kN>, nc, kThreads, 0, st, pdl, pk, tb, s, c0);
+  if (pd == LF_F32) return launch(adam_update_kernel<float, float, kN>, ctas, kThreads, 0, st, pdl, pk, tb, s, c0);
   if (pd == LF_BF16) {
     if (gd == LF_F32)
-      return launch(adam_update_kernel<__nv_bfloat16, float, kN>, nc, kThreads, 0, st, pdl, pk, tb, s, c0);
-    return launch(adam_update_kernel<__nv_bfloat16, __nv_bfloat16, kN>, nc, kThreads, 0, st, pdl, pk, tb, s, c0);
+      return launch(adam_update_kernel<__nv_bfloat16, float, kN>, ctas, kThreads, 0, st, pdl, pk, tb, s, c0);
+    return launch(adam_update_kernel<__nv_bfloat16, __nv_bfloat16, kN>, ctas, kThreads, 0, st, pdl, pk, tb, s, c0);
   }
-  if (gd == LF_F32) return launch(adam_update_kernel<__half, float, kN>, nc, kThreads, 0, st, pdl, pk, tb, s, c0);
-  return launch(adam_update_kernel<__half, __half, kN>, nc, kThreads, 0, st, pdl, pk, tb, s, c0);
+  if (gd == LF_F32) return launch(adam_update_kernel<__half, float, kN>, ctas, kThreads, 0, st, pdl, pk, tb, s, c0);
+  return launch(adam_update_kernel<__half, __half, kN>, ctas, kThreads, 0, st, pdl, pk, tb, s, c0);
 }
 
 cudaError_t adam_pass(const lf_adamw_args* a, int pass, const AdamTables& tb, const AdamState& s, double* part,
@@ -657,7 +667,7 @@ extern "C" int lf_adamw_plan(lf_adamw_tensor* tensors, int32_t n_tensors, int32_
     if (t.group < 0 || t.group >= n_groups || t.numel > 0xffffffffu - kChunk || (t.numel > 0 && t.param == 0))
       return LF_ERR_INVALID_ARG;
     const int64_t c = static_cast<int64_t>(chunks_of(t.numel));
-    if (chunks + c > 0x7fffffff) return LF_ERR_INVALID_ARG;
+    if (chunks + c > 0x7fffffff / kUpdateParts) return LF_ERR_INVALID_ARG;  // CTAs of a launch
     t.state_off = off;
     t.chunk0 = static_cast<int32_t>(chunks);
     t.n_chunks = static_cast<int32_t>(c);
