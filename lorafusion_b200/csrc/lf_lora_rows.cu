@@ -262,8 +262,8 @@ __device__ __forceinline__ void halves(float w, T& hi, T& lo) {
   lo = from_f32<T>(fabsf(w) <= 4.f ? w - to_f32(hi) : 0.f);
 }
 
-// One group of 8 rows as the second product sees it: S halves of row g (8 kSPitch from step to step), rows and factors of columns 2q, 2q + 1 (-1:
-// the group has no such row).
+// One group of 8 rows as the second product sees it: S halves of row g (8 kSPitch from step to step), rows and
+// factors of columns 2q, 2q + 1 (-1: the group has no such row).
 template <typename T>
 struct GroupRows {
   const T* hi;
@@ -1605,7 +1605,9 @@ bool rows_use_pairs(int T, int K, int N, int num_sms) {
 cudaError_t bank_load(const BankLoad& p, int dtype, int num_sms, cudaStream_t st) {
   const int64_t blocks = (static_cast<int64_t>(p.r_pad) * (static_cast<int64_t>(p.K) + p.N) + 255) / 256;
   const unsigned grid = static_cast<unsigned>(blocks < 16 * num_sms ? blocks : 16 * num_sms);
-  auto* k = dtype == LF_F32 ? bank_load_kernel<float> : dtype == LF_BF16 ? bank_load_kernel<__nv_bfloat16> : bank_load_kernel<__half>;
+  auto* k = dtype == LF_F32    ? bank_load_kernel<float>
+            : dtype == LF_BF16 ? bank_load_kernel<__nv_bfloat16>
+                               : bank_load_kernel<__half>;
   return launch(k, grid, 256, 0, st, false, p);
 }
 

@@ -126,8 +126,8 @@ PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.dtype = dtype_code(ba.scalar_type());
   if (p.dtype < 0 || la.scalar_type() != ba.scalar_type() || lb.scalar_type() != ba.scalar_type() ||
       la.device() != ba.device() || lb.device() != ba.device() || la.dim() != 2 || lb.dim() != 2 ||
-      (la.size(1) > 1 && la.stride(1) != 1) || (lb.size(1) > 1 && lb.stride(1) != 1) || la.size(0) > ba.size(1) || la.size(1) != ba.size(2) || lb.size(0) != bb.size(2) ||
-      lb.size(1) != la.size(0) || slot < 0 || slot >= ba.size(0))
+      (la.size(1) > 1 && la.stride(1) != 1) || (lb.size(1) > 1 && lb.stride(1) != 1) || la.size(0) > ba.size(1) ||
+      la.size(1) != ba.size(2) || lb.size(0) != bb.size(2) || lb.size(1) != la.size(0) || slot < 0 || slot >= ba.size(0))
     Py_RETURN_NONE;
   p.K = static_cast<int32_t>(ba.size(2));
   p.N = static_cast<int32_t>(bb.size(2));

@@ -53,8 +53,8 @@ class AdapterBank:
             raise ValueError(f"in_features and out_features must be 1 .. {1 << 24}, got {in_features}, {out_features}")
         self.r_pad = next(r for r in (16, 32, 64, nat.BANK_MAX_RANK) if max_rank <= r)
         if n_slots * (self.r_pad // 16) * max(out_features, 16) >= 1 << 31:
-            raise ValueError(f"{n_slots} slots of rank {self.r_pad} and {out_features} features are too many for one bank: "
-                             "n_slots * padded rank / 16 * out_features must stay below 2**31")
+            raise ValueError(f"{n_slots} slots of rank {self.r_pad} and {out_features} features are too many for one "
+                             "bank: n_slots * padded rank / 16 * out_features must stay below 2**31")
         if device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
         self.n_slots, self.max_rank = n_slots, max_rank
@@ -105,10 +105,10 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor; it must not
     overlap ``x``, ``base_weight`` or the bank.
 
-    Two launches on the current stream of ``x``'s device, long batches (above 256 rows,
-    or 512 where the bank's padded rank is at most 32) in chunks of 8192 rows of four launches each.  bf16/f16 problems whose in_features or
-    out_features is not a multiple of 8, or whose buffers are not 16-byte aligned, run on CUDA cores
-    with a ``CudaCorePathWarning``.
+    Two launches on the current stream of ``x``'s device; long batches (above 256 rows, or 512 where the
+    bank's padded rank is at most 32) run in chunks of 8192 rows of four launches each.  bf16/f16
+    problems whose in_features or out_features is not a multiple of 8, or whose buffers are not 16-byte
+    aligned, run on CUDA cores with a ``CudaCorePathWarning``.
     """
     y = nat.glue().rows_forward(
         x, base_weight, bank.lora_a, bank.lora_b, bank.ranks, bank.scales, row_slot, out, bank.r_pad,
