@@ -40,6 +40,11 @@ PyObject* fail(int rc, const char* what) {
   return nullptr;
 }
 
+// What a kernel has written: the caches of b200_ops and autograd's check of saved tensors go by the version.
+void bump(const at::Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // rows_forward(x, weight, bank_a, bank_b, ranks, scales, row_slot, out or None, the bank's padded rank, its output
 // features): the call of fused_lora_forward_rows on operands that need no copy.  None otherwise.
 PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -104,7 +109,10 @@ PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor ws = at::detail::empty_cuda({static_cast<int64_t>(bytes)}, at::kByte, dev, std::nullopt);
   const int rc = lf_rows_forward(&p, yp, ws.data_ptr(), bytes, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
   if (rc != LF_OK) return fail(rc, "lf_rows_forward");
-  if (a[7] != Py_None) return Py_NewRef(a[7]);
+  if (a[7] != Py_None) {
+    bump(y);
+    return Py_NewRef(a[7]);
+  }
   return THPVariable_Wrap(std::move(y));
 }
 
@@ -147,10 +155,6 @@ PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int rc = lf_bank_load(&p, c10::cuda::getCurrentCUDAStream(ba.device().index()).stream());
   if (rc != LF_OK) return fail(rc, "lf_bank_load");
   Py_RETURN_TRUE;
-}
-
-void bump(const at::Tensor& t) {
-  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
 }
 
 // clip(grads, per_adapter, inf_norm, max_norm or None): norms of clip_adapter_grads, or None.

@@ -169,5 +169,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     with nat.on_device(device.index):
         rc = L.lf_rows_forward(p, out.data_ptr(), ws.data_ptr(), ws.numel(), nat.raw_stream(device.index))
     nat.check(rc, "lf_rows_forward")
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     b200_ops._last_launches = _launches(T, bank.r_pad, tensor_cores)
     return out

@@ -369,3 +369,37 @@ def test_a_single_slot_and_a_single_feature_block():
     x, w, bank, adapters, _ = make(F16, T, K, N, [7], 8)
     slots = torch.zeros(T, dtype=torch.int32, device="cuda")
     check(fused_lora_forward_rows(x, w, bank, slots), x, w, adapters, slots)
+
+
+@pytest.mark.parametrize("T", [40, 1100])
+def test_an_output_buffer_advances_its_version(T):
+    x, w, bank, _, slots = make(BF16, T, 256, 264, [16, 4], 16)
+    out = torch.empty(T, 264, dtype=BF16, device="cuda")
+    odd = torch.zeros(T, 259, dtype=BF16, device="cuda")[:, :256]  # needs a dense copy: checked in Python
+    odd.copy_(x)
+    for rows in (x, odd):
+        before = out._version
+        assert fused_lora_forward_rows(rows, w, bank, slots, out=out) is out
+        assert out._version == before + 1
+    with torch.inference_mode():  # such tensors have no version
+        fused_lora_forward_rows(x, w, bank, slots, out=torch.empty_like(out))
+        fused_lora_forward_rows(odd, w, bank, slots, out=torch.empty_like(out))
+
+
+def test_packed_backward_after_its_input_was_overwritten_by_rows():
+    """The packed backward may keep x A^T of a forward only while x holds what that forward read."""
+    from lorafusion_b200.config import AdapterSpec, TileRoute, TileRoutingConfig
+    T, K = 200, 256
+    x, w, bank, adapters, slots = make(BF16, T, K, K, [16, 8], 16)
+    lora_a, lora_b = ({i: ad[k] for i, ad in enumerate(adapters)} for k in (0, 1))
+    specs = {i: AdapterSpec(i, a.shape[0], 2.0 * a.shape[0], K, K) for i, a in lora_a.items()}
+    routing = TileRoutingConfig(128, [TileRoute(0, 90, 0), TileRoute(90, T, 1)])
+    g = torch.randn(T, K, device="cuda").to(BF16)
+    buf = torch.randn(T, K, device="cuda").to(BF16)
+    b200_ops.fused_lora_forward(buf, w, lora_a, lora_b, specs, routing)
+    fused_lora_forward_rows(x, w, bank, slots, out=buf)
+    _, got_a, got_b = b200_ops.fused_lora_backward(g, buf, w, lora_a, lora_b, specs, routing)
+    _, want_a, want_b = b200_ops.fused_lora_backward(g, buf.clone(), w, lora_a, lora_b, specs, routing)
+    for got, want in ((got_a, want_a), (got_b, want_b)):
+        # both compute S anew: one in the backward's own launches, so the same bits
+        assert all(torch.equal(got[i], want[i]) for i in want)
