@@ -154,6 +154,7 @@ PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::cuda::OptionalCUDAGuard guard(ba.device());
   const int rc = lf_bank_load(&p, c10::cuda::getCurrentCUDAStream(ba.device().index()).stream());
   if (rc != LF_OK) return fail(rc, "lf_bank_load");
+  for (int i = 0; i < 4; ++i) bump(*t[i]);
   Py_RETURN_TRUE;
 }
 

@@ -403,3 +403,29 @@ def test_packed_backward_after_its_input_was_overwritten_by_rows():
     for got, want in ((got_a, want_a), (got_b, want_b)):
         # both compute S anew: one in the backward's own launches, so the same bits
         assert all(torch.equal(got[i], want[i]) for i in want)
+
+
+def test_load_and_unload_advance_the_versions_of_the_bank():
+    _, _, bank, adapters, _ = make(BF16, 4, 64, 64, [16, 16], 16)
+    tensors = (bank.lora_a, bank.lora_b, bank.ranks, bank.scales)
+    for a in (adapters[0][0], adapters[0][0].float()):  # as it is, and converted first
+        before = [t._version for t in tensors]
+        bank.load(1, a, adapters[0][1], 1.0)
+        assert [t._version for t in tensors] == [v + 1 for v in before]
+    before = bank.ranks._version
+    bank.unload(1)
+    assert bank.ranks._version > before
+
+
+def test_packed_forward_with_a_view_of_the_bank_follows_a_load():
+    """The packed operator keeps packed copies of weights whose version has not changed."""
+    from lorafusion_b200.config import AdapterSpec, TileRoute, TileRoutingConfig
+    T, K = 64, 128
+    x, w, bank, adapters, _ = make(BF16, T, K, K, [16, 16], 16)
+    view = bank.lora_a[0]
+    b, specs = {0: adapters[0][1]}, {0: AdapterSpec(0, 16, 16.0, K, K)}
+    routing = TileRoutingConfig(64, [TileRoute(0, T, 0)])
+    b200_ops.fused_lora_forward(x, w, {0: view}, b, specs, routing)
+    bank.load(0, 4 * adapters[1][0], adapters[1][1], 1.0)
+    got = b200_ops.fused_lora_forward(x, w, {0: view}, b, specs, routing)
+    assert torch.equal(got, b200_ops.fused_lora_forward(x, w, {0: view.clone()}, b, specs, routing))
