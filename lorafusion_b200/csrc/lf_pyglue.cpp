@@ -293,7 +293,7 @@ struct Buffer {  // a contiguous buffer for the length of a call
 
 // adamw_step(weights, addresses, records, device records, chunks, hyper, steps, exp_avg, exp_avg_sq, master or None,
 // n_chunks, n_groups, workspace bytes, (beta1, beta2), eps, max_norm or None, skip_nonfinite, dtype codes of the
-// weights and the gradients): lf_adamw_step, and the version counter of every weight that has a gradient.
+// weights and the gradients): lf_adamw_step, and the version counters of the state and of every weight that has a gradient.
 // Returns the norms, or None when neither clipping nor skip_nonfinite asks for them.
 PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 19 || !PyList_CheckExact(a[0]) || !PyTuple_CheckExact(a[13]) || PyTuple_GET_SIZE(a[13]) != 2) {
@@ -362,6 +362,8 @@ PyObject* adamw_step(PyObject*, PyObject* const* a, Py_ssize_t n) {
     PyObject* o = PyList_GET_ITEM(a[0], i);
     if (p.grads[i] && THPVariable_Check(o)) bump(THPVariable_Unpack(o));
   }
+  for (int i = 3; i < 7; ++i)  // steps, both moments, masters
+    if (t[i]) bump(*t[i]);
   if (!norms.defined()) Py_RETURN_NONE;
   return THPVariable_Wrap(std::move(norms));
 }

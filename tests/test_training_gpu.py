@@ -376,3 +376,20 @@ def test_train_then_serve():
         want[lo:hi] += 2.0 * (x[lo:hi].double() @ lora_a[i].double().T) @ lora_b[i].double().T
     for got in (served, y):
         torch.testing.assert_close(got.double(), want, rtol=2e-2, atol=2e-2)
+
+
+def test_a_step_advances_the_versions_of_its_state():
+    """Float32 masters used as weights of the packed operator, which keeps packed copies by version."""
+    from lorafusion_b200.config import AdapterSpec, TileRoute, TileRoutingConfig
+    K = 64
+    opt = AdapterAdamW(make_params(BF16, [(K, K)], {0: 8}), lr=0.1)
+    a, b = ({0: opt.state(0)[j]["master"]} for j in (0, 1))
+    x, w = torch.randn(16, K, device="cuda"), torch.randn(K, K, device="cuda")
+    forward = lambda a, b: b200_ops.fused_lora_forward(  # noqa: E731
+        x, w, a, b, {0: AdapterSpec(0, 8, 8.0, K, K)}, TileRoutingConfig(64, [TileRoute(0, 16, 0)]))
+    forward(a, b)
+    state = (opt.exp_avg, opt.exp_avg_sq, opt.master, opt.steps)
+    before = [t._version for t in state]
+    opt.step(make_grads(F32, [(K, K)], {0: 8}))
+    assert all(t._version > v for t, v in zip(state, before))
+    assert torch.equal(forward(a, b), forward({0: a[0].clone()}, {0: b[0].clone()}))
