@@ -221,6 +221,7 @@ class AdapterAdamW:
         off = int(self._rec["state_off"][k])
         return flat[off:off + self._tensors[k].numel()].view(self._shapes[k])
 
+    @torch.no_grad()
     def refresh_masters(self) -> None:
         """Take the float32 masters from the weights as they are now (16-bit weights only)."""
         if self.master is not None:
@@ -241,6 +242,7 @@ class AdapterAdamW:
                 "master": None if self.master is None else self.master.clone(), "steps": self.steps.clone(),
                 "hyper": self._hyper.tolist()}
 
+    @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
         """Restore ``state_dict()`` of an optimizer over the same adapters and shapes; 16-bit weights are
         rounded from the restored masters."""
@@ -259,8 +261,7 @@ class AdapterAdamW:
         if self.master is not None:
             self.master.copy_(state["master"])
             masters = [self._block(self.master, k) for k in range(len(self._tensors))]
-            with torch.no_grad():
-                torch._foreach_copy_(self._tensors, masters)
+            torch._foreach_copy_(self._tensors, masters)
 
     def step(self, grads: Sequence[Mapping]) -> torch.Tensor | None:
         """One update; returns each adapter's gradient norm before clipping (float32, in the order of

@@ -393,3 +393,23 @@ def test_a_step_advances_the_versions_of_its_state():
     opt.step(make_grads(F32, [(K, K)], {0: 8}))
     assert all(t._version > v for t, v in zip(state, before))
     assert torch.equal(forward(a, b), forward({0: a[0].clone()}, {0: b[0].clone()}))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_weights_that_require_gradients_leave_no_graph_in_the_state(dtype):
+    import copy
+    layers, ranks = [(64, 48)], {0: 4, 1: 8}
+    params = [{i: torch.nn.Parameter(t) for i, t in d.items()} for d in make_params(dtype, layers, ranks)]
+    opt = AdapterAdamW(params, lr=1e-2, max_norm=1.0)
+    grads = make_grads(dtype, layers, ranks)
+    for k in range(2):
+        Adam64(opt).step_and_check(grads)
+        saved = copy.deepcopy(opt.state_dict())
+        opt.refresh_masters()
+        opt.load_state_dict(saved)
+        for t in (opt.exp_avg, opt.exp_avg_sq) + (() if opt.master is None else (opt.master,)):
+            assert not t.requires_grad and t.grad_fn is None
+        assert all(p.requires_grad and p.is_leaf for d in params for p in d.values())
+    reader = opt.state(0)[0]["exp_avg"] * torch.ones(1, device="cuda", requires_grad=True)
+    opt.load_state_dict({k: v.requires_grad_() if k == "exp_avg" else v for k, v in opt.state_dict().items()})
+    assert not opt.exp_avg.requires_grad and reader.requires_grad
