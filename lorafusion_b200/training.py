@@ -237,22 +237,30 @@ class AdapterAdamW:
                 for k, (j, aid) in enumerate(self._names) if aid == adapter_id}
 
     def state_dict(self) -> dict:
-        """Copies of the state, step counts and hyperparameters (``load_state_dict`` takes them back)."""
-        return {"ids": list(self.ids), "exp_avg": self.exp_avg.clone(), "exp_avg_sq": self.exp_avg_sq.clone(),
-                "master": None if self.master is None else self.master.clone(), "steps": self.steps.clone(),
-                "hyper": self._hyper.tolist()}
+        """Copies of the state, step counts and hyperparameters (``load_state_dict`` takes them back), and
+        ``layout``: dict index, adapter id and shape of the weight of each block, in the state's order."""
+        return {"ids": list(self.ids), "layout": self._layout(), "exp_avg": self.exp_avg.clone(),
+                "exp_avg_sq": self.exp_avg_sq.clone(), "master": None if self.master is None else self.master.clone(),
+                "steps": self.steps.clone(), "hyper": self._hyper.tolist()}
+
+    def _layout(self) -> list:
+        return [(j, aid, tuple(shape)) for (j, aid), shape in zip(self._names, self._shapes)]
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
-        """Restore ``state_dict()`` of an optimizer over the same adapters and shapes; 16-bit weights are
-        rounded from the restored masters."""
-        same = (state["ids"] == self.ids and state["exp_avg"].shape == self.exp_avg.shape
+        """Restore ``state_dict()`` of an optimizer over the same adapters and shapes in the same order;
+        16-bit weights are rounded from the restored masters.  A state of another layout is refused before anything
+        is written; so is one without a ``layout`` (its blocks could belong to other weights)."""
+        if "layout" not in state:
+            raise ValueError("the state has no record of the weights its blocks belong to (\"layout\")")
+        same = (state["ids"] == self.ids and [(j, aid, tuple(s)) for j, aid, s in state["layout"]] == self._layout()
+                and state["exp_avg"].shape == self.exp_avg.shape
                 and state["exp_avg_sq"].shape == self.exp_avg_sq.shape and state["steps"].shape == self.steps.shape
                 and (state["master"] is None) == (self.master is None)
                 and (self.master is None or state["master"].shape == self.master.shape)
                 and np.shape(state["hyper"]) == self._hyper.shape)
         if not same:
-            raise ValueError("the state belongs to other adapters, shapes or weight types")
+            raise ValueError("the state belongs to other adapters, shapes, weight types or another order of them")
         self.exp_avg.copy_(state["exp_avg"])
         self.exp_avg_sq.copy_(state["exp_avg_sq"])
         self.steps.copy_(state["steps"])

@@ -413,3 +413,28 @@ def test_weights_that_require_gradients_leave_no_graph_in_the_state(dtype):
     reader = opt.state(0)[0]["exp_avg"] * torch.ones(1, device="cuda", requires_grad=True)
     opt.load_state_dict({k: v.requires_grad_() if k == "exp_avg" else v for k, v in opt.state_dict().items()})
     assert not opt.exp_avg.requires_grad and reader.requires_grad
+
+
+def test_state_of_another_layout_is_refused():
+    """The same adapters and totals in another order: loading would give every block to another weight."""
+    ranks = {0: 4, 1: 8}
+    (a, b), (c, d) = (make_params(BF16, [shape], ranks, seed=k) for k, shape in enumerate([(64, 48), (48, 64)]))
+    opt = AdapterAdamW([a, b], lr=1e-2)
+    opt.step(make_grads(F32, [(64, 48)], ranks))
+    saved = opt.state_dict()
+    for params in ([c, d],                                   # [r, 48] and [64, r]: equal totals
+                   [{i: t.view(64, -1) for i, t in a.items()}, b], [a, {1: b[1], 0: b[0]}]):
+        other = AdapterAdamW([{i: t.clone() for i, t in p.items()} for p in params], lr=1e-2)
+        assert other.ids == opt.ids and other.exp_avg.shape == opt.exp_avg.shape
+        kept = [t.clone() for t in (other.exp_avg, other.master, other.steps)]
+        weights = [t.clone() for p in other.params for t in p.values()]
+        with pytest.raises(ValueError):
+            other.load_state_dict(saved)
+        assert all(torch.equal(t, k) for t, k in zip((other.exp_avg, other.master, other.steps), kept))
+        assert all(torch.equal(t, k) for t, k in zip([t for p in other.params for t in p.values()], weights))
+    twin = AdapterAdamW([a, b], lr=1e-2)
+    with pytest.raises(ValueError):
+        twin.load_state_dict({k: v for k, v in saved.items() if k != "layout"})
+    assert not twin.exp_avg.any()
+    twin.load_state_dict({**saved, "layout": [[j, aid, list(s)] for j, aid, s in saved["layout"]]})  # as JSON has it
+    assert torch.equal(twin.exp_avg, opt.exp_avg) and torch.equal(twin.steps, opt.steps)
