@@ -151,14 +151,10 @@ class AdapterAdamW:
             raise ValueError(f"weights must share one dtype (float32, bfloat16, float16), got {dtypes}")
         if not all(map(_CONTIGUOUS, self._tensors)):
             raise ValueError("weights must be contiguous")
-        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or not eps >= 0.0:
-            raise ValueError(f"betas must be in [0, 1) and eps non-negative, got {betas}, {eps}")
-        if max_norm is not None and not max_norm >= 0.0:
-            raise ValueError(f"max_norm must be non-negative, got {max_norm}")
+        common = self._common_hyper(betas, eps, max_norm, skip_nonfinite)
         self.device = torch.device("cuda", index)
         self.dtype = dtypes.pop()
-        self.betas, self.eps = (float(betas[0]), float(betas[1])), float(eps)
-        self.max_norm, self.skip_nonfinite = max_norm, skip_nonfinite
+        self.betas, self.eps, self.max_norm, self.skip_nonfinite = common
         self.ids = list(dict.fromkeys(aid for _, aid in self._names))
         self._group = {aid: i for i, aid in enumerate(self.ids)}
         self._hyper = np.empty((len(self.ids), 2))
@@ -208,6 +204,15 @@ class AdapterAdamW:
             raise ValueError(f"{name} must be finite and non-negative, got {value}")
         return value
 
+    @staticmethod
+    def _common_hyper(betas, eps, max_norm, skip_nonfinite):
+        """(betas, eps, max_norm, skip_nonfinite), checked."""
+        if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0) or not eps >= 0.0:
+            raise ValueError(f"betas must be in [0, 1) and eps non-negative, got {betas}, {eps}")
+        if max_norm is not None and not max_norm >= 0.0:
+            raise ValueError(f"max_norm must be non-negative, got {max_norm}")
+        return (float(betas[0]), float(betas[1])), float(eps), max_norm, bool(skip_nonfinite)
+
     def set_adapter(self, adapter_id, *, lr: float | None = None, weight_decay: float | None = None) -> None:
         """Change one adapter's learning rate or decay, from the next step on."""
         row = self._hyper[self._group[adapter_id]]
@@ -241,15 +246,16 @@ class AdapterAdamW:
         ``layout``: dict index, adapter id and shape of the weight of each block, in the state's order."""
         return {"ids": list(self.ids), "layout": self._layout(), "exp_avg": self.exp_avg.clone(),
                 "exp_avg_sq": self.exp_avg_sq.clone(), "master": None if self.master is None else self.master.clone(),
-                "steps": self.steps.clone(), "hyper": self._hyper.tolist()}
+                "steps": self.steps.clone(), "hyper": self._hyper.tolist(), "betas": self.betas, "eps": self.eps,
+                "max_norm": self.max_norm, "skip_nonfinite": self.skip_nonfinite}
 
     def _layout(self) -> list:
         return [(j, aid, tuple(shape)) for (j, aid), shape in zip(self._names, self._shapes)]
 
     @torch.no_grad()
     def load_state_dict(self, state: dict) -> None:
-        """Restore ``state_dict()`` of an optimizer over the same adapters and shapes in the same order;
-        16-bit weights are rounded from the restored masters.  A state of another layout is refused before anything
+        """Restore ``state_dict()`` of an optimizer over the same adapters and shapes in the same order, with
+        its hyperparameters; 16-bit weights are rounded from the restored masters.  A state of another layout is refused before anything
         is written; so is one without a ``layout`` (its blocks could belong to other weights)."""
         if "layout" not in state:
             raise ValueError("the state has no record of the weights its blocks belong to (\"layout\")")
@@ -261,10 +267,14 @@ class AdapterAdamW:
                 and np.shape(state["hyper"]) == self._hyper.shape)
         if not same:
             raise ValueError("the state belongs to other adapters, shapes, weight types or another order of them")
+        hyper = [[self._hyper_value(name, v) for name, v in zip(("lr", "weight_decay"), row)] for row in state["hyper"]]
+        common = self._common_hyper(*(state.get(name, getattr(self, name))
+                                      for name in ("betas", "eps", "max_norm", "skip_nonfinite")))
+        self.betas, self.eps, self.max_norm, self.skip_nonfinite = common
         self.exp_avg.copy_(state["exp_avg"])
         self.exp_avg_sq.copy_(state["exp_avg_sq"])
         self.steps.copy_(state["steps"])
-        self._hyper[:] = state["hyper"]
+        self._hyper[:] = hyper
         self._hyper_changed = True
         if self.master is not None:
             self.master.copy_(state["master"])

@@ -438,3 +438,23 @@ def test_state_of_another_layout_is_refused():
     assert not twin.exp_avg.any()
     twin.load_state_dict({**saved, "layout": [[j, aid, list(s)] for j, aid, s in saved["layout"]]})  # as JSON has it
     assert torch.equal(twin.exp_avg, opt.exp_avg) and torch.equal(twin.steps, opt.steps)
+
+
+def test_state_carries_every_hyperparameter():
+    layers, ranks = [(65, 31)], {0: 4, 7: 3}
+    one = AdapterAdamW(make_params(BF16, layers, ranks), lr=1e-2, weight_decay=0.1, betas=(0.8, 0.97), eps=1e-5,
+                       max_norm=0.5, skip_nonfinite=True)
+    two = AdapterAdamW(make_params(BF16, layers, ranks))
+    one.step(make_grads(F32, layers, ranks))
+    saved = one.state_dict()
+    for bad in (dict(betas=(1.0, 0.9)), dict(eps=-1.0), dict(max_norm=-1.0), dict(hyper=[[-1.0, 0.0]] * 2),
+                dict(hyper=[[1.0, float("nan")]] * 2)):
+        with pytest.raises(ValueError):
+            two.load_state_dict({**saved, **bad})
+    assert not two.exp_avg.any() and two.betas == (0.9, 0.999) and two.max_norm is None
+    two.load_state_dict(saved)
+    grads = make_grads(F32, layers, ranks, seed=4)
+    grads[0][7][0, 0] = float("inf")
+    norms = [opt.step(grads) for opt in (one, two)]
+    assert torch.equal(*norms) and one.steps.tolist() == two.steps.tolist() == [2, 1]
+    assert torch.equal(one.exp_avg, two.exp_avg) and torch.equal(one.master, two.master)
