@@ -216,10 +216,8 @@ class AdapterAdamW:
     def set_adapter(self, adapter_id, *, lr: float | None = None, weight_decay: float | None = None) -> None:
         """Change one adapter's learning rate or decay, from the next step on."""
         row = self._hyper[self._group[adapter_id]]
-        if lr is not None:
-            row[0] = self._hyper_value("lr", lr)
-        if weight_decay is not None:
-            row[1] = self._hyper_value("weight_decay", weight_decay)
+        row[:] = (row[0] if lr is None else self._hyper_value("lr", lr),
+                  row[1] if weight_decay is None else self._hyper_value("weight_decay", weight_decay))
         self._hyper_changed = True
 
     def _block(self, flat: torch.Tensor, k: int) -> torch.Tensor:

@@ -458,3 +458,16 @@ def test_state_carries_every_hyperparameter():
     norms = [opt.step(grads) for opt in (one, two)]
     assert torch.equal(*norms) and one.steps.tolist() == two.steps.tolist() == [2, 1]
     assert torch.equal(one.exp_avg, two.exp_avg) and torch.equal(one.master, two.master)
+
+
+def test_set_adapter_writes_both_values_or_none():
+    opt = AdapterAdamW(make_params(F32, [(16, 16)], {0: 4, 1: 4}), lr=1e-3, weight_decay=0.1)
+    for kw in (dict(lr=0.5, weight_decay=-1.0), dict(lr=float("inf"), weight_decay=0.2), dict(lr=0.5, weight_decay="x")):
+        with pytest.raises(ValueError):
+            opt.set_adapter(1, **kw)
+        assert opt.state_dict()["hyper"] == [[1e-3, 0.1], [1e-3, 0.1]]
+    with pytest.raises(KeyError):
+        opt.set_adapter(2, lr=0.5)
+    opt.set_adapter(1, weight_decay=0.0)
+    opt.set_adapter(0, lr=0.0)
+    assert opt.state_dict()["hyper"] == [[0.0, 0.1], [1e-3, 0.0]]
