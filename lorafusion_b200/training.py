@@ -297,9 +297,12 @@ class AdapterAdamW:
         if code < 0:
             return self._no_gradients()
         if self._hyper_changed:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdapterAdamW.step cannot be captured into a CUDA graph")
-            self._hyper_dev.copy_(torch.from_numpy(self._hyper))
+            with nat.on_device(self.device.index):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdapterAdamW.step cannot be captured into a CUDA graph")
+                # a pinned copy of its own for each upload: the allocator hands it out again only after the copy, and
+                # the host waits for nothing that is queued (from pageable memory it waits for all of it)
+                self._hyper_dev.copy_(torch.from_numpy(self._hyper).pin_memory(), non_blocking=True)
             self._hyper_changed = False
         return nat.glue().adamw_step(
             self._tensors, ptrs, self._rec, self._rec_dev, self._chunk_dev, self._hyper_dev, self.steps, self.exp_avg,

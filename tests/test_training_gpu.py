@@ -471,3 +471,30 @@ def test_set_adapter_writes_both_values_or_none():
     opt.set_adapter(1, weight_decay=0.0)
     opt.set_adapter(0, lr=0.0)
     assert opt.state_dict()["hyper"] == [[0.0, 0.1], [1e-3, 0.0]]
+
+
+def test_a_step_with_new_rates_does_not_wait_for_the_queue():
+    """Every step gets rates of its own while the stream is busy: the host runs ahead, no upload overtakes another."""
+    layers, ranks = [(64, 48)], {0: 4, 1: 8}
+    ahead, behind = (AdapterAdamW(make_params(BF16, layers, ranks)) for _ in range(2))
+    grads = [make_grads(F32, layers, ranks, seed=k) for k in range(8)]
+
+    def steps(opt, wait):
+        for k, g in enumerate(grads):
+            opt.set_adapter(k % 2, lr=1e-3 * (k + 1), weight_decay=0.1 * (k % 3))
+            opt.step(g)
+            if wait:
+                torch.cuda.synchronize()
+
+    start = {k: v.clone() if torch.is_tensor(v) else v for k, v in ahead.state_dict().items()}
+    steps(behind, True)
+    steps(ahead, False)  # the pinned buffers and the launches' first use
+    ahead.load_state_dict(start)
+    torch.cuda.synchronize()
+    done = torch.cuda.Event()
+    torch.cuda._sleep(2_000_000_000)  # about a second
+    done.record()
+    steps(ahead, False)
+    assert not done.query()
+    assert torch.equal(ahead.master, behind.master) and torch.equal(ahead.exp_avg_sq, behind.exp_avg_sq)
+    assert ahead.state_dict()["hyper"] == behind.state_dict()["hyper"]
