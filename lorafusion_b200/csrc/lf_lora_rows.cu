@@ -15,9 +15,10 @@
 //                the CTA-pair GEMM of lf_tc.cu where its tiles fit better.
 // Any order of rows works and no host plan is needed: the adapters are read on the device.
 //
-// S enters the second product as hi + lo halves of the input type after a per-row power-of-two scaling (the
-// row's largest magnitude becomes 1..2), so it is exact to about 2^-16 (bf16) or 2^-22 (f16)
-// relative and a float16 S cannot overflow.  All sums are float32.
+// S enters the second product as hi + lo halves of the input type after a per-row power-of-two scaling, so it is exact
+// to about 2^-16 (bf16) or 2^-22 (f16) relative and a float16 S cannot overflow.  The row's largest magnitude becomes
+// 1..2 (bf16) or 2^13..2^14 (f16, whose low halves of smaller values would leave its normal range otherwise: 2^-22
+// then holds down to 2^-15 of the largest, 2^-37 of the largest below).  All sums are float32.
 //
 // Measured (replayed graph, weights from HBM; the shared projection alone by cuBLAS in brackets): 1 row 4096 -> 4096, rank 16
 // 12.7 us (12.9); 64 rows of 56 adapters, ranks 8 to 64, 4096 -> 14336 42 us (23); 250 rows of 219 adapters
@@ -27,6 +28,7 @@
 #include <cuda_fp16.h>
 
 #include <mutex>
+#include <type_traits>
 
 #include "lf_internal.cuh"
 #include "lf_launch.cuh"
@@ -251,15 +253,19 @@ __device__ __forceinline__ int group_rows(const RowsArgs& p, int t0, int rows, b
   return n_groups;
 }
 
-// 2^ex with the largest of a row's values over 1..2; 0 for a row that is all zero or not finite.
+// A row's values are divided by 2^ex, which brings the largest to 2^kTop .. 2^(kTop + 1); 0 for a row that is all zero
+// or not finite.
+template <typename T>
+constexpr int kTop = std::is_same<T, __half>::value ? 13 : 0;
+template <typename T>
 __device__ __forceinline__ int row_exponent(float top) {
-  return top > 0.f && top <= 3.402823466e38f ? max(-126, min(126, ilogbf(top))) : 0;
+  return top > 0.f && top <= 3.402823466e38f ? max(-126, min(126, ilogbf(top) - kTop<T>)) : 0;
 }
 // v scaled, as high and low halves; the high half of a value that is not finite says it all
 template <typename T>
 __device__ __forceinline__ void halves(float w, T& hi, T& lo) {
   hi = from_f32<T>(w);
-  lo = from_f32<T>(fabsf(w) <= 4.f ? w - to_f32(hi) : 0.f);
+  lo = from_f32<T>(fabsf(w) <= static_cast<float>(4 << kTop<T>) ? w - to_f32(hi) : 0.f);
 }
 
 // One group of 8 rows as the second product sees it: S halves of row g (8 kSPitch from step to step), rows and
@@ -490,7 +496,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
         }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        const int ex = row_exponent(top);
+        const int ex = row_exponent<T>(top);
         const float down = scalbnf(1.f, -ex), fac = p.slot_scale[slot_of(e)] * scalbnf(1.f, ex);
         if (lane < 8) s_fac[u][lane] = fac;
 #pragma unroll
@@ -1064,7 +1070,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
         }
       }
       for (int o = 1; o < 2 * ks; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      const int ex = row_exponent(top);
+      const int ex = row_exponent<T>(top);
       const float down = scalbnf(1.f, -ex);
       if (row < tile.rows) {
         if (sub == 0) p.factor[to] = p.slot_scale[slot] * scalbnf(1.f, ex);

@@ -429,3 +429,36 @@ def test_packed_forward_with_a_view_of_the_bank_follows_a_load():
     bank.load(0, 4 * adapters[1][0], adapters[1][1], 1.0)
     got = b200_ops.fused_lora_forward(x, w, {0: view}, b, specs, routing)
     assert torch.equal(got, b200_ops.fused_lora_forward(x, w, {0: view.clone()}, b, specs, routing))
+
+
+def whole_numbers(*shape, most):
+    return torch.randint(-most, most + 1, shape, device="cuda").float()
+
+
+def one_adapter(dtype, T, w, a, b, s=1.0):
+    """(a bank that holds it, slots that name it); W beside it."""
+    bank = AdapterBank(1, a.shape[0], a.shape[1], w.shape[0], dtype, "cuda")
+    bank.load(0, a, b, s)
+    return bank, torch.zeros(T, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("T", [3, 200, 1500])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_small_and_large_rank_products_in_one_row(T, dtype):
+    """One S 2^-18 of the other, which B takes no part of.  S is exact (sums of whole numbers times powers of two), so
+    the bound is: two halves of S (2^-16 or 2^-22 of it, and 2^-35 of the row's largest), the float32 sums, one
+    rounding."""
+    K, N = 64, 136
+    x = whole_numbers(T, K, most=4).to(dtype)
+    a = whole_numbers(2, K, most=4) * torch.tensor([[2.0 ** 6], [2.0 ** -12]], device="cuda")
+    a, b = a.to(dtype), torch.zeros(N, 2, dtype=dtype, device="cuda")
+    b[:, 1] = 4 * torch.randn(N, device="cuda")
+    w = torch.zeros(N, K, dtype=dtype, device="cuda")
+    bank, slots = one_adapter(dtype, T, w, a, b)
+    S = x.double() @ a.double().T
+    want = S @ b.double().T
+    off = (2.0 ** -16 if dtype is BF16 else 2.0 ** -22) * S.abs() + 2.0 ** -35 * S.abs().amax(1, keepdim=True)
+    bound = off @ b.double().abs().T + (torch.finfo(dtype).eps / 2 + 200 * 2.0 ** -23) * want.abs()
+    bound += torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
+    got = fused_lora_forward_rows(x, w, bank, slots).double()
+    assert ((got - want).abs() <= bound).all()
