@@ -253,13 +253,16 @@ __device__ __forceinline__ int group_rows(const RowsArgs& p, int t0, int rows, b
   return n_groups;
 }
 
-// A row's values are divided by 2^ex, which brings the largest to 2^kTop .. 2^(kTop + 1); 0 for a row that is all zero
-// or not finite.
+// A row's values are divided by 2^ex, which brings the largest finite one to 2^kTop .. 2^(kTop + 1); 0 for a row that
+// has none but zeros.  (Values that are not finite stay so, and must not take the others out of T's range.)
 template <typename T>
 constexpr int kTop = std::is_same<T, __half>::value ? 13 : 0;
 template <typename T>
 __device__ __forceinline__ int row_exponent(float top) {
-  return top > 0.f && top <= 3.402823466e38f ? max(-126, min(126, ilogbf(top) - kTop<T>)) : 0;
+  return top > 0.f ? max(-126, min(126, ilogbf(top) - kTop<T>)) : 0;
+}
+__device__ __forceinline__ float larger_finite(float top, float v) {
+  return fabsf(v) <= 3.402823466e38f ? fmaxf(top, fabsf(v)) : top;
 }
 // v scaled, as high and low halves; the high half of a value that is not finite says it all
 template <typename T>
@@ -490,10 +493,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
 #pragma unroll
         for (int i = 0; i < kRP / 4; ++i) v[i] = (lane >> 3) + 4 * i < rank ? s_sum[slot_at][lane + 32 * i] : 0.f;
 #pragma unroll
-        for (int i = 0; i < kRP / 4; ++i) {
-          top = fmaxf(top, fabsf(v[i]));
-          if (!(fabsf(v[i]) <= 3.402823466e38f)) top = __int_as_float(0x7f800000);
-        }
+        for (int i = 0; i < kRP / 4; ++i) top = larger_finite(top, v[i]);
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
         const int ex = row_exponent<T>(top);
@@ -1064,8 +1064,7 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             if (j0 + j >= rank) v[c][j] = 0.f;  // columns past the rank: zero times x, which may not be finite
-            top = fmaxf(top, fabsf(v[c][j]));
-            if (!(fabsf(v[c][j]) <= 3.402823466e38f)) top = __int_as_float(0x7f800000);
+            top = larger_finite(top, v[c][j]);
           }
         }
       }

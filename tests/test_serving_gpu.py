@@ -462,3 +462,32 @@ def test_small_and_large_rank_products_in_one_row(T, dtype):
     bound += torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps
     got = fused_lora_forward_rows(x, w, bank, slots).double()
     assert ((got - want).abs() <= bound).all()
+
+
+def check_not_finite(y, x, a, b, s=1.0):
+    """Infinities and NaN of y where the formula (in 64 bits, term by term) has them."""
+    S = (x.double()[:, None] * a.double()[None]).sum(2)
+    want = s * (S[:, None] * b.double()[None]).sum(2)
+    for kind in (torch.isposinf, torch.isneginf, torch.isnan):
+        assert torch.equal(kind(y), kind(want))
+    return want
+
+
+@pytest.mark.parametrize("T", [9, 1100])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_one_infinite_rank_product(T, dtype):
+    """S of one rank is infinite, of another beyond float16's range: the infinities of the result are the first's."""
+    K, N = 64, 72
+    x = (torch.rand(T, K, device="cuda") + 0.5).to(dtype)
+    a = torch.full((3, K), 400.0, device="cuda")
+    a[1] *= -50  # S up to 2e6
+    a[0, 5] = float("inf")
+    b = torch.randn(N, 3, device="cuda")
+    b[:, 0] = torch.where(b[:, 0] < 0, -1.0, 1.0)  # x 0 would be NaN
+    a, b = a.to(dtype), b.to(dtype)
+    w = torch.zeros(N, K, dtype=dtype, device="cuda")
+    for A in (a, -a):
+        bank, slots = one_adapter(dtype, T, w, A, b, 0.5)
+        y = fused_lora_forward_rows(x, w, bank, slots)
+        want = check_not_finite(y, x, A, b, 0.5)
+        assert torch.isposinf(want).any() and torch.isneginf(want).any()
