@@ -491,3 +491,27 @@ def test_one_infinite_rank_product(T, dtype):
         y = fused_lora_forward_rows(x, w, bank, slots)
         want = check_not_finite(y, x, A, b, 0.5)
         assert torch.isposinf(want).any() and torch.isneginf(want).any()
+
+
+@pytest.mark.parametrize("T", [9, 1100])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("r", [1, 16, 40])
+def test_infinite_entries_of_b(T, dtype, r):
+    """S (whole numbers: those one half holds, those it does not, zero) times an infinite entry of B."""
+    K, N = 64, 136
+    x = whole_numbers(T, K, most=9).to(dtype)
+    x[0] = 0.0
+    x[1], x[2, 1:] = 0.0, 0.0
+    a = whole_numbers(r, K, most=9)
+    a[:, 0] = 1.0
+    x[1, 0], x[2, 0] = 1.0, -4.0  # S of one and of minus four
+    a, b = a.to(dtype), torch.randn(N, r, device="cuda").to(dtype)
+    b[::3, 0], b[1::3, r // 2], b[4, r - 1] = float("inf"), -float("inf"), float("nan")
+    w = torch.zeros(N, K, dtype=dtype, device="cuda")
+    a2 = a.clone()
+    a2[0, 0] = float("inf")  # S of rank 0 infinite (NaN where x is zero)
+    for A in (a, a2):
+        bank, slots = one_adapter(dtype, T, w, A, b, -2.0)
+        y = fused_lora_forward_rows(x, w, bank, slots)
+        want = check_not_finite(y, x, A, b, -2.0)
+        assert torch.isposinf(want).any() and torch.isneginf(want).any()
