@@ -264,33 +264,28 @@ __device__ __forceinline__ int row_exponent(float top) {
 __device__ __forceinline__ float larger_finite(float top, float v) {
   return fabsf(v) <= 3.402823466e38f ? fmaxf(top, fabsf(v)) : top;
 }
-// w as high and low halves of one sign, of which neither is zero unless w is: both are multiplied by every entry of
+// w as high and low parts of one sign, of which neither is zero unless w is: both are multiplied by every entry of
 // B_i, and with an infinite one the sum of both products has to be the infinity that w itself would give.  So the
-// high half is rounded toward zero and, where it would hold all of w, takes one step less.  What is left is
-// exact before the low half's rounding; a half that would still be zero (w 2^-36 of the row's largest, 2^-126 for bf16)
-// gets the smallest value.
+// high part is rounded toward zero, and a w that it would hold alone becomes two equal parts (exact, and nothing
+// below half of w's last bit, so sums that were exact stay so).  A part that would still be zero (w 2^-36 of the row's
+// largest, 2^-126 for bf16) gets the smallest value.
 __device__ __forceinline__ __nv_bfloat16 toward_zero(float w, __nv_bfloat16*) { return __float2bfloat16_rz(w); }
 __device__ __forceinline__ __half toward_zero(float w, __half*) { return __float2half_rz(w); }
-__device__ __forceinline__ uint16_t bits_of(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
-__device__ __forceinline__ uint16_t bits_of(__half v) { return __half_as_ushort(v); }
-__device__ __forceinline__ __nv_bfloat16 of_bits(uint16_t b, __nv_bfloat16*) { return __ushort_as_bfloat16(b); }
-__device__ __forceinline__ __half of_bits(uint16_t b, __half*) { return __ushort_as_half(b); }
+template <typename T>
+__device__ __forceinline__ T at_least(T v, float w, float least) {
+  return w != 0.f && to_f32(v) == 0.f ? from_f32<T>(copysignf(least, w)) : v;
+}
 template <typename T>
 __device__ __forceinline__ void halves(float w, T& hi, T& lo) {
   T* const tag = nullptr;
-  // the smallest float16; the smallest normal bf16
-  const uint16_t sign = static_cast<uint16_t>(__float_as_uint(w) >> 16 & 0x8000u), least = std::is_same<T, __half>::value ? 1 : 0x80;
+  constexpr float least = std::is_same<T, __half>::value ? 5.9604644775390625e-8f : 1.175494350822287508e-38f;  // 2^-24, 2^-126
   hi = toward_zero(w, tag);
-  float rest = w - to_f32(hi);
-  if (rest == 0.f && (bits_of(hi) & 0x7fff) > least) {
-    hi = of_bits(bits_of(hi) - 1, tag);
-    rest = w - to_f32(hi);
-  }
-  lo = from_f32<T>(fabsf(w) <= 3.402823466e38f ? rest : copysignf(1.f, w));
-  if (w != 0.f) {
-    if ((bits_of(hi) & 0x7fff) == 0) hi = of_bits(sign | least, tag);
-    if ((bits_of(lo) & 0x7fff) == 0) lo = of_bits(sign | least, tag);
-  }
+  const float rest = w - to_f32(hi);
+  const bool two = !(fabsf(rest) > 0.f);  // also infinities and NaN
+  if (two) hi = toward_zero(0.5f * w, tag);
+  lo = two ? hi : from_f32<T>(rest);
+  hi = at_least(hi, w, least);
+  lo = at_least(lo, w, least);
 }
 
 // One group of 8 rows as the second product sees it: S halves of row g (8 kSPitch from step to step), rows and

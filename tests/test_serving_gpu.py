@@ -515,3 +515,30 @@ def test_infinite_entries_of_b(T, dtype, r):
         y = fused_lora_forward_rows(x, w, bank, slots)
         want = check_not_finite(y, x, A, b, -2.0)
         assert torch.isposinf(want).any() and torch.isneginf(want).any()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("T, N, ranks", [(1, 136, [16]), (40, 264, [3, 16, 1]), (200, 520, [40, 64, 17]),
+                                         (300, 264, [16, 9, 30]), (700, 392, [128, 90, 16]), (1500, 136, [16, 33, 64])])
+def test_whole_numbers_are_exact_before_the_rounding(dtype, T, N, ranks):
+    """x, W, A and B of whole numbers whose sums all fit float32 and whose S (up to 2^14) both halves hold: what is left
+    is the one rounding of y.  S alone needs more bits than one half has, so this sees the low ones."""
+    K = 512
+    torch.manual_seed(T)
+    x = whole_numbers(T, K, most=15).to(dtype)
+    w = whole_numbers(N, K, most=3).to(dtype)
+    bank = AdapterBank(len(ranks), max(ranks), K, N, dtype, "cuda")
+    slots = torch.arange(T, device="cuda") * 5 % (len(ranks) + 1) - 1
+    if T == 1:
+        slots += 1
+    want = x.double() @ w.double().T
+    for i, r in enumerate(ranks):
+        a, b = whole_numbers(r, K, most=15).to(dtype), whole_numbers(N, r, most=1).to(dtype)
+        b *= (torch.arange(r, device="cuda") < 16).to(dtype)  # y stays in float16's range
+        bank.load(i, a, b, 0.5)
+        S = x.double() @ a.double().T
+        assert S.abs().max() < 2 ** 14 and (T == 1 or S.abs().max() > 2 ** 11)
+        want += torch.where((slots == i)[:, None], 0.5 * S @ b.double().T, 0.0)
+    assert want.abs().max() < 65504
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    assert torch.equal(y, want.to(dtype))
