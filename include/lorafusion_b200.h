@@ -521,6 +521,10 @@ LF_API int lf_rows_forward(const lf_rows_problem* prob, void* y_dev, void* works
 /* Launches of lf_rows_forward of T rows on the tensor cores (on CUDA cores there are 2). */
 LF_API int lf_rows_launch_count(int32_t T, int32_t r_pad);
 
+/* 1 if lf_rows_forward on tensor cores puts the shared projection of a chunk of T rows through the CTA-pair GEMM on a
+ * GPU of num_sms SMs, 0 if through the tiles of W as the M operand (host only). */
+LF_API int lf_rows_uses_pairs(int32_t T, int32_t K, int32_t N, int32_t num_sms);
+
 /* ------------------------------------------------------------------------------------------------
  * Training: gradient norms, clipping and AdamW of many adapters.  No counterpart in the reference
  * (it has no optimizer).

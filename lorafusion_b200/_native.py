@@ -192,6 +192,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_bank_load.restype = ctypes.c_int
     L.lf_rows_launch_count.argtypes = [_c_i32, _c_i32]
     L.lf_rows_launch_count.restype = ctypes.c_int
+    L.lf_rows_uses_pairs.argtypes = [_c_i32, _c_i32, _c_i32, _c_i32]
+    L.lf_rows_uses_pairs.restype = ctypes.c_int
     L.lf_grad_clip_workspace_bytes.argtypes = [_c_p, _c_i32, _c_i32]
     L.lf_grad_clip_workspace_bytes.restype = ctypes.c_size_t
     L.lf_grad_clip.argtypes = [_c_p, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_double, _c_p, _c_p, ctypes.c_size_t,

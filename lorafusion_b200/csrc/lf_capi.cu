@@ -886,6 +886,10 @@ extern "C" int lf_rows_launch_count(int32_t T, int32_t r_pad) {
   return n;
 }
 
+extern "C" int lf_rows_uses_pairs(int32_t T, int32_t K, int32_t N, int32_t num_sms) {
+  return T > 0 && K > 0 && N > 0 && num_sms > 1 && rows_use_pairs(T, K, N, num_sms);
+}
+
 extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* workspace_dev, size_t workspace_bytes,
                                lf_stream_t stream) {
   if (!p || p->T < 0 || p->K < 0 || p->N < 0 || p->n_slots < 0) return LF_ERR_INVALID_ARG;

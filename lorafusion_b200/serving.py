@@ -105,6 +105,9 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor; it must not
     overlap ``x``, ``base_weight`` or the bank.
 
+    The same call gives the same bits every time.  In a batch of four launches (below) a row's bits do not depend on the
+    rows beside it; in a shorter one its last bit may.
+
     Two launches on the current stream of ``x``'s device; long batches (above 256 rows, or 512 where the
     bank's padded rank is at most 32) run in chunks of 8192 rows of four launches each.  bf16/f16
     problems whose in_features or out_features is not a multiple of 8, or whose buffers are not 16-byte

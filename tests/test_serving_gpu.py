@@ -542,3 +542,32 @@ def test_whole_numbers_are_exact_before_the_rounding(dtype, T, N, ranks):
     assert want.abs().max() < 65504
     y = fused_lora_forward_rows(x, w, bank, slots)
     assert torch.equal(y, want.to(dtype))
+
+
+TALL_TILES = [  # dtype, T, K, N, ranks, max_rank: above 256 rows and not through the CTA-pair GEMM
+    (BF16, 300, 4096, 1024, [64, 33], 64),       # K in 8 parts, sorted rows
+    (F16, 512, 4096, 4096, [16] * 40, 16),       # in 2, the single launch of few rows
+    (BF16, 400, 4096, 1032, [16, 3, 30], 32),    # in 4, a last tile of 8 features
+    (BF16, 1000, 4096, 1024, [128, 16], 128),    # in 4, four row tiles
+    (F16, 2048, 4096, 1024, [64] * 5, 64),       # in 2, eight
+    (BF16, 400, 14336, 4096, [16, 8], 16),
+    (BF16, 300, 4096, 4096, [16, 64], 64),       # two adapters: few tiles, K of x A_i in 8 parts
+]
+
+
+@pytest.mark.parametrize("case", TALL_TILES, ids=lambda c: f"{str(c[0])[6:]}-{c[1]}x{c[2]}x{c[3]}-r{c[5]}")
+def test_row_tiles_beside_one_another(case):
+    dtype, T, K, N, ranks, max_rank = case
+    assert nat.lib().lf_rows_uses_pairs(T, K, N, torch.cuda.get_device_properties(0).multi_processor_count) == 0
+    x, w, bank, adapters, slots = make(dtype, T, K, N, ranks, max_rank)
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    check(y, x, w, adapters, slots)
+    order = torch.randperm(T, device="cuda")
+    moved = fused_lora_forward_rows(x[order], w, bank, slots[order])
+    if nat.lib().lf_rows_launch_count(T, bank.r_pad) == 4:
+        assert torch.equal(moved, y[order])
+    else:  # how many warps share K depends on the adapters beside a row there: the order of a sum may change
+        check(moved, x[order], w, adapters, slots[order])
+    none = torch.full_like(slots, -1)
+    check(fused_lora_forward_rows(x, w, bank, none), x, w, adapters, none)
+    assert nat.device_error() == 0

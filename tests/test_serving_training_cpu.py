@@ -184,3 +184,14 @@ def test_adamw_entry_refuses_before_any_launch():
     assert call(n_tensors=0) == nat.LF_OK
     grads[1] = 8194  # float32 gradients off a multiple of 4 bytes
     assert call() == nat.LF_ERR_INVALID_ARG
+
+
+def test_both_gemms_of_long_batches_are_chosen():
+    """Which GEMM a long batch takes, at the 148 SMs of a B200: the sizes that the numeric tests rely on."""
+    from tests.test_serving_gpu import CASES, TALL_TILES
+    uses = nat.lib().lf_rows_uses_pairs
+    assert all(uses(T, K, N, 148) == 0 for _, T, K, N, _, _ in TALL_TILES)
+    long = [(T, K, N) for dtype, T, K, N, _, _ in CASES if T > 256 and dtype is not torch.float32]
+    assert sum(uses(T, K, N, 148) for T, K, N in long) >= 5
+    assert uses(256, 4096, 4096, 148) == uses(0, 4096, 4096, 148) == uses(1000, 4096, 4096, 0) == 0
+    assert uses(8192, 4096, 4096, 148) == 1
