@@ -507,9 +507,8 @@ LF_API int lf_bank_load(const lf_bank_adapter* adapter, lf_stream_t stream);
 LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32_t dtype);
 
 /*
- * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense, shares no memory with x, W or
- * the bank.  row_slot is read on
- * the device, so a captured call follows later changes of it and of the bank's contents.  A
+ * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense, shares no memory with x, W,
+ * the bank or row_slot.  row_slot is read on the device, so a captured call follows later changes of it and of the bank's contents.  A
  * slot at or above n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
  * bf16/f16 with K, N and ldx multiples of 8 and 16-byte aligned buffers run on the tensor cores, other
  * problems on CUDA cores.  Long batches run in chunks of 8192 rows, of 4

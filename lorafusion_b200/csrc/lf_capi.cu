@@ -908,12 +908,15 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   if (!aligned16(workspace_dev) || !aligned16(p->b_bank_dev)) return LF_ERR_INVALID_ARG;
   const uint64_t es = static_cast<uint64_t>(elem_bytes(p->dtype)), T = p->T, K = p->K, N = p->N;
   const uint64_t ranks = static_cast<uint64_t>(p->n_slots) * p->r_pad, y0 = reinterpret_cast<uint64_t>(y_dev);
-  auto meets_y = [&](const void* base, uint64_t elems) {
+  auto meets_y = [&](const void* base, uint64_t bytes) {
     const uint64_t b = reinterpret_cast<uint64_t>(base);
-    return elems > 0 && b < y0 + T * N * es && y0 < b + elems * es;
+    return bytes > 0 && b < y0 + T * N * es && y0 < b + bytes;
   };
-  if (meets_y(p->x_dev, (T - 1) * p->ldx + K) || meets_y(p->w_dev, N * K) || meets_y(p->a_bank_dev, ranks * K) ||
-      meets_y(p->b_bank_dev, ranks * N))
+  const uint64_t n_slots = p->n_slots;
+  if (meets_y(p->x_dev, ((T - 1) * p->ldx + K) * es) || meets_y(p->w_dev, N * K * es) ||
+      meets_y(p->a_bank_dev, ranks * K * es) || meets_y(p->b_bank_dev, ranks * N * es) ||
+      meets_y(p->slot_rank_dev, n_slots * 4) || meets_y(p->slot_scale_dev, n_slots * 4) ||
+      meets_y(p->row_slot_dev, T * p->row_slot_bytes))
     return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;

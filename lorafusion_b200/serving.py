@@ -103,7 +103,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     empty slot.  An entry at or above ``bank.n_slots`` also gets the shared projection alone and is
     reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor; it must not
-    overlap ``x``, ``base_weight`` or the bank.
+    overlap ``x``, ``base_weight``, the bank or ``row_slot``.
 
     The same call gives the same bits every time.  In a batch of four launches (below) a row's bits do not depend on the
     rows beside it; in a shorter one its last bit may.

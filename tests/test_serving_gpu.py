@@ -571,3 +571,13 @@ def test_row_tiles_beside_one_another(case):
     none = torch.full_like(slots, -1)
     check(fused_lora_forward_rows(x, w, bank, none), x, w, adapters, none)
     assert nat.device_error() == 0
+
+
+def test_an_output_over_the_slots_is_refused():
+    x, w, bank, _, slots = make(BF16, 8, 64, 64, [16], 16)
+    memory = torch.zeros(8 * 64, dtype=BF16, device="cuda")
+    for shared in (memory[16:32].view(torch.int32), memory[-32:].view(torch.int64)):
+        shared.copy_(slots)
+        with pytest.raises(ValueError):
+            fused_lora_forward_rows(x, w, bank, shared, out=memory.view(8, 64))
+        assert torch.equal(shared, slots.to(shared.dtype))

@@ -195,3 +195,17 @@ def test_both_gemms_of_long_batches_are_chosen():
     assert sum(uses(T, K, N, 148) for T, K, N in long) >= 5
     assert uses(256, 4096, 4096, 148) == uses(0, 4096, 4096, 148) == uses(1000, 4096, 4096, 0) == 0
     assert uses(8192, 4096, 4096, 148) == 1
+
+
+def test_rows_output_may_not_share_memory_with_anything_read():
+    """4 x 16 bf16 output at 4096; an operand whose last byte is its first, or the other way round."""
+    L = nat.lib()
+    ws = L.lf_rows_workspace_bytes(4, 16, 16, nat.LF_BF16)
+    apart = dict(x_dev=1 << 20, w_dev=2 << 20, a_bank_dev=3 << 20, b_bank_dev=4 << 20, slot_rank_dev=5 << 20,
+                 slot_scale_dev=6 << 20, row_slot_dev=7 << 20)
+    sizes = dict(x_dev=4 * 16 * 2, w_dev=16 * 16 * 2, a_bank_dev=2 * 16 * 16 * 2, b_bank_dev=2 * 16 * 16 * 2,
+                 slot_rank_dev=8, slot_scale_dev=8, row_slot_dev=16)
+    for name, size in sizes.items():
+        for at in (4096, 4096 + 4 * 16 * 2 - 16, 4096 - size + 16 if size > 16 else 4096):
+            p = _rows(**{**apart, name: at})
+            assert L.lf_rows_forward(p, 4096, 256, ws, None) == nat.LF_ERR_INVALID_ARG, (name, at)
