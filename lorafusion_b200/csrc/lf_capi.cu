@@ -881,9 +881,9 @@ extern "C" int lf_bank_load(const lf_bank_adapter* p, lf_stream_t stream) {
 }
 
 extern "C" int lf_rows_launch_count(int32_t T, int32_t r_pad) {
-  int n = 0;
-  for (int t0 = 0; t0 < T; t0 += kRowsChunk) n += T - t0 > few_rows(r_pad) ? 4 : 2;
-  return n;
+  if (T <= 0) return 0;
+  const int rest = T % kRowsChunk;
+  return T / kRowsChunk * 4 + (rest > few_rows(r_pad) ? 4 : rest > 0 ? 2 : 0);
 }
 
 extern "C" int lf_rows_uses_pairs(int32_t T, int32_t K, int32_t N, int32_t num_sms) {
@@ -958,11 +958,11 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   const char* x = static_cast<const char*>(p->x_dev);
   const char* slots = static_cast<const char*>(p->row_slot_dev);
   char* y = static_cast<char*>(y_dev);
-  for (int t0 = 0; t0 < p->T; t0 += kRowsChunk) {
-    a.T = p->T - t0 < kRowsChunk ? p->T - t0 : kRowsChunk;
-    a.x = x + static_cast<size_t>(t0) * p->ldx * 2;
-    a.row_slot = slots + static_cast<size_t>(t0) * p->row_slot_bytes;
-    a.y = y + static_cast<size_t>(t0) * p->N * 2;
+  for (int64_t t0 = 0; t0 < p->T; t0 += kRowsChunk) {
+    a.T = static_cast<int>(p->T - t0 < kRowsChunk ? p->T - t0 : kRowsChunk);
+    a.x = x + t0 * p->ldx * 2;
+    a.row_slot = slots + t0 * p->row_slot_bytes;
+    a.y = y + t0 * p->N * 2;
     const uint64_t x_pitch = static_cast<uint64_t>(p->ldx) * 2, w_pitch = static_cast<uint64_t>(p->K) * 2;
     cudaError_t e;
     ManyMaps maps_of_many;

@@ -22,6 +22,7 @@ from lorafusion_b200 import b200_ops
 __all__ = ["AdapterBank", "fused_lora_forward_rows"]
 
 _DTYPE_CODE = b200_ops._DTYPE_CODE
+_MAX_ROWS = (1 << 31) - 1
 
 
 def _launches(rows: int, r_pad: int, tensor_cores: bool) -> int:
@@ -127,6 +128,8 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
         raise ValueError("x must be a CUDA tensor: lorafusion_b200 has no CPU path")
     T, K = x.shape
     N = bank.out_features
+    if T > _MAX_ROWS:
+        raise ValueError(f"x has {T} rows: at most {_MAX_ROWS} are supported")
     if K != bank.in_features or base_weight.shape != (N, K):
         raise ValueError(f"x {tuple(x.shape)}, base_weight {tuple(base_weight.shape)} and a bank of "
                          f"{bank.in_features} -> {N} features do not match")

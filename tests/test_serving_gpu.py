@@ -581,3 +581,11 @@ def test_an_output_over_the_slots_is_refused():
         with pytest.raises(ValueError):
             fused_lora_forward_rows(x, w, bank, shared, out=memory.view(8, 64))
         assert torch.equal(shared, slots.to(shared.dtype))
+
+
+def test_more_rows_than_32_bits_count_are_refused():
+    _, w, bank, _, _ = make(BF16, 8, 64, 64, [16], 16)
+    for T in (2 ** 31, 2 ** 32 + 5):
+        x = torch.zeros(1, 64, dtype=BF16, device="cuda").expand(T, 64)
+        with pytest.raises(ValueError):
+            fused_lora_forward_rows(x, w, bank, torch.zeros(1, dtype=torch.int32, device="cuda").expand(T))

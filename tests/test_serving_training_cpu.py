@@ -209,3 +209,9 @@ def test_rows_output_may_not_share_memory_with_anything_read():
         for at in (4096, 4096 + 4 * 16 * 2 - 16, 4096 - size + 16 if size > 16 else 4096):
             p = _rows(**{**apart, name: at})
             assert L.lf_rows_forward(p, 4096, 256, ws, None) == nat.LF_ERR_INVALID_ARG, (name, at)
+
+
+def test_launch_count_of_the_largest_batches():
+    count = nat.lib().lf_rows_launch_count
+    assert count(2 ** 31 - 1, 64) == 4 * 2 ** 18 and count(2 ** 31 - 8192, 64) == 4 * (2 ** 18 - 1)
+    assert count(-1, 64) == count(-2 ** 31, 16) == 0
