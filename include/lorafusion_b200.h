@@ -517,7 +517,7 @@ LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32
 LF_API int lf_rows_forward(const lf_rows_problem* prob, void* y_dev, void* workspace_dev, size_t workspace_bytes,
                            lf_stream_t stream);
 
-/* Launches of lf_rows_forward of T rows on the tensor cores (on CUDA cores there are 2). */
+/* Launches of lf_rows_forward of T rows on the tensor cores (on CUDA cores there are 2 for each 2,097,120 rows). */
 LF_API int lf_rows_launch_count(int32_t T, int32_t r_pad);
 
 /* 1 if lf_rows_forward on tensor cores puts the shared projection of a chunk of T rows through the CTA-pair GEMM on a

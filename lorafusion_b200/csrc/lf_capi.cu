@@ -950,14 +950,21 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = p->dtype != LF_F32 && p->K > 0 && p->K % 8 == 0 && p->N % 8 == 0 && p->ldx % 8 == 0 &&
                   aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) && aligned16(y_dev);
-  if (!tc) {
-    if ((p->T + 31) / 32 > 65535) return LF_ERR_UNSUPPORTED;
-    return to_status(rows_forward_simt(a, p->dtype, st));
-  }
-  // chunks of kRowsChunk rows share the adapters' part, one after another on the stream
+  // chunks of rows share the workspace, one after another on the stream
   const char* x = static_cast<const char*>(p->x_dev);
   const char* slots = static_cast<const char*>(p->row_slot_dev);
   char* y = static_cast<char*>(y_dev);
+  if (!tc) {
+    for (int64_t t0 = 0; t0 < p->T; t0 += kRowsSimtChunk) {
+      a.T = static_cast<int>(p->T - t0 < kRowsSimtChunk ? p->T - t0 : kRowsSimtChunk);
+      a.x = x + t0 * p->ldx * static_cast<int64_t>(es);
+      a.row_slot = slots + t0 * p->row_slot_bytes;
+      a.y = y + t0 * p->N * static_cast<int64_t>(es);
+      const int rc = to_status(rows_forward_simt(a, p->dtype, st));
+      if (rc != LF_OK) return rc;
+    }
+    return LF_OK;
+  }
   for (int64_t t0 = 0; t0 < p->T; t0 += kRowsChunk) {
     a.T = static_cast<int>(p->T - t0 < kRowsChunk ? p->T - t0 : kRowsChunk);
     a.x = x + t0 * p->ldx * 2;

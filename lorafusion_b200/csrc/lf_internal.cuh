@@ -205,6 +205,7 @@ struct ManyMaps {
   CUtensorMap b;           // bank B [n_slots r_pad/16 N, 16] box (16, 256), 32-byte swizzle
 };
 constexpr int kRowsChunk = 8192;  // rows whose adapters' part is held at a time
+constexpr int kRowsSimtChunk = 32 * 65535;  // on CUDA cores: what a grid of 32-row tiles covers
 // Rows up to which the adapters' part is one launch that groups 8 rows of an adapter; more are sorted first.  At 512
 // rows of 4096 -> 4096: rank 16, 64 adapters in any order 34 us against 54, rank 64 in prompts 35 against 49; but
 // at rank 64 and tokens in any order 344 against 191 (to 14336 features, 128 adapters), 70 against 57 at 300 rows.

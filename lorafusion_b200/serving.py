@@ -26,7 +26,9 @@ _MAX_ROWS = (1 << 31) - 1
 
 
 def _launches(rows: int, r_pad: int, tensor_cores: bool) -> int:
-    return 2 if rows <= 256 or not tensor_cores else nat.lib().lf_rows_launch_count(rows, r_pad)
+    if not tensor_cores:
+        return 2 * -(-rows // (32 * 65535))
+    return 2 if rows <= 256 else nat.lib().lf_rows_launch_count(rows, r_pad)
 
 
 class AdapterBank:

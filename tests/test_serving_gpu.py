@@ -589,3 +589,15 @@ def test_more_rows_than_32_bits_count_are_refused():
         x = torch.zeros(1, 64, dtype=BF16, device="cuda").expand(T, 64)
         with pytest.raises(ValueError):
             fused_lora_forward_rows(x, w, bank, torch.zeros(1, dtype=torch.int32, device="cuda").expand(T))
+
+
+@pytest.mark.filterwarnings("ignore::lorafusion_b200.b200_ops.CudaCorePathWarning")
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_more_rows_on_cuda_cores_than_one_grid_covers(dtype):
+    T, K, N = 32 * 65535 + 37, 5, 3
+    x, w, bank, adapters, slots = make(dtype, T, K, N, [2, 1], 2)
+    out = torch.full((T + 1, N), 7.0, dtype=dtype, device="cuda")
+    fused_lora_forward_rows(x, w, bank, slots, out=out[:T])
+    assert b200_ops.last_launch_count() == 4
+    check(out[:T], x, w, adapters, slots)
+    assert bool((out[T] == 7).all())
