@@ -394,6 +394,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
   __shared__ __align__(16) T s_hi[kSteps][8][kSPitch], s_lo[kSteps][8][kSPitch];
   __shared__ float s_fac[kSteps][8];
   __shared__ __align__(16) float s_sum[kSteps][16 * 8];
+  __shared__ int s_more, s_go;  // whether this CTA, and so the cluster, has another batch
   pdl_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, q = lane & 3;
@@ -415,7 +416,9 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
     auto group_at = [&](int j) { return static_cast<int>(s.order[j * slices + (j & 1 ? slices - 1 - slice : slice)]); };
     const int rest = n_groups % slices, rounds = n_groups / slices;
     const int mine = rounds + ((rounds & 1 ? slices - 1 - slice : slice) < rest);
-    for (int first = 0, batch; first < mine; first += batch) {
+    // Every CTA of a cluster sorts for itself, from slots that another stream must not change meanwhile.  If one does all the
+    // same, they differ about the groups; the cluster's barriers must not: the first CTA says whether a batch follows.
+    for (int first = 0, batch; kparts > 1 || first < mine; first += batch) {
       int steps = 0, ranks = 0;  // as many groups as there is room for
       for (batch = 0; first + batch < mine; ++batch) {
         const uint32_t e = s.eff[s.start[group_at(first + batch)]];
@@ -482,7 +485,10 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
         else part[0][0][i] = v;
       }
       if (kparts > 1) {
+        if (tid == 0) s_more = first + batch < mine;
         cluster_sync_all();
+        float go = 0.f;  // the last warp has the least to add up
+        if (tid == kShrinkThreads - 1) go = ld_cluster_f32(map_to_cta(smem_u32(&s_more), 0));
         for (int i = 4 * tid; i < steps * 128; i += 4 * kShrinkThreads) {
           const uint32_t at = smem_u32(&part[0][0][i]);
           float4 v[8];
@@ -494,6 +500,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
             if (c < kparts) v[0].x += v[c].x, v[0].y += v[c].y, v[0].z += v[c].z, v[0].w += v[c].w;
           *reinterpret_cast<float4*>(&s_sum[0][i]) = v[0];
         }
+        if (tid == kShrinkThreads - 1) s_go = __float_as_int(go);
         __syncwarp();
         cluster_arrive();  // the others may write their sums again once all have come here
       }
@@ -528,7 +535,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
       // one warp would have four times another's work (64 rows of ranks 8 to 64 to 14336 features 46 -> 42 us; with equal
       // widths the other way was slower, 250 rows of rank 16 37.1 against 36.5).
       int lanes_b = lanes;
-      if (width_of(s.eff[s.start[group_at(first)]]) != width_of(s.eff[s.start[group_at(first + batch - 1)]]))
+      if (batch > 1 && width_of(s.eff[s.start[group_at(first)]]) != width_of(s.eff[s.start[group_at(first + batch - 1)]]))
         for (lanes_b = 1; lanes_b < lanes && (nb1 - nb0) * lanes_b < 4 * kShrinkWarps;) lanes_b *= 2;
       const int subs_b = kShrinkWarps / lanes_b, sub_b = warp / lanes_b;
       const int f0 = nb0 + (nb1 - nb0) * sub_b / subs_b, f1 = nb0 + (nb1 - nb0) * (sub_b + 1) / subs_b;
@@ -555,7 +562,10 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
           expand_group<T, 8, 1>(p, e, f0, f1, rows_of);
         }
       }
-      if (kparts > 1) cluster_wait();
+      if (kparts > 1) {
+        cluster_wait();
+        if (!s_go) break;
+      }
       __syncthreads();
     }
     __syncthreads();

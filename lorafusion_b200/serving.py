@@ -38,7 +38,8 @@ class AdapterBank:
     (``alpha / r``); an empty slot adds nothing to its rows.  Memory: ``n_slots * r_pad *
     (in_features + out_features)`` elements of ``dtype``, ``r_pad`` being ``max_rank`` rounded up to 16,
     32, 64 or 128.  ``load`` and ``unload`` copy on the device's current stream: a forward enqueued
-    there earlier still sees the old contents, a later one the new.
+    there earlier still sees the old contents, a later one the new.  On another stream than the forwards', order
+    them with events: the rows of a slot that changes under a running forward are undefined.
     """
 
     def __init__(self, n_slots: int, max_rank: int, in_features: int, out_features: int,
@@ -104,7 +105,8 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     bank share one dtype (float32, bfloat16, float16) and device.  ``row_slot [T]`` is an int32 or int64
     tensor on that device, in any order; a negative entry means no adapter, and so does an
     empty slot.  An entry at or above ``bank.n_slots`` also gets the shared projection alone and is
-    reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.
+    reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.  Until the call
+    has run, ``row_slot`` and the bank must not change on another stream (the result would be undefined).
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor; it must not
     overlap ``x``, ``base_weight``, the bank or ``row_slot``.
 

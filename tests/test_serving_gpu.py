@@ -601,3 +601,23 @@ def test_more_rows_on_cuda_cores_than_one_grid_covers(dtype):
     assert b200_ops.last_launch_count() == 4
     check(out[:T], x, w, adapters, slots)
     assert bool((out[T] == 7).all())
+
+
+@pytest.mark.parametrize("T", [1, 64, 400])
+def test_slots_that_change_under_a_call_leave_no_wait_behind(T):
+    """Not allowed, and the rows are undefined; but the CTAs of a cluster, which then disagree about the batches, end."""
+    ranks = [16, 8, 32, 3] * 40
+    x, w, bank, adapters, slots = make(BF16, T, 4096, 512, ranks, 32)
+    patterns = [torch.full_like(slots, -1), slots.clone(), torch.arange(T, device="cuda", dtype=torch.int32) % 160,
+                torch.zeros_like(slots)]
+    changing, writer = slots.clone(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for k in range(200):
+        with torch.cuda.stream(writer):
+            for p in patterns:
+                changing.copy_(p)
+            bank.ranks[k % 4::4] = ranks[k % 4]  # as they are
+        fused_lora_forward_rows(x, w, bank, changing)
+    torch.cuda.synchronize()
+    check(fused_lora_forward_rows(x, w, bank, slots), x, w, adapters, slots)
+    assert nat.device_error() == 0
