@@ -8,6 +8,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -79,7 +80,7 @@ PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   } else {
     const at::Tensor* o = cuda_tensor(a[7]);
     if (!o || o->dim() != 2 || o->size(0) != T || o->size(1) != N || o->scalar_type() != x.scalar_type() ||
-        o->device() != dev || !o->is_contiguous())
+        o->device() != dev || !o->is_contiguous() || (o->requires_grad() && c10::GradMode::is_enabled()))
       Py_RETURN_NONE;
     y = *o;
   }

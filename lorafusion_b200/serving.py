@@ -108,7 +108,9 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.  Until the call
     has run, ``row_slot`` and the bank must not change on another stream (the result would be undefined).
     ``out`` (contiguous, ``[T, out_features]``) receives the result in place of a new tensor; it must not
-    overlap ``x``, ``base_weight``, the bank or ``row_slot``.
+    overlap ``x``, ``base_weight``, the bank or ``row_slot``, and not require a gradient unless under
+    ``torch.no_grad()``.  Autograd does not record the call: the result has no gradient, whatever ``x`` and the
+    weights require (``b200_ops.fused_lora_forward`` and ``fused_lora_backward`` are the pair for training).
 
     The same call gives the same bits every time.  In a batch of four launches (below) a row's bits do not depend on the
     rows beside it; in a shorter one its last bit may.
@@ -160,6 +162,8 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
         out = torch.empty((T, N), dtype=dtype, device=device)
     elif out.shape != (T, N) or out.dtype != dtype or out.device != device or not out.is_contiguous():
         raise ValueError(f"out must be a contiguous {dtype} tensor of shape ({T}, {N}) on {device}")
+    elif out.requires_grad and torch.is_grad_enabled():
+        raise ValueError("out requires a gradient, and this operator records none: call it under torch.no_grad()")
     b200_ops._last_launches = 0
     if T == 0:
         return out

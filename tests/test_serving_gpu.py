@@ -621,3 +621,19 @@ def test_slots_that_change_under_a_call_leave_no_wait_behind(T):
     torch.cuda.synchronize()
     check(fused_lora_forward_rows(x, w, bank, slots), x, w, adapters, slots)
     assert nat.device_error() == 0
+
+
+def test_nothing_is_recorded_and_an_output_that_requires_a_gradient_is_refused():
+    x, w, bank, adapters, slots = make(BF16, 8, 64, 64, [16], 16)
+    y = fused_lora_forward_rows(x, w, bank, slots)
+    xg, wg = x.clone().requires_grad_(), torch.nn.Parameter(w)
+    got = fused_lora_forward_rows(xg, wg, bank, slots)
+    assert torch.equal(got, y) and not got.requires_grad
+    leaf = torch.zeros_like(y).requires_grad_()
+    for out in (leaf, leaf * 2):
+        kept = out.detach().clone()
+        with pytest.raises(ValueError):
+            fused_lora_forward_rows(x, w, bank, slots, out=out)
+        assert torch.equal(out, kept)
+        with torch.no_grad():
+            assert torch.equal(fused_lora_forward_rows(x, w, bank, slots, out=out), y)
