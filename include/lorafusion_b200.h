@@ -500,7 +500,8 @@ typedef struct lf_bank_adapter {
   float* slot_scale_dev;
 } lf_bank_adapter;
 
-/* Copies an adapter into its slot in one launch, zeros past its rank; `stream` orders it with the forwards. */
+/* Copies an adapter into its slot in one launch, zeros past its rank; `stream` orders it with the forwards.  An adapter
+ * that shares memory with the slot is refused. */
 LF_API int lf_bank_load(const lf_bank_adapter* adapter, lf_stream_t stream);
 
 /* Workspace bytes of lf_rows_forward (256-byte aligned buffer). */

@@ -873,6 +873,17 @@ extern "C" int lf_bank_load(const lf_bank_adapter* p, lf_stream_t stream) {
   if ((p->rank > 1 && p->lda < p->K) || (p->N > 1 && p->ldb < p->rank)) return LF_ERR_INVALID_ARG;
   if (!p->a_dev || !p->b_dev || !p->slot_a_dev || !p->slot_b_dev || !p->slot_rank_dev || !p->slot_scale_dev)
     return LF_ERR_INVALID_ARG;
+  // threads zero and write the slot while others still read the adapter
+  const uint64_t es = static_cast<uint64_t>(elem_bytes(p->dtype)), r_pad = p->r_pad, K = p->K, N = p->N;
+  const uint64_t rows_a = p->rank - 1, rows_b = N - 1;  // beyond the first
+  auto meet = [](const void* a, uint64_t na, const void* b, uint64_t nb) {
+    const uint64_t a0 = reinterpret_cast<uint64_t>(a), b0 = reinterpret_cast<uint64_t>(b);
+    return a0 < b0 + nb && b0 < a0 + na;
+  };
+  const uint64_t bytes_a = (rows_a * (rows_a ? p->lda : 0) + K) * es, bytes_b = (rows_b * (rows_b ? p->ldb : 0) + p->rank) * es;
+  if (meet(p->a_dev, bytes_a, p->slot_a_dev, r_pad * K * es) || meet(p->a_dev, bytes_a, p->slot_b_dev, r_pad * N * es) ||
+      meet(p->b_dev, bytes_b, p->slot_a_dev, r_pad * K * es) || meet(p->b_dev, bytes_b, p->slot_b_dev, r_pad * N * es))
+    return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
   const BankLoad b{p->a_dev, p->b_dev,  p->slot_a_dev, p->slot_b_dev, p->slot_rank_dev, p->slot_scale_dev, p->lda,

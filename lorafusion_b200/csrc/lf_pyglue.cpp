@@ -154,6 +154,7 @@ PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.slot_scale_dev = static_cast<float*>(t[3]->data_ptr()) + slot;
   const c10::cuda::OptionalCUDAGuard guard(ba.device());
   const int rc = lf_bank_load(&p, c10::cuda::getCurrentCUDAStream(ba.device().index()).stream());
+  if (rc == LF_ERR_INVALID_ARG) Py_RETURN_NONE;  // the adapter lies in the slot itself
   if (rc != LF_OK) return fail(rc, "lf_bank_load");
   for (int i = 0; i < 4; ++i) bump(*t[i]);
   Py_RETURN_TRUE;

@@ -86,8 +86,9 @@ class AdapterBank:
         scaling = float(scaling)
         if nat.glue().bank_load(self.lora_a, self.lora_b, self.ranks, self.scales, slot, lora_a, lora_b, scaling):
             return
-        # another dtype or device, or rows that are not dense: as the bank has them, then the same call
-        lora_a, lora_b = (t.to(self.device, self.dtype).contiguous() for t in (lora_a, lora_b))
+        # another dtype or device, rows that are not dense, parts of the slot itself: a copy as the bank has them, then
+        # the same call
+        lora_a, lora_b = (t.to(self.device, self.dtype, copy=True).contiguous() for t in (lora_a, lora_b))
         if not nat.glue().bank_load(self.lora_a, self.lora_b, self.ranks, self.scales, slot, lora_a, lora_b, scaling):
             raise ValueError(f"slot {slot}: the adapter cannot be copied into the bank's tensors")
 

@@ -637,3 +637,21 @@ def test_nothing_is_recorded_and_an_output_that_requires_a_gradient_is_refused()
         assert torch.equal(out, kept)
         with torch.no_grad():
             assert torch.equal(fused_lora_forward_rows(x, w, bank, slots, out=out), y)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_load_of_parts_of_the_slot_itself(dtype):
+    """Half of an adapter's ranks, moved to the front, while the kernel zeroes the others."""
+    K, N = 8192, 4096
+    bank = AdapterBank(2, 16, K, N, dtype, "cuda")
+    for _ in range(3):
+        a, b = torch.randn(16, K, device="cuda").to(dtype), torch.randn(N, 16, device="cuda").to(dtype)
+        bank.load(1, a, b, 1.0)
+        bank.load(1, bank.lora_a[1, 8:], bank.lora_b[1, 0][:, 8:], 2.0)
+        assert torch.equal(bank.lora_a[1, :8], a[8:]) and not bank.lora_a[1, 8:].any()
+        assert torch.equal(bank.lora_b[1, 0, :, :8], b[:, 8:]) and not bank.lora_b[1, 0, :, 8:].any()
+        assert bank.ranks.tolist() == [0, 8] and not bank.lora_a[0].any()
+        bank.load(0, bank.lora_a[1, :8], bank.lora_b[1, 0][:, :8], 2.0)  # from another slot: no copy between
+        assert torch.equal(bank.lora_a[0], bank.lora_a[1]) and torch.equal(bank.lora_b[0], bank.lora_b[1])
+        bank.unload(0)
+        bank.lora_a[0].zero_()

@@ -215,3 +215,16 @@ def test_launch_count_of_the_largest_batches():
     count = nat.lib().lf_rows_launch_count
     assert count(2 ** 31 - 1, 64) == 4 * 2 ** 18 and count(2 ** 31 - 8192, 64) == 4 * (2 ** 18 - 1)
     assert count(-1, 64) == count(-2 ** 31, 16) == 0
+
+
+def test_bank_load_from_its_own_slot_is_refused():
+    def call(**kw):
+        d = dict(dtype=nat.LF_BF16, K=32, N=24, r_pad=16, rank=4, scale=1.0, lda=40, ldb=6, a_dev=1 << 20, b_dev=2 << 20,
+                 slot_a_dev=3 << 20, slot_b_dev=4 << 20, slot_rank_dev=256, slot_scale_dev=256)
+        return nat.lib().lf_bank_load(nat.BankAdapter(**{**d, **kw}), None)
+
+    last_a, last_b = 2 * (3 * 40 + 32) - 2, 2 * (23 * 6 + 4) - 2  # bytes to an operand's last element
+    for slot, size in ((3 << 20, 16 * 32 * 2), (4 << 20, 16 * 24 * 2)):
+        for name, last in (("a_dev", last_a), ("b_dev", last_b)):
+            for at in (slot, slot + size - 2, slot - last):
+                assert call(**{name: at}) == nat.LF_ERR_INVALID_ARG, (name, at)
