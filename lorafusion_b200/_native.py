@@ -14,8 +14,6 @@ import re
 import threading
 from contextlib import nullcontext
 
-import torch
-
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "_lib", "liblorafusion_b200.so")
 HEADER_PATH = os.path.join(os.path.dirname(_HERE), "include", "lorafusion_b200.h")
@@ -275,11 +273,13 @@ def check(code: int, what: str) -> None:
 
 def raw_stream(device_index: int) -> int:
     """cudaStream_t of the device's current stream (without building a Stream object: 0.1 us, not 2)."""
+    import torch
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
 def on_device(device_index: int):
     """Context that makes a device current; nothing to do where it already is."""
+    import torch
     return nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
 
 

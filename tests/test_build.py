@@ -1,0 +1,28 @@
+"""The library and its ctypes binding without PyTorch, and the Python module that belongs to one PyTorch (no GPU)."""
+
+import os
+import subprocess
+import sys
+
+REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+
+NO_TORCH = """
+import sys
+class Block:
+    def find_spec(self, name, path=None, target=None):
+        if name.split(".")[0] == "torch":
+            raise ModuleNotFoundError("No module named 'torch'", name="torch")
+sys.meta_path.insert(0, Block())
+"""
+
+
+def without_torch(code):
+    return subprocess.run([sys.executable, "-c", NO_TORCH + code], cwd=REPO, capture_output=True, text=True, timeout=300)
+
+
+def test_the_binding_needs_no_torch():
+    res = without_torch("from lorafusion_b200 import _native, config, workloads\n"
+                        "print(_native.lib().lf_version().decode())\n"
+                        "print(len(_native.header_symbols()))")
+    assert res.returncode == 0, res.stderr
+    assert res.stdout.startswith("lorafusion_b200")
