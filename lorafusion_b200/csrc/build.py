@@ -5,8 +5,9 @@
 Every translation unit is compiled by nvcc for ``compute_100a``/``sm_100a`` only
 (with ``-lineinfo``), in parallel, then linked into one position-independent
 shared library with a static CUDA runtime.  Objects are rebuilt when a source
-or header is newer than the object.  ``_lib/lf_pyglue.so``, a Python module that
-links PyTorch and that library, is built beside it.
+or header is newer than the object.  The Python module of ``lf_pyglue.cpp``, which
+links PyTorch and that library, is built beside it where PyTorch is installed; the
+library itself, the C ABI, needs neither.
 """
 
 from __future__ import annotations
@@ -68,10 +69,16 @@ def _compile(src: str, force: bool, verbose: bool, extra: list[str]) -> str:
 
 
 def _build_glue(force: bool, verbose: bool) -> None:
-    """The Python module of csrc/lf_pyglue.cpp, beside the library it calls."""
+    """The Python module of csrc/lf_pyglue.cpp, beside the library it calls; nothing where PyTorch is missing."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        torch = None
+    if torch is None or torch.version.cuda is None:
+        print(f"{GLUE_NAME} not built: no PyTorch with CUDA here (the C library is complete without it)", file=sys.stderr)
+        return
     src, out = os.path.join(HERE, GLUE_SOURCE), os.path.join(LIB_DIR, GLUE_NAME)
     header = os.path.join(REPO, "include", "lorafusion_b200.h")
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(header)):

@@ -26,3 +26,11 @@ def test_the_binding_needs_no_torch():
                         "print(len(_native.header_symbols()))")
     assert res.returncode == 0, res.stderr
     assert res.stdout.startswith("lorafusion_b200")
+
+
+def test_the_library_builds_without_torch(tmp_path):
+    """What a build does after the library is linked (nothing is compiled here)."""
+    res = without_torch(f"from lorafusion_b200.csrc import build\nbuild.LIB_DIR = {str(tmp_path)!r}\n"
+                        "build._build_glue(False, False)")
+    assert res.returncode == 0, res.stderr
+    assert "no PyTorch" in res.stderr and not os.listdir(tmp_path)
