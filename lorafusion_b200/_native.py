@@ -11,6 +11,7 @@ import ctypes
 import importlib.util
 import os
 import re
+import sysconfig
 import threading
 from contextlib import nullcontext
 
@@ -232,15 +233,23 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+def glue_path() -> str:
+    """Where the Python module of ``csrc/lf_pyglue.cpp`` for this Python and this PyTorch is built.  It is C++
+    against both, so one built for another version must not be loaded: the name holds the versions."""
+    import torch
+    tag = f"{sysconfig.get_config_var('SOABI')}.torch-{torch.__version__}"
+    return os.path.join(_HERE, "_lib", f"lf_pyglue.{tag}.so")
+
+
 def glue():
     """The Python module of ``csrc/lf_pyglue.cpp`` (tensor checks and calls without a Python step per
-    tensor); ``RuntimeError`` if it has not been built."""
+    tensor); ``RuntimeError`` if it has not been built for this Python and PyTorch."""
     global _glue
     if _glue is None:
         L = lib()
         with _lock:
             if _glue is None:
-                path = os.path.join(_HERE, "_lib", "lf_pyglue.so")
+                path = glue_path()
                 if not os.path.exists(path):
                     raise RuntimeError(f"{path} not found; build it with `python -m lorafusion_b200.csrc.build`")
                 spec = importlib.util.spec_from_file_location("lf_pyglue", path)

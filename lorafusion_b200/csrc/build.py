@@ -25,7 +25,7 @@ REPO = os.path.dirname(PKG)
 OBJ_DIR = os.path.join(PKG, "_build")
 LIB_DIR = os.path.join(PKG, "_lib")
 LIB_NAME = "liblorafusion_b200.so"
-GLUE_SOURCE, GLUE_NAME = "lf_pyglue.cpp", "lf_pyglue.so"  # Python module: tensor checks and calls for PyTorch
+GLUE_SOURCE = "lf_pyglue.cpp"  # Python module: tensor checks and calls for PyTorch
 SOURCES = ["lf_tables.cpp", "lf_sched.cpp", "lf_simt.cu", "lf_tc.cu", "lf_rows.cu", "lf_lora_rows.cu", "lf_train.cu",
            "lf_capi.cu", "lf_noalloc.cu"]
 HEADERS = ["lf_ptx.cuh", "lf_internal.cuh", "lf_launch.cuh", os.path.join("..", "..", "include", "lorafusion_b200.h")]
@@ -72,14 +72,15 @@ def _build_glue(force: bool, verbose: bool) -> None:
     """The Python module of csrc/lf_pyglue.cpp, beside the library it calls; nothing where PyTorch is missing."""
     import sysconfig
 
+    from lorafusion_b200 import _native
     try:
         import torch
     except ImportError:
         torch = None
     if torch is None or torch.version.cuda is None:
-        print(f"{GLUE_NAME} not built: no PyTorch with CUDA here (the C library is complete without it)", file=sys.stderr)
+        print(f"{GLUE_SOURCE} not built: no PyTorch with CUDA here (the C library is complete without it)", file=sys.stderr)
         return
-    src, out = os.path.join(HERE, GLUE_SOURCE), os.path.join(LIB_DIR, GLUE_NAME)
+    src, out = os.path.join(HERE, GLUE_SOURCE), os.path.join(LIB_DIR, os.path.basename(_native.glue_path()))
     header = os.path.join(REPO, "include", "lorafusion_b200.h")
     if not force and os.path.exists(out) and os.path.getmtime(out) >= max(os.path.getmtime(src), os.path.getmtime(header)):
         return

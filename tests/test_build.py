@@ -4,6 +4,12 @@ import os
 import subprocess
 import sys
 
+import pytest
+import torch
+
+from lorafusion_b200 import _native as nat
+from lorafusion_b200.csrc import build
+
 REPO = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 NO_TORCH = """
@@ -34,3 +40,29 @@ def test_the_library_builds_without_torch(tmp_path):
                         "build._build_glue(False, False)")
     assert res.returncode == 0, res.stderr
     assert "no PyTorch" in res.stderr and not os.listdir(tmp_path)
+
+
+def test_the_python_module_belongs_to_one_torch(monkeypatch, tmp_path):
+    """After another PyTorch is installed the old module is neither loaded nor taken for built."""
+    here = nat.glue_path()
+    assert torch.__version__ in here
+    monkeypatch.setattr(torch, "__version__", "99.0+cu999")
+    assert nat.glue_path() != here
+    monkeypatch.setattr(nat, "_glue", None)
+    with pytest.raises(RuntimeError, match="99.0"):
+        nat.glue()
+
+    class Stop(Exception):
+        pass
+
+    def compile_(cmd, **kw):
+        assert os.path.basename(nat.glue_path()) in " ".join(cmd)
+        raise Stop
+
+    monkeypatch.setattr(build.subprocess, "run", compile_)
+    with pytest.raises(Stop):
+        build._build_glue(False, False)
+    monkeypatch.undo()
+    if os.path.exists(here):
+        monkeypatch.setattr(build.subprocess, "run", compile_)
+        build._build_glue(False, False)  # built for this one: nothing to do
