@@ -893,6 +893,10 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
 // would (a TMA gather of four rows takes about 50 ns however many are in flight: 99 us for 8192 rows); TMA
 // loads A_i.  24 us for 8192 x 4096 and 64 adapters of ranks 8 to 64: a round of 87 tiles, half a microsecond for 128
 // elements of K, where the MMA warp's eight small MMAs and their waits take what the copies do.
+// All of a CTA's K goes into one accumulator.  The tensor core drops up to 2^-25 of the running sum a step of 16, so
+// 14336 elements of one sign lose at most 2^-15 of S, as the shared projection beside it does: a hundredth of a bf16
+// rounding of y, a sixteenth of a float16 one.  (The packed shrink rotates accumulators because its S also goes into gradients,
+// which sum over all tokens.)
 constexpr int kXBytes = kTileRows * kBK * 2;
 constexpr int kShrinkMaxStages = 8;
 constexpr int kLoadWarps = 4;
@@ -1324,7 +1328,11 @@ __global__ void __launch_bounds__(kGemmThreads, 1)
 }
 
 // ============================================================================ CUDA cores
-// Float32 problems and shapes TMA cannot address.  One CTA a row for S; then 32 x 32 output tiles.
+// Float32 problems and shapes TMA cannot address.  One CTA a row for S; then 32 x 32 output tiles.  Sums are float32, cut
+// so that their errors grow with K / 128 (S, one lane's share) or K / 32 (a step's sum first): 1.2e-7 of the
+// result's norm at K = 256, where one float32 product with the library is off by 2.9e-7.  (The packed float32 path
+// sums in 64 bits, for gradients and an oracle that it meets to the last bits; a served row needs no more than
+// float32 products give.)
 constexpr int kSimtShrink = 128;
 template <typename T>
 __global__ void __launch_bounds__(kSimtShrink) rows_shrink_simt_kernel(const RowsArgs p) {

@@ -12,8 +12,6 @@ No counterpart in the reference (``lorafusion/ops/mock_ops.py:15-48`` is the pac
 
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
 from lorafusion_b200 import _native as nat
@@ -173,7 +171,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
                         bank.ranks.data_ptr(), bank.scales.data_ptr(), row_slot.data_ptr())
     tensor_cores = dtype is not torch.float32
     if tensor_cores and (K % 8 or N % 8 or ldx % 8 or
-                                       (p.x_dev | p.w_dev | p.a_bank_dev | p.b_bank_dev | out.data_ptr()) % 16):
+                         (p.x_dev | p.w_dev | p.a_bank_dev | p.b_bank_dev | out.data_ptr()) % 16):
         if ldx % 8 or p.x_dev % 16:  # only x's rows: a dense copy of x is far cheaper than CUDA cores
             x = x.clone(memory_format=torch.contiguous_format)
             p.x_dev, p.ldx = x.data_ptr(), K
