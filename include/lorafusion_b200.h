@@ -509,8 +509,9 @@ LF_API size_t lf_rows_workspace_bytes(int32_t T, int32_t N, int32_t r_pad, int32
 
 /*
  * y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T with i = row_slot[t]; y [T,N], dense, shares no memory with x, W,
- * the bank or row_slot.  row_slot is read on the device, so a captured call follows later changes of it and of the bank's contents.  A
- * slot at or above n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
+ * the bank or row_slot.  row_slot is read on the device, so a captured call follows later changes of it
+ * and of the bank's contents; until the call has run neither may change on another stream.  A slot at or above
+ * n_slots is treated as "no adapter" and recorded for lf_device_error (0x106).
  * bf16/f16 with K, N and ldx multiples of 8 and 16-byte aligned buffers run on the tensor cores, other
  * problems on CUDA cores.  Long batches run in chunks of 8192 rows, of 4
  * launches each (2 up to 256 rows, or 512 where r_pad is at most 32).  Enqueued on `stream`; never synchronizes.

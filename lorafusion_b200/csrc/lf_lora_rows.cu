@@ -21,9 +21,9 @@
 // then holds down to 2^-15 of the largest, 2^-37 of the largest below).  All sums are float32.
 //
 // Measured (replayed graph, weights from HBM; the shared projection alone by cuBLAS in brackets): 1 row 4096 -> 4096, rank 16
-// 12.7 us (12.9); 64 rows of 56 adapters, ranks 8 to 64, 4096 -> 14336 42 us (23); 250 rows of 219 adapters
-// of rank 16, 4096 -> 4096 37 us (11); 8192 rows of prompts, 64 adapters of ranks 8 to 64, 4096 -> 4096
-// 252 us (178).
+// 13.0 us (12.9); 64 rows of 56 adapters, ranks 8 to 64, 4096 -> 14336 43 us (23); 250 rows of 219 adapters
+// of rank 16, 4096 -> 4096 37.5 us (11); 8192 rows of prompts, 64 adapters of ranks 8 to 64, 4096 -> 4096
+// 254 us (178) in a burst, 300 after some seconds at the power cap (SM clock 1965 -> 1507 MHz).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -278,7 +278,7 @@ __device__ __forceinline__ T at_least(T v, float w, float least) {
 template <typename T>
 __device__ __forceinline__ void halves(float w, T& hi, T& lo) {
   T* const tag = nullptr;
-  constexpr float least = std::is_same<T, __half>::value ? 5.9604644775390625e-8f : 1.175494350822287508e-38f;  // 2^-24, 2^-126
+  constexpr float least = std::is_same<T, __half>::value ? 0x1p-24f : 0x1p-126f;
   hi = toward_zero(w, tag);
   const float rest = w - to_f32(hi);
   const bool two = !(fabsf(rest) > 0.f);  // also infinities and NaN
@@ -416,8 +416,9 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
     auto group_at = [&](int j) { return static_cast<int>(s.order[j * slices + (j & 1 ? slices - 1 - slice : slice)]); };
     const int rest = n_groups % slices, rounds = n_groups / slices;
     const int mine = rounds + ((rounds & 1 ? slices - 1 - slice : slice) < rest);
-    // Every CTA of a cluster sorts for itself, from slots that another stream must not change meanwhile.  If one does all the
-    // same, they differ about the groups; the cluster's barriers must not: the first CTA says whether a batch follows.
+    // Every CTA of a cluster sorts for itself, from slots that another stream must not change meanwhile.  If one does
+    // all the same, the CTAs differ about the groups, and must not about the cluster's barriers: the first CTA says
+    // whether a batch follows.
     for (int first = 0, batch; kparts > 1 || first < mine; first += batch) {
       int steps = 0, ranks = 0;  // as many groups as there is room for
       for (batch = 0; first + batch < mine; ++batch) {
@@ -895,8 +896,8 @@ __global__ void __launch_bounds__(kPlanThreads, 1) many_plan_kernel(const RowsAr
 // elements of K, where the MMA warp's eight small MMAs and their waits take what the copies do.
 // All of a CTA's K goes into one accumulator.  The tensor core drops up to 2^-25 of the running sum a step of 16, so
 // 14336 elements of one sign lose at most 2^-15 of S, as the shared projection beside it does: a hundredth of a bf16
-// rounding of y, a sixteenth of a float16 one.  (The packed shrink rotates accumulators because its S also goes into gradients,
-// which sum over all tokens.)
+// rounding of y, a sixteenth of a float16 one.  (The packed shrink rotates accumulators because its S also goes into
+// gradients, which sum over all tokens.)
 constexpr int kXBytes = kTileRows * kBK * 2;
 constexpr int kShrinkMaxStages = 8;
 constexpr int kLoadWarps = 4;

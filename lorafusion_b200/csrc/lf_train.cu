@@ -12,10 +12,10 @@
 // the rounded weight.  They are bound by HBM; passes that follow a norm pass walk the chunks
 // backwards, so they start on what the norm pass left in the 126 MB L2.
 //
-// Measured, the seven projections of a Llama-3-8B block (896 tensors of 64 adapters, ranks 8 to 64): clipping 315 MB of
-// bf16 gradients by adapter 110 us (one read, and a write of the 231 MB beyond the limit: 83 us at the rate
-// of a copy), the AdamW step, 4.4 GB, 725 us (673); 256 adapters of rank 64 on 8192 x 28672, 16.9 GB
-// 2530 us (2586).  Chunks of 8192 elements, all loads of a thread before the first use; small
+// Measured, the seven projections of a Llama-3-8B block (896 tensors of 64 adapters, ranks 8 to 64), in brackets the time
+// of the bytes at the rate of a copy: clipping 315 MB of bf16 gradients by adapter, of which 231 MB are
+// beyond the limit and written, 144 us (83; the scale pass reads them from HBM again, 35); the AdamW step, 4.4 GB, 723 to
+// 749 us (673); 256 adapters of rank 64 on 8192 x 28672, 16.9 GB, 2494 to 2594 us (2586).  Chunks of 8192 elements, all loads of a thread before the first use; small
 // calls (11 us) are the launches and their host side.
 //
 // Sums of squares are held in float64 from the first product on: a float32 square overflows above
@@ -39,8 +39,8 @@ namespace {
 constexpr int kChunk = 8192;      // elements a CTA handles: 4 to 8 16-byte loads a thread
 constexpr int kThreads = 256;
 constexpr int kFinalThreads = 512;
-// CTAs that share a chunk's update (1 / 2 / 4: 16 adapters of rank 16, 4096 -> 4096 22.4 / 20.8 / 20.5 us, the 896 tensors
-// named above 721 / 711 / 738).
+// CTAs that share a chunk's update (1 / 2 / 4, in turn on one GPU: 16 adapters of rank 16, 4096 -> 4096 22.4 / 20.8 / 20.5
+// us, the 896 tensors named above 721 / 711 / 738).
 constexpr int kUpdateParts = 2;
 constexpr int kGroupsPerLaunch = 4096;  // groups whose presence bits fit one launch's parameters
 
