@@ -487,6 +487,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
       }
       if (kparts > 1) {
         if (tid == 0) s_more = first + batch < mine;
+        __syncwarp();
         cluster_sync_all();
         float go = 0.f;  // the last warp has the least to add up
         if (tid == kShrinkThreads - 1) go = ld_cluster_f32(map_to_cta(smem_u32(&s_more), 0));
@@ -564,6 +565,7 @@ __global__ void __launch_bounds__(kShrinkThreads, 2) rows_lora_kernel(const Rows
         }
       }
       if (kparts > 1) {
+        __syncwarp();
         cluster_wait();
         if (!s_go) break;
       }
