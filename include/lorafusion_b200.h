@@ -51,6 +51,9 @@ typedef enum lf_status {
 
 typedef enum lf_dtype { LF_F32 = 0, LF_BF16 = 1, LF_F16 = 2 } lf_dtype;
 
+/* How a frozen weight is held: dense in the problem's dtype, or in 4 bits (lf_mx4_quantize). */
+typedef enum lf_weight_format { LF_WEIGHT_DENSE = 0, LF_WEIGHT_MX4 = 1 } lf_weight_format;
+
 /* Rows per fused-row tile used by every kernel's routing tables. */
 #define LF_TILE_ROWS 128
 
@@ -475,10 +478,10 @@ typedef struct lf_rows_problem {
   int32_t T, K, N;           /* rows, in_features, out_features */
   int32_t n_slots, r_pad;    /* slots of the bank; its padded rank: 16, 32, 64 or 128 */
   int32_t row_slot_bytes;    /* bytes of one row_slot entry: 4 or 8 (signed) */
-  int32_t reserved;
+  int32_t weight_format;     /* lf_weight_format of w_dev (0: dense) */
   int64_t ldx;               /* elements from one row of x to the next, at least K */
   const void* x_dev;         /* [T] rows of K */
-  const void* w_dev;         /* [N,K] */
+  const void* w_dev;         /* [N,K], or lf_mx4_bytes(N, K) bytes in 4 bits (16-bit dtypes on the tensor-core path) */
   const void* a_bank_dev;    /* [n_slots, r_pad, K] */
   const void* b_bank_dev;    /* [n_slots, r_pad/16, N, 16]: B_i in steps of 16 ranks, 16-byte aligned */
   const int32_t* slot_rank_dev;  /* [n_slots] */
@@ -525,6 +528,78 @@ LF_API int lf_rows_launch_count(int32_t T, int32_t r_pad);
 /* 1 if lf_rows_forward on tensor cores puts the shared projection of a chunk of T rows through the CTA-pair GEMM on a
  * GPU of num_sms SMs, 0 if through the tiles of W as the M operand (host only). */
 LF_API int lf_rows_uses_pairs(int32_t T, int32_t K, int32_t N, int32_t num_sms);
+
+/* ------------------------------------------------------------------------------------------------
+ * A frozen weight in 4 bits, and dropout in front of the adapters.  No counterpart in the reference.
+ *
+ * Weights: microscaled 4-bit floating point (OCP MXFP4).  32 neighbours along K share a power of two 2^E, E = floor(log2
+ * of their largest magnitude) - 2, at least -127; a value is the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6 times 2^E, ties
+ * to the even code, larger ones 6.  A block that holds an infinity or NaN is NaN throughout.  Products take V, the values
+ * that the codes stand for, which bfloat16 holds exactly, and so does float16 where the weight was float16.
+ */
+
+/* Bytes of a weight [N, K] in 4 bits: 17/32 byte an element, N and K rounded up to 128. */
+LF_API size_t lf_mx4_bytes(int32_t N, int32_t K);
+
+/* mx4 = the weight w [N, K] (bf16 / f16, rows ldw elements apart) in 4 bits; mx4_dev 16-byte aligned, apart from w. */
+LF_API int lf_mx4_quantize(int32_t dtype, const void* w_dev, int32_t N, int32_t K, int64_t ldw, void* mx4_dev,
+                           lf_stream_t stream);
+
+/* w [N, K], dense, = the values of mx4 in `dtype` (bf16 / f16). */
+LF_API int lf_mx4_dequantize(int32_t dtype, const void* mx4_dev, int32_t N, int32_t K, void* w_dev, lf_stream_t stream);
+
+typedef struct lf_mx4_problem {
+  int32_t dtype;        /* LF_BF16 or LF_F16: of in and out */
+  int32_t T, K, N;      /* rows; in_features and out_features of the weight */
+  int32_t transpose;    /* 0: out [T,N] = in [T,K] V^T; 1: out [T,K] = in [T,N] V */
+  int32_t reserved;
+  int64_t ld;           /* elements from one row of in to the next */
+  const void* in_dev;
+  const void* mx4_dev;  /* lf_mx4_bytes(N, K) */
+} lf_mx4_problem;
+
+/* Workspace bytes of lf_mx4_linear (16-byte aligned buffer).  Where K and N are multiples of 8 it is optional: with less,
+ * or null, the last round of tiles is not split.  Elsewhere it takes a dense copy of the weight. */
+LF_API size_t lf_mx4_linear_workspace_bytes(int32_t K, int32_t N);
+
+/* A product with a weight in 4 bits; out is dense and shares no memory with the operands.  With K, N and ld multiples of
+ * 8 and 16-byte aligned buffers it runs on the tensor cores in one launch, otherwise in two on CUDA cores. */
+LF_API int lf_mx4_linear(const lf_mx4_problem* prob, void* out_dev, void* workspace_dev, size_t workspace_bytes,
+                         lf_stream_t stream);
+
+/*
+ * Dropout of the adapters' input: y = x W^T + s_i (m x) A_i^T B_i^T, and in the backward grad_x = g W + m (s_i g B_i A_i),
+ * grad_A_i from m x, grad_B_i from s_i (m x) A_i^T.  The factor 1 / (1 - p_i) belongs into s_i (lf_plan_tables' scales).
+ * m is 0 or 1, computed where it is used and never stored: Philox 4x32 with ten rounds, key = seed's halves, counter =
+ * (k / 8, row, offset's halves); element k of a row takes 16 of the 128 bits, word (k % 8) / 2, low half for an even k,
+ * and is kept where that number is at least its adapter's threshold.
+ */
+typedef struct lf_dropout {
+  uint64_t seed, offset;
+  const uint32_t* slot_threshold_dev; /* [n_slots] (virtual slots): 65536 times the rate, below 65536 */
+  void* scratch_dev;                  /* 16-byte aligned */
+  size_t scratch_bytes;               /* at least lf_dropout_scratch_bytes */
+} lf_dropout;
+
+/* Scratch of dropout in lf_forward_opt (backward 0) or lf_backward_opt (1). */
+LF_API size_t lf_dropout_scratch_bytes(int32_t T, int32_t K, int32_t dtype, int32_t backward);
+
+typedef struct lf_options {
+  int32_t weight_format;      /* of prob->w_dev: lf_weight_format; LF_WEIGHT_MX4 on the tensor-core path only */
+  int32_t reserved;
+  const lf_dropout* dropout;  /* null: none */
+} lf_options;
+
+/* lf_forward_sf with options (null: none).  A backward may take S_f from a forward with the same options only. */
+LF_API int lf_forward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
+                          const lf_options* options, void* y_dev, void* workspace_dev, size_t workspace_bytes,
+                          void* tail_dev, size_t tail_bytes, int32_t* s_f_planes, lf_stream_t stream);
+
+/* lf_backward_ex, or lf_backward_peer with `peer`, with options (null: none). */
+LF_API int lf_backward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
+                           const lf_options* options, const void* grad_out_dev, const void* s_f_dev, int32_t s_f_planes,
+                           int32_t grad_ab_dtype, void* grad_x_dev, void* grad_a_dev, void* grad_b_dev,
+                           void* workspace_dev, size_t workspace_bytes, const lf_peer_reduce* peer, lf_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------------
  * Training: gradient norms, clipping and AdamW of many adapters.  No counterpart in the reference

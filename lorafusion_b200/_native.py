@@ -28,6 +28,7 @@ LF_ERR_CAPACITY = 5
 LF_ERR_DEVICE = 6
 
 LF_F32, LF_BF16, LF_F16 = 0, 1, 2
+LF_WEIGHT_DENSE, LF_WEIGHT_MX4 = 0, 1
 LF_STAGE_SHRINK, LF_STAGE_EXPAND, LF_STAGE_BASE, LF_STAGE_SINGLE_CTA, LF_STAGE_SEPARATE = 1, 2, 4, 8, 16
 LF_BSTAGE_SHRINK, LF_BSTAGE_GRAD_X, LF_BSTAGE_GRAD_AB = 1, 2, 4
 TILE_ROWS = 128
@@ -77,7 +78,7 @@ class HostChunk(ctypes.Structure):
 
 class RowsProblem(ctypes.Structure):
     _fields_ = [("dtype", _c_i32), ("T", _c_i32), ("K", _c_i32), ("N", _c_i32), ("n_slots", _c_i32),
-                ("r_pad", _c_i32), ("row_slot_bytes", _c_i32), ("reserved", _c_i32), ("ldx", ctypes.c_int64),
+                ("r_pad", _c_i32), ("row_slot_bytes", _c_i32), ("weight_format", _c_i32), ("ldx", ctypes.c_int64),
                 ("x_dev", _c_p), ("w_dev", _c_p), ("a_bank_dev", _c_p), ("b_bank_dev", _c_p),
                 ("slot_rank_dev", _c_p), ("slot_scale_dev", _c_p), ("row_slot_dev", _c_p)]
 
@@ -87,6 +88,21 @@ class BankAdapter(ctypes.Structure):
                 ("scale", ctypes.c_float), ("lda", ctypes.c_int64), ("ldb", ctypes.c_int64), ("a_dev", _c_p),
                 ("b_dev", _c_p), ("slot_a_dev", _c_p), ("slot_b_dev", _c_p), ("slot_rank_dev", _c_p),
                 ("slot_scale_dev", _c_p)]
+
+
+class Mx4Problem(ctypes.Structure):
+    _fields_ = [("dtype", _c_i32), ("T", _c_i32), ("K", _c_i32), ("N", _c_i32), ("transpose", _c_i32),
+                ("reserved", _c_i32), ("ld", ctypes.c_int64), ("in_dev", _c_p), ("mx4_dev", _c_p)]
+
+
+class Dropout(ctypes.Structure):
+    _fields_ = [("seed", ctypes.c_uint64), ("offset", ctypes.c_uint64), ("slot_threshold_dev", _c_p),
+                ("scratch_dev", _c_p), ("scratch_bytes", ctypes.c_size_t)]
+
+
+class Options(ctypes.Structure):
+    """lf_options: how the base weight is held, and dropout in front of the adapters."""
+    _fields_ = [("weight_format", _c_i32), ("reserved", _c_i32), ("dropout", ctypes.POINTER(Dropout))]
 
 
 class AdamWArgs(ctypes.Structure):
@@ -193,6 +209,24 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_rows_launch_count.restype = ctypes.c_int
     L.lf_rows_uses_pairs.argtypes = [_c_i32, _c_i32, _c_i32, _c_i32]
     L.lf_rows_uses_pairs.restype = ctypes.c_int
+    L.lf_mx4_bytes.argtypes = [_c_i32, _c_i32]
+    L.lf_mx4_bytes.restype = ctypes.c_size_t
+    L.lf_mx4_quantize.argtypes = [_c_i32, _c_p, _c_i32, _c_i32, ctypes.c_int64, _c_p, _c_p]
+    L.lf_mx4_quantize.restype = ctypes.c_int
+    L.lf_mx4_dequantize.argtypes = [_c_i32, _c_p, _c_i32, _c_i32, _c_p, _c_p]
+    L.lf_mx4_dequantize.restype = ctypes.c_int
+    L.lf_mx4_linear_workspace_bytes.argtypes = [_c_i32, _c_i32]
+    L.lf_mx4_linear_workspace_bytes.restype = ctypes.c_size_t
+    L.lf_mx4_linear.argtypes = [P(Mx4Problem), _c_p, _c_p, ctypes.c_size_t, _c_p]
+    L.lf_mx4_linear.restype = ctypes.c_int
+    L.lf_dropout_scratch_bytes.argtypes = [_c_i32, _c_i32, _c_i32, _c_i32]
+    L.lf_dropout_scratch_bytes.restype = ctypes.c_size_t
+    L.lf_forward_opt.argtypes = [P(Problem), P(PlanInfo), _c_p, P(Options), _c_p, _c_p, ctypes.c_size_t, _c_p,
+                                 ctypes.c_size_t, P(_c_i32), _c_p]
+    L.lf_forward_opt.restype = ctypes.c_int
+    L.lf_backward_opt.argtypes = [P(Problem), P(PlanInfo), _c_p, P(Options), _c_p, _c_p, _c_i32, _c_i32, _c_p, _c_p,
+                                  _c_p, _c_p, ctypes.c_size_t, P(PeerReduce), _c_p]
+    L.lf_backward_opt.restype = ctypes.c_int
     L.lf_grad_clip_workspace_bytes.argtypes = [_c_p, _c_i32, _c_i32]
     L.lf_grad_clip_workspace_bytes.restype = ctypes.c_size_t
     L.lf_grad_clip.argtypes = [_c_p, _c_i32, _c_i32, _c_i32, _c_i32, ctypes.c_double, _c_p, _c_p, ctypes.c_size_t,

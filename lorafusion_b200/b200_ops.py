@@ -36,10 +36,12 @@ import numpy as np
 import torch
 
 from lorafusion_b200 import _native as nat
+from lorafusion_b200.config import AdapterDropout
+from lorafusion_b200.quant import MX4Weight
 
 _DTYPE_CODE = {torch.float32: nat.LF_F32, torch.bfloat16: nat.LF_BF16, torch.float16: nat.LF_F16}
 
-__all__ = ["fused_lora_forward", "fused_lora_backward", "fused_lora_forward_host", "prepare_forward",
+__all__ = ["AdapterDropout", "fused_lora_forward", "fused_lora_backward", "fused_lora_forward_host", "prepare_forward",
            "PreparedForward", "prepare_backward", "PreparedBackward", "clear_weight_cache", "release",
            "last_launch_count", "use_cooperative_launch", "CudaCorePathWarning"]
 
@@ -206,7 +208,7 @@ def _plan_tables(starts, ends, route_slot, total_rows, ranks, scales, n_slots):
 
 
 class _Plan:
-    __slots__ = ("info", "table_dev", "slots", "ranks", "vslots")
+    __slots__ = ("info", "table_dev", "slots", "ranks", "vslots", "thresholds")
 
     def __init__(self, info, table_dev, slots, ranks):
         self.info = info
@@ -214,6 +216,7 @@ class _Plan:
         self.slots = slots
         self.ranks = ranks
         self.vslots = _virtual_slots(ranks)
+        self.thresholds: dict = {}  # dropout thresholds of the slots -> those of the virtual slots on the device
 
 
 class _AdapterSet:
@@ -268,8 +271,8 @@ def _adapters(rts: _Routes, lora_a, lora_b, adapters) -> _AdapterSet:
     return rec
 
 
-def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device) -> _Plan:
-    ranks, scales = aset.ranks, aset.scales
+def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, scales=None) -> _Plan:
+    ranks, scales = aset.ranks, aset.scales if scales is None else scales
     for pr, ps, pd, plan in rts.plans:
         if pd == device and pr == ranks and ps == scales:
             return plan
@@ -360,6 +363,8 @@ def _fill_packs(entry, plan: _Plan, dtype, K, N, device, which) -> None:
 
 def _weight(base_weight: torch.Tensor, dtype, device) -> torch.Tensor:
     """Base weight as a contiguous tensor of the activation dtype (converted copies cached)."""
+    if isinstance(base_weight, MX4Weight):
+        raise ValueError("this call takes a dense base_weight (MX4Weight.dequantize)")
     if base_weight.device != device:
         raise ValueError(f"base_weight must live on {device}")
     if base_weight.dtype == dtype and base_weight.is_contiguous():
@@ -403,12 +408,82 @@ def _problem(code, T, K, N, x, w, packs) -> nat.Problem:
     return p
 
 
-def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing) -> torch.Tensor:
+def _base(base_weight, x: torch.Tensor):
+    """(tensor that holds the base weight, whether it is the data of one in 4 bits).  A problem the tensor-core path
+    cannot address takes a dense copy of a weight in 4 bits, made within the call."""
+    if not isinstance(base_weight, MX4Weight):
+        return _weight(base_weight, x.dtype, x.device), False
+    if base_weight.dtype is not x.dtype:
+        raise ValueError(f"x ({x.dtype}) must have the dtype of the weight in 4 bits ({base_weight.dtype})")
+    if base_weight.device != x.device:
+        raise ValueError(f"base_weight must live on {x.device}")
+    N, K = base_weight.shape
+    if N % 8 or K % 8:
+        return base_weight.dequantize(), False
+    return base_weight.data, True
+
+
+def _shape_of(base_weight, K: int) -> int:
+    """out_features of a base weight that fits activations of K features."""
+    shape = tuple(base_weight.shape)
+    if len(shape) != 2 or shape[1] != K:
+        raise ValueError(f"base_weight {shape} does not match x of {K} features")
+    return shape[0]
+
+
+class _Drop:
+    """Dropout of one call: thresholds of its slots and the factors that go with them."""
+
+    __slots__ = ("thresholds", "seed", "offset")
+
+    def __init__(self, thresholds, seed, offset):
+        self.thresholds, self.seed, self.offset = thresholds, seed, offset
+
+    def scales(self, scales):
+        return tuple(s * (65536.0 / (65536 - t)) for s, t in zip(scales, self.thresholds))
+
+    def args(self, plan: _Plan, T: int, K: int, code: int, backward: bool, device):
+        """lf_dropout, and what it points at."""
+        table = plan.thresholds.get(self.thresholds)
+        if table is None:
+            while len(plan.thresholds) >= 8:
+                plan.thresholds.pop(next(iter(plan.thresholds)))
+            host = torch.tensor([self.thresholds[i] for i, _, _ in plan.vslots] or [0], dtype=torch.int32)
+            table = plan.thresholds[self.thresholds] = host.to(device)
+        scratch = torch.empty(max(int(nat.lib().lf_dropout_scratch_bytes(T, K, code, int(backward))), 16),
+                              dtype=torch.uint8, device=device)
+        return nat.Dropout(self.seed, self.offset, table.data_ptr(), scratch.data_ptr(), scratch.numel()), scratch
+
+
+# A float16 rank product s / (1 - p) x A^T must stay below 65504: factors beyond this one, which float16 training would
+# hardly survive, are refused there rather than turned into infinities.
+_F16_MAX_FACTOR = 64.0
+
+
+def _drop(dropout, rts: _Routes, dtype) -> _Drop | None:
+    """The call's dropout, or None where no adapter of the call has any."""
+    if dropout is None:
+        return None
+    if not isinstance(dropout, AdapterDropout):
+        raise ValueError(f"dropout must be an AdapterDropout or None, got {type(dropout).__name__}")
+    thresholds = tuple(map(dropout.threshold, rts.slots))
+    if dtype == torch.float16 and any(t > 65536 - 65536 / _F16_MAX_FACTOR for t in thresholds):
+        raise ValueError(f"float16 calls take dropout rates up to {1 - 1 / _F16_MAX_FACTOR}")
+    return _Drop(thresholds, dropout.seed, dropout.offset) if any(thresholds) else None
+
+
+def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
+                       dropout: AdapterDropout | None = None) -> torch.Tensor:
     """``y = x W^T + s_i (x A_i^T) B_i^T`` per routed row range.
 
     Same contract as ``mock_ops.fused_lora_forward`` (mock_ops.py:15-48):
     ``routing.validate`` runs first (``ValueError``); the result is a new
     ``[T, out_features]`` tensor in ``x.dtype``.
+
+    Two things have no counterpart in the reference.  ``base_weight`` may be a ``quant.MX4Weight`` of x's dtype
+    and device.  ``dropout`` (keyword only) puts a mask in front of the adapters: ``y = x W^T + s_i / (1 - p_i) (m x)
+    A_i^T B_i^T``, a dropped element being zero whatever it was.  A call captured into a CUDA graph repeats its mask
+    in every replay.
     """
     global _last_launches
     rts = _routes(routing, x.shape[0])
@@ -417,14 +492,15 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing) -> tor
     x = _activation(x, "x")
     device = x.device
     T, K = x.shape
-    N = base_weight.shape[0]
-    if base_weight.dim() != 2 or base_weight.shape[1] != K:
-        raise ValueError(f"base_weight {tuple(base_weight.shape)} does not match x {tuple(x.shape)}")
+    N = _shape_of(base_weight, K)
     dtype = x.dtype
     code = _DTYPE_CODE[dtype]
+    drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    w = _weight(base_weight, dtype, device)
-    plan = _plan(rts, aset, T, device)
+    w, mx4 = _base(base_weight, x)
+    if mx4 and x.data_ptr() % 16:
+        x = x.detach().clone()
+    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
     packs = _pack(plan, aset, dtype, K, N, device, backward=False)
     y = torch.empty((T, N), dtype=dtype, device=device)
     if T == 0 or N == 0:
@@ -441,14 +517,30 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing) -> tor
     prob = _problem(code, T, K, N, x, w, packs)
     stream = torch.cuda.current_stream(device).cuda_stream
     planes = ctypes.c_int32(0)
-    rc = L.lf_forward_sf(ctypes.byref(prob), info, plan.table_dev.data_ptr(), y.data_ptr(), ws.data_ptr(), ws.numel(),
-                         tail.data_ptr(), tail.numel(), ctypes.byref(planes), stream)
-    nat.check(rc, "lf_forward_sf")
+    opt, keep = _options(mx4, drop, plan, T, K, code, False, device)
+    with nat.on_device(device.index):
+        rc = L.lf_forward_opt(ctypes.byref(prob), info, plan.table_dev.data_ptr(), opt, y.data_ptr(), ws.data_ptr(),
+                              ws.numel(), tail.data_ptr(), tail.numel(), ctypes.byref(planes), stream)
+    nat.check(rc, "lf_forward_opt")
     # 2 K-half planes: shrink inside the GEMM launch (1 launch); 1: shrink launched on its own
     _last_launches = {2: 1, 1: 2}.get(planes.value) or int(L.lf_forward_launch_count(ctypes.byref(prob), info))
-    if planes.value > 0 and plan.info.n_segtiles > 0:
+    if drop is not None:
+        _last_launches += 1
+    elif planes.value > 0 and plan.info.n_segtiles > 0:
         _save_sf(x_in, rts, plan, aset, ws, planes.value)
     return y
+
+
+def _options(mx4: bool, drop: _Drop | None, plan: _Plan, T: int, K: int, code: int, backward: bool, device):
+    """lf_options of a call (None for a plain one), and what must live until it is enqueued."""
+    if not mx4 and drop is None:
+        return None, None
+    opt = nat.Options(nat.LF_WEIGHT_MX4 if mx4 else nat.LF_WEIGHT_DENSE, 0, None)
+    keep = None
+    if drop is not None:
+        args, keep = drop.args(plan, T, K, code, backward, device)
+        opt.dropout = ctypes.pointer(args)
+    return ctypes.byref(opt), (opt, keep)
 
 
 def _save_sf(x, rts, plan, aset, ws, planes: int) -> None:
@@ -527,7 +619,7 @@ def prepare_forward(x, base_weight, lora_a, lora_b, adapters, routing) -> Prepar
 
 
 def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, *, grad_dtype=None,
-                        peer=None):
+                        peer=None, dropout: AdapterDropout | None = None):
     """Return ``(grad_x, grad_lora_a, grad_lora_b)`` as ``mock_ops.fused_lora_backward``.
 
     mock_ops.py:51-95: the base weight is frozen (no gradient); the dicts hold
@@ -539,6 +631,8 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     gradients of adapters whose rows span GPUs inside the dA/dB kernel, over NVLink: every rank
     calls it for its own rows, and each rank's dicts then hold the summed gradients of every
     spanning adapter, held here or not (``lf_backward_peer``).
+    ``base_weight`` and ``dropout`` as in :func:`fused_lora_forward`: with the forward's ``dropout`` these are the
+    gradients of its result, ``grad_x = g W + m (s_i / (1 - p_i) g B_i A_i)``.
     """
     global _last_launches
     rts = _routes(routing, x.shape[0])
@@ -548,11 +642,9 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     g = _activation(grad_out, "grad_out")
     device = x.device
     T, K = x.shape
-    N = base_weight.shape[0]
+    N = _shape_of(base_weight, K)
     if g.shape != (T, N):
         raise ValueError(f"grad_out {tuple(g.shape)} does not match [{T}, {N}]")
-    if base_weight.dim() != 2 or base_weight.shape[1] != K:
-        raise ValueError(f"base_weight {tuple(base_weight.shape)} does not match x {tuple(x.shape)}")
     dtype = x.dtype
     if g.dtype != dtype:
         g = g.to(dtype)
@@ -560,9 +652,12 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     gdt = dtype if grad_dtype is None else grad_dtype
     if gdt not in (dtype, torch.float32):
         raise ValueError(f"grad_dtype must be None, x.dtype or torch.float32, got {grad_dtype}")
+    drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    w = _weight(base_weight, dtype, device)
-    plan = _plan(rts, aset, T, device)
+    w, mx4 = _base(base_weight, x)
+    if mx4:
+        x, g = (t.detach().clone() if t.data_ptr() % 16 else t for t in (x, g))
+    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
     packs = _pack(plan, aset, dtype, K, N, device, backward=True)
     info = plan.info
     rtot = info.rank_total
@@ -577,9 +672,10 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=device)
     prob = _problem(code, T, K, N, x, w, packs)
     stream = torch.cuda.current_stream(device).cuda_stream
-    saved = _saved_sf(x_in, rts, plan, aset) if dtype != torch.float32 else None
+    saved = _saved_sf(x_in, rts, plan, aset) if dtype != torch.float32 and drop is None else None
     sf_ptr, sf_planes = (saved[0].data_ptr(), saved[1]) if saved is not None else (None, 0)
     # S_f from the forward on these inputs, when there was one: no second s x A^T shrink
+    pr = None
     if ext is not None:
         peer.ensure(len(peer.vslots) * (-(-N // 128) + -(-K // 128)))
         pr = nat.PeerReduce(world=peer.world, rank=peer.rank, n_span=len(peer.vslots), r_pad_x=peer.r_pad_x,
@@ -588,18 +684,18 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
             pr.exchange[r] = ptr
         pr.slot_span_dev = ext.slot_span.data_ptr()
         pr.span_info_dev = ext.span_info.data_ptr()
-        rc = L.lf_backward_peer(ctypes.byref(prob), ctypes.byref(info), plan.table_dev.data_ptr(), g.data_ptr(),
-                                sf_ptr, sf_planes, _DTYPE_CODE[gdt], grad_x.data_ptr(), ga_flat.data_ptr(),
-                                gb_flat.data_ptr(), ws.data_ptr(), ws.numel(), ctypes.byref(pr), stream)
-    else:
-        rc = L.lf_backward_ex(ctypes.byref(prob), ctypes.byref(info), plan.table_dev.data_ptr(), g.data_ptr(),
-                              sf_ptr, sf_planes, _DTYPE_CODE[gdt], grad_x.data_ptr(), ga_flat.data_ptr(),
-                              gb_flat.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+    opt, keep = _options(mx4, drop, plan, T, K, code, True, device)
+    with nat.on_device(device.index):
+        rc = L.lf_backward_opt(ctypes.byref(prob), ctypes.byref(info), plan.table_dev.data_ptr(), opt, g.data_ptr(),
+                               sf_ptr, sf_planes, _DTYPE_CODE[gdt], grad_x.data_ptr(), ga_flat.data_ptr(),
+                               gb_flat.data_ptr(), ws.data_ptr(), ws.numel(), pr and ctypes.byref(pr), stream)
     if saved is not None:
         saved[0].record_stream(torch.cuda.current_stream(device))
-    nat.check(rc, "lf_backward_peer" if ext is not None else "lf_backward_ex")
+    nat.check(rc, "lf_backward_opt")
     n_launch = max(0, int(L.lf_backward_launch_count(ctypes.byref(prob), ctypes.byref(info))))
     _last_launches = n_launch - 1 if saved is not None and n_launch == 4 else n_launch
+    if drop is not None:
+        _last_launches = 6  # mask, two shrinks, expand, grad_x, dA and dB; on CUDA cores mask, two, grad_x, two
     grad_a, grad_b = _grad_dicts(plan, ga_flat, gb_flat, K, N)
     if ext is not None:  # spanning adapters not held here: their summed blocks after the local ones
         for aid, parts in ext.nonheld.items():
@@ -832,6 +928,8 @@ def fused_lora_forward_host(x_host, base_weight, lora_a, lora_b, adapters, routi
     """
     global _last_launches
     rts = _routes(routing, x_host.shape[0])
+    if isinstance(base_weight, MX4Weight):
+        raise ValueError("this call takes a dense base_weight (MX4Weight.dequantize)")
     if x_host.is_cuda or not base_weight.is_cuda:
         raise ValueError("x_host must be a host tensor and base_weight a CUDA tensor")
     if chunk_rows <= 0 or chunk_rows % 256:

@@ -11,6 +11,7 @@ reference's own dataclasses work unchanged as inputs.
 
 from __future__ import annotations
 
+from collections.abc import Mapping
 from dataclasses import dataclass, field
 
 
@@ -79,3 +80,38 @@ class TileRoutingConfig:
             expected_start = r.row_end
         if covered != total_rows:
             raise ValueError(f"Routing covers {covered} rows, expected {total_rows}")
+
+
+@dataclass(frozen=True)
+class AdapterDropout:
+    """Dropout in front of the adapters of one fused call (no counterpart in the reference).
+
+    ``rates``: one rate for all adapters, or a mapping adapter id -> rate that names every adapter of the call; ``0 <= rate
+    < 1``, taken to the nearest multiple of 1/65536 (and then below 1; float16 calls take rates up to 63/64).  ``seed`` and ``offset``, ``0 .. 2**64 - 1``,
+    choose the mask: element ``(t, k)`` of ``x`` is dropped by a number that depends on seed, offset, ``t`` and ``k`` alone
+    (Philox 4x32-10), so the forward and the backward that get the same object agree on it and nothing of it is
+    stored.  Take another offset for every step and every projection whose mask should be its own.
+    """
+
+    rates: float | Mapping[int, float]
+    seed: int
+    offset: int = 0
+
+    def __post_init__(self) -> None:
+        for name in ("seed", "offset"):
+            v = getattr(self, name)
+            if isinstance(v, bool) or not isinstance(v, int) or not 0 <= v < 1 << 64:
+                raise ValueError(f"{name} must be a whole number 0 .. 2**64 - 1, got {v!r}")
+        for r in self.rates.values() if isinstance(self.rates, Mapping) else (self.rates,):
+            self._threshold(r)
+
+    @staticmethod
+    def _threshold(rate: float) -> int:
+        t = round(float(rate) * 65536) if 0.0 <= rate < 1.0 else 65536
+        if t >= 65536:
+            raise ValueError(f"a dropout rate must be at least 0 and below 1 (to 1/65536), got {rate!r}")
+        return t
+
+    def threshold(self, adapter_id: int) -> int:
+        """65536 times the adapter's rate, a whole number (``KeyError`` for an adapter that the mapping lacks)."""
+        return self._threshold(self.rates[adapter_id] if isinstance(self.rates, Mapping) else self.rates)

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "lf_internal.cuh"
+#include "lf_mx4.cuh"
 #include "lf_ptx.cuh"
 
 namespace lf {
@@ -278,14 +279,57 @@ extern "C" int lf_pack_adapters(int32_t src_dtype, int32_t dst_dtype, const uint
 }
 
 namespace {
+// What lf_options asks for, checked.
+struct Options {
+  bool mx4 = false;
+  DropArgs drop{0, 0, nullptr};
+  char* scratch = nullptr;  // dropout's
+};
+size_t drop_scratch_mask(const lf_problem* p) {
+  return align256(static_cast<size_t>(p->T) * static_cast<size_t>(p->K) * static_cast<size_t>(elem_bytes(p->dtype)));
+}
+int read_options(const lf_options* opt, const lf_problem* prob, const lf_plan_info* info, bool backward, Options* out) {
+  if (!opt) return LF_OK;
+  if (opt->weight_format != LF_WEIGHT_DENSE && opt->weight_format != LF_WEIGHT_MX4) return LF_ERR_INVALID_ARG;
+  out->mx4 = opt->weight_format == LF_WEIGHT_MX4;
+  if (out->mx4 && prob->dtype == LF_F32) return LF_ERR_UNSUPPORTED;
+  const lf_dropout* d = opt->dropout;
+  if (!d || info->n_slots == 0 || info->n_segtiles == 0) return LF_OK;
+  if (!d->slot_threshold_dev) return LF_ERR_INVALID_ARG;
+  if (!d->scratch_dev || !aligned16(d->scratch_dev)) return LF_ERR_INVALID_ARG;
+  if (d->scratch_bytes < lf_dropout_scratch_bytes(prob->T, prob->K, prob->dtype, backward ? 1 : 0)) return LF_ERR_CAPACITY;
+  out->drop = DropArgs{d->seed, d->offset, d->slot_threshold_dev};
+  out->scratch = static_cast<char*>(d->scratch_dev);
+  return LF_OK;
+}
+// Launches hand results to one another inside a grid through flags that hold a number no earlier launch used.  A launch
+// captured into a graph repeats its number in every replay, so there the flags are cleared first, in the graph.
+cudaError_t fresh_flags(bool captured, void* flags, size_t bytes, cudaStream_t st) {
+  return captured && flags ? cudaMemsetAsync(flags, 0, bytes, st) : cudaSuccess;
+}
+bool is_captured(cudaStream_t st) {
+  cudaStreamCaptureStatus s = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &s) != cudaSuccess) {
+    (void)cudaGetLastError();  // the legacy stream beside another one's capture: not captured itself
+    return false;
+  }
+  return s == cudaStreamCaptureStatusActive;
+}
+PairMx4 mx4_view(const void* data, int N, int K) {
+  return PairMx4{static_cast<const uint8_t*>(data), mx4_row_tiles(N), mx4_col_blocks(K)};
+}
+
 // The forward stages; *sf_planes (if given) receives the K-half planes of S_f the shrink left in
 // the workspace (2 when it ran inside the GEMM launch, 1 as a launch of its own, 0 without a
 // tensor-core shrink), the value lf_backward_sf needs.
 int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev, void* y_dev,
                  void* workspace_dev, size_t workspace_bytes, void* tail_dev, size_t tail_bytes, int32_t stages,
-                 lf_stream_t stream, int32_t* sf_planes) {
+                 lf_stream_t stream, int32_t* sf_planes, const lf_options* options = nullptr) {
   if (sf_planes) *sf_planes = 0;
   int rc = check_problem(prob, info, table_dev);
+  if (rc != LF_OK) return rc;
+  Options opt;
+  rc = read_options(options, prob, info, false, &opt);
   if (rc != LF_OK) return rc;
   if (stages <= 0 || stages > 31 || ((stages & LF_STAGE_EXPAND) && (stages & LF_STAGE_BASE))) return LF_ERR_INVALID_ARG;
   const int T = prob->T, K = prob->K, N = prob->N;
@@ -303,16 +347,26 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
   const bool do_shrink = (stages & LF_STAGE_SHRINK) != 0;
   const bool do_gemm = (stages & (LF_STAGE_EXPAND | LF_STAGE_BASE)) != 0;
   const bool lora = (stages & LF_STAGE_EXPAND) != 0 && info->n_segtiles > 0;
+  const PairMx4 mx4 = opt.mx4 ? mx4_view(prob->w_dev, N, K) : PairMx4{};
+  const PairMx4* mx4p = opt.mx4 ? &mx4 : nullptr;
+  const void* xa = prob->x_dev;  // the adapters' input
+  if (opt.drop.threshold && do_shrink) {
+    e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);
+    if (e != cudaSuccess) return LF_ERR_CUDA;
+    xa = opt.scratch;
+  }
 
   if (tc_eligible(prob, {prob->x_dev, prob->w_dev, prob->a_pack_dev, prob->b_pack_dev, y_dev, workspace_dev})) {
     const bool single = (stages & LF_STAGE_SINGLE_CTA) != 0;
+    if (single && opt.mx4) return LF_ERR_UNSUPPORTED;
     const uint32_t nbox = single ? 256 : 128;  // rows of W / B_i per CTA and tile
     TcMaps maps;
-    CUtensorMap a_map;
+    CUtensorMap a_map, xa_map;
     const size_t es = 2;
     const uint64_t s_rows = kSextPlanes * static_cast<uint64_t>(info->n_segtiles + 1) * LF_TILE_ROWS;
     bool ok = make_map(&maps.p, dt, prob->x_dev, K, T, K * es, 64, 128) &&
-              make_map(&maps.q, dt, prob->w_dev, K, N, K * es, 64, nbox) &&
+              (opt.mx4 || make_map(&maps.q, dt, prob->w_dev, K, N, K * es, 64, nbox)) &&
+              make_map(&xa_map, dt, xa, K, T, K * es, 64, 128) &&
               make_map(&a_map, dt, prob->a_pack_dev, K, static_cast<uint64_t>(info->n_slots) * rp, K * es, 64, rp);
     if (info->n_segtiles > 0)
       ok = ok && make_map(&maps.s, dt, workspace_dev, rp, s_rows, rp * es, rp, 128) &&
@@ -321,14 +375,20 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       maps.s = maps.l = maps.p;
     ok = ok && make_map(&maps.o, dt, y_dev, N, T, N * es, 64, 32);
     if (!ok) return LF_ERR_UNSUPPORTED;
+    if (opt.mx4) maps.q = maps.p;  // not used
     // Shrink and expand requested together: run the shrink on CTA pairs the GEMM's round count
     // leaves idle, inside the same launch, when there are enough of them.
     const bool separate = (stages & LF_STAGE_SEPARATE) != 0;
-    const bool fuse = !single && !separate && do_shrink && lora && cosched_allowed(ds);
+    const bool fuse = !single && !separate && do_shrink && lora && cosched_allowed(ds) && !opt.drop.threshold;
     const int spare = fuse && !cosched_prologue() ? pair_spare_pairs(T, N, ds->num_sms, info->n_shrink_units) : 0;
     // the K-split tail needs a cooperative launch too
     const PairTail tail = tail_dev ? tail_scratch(tail_dev, tail_bytes, 0)
                                    : tail_scratch(workspace_dev, workspace_bytes, forward_min_workspace_bytes(info));
+    const bool captured = is_captured(st);
+    if (do_gemm) e = fresh_flags(captured, tail.flags, kTailFlagBytes, st);
+    if (fuse && e == cudaSuccess)
+      e = fresh_flags(captured, static_cast<char*>(workspace_dev) + sext_bytes(info), flag_bytes(info), st);
+    if (e != cudaSuccess) return LF_ERR_CUDA;
     if (fuse && (spare > 0 || cosched_prologue())) {
       PairShrink sh{};
       sh.a_map = a_map;
@@ -338,7 +398,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       sh.wait_gen = wait_generation(sh.gen);
       sh.n_pairs = spare;
       sh.prologue = cosched_prologue();
-      e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, &sh, &tail);
+      e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, &sh, &tail, nullptr, mx4p);
       if (e == cudaSuccess) {
         if (sf_planes) *sf_planes = 2;
         return LF_OK;
@@ -348,7 +408,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       refuse_cosched(ds, e);
     }
     if (do_shrink) {
-      e = tc_shrink(dt, maps.p, a_map, K, tb, workspace_dev, ds->num_sms, st);
+      e = tc_shrink(dt, xa_map, a_map, K, tb, workspace_dev, ds->num_sms, st);
       if (e != cudaSuccess) return LF_ERR_CUDA;
       if (sf_planes) *sf_planes = 1;
     }
@@ -357,24 +417,25 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
         e = tc_gemm(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st);
       } else {
         e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr,
-                         cosched_allowed(ds) ? &tail : nullptr);
+                         cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p);
         if (e != cudaSuccess && cosched_allowed(ds)) {  // cooperative launch refused: nothing ran
           refuse_cosched(ds, e);
-          e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st);
+          e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p);
         }
       }
     }
     return to_status(e);
   }
 
+  if (opt.mx4) return LF_ERR_UNSUPPORTED;
   double* s_ext = static_cast<double*>(workspace_dev);
   if (do_shrink) {
-    e = simt_shrink(dt, prob->x_dev, K, K, prob->a_pack_dev, tb, s_ext, st);
+    e = simt_shrink(dt, xa, K, K, prob->a_pack_dev, tb, s_ext, st);
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }
   if (do_gemm)
     e = simt_gemm(dt, prob->x_dev, K, prob->w_dev, K, 1, T, N, K, s_ext, lora ? prob->b_pack_dev : nullptr, tb, y_dev,
-                  N, st);
+                  N, DropArgs{}, st);
   return to_status(e);
 }
 }  // namespace
@@ -392,6 +453,25 @@ extern "C" int lf_forward_sf(const lf_problem* prob, const lf_plan_info* info, c
   if (!s_f_planes) return LF_ERR_INVALID_ARG;
   return forward_impl(prob, info, table_dev, y_dev, workspace_dev, workspace_bytes, tail_dev, tail_bytes,
                       LF_STAGE_SHRINK | LF_STAGE_EXPAND, stream, s_f_planes);
+}
+
+extern "C" size_t lf_dropout_scratch_bytes(int32_t T, int32_t K, int32_t dtype, int32_t backward) {
+  if (T < 0 || K < 0) return 0;
+  lf_problem p{};
+  p.T = T, p.K = K, p.dtype = dtype;
+  size_t n = drop_scratch_mask(&p);
+  if (backward && dtype != LF_F32) n += align256(static_cast<size_t>(T) * static_cast<size_t>(K) * 4);
+  return n;
+}
+
+extern "C" int lf_forward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
+                              const lf_options* options, void* y_dev, void* workspace_dev, size_t workspace_bytes,
+                              void* tail_dev, size_t tail_bytes, int32_t* s_f_planes, lf_stream_t stream) {
+  int32_t planes = 0;
+  const int rc = forward_impl(prob, info, table_dev, y_dev, workspace_dev, workspace_bytes, tail_dev, tail_bytes,
+                              LF_STAGE_SHRINK | LF_STAGE_EXPAND, stream, &planes, options);
+  if (s_f_planes) *s_f_planes = planes;
+  return rc;
 }
 
 extern "C" size_t lf_forward_fixed_workspace_bytes(const lf_plan_info* info, int32_t dtype) {
@@ -554,8 +634,11 @@ namespace {
 int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev, const void* grad_out_dev,
                   const void* sf_given, int sf_planes, int grad_f32, void* grad_x_dev, void* grad_a_dev,
                   void* grad_b_dev, void* workspace_dev, size_t workspace_bytes, lf_stream_t stream,
-                  int stages = 0, const lf_peer_reduce* peer = nullptr) {
+                  int stages = 0, const lf_peer_reduce* peer = nullptr, const lf_options* options = nullptr) {
   int rc = check_problem(prob, info, table_dev);
+  if (rc != LF_OK) return rc;
+  Options opt;
+  rc = read_options(options, prob, info, true, &opt);
   if (rc != LF_OK) return rc;
   GramPeer gp{};
   if (peer != nullptr) {  // spanning adapters' blocks exchanged by the gram: tensor-core path only
@@ -615,15 +698,31 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
 
   const bool tc_path = tc_eligible(prob, {prob->x_dev, prob->w_dev, prob->a_pack_dev, prob->bt_pack_dev,
                                           prob->at_pack_dev, grad_out_dev, grad_x_dev, workspace_dev});
-  if (peer != nullptr && !tc_path) return LF_ERR_UNSUPPORTED;
+  if ((peer != nullptr || opt.mx4) && !tc_path) return LF_ERR_UNSUPPORTED;
+  const PairMx4 mx4 = opt.mx4 ? mx4_view(prob->w_dev, N, K) : PairMx4{};
+  const PairMx4* mx4p = opt.mx4 ? &mx4 : nullptr;
+  const bool drop = opt.drop.threshold != nullptr;
+  const void* xa = prob->x_dev;  // the adapters' input
+  if (drop && (do_gab || (do_shrink && !reuse_sf))) {
+    e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);
+    if (e != cudaSuccess) return LF_ERR_CUDA;
+    xa = opt.scratch;
+  }
   if (tc_path) {
     CUtensorMap p_x, p_g, a_map, bt_map, sf_map, sb_map;
     TcMaps dx;
     const PairTail tail = tail_scratch(workspace_dev, workspace_bytes, backward_min_workspace_bytes(info));
+    const bool captured = is_captured(st);
+    void* gram_scratch = ws + 2 * sb + flag_bytes(info, 2);
+    if (do_gx) e = fresh_flags(captured, tail.flags, kTailFlagBytes, st);
+    if (do_gx && e == cudaSuccess) e = fresh_flags(captured, ws + 2 * sb, flag_bytes(info, 2), st);
+    if (do_gab && e == cudaSuccess)
+      e = fresh_flags(captured, static_cast<char*>(gram_scratch) + gram_counters_offset(rp), kGramMaxCounters * 4 * 8, st);
+    if (e != cudaSuccess) return LF_ERR_CUDA;
     const uint64_t s_rows = kSextPlanes * static_cast<uint64_t>(info->n_segtiles + 1) * LF_TILE_ROWS;
-    bool ok = make_map(&p_x, dt, prob->x_dev, K, T, K * es, 64, 128) &&
+    bool ok = make_map(&p_x, dt, xa, K, T, K * es, 64, 128) &&
               make_map(&p_g, dt, grad_out_dev, N, T, N * es, 64, 128) &&
-              make_map(&dx.q, dt, prob->w_dev, K, N, K * es, 64, 64);
+              (opt.mx4 || make_map(&dx.q, dt, prob->w_dev, K, N, K * es, 64, 64));
     const bool lora = info->n_segtiles > 0 && info->n_slots > 0;
     if (lora)
       ok = ok &&
@@ -635,6 +734,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
     if (do_gx) ok = ok && make_map(&dx.o, dt, grad_x_dev, K, T, K * es, 64, 32);
     if (!ok) return LF_ERR_UNSUPPORTED;
     dx.p = p_g;
+    if (opt.mx4) dx.q = p_g;  // not used
     int planes = 1;  // S_b's K-half planes (S_f's: sf_planes when reused, else the same as S_b's)
     bool gemm_done = !do_gx;
     if (lora && staged) {
@@ -654,7 +754,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
       // the forward's is reused.
       const int spare =
           cosched_allowed(ds) && !cosched_prologue() ? pair_spare_pairs(T, K, ds->num_sms, info->n_shrink_units) : 0;
-      if (cosched_allowed(ds) && (spare > 0 || cosched_prologue())) {
+      if (!drop && cosched_allowed(ds) && (spare > 0 || cosched_prologue())) {
         PairShrink sh{};
         sh.a_map = bt_map;
         sh.s_ext = s_b;
@@ -668,7 +768,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
         sh.a2_map = a_map;
         sh.s_ext2 = s_f;
         sh.K2 = K;
-        e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, &sh, &tail);
+        e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, &sh, &tail, nullptr, mx4p);
         if (e == cudaSuccess) {
           planes = 2;
           gemm_done = true;
@@ -687,12 +787,21 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
     } else {
       dx.s = dx.l = p_g;
     }
+    if (!gemm_done && drop) {  // the mask is of grad_x's adapters' part alone: it is added to g W
+      float* delta = reinterpret_cast<float*>(opt.scratch + drop_scratch_mask(prob));
+      const PairDelta d{delta, nullptr, K};
+      e = drop_expand(dt, s_b, prob->at_pack_dev, T, K, tb, opt.drop, delta, st);
+      if (e == cudaSuccess)
+        e = tc_gemm_pair(dt, true, dx, T, K, N, false, tb, grad_x_dev, K, ds->num_sms, st, nullptr, nullptr, &d, mx4p);
+      if (e != cudaSuccess) return LF_ERR_CUDA;
+      gemm_done = true;
+    }
     if (!gemm_done) {
       e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, nullptr,
-                       cosched_allowed(ds) ? &tail : nullptr);
+                       cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p);
       if (e != cudaSuccess && cosched_allowed(ds)) {  // cooperative launch refused: nothing ran
         refuse_cosched(ds, e);
-        e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st);
+        e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p);
       }
       if (e != cudaSuccess) return LF_ERR_CUDA;
     }
@@ -710,7 +819,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
       jobs[1].out = grad_a_dev;
       jobs[1].transpose_out = 1;
       jobs[1].out_f32 = grad_f32;
-      void* scratch = ws + 2 * sb + flag_bytes(info, 2);
+      void* scratch = gram_scratch;
       // the grams read hi and lo planes: 2 per K half
       const int f_planes = reuse_sf ? sf_planes : planes;
       if (f_planes == planes) {
@@ -728,19 +837,20 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
   double* sf = reinterpret_cast<double*>(ws);  // the CUDA-core path computes its own f64 S_f
   double* sbp = static_cast<double*>(s_b);
   if (do_shrink) {
-    e = simt_shrink(dt, prob->x_dev, K, K, prob->a_pack_dev, tb, sf, st);
+    e = simt_shrink(dt, xa, K, K, prob->a_pack_dev, tb, sf, st);
     if (e != cudaSuccess) return LF_ERR_CUDA;
     e = simt_shrink(dt, grad_out_dev, N, N, prob->bt_pack_dev, tb, sbp, st);
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }
   if (do_gx) {  // grad_x = g W + S_b . A   (Q(c, m) = W[m][c])
-    e = simt_gemm(dt, grad_out_dev, N, prob->w_dev, 1, K, T, K, N, sbp, prob->at_pack_dev, tb, grad_x_dev, K, st);
+    e = simt_gemm(dt, grad_out_dev, N, prob->w_dev, 1, K, T, K, N, sbp, prob->at_pack_dev, tb, grad_x_dev, K, opt.drop,
+                  st);
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }
   if (do_gab) {
     e = simt_gram(dt, grad_out_dev, N, N, sf, tb, grad_b_dev, 0, grad_f32, st);
     if (e != cudaSuccess) return LF_ERR_CUDA;
-    e = simt_gram(dt, prob->x_dev, K, K, sbp, tb, grad_a_dev, 1, grad_f32, st);
+    e = simt_gram(dt, xa, K, K, sbp, tb, grad_a_dev, 1, grad_f32, st);
   }
   return to_status(e);
 }
@@ -798,6 +908,19 @@ extern "C" int lf_backward_peer(const lf_problem* prob, const lf_plan_info* info
   return backward_impl(prob, info, table_dev, grad_out_dev, s_f_dev, s_f_dev ? s_f_planes : 0,
                        grad_ab_dtype == LF_F32 ? 1 : 0, grad_x_dev, grad_a_dev, grad_b_dev, workspace_dev,
                        workspace_bytes, stream, 0, peer);
+}
+
+extern "C" int lf_backward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
+                               const lf_options* options, const void* grad_out_dev, const void* s_f_dev,
+                               int32_t s_f_planes, int32_t grad_ab_dtype, void* grad_x_dev, void* grad_a_dev,
+                               void* grad_b_dev, void* workspace_dev, size_t workspace_bytes, const lf_peer_reduce* peer,
+                               lf_stream_t stream) {
+  if (!prob) return LF_ERR_INVALID_ARG;
+  if (s_f_dev && s_f_planes != 1 && s_f_planes != 2) return LF_ERR_INVALID_ARG;
+  if (grad_ab_dtype != prob->dtype && grad_ab_dtype != LF_F32) return LF_ERR_INVALID_ARG;
+  return backward_impl(prob, info, table_dev, grad_out_dev, s_f_dev, s_f_dev ? s_f_planes : 0,
+                       grad_ab_dtype == LF_F32 ? 1 : 0, grad_x_dev, grad_a_dev, grad_b_dev, workspace_dev,
+                       workspace_bytes, stream, 0, peer, options);
 }
 
 extern "C" size_t lf_peer_exchange_bytes(int32_t world, int32_t n_blocks, int32_t r_pad) {
@@ -907,6 +1030,8 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   if (p->dtype != LF_F32 && p->dtype != LF_BF16 && p->dtype != LF_F16) return LF_ERR_INVALID_ARG;
   if (p->r_pad != 16 && p->r_pad != 32 && p->r_pad != 64 && p->r_pad != LF_BANK_MAX_RANK) return LF_ERR_INVALID_ARG;
   if (p->row_slot_bytes != 4 && p->row_slot_bytes != 8) return LF_ERR_INVALID_ARG;
+  if (p->weight_format != LF_WEIGHT_DENSE && p->weight_format != LF_WEIGHT_MX4) return LF_ERR_INVALID_ARG;
+  const bool mx4 = p->weight_format == LF_WEIGHT_MX4;
   // what 32-bit indices of elements and of bank rows hold
   if (p->K > (1 << 24) || p->N > (1 << 24) || p->n_slots >= (1 << 24) ||
       static_cast<int64_t>(p->n_slots) * (p->r_pad / 16) * (p->N > 16 ? p->N : 16) > INT32_MAX)
@@ -924,7 +1049,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     return bytes > 0 && b < y0 + T * N * es && y0 < b + bytes;
   };
   const uint64_t n_slots = p->n_slots;
-  if (meets_y(p->x_dev, ((T - 1) * p->ldx + K) * es) || meets_y(p->w_dev, N * K * es) ||
+  if (meets_y(p->x_dev, ((T - 1) * p->ldx + K) * es) || meets_y(p->w_dev, mx4 ? mx4_bytes(p->N, p->K) : N * K * es) ||
       meets_y(p->a_bank_dev, ranks * K * es) || meets_y(p->b_bank_dev, ranks * N * es) ||
       meets_y(p->slot_rank_dev, n_slots * 4) || meets_y(p->slot_scale_dev, n_slots * 4) ||
       meets_y(p->row_slot_dev, T * p->row_slot_bytes))
@@ -961,6 +1086,8 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool tc = p->dtype != LF_F32 && p->K > 0 && p->K % 8 == 0 && p->N % 8 == 0 && p->ldx % 8 == 0 &&
                   aligned16(p->x_dev) && aligned16(p->w_dev) && aligned16(p->a_bank_dev) && aligned16(y_dev);
+  if (mx4 && !tc) return LF_ERR_UNSUPPORTED;
+  if (mx4) a.mx4 = mx4_view(p->w_dev, p->N, p->K);
   // chunks of rows share the workspace, one after another on the stream
   const char* x = static_cast<const char*>(p->x_dev);
   const char* slots = static_cast<const char*>(p->row_slot_dev);
@@ -988,8 +1115,8 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     if (many) {
       const uint64_t bank_rows = static_cast<uint64_t>(a.n_slots > 0 ? a.n_slots : 1) * a.r_pad;
       const uint64_t s_pitch = static_cast<uint64_t>(a.r_pad) * 2;
-      const void* a_bank = a.n_slots > 0 ? a.a_bank : a.w;  // an empty bank: a map that nothing uses
-      const void* b_bank = a.n_slots > 0 ? a.b_bank : a.w;
+      const void* a_bank = a.n_slots > 0 ? a.a_bank : a.x;  // an empty bank: a map that nothing uses
+      const void* b_bank = a.n_slots > 0 ? a.b_bank : a.x;
       if (!make_map(&many->a, p->dtype, a_bank, a.K, bank_rows, w_pitch, 64, 16) ||
           !make_map(&many->s_hi, p->dtype, a.s_hi, a.r_pad, a.T, s_pitch, 16, 128) ||
           !make_map(&many->s_lo, p->dtype, a.s_lo, a.r_pad, a.T, s_pitch, 16, 128) ||
@@ -999,10 +1126,11 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
     if (rows_use_pairs(a.T, a.K, a.N, ds->num_sms)) {
       TcMaps maps;
       if (!make_map(&maps.p, p->dtype, a.x, a.K, a.T, x_pitch, 64, 128) ||
-          !make_map(&maps.q, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128) ||
+          (!mx4 && !make_map(&maps.q, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128)) ||
           !make_map(&maps.o, p->dtype, a.y, a.N, a.T, static_cast<uint64_t>(a.N) * 2, 64, 32))
         return LF_ERR_UNSUPPORTED;
       maps.s = maps.l = maps.p;
+      if (mx4) maps.q = maps.p;
       Tables tb{};
       tb.r_pad = 16;
       tb.err = ds->status;
@@ -1010,18 +1138,129 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
       e = rows_lora_part(a, p->dtype, many, ds->num_sms, st);
       if (e == cudaSuccess)
         e = tc_gemm_pair(p->dtype, false, maps, a.T, a.N, a.K, false, tb, a.y, a.N, ds->num_sms, st, nullptr, nullptr,
-                         &delta);
+                         &delta, mx4 ? &a.mx4 : nullptr);
     } else {
       const RowsTiles tiles = rows_tiles(a.T, a.K, a.N, ds->num_sms);
       CUtensorMap w_map, x_map;
-      if (!make_map(&w_map, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128) ||
+      if ((!mx4 && !make_map(&w_map, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128)) ||
           !make_map(&x_map, p->dtype, a.x, a.K, a.T, x_pitch, 64, tiles.rows))
         return LF_ERR_UNSUPPORTED;
+      if (mx4) w_map = x_map;
       e = rows_forward_tc(a, p->dtype, w_map, x_map, tiles, many, ds->num_sms, st);
     }
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }
   return LF_OK;
+}
+
+// ------------------------------------------------------------------------------------- weights in 4 bits
+extern "C" size_t lf_mx4_bytes(int32_t N, int32_t K) { return N < 0 || K < 0 ? 0 : mx4_bytes(N, K); }
+
+namespace {
+bool meet(const void* a, size_t na, const void* b, size_t nb) {
+  const uintptr_t a0 = reinterpret_cast<uintptr_t>(a), b0 = reinterpret_cast<uintptr_t>(b);
+  return na > 0 && nb > 0 && a0 < b0 + nb && b0 < a0 + na;
+}
+int mx4_check(int32_t dtype, int32_t N, int32_t K) {
+  if (N < 0 || K < 0) return LF_ERR_INVALID_ARG;
+  if (dtype != LF_BF16 && dtype != LF_F16) return dtype == LF_F32 ? LF_ERR_UNSUPPORTED : LF_ERR_INVALID_ARG;
+  return N > (1 << 24) || K > (1 << 24) ? LF_ERR_UNSUPPORTED : LF_OK;
+}
+}  // namespace
+
+extern "C" int lf_mx4_quantize(int32_t dtype, const void* w_dev, int32_t N, int32_t K, int64_t ldw, void* mx4_dev,
+                               lf_stream_t stream) {
+  const int rc = mx4_check(dtype, N, K);
+  if (rc != LF_OK) return rc;
+  if (N == 0 || K == 0) return LF_OK;
+  if (!w_dev || !mx4_dev || !aligned16(mx4_dev) || (N > 1 && ldw < K)) return LF_ERR_INVALID_ARG;
+  if (meet(w_dev, (static_cast<size_t>(N - 1) * (N > 1 ? ldw : 0) + K) * 2, mx4_dev, mx4_bytes(N, K)))
+    return LF_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
+  return to_status(mx4_quantize(dtype, w_dev, N, K, ldw, mx4_dev, ds->num_sms, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" int lf_mx4_dequantize(int32_t dtype, const void* mx4_dev, int32_t N, int32_t K, void* w_dev,
+                                 lf_stream_t stream) {
+  const int rc = mx4_check(dtype, N, K);
+  if (rc != LF_OK) return rc;
+  if (N == 0 || K == 0) return LF_OK;
+  if (!w_dev || !mx4_dev || !aligned16(mx4_dev)) return LF_ERR_INVALID_ARG;
+  if (meet(w_dev, static_cast<size_t>(N) * K * 2, mx4_dev, mx4_bytes(N, K))) return LF_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
+  return to_status(mx4_dequantize(dtype, mx4_dev, N, K, w_dev, ds->num_sms, static_cast<cudaStream_t>(stream)));
+}
+
+extern "C" size_t lf_mx4_linear_workspace_bytes(int32_t K, int32_t N) {
+  if (K <= 0 || N <= 0) return 0;
+  return K % 8 || N % 8 ? align256(static_cast<size_t>(N) * static_cast<size_t>(K) * 2) : tail_scratch_bytes();
+}
+
+extern "C" int lf_mx4_linear(const lf_mx4_problem* p, void* out_dev, void* workspace_dev, size_t workspace_bytes,
+                             lf_stream_t stream) {
+  if (!p || p->T < 0 || (p->transpose != 0 && p->transpose != 1)) return LF_ERR_INVALID_ARG;
+  const int rc = mx4_check(p->dtype, p->N, p->K);
+  if (rc != LF_OK) return rc;
+  const int T = p->T, K = p->K, N = p->N, dt = p->dtype;
+  const int in = p->transpose ? N : K, out = p->transpose ? K : N;
+  if (T == 0 || out == 0) return LF_OK;
+  if (!p->in_dev || !p->mx4_dev || !out_dev || p->ld < in) return LF_ERR_INVALID_ARG;
+  if (in == 0 || !aligned16(p->mx4_dev) || !aligned16(workspace_dev)) return LF_ERR_INVALID_ARG;
+  const size_t out_bytes = static_cast<size_t>(T) * out * 2;
+  if (meet(out_dev, out_bytes, p->in_dev, (static_cast<size_t>(T - 1) * p->ld + in) * 2) ||
+      meet(out_dev, out_bytes, p->mx4_dev, mx4_bytes(N, K)))
+    return LF_ERR_INVALID_ARG;
+  DeviceState* ds = nullptr;
+  if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (K % 8 || N % 8 || p->ld % 8 || !aligned16(p->in_dev) || !aligned16(out_dev)) {
+    const size_t dense = static_cast<size_t>(N) * K * 2;
+    if (!workspace_dev || workspace_bytes < dense) return LF_ERR_CAPACITY;
+    if (meet(workspace_dev, dense, p->mx4_dev, mx4_bytes(N, K)) || meet(workspace_dev, dense, out_dev, out_bytes))
+      return LF_ERR_INVALID_ARG;
+    cudaError_t e = mx4_dequantize(dt, p->mx4_dev, N, K, workspace_dev, ds->num_sms, st);
+    const int64_t qsn = p->transpose ? 1 : K, qsk = p->transpose ? K : 1;
+    if (e == cudaSuccess)
+      e = simt_gemm(dt, p->in_dev, p->ld, workspace_dev, qsn, qsk, T, out, in, nullptr, nullptr, Tables{}, out_dev, out,
+                    DropArgs{}, st);
+    return to_status(e);
+  }
+  const PairMx4 mx4 = mx4_view(p->mx4_dev, N, K);
+  const uint64_t pitch = static_cast<uint64_t>(p->ld) * 2;
+  if (!p->transpose && T <= kRowsChunk && !rows_use_pairs(T, K, N, ds->num_sms)) {
+    RowsArgs a{};
+    a.x = p->in_dev;
+    a.y = out_dev;
+    a.ldx = p->ld;
+    a.T = T, a.K = K, a.N = N, a.r_pad = 16;
+    a.mx4 = mx4;
+    a.err = ds->status;
+    const RowsTiles tiles = rows_tiles(T, K, N, ds->num_sms);
+    CUtensorMap x_map;
+    if (!make_map(&x_map, dt, a.x, K, T, pitch, 64, tiles.rows)) return LF_ERR_UNSUPPORTED;
+    return to_status(rows_forward_tc(a, dt, x_map, x_map, tiles, nullptr, ds->num_sms, st));
+  }
+  TcMaps maps;
+  if (!make_map(&maps.p, dt, p->in_dev, in, T, pitch, 64, 128) ||
+      !make_map(&maps.o, dt, out_dev, out, T, static_cast<uint64_t>(out) * 2, 64, 32))
+    return LF_ERR_UNSUPPORTED;
+  maps.q = maps.s = maps.l = maps.p;
+  Tables tb{};
+  tb.r_pad = 16;
+  tb.err = ds->status;
+  const PairTail tail = tail_scratch(workspace_dev, workspace_bytes, 0);
+  const bool split = cosched_allowed(ds);
+  if (fresh_flags(split && is_captured(st), tail.flags, kTailFlagBytes, st) != cudaSuccess) return LF_ERR_CUDA;
+  cudaError_t e = tc_gemm_pair(dt, p->transpose != 0, maps, T, out, in, false, tb, out_dev, out, ds->num_sms, st, nullptr,
+                               split ? &tail : nullptr, nullptr, &mx4);
+  if (e != cudaSuccess && split) {  // cooperative launch refused: nothing ran
+    refuse_cosched(ds, e);
+    e = tc_gemm_pair(dt, p->transpose != 0, maps, T, out, in, false, tb, out_dev, out, ds->num_sms, st, nullptr, nullptr,
+                     nullptr, &mx4);
+  }
+  return to_status(e);
 }
 
 extern "C" int lf_device_error(int32_t* code) {

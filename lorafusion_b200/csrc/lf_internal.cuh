@@ -40,16 +40,23 @@ struct Tables {
   __device__ __forceinline__ int32_t tile_unit(int t) const { return base[off_tile_unit + t]; }
 };
 
+// Dropout in front of the adapters (lf_drop.cuh).
+struct DropArgs {
+  uint64_t seed, offset;
+  const uint32_t* threshold;  // [n_slots] 65536 times the rate of each virtual slot, on the device; null: no dropout
+};
+
 Tables make_tables(const lf_plan_info* info, const int32_t* table_dev);
 
 // --------------------------------------------------------------- SIMT (any dtype, f64 sums)
 // S_ext[st][row][j] = (row in segment) ? scale * sum_k P[tile*128+row][k] * Apk[slot][j][k] : 0
 cudaError_t simt_shrink(int dtype, const void* P, int64_t ldp, int Kred, const void* apk, const Tables& tb,
                         double* s_ext, cudaStream_t st);
+// (with `drop` the second sum is masked by element (t, n))
 // out[t][n] = sum_k P[t][k] Q(n,k) + sum_j S_ext[st(t)][row][j] * L[slot][n][j],  Q(n,k) = Q[n*qsn + k*qsk]
 cudaError_t simt_gemm(int dtype, const void* P, int64_t ldp, const void* Q, int64_t qsn, int64_t qsk, int T, int Nout,
                       int Kred, const double* s_ext, const void* lpk, const Tables& tb, void* out, int64_t ldo,
-                      cudaStream_t st);
+                      const DropArgs& drop, cudaStream_t st);
 // grad[slot] = sum_{rows of slot} D[row][c] * S_ext[..][row][j]; layout [C][rank] or [rank][C] (transpose_out),
 // in the input type or (out_f32) in float
 cudaError_t simt_gram(int dtype, const void* D, int64_t ldd, int C, const double* s_ext, const Tables& tb,
@@ -101,12 +108,17 @@ struct PairTail {
   int slots;
   uint64_t gen;
 };
-// Float32 [T][ld] added to the product of rows whose word in `eff` is not all ones, written by the launch
-// ahead on the stream (this one starts before it has finished).
+// Float32 [T][ld] added to the product of rows whose word in `eff` is not all ones (of every row without `eff`), written
+// by the launch ahead on the stream (this one starts before it has finished).
 struct PairDelta {
   const float* delta;
   const uint32_t* eff;
   int64_t ld;  // a multiple of 4
+};
+// A weight held in 4 bits (lf_mx4.cuh) in the place of Q.
+struct PairMx4 {
+  const uint8_t* data;
+  int row_tiles, col_blocks;
 };
 // CTA pairs the pair GEMM can leave to a co-scheduled shrink without adding a round (0: none).
 int pair_spare_pairs(int T, int Nout, int num_sms, int n_units);
@@ -114,7 +126,7 @@ int pair_spare_pairs(int T, int Nout, int num_sms, int n_units);
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
                          const PairShrink* shrink = nullptr, const PairTail* tail = nullptr,
-                         const PairDelta* delta = nullptr);
+                         const PairDelta* delta = nullptr, const PairMx4* mx4 = nullptr);
 // Forward workspace without the tail scratch (the least lf_forward accepts).
 size_t forward_min_workspace_bytes(const lf_plan_info* info);
 // Gram load balance: slots (slot_order positions) the kernel can split into parts, and the
@@ -122,6 +134,7 @@ size_t forward_min_workspace_bytes(const lf_plan_info* info);
 constexpr int kGramMaxSlots = 512;
 constexpr int kGramMaxPartials = 640;
 constexpr int kGramMaxCounters = 1280;
+inline size_t gram_counters_offset(int r_pad) { return static_cast<size_t>(kGramMaxPartials) * 128 * r_pad * 4; }
 inline size_t gram_scratch_bytes(int r_pad) {
   return (static_cast<size_t>(kGramMaxPartials) * 128 * r_pad * 4 + static_cast<size_t>(kGramMaxCounters) * 4 * 8 +
           255) & ~size_t(255);
@@ -177,7 +190,7 @@ struct RowsArgs {
   const void* b_bank;
   const int32_t* slot_rank;
   const float* slot_scale;
-  const void* row_slot;
+  const void* row_slot;  // null: no adapters at all
   void* y;
   int64_t ldx;
   int T, K, N, n_slots, r_pad;
@@ -191,6 +204,7 @@ struct RowsArgs {
   void* tiles;       // [T] runs of sorted rows of one adapter, 16 bytes each
   int* n_tiles;
   float* delta;      // [T][N rounded up to 16] the adapters' part of rows that have one
+  PairMx4 mx4;       // the weight in 4 bits (data null: `w`)
   int* err;          // device status word
 };
 struct RowsTiles {
@@ -227,6 +241,18 @@ struct BankLoad {
 };
 cudaError_t bank_load(const BankLoad& p, int dtype, int num_sms, cudaStream_t st);
 cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
+
+// --------------------------------------------------------------- dropout in front of the adapters
+cudaError_t drop_mask(int dtype, const void* x, int T, int K, const Tables& tb, const DropArgs& d, void* out,
+                      cudaStream_t st);
+// delta[t][k] = m(t, k) sum_j S[t][j] A_i[j][k], S the hi and lo planes of an s_ext (one product, not K halves); bf16 / f16
+cudaError_t drop_expand(int dtype, const void* s_ext, const void* at_pack, int T, int K, const Tables& tb, const DropArgs& d,
+                        float* delta, cudaStream_t st);
+
+// --------------------------------------------------------------- weights in 4 bits
+size_t mx4_bytes(int N, int K);
+cudaError_t mx4_quantize(int dtype, const void* w, int N, int K, int64_t ld, void* out, int num_sms, cudaStream_t st);
+cudaError_t mx4_dequantize(int dtype, const void* in, int N, int K, void* w, int num_sms, cudaStream_t st);
 
 // --------------------------------------------------------------- packing
 cudaError_t pack_adapters(int src_dtype, int dst_dtype, const uint64_t* src_ptrs, const int32_t* ranks,

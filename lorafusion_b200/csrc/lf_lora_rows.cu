@@ -32,6 +32,7 @@
 
 #include "lf_internal.cuh"
 #include "lf_launch.cuh"
+#include "lf_mx4.cuh"
 #include "lf_ptx.cuh"
 
 namespace lf {
@@ -609,9 +610,14 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
 template <>
 __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) { return pack_f16x2(a, b); }
 
+// kMx4: stages that a lane of the decoding warps has loads of in flight.  256 lanes x 17 bytes x 8 are 35 KB an SM, about
+// what HBM's latency asks for.
+constexpr int kMx4Ahead = 8;
+
 // kTN: rows (tokens) of a tile, the N of the MMA.  Warp 0 loads, warp 1 issues the MMAs, eight epilogue warps
-// finish the tile.
-template <typename T, int kTN>
+// finish the tile.  kMx4: the weight is held in 4 bits (lf_mx4.cuh, map_w is not used), and the epilogue warps, idle until
+// the tile is done, decode it into the ring.
+template <typename T, int kTN, bool kMx4>
 __global__ void __maxnreg__(80)
     rows_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                      const __grid_constant__ RowsGemm prm) {
@@ -640,14 +646,14 @@ __global__ void __maxnreg__(80)
 
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], kMx4 ? 1 + kEpiWarps : 1);
       mbar_init(&empty[s], 1);
     }
     mbar_init(&acc_bar, 1);
     mbar_init(&drain_bar, 1);
     abort_flag = 0;
     fence_mbar_init();
-    tma_prefetch_desc(&map_w);
+    if (!kMx4) tma_prefetch_desc(&map_w);
     tma_prefetch_desc(&map_x);
   }
   if (warp == 1) {
@@ -671,9 +677,9 @@ __global__ void __maxnreg__(80)
       if (elect_one()) {
         uint8_t* w = ring + stage * stage_bytes;
         const int n = min(sub, kb1 - kb);
-        mbar_arrive_expect_tx(&full[stage], n * block_bytes);
+        mbar_arrive_expect_tx(&full[stage], n * (kMx4 ? kXBytes : block_bytes));
         for (int i = 0; i < n; ++i, w += block_bytes) {
-          tma_load_2d(w, &map_w, &full[stage], (kb + i) * kBK, n0);
+          if (!kMx4) tma_load_2d(w, &map_w, &full[stage], (kb + i) * kBK, n0);
           tma_load_2d(w + w_bytes, &map_x, &full[stage], (kb + i) * kBK, t0);
         }
       }
@@ -727,9 +733,51 @@ __global__ void __maxnreg__(80)
     }
     __syncwarp();
   } else {
+    const int w = warp - 2, row = (w & 3) * 32 + lane, half = w >> 2;  // kMx4: the codes of this lane in a block
+    const uint8_t* src = nullptr;
+    Mx4Piece ahead[kMx4Ahead];
+    auto fetch = [&](int kb) {
+      const uint8_t* b = src + static_cast<int64_t>(kb) * kMx4Block;
+      return mx4_load(b + half * kMx4HalfBytes + row * 16, b + kMx4Codes + half * kMx4Rows + row);
+    };
+    if constexpr (kMx4) {
+      src = p.mx4.data + static_cast<int64_t>(n0 / kWRows) * p.mx4.col_blocks * kMx4Block;
+#pragma unroll
+      for (int i = 0; i < kMx4Ahead; ++i)
+        if (kb0 + i < kb1) ahead[i] = fetch(kb0 + i);
+    }
     for (int i = tid - 64; i < kTN; i += kEpiWarps * 32)
-      s_on[i] = t0 + i < p.T && row_adapter(p, t0 + i, false) != kNoSlot;
+      s_on[i] = p.row_slot != nullptr && t0 + i < p.T && row_adapter(p, t0 + i, false) != kNoSlot;
     named_barrier(1, kEpiWarps * 32);
+    if constexpr (kMx4) {
+      int stage = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      int kb = kb0, in = 0;  // block, its place in the stage
+      while (ok && kb < kb1) {
+#pragma unroll
+        for (int i = 0; i < kMx4Ahead; ++i) {
+          if (!ok || kb >= kb1) break;
+          if (in == 0) {
+            ok = warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
+            if (!ok) break;
+          }
+          mx4_store<T>(ring + stage * stage_bytes + in * block_bytes + row * 128, row, 4 * half, ahead[i]);
+          if (kb + kMx4Ahead < kb1) ahead[i] = fetch(kb + kMx4Ahead);
+          ++kb;
+          if (++in < sub && kb < kb1) continue;
+          in = 0;
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[stage]);
+          if (++stage == stages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      __syncwarp();
+    }
   }
   const bool ok = warp_wait(&acc_bar, 0, &abort_flag, p.err, kErrTimeoutAcc);
   tc_fence_after();
@@ -1501,14 +1549,15 @@ cudaError_t allow_smem(const void* kernel, int bytes) {
 constexpr int ring_bytes(int tn) { return tn > 256 ? 0 : 160 * 1024; }
 static_assert(ring_bytes(256) >= 256 * 512, "the sums fit the ring");
 
-template <typename T, int kTN>
+template <typename T, int kTN, bool kMx4>
 cudaError_t launch_gemm(const RowsGemm& g, const CUtensorMap& w, const CUtensorMap& x, cudaStream_t st) {
-  auto* k = rows_gemm_kernel<T, kTN>;
+  auto* k = rows_gemm_kernel<T, kTN, kMx4>;
   cudaError_t e = allow_smem(reinterpret_cast<const void*>(k), ring_bytes(kTN) + 1024);
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>((g.a.N + kWRows - 1) / kWRows * g.ksplit),
                   static_cast<unsigned>((g.a.T + kTN - 1) / kTN));
-  return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), ring_bytes(kTN) + 1024, st, true, w, x, g);
+  return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), ring_bytes(kTN) + 1024, st,
+                        g.a.row_slot != nullptr, w, x, g);  // early beside the adapters' part only, which came after x
 }
 
 // The adapters' part of up to 256 rows: one CTA an SM, beside the GEMM's; few rows are cut over a larger cluster.
@@ -1579,10 +1628,10 @@ cudaError_t adapters_part(const RowsArgs& a, int dtype, const ManyMaps* m, int n
   return m ? many_part<T>(a, dtype, *m, num_sms, st) : lora_part<T>(a, num_sms, st);
 }
 
-template <typename T>
+template <typename T, bool kMx4>
 cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const ManyMaps* m, int tn,
                     int ksplit, int num_sms, cudaStream_t st) {
-  const cudaError_t e = adapters_part<T>(a, dtype, m, num_sms, st);
+  const cudaError_t e = a.row_slot ? adapters_part<T>(a, dtype, m, num_sms, st) : cudaSuccess;
   if (e != cudaSuccess) return e;
   RowsGemm g{};
   g.a = a;
@@ -1591,11 +1640,11 @@ cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CU
   const int room = ring_bytes(tn), block = (kWRows + tn) * kBK * 2;
   g.sub = room / (2 * block) >= 3 ? 2 : 1;
   g.stages = room / (g.sub * block);
-  if (tn == 16) return launch_gemm<T, 16>(g, w, x, st);
-  if (tn == 32) return launch_gemm<T, 32>(g, w, x, st);
-  if (tn == 64) return launch_gemm<T, 64>(g, w, x, st);
-  if (tn == 128) return launch_gemm<T, 128>(g, w, x, st);
-  return launch_gemm<T, 256>(g, w, x, st);
+  if (tn == 16) return launch_gemm<T, 16, kMx4>(g, w, x, st);
+  if (tn == 32) return launch_gemm<T, 32, kMx4>(g, w, x, st);
+  if (tn == 64) return launch_gemm<T, 64, kMx4>(g, w, x, st);
+  if (tn == 128) return launch_gemm<T, 128, kMx4>(g, w, x, st);
+  return launch_gemm<T, 256, kMx4>(g, w, x, st);
 }
 
 template <typename T>
@@ -1624,8 +1673,11 @@ RowsTiles rows_tiles(int T, int K, int N, int num_sms) {
 
 cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CUtensorMap& x, const RowsTiles& t,
                             const ManyMaps* m, int num_sms, cudaStream_t st) {
-  return dtype == LF_BF16 ? rows_tc<__nv_bfloat16>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st)
-                          : rows_tc<__half>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st);
+  if (a.mx4.data)
+    return dtype == LF_BF16 ? rows_tc<__nv_bfloat16, true>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st)
+                            : rows_tc<__half, true>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st);
+  return dtype == LF_BF16 ? rows_tc<__nv_bfloat16, false>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st)
+                          : rows_tc<__half, false>(a, dtype, w, x, m, t.rows, t.ksplit, num_sms, st);
 }
 
 cudaError_t rows_lora_part(const RowsArgs& a, int dtype, const ManyMaps* m, int num_sms, cudaStream_t st) {

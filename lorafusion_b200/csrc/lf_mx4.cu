@@ -1,0 +1,162 @@
+// A weight to microscaled 4-bit floating point and back (formats and layout: lf_mx4.cuh).
+//
+// Both are one pass: 2 bytes an element on the one side, 17/32 on the other.  Four lanes share a block of 32 along K, a
+// warp takes 8 rows of 128 columns: 16-byte accesses on the dense side in runs of 64 bytes, runs of 128 bytes
+// on the packed side, four loads of a lane in flight.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "lf_internal.cuh"
+#include "lf_mx4.cuh"
+
+namespace lf {
+namespace {
+
+constexpr int kThreads = 256;
+
+template <typename T>
+__device__ __forceinline__ float to_f(uint32_t bits);
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(uint32_t bits) { return __uint_as_float(bits << 16); }
+template <>
+__device__ __forceinline__ float to_f<__half>(uint32_t bits) {
+  return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
+}
+
+// Eight 16-bit elements k .. k + 7 of row n, zeros past the matrix.
+__device__ __forceinline__ uint4 load8(const uint16_t* w, int n, int k, int N, int K, int64_t ld, bool vec) {
+  uint4 v = make_uint4(0, 0, 0, 0);
+  if (n >= N || k >= K) return v;
+  const uint16_t* p = w + n * ld + k;
+  if (vec) return *reinterpret_cast<const uint4*>(p);  // K and the row pitch are multiples of 8
+  uint32_t e[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) e[i] = k + i < K ? p[i] : 0u;
+  v.x = e[0] | e[1] << 16, v.y = e[2] | e[3] << 16, v.z = e[4] | e[5] << 16, v.w = e[6] | e[7] << 16;
+  return v;
+}
+
+// Two codes, the nearest of a and b with ties to the even code and 6 for what is larger, in one byte.
+__device__ __forceinline__ uint32_t encode2(float low, float high) {
+  uint32_t r;
+  asm("{\n\t.reg .b8 c;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\t"
+      "cvt.u32.u8 %0, c;\n\t}"
+      : "=r"(r)
+      : "f"(low), "f"(high));
+  return r;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const uint16_t* __restrict__ w, int N, int K, int64_t ld,
+                                                                int vec, int64_t units, uint8_t* __restrict__ out) {
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const int spans = mx4_col_blocks(K) / 2;
+  for (int64_t u = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5; u < units;
+       u += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+    // a unit: 8 rows of one span of 128 columns; units of a span's 128 rows follow one another
+    const int64_t at = u >> 4;
+    const int span = static_cast<int>(at % spans), tile = static_cast<int>(at / spans);
+    const int r = static_cast<int>(u & 15) * 8 + (lane >> 2), n = tile * kMx4Rows + r;
+    uint4 v[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) v[c] = load8(w, n, span * 128 + c * 32 + j * 8, N, K, ld, vec != 0);
+    uint8_t* blocks = out + (static_cast<int64_t>(tile) * spans + span) * (2 * kMx4Block);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint32_t word[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[2 * i] = to_f<T>(word[i] & 0xffffu), f[2 * i + 1] = to_f<T>(word[i] >> 16);
+      uint32_t top = 0;  // magnitudes compare as whole numbers; infinities and NaN are the largest
+#pragma unroll
+      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const uint32_t e = top >> 23;  // floor(log2) + 127; 0 of a zero and of float32's subnormals (bf16 has them)
+      const bool bad = e == 255u;
+      const uint32_t s = bad ? 255u : e < 2u ? 0u : e - 2u;  // E = floor(log2) - 2, at least -127
+      const float up = __uint_as_float((254u - (bad ? 127u : s)) << 23);  // 2^-E
+      uint32_t code = 0;
+      if (!bad) {
+        // element 2p at nibble p, element 2p + 1 at nibble p + 4
+        code = encode2(f[0] * up, f[2] * up) | encode2(f[4] * up, f[6] * up) << 8 | encode2(f[1] * up, f[3] * up) << 16 |
+               encode2(f[5] * up, f[7] * up) << 24;
+      }
+      uint8_t* b = blocks + (c >> 1) * kMx4Block;
+      *reinterpret_cast<uint32_t*>(b + (c & 1) * kMx4HalfBytes + r * 16 + j * 4) = code;
+      if (j == 0) b[kMx4Codes + (c & 1) * kMx4Rows + r] = static_cast<uint8_t>(s);
+    }
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(const uint8_t* __restrict__ in, int N, int K, int vec,
+                                                                  int64_t units, uint16_t* __restrict__ w) {
+  const int lane = threadIdx.x & 31, j = lane & 3;
+  const int spans = mx4_col_blocks(K) / 2;
+  for (int64_t u = (static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x) >> 5; u < units;
+       u += static_cast<int64_t>(gridDim.x) * (kThreads / 32)) {
+    const int64_t at = u >> 4;
+    const int span = static_cast<int>(at % spans), tile = static_cast<int>(at / spans);
+    const int r = static_cast<int>(u & 15) * 8 + (lane >> 2), n = tile * kMx4Rows + r;
+    const uint8_t* blocks = in + (static_cast<int64_t>(tile) * spans + span) * (2 * kMx4Block);
+    uint32_t code[4], scale[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint8_t* b = blocks + (c >> 1) * kMx4Block;
+      code[c] = *reinterpret_cast<const uint32_t*>(b + (c & 1) * kMx4HalfBytes + r * 16 + j * 4);
+      scale[c] = b[kMx4Codes + (c & 1) * kMx4Rows + r];
+    }
+    if (n >= N) continue;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int k = span * 128 + c * 32 + j * 8;
+      if (k >= K) continue;
+      const uint4 v = Mx4<T>::decode(code[c], Mx4<T>::scale(scale[c]));
+      uint16_t* p = w + static_cast<int64_t>(n) * K + k;
+      if (vec) {
+        *reinterpret_cast<uint4*>(p) = v;
+        continue;
+      }
+      const uint32_t word[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < K) p[i] = static_cast<uint16_t>(i & 1 ? word[i >> 1] >> 16 : word[i >> 1] & 0xffffu);
+    }
+  }
+}
+
+int64_t units_of(int N, int K) { return static_cast<int64_t>(mx4_row_tiles(N)) * (mx4_col_blocks(K) / 2) * 16; }
+unsigned blocks_of(int64_t units, int num_sms) {
+  const int64_t b = (units + kThreads / 32 - 1) / (kThreads / 32);
+  return static_cast<unsigned>(b < 8 * num_sms ? b : 8 * num_sms);
+}
+
+}  // namespace
+
+size_t mx4_bytes(int N, int K) {
+  return static_cast<size_t>(mx4_row_tiles(N)) * static_cast<size_t>(mx4_col_blocks(K)) * kMx4Block;
+}
+
+cudaError_t mx4_quantize(int dtype, const void* w, int N, int K, int64_t ld, void* out, int num_sms, cudaStream_t st) {
+  const int64_t units = units_of(N, K);
+  if (units == 0) return cudaSuccess;
+  const int vec = K % 8 == 0 && ld % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+  auto* k = dtype == LF_BF16 ? mx4_quantize_kernel<__nv_bfloat16> : mx4_quantize_kernel<__half>;
+  k<<<blocks_of(units, num_sms), kThreads, 0, st>>>(static_cast<const uint16_t*>(w), N, K, ld, vec, units,
+                                                    static_cast<uint8_t*>(out));
+  return cudaGetLastError();
+}
+
+cudaError_t mx4_dequantize(int dtype, const void* in, int N, int K, void* w, int num_sms, cudaStream_t st) {
+  const int64_t units = units_of(N, K);
+  if (units == 0) return cudaSuccess;
+  const int vec = K % 8 == 0 && reinterpret_cast<uintptr_t>(w) % 16 == 0;
+  auto* k = dtype == LF_BF16 ? mx4_dequantize_kernel<__nv_bfloat16> : mx4_dequantize_kernel<__half>;
+  k<<<blocks_of(units, num_sms), kThreads, 0, st>>>(static_cast<const uint8_t*>(in), N, K, vec, units,
+                                                    static_cast<uint16_t*>(w));
+  return cudaGetLastError();
+}
+
+}  // namespace lf

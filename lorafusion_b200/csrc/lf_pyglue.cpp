@@ -47,10 +47,11 @@ void bump(const at::Tensor& t) {
 }
 
 // rows_forward(x, weight, bank_a, bank_b, ranks, scales, row_slot, out or None, the bank's padded rank, its output
-// features): the call of fused_lora_forward_rows on operands that need no copy.  None otherwise.
+// features, 1 if the weight is the data of one in 4 bits (its shape and dtype were checked)): the call of
+// fused_lora_forward_rows on operands that need no copy.  None otherwise.
 PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  if (n != 10) {
-    PyErr_SetString(PyExc_TypeError, "rows_forward takes 10 arguments");
+  if (n != 11) {
+    PyErr_SetString(PyExc_TypeError, "rows_forward takes 11 arguments");
     return nullptr;
   }
   const at::Tensor* t[7];
@@ -58,16 +59,19 @@ PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!(t[i] = cuda_tensor(a[i]))) Py_RETURN_NONE;
   const at::Tensor &x = *t[0], &w = *t[1], &ba = *t[2], &bb = *t[3], &ranks = *t[4], &scales = *t[5], &slot = *t[6];
   const long r_pad = PyLong_AsLong(a[8]), features = PyLong_AsLong(a[9]);
+  const bool mx4 = PyLong_AsLong(a[10]) == 1;
   if (PyErr_Occurred()) return nullptr;
   const int code = dtype_code(x.scalar_type());
-  if (code < 0 || x.dim() != 2 || w.dim() != 2 || slot.dim() != 1) Py_RETURN_NONE;
-  const int64_t T = x.size(0), K = x.size(1), N = w.size(0);
+  if (code < 0 || x.dim() != 2 || w.dim() != (mx4 ? 1 : 2) || slot.dim() != 1) Py_RETURN_NONE;
+  const int64_t T = x.size(0), K = x.size(1), N = mx4 ? features : w.size(0);
   const auto dev = x.device();
   for (int i = 1; i < 7; ++i)
     if (t[i]->device() != dev) Py_RETURN_NONE;
   const bool wide = slot.scalar_type() == at::kLong;
-  if (w.scalar_type() != x.scalar_type() || ba.scalar_type() != x.scalar_type() || w.size(1) != K ||
-      N != features ||
+  if (mx4 ? w.scalar_type() != at::kByte || code == LF_F32
+          : w.scalar_type() != x.scalar_type() || w.size(1) != K || N != features)
+    Py_RETURN_NONE;
+  if (ba.scalar_type() != x.scalar_type() ||
       slot.size(0) != T || (!wide && slot.scalar_type() != at::kInt) || !slot.is_contiguous() || !w.is_contiguous() ||
       ba.size(2) != K || T == 0 || T > INT32_MAX || K > INT32_MAX || N > INT32_MAX)
     Py_RETURN_NONE;
@@ -97,6 +101,7 @@ PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
   p.n_slots = static_cast<int32_t>(ba.size(0));
   p.r_pad = static_cast<int32_t>(r_pad);
   p.row_slot_bytes = wide ? 8 : 4;
+  p.weight_format = mx4 ? LF_WEIGHT_MX4 : LF_WEIGHT_DENSE;
   p.ldx = ldx;
   p.x_dev = xp;
   p.w_dev = wp;
@@ -114,6 +119,44 @@ PyObject* rows_forward(PyObject*, PyObject* const* a, Py_ssize_t n) {
     bump(y);
     return Py_NewRef(a[7]);
   }
+  return THPVariable_Wrap(std::move(y));
+}
+
+// mx4_linear(x, data, out_features, in_features, dtype code, transpose): x V^T, or x V with transpose, on operands that
+// need no copy; V the values of the weight in 4 bits whose data and shape these are.  None otherwise.
+PyObject* mx4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 6) {
+    PyErr_SetString(PyExc_TypeError, "mx4_linear takes 6 arguments");
+    return nullptr;
+  }
+  const at::Tensor *xt = cuda_tensor(a[0]), *wt = cuda_tensor(a[1]);
+  if (!xt || !wt) Py_RETURN_NONE;
+  const at::Tensor &x = *xt, &w = *wt;
+  lf_mx4_problem p{};
+  p.N = static_cast<int32_t>(PyLong_AsLong(a[2]));
+  p.K = static_cast<int32_t>(PyLong_AsLong(a[3]));
+  p.dtype = static_cast<int32_t>(PyLong_AsLong(a[4]));
+  p.transpose = static_cast<int32_t>(PyLong_AsLong(a[5]));
+  if (PyErr_Occurred()) return nullptr;
+  const int64_t in = p.transpose ? p.N : p.K, out = p.transpose ? p.K : p.N;
+  if (dtype_code(x.scalar_type()) != p.dtype || x.dim() != 2 || x.size(1) != in || x.device() != w.device() ||
+      x.size(0) == 0 || x.size(0) > INT32_MAX || p.K % 8 || p.N % 8)
+    Py_RETURN_NONE;
+  const int64_t ld = x.is_contiguous() ? in : x.stride(0);
+  if (!x.is_contiguous() && (x.stride(1) != 1 || ld < in)) Py_RETURN_NONE;
+  if (ld % 8 || !aligned16(x.const_data_ptr())) Py_RETURN_NONE;
+  p.T = static_cast<int32_t>(x.size(0));
+  p.ld = ld;
+  p.in_dev = x.const_data_ptr();
+  p.mx4_dev = w.const_data_ptr();
+  const auto dev = x.device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  at::Tensor y = at::detail::empty_cuda({x.size(0), out}, x.scalar_type(), dev, std::nullopt);
+  const int64_t bytes = static_cast<int64_t>(lf_mx4_linear_workspace_bytes(p.K, p.N));
+  at::Tensor ws = at::detail::empty_cuda({bytes}, at::kByte, dev, std::nullopt);
+  const int rc = lf_mx4_linear(&p, y.data_ptr(), ws.data_ptr(), static_cast<size_t>(bytes),
+                               c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (rc != LF_OK) return fail(rc, "lf_mx4_linear");
   return THPVariable_Wrap(std::move(y));
 }
 
@@ -391,6 +434,7 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 
 PyMethodDef methods[] = {
     {"rows_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<rows_forward>)), METH_FASTCALL, nullptr},
+    {"mx4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_linear>)), METH_FASTCALL, nullptr},
     {"bank_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<bank_load>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},
     {"gather_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<gather_step>)), METH_FASTCALL, nullptr},

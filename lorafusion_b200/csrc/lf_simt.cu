@@ -7,6 +7,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "lf_drop.cuh"
 #include "lf_internal.cuh"
 
 namespace lf {
@@ -83,7 +84,7 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(const T* __restrict__ P,
                                                         const T* __restrict__ Q, int64_t qsn, int64_t qsk, int Trows,
                                                         int Nout, int Kred, const double* __restrict__ s_ext,
                                                         const T* __restrict__ lpk, Tables tb, T* __restrict__ out,
-                                                        int64_t ldo) {
+                                                        int64_t ldo, DropArgs drop) {
   __shared__ float ps[SG_BK][SG_BM + 4];
   __shared__ float qs[SG_BK][SG_BN + 4];
   const int m0 = blockIdx.y * SG_BM, n0 = blockIdx.x * SG_BN;
@@ -143,6 +144,11 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(const T* __restrict__ P,
         for (int j = 0; j < 4; ++j) {
           const int gn = n0 + tc * 4 + j;
           if (gn >= Nout) continue;
+          if (drop.threshold != nullptr) {
+            const uint4 r = philox(static_cast<uint32_t>(gn >> 3), static_cast<uint32_t>(gr), drop.offset, drop.seed);
+            const uint32_t w = (gn & 4) ? ((gn & 2) ? r.w : r.z) : ((gn & 2) ? r.y : r.x);
+            if (((gn & 1) ? w >> 16 : w & 0xffffu) < drop.threshold[tb.st_slot(st)]) continue;
+          }
           double d = 0.0;
           for (int q = 0; q < r_pad; ++q)
             d = fma(srow[q], static_cast<double>(to_f(lb[static_cast<int64_t>(gn) * r_pad + q])), d);
@@ -240,22 +246,22 @@ cudaError_t simt_shrink(int dtype, const void* P, int64_t ldp, int Kred, const v
 
 cudaError_t simt_gemm(int dtype, const void* P, int64_t ldp, const void* Q, int64_t qsn, int64_t qsk, int T, int Nout,
                       int Kred, const double* s_ext, const void* lpk, const Tables& tb, void* out, int64_t ldo,
-                      cudaStream_t st) {
+                      const DropArgs& drop, cudaStream_t st) {
   if (T == 0 || Nout == 0) return cudaSuccess;
   dim3 grid((Nout + SG_BN - 1) / SG_BN, (T + SG_BM - 1) / SG_BM);
   switch (dtype) {
     case LF_F32:
       simt_gemm_kernel<float><<<grid, 256, 0, st>>>((const float*)P, ldp, (const float*)Q, qsn, qsk, T, Nout, Kred,
-                                                    s_ext, (const float*)lpk, tb, (float*)out, ldo);
+                                                    s_ext, (const float*)lpk, tb, (float*)out, ldo, drop);
       break;
     case LF_BF16:
       simt_gemm_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(
           (const __nv_bfloat16*)P, ldp, (const __nv_bfloat16*)Q, qsn, qsk, T, Nout, Kred, s_ext,
-          (const __nv_bfloat16*)lpk, tb, (__nv_bfloat16*)out, ldo);
+          (const __nv_bfloat16*)lpk, tb, (__nv_bfloat16*)out, ldo, drop);
       break;
     default:
       simt_gemm_kernel<__half><<<grid, 256, 0, st>>>((const __half*)P, ldp, (const __half*)Q, qsn, qsk, T, Nout, Kred,
-                                                     s_ext, (const __half*)lpk, tb, (__half*)out, ldo);
+                                                     s_ext, (const __half*)lpk, tb, (__half*)out, ldo, drop);
       break;
   }
   return cudaGetLastError();

@@ -19,6 +19,7 @@
 
 #include "lf_internal.cuh"
 #include "lf_launch.cuh"
+#include "lf_mx4.cuh"
 #include "lf_ptx.cuh"
 
 namespace lf {
@@ -426,6 +427,7 @@ struct PairParams {
   int job2, Kred2;
   void* s_ext2;
   PairDelta delta;  // kDelta kernels
+  PairMx4 mx4;      // kMx4 kernels
   Tables tb;
 };
 
@@ -659,7 +661,7 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
       }
     }
     __syncwarp();
-  } else {
+  } else if (warp < kThreads / 32) {  // the decoding warps of a kMx4 kernel have no part in it
     const int q = warp & 3;
     const int row = q * 32 + lane;
     OutT* s_ext = reinterpret_cast<OutT*>(prm.s_ext);
@@ -751,9 +753,100 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
   if (kPrologue) __syncthreads();
 }
 
+// The decoding warps of a kMx4 pair: Q is held in 4 bits (lf_mx4.cuh), and its 128 x 64 tile of every stage is written by
+// these eight warps instead of a copy, the 16-bit values in the layout the copy would have left: row r of 64 columns of K
+// for x V^T, for g V (kQMN) two panels of 64 columns by 64 rows.  A lane has 32 codes of a stage: it loads them
+// kMx4Ahead stages ahead (a stage takes about 0.3 us, HBM two to three times that), waits for the
+// stage to be free, stores the values and reports to the even CTA's `full` barrier, whose phase also counts the P
+// tiles' bytes.  LoRA stages are filled by copies alone; the warps report them unseen.
+constexpr int kMx4Warps = 8;
+constexpr int kMx4Threads = kThreads + 32 * kMx4Warps;
+constexpr int kMx4Ahead = 4;
+
+template <bool kQMN, typename OutT>
+__device__ __forceinline__ void pair_decode_role(const PairParams& prm, const PairSched& sched, int pair, int n_pairs,
+                                                 int n_units, int nkb, int crank, uint8_t* sB, uint32_t full_lead,
+                                                 uint64_t* empty, volatile int* abort_flag) {
+  const int w = (threadIdx.x >> 5) - kThreads / 32, lane = threadIdx.x & 31;
+  const Tables& tb = prm.tb;
+  const int half = w >> 2;                                          // which 32 columns of a block
+  const int row = kQMN ? (w & 1) * 32 + lane : (w & 3) * 32 + lane;  // of the stage's tile
+  const int panel = (w >> 1) & 1;                                   // kQMN: which 64 of the 128 columns
+  uint8_t* dst = sB + (kQMN ? panel * 8192 : 0) + row * 128;
+  auto fetch = [&](int n, int kb) {  // tiles past the weight's last one repeat it: their columns are not stored
+    int64_t block;
+    int r = row;
+    if (kQMN) {
+      block = static_cast<int64_t>(kb >> 1) * prm.mx4.col_blocks + min(2 * (2 * n + crank) + panel, prm.mx4.col_blocks - 1);
+      r += (kb & 1) * 64;
+    } else {
+      block = static_cast<int64_t>(min(2 * n + crank, prm.mx4.row_tiles - 1)) * prm.mx4.col_blocks + kb;
+    }
+    const uint8_t* b = prm.mx4.data + block * kMx4Block;
+    return mx4_load(b + half * kMx4HalfBytes + r * 16, b + kMx4Codes + half * kMx4Rows + r);
+  };
+  // the next piece to load: unit fk, k-block fkb
+  int fk = 0, fkb = 0, fkb1 = 0, fn = 0;
+  auto open = [&]() {
+    if (fk >= n_units) return;
+    const PairUnit un = pair_unit(prm, sched, pair, n_pairs, fk, nkb);
+    fkb = un.kb0, fkb1 = un.kb1, fn = un.n;
+  };
+  Mx4Piece ring[kMx4Ahead];
+  auto refill = [&](Mx4Piece& p) {
+    if (fk >= n_units) return;
+    p = fetch(fn, fkb);
+    if (++fkb == fkb1) {
+      ++fk;
+      open();
+    }
+  };
+  open();
+#pragma unroll
+  for (int i = 0; i < kMx4Ahead; ++i) refill(ring[i]);
+  int k = 0, stage = 0;
+  uint32_t phase = 0;
+  PairUnit un = n_units > 0 ? pair_unit(prm, sched, pair, n_pairs, 0, nkb) : PairUnit{};
+  int kb = un.kb0;
+  bool ok = true;
+  auto report = [&]() {
+    __syncwarp();
+    if (lane == 0) mbar_arrive_cluster(full_lead + static_cast<uint32_t>(stage * 8));
+    if (++stage == kPairStages) {
+      stage = 0;
+      phase ^= 1;
+    }
+  };
+  while (ok && k < n_units) {
+#pragma unroll
+    for (int i = 0; i < kMx4Ahead; ++i) {
+      if (!ok || k >= n_units) break;
+      ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
+      if (!ok) break;
+      mx4_store<OutT>(dst + stage * kPairBBytes, row, 4 * half, ring[i]);
+      fence_proxy_async_smem();
+      report();
+      refill(ring[i]);
+      if (++kb < un.kb1) continue;
+      int n_lora = 0;
+      if (prm.lora && un.last)
+        n_lora = (tb.pair_lora(un.mp + 1) - tb.pair_lora(un.mp)) * prm.s_planes;
+      for (int j = 0; ok && j < n_lora; j += prm.lora_per_stage) {
+        ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
+        if (ok) report();
+      }
+      if (++k < n_units) {
+        un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
+        kb = un.kb0;
+      }
+    }
+  }
+}
+
 // kDelta: a float32 matrix is added to the product (prm.delta).
-template <bool kQMN, typename OutT, bool kDelta>
-__global__ void __launch_bounds__(kThreads, 1)
+// kMx4: Q is held in 4 bits (prm.mx4) and decoded on the way into shared memory; map_q is not used.
+template <bool kQMN, typename OutT, bool kDelta, bool kMx4>
+__global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
     tc_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_l,
                         const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_a,
@@ -801,7 +894,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], kMx4 ? 1 + 2 * kMx4Warps : 1);
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -813,7 +906,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     *abort_flag = 0;
     fence_mbar_init();
     tma_prefetch_desc(&map_p);
-    tma_prefetch_desc(&map_q);
+    if (!kMx4) tma_prefetch_desc(&map_q);
     tma_prefetch_desc(&map_o);
     if (prm.lora) {
       tma_prefetch_desc(&map_s);
@@ -840,7 +933,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int stage = 0;
     uint32_t phase = 0, issued_mask = 0, last_parity = 0;
     bool ok = true;
-    const uint32_t main_bytes = 2u * (kPairABytes + kPairBBytes);
+    const uint32_t main_bytes = 2u * (kPairABytes + (kMx4 ? 0 : kPairBBytes));
     const uint32_t lora_bytes = static_cast<uint32_t>(2 * 2 * kBM * prm.r_pad * 2);
     const int lora_item_bytes = kBM * prm.r_pad * 2;  // one operand of one item, this CTA
     const int32_t* st_of = tb.base + (crank ? tb.off_pl_b : tb.off_pl_a);
@@ -882,7 +975,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (crank == 0) mbar_arrive_expect_tx(&full[stage], main_bytes);
           const uint32_t fb = full_lead + static_cast<uint32_t>(stage * 8);
           tma_load_2d_pair(sA + stage * kPairABytes, &map_p, fb, kb * kBK, mtile * kBM);
-          if (kQMN) {
+          if (kMx4) {
+            // decoded there by this CTA's warps
+          } else if (kQMN) {
             tma_load_2d_pair(sB + stage * kPairBBytes, &map_q, fb, n * 256 + static_cast<int>(crank) * 128, kb * kBK);
             tma_load_2d_pair(sB + stage * kPairBBytes + 64 * kBK * 2, &map_q, fb,
                              n * 256 + static_cast<int>(crank) * 128 + 64, kb * kBK);
@@ -1038,6 +1133,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
+  } else if (kMx4 && warp >= kThreads / 32) {
+    pair_decode_role<kQMN, OutT>(prm, sched, pair, n_pairs, n_units, nkb, static_cast<int>(crank), sB, full_lead, empty,
+                                 abort_flag);
   } else {
     const int q = warp & 3;
     int it = 0;
@@ -1156,7 +1254,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (row0 >= prm.T || col0 >= prm.Nout) continue;
         if constexpr (kDelta) {
           const int row = row0 + lane;
-          if (row < prm.T && prm.delta.eff[row] != 0xffffffffu) {
+          if (row < prm.T && (prm.delta.eff == nullptr || prm.delta.eff[row] != 0xffffffffu)) {
             const float4* d = reinterpret_cast<const float4*>(prm.delta.delta + row * prm.delta.ld + col0);
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
@@ -2195,8 +2293,9 @@ int pair_spare_pairs(int T, int Nout, int num_sms, int n_units) {
 
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
-                         const PairShrink* shrink, const PairTail* tail, const PairDelta* delta) {
+                         const PairShrink* shrink, const PairTail* tail, const PairDelta* delta, const PairMx4* mx4) {
   PairParams p{};
+  if (mx4 != nullptr) p.mx4 = *mx4;
   p.out = out;
   p.ldo = ldo;
   p.T = T;
@@ -2275,7 +2374,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (gemm_pairs + p.n_shrink_pairs));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(mx4 != nullptr ? kMx4Threads : kThreads);
   cfg.dynamicSmemBytes = kPairSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -2290,37 +2389,36 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cfg.attrs = attr;
   cfg.numAttrs = p.n_shrink_pairs > 0 || p.shrink_prologue || p.tail_parts > 1 ? 2 : 1;
   cudaError_t e;
-#define LF_LAUNCH_PAIR(QMN, OT, DELTA)                                                          \
-  e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA>, kPairSmem);                              \
-  if (e != cudaSuccess) return e;                                                               \
-  e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT, DELTA>, maps.p, maps.q, maps.s, maps.l, maps.o, *a_map, *p2_map, \
-                         *a2_map, p);
+#define LF_LAUNCH_PAIR(QMN, OT, DELTA, MX4)                                                                         \
+  {                                                                                                                  \
+    e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, kPairSmem);                                            \
+    if (e != cudaSuccess) return e;                                                                                  \
+    e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, maps.p, maps.q, maps.s, maps.l, maps.o,   \
+                           *a_map, *p2_map, *a2_map, p);                                                             \
+  }
+#define LF_LAUNCH_PAIR_TYPES(DELTA, MX4)                            \
+  {                                                                 \
+    if (dtype == LF_BF16) {                                         \
+      if (q_mn_major) LF_LAUNCH_PAIR(true, __nv_bfloat16, DELTA, MX4) \
+      else LF_LAUNCH_PAIR(false, __nv_bfloat16, DELTA, MX4)         \
+    } else {                                                        \
+      if (q_mn_major) LF_LAUNCH_PAIR(true, __half, DELTA, MX4)      \
+      else LF_LAUNCH_PAIR(false, __half, DELTA, MX4)                \
+    }                                                               \
+  }
   if (delta != nullptr) {
-    if (q_mn_major || shrink != nullptr || tail != nullptr) return cudaErrorInvalidValue;
+    if (shrink != nullptr || tail != nullptr) return cudaErrorInvalidValue;
     p.delta = *delta;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
-    if (dtype == LF_BF16) {
-      LF_LAUNCH_PAIR(false, __nv_bfloat16, true)
-    } else {
-      LF_LAUNCH_PAIR(false, __half, true)
-    }
+    if (mx4 != nullptr) LF_LAUNCH_PAIR_TYPES(true, true)
+    else LF_LAUNCH_PAIR_TYPES(true, false)
     return e;
   }
-  if (dtype == LF_BF16) {
-    if (q_mn_major) {
-      LF_LAUNCH_PAIR(true, __nv_bfloat16, false)
-    } else {
-      LF_LAUNCH_PAIR(false, __nv_bfloat16, false)
-    }
-  } else {
-    if (q_mn_major) {
-      LF_LAUNCH_PAIR(true, __half, false)
-    } else {
-      LF_LAUNCH_PAIR(false, __half, false)
-    }
-  }
+  if (mx4 != nullptr) LF_LAUNCH_PAIR_TYPES(false, true)
+  else LF_LAUNCH_PAIR_TYPES(false, false)
+#undef LF_LAUNCH_PAIR_TYPES
 #undef LF_LAUNCH_PAIR
   if (e != cudaSuccess) return e;
   return cudaGetLastError();
@@ -2423,8 +2521,7 @@ cudaError_t tc_gram(int dtype, const GramJobDesc* jobs, int n_jobs, const Tables
     const int64_t share = (steps + 8 * grid - 1) / (8 * grid);
     p.cap = static_cast<int>(share < 2 ? 2 : share);
     p.partial = static_cast<float*>(scratch);
-    p.counters = reinterpret_cast<uint64_t*>(static_cast<char*>(scratch) +
-                                             static_cast<size_t>(kGramMaxPartials) * 128 * tb.r_pad * 4);
+    p.counters = reinterpret_cast<uint64_t*>(static_cast<char*>(scratch) + gram_counters_offset(tb.r_pad));
     p.gen32 = static_cast<uint32_t>(gen);
   }
   const CUtensorMap& d1 = jobs[n_jobs - 1].d_map;

@@ -16,6 +16,7 @@ import torch
 
 from lorafusion_b200 import _native as nat
 from lorafusion_b200 import b200_ops
+from lorafusion_b200.quant import MX4Weight
 
 __all__ = ["AdapterBank", "fused_lora_forward_rows"]
 
@@ -96,12 +97,13 @@ class AdapterBank:
         self.ranks[slot] = 0
 
 
-def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: AdapterBank, row_slot: torch.Tensor,
-                            out: torch.Tensor | None = None) -> torch.Tensor:
+def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor | MX4Weight, bank: AdapterBank,
+                            row_slot: torch.Tensor, out: torch.Tensor | None = None) -> torch.Tensor:
     """``y[t] = x[t] W^T + s_i (x[t] A_i^T) B_i^T`` with ``i = row_slot[t]``, a slot of ``bank``.
 
     ``x [T, in_features]`` (rows may be strided), ``base_weight [out_features, in_features]`` and the
-    bank share one dtype (float32, bfloat16, float16) and device.  ``row_slot [T]`` is an int32 or int64
+    bank share one dtype (float32, bfloat16, float16) and device.  ``base_weight`` may be a ``quant.MX4Weight``
+    (bfloat16, float16), whose values W then are.  ``row_slot [T]`` is an int32 or int64
     tensor on that device, in any order; a negative entry means no adapter, and so does an
     empty slot.  An entry at or above ``bank.n_slots`` also gets the shared projection alone and is
     reported by ``_native.device_error()`` (``ERR_ROW_SLOT``): the slots are never read on the host.  Until the call
@@ -119,9 +121,13 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     problems whose in_features or out_features is not a multiple of 8, or whose buffers are not 16-byte
     aligned, run on CUDA cores with a ``CudaCorePathWarning``.
     """
-    y = nat.glue().rows_forward(
-        x, base_weight, bank.lora_a, bank.lora_b, bank.ranks, bank.scales, row_slot, out, bank.r_pad,
-        bank.out_features) if bank is not None else None
+    mx4 = isinstance(base_weight, MX4Weight)
+    y = None
+    if bank is not None and not (mx4 and (base_weight.dtype is not x.dtype or base_weight.shape != (
+            bank.out_features, bank.in_features))):
+        y = nat.glue().rows_forward(
+            x, base_weight.data if mx4 else base_weight, bank.lora_a, bank.lora_b, bank.ranks, bank.scales, row_slot,
+            out, bank.r_pad, bank.out_features, int(mx4))
     if y is not None:
         b200_ops._last_launches = _launches(x.shape[0], bank.r_pad, x.dtype is not torch.float32)
         return y
@@ -148,7 +154,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
         raise ValueError(f"row_slot must be int32 or int64, got {slot_dtype}")
     if base_weight.device != device or bank.device != device or row_slot.device != device:
         raise ValueError(f"base_weight, the bank and row_slot must live on {device}")
-    if not base_weight.is_contiguous():
+    if not mx4 and not base_weight.is_contiguous():
         raise ValueError("base_weight must be contiguous")
     if not row_slot.is_contiguous():
         row_slot = row_slot.contiguous()
@@ -166,8 +172,11 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
     b200_ops._last_launches = 0
     if T == 0:
         return out
+    if mx4 and (K % 8 or N % 8 or out.data_ptr() % 16):  # CUDA cores: from a dense copy, made within the call
+        base_weight, mx4 = base_weight.dequantize(), False
+    weight = base_weight.data if mx4 else base_weight
     p = nat.RowsProblem(_DTYPE_CODE[dtype], T, K, N, bank.n_slots, bank.r_pad, 4 if slot_dtype is torch.int32 else 8,
-                        0, ldx, x.data_ptr(), base_weight.data_ptr(), bank.lora_a.data_ptr(), bank.lora_b.data_ptr(),
+                        int(mx4), ldx, x.data_ptr(), weight.data_ptr(), bank.lora_a.data_ptr(), bank.lora_b.data_ptr(),
                         bank.ranks.data_ptr(), bank.scales.data_ptr(), row_slot.data_ptr())
     tensor_cores = dtype is not torch.float32
     if tensor_cores and (K % 8 or N % 8 or ldx % 8 or
@@ -176,7 +185,7 @@ def fused_lora_forward_rows(x: torch.Tensor, base_weight: torch.Tensor, bank: Ad
             x = x.clone(memory_format=torch.contiguous_format)
             p.x_dev, p.ldx = x.data_ptr(), K
         tensor_cores = not (K % 8 or N % 8 or (p.w_dev | p.a_bank_dev | p.b_bank_dev | out.data_ptr()) % 16)
-        b200_ops._warn_if_cuda_core(dtype, K, N, (x, base_weight, bank.lora_a, bank.lora_b, out))
+        b200_ops._warn_if_cuda_core(dtype, K, N, (x, weight, bank.lora_a, bank.lora_b, out))
     L = nat.lib()
     ws = torch.empty(L.lf_rows_workspace_bytes(T, N, bank.r_pad, p.dtype), dtype=torch.uint8, device=device)
     with nat.on_device(device.index):
