@@ -588,6 +588,7 @@ struct RowsGemm {
   RowsArgs a;
   int ksplit, stages;
   int sub;  // 64-element K blocks of a stage
+  int slots;  // blocks of codes behind the stages (kMx4)
   uint32_t idesc;
 };
 
@@ -610,13 +611,11 @@ __device__ __forceinline__ uint32_t pack_pair<__nv_bfloat16>(float a, float b) {
 template <>
 __device__ __forceinline__ uint32_t pack_pair<__half>(float a, float b) { return pack_f16x2(a, b); }
 
-// kMx4: stages that a lane of the decoding warps has loads of in flight.  256 lanes x 17 bytes x 8 are 35 KB an SM, about
-// what HBM's latency asks for.
-constexpr int kMx4Ahead = 8;
+constexpr int kMaxSlots = 16;  // of codes (kMx4)
 
 // kTN: rows (tokens) of a tile, the N of the MMA.  Warp 0 loads, warp 1 issues the MMAs, eight epilogue warps
-// finish the tile.  kMx4: the weight is held in 4 bits (lf_mx4.cuh, map_w is not used), and the epilogue warps, idle until
-// the tile is done, decode it into the ring.
+// finish the tile.  kMx4: the weight is held in 4 bits (lf_mx4.cuh, map_w is not used).  One more warp copies its codes into
+// a ring of their own, and the epilogue warps, idle until the tile is done, decode them into the stages.
 template <typename T, int kTN, bool kMx4>
 __global__ void __maxnreg__(80)
     rows_gemm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
@@ -626,6 +625,7 @@ __global__ void __maxnreg__(80)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ uint64_t full[kMaxStages], empty[kMaxStages], acc_bar, drain_bar;
+  __shared__ uint64_t code_full[kMx4 ? kMaxSlots : 1], code_empty[kMx4 ? kMaxSlots : 1];
   __shared__ uint32_t tmem_slot;
   __shared__ volatile int abort_flag;
   __shared__ uint8_t s_on[kTN];  // whether the row has an adapter
@@ -649,6 +649,11 @@ __global__ void __maxnreg__(80)
       mbar_init(&full[s], kMx4 ? 1 + kEpiWarps : 1);
       mbar_init(&empty[s], 1);
     }
+    if (kMx4)
+      for (int i = 0; i < prm.slots; ++i) {
+        mbar_init(&code_full[i], 1);
+        mbar_init(&code_empty[i], kEpiWarps);
+      }
     mbar_init(&acc_bar, 1);
     mbar_init(&drain_bar, 1);
     abort_flag = 0;
@@ -732,40 +737,50 @@ __global__ void __maxnreg__(80)
       }
     }
     __syncwarp();
-  } else {
-    const int w = warp - 2, row = (w & 3) * 32 + lane, half = w >> 2;  // kMx4: the codes of this lane in a block
-    const uint8_t* src = nullptr;
-    Mx4Piece ahead[kMx4Ahead];
-    auto fetch = [&](int kb) {
-      const uint8_t* b = src + static_cast<int64_t>(kb) * kMx4Block;
-      return mx4_load(b + half * kMx4HalfBytes + row * 16, b + kMx4Codes + half * kMx4Rows + row);
-    };
-    if constexpr (kMx4) {
-      src = p.mx4.data + static_cast<int64_t>(n0 / kWRows) * p.mx4.col_blocks * kMx4Block;
-#pragma unroll
-      for (int i = 0; i < kMx4Ahead; ++i)
-        if (kb0 + i < kb1) ahead[i] = fetch(kb0 + i);
+  } else if (kMx4 && warp == 2 + kEpiWarps) {
+    const uint8_t* src = p.mx4.data + static_cast<int64_t>(n0 / kWRows) * p.mx4.col_blocks * kMx4Block;
+    uint8_t* codes_at = ring + stages * stage_bytes;
+    int slot = 0;
+    uint32_t phase = 0, issued = 0, parity = 0;
+    bool ok = true;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait_stage(&code_empty[slot], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) {
+        ok = false;
+        break;
+      }
+      if (elect_one()) {
+        mbar_arrive_expect_tx(&code_full[slot], kMx4Block);
+        bulk_load(codes_at + slot * kMx4Block, src + static_cast<int64_t>(kb) * kMx4Block, kMx4Block, &code_full[slot]);
+      }
+      __syncwarp();
+      issued |= 1u << slot;
+      parity = (parity & ~(1u << slot)) | (phase << slot);
+      if (++slot == prm.slots) {
+        slot = 0;
+        phase ^= 1;
+      }
     }
+    if (!ok && lane == 0)
+      for (int i = 0; i < prm.slots; ++i)
+        if (issued & (1u << i)) drain_wait(&code_full[i], (parity >> i) & 1u, p.err);
+    __syncwarp();
+  } else {
     for (int i = tid - 64; i < kTN; i += kEpiWarps * 32)
       s_on[i] = p.row_slot != nullptr && t0 + i < p.T && row_adapter(p, t0 + i, false) != kNoSlot;
     named_barrier(1, kEpiWarps * 32);
     if constexpr (kMx4) {
-      int stage = 0;
-      uint32_t phase = 0;
-      bool ok = true;
-      int kb = kb0, in = 0;  // block, its place in the stage
-      while (ok && kb < kb1) {
-#pragma unroll
-        for (int i = 0; i < kMx4Ahead; ++i) {
-          if (!ok || kb >= kb1) break;
-          if (in == 0) {
-            ok = warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
-            if (!ok) break;
-          }
-          mx4_store<T>(ring + stage * stage_bytes + in * block_bytes + row * 128, row, 4 * half, ahead[i]);
-          if (kb + kMx4Ahead < kb1) ahead[i] = fetch(kb + kMx4Ahead);
-          ++kb;
-          if (++in < sub && kb < kb1) continue;
+      const int w = warp - 2, row = (w & 3) * 32 + lane, half = w >> 2;  // this lane's codes in a block
+      const uint8_t* codes_at = ring + stages * stage_bytes;
+      int stage = 0, slot = 0, in = 0;  // in: the block's place in the stage
+      uint32_t phase = 0, slot_phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!warp_wait_stage(&code_full[slot], slot_phase, &abort_flag, p.err, kErrTimeoutFull)) break;
+        uint4 codes;
+        uint32_t scale;
+        mx4_fetch(codes_at + slot * kMx4Block, row, half, codes, scale);
+        if (in == 0 && !warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) break;
+        mx4_store<T>(ring + stage * stage_bytes + in * block_bytes + row * 128, row, half, codes, scale);
+        if (++in == sub || kb + 1 == kb1) {
           in = 0;
           fence_proxy_async_smem();
           __syncwarp();
@@ -774,6 +789,13 @@ __global__ void __maxnreg__(80)
             stage = 0;
             phase ^= 1;
           }
+        } else {
+          __syncwarp();
+        }
+        if (lane == 0) mbar_arrive(&code_empty[slot]);
+        if (++slot == prm.slots) {
+          slot = 0;
+          slot_phase ^= 1;
         }
       }
       __syncwarp();
@@ -788,7 +810,7 @@ __global__ void __maxnreg__(80)
   const int ew = warp - 2, quad = warp & 3;
   const int own = kWRows / ks, rows = min(kTN, p.T - t0);
   if (ks > 1) cluster_sync_all();  // every ring is idle
-  if (ok && ew >= 0) {
+  if (ok && ew >= 0 && ew < kEpiWarps) {
     constexpr int kN = kTN >= 64 ? 32 : 8;  // rows a load
     constexpr int kHalf = kTN / 2;          // the two warps of a lane quarter take half the rows each
     const int f = quad * 32 + lane, first = (ew >> 2) * kHalf;
@@ -811,7 +833,7 @@ __global__ void __maxnreg__(80)
     const int shift = 4 - (31 - __clz(ks));               // log2 of 8-feature pieces a row
     const float* sums = reinterpret_cast<const float*>(ring);
     const int pitch = (p.N + 15) & ~15;
-    for (int i = tid; i < rows << shift; i += kGemmThreads) {
+    for (int i = tid; i < rows << shift; i += kMx4 ? kGemmThreads + 32 : kGemmThreads) {
       const int r = i >> shift, f = (i & ((1 << shift) - 1)) * 8, n = nb + f;
       if (n >= p.N) continue;  // N is a multiple of 8
       float4 lo = make_float4(0.f, 0.f, 0.f, 0.f), hi = lo;
@@ -1556,7 +1578,7 @@ cudaError_t launch_gemm(const RowsGemm& g, const CUtensorMap& w, const CUtensorM
   if (e != cudaSuccess) return e;
   const dim3 grid(static_cast<unsigned>((g.a.N + kWRows - 1) / kWRows * g.ksplit),
                   static_cast<unsigned>((g.a.T + kTN - 1) / kTN));
-  return launch_cluster(k, grid, g.ksplit, dim3(kGemmThreads), ring_bytes(kTN) + 1024, st,
+  return launch_cluster(k, grid, g.ksplit, dim3(kMx4 ? kGemmThreads + 32 : kGemmThreads), ring_bytes(kTN) + 1024, st,
                         g.a.row_slot != nullptr, w, x, g);  // early beside the adapters' part only, which came after x
 }
 
@@ -1640,6 +1662,12 @@ cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CU
   const int room = ring_bytes(tn), block = (kWRows + tn) * kBK * 2;
   g.sub = room / (2 * block) >= 3 ? 2 : 1;
   g.stages = room / (g.sub * block);
+  if (kMx4) {  // three stages (two of 64 rows' pairs of blocks), the rest for codes: a CTA's K range of a few rows at once
+    g.sub = tn <= 64 ? 2 : 1;
+    g.stages = tn == 64 ? 2 : 3;
+    g.slots = (room - g.stages * g.sub * block) / kMx4Block;
+    if (g.slots > kMaxSlots) g.slots = kMaxSlots;
+  }
   if (tn == 16) return launch_gemm<T, 16, kMx4>(g, w, x, st);
   if (tn == 32) return launch_gemm<T, 32, kMx4>(g, w, x, st);
   if (tn == 64) return launch_gemm<T, 64, kMx4>(g, w, x, st);

@@ -84,8 +84,8 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const uint16_t* 
                encode2(f[5] * up, f[7] * up) << 24;
       }
       uint8_t* b = blocks + (c >> 1) * kMx4Block;
-      *reinterpret_cast<uint32_t*>(b + (c & 1) * kMx4HalfBytes + r * 16 + j * 4) = code;
-      if (j == 0) b[kMx4Codes + (c & 1) * kMx4Rows + r] = static_cast<uint8_t>(s);
+      *reinterpret_cast<uint32_t*>(b + mx4_code_at(r, c & 1) + j * 4) = code;
+      if (j == 0) b[mx4_scale_at(r, c & 1)] = static_cast<uint8_t>(s);
     }
   }
 }
@@ -105,8 +105,8 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(const uint8_t*
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint8_t* b = blocks + (c >> 1) * kMx4Block;
-      code[c] = *reinterpret_cast<const uint32_t*>(b + (c & 1) * kMx4HalfBytes + r * 16 + j * 4);
-      scale[c] = b[kMx4Codes + (c & 1) * kMx4Rows + r];
+      code[c] = *reinterpret_cast<const uint32_t*>(b + mx4_code_at(r, c & 1) + j * 4);
+      scale[c] = b[mx4_scale_at(r, c & 1)];
     }
     if (n >= N) continue;
 #pragma unroll

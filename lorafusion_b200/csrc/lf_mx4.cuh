@@ -3,12 +3,13 @@
 // A value is q 2^E: q = (-1)^s {0, 0.5, 1, 1.5, 2, 3, 4, 6} in 4 bits (sign, two exponent bits, one of mantissa) and E
 // shared by 32 neighbours along K, stored as the byte E + 127 (255: not a number), after the OCP microscaling formats.
 //
-// A weight [N, K] is cut into blocks of 128 rows x 64 columns, block (n / 128, k / 64) after block, K padded to 128 and
-// N to 128 with zeros, so that whatever a tile of a product reads lies in the buffer.  A block is
-//   codes   [2 halves of 32 columns][128 rows][16 bytes],
-//   scales  [2 halves][128 rows], one byte each:
-// a warp whose lanes are 32 rows reads 512 contiguous bytes, and the same bytes serve y = x V^T (64 columns of 128 rows)
-// and grad_x = g V (64 rows of 128 columns).  Of eight codes in a 32-bit word, elements 0, 2, 4, 6 are in the low half
+// A weight [N, K] is cut into pieces of 64 rows x 64 columns, two rows of pieces to a tile of 128 rows: piece
+// ((n / 128, k / 64), n / 64 % 2) after piece, K padded to 128 and N to 128 with zeros, so that whatever a tile of a
+// product reads lies in the buffer.  A piece is
+//   codes   [2 halves of 32 columns][64 rows][16 bytes],
+//   scales  [2 halves][64 rows], one byte each.
+// Two pieces make a stage of either product, y = x V^T (128 rows of 64 columns: neighbours) or grad_x = g V (64
+// rows of 128 columns: two copies), and a warp whose lanes are 32 rows reads 512 contiguous bytes.  Of eight codes in a 32-bit word, elements 0, 2, 4, 6 are in the low half
 // and 1, 3, 5, 7 in the high half: elements 2p and 2p + 1 come out as one register of two 16-bit values.
 #pragma once
 
@@ -19,9 +20,13 @@
 namespace lf {
 
 constexpr int kMx4Rows = 128, kMx4Cols = 64;
-constexpr int kMx4HalfBytes = kMx4Rows * 16;                    // codes of 32 columns
-constexpr int kMx4Codes = 2 * kMx4HalfBytes;                    // where the scales start
-constexpr int kMx4Block = kMx4Codes + 2 * kMx4Rows;             // 4352 bytes
+constexpr int kMx4HalfBytes = 64 * 16;                // codes of 64 rows x 32 columns
+constexpr int kMx4Codes = 2 * kMx4HalfBytes;          // where a piece's scales start
+constexpr int kMx4Piece = kMx4Codes + 2 * 64;         // 2176 bytes
+constexpr int kMx4Block = 2 * kMx4Piece;              // 128 rows x 64 columns
+// Byte offsets in a block (or a stage of two pieces) of row r's 16 bytes of codes and its scale in half c.
+__host__ __device__ inline int mx4_code_at(int r, int c) { return (r >> 6) * kMx4Piece + c * kMx4HalfBytes + (r & 63) * 16; }
+__host__ __device__ inline int mx4_scale_at(int r, int c) { return (r >> 6) * kMx4Piece + kMx4Codes + c * 64 + (r & 63); }
 __host__ __device__ inline int mx4_row_tiles(int N) { return (N + kMx4Rows - 1) / kMx4Rows; }
 __host__ __device__ inline int mx4_col_blocks(int K) { return (K + 127) / 128 * 2; }
 
@@ -83,27 +88,18 @@ struct Mx4<__half> {
   }
 };
 
-// 32 codes and their scale byte, in flight.  Weights are read once a tile: they do not displace what L1 holds.
-struct Mx4Piece {
-  uint4 codes;
-  uint32_t scale;
-};
-__device__ __forceinline__ Mx4Piece mx4_load(const uint8_t* codes, const uint8_t* scale) {
-  Mx4Piece p;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(p.codes.x), "=r"(p.codes.y), "=r"(p.codes.z), "=r"(p.codes.w)
-               : "l"(codes));
-  asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(p.scale) : "l"(scale));
-  return p;
-}
-// The piece's 32 values as four 16-byte granules first .. first + 3 of a 128-byte row of shared memory with the 128-byte
+// 32 codes (half c of row r of a stage in shared memory) as granules 4c .. 4c + 3 of a 128-byte row with the 128-byte
 // swizzle: granule g of row r lies at slot g ^ (r % 8).
+__device__ __forceinline__ void mx4_fetch(const uint8_t* stage, int r, int c, uint4& codes, uint32_t& scale) {
+  codes = *reinterpret_cast<const uint4*>(stage + mx4_code_at(r, c));
+  scale = stage[mx4_scale_at(r, c)];
+}
 template <typename T>
-__device__ __forceinline__ void mx4_store(uint8_t* row, int r, int first, const Mx4Piece& p) {
-  const uint32_t s = Mx4<T>::scale(p.scale);
-  const uint32_t w[4] = {p.codes.x, p.codes.y, p.codes.z, p.codes.w};
+__device__ __forceinline__ void mx4_store(uint8_t* row, int r, int c, const uint4& codes, uint32_t scale) {
+  const uint32_t s = Mx4<T>::scale(scale);
+  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
 #pragma unroll
-  for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(row + (((first + j) ^ (r & 7)) << 4)) = Mx4<T>::decode(w[j], s);
+  for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(row + (((4 * c + j) ^ (r & 7)) << 4)) = Mx4<T>::decode(w[j], s);
 }
 
 }  // namespace lf

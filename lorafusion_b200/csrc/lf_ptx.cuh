@@ -379,6 +379,12 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
+// The same at CTA scope: for what the other CTA's thread takes note of but does not read itself.  A release at cluster
+// scope waits for all of the thread's outstanding memory operations, about 0.8 us.
+__device__ __forceinline__ void mbar_arrive_cluster_cta(uint32_t bar_cluster) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
+}
+
 // ---------------------------------------------------------------- clusters
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

@@ -393,6 +393,19 @@ constexpr int kTailBufBytes = 3 * kTailChunkBytes;
 static_assert(4 * 2 * kTailBufBytes <= kPairStages * (kPairABytes + kPairBBytes), "tail buffers fit the ring");
 constexpr int kPairSmem = 1024 + kPairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kPairBarBytes + kPairEntBytes;
 static_assert(kPairSmem <= 227 * 1024, "pair kernel shared memory");
+// A pair whose Q is held in 4 bits gives one stage of the ring for kMx4Slots stages of codes (and their barriers).  Its
+// tail tiles have at most three parts, so that an epilogue warp's buffers fit its share of the shorter ring.
+constexpr int kMx4Slots = 7;
+constexpr int kMx4PairStages = 5;
+constexpr int kMx4CodeBytes = kMx4Slots * kMx4Block;
+constexpr int kMx4BarBytes = 2 * kMx4Slots * 8;
+constexpr int kMx4PairSmem =
+    1024 + kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes + kPairBarBytes + kPairEntBytes + kMx4BarBytes;
+static_assert(kMx4PairSmem <= 227 * 1024, "pair kernel shared memory");
+static_assert(kRoleStages * kRoleStageBytes <= kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes,
+              "shrink-role stages must fit");
+__host__ __device__ constexpr int pair_tail_share(bool mx4) { return (mx4 ? kMx4PairStages : kPairStages) * (kPairABytes + kPairBBytes) / 4; }
+static_assert(pair_tail_share(false) == 2 * kTailBufBytes && pair_tail_share(true) >= 4 * kTailChunkBytes, "tail buffers");
 
 struct PairParams {
   void* out;
@@ -753,92 +766,110 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
   if (kPrologue) __syncthreads();
 }
 
-// The decoding warps of a kMx4 pair: Q is held in 4 bits (lf_mx4.cuh), and its 128 x 64 tile of every stage is written by
-// these eight warps instead of a copy, the 16-bit values in the layout the copy would have left: row r of 64 columns of K
-// for x V^T, for g V (kQMN) two panels of 64 columns by 64 rows.  A lane has 32 codes of a stage: it loads them
-// kMx4Ahead stages ahead (a stage takes about 0.3 us, HBM two to three times that), waits for the
-// stage to be free, stores the values and reports to the even CTA's `full` barrier, whose phase also counts the P
-// tiles' bytes.  LoRA stages are filled by copies alone; the warps report them unseen.
+// The extra warps of a kMx4 pair: Q is held in 4 bits (lf_mx4.cuh), and its 128 x 64 tile of every stage is written by
+// eight warps instead of a copy, the 16-bit values in the layout that the copy would have left: 128 rows of 64 columns of K
+// for x V^T, for g V (kQMN) two panels of 64 columns by 64 rows.  The codes of a stage are two pieces that one more warp
+// copies into a ring of their own, kMx4Slots stages ahead.  (Loaded by the decoding warps themselves they were waited for
+// at every fence: 0.8 us a stage.)  A warp waits for the codes and for the stage to be free, stores the values and
+// reports to the even CTA's `full` barrier, whose phase also counts the P tiles' bytes; at CTA scope, since what the
+// even CTA's MMAs read of the odd CTA lies in that one's shared memory and was fenced there (released at cluster scope,
+// every stage waited 0.8 us for the release).  LoRA stages are filled by copies alone; the warps report them unseen.
 constexpr int kMx4Warps = 8;
-constexpr int kMx4Threads = kThreads + 32 * kMx4Warps;
-constexpr int kMx4Ahead = 4;
+constexpr int kMx4Threads = kThreads + 32 * kMx4Warps + 32;
 
-template <bool kQMN, typename OutT>
+struct Mx4Ring {
+  uint8_t* slots;
+  uint64_t *full, *empty;
+};
+
+template <bool kQMN>
+__device__ __forceinline__ void pair_codes_role(const PairParams& prm, const PairSched& sched, int pair, int n_pairs,
+                                                int n_units, int nkb, int crank, const Mx4Ring& ring,
+                                                volatile int* abort_flag) {
+  const Tables& tb = prm.tb;
+  int slot = 0;
+  uint32_t phase = 0, issued = 0, parity = 0;
+  bool ok = true;
+  for (int k = 0; k < n_units && ok; ++k) {
+    const PairUnit un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
+    const int cols = 2 * un.n + crank;  // of 128 output columns; past the weight's last the last again, not stored
+    for (int kb = un.kb0; kb < un.kb1; ++kb) {
+      ok = warp_wait_stage(&ring.empty[slot], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
+      if (!ok) break;
+      if (elect_one()) {
+        uint8_t* dst = ring.slots + slot * kMx4Block;
+        mbar_arrive_expect_tx(&ring.full[slot], kMx4Block);
+        if (kQMN) {
+          const int64_t first = static_cast<int64_t>(kb >> 1) * prm.mx4.col_blocks;
+#pragma unroll
+          for (int panel = 0; panel < 2; ++panel)
+            bulk_load(dst + panel * kMx4Piece,
+                      prm.mx4.data + (first + min(2 * cols + panel, prm.mx4.col_blocks - 1)) * kMx4Block + (kb & 1) * kMx4Piece,
+                      kMx4Piece, &ring.full[slot]);
+        } else {
+          const int64_t first = static_cast<int64_t>(min(cols, prm.mx4.row_tiles - 1)) * prm.mx4.col_blocks;
+          bulk_load(dst, prm.mx4.data + (first + kb) * kMx4Block, kMx4Block, &ring.full[slot]);
+        }
+      }
+      __syncwarp();
+      issued |= 1u << slot;
+      parity = (parity & ~(1u << slot)) | (phase << slot);
+      if (++slot == kMx4Slots) {
+        slot = 0;
+        phase ^= 1;
+      }
+    }
+  }
+  if (!ok && (threadIdx.x & 31) == 0)  // let every copy that was started land
+    for (int i = 0; i < kMx4Slots; ++i)
+      if (issued & (1u << i)) drain_wait(&ring.full[i], (parity >> i) & 1u, tb.err);
+  __syncwarp();
+}
+
+template <int kStages, typename OutT>
 __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const PairSched& sched, int pair, int n_pairs,
-                                                 int n_units, int nkb, int crank, uint8_t* sB, uint32_t full_lead,
-                                                 uint64_t* empty, volatile int* abort_flag) {
+                                                 int n_units, int nkb, uint8_t* sB, uint32_t full_lead, uint64_t* empty,
+                                                 const Mx4Ring& ring, volatile int* abort_flag) {
   const int w = (threadIdx.x >> 5) - kThreads / 32, lane = threadIdx.x & 31;
   const Tables& tb = prm.tb;
-  const int half = w >> 2;                                          // which 32 columns of a block
-  const int row = kQMN ? (w & 1) * 32 + lane : (w & 3) * 32 + lane;  // of the stage's tile
-  const int panel = (w >> 1) & 1;                                   // kQMN: which 64 of the 128 columns
-  uint8_t* dst = sB + (kQMN ? panel * 8192 : 0) + row * 128;
-  auto fetch = [&](int n, int kb) {  // tiles past the weight's last one repeat it: their columns are not stored
-    int64_t block;
-    int r = row;
-    if (kQMN) {
-      block = static_cast<int64_t>(kb >> 1) * prm.mx4.col_blocks + min(2 * (2 * n + crank) + panel, prm.mx4.col_blocks - 1);
-      r += (kb & 1) * 64;
-    } else {
-      block = static_cast<int64_t>(min(2 * n + crank, prm.mx4.row_tiles - 1)) * prm.mx4.col_blocks + kb;
-    }
-    const uint8_t* b = prm.mx4.data + block * kMx4Block;
-    return mx4_load(b + half * kMx4HalfBytes + r * 16, b + kMx4Codes + half * kMx4Rows + r);
-  };
-  // the next piece to load: unit fk, k-block fkb
-  int fk = 0, fkb = 0, fkb1 = 0, fn = 0;
-  auto open = [&]() {
-    if (fk >= n_units) return;
-    const PairUnit un = pair_unit(prm, sched, pair, n_pairs, fk, nkb);
-    fkb = un.kb0, fkb1 = un.kb1, fn = un.n;
-  };
-  Mx4Piece ring[kMx4Ahead];
-  auto refill = [&](Mx4Piece& p) {
-    if (fk >= n_units) return;
-    p = fetch(fn, fkb);
-    if (++fkb == fkb1) {
-      ++fk;
-      open();
-    }
-  };
-  open();
-#pragma unroll
-  for (int i = 0; i < kMx4Ahead; ++i) refill(ring[i]);
-  int k = 0, stage = 0;
-  uint32_t phase = 0;
-  PairUnit un = n_units > 0 ? pair_unit(prm, sched, pair, n_pairs, 0, nkb) : PairUnit{};
-  int kb = un.kb0;
+  const int half = w >> 2;             // which 32 columns of a piece
+  const int row = (w & 3) * 32 + lane;  // of the stage: rows 0..63 of the first piece, then of the second
+  uint8_t* dst = sB + row * 128;
+  int stage = 0, slot = 0;
+  uint32_t phase = 0, slot_phase = 0;
   bool ok = true;
   auto report = [&]() {
     __syncwarp();
-    if (lane == 0) mbar_arrive_cluster(full_lead + static_cast<uint32_t>(stage * 8));
-    if (++stage == kPairStages) {
+    if (lane == 0) mbar_arrive_cluster_cta(full_lead + static_cast<uint32_t>(stage * 8));
+    if (++stage == kStages) {
       stage = 0;
       phase ^= 1;
     }
   };
-  while (ok && k < n_units) {
-#pragma unroll
-    for (int i = 0; i < kMx4Ahead; ++i) {
-      if (!ok || k >= n_units) break;
+  for (int k = 0; k < n_units && ok; ++k) {
+    const PairUnit un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
+    for (int kb = un.kb0; kb < un.kb1; ++kb) {
+      ok = warp_wait_stage(&ring.full[slot], slot_phase, abort_flag, tb.err, kErrTimeoutFull);
+      if (!ok) break;
+      uint4 codes;
+      uint32_t scale;
+      mx4_fetch(ring.slots + slot * kMx4Block, row, half, codes, scale);
       ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
       if (!ok) break;
-      mx4_store<OutT>(dst + stage * kPairBBytes, row, 4 * half, ring[i]);
+      mx4_store<OutT>(dst + stage * kPairBBytes, row, half, codes, scale);
       fence_proxy_async_smem();
       report();
-      refill(ring[i]);
-      if (++kb < un.kb1) continue;
-      int n_lora = 0;
-      if (prm.lora && un.last)
-        n_lora = (tb.pair_lora(un.mp + 1) - tb.pair_lora(un.mp)) * prm.s_planes;
-      for (int j = 0; ok && j < n_lora; j += prm.lora_per_stage) {
-        ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
-        if (ok) report();
+      if (lane == 0) mbar_arrive(&ring.empty[slot]);  // every lane has its codes: they were stored
+      if (++slot == kMx4Slots) {
+        slot = 0;
+        slot_phase ^= 1;
       }
-      if (++k < n_units) {
-        un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
-        kb = un.kb0;
-      }
+    }
+    if (!ok || !prm.lora || !un.last) continue;
+    const int n_lora = (tb.pair_lora(un.mp + 1) - tb.pair_lora(un.mp)) * prm.s_planes;
+    for (int j = 0; ok && j < n_lora; j += prm.lora_per_stage) {
+      ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
+      if (ok) report();
     }
   }
 }
@@ -852,12 +883,14 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
                         const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_a,
                         const __grid_constant__ CUtensorMap map_p2, const __grid_constant__ CUtensorMap map_a2,
                         const PairParams prm) {
+  constexpr int kStages = kMx4 ? kMx4PairStages : kPairStages;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
-  uint8_t* sB = smem + kPairStages * kPairABytes;
-  uint8_t* sOut = sB + kPairStages * kPairBBytes;
-  uint64_t* full = reinterpret_cast<uint64_t*>(sOut + kPairOutBytes);
+  uint8_t* sB = smem + kStages * kPairABytes;
+  uint8_t* sOut = sB + kStages * kPairBBytes;
+  uint8_t* bars = sOut + kPairOutBytes + (kMx4 ? kMx4CodeBytes : 0);
+  uint64_t* full = reinterpret_cast<uint64_t*>(bars);
   uint64_t* empty = full + kPairBars;
   uint64_t* tfull = empty + kPairBars;
   uint64_t* tempty = tfull + 2;
@@ -866,14 +899,16 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pub + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   // a shrink prologue's barriers: never re-initialized while its last arrivals may be in flight
-  uint64_t* rfull = reinterpret_cast<uint64_t*>(sOut + kPairOutBytes + 256);
+  uint64_t* rfull = reinterpret_cast<uint64_t*>(bars + 256);
   uint64_t* rempty = rfull + kRoleStages;
   uint64_t* rtfull = rempty + kRoleStages;
   uint64_t* rtempty = rtfull + 2;
   uint64_t* rdrain = rtempty + 2;
   uint64_t* rpub = rdrain + 1;
-  uint64_t* tail_bar = reinterpret_cast<uint64_t*>(sOut + kPairOutBytes + kPairTailBarOff);
-  int* pair_ent = reinterpret_cast<int*>(sOut + kPairOutBytes + kPairBarBytes);
+  uint64_t* tail_bar = reinterpret_cast<uint64_t*>(bars + kPairTailBarOff);
+  int* pair_ent = reinterpret_cast<int*>(bars + kPairBarBytes);
+  Mx4Ring codes{sOut + kPairOutBytes, reinterpret_cast<uint64_t*>(bars + kPairBarBytes + kPairEntBytes), nullptr};
+  codes.empty = codes.full + kMx4Slots;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) < 2 * prm.n_shrink_pairs) {
@@ -893,7 +928,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
   const Tables& tb = prm.tb;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kPairStages; ++s) {
+    for (int s = 0; s < kStages; ++s) {
       mbar_init(&full[s], kMx4 ? 1 + 2 * kMx4Warps : 1);
       mbar_init(&empty[s], 1);
     }
@@ -902,6 +937,11 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
       mbar_init(&tempty[b], 8);  // one arrive per epilogue warp of both CTAs
     }
     for (int b = 0; b < 8; ++b) mbar_init(&tail_bar[b], 1);
+    if (kMx4)
+      for (int i = 0; i < kMx4Slots; ++i) {
+        mbar_init(&codes.full[i], 1);
+        mbar_init(&codes.empty[i], kMx4Warps);
+      }
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -986,7 +1026,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
           }
           issued_mask |= 1u << stage;
           last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == kPairStages) {
+          if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
@@ -1041,7 +1081,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
           }
           issued_mask |= 1u << stage;
           last_parity = (last_parity & ~(1u << stage)) | (phase << stage);
-          if (++stage == kPairStages) {
+          if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
@@ -1051,7 +1091,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
       if (!ok) break;
     }
     if (lane == 0 && !ok && crank == 0)  // copies of both CTAs complete on the even CTA's barriers
-      for (int s = 0; s < kPairStages; ++s)
+      for (int s = 0; s < kStages; ++s)
         if (issued_mask & (1u << s)) drain_wait(&full[s], (last_parity >> s) & 1u, tb.err);
     __syncwarp();
   } else if (warp == 1) {
@@ -1095,7 +1135,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
           }
           issued_any = true;
           umma_commit_pair_both(empty_local + stage * 8);
-          if (++stage == kPairStages) {
+          if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
@@ -1119,7 +1159,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
           }
           issued_any = true;
           umma_commit_pair_both(empty_local + stage * 8);
-          if (++stage == kPairStages) {
+          if (++stage == kStages) {
             stage = 0;
             phase ^= 1;
           }
@@ -1134,8 +1174,10 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
     }
     __syncwarp();
   } else if (kMx4 && warp >= kThreads / 32) {
-    pair_decode_role<kQMN, OutT>(prm, sched, pair, n_pairs, n_units, nkb, static_cast<int>(crank), sB, full_lead, empty,
-                                 abort_flag);
+    if (warp == kMx4Threads / 32 - 1)
+      pair_codes_role<kQMN>(prm, sched, pair, n_pairs, n_units, nkb, static_cast<int>(crank), codes, abort_flag);
+    else
+      pair_decode_role<kStages, OutT>(prm, sched, pair, n_pairs, n_units, nkb, sB, full_lead, empty, codes, abort_flag);
   } else {
     const int q = warp & 3;
     int it = 0;
@@ -1154,7 +1196,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
       // there and bulk-copies it out.  The last part copies the earlier parts' chunks in: all
       // four at once after one earlier part, else chunk c into buffer c & 1 while c - 1 is added.
       const bool tail_last = un.part > 0 && un.last;
-      uint8_t* tail_w = sA + q * (2 * kTailBufBytes);  // this warp's share of the ring
+      uint8_t* tail_w = sA + q * pair_tail_share(kMx4);  // this warp's share of the ring
       auto tail_chunk = [&](int c, int p) {  // chunk c of earlier part p in shared memory
         return tail_w + (un.part == 1 ? c : (c & 1) * un.part + p) * kTailChunkBytes;
       };
@@ -1193,7 +1235,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
       // The pair's last unit: the ring is idle (every MMA of the pair is done), so each warp
       // stages all four chunks there, after its partial-tile buffers, and no store waits for an
       // earlier one to have read its buffer.
-      const bool ring_stage = k == n_units - 1 && un.part <= 2;
+      const bool ring_stage = k == n_units - 1 && un.part <= (kMx4 ? 0 : 2);
       uint8_t* ring_w = tail_w + (tail_last ? (un.part == 1 ? 4 : 2 * un.part) * kTailChunkBytes : 0);
 #pragma unroll 1
       for (int c = 0; c < 256 / 64; ++c) {
@@ -2362,7 +2404,8 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
     const int avail = few && p.n_shrink_pairs == 0 ? all_pairs : gemm_pairs;
     const int rem = few ? total : total - (total / gemm_pairs) * gemm_pairs;
     int parts = rem > 0 && 2 * rem <= avail ? avail / rem : 1;
-    if (parts > 4) parts = 4;
+    const int most = mx4 != nullptr ? 3 : 4;
+    if (parts > most) parts = most;
     while (parts > 1 && (rem * (parts - 1) > tail->slots || nkb < 2 * parts)) --parts;
     if (parts > 1) {
       if (few) gemm_pairs = total * parts;  // every tile is a tail tile, one part per pair
@@ -2375,7 +2418,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (gemm_pairs + p.n_shrink_pairs));
   cfg.blockDim = dim3(mx4 != nullptr ? kMx4Threads : kThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = mx4 != nullptr ? kMx4PairSmem : kPairSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -2391,7 +2434,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cudaError_t e;
 #define LF_LAUNCH_PAIR(QMN, OT, DELTA, MX4)                                                                         \
   {                                                                                                                  \
-    e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, kPairSmem);                                            \
+    e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, MX4 ? kMx4PairSmem : kPairSmem);                       \
     if (e != cudaSuccess) return e;                                                                                  \
     e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, maps.p, maps.q, maps.s, maps.l, maps.o,   \
                            *a_map, *p2_map, *a2_map, p);                                                             \

@@ -219,7 +219,8 @@ def adapters_of(K, N, ranks, dtype, seed=30):
 
 
 def same_as_dense(T, K, N, ranks, cuts, dtype):
-    """Over a weight in 4 bits the fused ops give what they give over its dense values."""
+    """Over a weight in 4 bits the fused ops give what they give over its dense values: the same bits of dA and dB (the
+    same launches), y and grad_x up to the order of their sums, which a tile split along K may change."""
     q = quantize_weight(rand(N, K, seed=21, scale=K ** -0.5, dtype=dtype))
     dense = q.dequantize()
     x, g = rand(T, K, seed=22, dtype=dtype), rand(T, N, seed=23, dtype=dtype)
@@ -232,7 +233,11 @@ def same_as_dense(T, K, N, ranks, cuts, dtype):
     b200_ops.clear_weight_cache()
     y0 = b200_ops.fused_lora_forward(x, dense, a, b, specs, routing)
     gx0, ga0, gb0 = b200_ops.fused_lora_backward(g, x, dense, a, b, specs, routing)
-    assert torch.equal(y, y0) and torch.equal(gx, gx0)
+    for got, ref, left, right, n in ((y, y0, x, dense.t(), K), (gx, gx0, g, dense, N)):
+        # each is off by its sum's error and half a step; the adapters' part, at most as large here, is summed with it
+        mag = left.double().abs() @ right.double().abs() + ref.double().abs()
+        tol = torch.finfo(dtype).eps * ref.double().abs() + 2 * (n + 64) * 2.0 ** -24 * 2 * mag
+        assert ((got.double() - ref.double()).abs() <= tol + torch.finfo(dtype).smallest_normal).all()
     assert ga.keys() == ga0.keys() and all(torch.equal(ga[i], ga0[i]) and torch.equal(gb[i], gb0[i]) for i in ga)
     assert nat.device_error() == 0
     return y, x, dense, a, b, specs, routing
