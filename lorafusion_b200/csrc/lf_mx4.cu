@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "lf_internal.cuh"
 #include "lf_mx4.cuh"
 
@@ -36,7 +38,7 @@ __device__ __forceinline__ uint4 load8(const uint16_t* w, int n, int k, int N, i
   return v;
 }
 
-// Two codes, the nearest of a and b with ties to the even code and 6 for what is larger, in one byte.
+// Two codes, the nearest of each value with ties to the even code and 6 for what is larger, one in each half.
 __device__ __forceinline__ uint32_t encode2(float low, float high) {
   uint32_t r;
   asm("{\n\t.reg .b8 c;\n\t"
@@ -44,7 +46,7 @@ __device__ __forceinline__ uint32_t encode2(float low, float high) {
       "cvt.u32.u8 %0, c;\n\t}"
       : "=r"(r)
       : "f"(low), "f"(high));
-  return r;
+  return (r | r << 12) & 0x000f000fu;
 }
 
 template <typename T>
@@ -75,13 +77,14 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const uint16_t* 
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const uint32_t e = top >> 23;  // floor(log2) + 127; 0 of a zero and of float32's subnormals (bf16 has them)
       const bool bad = e == 255u;
-      const uint32_t s = bad ? 255u : e < 2u ? 0u : e - 2u;  // E = floor(log2) - 2, at least -127
+      // E = floor(log2) - 2, at least -127; float16's blocks of zeros get the smallest scale that its other blocks have
+      constexpr uint32_t kLeast = std::is_same_v<T, __half> ? 101u : 0u;
+      const uint32_t s = bad ? 255u : e < kLeast + 2u ? kLeast : e - 2u;
       const float up = __uint_as_float((254u - (bad ? 127u : s)) << 23);  // 2^-E
       uint32_t code = 0;
       if (!bad) {
-        // element 2p at nibble p, element 2p + 1 at nibble p + 4
-        code = encode2(f[0] * up, f[2] * up) | encode2(f[4] * up, f[6] * up) << 8 | encode2(f[1] * up, f[3] * up) << 16 |
-               encode2(f[5] * up, f[7] * up) << 24;
+        code = Mx4<T>::word(encode2(f[0] * up, f[1] * up), encode2(f[2] * up, f[3] * up), encode2(f[4] * up, f[5] * up),
+                            encode2(f[6] * up, f[7] * up));
       }
       uint8_t* b = blocks + (c >> 1) * kMx4Block;
       *reinterpret_cast<uint32_t*>(b + mx4_code_at(r, c & 1) + j * 4) = code;
@@ -113,7 +116,10 @@ __global__ void __launch_bounds__(kThreads) mx4_dequantize_kernel(const uint8_t*
     for (int c = 0; c < 4; ++c) {
       const int k = span * 128 + c * 32 + j * 8;
       if (k >= K) continue;
-      const uint4 v = Mx4<T>::decode(code[c], Mx4<T>::scale(scale[c]));
+      const uint32_t one[1] = {code[c]};
+      uint4 v;
+      if (Mx4<T>::one_factor(scale[c], scale[c])) mx4_values<T, 1, true>(one, scale[c], &v);
+      else mx4_values<T, 1, false>(one, scale[c], &v);
       uint16_t* p = w + static_cast<int64_t>(n) * K + k;
       if (vec) {
         *reinterpret_cast<uint4*>(p) = v;

@@ -770,8 +770,8 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
 // eight warps instead of a copy, the 16-bit values in the layout that the copy would have left: 128 rows of 64 columns of K
 // for x V^T, for g V (kQMN) two panels of 64 columns by 64 rows.  The codes of a stage are two pieces that one more warp
 // copies into a ring of their own, kMx4Slots stages ahead.  (Loaded by the decoding warps themselves they were waited for
-// at every fence: 0.8 us a stage.)  A warp waits for the codes and for the stage to be free, stores the values and
-// reports to the even CTA's `full` barrier, whose phase also counts the P tiles' bytes; at CTA scope, since what the
+// at every fence: 0.8 us a stage.)  Two groups of four warps take the stages in turn, so that one decodes while the
+// other waits or stores.  A warp decodes its rows, waits for the stage to be free, stores the values and reports to the even CTA's `full` barrier, whose phase also counts the P tiles' bytes; at CTA scope, since what the
 // even CTA's MMAs read of the odd CTA lies in that one's shared memory and was fenced there (released at cluster scope,
 // every stage waited 0.8 us for the release).  LoRA stages are filled by copies alone; the warps report them unseen.
 constexpr int kMx4Warps = 8;
@@ -832,15 +832,18 @@ __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const Pa
                                                  const Mx4Ring& ring, volatile int* abort_flag) {
   const int w = (threadIdx.x >> 5) - kThreads / 32, lane = threadIdx.x & 31;
   const Tables& tb = prm.tb;
-  const int half = w >> 2;             // which 32 columns of a piece
+  const int group = w >> 2;
   const int row = (w & 3) * 32 + lane;  // of the stage: rows 0..63 of the first piece, then of the second
   uint8_t* dst = sB + row * 128;
-  int stage = 0, slot = 0;
+  int stage = 0, slot = 0, turn = 0;
   uint32_t phase = 0, slot_phase = 0;
   bool ok = true;
   auto report = [&]() {
     __syncwarp();
     if (lane == 0) mbar_arrive_cluster_cta(full_lead + static_cast<uint32_t>(stage * 8));
+  };
+  auto next_stage = [&]() {
+    turn ^= 1;
     if (++stage == kStages) {
       stage = 0;
       phase ^= 1;
@@ -849,17 +852,24 @@ __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const Pa
   for (int k = 0; k < n_units && ok; ++k) {
     const PairUnit un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
     for (int kb = un.kb0; kb < un.kb1; ++kb) {
-      ok = warp_wait_stage(&ring.full[slot], slot_phase, abort_flag, tb.err, kErrTimeoutFull);
-      if (!ok) break;
-      uint4 codes;
-      uint32_t scale;
-      mx4_fetch(ring.slots + slot * kMx4Block, row, half, codes, scale);
-      ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
-      if (!ok) break;
-      mx4_store<OutT>(dst + stage * kPairBBytes, row, half, codes, scale);
-      fence_proxy_async_smem();
-      report();
-      if (lane == 0) mbar_arrive(&ring.empty[slot]);  // every lane has its codes: they were stored
+      if (turn == group) {
+        ok = warp_wait_stage(&ring.full[slot], slot_phase, abort_flag, tb.err, kErrTimeoutFull);
+        if (!ok) break;
+        uint4 codes[2], v[8];
+        uint32_t scale[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) mx4_fetch(ring.slots + slot * kMx4Block, row, c, codes[c], scale[c]);
+        mx4_decode<OutT>(codes, scale, v);
+        ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
+        if (!ok) break;
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          *reinterpret_cast<uint4*>(dst + stage * kPairBBytes + ((g ^ (row & 7)) << 4)) = v[g];
+        fence_proxy_async_smem();
+        report();
+        if (lane == 0) mbar_arrive(&ring.empty[slot]);  // every lane has its codes: they were stored
+      }
+      next_stage();
       if (++slot == kMx4Slots) {
         slot = 0;
         slot_phase ^= 1;
@@ -868,8 +878,11 @@ __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const Pa
     if (!ok || !prm.lora || !un.last) continue;
     const int n_lora = (tb.pair_lora(un.mp + 1) - tb.pair_lora(un.mp)) * prm.s_planes;
     for (int j = 0; ok && j < n_lora; j += prm.lora_per_stage) {
-      ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
-      if (ok) report();
+      if (turn == group) {
+        ok = warp_wait_stage(&empty[stage], phase ^ 1, abort_flag, tb.err, kErrTimeoutEmpty);
+        if (ok) report();
+      }
+      next_stage();
     }
   }
 }
@@ -929,7 +942,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(&full[s], kMx4 ? 1 + 2 * kMx4Warps : 1);
+      mbar_init(&full[s], kMx4 ? 1 + kMx4Warps : 1);  // half of the warps of each CTA decode a stage
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -940,7 +953,7 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
     if (kMx4)
       for (int i = 0; i < kMx4Slots; ++i) {
         mbar_init(&codes.full[i], 1);
-        mbar_init(&codes.empty[i], kMx4Warps);
+        mbar_init(&codes.empty[i], kMx4Warps / 2);
       }
     mbar_init(drain, 1);
     *abort_flag = 0;
