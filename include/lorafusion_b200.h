@@ -577,12 +577,13 @@ LF_API int lf_mx4_linear(const lf_mx4_problem* prob, void* out_dev, void* worksp
 typedef struct lf_dropout {
   uint64_t seed, offset;
   const uint32_t* slot_threshold_dev; /* [n_slots] (virtual slots): 65536 times the rate, below 65536 */
-  void* scratch_dev;                  /* 16-byte aligned */
+  void* scratch_dev;                  /* 16-byte aligned; null where lf_dropout_scratch_bytes is 0 */
   size_t scratch_bytes;               /* at least lf_dropout_scratch_bytes */
 } lf_dropout;
 
-/* Scratch of dropout in lf_forward_opt (backward 0) or lf_backward_opt (1). */
-LF_API size_t lf_dropout_scratch_bytes(int32_t T, int32_t K, int32_t dtype, int32_t backward);
+/* Scratch of dropout in lf_forward_opt (backward 0: none on the tensor-core path) or lf_backward_opt (1), by the
+ * problem's sizes, dtype, x_dev and w_dev, where its other buffers are 16-byte aligned. */
+LF_API size_t lf_dropout_scratch_bytes(const lf_problem* prob, int32_t backward);
 
 typedef struct lf_options {
   int32_t weight_format;      /* of prob->w_dev: lf_weight_format; LF_WEIGHT_MX4 on the tensor-core path only */

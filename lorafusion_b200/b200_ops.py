@@ -442,7 +442,7 @@ class _Drop:
     def scales(self, scales):
         return tuple(s * (65536.0 / (65536 - t)) for s, t in zip(scales, self.thresholds))
 
-    def args(self, plan: _Plan, T: int, K: int, code: int, backward: bool, device):
+    def args(self, plan: _Plan, prob, backward: bool, device):
         """lf_dropout, and what it points at."""
         table = plan.thresholds.get(self.thresholds)
         if table is None:
@@ -450,9 +450,9 @@ class _Drop:
                 plan.thresholds.pop(next(iter(plan.thresholds)))
             host = torch.tensor([self.thresholds[i] for i, _, _ in plan.vslots] or [0], dtype=torch.int32)
             table = plan.thresholds[self.thresholds] = host.to(device)
-        scratch = torch.empty(max(int(nat.lib().lf_dropout_scratch_bytes(T, K, code, int(backward))), 16),
-                              dtype=torch.uint8, device=device)
-        return nat.Dropout(self.seed, self.offset, table.data_ptr(), scratch.data_ptr(), scratch.numel()), scratch
+        n = int(nat.lib().lf_dropout_scratch_bytes(ctypes.byref(prob), int(backward)))
+        scratch = torch.empty(n, dtype=torch.uint8, device=device) if n else None
+        return nat.Dropout(self.seed, self.offset, table.data_ptr(), scratch.data_ptr() if n else None, n), scratch
 
 
 # A float16 rank product s / (1 - p) x A^T must stay below 65504: factors beyond this one, which float16 training would
@@ -517,7 +517,7 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     prob = _problem(code, T, K, N, x, w, packs)
     stream = torch.cuda.current_stream(device).cuda_stream
     planes = ctypes.c_int32(0)
-    opt, keep = _options(mx4, drop, plan, T, K, code, False, device)
+    opt, keep = _options(mx4, drop, plan, prob, False, device)
     with nat.on_device(device.index):
         rc = L.lf_forward_opt(ctypes.byref(prob), info, plan.table_dev.data_ptr(), opt, y.data_ptr(), ws.data_ptr(),
                               ws.numel(), tail.data_ptr(), tail.numel(), ctypes.byref(planes), stream)
@@ -525,20 +525,20 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     # 2 K-half planes: shrink inside the GEMM launch (1 launch); 1: shrink launched on its own
     _last_launches = {2: 1, 1: 2}.get(planes.value) or int(L.lf_forward_launch_count(ctypes.byref(prob), info))
     if drop is not None:
-        _last_launches += 1
+        _last_launches += planes.value == 0  # the masked copy on CUDA cores
     elif planes.value > 0 and plan.info.n_segtiles > 0:
         _save_sf(x_in, rts, plan, aset, ws, planes.value)
     return y
 
 
-def _options(mx4: bool, drop: _Drop | None, plan: _Plan, T: int, K: int, code: int, backward: bool, device):
+def _options(mx4: bool, drop: _Drop | None, plan: _Plan, prob, backward: bool, device):
     """lf_options of a call (None for a plain one), and what must live until it is enqueued."""
     if not mx4 and drop is None:
         return None, None
     opt = nat.Options(nat.LF_WEIGHT_MX4 if mx4 else nat.LF_WEIGHT_DENSE, 0, None)
     keep = None
     if drop is not None:
-        args, keep = drop.args(plan, T, K, code, backward, device)
+        args, keep = drop.args(plan, prob, backward, device)
         opt.dropout = ctypes.pointer(args)
     return ctypes.byref(opt), (opt, keep)
 
@@ -684,7 +684,7 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
             pr.exchange[r] = ptr
         pr.slot_span_dev = ext.slot_span.data_ptr()
         pr.span_info_dev = ext.span_info.data_ptr()
-    opt, keep = _options(mx4, drop, plan, T, K, code, True, device)
+    opt, keep = _options(mx4, drop, plan, prob, True, device)
     with nat.on_device(device.index):
         rc = L.lf_backward_opt(ctypes.byref(prob), ctypes.byref(info), plan.table_dev.data_ptr(), opt, g.data_ptr(),
                                sf_ptr, sf_planes, _DTYPE_CODE[gdt], grad_x.data_ptr(), ga_flat.data_ptr(),

@@ -283,12 +283,13 @@ namespace {
 struct Options {
   bool mx4 = false;
   DropArgs drop{0, 0, nullptr};
-  char* scratch = nullptr;  // dropout's
+  char* scratch = nullptr;  // dropout's, and its size
+  size_t scratch_bytes = 0;
 };
 size_t drop_scratch_mask(const lf_problem* p) {
   return align256(static_cast<size_t>(p->T) * static_cast<size_t>(p->K) * static_cast<size_t>(elem_bytes(p->dtype)));
 }
-int read_options(const lf_options* opt, const lf_problem* prob, const lf_plan_info* info, bool backward, Options* out) {
+int read_options(const lf_options* opt, const lf_problem* prob, const lf_plan_info* info, Options* out) {
   if (!opt) return LF_OK;
   if (opt->weight_format != LF_WEIGHT_DENSE && opt->weight_format != LF_WEIGHT_MX4) return LF_ERR_INVALID_ARG;
   out->mx4 = opt->weight_format == LF_WEIGHT_MX4;
@@ -296,10 +297,10 @@ int read_options(const lf_options* opt, const lf_problem* prob, const lf_plan_in
   const lf_dropout* d = opt->dropout;
   if (!d || info->n_slots == 0 || info->n_segtiles == 0) return LF_OK;
   if (!d->slot_threshold_dev) return LF_ERR_INVALID_ARG;
-  if (!d->scratch_dev || !aligned16(d->scratch_dev)) return LF_ERR_INVALID_ARG;
-  if (d->scratch_bytes < lf_dropout_scratch_bytes(prob->T, prob->K, prob->dtype, backward ? 1 : 0)) return LF_ERR_CAPACITY;
+  if (!aligned16(d->scratch_dev)) return LF_ERR_INVALID_ARG;
   out->drop = DropArgs{d->seed, d->offset, d->slot_threshold_dev};
   out->scratch = static_cast<char*>(d->scratch_dev);
+  out->scratch_bytes = d->scratch_dev ? d->scratch_bytes : 0;
   return LF_OK;
 }
 // Launches hand results to one another inside a grid through flags that hold a number no earlier launch used.  A launch
@@ -329,7 +330,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
   int rc = check_problem(prob, info, table_dev);
   if (rc != LF_OK) return rc;
   Options opt;
-  rc = read_options(options, prob, info, false, &opt);
+  rc = read_options(options, prob, info, &opt);
   if (rc != LF_OK) return rc;
   if (stages <= 0 || stages > 31 || ((stages & LF_STAGE_EXPAND) && (stages & LF_STAGE_BASE))) return LF_ERR_INVALID_ARG;
   const int T = prob->T, K = prob->K, N = prob->N;
@@ -349,24 +350,18 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
   const bool lora = (stages & LF_STAGE_EXPAND) != 0 && info->n_segtiles > 0;
   const PairMx4 mx4 = opt.mx4 ? mx4_view(prob->w_dev, N, K) : PairMx4{};
   const PairMx4* mx4p = opt.mx4 ? &mx4 : nullptr;
-  const void* xa = prob->x_dev;  // the adapters' input
-  if (opt.drop.threshold && do_shrink) {
-    e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);
-    if (e != cudaSuccess) return LF_ERR_CUDA;
-    xa = opt.scratch;
-  }
+  const bool drop = opt.drop.threshold != nullptr;
 
   if (tc_eligible(prob, {prob->x_dev, prob->w_dev, prob->a_pack_dev, prob->b_pack_dev, y_dev, workspace_dev})) {
     const bool single = (stages & LF_STAGE_SINGLE_CTA) != 0;
     if (single && opt.mx4) return LF_ERR_UNSUPPORTED;
     const uint32_t nbox = single ? 256 : 128;  // rows of W / B_i per CTA and tile
     TcMaps maps;
-    CUtensorMap a_map, xa_map;
+    CUtensorMap a_map;
     const size_t es = 2;
     const uint64_t s_rows = kSextPlanes * static_cast<uint64_t>(info->n_segtiles + 1) * LF_TILE_ROWS;
     bool ok = make_map(&maps.p, dt, prob->x_dev, K, T, K * es, 64, 128) &&
               (opt.mx4 || make_map(&maps.q, dt, prob->w_dev, K, N, K * es, 64, nbox)) &&
-              make_map(&xa_map, dt, xa, K, T, K * es, 64, 128) &&
               make_map(&a_map, dt, prob->a_pack_dev, K, static_cast<uint64_t>(info->n_slots) * rp, K * es, 64, rp);
     if (info->n_segtiles > 0)
       ok = ok && make_map(&maps.s, dt, workspace_dev, rp, s_rows, rp * es, rp, 128) &&
@@ -379,7 +374,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
     // Shrink and expand requested together: run the shrink on CTA pairs the GEMM's round count
     // leaves idle, inside the same launch, when there are enough of them.
     const bool separate = (stages & LF_STAGE_SEPARATE) != 0;
-    const bool fuse = !single && !separate && do_shrink && lora && cosched_allowed(ds) && !opt.drop.threshold;
+    const bool fuse = !single && !separate && do_shrink && lora && cosched_allowed(ds) && !(drop && cosched_prologue());
     const int spare = fuse && !cosched_prologue() ? pair_spare_pairs(T, N, ds->num_sms, info->n_shrink_units) : 0;
     // the K-split tail needs a cooperative launch too
     const PairTail tail = tail_dev ? tail_scratch(tail_dev, tail_bytes, 0)
@@ -398,6 +393,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       sh.wait_gen = wait_generation(sh.gen);
       sh.n_pairs = spare;
       sh.prologue = cosched_prologue();
+      sh.drop = opt.drop;
       e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, &sh, &tail, nullptr, mx4p);
       if (e == cudaSuccess) {
         if (sf_planes) *sf_planes = 2;
@@ -408,7 +404,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       refuse_cosched(ds, e);
     }
     if (do_shrink) {
-      e = tc_shrink(dt, xa_map, a_map, K, tb, workspace_dev, ds->num_sms, st);
+      e = tc_shrink(dt, maps.p, a_map, K, tb, workspace_dev, ds->num_sms, st, &opt.drop);
       if (e != cudaSuccess) return LF_ERR_CUDA;
       if (sf_planes) *sf_planes = 1;
     }
@@ -428,8 +424,15 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
   }
 
   if (opt.mx4) return LF_ERR_UNSUPPORTED;
+  if (drop && do_shrink && opt.scratch_bytes < drop_scratch_mask(prob)) return LF_ERR_CAPACITY;
   double* s_ext = static_cast<double*>(workspace_dev);
   if (do_shrink) {
+    const void* xa = prob->x_dev;  // the adapters' input
+    if (drop) {
+      e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);
+      if (e != cudaSuccess) return LF_ERR_CUDA;
+      xa = opt.scratch;
+    }
     e = simt_shrink(dt, xa, K, K, prob->a_pack_dev, tb, s_ext, st);
     if (e != cudaSuccess) return LF_ERR_CUDA;
   }
@@ -455,13 +458,11 @@ extern "C" int lf_forward_sf(const lf_problem* prob, const lf_plan_info* info, c
                       LF_STAGE_SHRINK | LF_STAGE_EXPAND, stream, s_f_planes);
 }
 
-extern "C" size_t lf_dropout_scratch_bytes(int32_t T, int32_t K, int32_t dtype, int32_t backward) {
-  if (T < 0 || K < 0) return 0;
-  lf_problem p{};
-  p.T = T, p.K = K, p.dtype = dtype;
-  size_t n = drop_scratch_mask(&p);
-  if (backward && dtype != LF_F32) n += align256(static_cast<size_t>(T) * static_cast<size_t>(K) * 4);
-  return n;
+extern "C" size_t lf_dropout_scratch_bytes(const lf_problem* p, int32_t backward) {
+  if (!p || p->T < 0 || p->K < 0) return 0;
+  const bool tc = tc_eligible(p, {p->x_dev, p->w_dev});
+  if (!backward) return tc ? 0 : drop_scratch_mask(p);
+  return drop_scratch_mask(p) + (tc ? align256(static_cast<size_t>(p->T) * static_cast<size_t>(p->K) * 4) : 0);
 }
 
 extern "C" int lf_forward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
@@ -638,7 +639,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
   int rc = check_problem(prob, info, table_dev);
   if (rc != LF_OK) return rc;
   Options opt;
-  rc = read_options(options, prob, info, true, &opt);
+  rc = read_options(options, prob, info, &opt);
   if (rc != LF_OK) return rc;
   GramPeer gp{};
   if (peer != nullptr) {  // spanning adapters' blocks exchanged by the gram: tensor-core path only
@@ -702,6 +703,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
   const PairMx4 mx4 = opt.mx4 ? mx4_view(prob->w_dev, N, K) : PairMx4{};
   const PairMx4* mx4p = opt.mx4 ? &mx4 : nullptr;
   const bool drop = opt.drop.threshold != nullptr;
+  if (drop && opt.scratch_bytes < lf_dropout_scratch_bytes(prob, 1)) return LF_ERR_CAPACITY;
   const void* xa = prob->x_dev;  // the adapters' input
   if (drop && (do_gab || (do_shrink && !reuse_sf))) {
     e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);

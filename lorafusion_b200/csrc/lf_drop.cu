@@ -32,8 +32,8 @@ __global__ void __launch_bounds__(kThreads) drop_mask_kernel(const uint8_t* __re
     if (vec) {  // rows of whole 16-byte pieces
       if (kB == 2) {
         uint4 v = reinterpret_cast<const uint4*>(xr)[g];
-        v.x &= keep2(r.x, threshold), v.y &= keep2(r.y, threshold), v.z &= keep2(r.z, threshold),
-            v.w &= keep2(r.w, threshold);
+        const uint32_t high = threshold << 16;
+        v.x = keep2(v.x, r.x, high), v.y = keep2(v.y, r.y, high), v.z = keep2(v.z, r.z, high), v.w = keep2(v.w, r.w, high);
         reinterpret_cast<uint4*>(o)[g] = v;
       } else {
 #pragma unroll

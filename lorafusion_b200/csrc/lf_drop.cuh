@@ -13,25 +13,40 @@
 
 namespace lf {
 
-__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint64_t offset, uint64_t seed) {
-  uint32_t c2 = static_cast<uint32_t>(offset), c3 = static_cast<uint32_t>(offset >> 32);
+// Numbers of N counters (c0[i], c1), round by round: 76 cycles of an SM quarter's issue a counter and warp, 97 where one
+// counter's ten dependent rounds are all a warp has to do.
+template <int N>
+__device__ __forceinline__ void philox(const uint32_t (&c0)[N], uint32_t c1, uint64_t offset, uint64_t seed, uint4 (&r)[N]) {
   uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
 #pragma unroll
+  for (int j = 0; j < N; ++j)
+    r[j] = make_uint4(c0[j], c1, static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32));
+#pragma unroll
   for (int i = 0; i < 10; ++i) {
-    const uint64_t a = static_cast<uint64_t>(c0) * 0xD2511F53u, b = static_cast<uint64_t>(c2) * 0xCD9E8D57u;
-    c0 = static_cast<uint32_t>(b >> 32) ^ c1 ^ k0;
-    c1 = static_cast<uint32_t>(b);
-    c2 = static_cast<uint32_t>(a >> 32) ^ c3 ^ k1;
-    c3 = static_cast<uint32_t>(a);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const uint64_t a = static_cast<uint64_t>(r[j].x) * 0xD2511F53u, b = static_cast<uint64_t>(r[j].z) * 0xCD9E8D57u;
+      r[j] = make_uint4(static_cast<uint32_t>(b >> 32) ^ r[j].y ^ k0, static_cast<uint32_t>(b),
+                        static_cast<uint32_t>(a >> 32) ^ r[j].w ^ k1, static_cast<uint32_t>(a));
+    }
     k0 += 0x9E3779B9u;
     k1 += 0xBB67AE85u;
   }
-  return make_uint4(c0, c1, c2, c3);
+}
+__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint64_t offset, uint64_t seed) {
+  const uint32_t c[1] = {c0};
+  uint4 r[1];
+  philox<1>(c, c1, offset, seed, r);
+  return r[0];
 }
 
-// All ones in each 16-bit half of `word` whose number keeps its element.  `threshold` is below 65536.
-__device__ __forceinline__ uint32_t keep2(uint32_t word, uint32_t threshold) {
-  return ((word & 0xffffu) >= threshold ? 0x0000ffffu : 0u) | ((word >> 16) >= threshold ? 0xffff0000u : 0u);
+// Two 16-bit elements, zeros where the word's halves drop them; `high` is the threshold (below 65536) shifted left by 16.
+// The upper number is below the threshold where the whole word is below `high`.  (Built as a mask of compares and
+// selects it took half as long as the generator itself.)
+__device__ __forceinline__ uint32_t keep2(uint32_t v, uint32_t word, uint32_t high) {
+  if (word < high) v &= 0x0000ffffu;
+  if ((word << 16) < high) v &= 0xffff0000u;
+  return v;
 }
 
 // Threshold of row `row` of tile `tile`: that of the segment that holds the row (several where the adapter has more than
@@ -41,6 +56,26 @@ __device__ __forceinline__ uint32_t row_threshold(const Tables& tb, const DropAr
   for (int st = tb.tile_st(tile); st < e; ++st)
     if (row >= tb.st_lo(st) && row < tb.st_hi(st)) return d.threshold[tb.st_slot(st)];
   return 0;
+}
+
+// Half `half` (32 of 64 columns) of row `row` of an x tile in shared memory (128 rows of 128 bytes, 128-byte swizzle),
+// K block kb, masked in place.  `t` is the row's number in the batch, `high` as in keep2.
+__device__ __forceinline__ void mask_half_row(uint8_t* tile, int row, int half, int kb, uint32_t t, uint32_t high,
+                                              const DropArgs& d) {
+  uint32_t c[4];
+  uint4 r[4], v[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    c[j] = static_cast<uint32_t>(kb * 8 + 4 * half + j);
+    v[j] = *reinterpret_cast<const uint4*>(tile + row * 128 + (((4 * half + j) ^ (row & 7)) << 4));
+  }
+  philox<4>(c, t, d.offset, d.seed, r);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    v[j].x = keep2(v[j].x, r[j].x, high), v[j].y = keep2(v[j].y, r[j].y, high);
+    v[j].z = keep2(v[j].z, r[j].z, high), v[j].w = keep2(v[j].w, r[j].w, high);
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((4 * half + j) ^ (row & 7)) << 4)) = v[j];
+  }
 }
 
 }  // namespace lf

@@ -17,6 +17,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include "lf_drop.cuh"
 #include "lf_internal.cuh"
 #include "lf_launch.cuh"
 #include "lf_mx4.cuh"
@@ -441,6 +442,7 @@ struct PairParams {
   void* s_ext2;
   PairDelta delta;  // kDelta kernels
   PairMx4 mx4;      // kMx4 kernels
+  DropArgs drop;    // kDrop kernels: of the co-scheduled shrink's input
   Tables tb;
 };
 
@@ -534,12 +536,15 @@ __device__ __forceinline__ bool wait_units_ready(const uint64_t* ready, int u0, 
 // flag is released.  The epilogue warps of CTA 0
 // also write the all-zero block before releasing item 0.  In prologue mode the role keeps the
 // TMEM allocation permit (the GEMM allocates after it) and its barriers are its own.
-template <typename OutT, bool kPrologue>
+// kDrop: eight more warps mask each x tile between its copy and its MMAs (rmasked).
+constexpr int kMaskWarps = 8;
+template <typename OutT, bool kPrologue, bool kDrop>
 __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CUtensorMap& map_p,
                                                  const CUtensorMap& map_a, const CUtensorMap& map_p2,
                                                  const CUtensorMap& map_a2, uint8_t* sA, uint8_t* sB, uint64_t* full,
                                                  uint64_t* empty, uint64_t* tfull, uint64_t* tempty, uint64_t* drain,
-                                                 uint64_t* pub, uint32_t* tmem_slot, volatile int* abort_flag) {
+                                                 uint64_t* pub, uint64_t* masked, uint32_t* tmem_slot,
+                                                 volatile int* abort_flag) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Tables& tb = prm.tb;
   const int me = static_cast<int>(blockIdx.x), n_me = kPrologue ? static_cast<int>(gridDim.x) : 2 * prm.n_shrink_pairs;
@@ -552,6 +557,7 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
     for (int s = 0; s < kRoleStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      if (kDrop) mbar_init(&masked[s], kMaskWarps);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&tfull[b], 1);
@@ -645,6 +651,10 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
         int step = 0;
         const int kb_end = min(nkb, (h + 1) * nkb_half);
         for (int kb = h * nkb_half; kb < kb_end; ++kb) {
+          if (kDrop && !mbar_wait_stage(&masked[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) {
+            ok = false;
+            break;
+          }
           if (!mbar_wait(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) {
             ok = false;
             break;
@@ -674,7 +684,37 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
       }
     }
     __syncwarp();
-  } else if (warp < kThreads / 32) {  // the decoding warps of a kMx4 kernel have no part in it
+  } else if (kDrop && warp >= kThreads / 32 && warp < kThreads / 32 + kMaskWarps) {
+    const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, half = w >> 2;
+    int stage = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (int item = me; item < n_items && ok; item += n_me) {
+      const int u = item >> 1, h = item & 1;
+      const int nkb = job_nkb(0), nkb_half = (nkb + 1) / 2;
+      const int tile = tb.unit_tile(u), st0 = tb.unit_st0(u), nst = tb.unit_nst(u);
+      uint32_t threshold = 0;
+      for (int q = 0; q < nst; ++q)
+        if (row >= tb.st_lo(st0 + q) && row < tb.st_hi(st0 + q)) threshold = prm.drop.threshold[tb.st_slot(st0 + q)];
+      const bool any = __any_sync(0xffffffffu, threshold != 0);
+      const int kb_end = min(nkb, (h + 1) * nkb_half);
+      for (int kb = h * nkb_half; kb < kb_end; ++kb) {
+        ok = warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull);
+        if (!ok) break;
+        if (any) {
+          mask_half_row(sA + stage * kRoleStageBytes, row, half, kb, static_cast<uint32_t>(tile * kBM + row), threshold << 16,
+                        prm.drop);
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&masked[stage]);
+        if (++stage == kRoleStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+    }
+  } else if (warp < kThreads / 32) {  // the extra warps of other kernels have no part in it
     const int q = warp & 3;
     const int row = q * 32 + lane;
     OutT* s_ext = reinterpret_cast<OutT*>(prm.s_ext);
@@ -889,8 +929,12 @@ __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const Pa
 
 // kDelta: a float32 matrix is added to the product (prm.delta).
 // kMx4: Q is held in 4 bits (prm.mx4) and decoded on the way into shared memory; map_q is not used.
-template <bool kQMN, typename OutT, bool kDelta, bool kMx4>
-__global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
+// kDrop: the co-scheduled shrink's input is masked (prm.drop), by warps that a kMx4 kernel has and others get for it.
+__host__ __device__ constexpr int pair_threads(bool mx4, bool drop) {
+  return mx4 ? kMx4Threads : kThreads + (drop ? 32 * kMaskWarps : 0);
+}
+template <bool kQMN, typename OutT, bool kDelta, bool kMx4, bool kDrop>
+__global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
     tc_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_l,
                         const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_a,
@@ -925,13 +969,13 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) < 2 * prm.n_shrink_pairs) {
-    pair_shrink_role<OutT, false>(prm, map_p, map_a, map_p2, map_a2, sA, sB, full, empty, tfull, tempty, drain, pub,
-                                  tmem_slot, abort_flag);
+    pair_shrink_role<OutT, false, kDrop>(prm, map_p, map_a, map_p2, map_a2, sA, sB, full, empty, tfull, tempty, drain, pub,
+                                         rfull, tmem_slot, abort_flag);
     return;
   }
-  if (prm.shrink_prologue && static_cast<int>(blockIdx.x) < (prm.job2 ? 4 : 2) * prm.tb.n_units)
-    pair_shrink_role<OutT, true>(prm, map_p, map_a, map_p2, map_a2, sA, sB, rfull, rempty, rtfull, rtempty, rdrain,
-                                 rpub, tmem_slot, abort_flag);
+  if (!kDrop && prm.shrink_prologue && static_cast<int>(blockIdx.x) < (prm.job2 ? 4 : 2) * prm.tb.n_units)
+    pair_shrink_role<OutT, true, false>(prm, map_p, map_a, map_p2, map_a2, sA, sB, rfull, rempty, rtfull, rtempty, rdrain,
+                                        rpub, nullptr, tmem_slot, abort_flag);
   const uint32_t crank = cluster_ctarank();  // 0: issues the MMAs
   const int pair = static_cast<int>(blockIdx.x >> 1) - prm.n_shrink_pairs;
   const int n_pairs = static_cast<int>(gridDim.x >> 1) - prm.n_shrink_pairs;
@@ -1186,6 +1230,8 @@ __global__ void __launch_bounds__(kMx4 ? kMx4Threads : kThreads, 1)
       }
     }
     __syncwarp();
+  } else if (!kMx4 && kDrop && warp >= kThreads / 32) {
+    // nothing to mask in a GEMM pair
   } else if (kMx4 && warp >= kThreads / 32) {
     if (warp == kMx4Threads / 32 - 1)
       pair_codes_role<kQMN>(prm, sched, pair, n_pairs, n_units, nkb, static_cast<int>(crank), codes, abort_flag);
@@ -1382,6 +1428,7 @@ struct ShrinkParams {
   int cluster;
   int r_pad;
   Tables tb;
+  DropArgs drop;  // kDrop kernels
 };
 
 constexpr int kShrABytes = kBM * kBK * 2;    // 16 KB
@@ -1391,8 +1438,9 @@ constexpr int kPartLd = kBM + 1;             // column-major partial sums, odd s
 constexpr int kMaxShrCluster = 4;             // K split across at most 4 CTAs (all resident at once)
 static_assert(64 * kPartLd * 4 <= kShrStages * (kShrABytes + kShrBBytes), "partials must fit the stage area");
 
-template <typename OutT>
-__global__ void __launch_bounds__(kThreads, 1)
+// kDrop: eight more warps mask each tile of P between its copy and its MMAs.
+template <typename OutT, bool kDrop>
+__global__ void __launch_bounds__(kThreads + (kDrop ? 32 * kMaskWarps : 0), 1)
     tc_shrink_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_a,
                      const ShrinkParams prm) {
   extern __shared__ uint8_t smem_raw[];
@@ -1409,6 +1457,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int* seg_lo = reinterpret_cast<int*>(tmem_slot + 2);  // per segment tile of the unit (<= 4)
   int* seg_hi = seg_lo + 8;
   float* seg_scale = reinterpret_cast<float*>(seg_hi + 8);
+  __shared__ uint64_t masked[kDrop ? kShrStages : 1];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Tables& tb = prm.tb;
@@ -1426,6 +1475,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int s = 0; s < kShrStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
+      if (kDrop) mbar_init(&masked[s], kMaskWarps);
     }
     mbar_init(tfull, 1);
     mbar_init(drain, 1);
@@ -1492,7 +1542,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t started = 0;  // accumulation chains holding a partial sum
       int step = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[stage], phase, abort_flag, prm.tb.err, kErrTimeoutFull)) {
+        if ((kDrop && !mbar_wait_stage(&masked[stage], phase, abort_flag, prm.tb.err, kErrTimeoutFull)) ||
+            !mbar_wait(&full[stage], phase, abort_flag, prm.tb.err, kErrTimeoutFull)) {
           ok = false;
           break;
         }
@@ -1520,6 +1571,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
     __syncwarp();
+  } else if (kDrop && warp >= kThreads / 32) {
+    const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, half = w >> 2;
+    uint32_t threshold = 0;
+    for (int q = 0; q < nst; ++q)
+      if (row >= seg_lo[q] && row < seg_hi[q]) threshold = prm.drop.threshold[tb.st_slot(st0 + q)];
+    const bool any = __any_sync(0xffffffffu, threshold != 0);
+    int stage = 0;
+    uint32_t phase = 0;
+    for (int kb = kb0; kb < kb1; ++kb) {
+      if (!warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) break;
+      if (any) {
+        mask_half_row(sA + stage * kShrABytes, row, half, kb, static_cast<uint32_t>(tile * kBM + row), threshold << 16,
+                      prm.drop);
+        fence_proxy_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&masked[stage]);
+      if (++stage == kShrStages) {
+        stage = 0;
+        phase ^= 1;
+      }
+    }
   } else {
     const int q = warp & 3;
     const int row = q * 32 + lane;
@@ -1558,7 +1631,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int total = rows_per * N;
     const uint32_t part_base = smem_u32(partial);
     OutT* out = reinterpret_cast<OutT*>(prm.s_ext);
-    for (int e = threadIdx.x; e < total; e += kThreads) {
+    for (int e = threadIdx.x; e < total; e += blockDim.x) {
       const int row = r0 + e / N, col = e % N;
       const uint32_t off = static_cast<uint32_t>((col * kPartLd + row) * 4);
       float part[kMaxShrCluster];
@@ -1582,7 +1655,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (blockIdx.x == 0) {  // the all-zero segment tile the pair GEMM pads odd row tiles with
     OutT* zero = reinterpret_cast<OutT*>(prm.s_ext) + static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad;
-    for (int e = threadIdx.x; e < kBM * r_pad; e += kThreads) zero[e] = cvt_out<OutT>(0.f);
+    for (int e = threadIdx.x; e < kBM * r_pad; e += blockDim.x) zero[e] = cvt_out<OutT>(0.f);
   }
 
   // keep this CTA's shared memory alive until every peer has read it
@@ -2430,7 +2503,12 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * (gemm_pairs + p.n_shrink_pairs));
-  cfg.blockDim = dim3(mx4 != nullptr ? kMx4Threads : kThreads);
+  const bool drop = shrink != nullptr && shrink->drop.threshold != nullptr;
+  if (drop) {
+    if (q_mn_major || delta != nullptr || shrink->prologue || shrink->job2) return cudaErrorInvalidValue;
+    p.drop = shrink->drop;
+  }
+  cfg.blockDim = dim3(pair_threads(mx4 != nullptr, drop));
   cfg.dynamicSmemBytes = mx4 != nullptr ? kMx4PairSmem : kPairSmem;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -2445,22 +2523,22 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cfg.attrs = attr;
   cfg.numAttrs = p.n_shrink_pairs > 0 || p.shrink_prologue || p.tail_parts > 1 ? 2 : 1;
   cudaError_t e;
-#define LF_LAUNCH_PAIR(QMN, OT, DELTA, MX4)                                                                         \
-  {                                                                                                                  \
-    e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, MX4 ? kMx4PairSmem : kPairSmem);                       \
-    if (e != cudaSuccess) return e;                                                                                  \
-    e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT, DELTA, MX4>, maps.p, maps.q, maps.s, maps.l, maps.o,   \
-                           *a_map, *p2_map, *a2_map, p);                                                             \
+#define LF_LAUNCH_PAIR(QMN, OT, DELTA, MX4, DROP)                                                                        \
+  {                                                                                                                      \
+    e = ensure_smem(tc_gemm_pair_kernel<QMN, OT, DELTA, MX4, DROP>, MX4 ? kMx4PairSmem : kPairSmem);                     \
+    if (e != cudaSuccess) return e;                                                                                      \
+    e = cudaLaunchKernelEx(&cfg, tc_gemm_pair_kernel<QMN, OT, DELTA, MX4, DROP>, maps.p, maps.q, maps.s, maps.l, maps.o, \
+                           *a_map, *p2_map, *a2_map, p);                                                                 \
   }
-#define LF_LAUNCH_PAIR_TYPES(DELTA, MX4)                            \
-  {                                                                 \
-    if (dtype == LF_BF16) {                                         \
-      if (q_mn_major) LF_LAUNCH_PAIR(true, __nv_bfloat16, DELTA, MX4) \
-      else LF_LAUNCH_PAIR(false, __nv_bfloat16, DELTA, MX4)         \
-    } else {                                                        \
-      if (q_mn_major) LF_LAUNCH_PAIR(true, __half, DELTA, MX4)      \
-      else LF_LAUNCH_PAIR(false, __half, DELTA, MX4)                \
-    }                                                               \
+#define LF_LAUNCH_PAIR_TYPES(DELTA, MX4)                                       \
+  {                                                                            \
+    if (dtype == LF_BF16) {                                                    \
+      if (q_mn_major) LF_LAUNCH_PAIR(true, __nv_bfloat16, DELTA, MX4, false)   \
+      else LF_LAUNCH_PAIR(false, __nv_bfloat16, DELTA, MX4, false)             \
+    } else {                                                                   \
+      if (q_mn_major) LF_LAUNCH_PAIR(true, __half, DELTA, MX4, false)          \
+      else LF_LAUNCH_PAIR(false, __half, DELTA, MX4, false)                    \
+    }                                                                          \
   }
   if (delta != nullptr) {
     if (shrink != nullptr || tail != nullptr) return cudaErrorInvalidValue;
@@ -2472,7 +2550,15 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
     else LF_LAUNCH_PAIR_TYPES(true, false)
     return e;
   }
-  if (mx4 != nullptr) LF_LAUNCH_PAIR_TYPES(false, true)
+  if (drop) {
+    if (dtype == LF_BF16) {
+      if (mx4 != nullptr) LF_LAUNCH_PAIR(false, __nv_bfloat16, false, true, true)
+      else LF_LAUNCH_PAIR(false, __nv_bfloat16, false, false, true)
+    } else {
+      if (mx4 != nullptr) LF_LAUNCH_PAIR(false, __half, false, true, true)
+      else LF_LAUNCH_PAIR(false, __half, false, false, true)
+    }
+  } else if (mx4 != nullptr) LF_LAUNCH_PAIR_TYPES(false, true)
   else LF_LAUNCH_PAIR_TYPES(false, false)
 #undef LF_LAUNCH_PAIR_TYPES
 #undef LF_LAUNCH_PAIR
@@ -2481,7 +2567,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
 }
 
 cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_map, int Kred, const Tables& tb,
-                      void* s_ext, int num_sms, cudaStream_t st) {
+                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop) {
   if (tb.n_units == 0) return cudaSuccess;
   const int nkb = (Kred + kBK - 1) / kBK;
   // split K across a cluster while every CTA still fits on the GPU at once (one per SM)
@@ -2510,14 +2596,16 @@ cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   cudaError_t e;
-  if (dtype == LF_BF16) {
-    e = ensure_smem(tc_shrink_kernel<__nv_bfloat16>, kShrSmem);
-    if (e != cudaSuccess) return e;
-    e = cudaLaunchKernelEx(&cfg, tc_shrink_kernel<__nv_bfloat16>, p_map, a_map, p);
+  auto start = [&](auto* kernel) {
+    e = ensure_smem(kernel, kShrSmem);
+    return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p_map, a_map, p) : e;
+  };
+  if (drop != nullptr && drop->threshold != nullptr) {
+    p.drop = *drop;
+    cfg.blockDim = dim3(kThreads + 32 * kMaskWarps);
+    e = dtype == LF_BF16 ? start(tc_shrink_kernel<__nv_bfloat16, true>) : start(tc_shrink_kernel<__half, true>);
   } else {
-    e = ensure_smem(tc_shrink_kernel<__half>, kShrSmem);
-    if (e != cudaSuccess) return e;
-    e = cudaLaunchKernelEx(&cfg, tc_shrink_kernel<__half>, p_map, a_map, p);
+    e = dtype == LF_BF16 ? start(tc_shrink_kernel<__nv_bfloat16, false>) : start(tc_shrink_kernel<__half, false>);
   }
   if (e != cudaSuccess) return e;
   return cudaGetLastError();

@@ -1,8 +1,8 @@
 """Dropout in front of the adapters, its mask never stored: forward, backward and refusals against 64-bit arithmetic.
 
 Tolerances.  A result is off by at most half a step of its type, plus: ``n 2^-24`` of the sum of magnitudes for a float32
-sum of n products; the rank product S, which the forward on tensor cores rounds to the type (half a step) and the
-backward keeps to 2^-15 (two 16-bit halves; the lower of float16 no finer than 2^-25); in float32 everything is summed in
+sum of n products; the rank product S, which the forward on tensor cores rounds to the type (half a step, of S or of its
+two halves along K, which share out the reduction) and the backward keeps to 2^-15 (two 16-bit halves; the lower of float16 no finer than 2^-25); in float32 everything is summed in
 64 bits and only the factor s / (1 - p) and the result are rounded.
 """
 
@@ -80,7 +80,10 @@ class Problem:
             else:
                 eS = 2.0 ** -15 * S.abs() + self.K * one * mS + 2.0 ** -24
                 eG = 2.0 ** -15 * G.abs() + self.N * one * mG + 2.0 ** -24
-                fwd = half * S.abs() + self.K * one * mS + torch.finfo(self.dtype).smallest_normal
+                # the forward takes S as one rounded number, or as two, of the halves of K (in blocks of 64)
+                k = (-(-self.K // 64) + 1) // 2 * 64
+                S0, S1 = f * xm[s, :k] @ a[:, :k].t(), f * xm[s, k:] @ a[:, k:].t()
+                fwd = half * (S0.abs() + S1.abs()) + self.K * one * mS + torch.finfo(self.dtype).smallest_normal
                 n = (a.shape[0] + self.T) * one
             y[s] += S @ b.t()
             by[s] += fwd @ b.abs().t() + n * (S.abs() @ b.abs().t())

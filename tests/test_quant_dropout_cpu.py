@@ -98,15 +98,18 @@ def test_the_library_refuses_before_any_launch():
         return L.lf_forward_opt(prob, info, 256, opt, 256, 256, 1 << 40, None, 0, None, None)
 
     assert forward(nat.Options(5, 0, None)) == bad
-    assert forward(nat.Options(0, 0, ctypes.pointer(drop))) == nat.LF_ERR_CAPACITY
-    drop.scratch_bytes, drop.slot_threshold_dev = 1 << 40, None
+    drop.slot_threshold_dev = None
     assert forward(nat.Options(0, 0, ctypes.pointer(drop))) == bad
     drop.slot_threshold_dev, drop.scratch_dev = 256, 8
     assert forward(nat.Options(0, 0, ctypes.pointer(drop))) == bad
     prob.dtype = nat.LF_F32
     assert forward(nat.Options(nat.LF_WEIGHT_MX4, 0, None)) == nat.LF_ERR_UNSUPPORTED
-    assert L.lf_dropout_scratch_bytes(-1, 8, 0, 0) == 0
-    assert L.lf_dropout_scratch_bytes(128, 64, nat.LF_BF16, 1) == 128 * 64 * 6
-    assert L.lf_dropout_scratch_bytes(128, 64, nat.LF_F32, 1) == 128 * 64 * 4
+    def scratch(dtype, K, backward):
+        return L.lf_dropout_scratch_bytes(nat.Problem(dtype, 128, K, 64, 256, 256), backward)
+
+    assert L.lf_dropout_scratch_bytes(None, 0) == 0
+    assert scratch(nat.LF_BF16, 64, 0) == 0 and scratch(nat.LF_BF16, 64, 1) == 128 * 64 * 6
+    assert scratch(nat.LF_F32, 64, 0) == 128 * 64 * 4 == scratch(nat.LF_F32, 64, 1)
+    assert scratch(nat.LF_BF16, 60, 0) == 128 * 60 * 2 == scratch(nat.LF_BF16, 60, 1)
     rows = nat.RowsProblem(dtype=nat.LF_BF16, T=1, K=64, N=64, n_slots=0, r_pad=16, row_slot_bytes=4, weight_format=2)
     assert L.lf_rows_forward(rows, 256, 256, 0, None) == bad
