@@ -695,7 +695,8 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     n_launch = max(0, int(L.lf_backward_launch_count(ctypes.byref(prob), ctypes.byref(info))))
     _last_launches = n_launch - 1 if saved is not None and n_launch == 4 else n_launch
     if drop is not None:
-        _last_launches = 6  # mask, two shrinks, expand, grad_x, dA and dB; on CUDA cores mask, two, grad_x, two
+        # S_b, (S_f,) expand, grad_x (with S_f), dA and dB; on CUDA cores mask, S_f, S_b, grad_x, dA, dB
+        _last_launches = {2: 4, 4: 5}.get(n_launch, 6)
     grad_a, grad_b = _grad_dicts(plan, ga_flat, gb_flat, K, N)
     if ext is not None:  # spanning adapters not held here: their summed blocks after the local ones
         for aid, parts in ext.nonheld.items():

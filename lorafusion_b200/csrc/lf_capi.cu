@@ -704,12 +704,8 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
   const PairMx4* mx4p = opt.mx4 ? &mx4 : nullptr;
   const bool drop = opt.drop.threshold != nullptr;
   if (drop && opt.scratch_bytes < lf_dropout_scratch_bytes(prob, 1)) return LF_ERR_CAPACITY;
-  const void* xa = prob->x_dev;  // the adapters' input
-  if (drop && (do_gab || (do_shrink && !reuse_sf))) {
-    e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);
-    if (e != cudaSuccess) return LF_ERR_CUDA;
-    xa = opt.scratch;
-  }
+  if (drop && (staged || reuse_sf)) return LF_ERR_UNSUPPORTED;
+  const void* xa = drop ? opt.scratch : prob->x_dev;  // the adapters' input: m x is written on the way
   if (tc_path) {
     CUtensorMap p_x, p_g, a_map, bt_map, sf_map, sb_map;
     TcMaps dx;
@@ -778,6 +774,31 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
           refuse_cosched(ds, e);  // cooperative launch refused: nothing ran
         }
       }
+      if (!gemm_done && drop) {
+        // the mask is of grad_x's adapters' part alone: it is added to g W.  S_f and m x, which dA and dB read, are computed
+        // on CTA pairs that this GEMM's rounds leave idle, or ahead of it.
+        CUtensorMap x_map;
+        float* delta = reinterpret_cast<float*>(opt.scratch + drop_scratch_mask(prob));
+        const PairDelta d{delta, nullptr, K};
+        if (!make_map(&x_map, dt, prob->x_dev, K, T, K * es, 64, 128)) return LF_ERR_UNSUPPORTED;
+        e = tc_shrink(dt, p_g, bt_map, N, tb, s_b, ds->num_sms, st);
+        PairShrink sh{};
+        sh.n_pairs = spare;
+        sh.job2 = sh.job2_only = true;
+        sh.p2_map = x_map;
+        sh.a2_map = a_map;
+        sh.a_map = p_x;
+        sh.s_ext2 = s_f;
+        sh.K2 = K;
+        sh.drop = opt.drop;
+        if (e == cudaSuccess && spare == 0) e = tc_shrink(dt, x_map, a_map, K, tb, s_f, ds->num_sms, st, &opt.drop, &p_x);
+        if (e == cudaSuccess) e = drop_expand(dt, s_b, prob->at_pack_dev, T, K, tb, opt.drop, delta, st);
+        if (e == cudaSuccess)
+          e = tc_gemm_pair(dt, true, dx, T, K, N, false, tb, grad_x_dev, K, ds->num_sms, st, spare > 0 ? &sh : nullptr, nullptr,
+                           &d, mx4p);
+        if (e != cudaSuccess) return LF_ERR_CUDA;
+        gemm_done = true;
+      }
       if (!gemm_done) {
         if (!reuse_sf) {
           e = tc_shrink(dt, p_x, a_map, K, tb, s_f, ds->num_sms, st);
@@ -788,15 +809,6 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
       }
     } else {
       dx.s = dx.l = p_g;
-    }
-    if (!gemm_done && drop) {  // the mask is of grad_x's adapters' part alone: it is added to g W
-      float* delta = reinterpret_cast<float*>(opt.scratch + drop_scratch_mask(prob));
-      const PairDelta d{delta, nullptr, K};
-      e = drop_expand(dt, s_b, prob->at_pack_dev, T, K, tb, opt.drop, delta, st);
-      if (e == cudaSuccess)
-        e = tc_gemm_pair(dt, true, dx, T, K, N, false, tb, grad_x_dev, K, ds->num_sms, st, nullptr, nullptr, &d, mx4p);
-      if (e != cudaSuccess) return LF_ERR_CUDA;
-      gemm_done = true;
     }
     if (!gemm_done) {
       e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, nullptr,
@@ -836,6 +848,10 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
     return LF_OK;
   }
 
+  if (drop) {
+    e = drop_mask(dt, prob->x_dev, T, K, tb, opt.drop, opt.scratch, st);
+    if (e != cudaSuccess) return LF_ERR_CUDA;
+  }
   double* sf = reinterpret_cast<double*>(ws);  // the CUDA-core path computes its own f64 S_f
   double* sbp = static_cast<double*>(s_b);
   if (do_shrink) {

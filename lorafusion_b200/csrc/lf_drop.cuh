@@ -58,23 +58,24 @@ __device__ __forceinline__ uint32_t row_threshold(const Tables& tb, const DropAr
   return 0;
 }
 
-// Half `half` (32 of 64 columns) of row `row` of an x tile in shared memory (128 rows of 128 bytes, 128-byte swizzle),
-// K block kb, masked in place.  `t` is the row's number in the batch, `high` as in keep2.
-__device__ __forceinline__ void mask_half_row(uint8_t* tile, int row, int half, int kb, uint32_t t, uint32_t high,
+// N granules of eight elements, first .. first + N - 1 of the eight of row `row` of an x tile in shared memory (128 rows of
+// 128 bytes, 128-byte swizzle), K block kb, masked in place.  `t` is the row's number in the batch, `high` as in keep2.
+template <int N>
+__device__ __forceinline__ void mask_granules(uint8_t* tile, int row, int first, int kb, uint32_t t, uint32_t high,
                                               const DropArgs& d) {
-  uint32_t c[4];
-  uint4 r[4], v[4];
+  uint32_t c[N];
+  uint4 r[N], v[N];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    c[j] = static_cast<uint32_t>(kb * 8 + 4 * half + j);
-    v[j] = *reinterpret_cast<const uint4*>(tile + row * 128 + (((4 * half + j) ^ (row & 7)) << 4));
+  for (int j = 0; j < N; ++j) {
+    c[j] = static_cast<uint32_t>(kb * 8 + first + j);
+    v[j] = *reinterpret_cast<const uint4*>(tile + row * 128 + (((first + j) ^ (row & 7)) << 4));
   }
-  philox<4>(c, t, d.offset, d.seed, r);
+  philox<N>(c, t, d.offset, d.seed, r);
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
+  for (int j = 0; j < N; ++j) {
     v[j].x = keep2(v[j].x, r[j].x, high), v[j].y = keep2(v[j].y, r[j].y, high);
     v[j].z = keep2(v[j].z, r[j].z, high), v[j].w = keep2(v[j].w, r[j].w, high);
-    *reinterpret_cast<uint4*>(tile + row * 128 + (((4 * half + j) ^ (row & 7)) << 4)) = v[j];
+    *reinterpret_cast<uint4*>(tile + row * 128 + (((first + j) ^ (row & 7)) << 4)) = v[j];
   }
 }
 

@@ -72,7 +72,8 @@ struct TcMaps {
 };
 
 cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_map, int Kred, const Tables& tb,
-                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop = nullptr);
+                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop = nullptr,
+                      const CUtensorMap* masked = nullptr);  // `masked`: where the masked P goes (a map like p_map's)
 cudaError_t tc_gemm(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                     const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st);
 // Same product with 256x256 tiles computed by CTA pairs (cta_group::2).  Maps: p box (64,128),
@@ -93,7 +94,8 @@ struct PairShrink {
   CUtensorMap a2_map;    // job 2 slab [n_slots*r_pad, K2] box (64, r_pad)
   void* s_ext2;
   int K2;
-  DropArgs drop;         // of job 1's input (no prologue, no job 2)
+  DropArgs drop;         // of the shrink's input (no prologue, one job)
+  bool job2_only;        // with job2 and drop: no job 1, a_map is where the masked activations go; beside a `delta`
 };
 // K-split tail of the pair GEMM (the last round of 256x256 tiles cut along K when it would
 // leave at least half of the CTA pairs idle): fp32 partial tiles and their release flags, in

@@ -437,8 +437,9 @@ struct PairParams {
   // S_ext planes the LoRA stages sum: 1 = the full product; 2 = two K-half partial products
   // (written by the co-scheduled shrink), plane p starting at S map row p * s_plane_rows
   int s_planes, s_plane_rows;
-  // optional second shrink job (own activations/slab/K), items after the first job's
-  int job2, Kred2;
+  // optional second shrink job (own activations/slab/K), items after the first job's; job2_only: no first job, whole K
+  // ranges (S_ext of one product, nobody waits for it), and the masked activations are stored (kDrop)
+  int job2, Kred2, job2_only;
   void* s_ext2;
   PairDelta delta;  // kDelta kernels
   PairMx4 mx4;      // kMx4 kernels
@@ -536,7 +537,9 @@ __device__ __forceinline__ bool wait_units_ready(const uint64_t* ready, int u0, 
 // flag is released.  The epilogue warps of CTA 0
 // also write the all-zero block before releasing item 0.  In prologue mode the role keeps the
 // TMEM allocation permit (the GEMM allocates after it) and its barriers are its own.
-// kDrop: eight more warps mask each x tile between its copy and its MMAs (rmasked).
+// kDrop: eight more warps mask each x tile between its copy and its MMAs (`masked`); with job2_only one more stores the
+// masked tiles, for a product that follows (map_a; by the first unit of a row tile, the others have the same), and a stage
+// is free when its MMAs and the store have read it.
 constexpr int kMaskWarps = 8;
 template <typename OutT, bool kPrologue, bool kDrop>
 __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CUtensorMap& map_p,
@@ -550,13 +553,18 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
   const int me = static_cast<int>(blockIdx.x), n_me = kPrologue ? static_cast<int>(gridDim.x) : 2 * prm.n_shrink_pairs;
   const int r_pad = prm.r_pad;
   // item = (job, unit, K half): half h of a job covers its k-blocks [h*half, min(nkb, (h+1)*half))
-  const int n_items = (prm.job2 ? 4 : 2) * tb.n_units;
+  const bool only2 = kDrop && prm.job2_only;
+  const int parts = only2 ? 1 : 2;  // of K
+  const int n_items = (prm.job2 && !only2 ? 4 : parts) * tb.n_units;
+  auto item_job = [&](int item) { return only2 || item >= 2 * tb.n_units ? 1 : 0; };
+  auto item_unit = [&](int item) { return only2 ? item : (item - (item >= 2 * tb.n_units ? 2 * tb.n_units : 0)) >> 1; };
+  auto item_part = [&](int item) { return only2 ? 0 : item & 1; };
   const int64_t plane_elems = static_cast<int64_t>(prm.s_plane_rows) * r_pad;
   auto job_nkb = [&](int job) { return ((job ? prm.Kred2 : prm.Kred) + kBK - 1) / kBK; };
   if (threadIdx.x == 0) {
     for (int s = 0; s < kRoleStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
+      mbar_init(&empty[s], only2 ? 2 : 1);
       if (kDrop) mbar_init(&masked[s], kMaskWarps);
     }
     for (int b = 0; b < 2; ++b) {
@@ -591,11 +599,10 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
       uint32_t phase = 0, issued_mask = 0, last_parity = 0;
       bool ok = true;
       for (int item = me; item < n_items && ok; item += n_me) {
-        const int job = item >= 2 * tb.n_units ? 1 : 0;
-        const int u = (item - job * 2 * tb.n_units) >> 1, h = item & 1;
+        const int job = item_job(item), u = item_unit(item), h = item_part(item);
         const CUtensorMap* mp = job ? &map_p2 : &map_p;
         const CUtensorMap* ma = job ? &map_a2 : &map_a;
-        const int nkb = job_nkb(job), nkb_half = (nkb + 1) / 2;
+        const int nkb = job_nkb(job), nkb_half = (nkb + parts - 1) / parts;
         const int tile = tb.unit_tile(u), st0 = tb.unit_st0(u), nst = tb.unit_nst(u);
         int arow[4];
 #pragma unroll
@@ -635,9 +642,8 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
       const uint32_t a_base = smem_u32(sA);
       int it = 0;
       for (int item = me; item < n_items && ok; item += n_me, ++it) {
-        const int job = item >= 2 * tb.n_units ? 1 : 0;
-        const int u = (item - job * 2 * tb.n_units) >> 1, h = item & 1;
-        const int nkb = job_nkb(job), nkb_half = (nkb + 1) / 2;
+        const int job = item_job(item), u = item_unit(item), h = item_part(item);
+        const int nkb = job_nkb(job), nkb_half = (nkb + parts - 1) / parts;
         const int N = tb.unit_nst(u) * r_pad;
         const uint32_t idesc = umma_idesc_f16(kBM, N, prm.ab_fmt, 0, 0);
         const int buf = it & 1;
@@ -690,20 +696,18 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
     uint32_t phase = 0;
     bool ok = true;
     for (int item = me; item < n_items && ok; item += n_me) {
-      const int u = item >> 1, h = item & 1;
-      const int nkb = job_nkb(0), nkb_half = (nkb + 1) / 2;
-      const int tile = tb.unit_tile(u), st0 = tb.unit_st0(u), nst = tb.unit_nst(u);
-      uint32_t threshold = 0;
-      for (int q = 0; q < nst; ++q)
-        if (row >= tb.st_lo(st0 + q) && row < tb.st_hi(st0 + q)) threshold = prm.drop.threshold[tb.st_slot(st0 + q)];
-      const bool any = __any_sync(0xffffffffu, threshold != 0);
+      const int u = item_unit(item), h = item_part(item);
+      const int nkb = job_nkb(item_job(item)), nkb_half = (nkb + parts - 1) / parts;
+      const int tile = tb.unit_tile(u);
+      const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
+      const bool any = __any_sync(0xffffffffu, high != 0);
       const int kb_end = min(nkb, (h + 1) * nkb_half);
       for (int kb = h * nkb_half; kb < kb_end; ++kb) {
         ok = warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull);
         if (!ok) break;
         if (any) {
-          mask_half_row(sA + stage * kRoleStageBytes, row, half, kb, static_cast<uint32_t>(tile * kBM + row), threshold << 16,
-                        prm.drop);
+          mask_granules<4>(sA + stage * kRoleStageBytes, row, 4 * half, kb, static_cast<uint32_t>(tile * kBM + row), high,
+                           prm.drop);
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -714,20 +718,56 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
         }
       }
     }
+  } else if (kDrop && warp == kThreads / 32 + kMaskWarps) {
+    if (only2 && lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      uint64_t* held = nullptr;  // `empty` of the stage whose store may still read it
+      bool ok = true;
+      for (int item = me; item < n_items && ok; item += n_me) {
+        const int u = item_unit(item), tile = tb.unit_tile(u), nkb = job_nkb(1);
+        const bool store = tb.tile_unit(tile) == u;
+        for (int kb = 0; kb < nkb; ++kb) {
+          ok = mbar_wait_stage(&masked[stage], phase, abort_flag, tb.err, kErrTimeoutFull);
+          if (!ok) break;
+          if (store) {
+            tma_store_2d(&map_a, sA + stage * kRoleStageBytes, kb * kBK, tile * kBM);
+            bulk_commit();
+            if (held) {
+              bulk_wait_read<1>();
+              mbar_arrive(held);
+            }
+            held = &empty[stage];
+          } else {
+            if (held) {
+              bulk_wait_read<0>();
+              mbar_arrive(held);
+              held = nullptr;
+            }
+            mbar_arrive(&empty[stage]);
+          }
+          if (++stage == kRoleStages) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      bulk_wait_all();  // (the last held stage is not used again)
+    }
+    __syncwarp();
   } else if (warp < kThreads / 32) {  // the extra warps of other kernels have no part in it
     const int q = warp & 3;
     const int row = q * 32 + lane;
     OutT* s_ext = reinterpret_cast<OutT*>(prm.s_ext);
-    if (me == 0)  // the all-zero segment tile of both planes, published with item 0
+    if (me == 0 && !only2)  // the all-zero segment tile of both planes, published with item 0
       for (int e = threadIdx.x - 64; e < kBM * r_pad; e += 128) {
         s_ext[static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad + e] = cvt_out<OutT>(0.f);
         s_ext[plane_elems + static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad + e] = cvt_out<OutT>(0.f);
       }
     int it = 0;
     for (int item = me; item < n_items; item += n_me, ++it) {
-      const int job = item >= 2 * tb.n_units ? 1 : 0;
-      const int u = (item - job * 2 * tb.n_units) >> 1, h = item & 1;
-      const int nkb = job_nkb(job), nkb_half = (nkb + 1) / 2;
+      const int job = item_job(item), u = item_unit(item), h = item_part(item);
+      const int nkb = job_nkb(job), nkb_half = (nkb + parts - 1) / parts;
       const bool has_k = h * nkb_half < nkb;  // an empty K half contributes zeros
       OutT* s_out = reinterpret_cast<OutT*>(job ? prm.s_ext2 : prm.s_ext);
       const int st0 = tb.unit_st0(u), nst = tb.unit_nst(u);
@@ -752,7 +792,7 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
                         row < (j == 0 ? hi[0] : j == 1 ? hi[1] : j == 2 ? hi[2] : hi[3]);
         const float scale = j == 0 ? sc[0] : j == 1 ? sc[1] : j == 2 ? sc[2] : sc[3];
         OutT* dst = s_out + h * plane_elems + (static_cast<int64_t>(st0 + j) * kBM + row) * r_pad;
-        OutT* dst_lo = dst + 2 * plane_elems;
+        OutT* dst_lo = dst + parts * plane_elems;
         for (int c = 0; c < r_pad; c += 16) {
           float f[16];
 #pragma unroll
@@ -777,6 +817,7 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
       }
       tc_fence_before();
       mbar_arrive(&tempty[buf]);
+      if (only2) continue;
       // publish: each warp orders its stores, then thread 64 sees all four warps and releases
       __threadfence();
       __syncwarp();
@@ -931,7 +972,7 @@ __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const Pa
 // kMx4: Q is held in 4 bits (prm.mx4) and decoded on the way into shared memory; map_q is not used.
 // kDrop: the co-scheduled shrink's input is masked (prm.drop), by warps that a kMx4 kernel has and others get for it.
 __host__ __device__ constexpr int pair_threads(bool mx4, bool drop) {
-  return mx4 ? kMx4Threads : kThreads + (drop ? 32 * kMaskWarps : 0);
+  return mx4 ? kMx4Threads : kThreads + (drop ? 32 * (kMaskWarps + 1) : 0);
 }
 template <bool kQMN, typename OutT, bool kDelta, bool kMx4, bool kDrop>
 __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
@@ -1428,7 +1469,8 @@ struct ShrinkParams {
   int cluster;
   int r_pad;
   Tables tb;
-  DropArgs drop;  // kDrop kernels
+  DropArgs drop;     // kDrop kernels
+  int store_masked;  // ... which leave the masked P in memory
 };
 
 constexpr int kShrABytes = kBM * kBK * 2;    // 16 KB
@@ -1438,11 +1480,15 @@ constexpr int kPartLd = kBM + 1;             // column-major partial sums, odd s
 constexpr int kMaxShrCluster = 4;             // K split across at most 4 CTAs (all resident at once)
 static_assert(64 * kPartLd * 4 <= kShrStages * (kShrABytes + kShrBBytes), "partials must fit the stage area");
 
-// kDrop: eight more warps mask each tile of P between its copy and its MMAs.
+// kDrop: sixteen more warps mask each tile of P between its copy and its MMAs, and with store_masked one more stores the
+// masked tile (map_m; by the first unit of a row tile, the others have the same).  The generator needs four warps a
+// scheduler to be issued back to back.
+constexpr int kShrMaskWarps = 16;
+constexpr int kShrDropThreads = kThreads + 32 * (kShrMaskWarps + 1);
 template <typename OutT, bool kDrop>
-__global__ void __launch_bounds__(kThreads + (kDrop ? 32 * kMaskWarps : 0), 1)
+__global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
     tc_shrink_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_a,
-                     const ShrinkParams prm) {
+                     const __grid_constant__ CUtensorMap map_m, const ShrinkParams prm) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
@@ -1474,10 +1520,10 @@ __global__ void __launch_bounds__(kThreads + (kDrop ? 32 * kMaskWarps : 0), 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < kShrStages; ++s) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 1);
-      if (kDrop) mbar_init(&masked[s], kMaskWarps);
+      mbar_init(&empty[s], kDrop && prm.store_masked ? 2 : 1);
+      if (kDrop) mbar_init(&masked[s], kShrMaskWarps);
     }
-    mbar_init(tfull, 1);
+    mbar_init(tfull, kDrop && prm.store_masked ? 2 : 1);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -1571,19 +1617,45 @@ __global__ void __launch_bounds__(kThreads + (kDrop ? 32 * kMaskWarps : 0), 1)
       }
     }
     __syncwarp();
+  } else if (kDrop && warp == kThreads / 32 + kShrMaskWarps) {
+    if (prm.store_masked && lane == 0) {
+      const bool store = tb.tile_unit(tile) == unit;
+      int stage = 0;
+      uint32_t phase = 0;
+      uint64_t* held = nullptr;  // `empty` of the stage whose store may still read it
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!mbar_wait_stage(&masked[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) break;
+        if (store) {
+          tma_store_2d(&map_m, sA + stage * kShrABytes, kb * kBK, tile * kBM);
+          bulk_commit();
+          if (held) {
+            bulk_wait_read<1>();
+            mbar_arrive(held);
+          }
+          held = &empty[stage];
+        } else {
+          mbar_arrive(&empty[stage]);
+        }
+        if (++stage == kShrStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      bulk_wait_read<0>();
+      mbar_arrive(tfull);  // the stages may become partial sums
+      bulk_wait_all();
+    }
+    __syncwarp();
   } else if (kDrop && warp >= kThreads / 32) {
-    const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, half = w >> 2;
-    uint32_t threshold = 0;
-    for (int q = 0; q < nst; ++q)
-      if (row >= seg_lo[q] && row < seg_hi[q]) threshold = prm.drop.threshold[tb.st_slot(st0 + q)];
-    const bool any = __any_sync(0xffffffffu, threshold != 0);
+    const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, quarter = w >> 2;
+    const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
+    const bool any = __any_sync(0xffffffffu, high != 0);
     int stage = 0;
     uint32_t phase = 0;
     for (int kb = kb0; kb < kb1; ++kb) {
       if (!warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) break;
       if (any) {
-        mask_half_row(sA + stage * kShrABytes, row, half, kb, static_cast<uint32_t>(tile * kBM + row), threshold << 16,
-                      prm.drop);
+        mask_granules<2>(sA + stage * kShrABytes, row, 2 * quarter, kb, static_cast<uint32_t>(tile * kBM + row), high, prm.drop);
         fence_proxy_async_smem();
       }
       __syncwarp();
@@ -2461,10 +2533,10 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   const CUtensorMap* p2_map = &maps.p;
   const CUtensorMap* a2_map = &maps.p;
   if (shrink != nullptr && (shrink->n_pairs > 0 || shrink->prologue)) {
-    p.group_m = 4;
+    if (!shrink->job2_only) p.group_m = 4;
     p.shrink_prologue = shrink->prologue ? 1 : 0;
     p.n_shrink_pairs = shrink->prologue ? 0 : shrink->n_pairs;
-    p.s_planes = 2;
+    p.s_planes = shrink->job2_only ? 1 : 2;
     p.s_ext = shrink->s_ext;
     p.unit_ready = shrink->unit_ready;
     p.gen = shrink->gen;
@@ -2505,8 +2577,9 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cfg.gridDim = dim3(2 * (gemm_pairs + p.n_shrink_pairs));
   const bool drop = shrink != nullptr && shrink->drop.threshold != nullptr;
   if (drop) {
-    if (q_mn_major || delta != nullptr || shrink->prologue || shrink->job2) return cudaErrorInvalidValue;
+    if (shrink->prologue || shrink->job2 != shrink->job2_only || (delta != nullptr) != shrink->job2_only) return cudaErrorInvalidValue;
     p.drop = shrink->drop;
+    p.job2_only = shrink->job2_only ? 1 : 0;
   }
   cfg.blockDim = dim3(pair_threads(mx4 != nullptr, drop));
   cfg.dynamicSmemBytes = mx4 != nullptr ? kMx4PairSmem : kPairSmem;
@@ -2541,16 +2614,26 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
     }                                                                          \
   }
   if (delta != nullptr) {
-    if (shrink != nullptr || tail != nullptr) return cudaErrorInvalidValue;
+    if ((shrink != nullptr && !shrink->job2_only) || tail != nullptr) return cudaErrorInvalidValue;
     p.delta = *delta;
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.numAttrs = 2;
-    if (mx4 != nullptr) LF_LAUNCH_PAIR_TYPES(true, true)
+    if (drop) {  // the backward's dX
+      if (!q_mn_major) return cudaErrorInvalidValue;
+      if (dtype == LF_BF16) {
+        if (mx4 != nullptr) LF_LAUNCH_PAIR(true, __nv_bfloat16, true, true, true)
+        else LF_LAUNCH_PAIR(true, __nv_bfloat16, true, false, true)
+      } else {
+        if (mx4 != nullptr) LF_LAUNCH_PAIR(true, __half, true, true, true)
+        else LF_LAUNCH_PAIR(true, __half, true, false, true)
+      }
+    } else if (mx4 != nullptr) LF_LAUNCH_PAIR_TYPES(true, true)
     else LF_LAUNCH_PAIR_TYPES(true, false)
     return e;
   }
-  if (drop) {
+  if (drop) {  // the forward
+    if (q_mn_major) return cudaErrorInvalidValue;
     if (dtype == LF_BF16) {
       if (mx4 != nullptr) LF_LAUNCH_PAIR(false, __nv_bfloat16, false, true, true)
       else LF_LAUNCH_PAIR(false, __nv_bfloat16, false, false, true)
@@ -2567,7 +2650,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
 }
 
 cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_map, int Kred, const Tables& tb,
-                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop) {
+                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop, const CUtensorMap* masked) {
   if (tb.n_units == 0) return cudaSuccess;
   const int nkb = (Kred + kBK - 1) / kBK;
   // split K across a cluster while every CTA still fits on the GPU at once (one per SM)
@@ -2598,11 +2681,12 @@ cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_
   cudaError_t e;
   auto start = [&](auto* kernel) {
     e = ensure_smem(kernel, kShrSmem);
-    return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p_map, a_map, p) : e;
+    return e == cudaSuccess ? cudaLaunchKernelEx(&cfg, kernel, p_map, a_map, masked ? *masked : p_map, p) : e;
   };
   if (drop != nullptr && drop->threshold != nullptr) {
     p.drop = *drop;
-    cfg.blockDim = dim3(kThreads + 32 * kMaskWarps);
+    p.store_masked = masked != nullptr;
+    cfg.blockDim = dim3(kShrDropThreads);
     e = dtype == LF_BF16 ? start(tc_shrink_kernel<__nv_bfloat16, true>) : start(tc_shrink_kernel<__half, true>);
   } else {
     e = dtype == LF_BF16 ? start(tc_shrink_kernel<__nv_bfloat16, false>) : start(tc_shrink_kernel<__half, false>);
