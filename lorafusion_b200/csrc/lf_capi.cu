@@ -130,7 +130,9 @@ bool make_map(CUtensorMap* m, int dtype, const void* base, uint64_t inner, uint6
   const cuuint64_t strides[1] = {pitch_bytes};
   const cuuint32_t box[2] = {box_inner, box_outer};
   const cuuint32_t estr[2] = {1, 1};
-  const CUtensorMapDataType dt = dtype == LF_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const CUtensorMapDataType dt = dtype == LF_BF16   ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                 : dtype == LF_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                   : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
   std::memset(m, 0, sizeof(*m));
   CUresult r = g_encode(m, dt, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
@@ -777,10 +779,12 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
       if (!gemm_done && drop) {
         // the mask is of grad_x's adapters' part alone: it is added to g W.  S_f and m x, which dA and dB read, are computed
         // on CTA pairs that this GEMM's rounds leave idle, or ahead of it.
-        CUtensorMap x_map;
+        CUtensorMap x_map, delta_map;
         float* delta = reinterpret_cast<float*>(opt.scratch + drop_scratch_mask(prob));
         const PairDelta d{delta, nullptr, K};
-        if (!make_map(&x_map, dt, prob->x_dev, K, T, K * es, 64, 128)) return LF_ERR_UNSUPPORTED;
+        if (!make_map(&x_map, dt, prob->x_dev, K, T, K * es, 64, 128) ||
+            !make_map(&delta_map, LF_F32, delta, K, T, static_cast<uint64_t>(K) * 4, 32, 32))
+          return LF_ERR_UNSUPPORTED;
         e = tc_shrink(dt, p_g, bt_map, N, tb, s_b, ds->num_sms, st);
         PairShrink sh{};
         sh.n_pairs = spare;
@@ -792,7 +796,7 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
         sh.K2 = K;
         sh.drop = opt.drop;
         if (e == cudaSuccess && spare == 0) e = tc_shrink(dt, x_map, a_map, K, tb, s_f, ds->num_sms, st, &opt.drop, &p_x);
-        if (e == cudaSuccess) e = drop_expand(dt, s_b, prob->at_pack_dev, T, K, tb, opt.drop, delta, st);
+        if (e == cudaSuccess) e = drop_expand(dt, sb_map, dx.l, delta_map, T, K, tb, opt.drop, ds->num_sms, st);
         if (e == cudaSuccess)
           e = tc_gemm_pair(dt, true, dx, T, K, N, false, tb, grad_x_dev, K, ds->num_sms, st, spare > 0 ? &sh : nullptr, nullptr,
                            &d, mx4p);

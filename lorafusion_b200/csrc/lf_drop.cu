@@ -2,12 +2,10 @@
 //
 //   drop_mask    xm = m x, bit for bit x or zero (1 / (1 - p) is in the adapters' factors: no rounding of its own).
 //   drop_expand  delta[t] = m[t] (S_b[t] A_i), float32, which the grad_x GEMM adds to g W in its epilogue.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-
 #include "lf_drop.cuh"
 #include "lf_internal.cuh"
 #include "lf_launch.cuh"
+#include "lf_ptx.cuh"
 
 namespace lf {
 namespace {
@@ -60,91 +58,196 @@ __global__ void __launch_bounds__(kThreads) drop_mask_kernel(const uint8_t* __re
   }
 }
 
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16*) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half*) {
-  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
+// delta [T, K] (float32) = m (S_b A_i), on tcgen05: units of 128 rows x 256 columns, persistent, one CTA an SM.  Warp 0 loads
+// for every segment of the row tile its S_b (hi and lo halves: both products go to one accumulator, so S enters to 2^-16) and
+// 256 rows of A_i^T [K, r_pad]; warp 1 issues the MMAs into one of two accumulators; eight warps mask 32 rows x 128
+// columns each and store them through shared memory.  A lane has a row, so eight columns are one counter's numbers.
+// The rank is short: what bounds it is the 4 T K bytes written, with the generator (1.3 us a unit of 2.9 us at the copy
+// rate) behind them.  (With warp-level MMAs that read both operands where they lie: 61 us at 4096 x 4096, rank 16, and 220 at
+// 8192 rows and rank 64, bound by L1.)
+constexpr int kExpandCols = 256;
+constexpr int kExpandThreads = 320;
+constexpr int kExpandRing = 128 * 1024;
+constexpr int kExpandMaxStages = 8;
+constexpr int kExpandStaging = 8 * 2 * 32 * 32 * 4;  // 8 warps x 2 buffers x (32 rows x 32 columns)
+constexpr int kExpandSmem = 1024 + kExpandRing + kExpandStaging;
+struct ExpandParams {
+  int T, K, n_cols, units;  // n_cols: column blocks
+  int stages, stage_bytes;
+  int lo_row;               // where the plane of the low halves starts in the S map
+  uint32_t idesc, layout, sbo;
+  DropArgs drop;
+  Tables tb;
+};
 
-// delta [T, K] (float32): a CTA takes 128 rows x 128 columns, a warp 16 of the rows.  S comes as hi and lo halves (two
-// products into one accumulator, so S enters to 2^-16), A_i^T [K, r_pad] per virtual slot.  The rank is short, so the
-// products are few and the time goes into the 4 T K bytes written; warp-level MMAs read both operands where
-// they lie.  Of a row's eight columns n .. n + 7, lane q of the four that hold them has 2q and 2q + 1, word q of one counter's
-// numbers: each lane computes every fourth counter and the four exchange words.
-constexpr int kExpandCols = 128;
-template <typename T16>
-__global__ void __launch_bounds__(kThreads) drop_expand_kernel(const uint16_t* __restrict__ s_hi, int64_t lo_off,
-                                                               const uint16_t* __restrict__ at, int T, int K, Tables tb,
-                                                               DropArgs d, float* __restrict__ delta) {
+__global__ void __launch_bounds__(kExpandThreads, 1)
+    drop_expand_kernel(const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_l,
+                       const __grid_constant__ CUtensorMap map_d, const ExpandParams prm) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = ring + kExpandRing;
+  __shared__ uint64_t full[kExpandMaxStages], empty[kExpandMaxStages], tfull[2], tempty[2], drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ volatile int abort_flag;
   pdl_launch_dependents();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
-  const int tile = blockIdx.x, k0 = blockIdx.y * kExpandCols;
-  const int row0 = warp * 16;
-  const int64_t t0 = static_cast<int64_t>(tile) * LF_TILE_ROWS + row0;
-  if (t0 >= T) return;
-  const int rp = tb.r_pad;
-  float acc[kExpandCols / 8][4];
-#pragma unroll
-  for (int n = 0; n < kExpandCols / 8; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.f;
-  uint32_t threshold[2] = {0, 0};
-  const int st1 = tb.tile_st(tile + 1);
-  for (int st = tb.tile_st(tile); st < st1; ++st) {
-    const int lo = tb.st_lo(st), hi = tb.st_hi(st);
-    if (hi <= row0 || lo >= row0 + 16) continue;
-    const int slot = tb.st_slot(st);
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = row0 + g + 8 * h;
-      if (row >= lo && row < hi) threshold[h] = d.threshold[slot];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const Tables& tb = prm.tb;
+  const int rp = tb.r_pad, s_bytes = 128 * rp * 2;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < prm.stages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
-    const uint16_t* s = s_hi + (static_cast<int64_t>(st) * LF_TILE_ROWS + row0) * rp;
-    for (int j = 0; j < rp; j += 16) {
-      uint32_t a[2][4];
-#pragma unroll
-      for (int p = 0; p < 2; ++p) {
-        const uint16_t* sp = s + (p ? lo_off : 0) + j + 2 * q;
-        a[p][0] = *reinterpret_cast<const uint32_t*>(sp + g * rp);
-        a[p][1] = *reinterpret_cast<const uint32_t*>(sp + (g + 8) * rp);
-        a[p][2] = *reinterpret_cast<const uint32_t*>(sp + g * rp + 8);
-        a[p][3] = *reinterpret_cast<const uint32_t*>(sp + (g + 8) * rp + 8);
-      }
-      const uint16_t* b = at + (static_cast<int64_t>(slot) * K + k0) * rp + j + 2 * q;
-#pragma unroll
-      for (int n = 0; n < kExpandCols / 8; ++n) {
-        if (k0 + n * 8 >= K) break;  // K is a multiple of 8
-        const uint16_t* bn = b + static_cast<int64_t>(n * 8 + g) * rp;
-        const uint32_t b0 = *reinterpret_cast<const uint32_t*>(bn), b1 = *reinterpret_cast<const uint32_t*>(bn + 8);
-        mma16816(acc[n], a[0], b0, b1, static_cast<T16*>(nullptr));
-        mma16816(acc[n], a[1], b0, b1, static_cast<T16*>(nullptr));
-      }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&tfull[b], 1);
+      mbar_init(&tempty[b], 8);
     }
+    mbar_init(&drain, 1);
+    abort_flag = 0;
+    fence_mbar_init();
+    tma_prefetch_desc(&map_s);
+    tma_prefetch_desc(&map_l);
+    tma_prefetch_desc(&map_d);
   }
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const int64_t t = t0 + g + 8 * h;
-#pragma unroll
-    for (int n4 = 0; n4 < kExpandCols / 32; ++n4) {
-      const uint4 r = philox(static_cast<uint32_t>(k0 / 8 + n4 * 4 + q), static_cast<uint32_t>(t), d.offset, d.seed);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        // counter n4 * 4 + i is lane i's: this lane wants word q of it
-        const uint32_t w0 = __shfl_sync(0xffffffffu, r.x, i, 4), w1 = __shfl_sync(0xffffffffu, r.y, i, 4);
-        const uint32_t w2 = __shfl_sync(0xffffffffu, r.z, i, 4), w3 = __shfl_sync(0xffffffffu, r.w, i, 4);
-        const uint32_t w = q == 0 ? w0 : q == 1 ? w1 : q == 2 ? w2 : w3;
-        const int n = n4 * 4 + i, k = k0 + n * 8 + 2 * q;
-        if (t < T && k < K) {
-          float2 v;
-          v.x = (w & 0xffffu) >= threshold[h] ? acc[n][2 * h] : 0.f;
-          v.y = (w >> 16) >= threshold[h] ? acc[n][2 * h + 1] : 0.f;
-          *reinterpret_cast<float2*>(delta + t * K + k) = v;
+  if (warp == 1) {
+    tmem_alloc(&tmem_slot, 512);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+
+  if (warp == 0) {
+    int stage = 0;
+    uint32_t phase = 0, issued = 0, parity = 0;
+    bool ok = true;
+    for (int u = blockIdx.x; u < prm.units && ok; u += gridDim.x) {
+      const int tile = u / prm.n_cols, c0 = (u - tile * prm.n_cols) * kExpandCols;
+      const int st1 = tb.tile_st(tile + 1);
+      for (int st = tb.tile_st(tile); st < st1; ++st) {
+        ok = warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, tb.err, kErrTimeoutEmpty);
+        if (!ok) break;
+        const int slot = tb.st_slot(st);
+        if (elect_one()) {
+          uint8_t* p = ring + stage * prm.stage_bytes;
+          mbar_arrive_expect_tx(&full[stage], 4 * s_bytes);
+          tma_load_2d(p, &map_s, &full[stage], 0, st * 128);
+          tma_load_2d(p + s_bytes, &map_s, &full[stage], 0, prm.lo_row + st * 128);
+          tma_load_2d(p + 2 * s_bytes, &map_l, &full[stage], 0, slot * prm.K + c0);
+          tma_load_2d(p + 3 * s_bytes, &map_l, &full[stage], 0, slot * prm.K + c0 + 128);
+        }
+        __syncwarp();
+        issued |= 1u << stage;
+        parity = (parity & ~(1u << stage)) | (phase << stage);
+        if (++stage == prm.stages) {
+          stage = 0;
+          phase ^= 1;
         }
       }
     }
+    if (!ok && lane == 0)  // let every copy that was started land
+      for (int i = 0; i < prm.stages; ++i)
+        if (issued & (1u << i)) drain_wait(&full[i], (parity >> i) & 1u, tb.err);
+    __syncwarp();
+  } else if (warp == 1) {
+    int stage = 0, it = 0;
+    uint32_t phase = 0;
+    bool ok = true, any = false;
+    for (int u = blockIdx.x; u < prm.units && ok; u += gridDim.x, ++it) {
+      const int tile = u / prm.n_cols, buf = it & 1;
+      ok = warp_wait_stage(&tempty[buf], ((it >> 1) & 1) ^ 1, &abort_flag, tb.err, kErrTimeoutAcc);
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t acc = 0;
+      const int st1 = tb.tile_st(tile + 1);
+      for (int st = tb.tile_st(tile); st < st1; ++st) {
+        ok = warp_wait_stage(&full[stage], phase, &abort_flag, tb.err, kErrTimeoutFull);
+        if (!ok) break;
+        tc_fence_after();
+        if (elect_one()) {
+          const uint32_t p = smem_u32(ring + stage * prm.stage_bytes);
+          for (int half = 0; half < 2; ++half)
+            for (int k = 0; k < rp / 16; ++k)
+              umma_f16(tmem + buf * 256, umma_sdesc(p + half * s_bytes + k * 32, 16, prm.sbo, prm.layout),
+                       umma_sdesc(p + 2 * s_bytes + k * 32, 16, prm.sbo, prm.layout), prm.idesc, acc | half | k);
+          umma_commit(&empty[stage]);
+        }
+        __syncwarp();
+        acc = 1;
+        any = true;
+        if (++stage == prm.stages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      }
+      if (ok && elect_one()) umma_commit(&tfull[buf]);
+      __syncwarp();
+    }
+    if (!ok && any && elect_one()) {
+      umma_commit(&drain);
+      drain_wait(&drain, 0, tb.err);
+    }
+    __syncwarp();
+  } else {
+    const int w = warp - 2, q = warp & 3, half = w >> 2;
+    uint8_t* mine = staging + w * (2 * 4096);
+    int it = 0, buf_out = 0;
+    for (int u = blockIdx.x; u < prm.units; u += gridDim.x, ++it) {
+      const int tile = u / prm.n_cols, c0 = (u - tile * prm.n_cols) * kExpandCols + half * 128, buf = it & 1;
+      const int row = q * 32 + lane;
+      const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
+      if (!warp_wait(&tfull[buf], (it >> 1) & 1, &abort_flag, tb.err, kErrTimeoutAcc)) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int c = 0; c < 128; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(tmem + (static_cast<uint32_t>(q * 32) << 16) + buf * 256 + half * 128 + c, v);
+        uint32_t ctr[4];
+        uint4 r[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ctr[j] = static_cast<uint32_t>((c0 + c) / 8 + j);
+        philox<4>(ctr, static_cast<uint32_t>(tile * LF_TILE_ROWS + row), prm.drop.offset, prm.drop.seed, r);
+        tmem_wait_ld();
+        if (c == 96) {  // accumulator fully read
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&tempty[buf]);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t word[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if ((word[i] << 16) < high) v[8 * j + 2 * i] = 0u;
+            if (word[i] < high) v[8 * j + 2 * i + 1] = 0u;
+          }
+        }
+        if (c0 + c >= prm.K || tile * LF_TILE_ROWS + q * 32 >= prm.T) continue;
+        uint8_t* out = mine + buf_out * 4096;
+        if (lane == 0) bulk_wait_read<1>();  // the store that used this buffer has read it
+        __syncwarp();
+#pragma unroll
+        for (int g = 0; g < 8; ++g)
+          *reinterpret_cast<uint4*>(out + lane * 128 + ((g ^ (lane & 7)) << 4)) =
+              make_uint4(v[4 * g], v[4 * g + 1], v[4 * g + 2], v[4 * g + 3]);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&map_d, out, c0 + c, tile * LF_TILE_ROWS + q * 32);
+          bulk_commit();
+        }
+        buf_out ^= 1;
+      }
+    }
+    if (lane == 0) bulk_wait_all();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -160,14 +263,28 @@ cudaError_t drop_mask(int dtype, const void* x, int T, int K, const Tables& tb, 
   return cudaGetLastError();
 }
 
-cudaError_t drop_expand(int dtype, const void* s_ext, const void* at_pack, int T, int K, const Tables& tb, const DropArgs& d,
-                        float* delta, cudaStream_t st) {
+cudaError_t drop_expand(int dtype, const CUtensorMap& s_map, const CUtensorMap& l_map, const CUtensorMap& delta_map, int T,
+                        int K, const Tables& tb, const DropArgs& d, int num_sms, cudaStream_t st) {
   if (T == 0 || K == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>(tb.n_tiles), static_cast<unsigned>((K + kExpandCols - 1) / kExpandCols));
-  const int64_t lo = static_cast<int64_t>(tb.n_segtiles + 1) * LF_TILE_ROWS * tb.r_pad;  // plane of the low halves
-  auto* k = dtype == LF_BF16 ? drop_expand_kernel<__nv_bfloat16> : drop_expand_kernel<__half>;
-  k<<<grid, kThreads, 0, st>>>(static_cast<const uint16_t*>(s_ext), lo, static_cast<const uint16_t*>(at_pack), T, K, tb, d,
-                               delta);
+  ExpandParams p{};
+  p.T = T, p.K = K;
+  p.n_cols = (K + kExpandCols - 1) / kExpandCols;
+  const int64_t units = static_cast<int64_t>(tb.n_tiles) * p.n_cols;
+  if (units > INT32_MAX) return cudaErrorInvalidValue;
+  p.units = static_cast<int>(units);
+  p.stage_bytes = 4 * 128 * tb.r_pad * 2;
+  p.stages = kExpandRing / p.stage_bytes;
+  if (p.stages > kExpandMaxStages) p.stages = kExpandMaxStages;
+  p.lo_row = (tb.n_segtiles + 1) * LF_TILE_ROWS;
+  p.idesc = umma_idesc_f16(128, kExpandCols, dtype == LF_BF16 ? 1 : 0, 0, 0);
+  p.layout = umma_layout_for_span(tb.r_pad * 2);
+  p.sbo = static_cast<uint32_t>(8 * tb.r_pad * 2);
+  p.drop = d;
+  p.tb = tb;
+  const cudaError_t e =
+      cudaFuncSetAttribute(drop_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kExpandSmem);  // of this device
+  if (e != cudaSuccess) return e;
+  drop_expand_kernel<<<p.units < num_sms ? p.units : num_sms, kExpandThreads, kExpandSmem, st>>>(s_map, l_map, delta_map, p);
   return cudaGetLastError();
 }
 

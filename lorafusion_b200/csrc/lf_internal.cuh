@@ -248,9 +248,10 @@ cudaError_t rows_forward_simt(const RowsArgs& a, int dtype, cudaStream_t st);
 // --------------------------------------------------------------- dropout in front of the adapters
 cudaError_t drop_mask(int dtype, const void* x, int T, int K, const Tables& tb, const DropArgs& d, void* out,
                       cudaStream_t st);
-// delta[t][k] = m(t, k) sum_j S[t][j] A_i[j][k], S the hi and lo planes of an s_ext (one product, not K halves); bf16 / f16
-cudaError_t drop_expand(int dtype, const void* s_ext, const void* at_pack, int T, int K, const Tables& tb, const DropArgs& d,
-                        float* delta, cudaStream_t st);
+// delta[t][k] = m(t, k) sum_j S[t][j] A_i[j][k], float32; bf16 / f16 operands.  Maps: S, the hi and lo planes of an s_ext
+// (one product, not K halves), box (r_pad, 128); A_i^T [n_slots K, r_pad] box (r_pad, 128); delta [T, K] box (32, 32).
+cudaError_t drop_expand(int dtype, const CUtensorMap& s_map, const CUtensorMap& l_map, const CUtensorMap& delta_map, int T,
+                        int K, const Tables& tb, const DropArgs& d, int num_sms, cudaStream_t st);
 
 // --------------------------------------------------------------- weights in 4 bits
 size_t mx4_bytes(int N, int K);
