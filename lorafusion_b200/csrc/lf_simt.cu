@@ -55,6 +55,7 @@ __global__ void __launch_bounds__(256) simt_shrink_kernel(const T* __restrict__ 
     double acc[16];
 #pragma unroll
     for (int jj = 0; jj < 16; ++jj) acc[jj] = 0.0;
+#pragma unroll 4  // loads of four steps in flight
     for (int k = lane; k < Kred; k += 32) {
       const double xv = to_f(xr[k]);
 #pragma unroll
@@ -76,52 +77,61 @@ __global__ void __launch_bounds__(256) simt_shrink_kernel(const T* __restrict__ 
   }
 }
 
-// 64x64 output tile, 256 threads, 4x4 per thread, K chunks of 16.
-constexpr int SG_BM = 64, SG_BN = 64, SG_BK = 16;
+// kB x kB output tile, 256 threads, kT x kT per thread, K chunks of kK.  Each result is one chain of fused multiply-adds
+// along K in float64, whatever the tile.  The next chunk is on its way while one is used, and operands are converted once, on
+// their way into shared memory (13 conversions a cycle and SM, 62 multiply-adds).  Tiles of 64 where they give
+// every SM one, else of 16: 128 x 256 -> 256 in float32 took 60 us with 8 tiles of 64, now 12.
+constexpr int SG_T = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(256) simt_gemm_kernel(const T* __restrict__ P, int64_t ldp,
-                                                        const T* __restrict__ Q, int64_t qsn, int64_t qsk, int Trows,
-                                                        int Nout, int Kred, const double* __restrict__ s_ext,
-                                                        const T* __restrict__ lpk, Tables tb, T* __restrict__ out,
-                                                        int64_t ldo, DropArgs drop) {
-  __shared__ float ps[SG_BK][SG_BM + 4];
-  __shared__ float qs[SG_BK][SG_BN + 4];
-  const int m0 = blockIdx.y * SG_BM, n0 = blockIdx.x * SG_BN;
+template <typename T, int kB, int kT, int kK>
+__global__ void __launch_bounds__(SG_T) simt_gemm_kernel(const T* __restrict__ P, int64_t ldp,
+                                                         const T* __restrict__ Q, int64_t qsn, int64_t qsk, int Trows,
+                                                         int Nout, int Kred, const double* __restrict__ s_ext,
+                                                         const T* __restrict__ lpk, Tables tb, T* __restrict__ out,
+                                                         int64_t ldo, DropArgs drop) {
+  constexpr int kSide = kB / kT;  // threads along a side
+  static_assert(kSide * kSide == SG_T, "256 threads");
+  constexpr int kLoads = kB * kK / SG_T;
+  __shared__ double ps[kK][kB + 1];
+  __shared__ double qs[kK][kB + 1];
+  const int m0 = blockIdx.y * kB, n0 = blockIdx.x * kB;
   const int tid = threadIdx.x;
-  const int tr = tid / 16, tc = tid % 16;  // 16x16 threads, 4x4 each
-  double acc[4][4] = {};
-  for (int k0 = 0; k0 < Kred; k0 += SG_BK) {
-    for (int e = tid; e < SG_BM * SG_BK; e += 256) {
-      const int r = e / SG_BK, k = e % SG_BK;
-      const int gr = m0 + r, gk = k0 + k;
-      ps[k][r] = (gr < Trows && gk < Kred) ? to_f(P[static_cast<int64_t>(gr) * ldp + gk]) : 0.f;
+  const int tr = tid / kSide, tc = tid % kSide;
+  double acc[kT][kT] = {};
+  T pv[kLoads], qv[kLoads];
+  const bool k_fast = qsk == 1;
+  auto fetch = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int e = tid + i * SG_T;
+      const int gr = m0 + e / kK, gk = k0 + e % kK;
+      pv[i] = (gr < Trows && gk < Kred) ? P[static_cast<int64_t>(gr) * ldp + gk] : from_f<T>(0.f);
+      const int n = k_fast ? e / kK : e % kB, k = k_fast ? e % kK : e / kB;
+      const int gn = n0 + n, gq = k0 + k;
+      qv[i] = (gn < Nout && gq < Kred) ? Q[static_cast<int64_t>(gn) * qsn + static_cast<int64_t>(gq) * qsk] : from_f<T>(0.f);
     }
-    for (int e = tid; e < SG_BN * SG_BK; e += 256) {
-      int n, k;
-      if (qsk == 1) {
-        n = e / SG_BK;
-        k = e % SG_BK;
-      } else {
-        k = e / SG_BN;
-        n = e % SG_BN;
-      }
-      const int gn = n0 + n, gk = k0 + k;
-      qs[k][n] = (gn < Nout && gk < Kred) ? to_f(Q[static_cast<int64_t>(gn) * qsn + static_cast<int64_t>(gk) * qsk])
-                                          : 0.f;
+  };
+  fetch(0);
+  for (int k0 = 0; k0 < Kred; k0 += kK) {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int e = tid + i * SG_T;
+      ps[e % kK][e / kK] = static_cast<double>(to_f(pv[i]));
+      qs[k_fast ? e % kK : e / kB][k_fast ? e / kK : e % kB] = static_cast<double>(to_f(qv[i]));
     }
     __syncthreads();
+    if (k0 + kK < Kred) fetch(k0 + kK);
 #pragma unroll
-    for (int k = 0; k < SG_BK; ++k) {
-      float a[4], b[4];
+    for (int k = 0; k < kK; ++k) {
+      double a[kT], b[kT];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = ps[k][tr * 4 + i];
+      for (int i = 0; i < kT; ++i) a[i] = ps[k][tr * kT + i];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) b[j] = qs[k][tc * 4 + j];
+      for (int j = 0; j < kT; ++j) b[j] = qs[k][tc * kT + j];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+      for (int i = 0; i < kT; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fma(static_cast<double>(a[i]), static_cast<double>(b[j]), acc[i][j]);
+        for (int j = 0; j < kT; ++j) acc[i][j] = fma(a[i], b[j], acc[i][j]);
     }
     __syncthreads();
   }
@@ -132,8 +142,8 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(const T* __restrict__ P,
     const int tile = m0 / LF_TILE_ROWS;
     const int st_b = tb.tile_st(tile), st_e = tb.tile_st(tile + 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int gr = m0 + tr * 4 + i;
+    for (int i = 0; i < kT; ++i) {
+      const int gr = m0 + tr * kT + i;
       if (gr >= Trows) continue;
       const int row = gr - tile * LF_TILE_ROWS;
       for (int st = st_b; st < st_e; ++st) {
@@ -141,8 +151,8 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(const T* __restrict__ P,
         const double* srow = s_ext + (static_cast<int64_t>(st) * LF_TILE_ROWS + row) * r_pad;
         const T* lb = lpk + static_cast<int64_t>(tb.st_slot(st)) * Nout * r_pad;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int gn = n0 + tc * 4 + j;
+        for (int j = 0; j < kT; ++j) {
+          const int gn = n0 + tc * kT + j;
           if (gn >= Nout) continue;
           if (drop.threshold != nullptr) {
             const uint4 r = philox(static_cast<uint32_t>(gn >> 3), static_cast<uint32_t>(gr), drop.offset, drop.seed);
@@ -158,12 +168,12 @@ __global__ void __launch_bounds__(256) simt_gemm_kernel(const T* __restrict__ P,
     }
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int gr = m0 + tr * 4 + i;
+  for (int i = 0; i < kT; ++i) {
+    const int gr = m0 + tr * kT + i;
     if (gr >= Trows) continue;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int gn = n0 + tc * 4 + j;
+    for (int j = 0; j < kT; ++j) {
+      const int gn = n0 + tc * kT + j;
       if (gn < Nout) out[static_cast<int64_t>(gr) * ldo + gn] = from_f<T>(static_cast<float>(acc[i][j]));
     }
   }
@@ -184,6 +194,7 @@ __global__ void __launch_bounds__(128) simt_gram_kernel(const T* __restrict__ D,
     const int st = tb.slot_list(i);
     const int lo = tb.st_lo(st), hi = tb.st_hi(st);
     const int64_t row0 = static_cast<int64_t>(tb.st_tile(st)) * LF_TILE_ROWS;
+#pragma unroll 4
     for (int r = lo; r < hi; ++r) {
       const double d = (c < C) ? static_cast<double>(to_f(D[(row0 + r) * ldd + c])) : 0.0;
       const double* s = s_ext + (static_cast<int64_t>(st) * LF_TILE_ROWS + r) * R;
@@ -248,22 +259,22 @@ cudaError_t simt_gemm(int dtype, const void* P, int64_t ldp, const void* Q, int6
                       int Kred, const double* s_ext, const void* lpk, const Tables& tb, void* out, int64_t ldo,
                       const DropArgs& drop, cudaStream_t st) {
   if (T == 0 || Nout == 0) return cudaSuccess;
-  dim3 grid((Nout + SG_BN - 1) / SG_BN, (T + SG_BM - 1) / SG_BM);
-  switch (dtype) {
-    case LF_F32:
-      simt_gemm_kernel<float><<<grid, 256, 0, st>>>((const float*)P, ldp, (const float*)Q, qsn, qsk, T, Nout, Kred,
-                                                    s_ext, (const float*)lpk, tb, (float*)out, ldo, drop);
-      break;
-    case LF_BF16:
-      simt_gemm_kernel<__nv_bfloat16><<<grid, 256, 0, st>>>(
-          (const __nv_bfloat16*)P, ldp, (const __nv_bfloat16*)Q, qsn, qsk, T, Nout, Kred, s_ext,
-          (const __nv_bfloat16*)lpk, tb, (__nv_bfloat16*)out, ldo, drop);
-      break;
-    default:
-      simt_gemm_kernel<__half><<<grid, 256, 0, st>>>((const __half*)P, ldp, (const __half*)Q, qsn, qsk, T, Nout, Kred,
-                                                     s_ext, (const __half*)lpk, tb, (__half*)out, ldo, drop);
-      break;
-  }
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return e;
+  const bool large = static_cast<int64_t>((Nout + 63) / 64) * ((T + 63) / 64) >= sms;
+  const int side = large ? 64 : 16;
+  const dim3 grid((Nout + side - 1) / side, (T + side - 1) / side);
+  auto run = [&](auto zero) {
+    using E = decltype(zero);
+    auto* k = large ? simt_gemm_kernel<E, 64, 4, 16> : simt_gemm_kernel<E, 16, 1, 32>;
+    k<<<grid, SG_T, 0, st>>>(static_cast<const E*>(P), ldp, static_cast<const E*>(Q), qsn, qsk, T, Nout, Kred, s_ext,
+                             static_cast<const E*>(lpk), tb, static_cast<E*>(out), ldo, drop);
+  };
+  if (dtype == LF_F32) run(float{});
+  else if (dtype == LF_BF16) run(__nv_bfloat16{});
+  else run(__half{});
   return cudaGetLastError();
 }
 
