@@ -646,13 +646,13 @@ __global__ void __maxnreg__(80)
 
   if (tid == 0) {
     for (int s = 0; s < stages; ++s) {
-      mbar_init(&full[s], kMx4 ? 1 + kEpiWarps : 1);
+      mbar_init(&full[s], kMx4 ? 1 + kEpiWarps / 2 * sub : 1);
       mbar_init(&empty[s], 1);
     }
     if (kMx4)
       for (int i = 0; i < prm.slots; ++i) {
         mbar_init(&code_full[i], 1);
-        mbar_init(&code_empty[i], kEpiWarps);
+        mbar_init(&code_empty[i], kEpiWarps / 2);
       }
     mbar_init(&acc_bar, 1);
     mbar_init(&drain_bar, 1);
@@ -769,35 +769,60 @@ __global__ void __maxnreg__(80)
       s_on[i] = p.row_slot != nullptr && t0 + i < p.T && row_adapter(p, t0 + i, false) != kNoSlot;
     named_barrier(1, kEpiWarps * 32);
     if constexpr (kMx4) {
-      const int w = warp - 2, row = (w & 3) * 32 + lane, half = w >> 2;  // this lane's codes in a block
+      // Two groups of four warps take the blocks in turn, so that one decodes while the other waits or stores; where a
+      // stage has two blocks each has one of them.
+      const int w = warp - 2, row = (w & 3) * 32 + lane, group = w >> 2;
       const uint8_t* codes_at = ring + stages * stage_bytes;
-      int stage = 0, slot = 0, in = 0;  // in: the block's place in the stage
+      uint8_t* dst = ring + row * 128 + (sub == 2 ? group * block_bytes : 0);
+      int stage = sub == 2 ? 0 : group, slot = group;
       uint32_t phase = 0, slot_phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
-        if (!warp_wait_stage(&code_full[slot], slot_phase, &abort_flag, p.err, kErrTimeoutFull)) break;
-        uint4 codes;
-        uint32_t scale;
-        mx4_fetch(codes_at + slot * kMx4Block, row, half, codes, scale);
-        if (in == 0 && !warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty)) break;
-        mx4_store<T>(ring + stage * stage_bytes + in * block_bytes + row * 128, row, half, codes, scale);
-        if (++in == sub || kb + 1 == kb1) {
-          in = 0;
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&full[stage]);
-          if (++stage == stages) {
-            stage = 0;
-            phase ^= 1;
-          }
-        } else {
-          __syncwarp();
+      bool fine = true;
+      auto advance = [&]() {
+        stage += sub == 2 ? 1 : 2;
+        if (stage >= stages) {
+          stage -= stages;
+          phase ^= 1;
         }
-        if (lane == 0) mbar_arrive(&code_empty[slot]);
-        if (++slot == prm.slots) {
-          slot = 0;
+      };
+      // A wait on a slot must not come while the slot's use before is still on its way (the phases' parity would match the
+      // one before that).  That use was another group's: it is over once this group's last stage, two blocks ago, was free
+      // of what it held before, if there are enough slots, or once this block's stage is (rows_tc has the sizes).
+      constexpr bool kStageFirst = kTN == 256;
+      for (int kb = kb0 + group; kb < kb1; kb += 2) {
+        if (kStageFirst) {
+          fine = warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
+          if (!fine) break;
+        }
+        fine = warp_wait_stage(&code_full[slot], slot_phase, &abort_flag, p.err, kErrTimeoutFull);
+        if (!fine) break;
+        uint4 codes[2], v[8];
+        uint32_t scale[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) mx4_fetch(codes_at + slot * kMx4Block, row, c, codes[c], scale[c]);
+        mx4_decode<T>(codes, scale, v);
+        if (!kStageFirst) {
+          fine = warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty);
+          if (!fine) break;
+        }
+#pragma unroll
+        for (int g = 0; g < 8; ++g) *reinterpret_cast<uint4*>(dst + stage * stage_bytes + ((g ^ (row & 7)) << 4)) = v[g];
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&full[stage]);
+          mbar_arrive(&code_empty[slot]);
+        }
+        advance();
+        slot += 2;
+        if (slot >= prm.slots) {
+          slot -= prm.slots;
           slot_phase ^= 1;
         }
       }
+      // a last stage with one block
+      if (fine && sub == 2 && group == 1 && ((kb1 - kb0) & 1) &&
+          warp_wait_stage(&empty[stage], phase ^ 1, &abort_flag, p.err, kErrTimeoutEmpty) && lane == 0)
+        mbar_arrive(&full[stage]);
       __syncwarp();
     }
   }
@@ -1667,6 +1692,7 @@ cudaError_t rows_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, const CU
     g.stages = tn == 64 ? 2 : 3;
     g.slots = (room - g.stages * g.sub * block) / kMx4Block;
     if (g.slots > kMaxSlots) g.slots = kMaxSlots;
+    if (g.slots < (tn == 256 ? g.stages : g.sub * g.stages + 2)) return cudaErrorInvalidValue;  // see the decoding loop
   }
   if (tn == 16) return launch_gemm<T, 16, kMx4>(g, w, x, st);
   if (tn == 32) return launch_gemm<T, 32, kMx4>(g, w, x, st);

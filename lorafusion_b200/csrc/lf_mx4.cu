@@ -38,15 +38,18 @@ __device__ __forceinline__ uint4 load8(const uint16_t* w, int n, int k, int N, i
   return v;
 }
 
-// Two codes, the nearest of each value with ties to the even code and 6 for what is larger, one in each half.
-__device__ __forceinline__ uint32_t encode2(float low, float high) {
+// Eight codes, the nearest of each value with ties to the even code and 6 for what is larger, value i in bits 4i .. 4i + 3.
+__device__ __forceinline__ uint32_t encode8(const float (&f)[8]) {
   uint32_t r;
-  asm("{\n\t.reg .b8 c;\n\t"
-      "cvt.rn.satfinite.e2m1x2.f32 c, %2, %1;\n\t"
-      "cvt.u32.u8 %0, c;\n\t}"
+  asm("{\n\t.reg .b8 a, b, c, d;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 a, %2, %1;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 b, %4, %3;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 c, %6, %5;\n\t"
+      "cvt.rn.satfinite.e2m1x2.f32 d, %8, %7;\n\t"
+      "mov.b32 %0, {a, b, c, d};\n\t}"
       : "=r"(r)
-      : "f"(low), "f"(high));
-  return (r | r << 12) & 0x000f000fu;
+      : "f"(f[0]), "f"(f[1]), "f"(f[2]), "f"(f[3]), "f"(f[4]), "f"(f[5]), "f"(f[6]), "f"(f[7]));
+  return r;
 }
 
 template <typename T>
@@ -67,15 +70,13 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const uint16_t* 
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const uint32_t word[4] = {v[c].x, v[c].y, v[c].z, v[c].w};
-      float f[8];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[2 * i] = to_f<T>(word[i] & 0xffffu), f[2 * i + 1] = to_f<T>(word[i] >> 16);
-      uint32_t top = 0;  // magnitudes compare as whole numbers; infinities and NaN are the largest
-#pragma unroll
-      for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(f[i]) & 0x7fffffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const uint32_t e = top >> 23;  // floor(log2) + 127; 0 of a zero and of float32's subnormals (bf16 has them)
+      // magnitudes compare as whole numbers; infinities and NaN are the largest
+      uint32_t top = __vmaxu2(__vmaxu2(word[0] & 0x7fff7fffu, word[1] & 0x7fff7fffu),
+                                   __vmaxu2(word[2] & 0x7fff7fffu, word[3] & 0x7fff7fffu));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = __vmaxu2(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      top = max(top & 0xffffu, top >> 16);
+      const uint32_t e = __float_as_uint(to_f<T>(top)) >> 23;  // floor(log2) + 127; 0 of a zero and of bf16's subnormals
       const bool bad = e == 255u;
       // E = floor(log2) - 2, at least -127; float16's blocks of zeros get the smallest scale that its other blocks have
       constexpr uint32_t kLeast = std::is_same_v<T, __half> ? 101u : 0u;
@@ -83,8 +84,10 @@ __global__ void __launch_bounds__(kThreads) mx4_quantize_kernel(const uint16_t* 
       const float up = __uint_as_float((254u - (bad ? 127u : s)) << 23);  // 2^-E
       uint32_t code = 0;
       if (!bad) {
-        code = Mx4<T>::word(encode2(f[0] * up, f[1] * up), encode2(f[2] * up, f[3] * up), encode2(f[4] * up, f[5] * up),
-                            encode2(f[6] * up, f[7] * up));
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[2 * i] = to_f<T>(word[i] & 0xffffu) * up, f[2 * i + 1] = to_f<T>(word[i] >> 16) * up;
+        code = Mx4<T>::word(encode8(f));
       }
       uint8_t* b = blocks + (c >> 1) * kMx4Block;
       *reinterpret_cast<uint32_t*>(b + mx4_code_at(r, c & 1) + j * 4) = code;

@@ -37,16 +37,23 @@ __host__ __device__ inline int mx4_col_blocks(int K) { return (K + 127) / 128 * 
 // values (codes in order took 15, and a byte table by permutes as many; the decoding warps of the CTA-pair GEMM are bound by
 // what they issue).  Where the factor leaves the type's range, scales above 1 and NaN, the two powers are applied one
 // after the other.
+__device__ __forceinline__ void mx4_pairs(uint32_t codes, uint32_t& a, uint32_t& b) {
+  const uint32_t even = codes & 0x0f0f0f0fu, odd = (codes >> 4) & 0x0f0f0f0fu;
+  a = __byte_perm(even, odd, 0x5410);
+  b = __byte_perm(even, odd, 0x7632);
+}
 template <typename T>
 struct Mx4;
 template <>
 struct Mx4<__nv_bfloat16> {
   static constexpr uint32_t kMask = 0x81c081c0u, kSign = 0x80008000u;
-  // the word of four registers of code pairs (element 2p in the low half, 2p + 1 in the high half)
-  static __device__ __forceinline__ uint32_t word(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
-    return (v0 & 0x00080008u) << 12 | (v0 & 0x00070007u) << 6 | (v1 & 0x00080008u) << 9 | (v1 & 0x00070007u) << 3 |
-           (v2 & 0x00080008u) << 6 | (v2 & 0x00070007u) | (v3 & 0x00080008u) << 11 | (v3 & 0x00060006u) << 9 |
-           (v3 & 0x00010001u) << 13;
+  // the word of eight codes in order, four bits each
+  static __device__ __forceinline__ uint32_t word(uint32_t codes) {
+    uint32_t a, b;  // of each half: elements 0 and 2 (1 and 3), then 4 and 6 (5 and 7), a byte each
+    mx4_pairs(codes, a, b);
+    return (a & 0x00080008u) << 12 | (a & 0x00070007u) << 6 | (a & 0x08000800u) << 1 | (a & 0x07000700u) >> 5 |
+           (b & 0x00080008u) << 6 | (b & 0x00070007u) | (b & 0x08000800u) << 3 | (b & 0x06000600u) << 1 |
+           (b & 0x01000100u) << 5;
   }
   static __device__ __forceinline__ uint4 bits(uint32_t w) {
     uint4 r;
@@ -70,9 +77,11 @@ struct Mx4<__nv_bfloat16> {
 template <>
 struct Mx4<__half> {
   static constexpr uint32_t kMask = 0x8e008e00u, kSign = 0x80008000u;
-  static __device__ __forceinline__ uint32_t word(uint32_t v0, uint32_t v1, uint32_t v2, uint32_t v3) {
-    return (v0 & 0x00080008u) << 12 | (v0 & 0x00070007u) << 9 | (v1 & 0x00080008u) << 9 | (v1 & 0x00070007u) << 6 |
-           (v2 & 0x00080008u) << 11 | (v2 & 0x00070007u) << 3 | (v3 & 0x00080008u) << 10 | (v3 & 0x00070007u);
+  static __device__ __forceinline__ uint32_t word(uint32_t codes) {
+    uint32_t a, b;
+    mx4_pairs(codes, a, b);
+    return (a & 0x00080008u) << 12 | (a & 0x00070007u) << 9 | (a & 0x08000800u) << 1 | (a & 0x07000700u) >> 2 |
+           (b & 0x00080008u) << 11 | (b & 0x00070007u) << 3 | (b & 0x08000800u) << 2 | (b & 0x07000700u) >> 8;
   }
   static __device__ __forceinline__ uint4 bits(uint32_t w) {
     constexpr uint32_t kMag = 0x0e000e00u;
@@ -120,7 +129,7 @@ __device__ __forceinline__ void mx4_fetch(const uint8_t* stage, int r, int c, ui
   codes = *reinterpret_cast<const uint4*>(stage + mx4_code_at(r, c));
   scale = stage[mx4_scale_at(r, c)];
 }
-// Both halves of a row, 64 values, or one of them.
+// Both halves of a row, 64 values.
 template <typename T>
 __device__ __forceinline__ void mx4_decode(const uint4 (&codes)[2], const uint32_t (&scale)[2], uint4 (&v)[8]) {
   const uint32_t w[2][4] = {{codes[0].x, codes[0].y, codes[0].z, codes[0].w}, {codes[1].x, codes[1].y, codes[1].z, codes[1].w}};
@@ -132,14 +141,4 @@ __device__ __forceinline__ void mx4_decode(const uint4 (&codes)[2], const uint32
     mx4_values<T, 4, false>(w[1], scale[1], v + 4);
   }
 }
-template <typename T>
-__device__ __forceinline__ void mx4_store(uint8_t* row, int r, int c, const uint4& codes, uint32_t scale) {
-  uint4 v[4];
-  const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-  if (Mx4<T>::one_factor(scale, scale)) mx4_values<T, 4, true>(w, scale, v);
-  else mx4_values<T, 4, false>(w, scale, v);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) *reinterpret_cast<uint4*>(row + (((4 * c + j) ^ (r & 7)) << 4)) = v[j];
-}
-
 }  // namespace lf

@@ -399,6 +399,9 @@ static_assert(kPairSmem <= 227 * 1024, "pair kernel shared memory");
 constexpr int kMx4Slots = 7;
 constexpr int kMx4PairStages = 5;
 constexpr int kMx4CodeBytes = kMx4Slots * kMx4Block;
+// A decoding group waits on a slot only once the slot's use before, another group's, is over: the stage that the group
+// filled two uses ago was free by then, so everything kMx4PairStages before that has been used.
+static_assert(kMx4Slots >= kMx4PairStages + 2, "a slot's parity is unambiguous");
 constexpr int kMx4BarBytes = 2 * kMx4Slots * 8;
 constexpr int kMx4PairSmem =
     1024 + kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes + kPairBarBytes + kPairEntBytes + kMx4BarBytes;

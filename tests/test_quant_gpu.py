@@ -163,6 +163,25 @@ def test_linear_many_rounds_and_split_tails():
     assert nat.device_error() == 0
 
 
+@pytest.mark.parametrize("T", [1, 20, 50, 100, 250, 600])
+def test_codes_that_come_late(T):
+    """The weight from memory, not from L2, many K blocks: loads arrive late and out of order."""
+    K, N = 4096, 1024
+    x, g = rand(T, K, seed=80), rand(T, N, seed=81)
+    q = quantize_weight(rand(N, K, seed=82, scale=K ** -0.5))
+    v = q.dequantize().double()
+    y, gx = mx4_linear(x, q), mx4_linear_backward(g, q)
+    check(y, x.double() @ v.t(), K * 2.0 ** -24 * (x.double().abs() @ v.abs().t()))
+    check(gx, g.double() @ v, N * 2.0 ** -24 * (g.double().abs() @ v.abs()))
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device=DEV)
+    for _ in range(20):
+        flush.fill_(0)
+        assert torch.equal(mx4_linear(x, q), y)
+        flush.fill_(1)
+        assert torch.equal(mx4_linear_backward(g, q), gx)
+    assert nat.device_error() == 0
+
+
 def test_linear_strided_misaligned_and_empty():
     q = quantize_weight(rand(256, 512, seed=14))
     x = rand(40, 1024, seed=15)
