@@ -1145,7 +1145,7 @@ extern "C" int lf_rows_forward(const lf_rows_problem* p, void* y_dev, void* work
           !make_map(&many->b, p->dtype, b_bank, 16, bank_rows / 16 * a.N, 32, 16, 256))
         return LF_ERR_UNSUPPORTED;
     }
-    if (rows_use_pairs(a.T, a.K, a.N, ds->num_sms)) {
+    if (mx4 ? mx4_use_pairs(a.T, a.N, ds->num_sms) : rows_use_pairs(a.T, a.K, a.N, ds->num_sms)) {
       TcMaps maps;
       if (!make_map(&maps.p, p->dtype, a.x, a.K, a.T, x_pitch, 64, 128) ||
           (!mx4 && !make_map(&maps.q, p->dtype, a.w, a.K, a.N, w_pitch, 64, 128)) ||
@@ -1251,7 +1251,7 @@ extern "C" int lf_mx4_linear(const lf_mx4_problem* p, void* out_dev, void* works
   }
   const PairMx4 mx4 = mx4_view(p->mx4_dev, N, K);
   const uint64_t pitch = static_cast<uint64_t>(p->ld) * 2;
-  if (!p->transpose && T <= kRowsChunk && !rows_use_pairs(T, K, N, ds->num_sms)) {
+  if (!p->transpose && !mx4_use_pairs(T, N, ds->num_sms)) {
     RowsArgs a{};
     a.x = p->in_dev;
     a.y = out_dev;

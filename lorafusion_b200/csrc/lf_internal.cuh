@@ -233,6 +233,7 @@ cudaError_t rows_forward_tc(const RowsArgs& a, int dtype, const CUtensorMap& w, 
 // The adapters' part alone (a.delta, a.eff), for a GEMM that adds it: tc_gemm_pair's `delta`.
 cudaError_t rows_lora_part(const RowsArgs& a, int dtype, const ManyMaps* m, int num_sms, cudaStream_t st);
 bool rows_use_pairs(int T, int K, int N, int num_sms);
+bool mx4_use_pairs(int T, int N, int num_sms);  // the same for a weight in 4 bits
 struct BankLoad {
   const void *a, *b;  // [rank][lda], [N][ldb]
   void *a_out, *b_out;

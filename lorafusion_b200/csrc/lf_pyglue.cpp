@@ -160,6 +160,54 @@ PyObject* mx4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(y));
 }
 
+// mx4_quantize(weight, dtype code): the data of a weight in 4 bits, on an operand that needs no copy.  None otherwise.
+PyObject* mx4_quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 2) {
+    PyErr_SetString(PyExc_TypeError, "mx4_quantize takes 2 arguments");
+    return nullptr;
+  }
+  const at::Tensor* wt = cuda_tensor(a[0]);
+  const long code = PyLong_AsLong(a[1]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!wt || wt->dim() != 2 || dtype_code(wt->scalar_type()) != code) Py_RETURN_NONE;
+  const at::Tensor& w = *wt;
+  const int64_t N = w.size(0), K = w.size(1), ld = w.is_contiguous() ? K : w.stride(0);
+  if (N < 1 || K < 1 || N > (1 << 24) || K > (1 << 24) || (!w.is_contiguous() && (w.stride(1) != 1 || ld < K)))
+    Py_RETURN_NONE;
+  const auto dev = w.device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  const int64_t bytes = static_cast<int64_t>(lf_mx4_bytes(static_cast<int32_t>(N), static_cast<int32_t>(K)));
+  at::Tensor data = at::detail::empty_cuda({bytes}, at::kByte, dev, std::nullopt);
+  const int rc = lf_mx4_quantize(static_cast<int32_t>(code), w.const_data_ptr(), static_cast<int32_t>(N),
+                                 static_cast<int32_t>(K), ld, data.data_ptr(),
+                                 c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (rc != LF_OK) return fail(rc, "lf_mx4_quantize");
+  return THPVariable_Wrap(std::move(data));
+}
+
+// mx4_dequantize(data, out_features, in_features, dtype code): the dense weight.
+PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 4) {
+    PyErr_SetString(PyExc_TypeError, "mx4_dequantize takes 4 arguments");
+    return nullptr;
+  }
+  const at::Tensor* dt = cuda_tensor(a[0]);
+  const long N = PyLong_AsLong(a[1]), K = PyLong_AsLong(a[2]), code = PyLong_AsLong(a[3]);
+  if (PyErr_Occurred()) return nullptr;
+  if (!dt || (code != LF_BF16 && code != LF_F16)) {
+    PyErr_SetString(PyExc_ValueError, "mx4_dequantize: not the data of a weight in 4 bits");
+    return nullptr;
+  }
+  const auto dev = dt->device();
+  const c10::cuda::OptionalCUDAGuard guard(dev);
+  at::Tensor w = at::detail::empty_cuda({N, K}, code == LF_BF16 ? at::kBFloat16 : at::kHalf, dev, std::nullopt);
+  const int rc = lf_mx4_dequantize(static_cast<int32_t>(code), dt->const_data_ptr(), static_cast<int32_t>(N),
+                                   static_cast<int32_t>(K), w.data_ptr(),
+                                   c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  if (rc != LF_OK) return fail(rc, "lf_mx4_dequantize");
+  return THPVariable_Wrap(std::move(w));
+}
+
 // bank_load(bank_a, bank_b, ranks, scales, slot, lora_a, lora_b, scaling): an adapter into its slot.  None unless its
 // tensors have the bank's dtype and device and dense rows; shapes were checked by the caller.
 PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -435,6 +483,8 @@ PyObject* guarded(PyObject* self, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"rows_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<rows_forward>)), METH_FASTCALL, nullptr},
     {"mx4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_linear>)), METH_FASTCALL, nullptr},
+    {"mx4_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_quantize>)), METH_FASTCALL, nullptr},
+    {"mx4_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_dequantize>)), METH_FASTCALL, nullptr},
     {"bank_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<bank_load>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},
     {"gather_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<gather_step>)), METH_FASTCALL, nullptr},

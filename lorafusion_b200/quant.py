@@ -64,13 +64,7 @@ class MX4Weight:
 
     def dequantize(self) -> torch.Tensor:
         """The values that the codes stand for, dense ``[out_features, in_features]`` in ``dtype``."""
-        device = self.device
-        out = torch.empty(self.shape, dtype=self.dtype, device=device)
-        with nat.on_device(device.index):
-            rc = nat.lib().lf_mx4_dequantize(_CODE[self.dtype], self.data.data_ptr(), self.out_features,
-                                             self.in_features, out.data_ptr(), nat.raw_stream(device.index))
-        nat.check(rc, "lf_mx4_dequantize")
-        return out
+        return nat.glue().mx4_dequantize(self.data, self.out_features, self.in_features, _CODE[self.dtype])
 
     def __repr__(self) -> str:
         return (f"MX4Weight(out_features={self.out_features}, in_features={self.in_features}, dtype={self.dtype}, "
@@ -82,29 +76,20 @@ def quantize_weight(weight: torch.Tensor) -> MX4Weight:
 
     One launch on the current stream of its device; nothing is read back.
     """
-    if weight.dim() != 2 or 0 in weight.shape or max(weight.shape) > _MAX:
-        raise ValueError(f"weight must be 2-D with sizes 1 .. {_MAX}, got shape {tuple(weight.shape)}")
-    if weight.device.type != "cuda":
-        raise ValueError("weight must be a CUDA tensor: lorafusion_b200 has no CPU path")
-    if weight.dtype not in _CODE:
-        raise ValueError(f"weight must be bfloat16 or float16 (convert a {weight.dtype} one to the activations' dtype "
-                         "first)")
-    weight = weight.detach()
-    N, K = weight.shape
-    if weight.is_contiguous():
-        ld = K
-    else:
-        ld = weight.stride(0)
-        if weight.stride(1) != 1 or ld < K:
-            weight, ld = weight.contiguous(), K
-    device = weight.device
-    L = nat.lib()
-    data = torch.empty(L.lf_mx4_bytes(N, K), dtype=torch.uint8, device=device)
-    with nat.on_device(device.index):
-        rc = L.lf_mx4_quantize(_CODE[weight.dtype], weight.data_ptr(), N, K, ld, data.data_ptr(),
-                               nat.raw_stream(device.index))
-    nat.check(rc, "lf_mx4_quantize")
-    return MX4Weight(data, N, K, weight.dtype)
+    code = _CODE.get(weight.dtype)
+    data = nat.glue().mx4_quantize(weight, code) if code is not None else None
+    if data is None:  # a copy, or an error
+        if weight.dim() != 2 or 0 in weight.shape or max(weight.shape) > _MAX:
+            raise ValueError(f"weight must be 2-D with sizes 1 .. {_MAX}, got shape {tuple(weight.shape)}")
+        if weight.device.type != "cuda":
+            raise ValueError("weight must be a CUDA tensor: lorafusion_b200 has no CPU path")
+        if code is None:
+            raise ValueError(f"weight must be bfloat16 or float16 (convert a {weight.dtype} one to the activations' dtype "
+                             "first)")
+        data = nat.glue().mx4_quantize(weight.detach().contiguous(), code)
+    out = MX4Weight.__new__(MX4Weight)
+    out.data, (out.out_features, out.in_features), out.dtype = data, weight.shape, weight.dtype
+    return out
 
 
 def _product(x: torch.Tensor, weight: MX4Weight, transpose: bool, name: str) -> torch.Tensor:
