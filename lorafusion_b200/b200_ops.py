@@ -450,6 +450,7 @@ class _Drop:
                 plan.thresholds.pop(next(iter(plan.thresholds)))
             host = torch.tensor([self.thresholds[i] for i, _, _ in plan.vslots] or [0], dtype=torch.int32)
             table = plan.thresholds[self.thresholds] = host.to(device)
+            torch.cuda.current_stream(device).synchronize()  # calls on other streams find it there
         n = int(nat.lib().lf_dropout_scratch_bytes(ctypes.byref(prob), int(backward)))
         scratch = torch.empty(n, dtype=torch.uint8, device=device) if n else None
         return nat.Dropout(self.seed, self.offset, table.data_ptr(), scratch.data_ptr() if n else None, n), scratch
@@ -515,7 +516,7 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     tail = torch.empty(max(int(L.lf_forward_workspace_bytes(info, code)) - fixed, 256), dtype=torch.uint8,
                        device=device)
     prob = _problem(code, T, K, N, x, w, packs)
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = nat.raw_stream(device.index)
     planes = ctypes.c_int32(0)
     opt, keep = _options(mx4, drop, plan, prob, False, device)
     with nat.on_device(device.index):
@@ -671,7 +672,7 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     ws_bytes = L.lf_backward_workspace_bytes(ctypes.byref(info), code)
     ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=device)
     prob = _problem(code, T, K, N, x, w, packs)
-    stream = torch.cuda.current_stream(device).cuda_stream
+    stream = nat.raw_stream(device.index)
     saved = _saved_sf(x_in, rts, plan, aset) if dtype != torch.float32 and drop is None else None
     sf_ptr, sf_planes = (saved[0].data_ptr(), saved[1]) if saved is not None else (None, 0)
     # S_f from the forward on these inputs, when there was one: no second s x A^T shrink

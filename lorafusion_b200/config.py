@@ -102,8 +102,9 @@ class AdapterDropout:
             v = getattr(self, name)
             if isinstance(v, bool) or not isinstance(v, int) or not 0 <= v < 1 << 64:
                 raise ValueError(f"{name} must be a whole number 0 .. 2**64 - 1, got {v!r}")
-        for r in self.rates.values() if isinstance(self.rates, Mapping) else (self.rates,):
-            self._threshold(r)
+        many = isinstance(self.rates, Mapping)
+        thresholds = {a: self._threshold(r) for a, r in self.rates.items()} if many else self._threshold(self.rates)
+        object.__setattr__(self, "_thresholds", thresholds)  # the rates as they are now
 
     @staticmethod
     def _threshold(rate: float) -> int:
@@ -114,4 +115,5 @@ class AdapterDropout:
 
     def threshold(self, adapter_id: int) -> int:
         """65536 times the adapter's rate, a whole number (``KeyError`` for an adapter that the mapping lacks)."""
-        return self._threshold(self.rates[adapter_id] if isinstance(self.rates, Mapping) else self.rates)
+        t = self._thresholds
+        return t if type(t) is int else t[adapter_id]

@@ -785,7 +785,6 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
         if (!make_map(&x_map, dt, prob->x_dev, K, T, K * es, 64, 128) ||
             !make_map(&delta_map, LF_F32, delta, K, T, static_cast<uint64_t>(K) * 4, 32, 32))
           return LF_ERR_UNSUPPORTED;
-        e = tc_shrink(dt, p_g, bt_map, N, tb, s_b, ds->num_sms, st);
         PairShrink sh{};
         sh.n_pairs = spare;
         sh.job2 = sh.job2_only = true;
@@ -795,7 +794,9 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
         sh.s_ext2 = s_f;
         sh.K2 = K;
         sh.drop = opt.drop;
-        if (e == cudaSuccess && spare == 0) e = tc_shrink(dt, x_map, a_map, K, tb, s_f, ds->num_sms, st, &opt.drop, &p_x);
+        const bool two = spare == 0;
+        if (two) e = tc_shrink(dt, x_map, a_map, K, tb, s_f, ds->num_sms, st, &opt.drop, &p_x, true, false);
+        if (e == cudaSuccess) e = tc_shrink(dt, p_g, bt_map, N, tb, s_b, ds->num_sms, st, nullptr, nullptr, two, two);
         if (e == cudaSuccess) e = drop_expand(dt, sb_map, dx.l, delta_map, T, K, tb, opt.drop, ds->num_sms, st);
         if (e == cudaSuccess)
           e = tc_gemm_pair(dt, true, dx, T, K, N, false, tb, grad_x_dev, K, ds->num_sms, st, spare > 0 ? &sh : nullptr, nullptr,

@@ -117,6 +117,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  pdl_wait();  // S_b
 
   if (warp == 0) {
     int stage = 0;
@@ -284,8 +285,8 @@ cudaError_t drop_expand(int dtype, const CUtensorMap& s_map, const CUtensorMap& 
   const cudaError_t e =
       cudaFuncSetAttribute(drop_expand_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kExpandSmem);  // of this device
   if (e != cudaSuccess) return e;
-  drop_expand_kernel<<<p.units < num_sms ? p.units : num_sms, kExpandThreads, kExpandSmem, st>>>(s_map, l_map, delta_map, p);
-  return cudaGetLastError();
+  return launch(drop_expand_kernel, static_cast<unsigned>(p.units < num_sms ? p.units : num_sms), kExpandThreads, kExpandSmem,
+                st, true, s_map, l_map, delta_map, p);
 }
 
 }  // namespace lf

@@ -73,7 +73,9 @@ struct TcMaps {
 
 cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_map, int Kred, const Tables& tb,
                       void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop = nullptr,
-                      const CUtensorMap* masked = nullptr);  // `masked`: where the masked P goes (a map like p_map's)
+                      const CUtensorMap* masked = nullptr, bool two = false, bool beside = false);
+// (`masked`: where the masked P goes, a map like p_map's.  `two`: one of two shrinks in a row, `beside`: the second, which
+// starts beside the first and is done when both are.)
 cudaError_t tc_gemm(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                     const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st);
 // Same product with 256x256 tiles computed by CTA pairs (cta_group::2).  Maps: p box (64,128),

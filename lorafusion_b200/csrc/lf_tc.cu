@@ -1507,6 +1507,7 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
   int* seg_hi = seg_lo + 8;
   float* seg_scale = reinterpret_cast<float*>(seg_hi + 8);
   __shared__ uint64_t masked[kDrop ? kShrStages : 1];
+  pdl_launch_dependents();
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Tables& tb = prm.tb;
@@ -1733,6 +1734,7 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
     for (int e = threadIdx.x; e < kBM * r_pad; e += blockDim.x) zero[e] = cvt_out<OutT>(0.f);
   }
 
+  pdl_wait();  // launched beside another shrink: done when both are
   // keep this CTA's shared memory alive until every peer has read it
   cluster_sync_all();
   if (warp == 1) {
@@ -2653,13 +2655,16 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
 }
 
 cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_map, int Kred, const Tables& tb,
-                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop, const CUtensorMap* masked) {
+                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop, const CUtensorMap* masked, bool two, bool beside) {
   if (tb.n_units == 0) return cudaSuccess;
   const int nkb = (Kred + kBK - 1) / kBK;
   // split K across a cluster while every CTA still fits on the GPU at once (one per SM)
   // and each keeps at least four k-blocks
   int cluster = 1;
   while (cluster < kMaxShrCluster && tb.n_units * cluster * 2 <= num_sms && nkb >= 4 * cluster * 2) cluster *= 2;
+  // Two shrinks in flight fill the SMs that one leaves: finer pieces pack better (8192 rows, 90 units each: one after the other
+  // 93 us, together and in halves of K 62).
+  if (two && cluster == 1 && nkb >= 8) cluster = 2;
   ShrinkParams p{};
   p.s_ext = s_ext;
   p.plane_elems = static_cast<int64_t>(tb.n_segtiles + 1) * kBM * tb.r_pad;
@@ -2674,13 +2679,15 @@ cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = kShrSmem;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = cluster;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = beside ? 2 : 1;
   cudaError_t e;
   auto start = [&](auto* kernel) {
     e = ensure_smem(kernel, kShrSmem);
