@@ -10,7 +10,7 @@ import numpy as np
 import pytest
 import torch
 
-from dropout_oracle import kept
+from oracle.dropout_oracle import kept
 from lorafusion_b200 import _native as nat
 from lorafusion_b200 import b200_ops
 from lorafusion_b200.b200_ops import fused_lora_backward, fused_lora_forward

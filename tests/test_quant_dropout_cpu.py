@@ -5,7 +5,7 @@ import ctypes
 import pytest
 import torch
 
-from dropout_oracle import kept, philox
+from oracle.dropout_oracle import kept, philox
 from lorafusion_b200 import _native as nat
 from lorafusion_b200.config import AdapterDropout
 from lorafusion_b200.quant import MX4Weight, mx4_linear, quantize_weight
