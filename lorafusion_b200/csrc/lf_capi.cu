@@ -284,7 +284,7 @@ namespace {
 // What lf_options asks for, checked.
 struct Options {
   bool mx4 = false;
-  DropArgs drop{0, 0, nullptr};
+  DropArgs drop{};
   char* scratch = nullptr;  // dropout's, and its size
   size_t scratch_bytes = 0;
 };
@@ -300,7 +300,12 @@ int read_options(const lf_options* opt, const lf_problem* prob, const lf_plan_in
   if (!d || info->n_slots == 0 || info->n_segtiles == 0) return LF_OK;
   if (!d->slot_threshold_dev) return LF_ERR_INVALID_ARG;
   if (!aligned16(d->scratch_dev)) return LF_ERR_INVALID_ARG;
-  out->drop = DropArgs{d->seed, d->offset, d->slot_threshold_dev};
+  out->drop.offset = d->offset;
+  out->drop.threshold = d->slot_threshold_dev;
+  for (uint32_t i = 0; i < 10; ++i) {
+    out->drop.key[2 * i] = static_cast<uint32_t>(d->seed) + i * 0x9E3779B9u;
+    out->drop.key[2 * i + 1] = static_cast<uint32_t>(d->seed >> 32) + i * 0xBB67AE85u;
+  }
   out->scratch = static_cast<char*>(d->scratch_dev);
   out->scratch_bytes = d->scratch_dev ? d->scratch_bytes : 0;
   return LF_OK;

@@ -25,7 +25,7 @@ __global__ void __launch_bounds__(kThreads) drop_mask_kernel(const uint8_t* __re
   const uint8_t* xr = x + t * K * kB;
   uint8_t* o = out + t * K * kB;
   for (int g = lane; g * 8 < K; g += 32) {
-    const uint4 r = philox(static_cast<uint32_t>(g), static_cast<uint32_t>(t), d.offset, d.seed);
+    const uint4 r = philox(static_cast<uint32_t>(g), static_cast<uint32_t>(t), d);
     const uint32_t word[4] = {r.x, r.y, r.z, r.w};
     if (vec) {  // rows of whole 16-byte pieces
       if (kB == 2) {
@@ -208,7 +208,7 @@ __global__ void __launch_bounds__(kExpandThreads, 1)
         uint4 r[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) ctr[j] = static_cast<uint32_t>((c0 + c) / 8 + j);
-        philox<4>(ctr, static_cast<uint32_t>(tile * LF_TILE_ROWS + row), prm.drop.offset, prm.drop.seed, r);
+        philox<4>(ctr, static_cast<uint32_t>(tile * LF_TILE_ROWS + row), prm.drop, r);
         tmem_wait_ld();
         if (c == 96) {  // accumulator fully read
           tc_fence_before();

@@ -16,27 +16,24 @@ namespace lf {
 // Numbers of N counters (c0[i], c1), round by round: 76 cycles of an SM quarter's issue a counter and warp, 97 where one
 // counter's ten dependent rounds are all a warp has to do.
 template <int N>
-__device__ __forceinline__ void philox(const uint32_t (&c0)[N], uint32_t c1, uint64_t offset, uint64_t seed, uint4 (&r)[N]) {
-  uint32_t k0 = static_cast<uint32_t>(seed), k1 = static_cast<uint32_t>(seed >> 32);
+__device__ __forceinline__ void philox(const uint32_t (&c0)[N], uint32_t c1, const DropArgs& d, uint4 (&r)[N]) {
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    r[j] = make_uint4(c0[j], c1, static_cast<uint32_t>(offset), static_cast<uint32_t>(offset >> 32));
+    r[j] = make_uint4(c0[j], c1, static_cast<uint32_t>(d.offset), static_cast<uint32_t>(d.offset >> 32));
 #pragma unroll
   for (int i = 0; i < 10; ++i) {
 #pragma unroll
     for (int j = 0; j < N; ++j) {
       const uint64_t a = static_cast<uint64_t>(r[j].x) * 0xD2511F53u, b = static_cast<uint64_t>(r[j].z) * 0xCD9E8D57u;
-      r[j] = make_uint4(static_cast<uint32_t>(b >> 32) ^ r[j].y ^ k0, static_cast<uint32_t>(b),
-                        static_cast<uint32_t>(a >> 32) ^ r[j].w ^ k1, static_cast<uint32_t>(a));
+      r[j] = make_uint4(static_cast<uint32_t>(b >> 32) ^ r[j].y ^ d.key[2 * i], static_cast<uint32_t>(b),
+                        static_cast<uint32_t>(a >> 32) ^ r[j].w ^ d.key[2 * i + 1], static_cast<uint32_t>(a));
     }
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
   }
 }
-__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, uint64_t offset, uint64_t seed) {
+__device__ __forceinline__ uint4 philox(uint32_t c0, uint32_t c1, const DropArgs& d) {
   const uint32_t c[1] = {c0};
   uint4 r[1];
-  philox<1>(c, c1, offset, seed, r);
+  philox<1>(c, c1, d, r);
   return r[0];
 }
 
@@ -70,7 +67,7 @@ __device__ __forceinline__ void mask_granules(uint8_t* tile, int row, int first,
     c[j] = static_cast<uint32_t>(kb * 8 + first + j);
     v[j] = *reinterpret_cast<const uint4*>(tile + row * 128 + (((first + j) ^ (row & 7)) << 4));
   }
-  philox<N>(c, t, d.offset, d.seed, r);
+  philox<N>(c, t, d, r);
 #pragma unroll
   for (int j = 0; j < N; ++j) {
     v[j].x = keep2(v[j].x, r[j].x, high), v[j].y = keep2(v[j].y, r[j].y, high);

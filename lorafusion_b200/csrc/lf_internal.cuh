@@ -42,8 +42,9 @@ struct Tables {
 
 // Dropout in front of the adapters (lf_drop.cuh).
 struct DropArgs {
-  uint64_t seed, offset;
+  uint64_t offset;
   const uint32_t* threshold;  // [n_slots] 65536 times the rate of each virtual slot, on the device; null: no dropout
+  uint32_t key[20];           // the generator's round keys, both halves of the seed round by round
 };
 
 Tables make_tables(const lf_plan_info* info, const int32_t* table_dev);

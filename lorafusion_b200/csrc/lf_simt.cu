@@ -155,7 +155,7 @@ __global__ void __launch_bounds__(SG_T) simt_gemm_kernel(const T* __restrict__ P
           const int gn = n0 + tc * kT + j;
           if (gn >= Nout) continue;
           if (drop.threshold != nullptr) {
-            const uint4 r = philox(static_cast<uint32_t>(gn >> 3), static_cast<uint32_t>(gr), drop.offset, drop.seed);
+            const uint4 r = philox(static_cast<uint32_t>(gn >> 3), static_cast<uint32_t>(gr), drop);
             const uint32_t w = (gn & 4) ? ((gn & 2) ? r.w : r.z) : ((gn & 2) ? r.y : r.x);
             if (((gn & 1) ? w >> 16 : w & 0xffffu) < drop.threshold[tb.st_slot(st)]) continue;
           }
