@@ -63,8 +63,8 @@ __global__ void __launch_bounds__(kThreads) drop_mask_kernel(const uint8_t* __re
 // 256 rows of A_i^T [K, r_pad]; warp 1 issues the MMAs into one of two accumulators; eight warps mask 32 rows x 128
 // columns each and store them through shared memory.  A lane has a row, so eight columns are one counter's numbers.
 // The rank is short: what bounds it is the 4 T K bytes written, with the generator (1.3 us a unit of 2.9 us at the copy
-// rate) behind them.  (With warp-level MMAs that read both operands where they lie: 61 us at 4096 x 4096, rank 16, and 220 at
-// 8192 rows and rank 64, bound by L1.)
+// rate) behind them.  4096 x 4096 with rank 16 takes 23 us, 8192 rows with rank 64 36 (profiler, cold caches).  (With
+// warp-level MMAs that read both operands where they lie: 61 and 220, bound by L1.)
 constexpr int kExpandCols = 256;
 constexpr int kExpandThreads = 320;
 constexpr int kExpandRing = 128 * 1024;

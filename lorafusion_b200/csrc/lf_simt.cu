@@ -80,7 +80,7 @@ __global__ void __launch_bounds__(256) simt_shrink_kernel(const T* __restrict__ 
 // kB x kB output tile, 256 threads, kT x kT per thread, K chunks of kK.  Each result is one chain of fused multiply-adds
 // along K in float64, whatever the tile.  The next chunk is on its way while one is used, and operands are converted once, on
 // their way into shared memory (13 conversions a cycle and SM, 62 multiply-adds).  Tiles of 64 where they give
-// every SM one, else of 16: 128 x 256 -> 256 in float32 took 60 us with 8 tiles of 64, now 12.
+// every SM one, else of 16: 128 x 256 -> 256 in float32 took 99 us with 8 tiles of 64, converted at every use, now 12.
 constexpr int SG_T = 256;
 
 template <typename T, int kB, int kT, int kK>
@@ -179,11 +179,14 @@ __global__ void __launch_bounds__(SG_T) simt_gemm_kernel(const T* __restrict__ P
   }
 }
 
-// One thread per output column c of one slot; accumulators over the padded rank.  O: output type.
+// One thread per output column c of one slot; accumulators over the padded rank, each one chain along the rows.  O: output
+// type.  Rows come in chunks, all loads of a chunk in flight at once (one row after the other took 1.4 us a row).
+constexpr int kGramRows = 16;
 template <typename T, typename O, int R>
 __global__ void __launch_bounds__(128) simt_gram_kernel(const T* __restrict__ D, int64_t ldd, int C,
                                                         const double* __restrict__ s_ext, Tables tb,
                                                         O* __restrict__ out, int transpose_out) {
+  __shared__ double s_rows[kGramRows * R];
   const int slot = blockIdx.x;
   const int c = blockIdx.y * 128 + threadIdx.x;
   double acc[R];
@@ -194,12 +197,22 @@ __global__ void __launch_bounds__(128) simt_gram_kernel(const T* __restrict__ D,
     const int st = tb.slot_list(i);
     const int lo = tb.st_lo(st), hi = tb.st_hi(st);
     const int64_t row0 = static_cast<int64_t>(tb.st_tile(st)) * LF_TILE_ROWS;
-#pragma unroll 4
-    for (int r = lo; r < hi; ++r) {
-      const double d = (c < C) ? static_cast<double>(to_f(D[(row0 + r) * ldd + c])) : 0.0;
-      const double* s = s_ext + (static_cast<int64_t>(st) * LF_TILE_ROWS + r) * R;
+    for (int r0 = lo; r0 < hi; r0 += kGramRows) {
+      T d[kGramRows];
 #pragma unroll
-      for (int j = 0; j < R; ++j) acc[j] = fma(d, s[j], acc[j]);
+      for (int q = 0; q < kGramRows; ++q)
+        d[q] = c < C && r0 + q < hi ? D[(row0 + r0 + q) * ldd + c] : from_f<T>(0.f);
+      const double* s = s_ext + (static_cast<int64_t>(st) * LF_TILE_ROWS + r0) * R;
+      __syncthreads();  // the chunk before has been used
+      for (int q = threadIdx.x; q < min(kGramRows, hi - r0) * R; q += 128) s_rows[q] = s[q];
+      __syncthreads();
+#pragma unroll
+      for (int q = 0; q < kGramRows; ++q) {
+        if (r0 + q >= hi) break;
+        const double dv = static_cast<double>(to_f(d[q]));
+#pragma unroll
+        for (int j = 0; j < R; ++j) acc[j] = fma(dv, s_rows[q * R + j], acc[j]);
+      }
     }
   }
   if (c >= C) return;

@@ -2662,8 +2662,8 @@ cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_
   // and each keeps at least four k-blocks
   int cluster = 1;
   while (cluster < kMaxShrCluster && tb.n_units * cluster * 2 <= num_sms && nkb >= 4 * cluster * 2) cluster *= 2;
-  // Two shrinks in flight fill the SMs that one leaves: finer pieces pack better (8192 rows, 90 units each: one after the other
-  // 93 us, together and in halves of K 62).
+  // Two shrinks in flight fill the SMs that one leaves, and finer pieces pack better (8192 rows, 90 units each: with them
+  // side by side and the launch behind them started early a backward took 431 us, else 457).
   if (two && cluster == 1 && nkb >= 8) cluster = 2;
   ShrinkParams p{};
   p.s_ext = s_ext;
