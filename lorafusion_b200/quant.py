@@ -29,7 +29,7 @@ _MAX = 1 << 24
 class MX4Weight:
     """A weight ``[out_features, in_features]`` in 4 bits, made by :func:`quantize_weight`.
 
-    ``data`` is its only tensor: uint8, in an order of its own, to be saved and restored as it is
+    ``data`` is its only tensor: uint8, in an order of its own that goes with ``dtype``, to be saved and restored as it is
     (``MX4Weight(data, out_features, in_features, dtype)``).  ``dtype`` (bfloat16 or float16) is that of the weight it was
     made from and of the activations it is multiplied with.  Its products read ``data`` on their stream: keep it
     unchanged until they have run.

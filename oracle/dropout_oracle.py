@@ -1,4 +1,8 @@
-"""Dropout's mask from the definition, in plain Python and numpy (no torch, nothing of the package)."""
+"""Dropout's mask from the definition, in plain Python and numpy (no torch, nothing of the package).
+
+No counterpart in the reference: the generator is Philox 4x32 with ten rounds (Salmon et al., 2011), pinned by the numbers its
+authors published (``tests/test_quant_dropout_cpu.py``).
+"""
 
 import numpy as np
 
@@ -6,7 +10,7 @@ M = 0xFFFFFFFF
 
 
 def philox(counter, key):
-    """Philox 4x32 with ten rounds of one counter of four words, in Python's whole numbers."""
+    """Ten rounds of one counter of four words, in Python's whole numbers."""
     c, k = list(counter), list(key)
     for _ in range(10):
         a, b = c[0] * 0xD2511F53, c[2] * 0xCD9E8D57
@@ -16,11 +20,19 @@ def philox(counter, key):
 
 
 def kept(rows, cols, thresholds, seed, offset):
-    """Truth values [rows, cols]; thresholds: one whole number a row."""
-    out = np.empty((rows, cols), dtype=bool)
-    for t in range(rows):
-        for g in range(-(-cols // 8)):
-            words = philox((g, t, offset & M, offset >> 32), (seed & M, seed >> 32))
-            for i in range(min(8, cols - 8 * g)):
-                out[t, 8 * g + i] = (words[i // 2] >> (16 * (i % 2)) & 0xFFFF) >= thresholds[t]
-    return out
+    """Truth values [rows, cols], which elements dropout keeps; thresholds: one whole number a row."""
+    groups = -(-cols // 8)
+    shape = (rows, groups)
+    c = [np.broadcast_to(np.arange(groups, dtype=np.uint64), shape),
+         np.broadcast_to(np.arange(rows, dtype=np.uint64)[:, None], shape),
+         np.full(shape, offset & M, dtype=np.uint64), np.full(shape, offset >> 32, dtype=np.uint64)]
+    low, half = np.uint64(M), np.uint64(32)
+    k = [seed & M, seed >> 32]
+    for _ in range(10):
+        a, b = c[0] * np.uint64(0xD2511F53), c[2] * np.uint64(0xCD9E8D57)
+        c = [(b >> half) ^ c[1] ^ np.uint64(k[0]), b & low, (a >> half) ^ c[3] ^ np.uint64(k[1]), a & low]
+        k = [(k[0] + 0x9E3779B9) & M, (k[1] + 0xBB67AE85) & M]
+    numbers = np.empty((*shape, 8), dtype=np.uint32)
+    for i, word in enumerate(c):
+        numbers[:, :, 2 * i], numbers[:, :, 2 * i + 1] = word & np.uint64(0xFFFF), word >> np.uint64(16)
+    return numbers.reshape(rows, -1)[:, :cols] >= np.asarray(thresholds, dtype=np.uint32)[:, None]

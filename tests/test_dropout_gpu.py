@@ -181,6 +181,64 @@ def test_co_scheduling_modes(mode):
         check(gb[i], rgb[i], f"dB {i}")
 
 
+@pytest.mark.parametrize("mx4", [False, True])
+@pytest.mark.parametrize("mode", [0, 1])
+def test_shrinks_beside_one_another(mode, mx4):
+    """More row tiles than half of the SMs and K blocks enough to cut: the backward's two shrinks share the GPU (mode 1: its
+    GEMM's rounds leave no pairs idle)."""
+    try:
+        nat.check(nat.lib().lf_set_co_scheduling(mode), "mode")
+        check_all(Problem(9400, 512, 576, [64, 20], [4000], [0.1, 0.3], BF16, mx4=mx4))
+    finally:
+        nat.lib().lf_set_co_scheduling(1)
+
+
+def test_rows_and_gradients_at_odd_addresses():
+    """Views of x and of the gradient that start in the middle of 16 bytes."""
+    p = Problem(150, 128, 192, [16], [], [0.2], BF16, mx4=True)
+    y, (gx, ga, gb) = p.forward(), p.backward()
+    for name in ("x", "g"):
+        t = getattr(p, name)
+        flat = torch.zeros(t.numel() + 1, dtype=BF16, device=DEV)
+        flat[1:] = t.reshape(-1)
+        setattr(p, name, flat[1:].view(t.shape))
+    assert torch.equal(p.forward(), y)
+    again = p.backward()
+    assert torch.equal(again[0], gx) and torch.equal(again[1][0], ga[0]) and torch.equal(again[2][0], gb[0])
+
+
+def test_two_streams_at_once():
+    """Calls of different masks, weights and sizes side by side give what each gives alone."""
+    ps = [Problem(700, 512, 640, [16, 8], [300], [0.1, 0.4], BF16, seed=i, mx4=bool(i)) for i in range(2)]
+    alone = [(p.forward(), p.backward()) for p in ps]
+    streams = [torch.cuda.Stream() for _ in ps]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(5):
+        for i, (p, s) in enumerate(zip(ps, streams)):
+            with torch.cuda.stream(s):
+                got[i].append((p.forward(), p.backward()))
+    torch.cuda.synchronize()
+    for i, calls in enumerate(got):
+        for y, (gx, ga, gb) in calls:
+            ry, (rgx, rga, rgb) = alone[i]
+            assert torch.equal(y, ry) and torch.equal(gx, rgx)
+            assert all(torch.equal(ga[k], rga[k]) and torch.equal(gb[k], rgb[k]) for k in rga)
+    assert nat.device_error() == 0
+
+
+def test_under_inference_mode_and_with_leaves():
+    """Operands that require gradients, or inference tensors: the same results, no graph."""
+    p = Problem(90, 64, 64, [8], [], [0.3], BF16, mx4=True)
+    y = p.forward()
+    p.x.requires_grad_(True)
+    again = p.forward()
+    assert torch.equal(again, y) and not again.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(p.forward(), y)
+
+
 def test_float32_gradients():
     p = Problem(300, 256, 128, [16, 8], [170], [0.2, 0.1], BF16)
     _, ga, gb = p.backward(grad_dtype=F32)

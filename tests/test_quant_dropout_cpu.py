@@ -16,6 +16,12 @@ def test_the_generator_gives_its_published_numbers():
     ones = 0xFFFFFFFF
     assert philox((ones,) * 4, (ones,) * 2) == [0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
     assert not kept(4, 9, [65536] * 4, 1, 2).any() and kept(4, 9, [0] * 4, 1, 2).all()
+    seed, offset, at = 0x123456789ABCDEF0, (7 << 32) + 5, [40000, 1, 65535]
+    got = kept(3, 21, at, seed, offset)
+    for t in range(3):
+        for k in range(21):
+            words = philox((k // 8, t, offset & ones, offset >> 32), (seed & ones, seed >> 32))
+            assert got[t, k] == ((words[k % 8 // 2] >> 16 * (k % 2) & 0xFFFF) >= at[t])
 
 
 @pytest.mark.parametrize("rate", [-0.1, 1.0, 1.5, float("nan"), 1 - 2.0 ** -18])

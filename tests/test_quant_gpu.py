@@ -409,6 +409,60 @@ def test_captured_fused_ops_follow_their_inputs(mx4):
     assert nat.device_error() == 0
 
 
+def test_a_wait_that_runs_out_reports_and_the_next_call_is_right():
+    """The co-scheduled launch over a weight in 4 bits waits for a shrink that never reports (the test hook)."""
+    T, K, N = 1024, 512, 768
+    q = quantize_weight(rand(N, K, seed=90, scale=K ** -0.5))
+    x = rand(T, K, seed=91)
+    a, b, specs = adapters_of(K, N, [16, 8], BF16)
+    routing = TileRoutingConfig(128, [TileRoute(0, 600, 0), TileRoute(600, T, 1)])
+    y = b200_ops.fused_lora_forward(x, q, a, b, specs, routing)
+    if b200_ops.last_launch_count() != 1:
+        pytest.skip("the shrink does not run inside the GEMM launch on this device")
+    assert nat.device_error() == 0
+    nat.set_wait_limit(50_000_000)
+    try:
+        nat.check(nat.lib().lf_inject_stale_ready(1), "lf_inject_stale_ready")
+        b200_ops.fused_lora_forward(x, q, a, b, specs, routing)
+        assert nat.device_error() in (nat.ERR_TIMEOUT_FULL, nat.ERR_TIMEOUT_EMPTY, nat.ERR_TIMEOUT_ACC,
+                                      nat.ERR_TIMEOUT_DRAIN, nat.ERR_TIMEOUT_FLAG)
+    finally:
+        nat.check(nat.lib().lf_inject_stale_ready(0), "lf_inject_stale_ready")
+        nat.set_wait_limit(0)
+    assert torch.equal(b200_ops.fused_lora_forward(x, q, a, b, specs, routing), y)
+    assert nat.device_error() == 0
+
+
+def test_random_sizes():
+    rng = np.random.default_rng(92)
+    for i in range(40):
+        T, K, N = int(2 ** rng.uniform(0, 11)), 8 * int(2 ** rng.uniform(0, 8)), 8 * int(2 ** rng.uniform(0, 8))
+        dtype = BF16 if i % 2 else F16
+        q = quantize_weight(rand(N, K, seed=93 + i, scale=K ** -0.5, dtype=dtype))
+        v = q.dequantize().double()
+        x, g = rand(T, K, seed=200 + i, dtype=dtype), rand(T, N, seed=300 + i, dtype=dtype)
+        check(mx4_linear(x, q), x.double() @ v.t(), K * 2.0 ** -24 * (x.double().abs() @ v.abs().t()))
+        check(mx4_linear_backward(g, q), g.double() @ v, N * 2.0 ** -24 * (g.double().abs() @ v.abs()))
+    assert nat.device_error() == 0
+
+
+def test_two_streams_at_once():
+    """Products of several sizes side by side give what each gives alone."""
+    qs = [quantize_weight(rand(n, 512, seed=95 + n)) for n in (1024, 264)]
+    xs = [rand(t, 512, seed=96 + t) for t in (900, 40)]
+    alone = [mx4_linear(x, q) for x, q in zip(xs, qs)]
+    streams = [torch.cuda.Stream() for _ in qs]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [[], []]
+    for _ in range(10):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(mx4_linear(xs[i], qs[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, alone[i]) for i in range(2) for y in got[i])
+
+
 def test_refusals():
     q = quantize_weight(rand(64, 128, seed=60))
     x = rand(4, 128, seed=61)
