@@ -591,12 +591,12 @@ typedef struct lf_options {
   const lf_dropout* dropout;  /* null: none */
 } lf_options;
 
-/* lf_forward_sf with options (null: none).  A backward may take S_f from a forward with the same options only. */
+/* lf_forward_sf with options (null: none).  S_f of a forward with dropout is not for a backward. */
 LF_API int lf_forward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
                           const lf_options* options, void* y_dev, void* workspace_dev, size_t workspace_bytes,
                           void* tail_dev, size_t tail_bytes, int32_t* s_f_planes, lf_stream_t stream);
 
-/* lf_backward_ex, or lf_backward_peer with `peer`, with options (null: none). */
+/* lf_backward_ex, or lf_backward_peer with `peer`, with options (null: none).  With dropout s_f_dev is null. */
 LF_API int lf_backward_opt(const lf_problem* prob, const lf_plan_info* info, const int32_t* table_dev,
                            const lf_options* options, const void* grad_out_dev, const void* s_f_dev, int32_t s_f_planes,
                            int32_t grad_ab_dtype, void* grad_x_dev, void* grad_a_dev, void* grad_b_dev,

@@ -86,11 +86,12 @@ class TileRoutingConfig:
 class AdapterDropout:
     """Dropout in front of the adapters of one fused call (no counterpart in the reference).
 
-    ``rates``: one rate for all adapters, or a mapping adapter id -> rate that names every adapter of the call; ``0 <= rate
-    < 1``, taken to the nearest multiple of 1/65536 (and then below 1; float16 calls take rates up to 63/64).  ``seed`` and ``offset``, ``0 .. 2**64 - 1``,
-    choose the mask: element ``(t, k)`` of ``x`` is dropped by a number that depends on seed, offset, ``t`` and ``k`` alone
-    (Philox 4x32-10), so the forward and the backward that get the same object agree on it and nothing of it is
-    stored.  Take another offset for every step and every projection whose mask should be its own.
+    ``rates``: one rate for all adapters, or a mapping adapter id -> rate that names every adapter of the call;
+    ``0 <= rate < 1``, taken to the nearest multiple of 1/65536 (and then below 1; float16 calls take rates up to
+    63/64).  ``seed`` and ``offset``, ``0 .. 2**64 - 1``, choose the mask: element ``(t, k)`` of ``x`` is dropped by a
+    number that depends on seed, offset, ``t`` and ``k`` alone (Philox 4x32-10), so the forward and the backward that
+    get the same object agree on it and nothing of it is stored.  Take another offset for every step and every
+    projection whose mask should be its own.
     """
 
     rates: float | Mapping[int, float]

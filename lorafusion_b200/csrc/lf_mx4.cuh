@@ -18,7 +18,7 @@
 
 namespace lf {
 
-constexpr int kMx4Rows = 128, kMx4Cols = 64;
+constexpr int kMx4Rows = 128;
 constexpr int kMx4HalfBytes = 64 * 16;                // codes of 64 rows x 32 columns
 constexpr int kMx4Codes = 2 * kMx4HalfBytes;          // where a piece's scales start
 constexpr int kMx4Piece = kMx4Codes + 2 * 64;         // 2176 bytes

@@ -403,12 +403,14 @@ constexpr int kMx4CodeBytes = kMx4Slots * kMx4Block;
 // filled two uses ago was free by then, so everything kMx4PairStages before that has been used.
 static_assert(kMx4Slots >= kMx4PairStages + 2, "a slot's parity is unambiguous");
 constexpr int kMx4BarBytes = 2 * kMx4Slots * 8;
-constexpr int kMx4PairSmem =
-    1024 + kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes + kPairBarBytes + kPairEntBytes + kMx4BarBytes;
+constexpr int kMx4PairSmem = 1024 + kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes +
+                             kPairBarBytes + kPairEntBytes + kMx4BarBytes;
 static_assert(kMx4PairSmem <= 227 * 1024, "pair kernel shared memory");
 static_assert(kRoleStages * kRoleStageBytes <= kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes,
               "shrink-role stages must fit");
-__host__ __device__ constexpr int pair_tail_share(bool mx4) { return (mx4 ? kMx4PairStages : kPairStages) * (kPairABytes + kPairBBytes) / 4; }
+__host__ __device__ constexpr int pair_tail_share(bool mx4) {  // of the ring, an epilogue warp's
+  return (mx4 ? kMx4PairStages : kPairStages) * (kPairABytes + kPairBBytes) / 4;
+}
 static_assert(pair_tail_share(false) == 2 * kTailBufBytes && pair_tail_share(true) >= 4 * kTailChunkBytes, "tail buffers");
 
 struct PairParams {
@@ -855,9 +857,11 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
 // for x V^T, for g V (kQMN) two panels of 64 columns by 64 rows.  The codes of a stage are two pieces that one more warp
 // copies into a ring of their own, kMx4Slots stages ahead.  (Loaded by the decoding warps themselves they were waited for
 // at every fence: 0.8 us a stage.)  Two groups of four warps take the stages in turn, so that one decodes while the
-// other waits or stores.  A warp decodes its rows, waits for the stage to be free, stores the values and reports to the even CTA's `full` barrier, whose phase also counts the P tiles' bytes; at CTA scope, since what the
-// even CTA's MMAs read of the odd CTA lies in that one's shared memory and was fenced there (released at cluster scope,
-// every stage waited 0.8 us for the release).  LoRA stages are filled by copies alone; the warps report them unseen.
+// other waits or stores.  A warp decodes its rows, waits for the stage to be free, stores the values and reports to the
+// even CTA's `full` barrier, whose phase also counts the P tiles' bytes; at CTA scope, since what the even CTA's MMAs read
+// of the odd CTA lies in that one's shared memory and was fenced there (released at cluster scope, every stage waited
+// 0.8 us for the release).  LoRA stages are filled by copies alone; the warps report them unseen.
+// 4096 x 4096 -> 4096 takes 119 us, the dense kernel 100; 101 without storing values, 109 storing the codes as they are.
 constexpr int kMx4Warps = 8;
 constexpr int kMx4Threads = kThreads + 32 * kMx4Warps + 32;
 
@@ -2582,7 +2586,8 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   cfg.gridDim = dim3(2 * (gemm_pairs + p.n_shrink_pairs));
   const bool drop = shrink != nullptr && shrink->drop.threshold != nullptr;
   if (drop) {
-    if (shrink->prologue || shrink->job2 != shrink->job2_only || (delta != nullptr) != shrink->job2_only) return cudaErrorInvalidValue;
+    if (shrink->prologue || shrink->job2 != shrink->job2_only || (delta != nullptr) != shrink->job2_only)
+      return cudaErrorInvalidValue;
     p.drop = shrink->drop;
     p.job2_only = shrink->job2_only ? 1 : 0;
   }
@@ -2655,7 +2660,8 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
 }
 
 cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_map, int Kred, const Tables& tb,
-                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop, const CUtensorMap* masked, bool two, bool beside) {
+                      void* s_ext, int num_sms, cudaStream_t st, const DropArgs* drop, const CUtensorMap* masked, bool two,
+                      bool beside) {
   if (tb.n_units == 0) return cudaSuccess;
   const int nkb = (Kred + kBK - 1) / kBK;
   // split K across a cluster while every CTA still fits on the GPU at once (one per SM)
