@@ -82,10 +82,12 @@ _CACHE_MAX = 256
 _last_launches = 0
 # S_f = s x A^T left by forwards, for a backward on the same inputs (what autograd would save as
 # the activation x A^T): (id(x), id(route record), id(adapter record)) -> (weakref x, x version,
-# route record, plan, adapter record, workspace, planes), least recently used first; entries whose
+# route record, plan, adapter record, workspace, planes, capture), least recently used first; entries whose
 # x has died are dropped on the next insertion
 _SAVED_SF: "OrderedDict[tuple, tuple]" = OrderedDict()
 _SAVED_MAX = 1024
+# (plan, packed slabs, base weight) of calls captured into CUDA graphs: the replays read them, whatever the caches drop
+_CAPTURED: list = []
 _VERSION = torch.Tensor._version.__get__
 _DATA_PTR = torch.Tensor.data_ptr
 
@@ -105,12 +107,14 @@ def use_cooperative_launch(enabled: bool, shrink_prologue: bool = False) -> None
 
 
 def clear_weight_cache() -> None:
-    """Drop every cached table, packed adapter slab and converted weight."""
+    """Drop every cached table, packed adapter slab and converted weight, those of captured calls too (their graphs must
+    not be replayed any more)."""
     _ROUTE_CACHE.clear()
     _ADAPTER_CACHE.clear()
     _PLAN_BY_CONTENT.clear()
     _SAVED_SF.clear()
     _WEIGHT_CACHE.clear()
+    _CAPTURED.clear()
 
 
 def release() -> None:
@@ -271,7 +275,11 @@ def _adapters(rts: _Routes, lora_a, lora_b, adapters) -> _AdapterSet:
     return rec
 
 
-def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, scales=None) -> _Plan:
+def _not_captured(what: str) -> RuntimeError:
+    return RuntimeError(f"{what} would be made within a CUDA graph capture: make the same call once before it")
+
+
+def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, scales=None, build=True) -> _Plan:
     ranks, scales = aset.ranks, aset.scales if scales is None else scales
     for pr, ps, pd, plan in rts.plans:
         if pd == device and pr == ranks and ps == scales:
@@ -284,6 +292,8 @@ def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device
                ranks, scales)
     plan = _PLAN_BY_CONTENT.get(content)
     if plan is None:
+        if not build:
+            raise _not_captured("the routing's tables")
         plan = _build_plan(rts, ranks, scales, total_rows, device)
         if len(_PLAN_BY_CONTENT) >= _CACHE_MAX:
             _PLAN_BY_CONTENT.clear()
@@ -299,10 +309,14 @@ def _build_plan(rts: _Routes, ranks, scales, total_rows: int, device) -> _Plan:
     return _Plan(info, table_dev, rts.slots, ranks)
 
 
-def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, backward: bool) -> dict:
+def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, backward: bool,
+          build=True) -> dict:
     """Zero-padded adapter slabs in the layouts the kernels read (cached in the adapter record)."""
     key = (dtype, K, N, device, plan.info.r_pad)
     entry = aset.packs.get(key)
+    want = ("a", "b", "bt", "at") if backward else ("a", "b")
+    if not build and (entry is None or any(w not in entry for w in want)):
+        raise _not_captured("the adapters' slabs")
     if entry is None:
         for aid, a, b, r in zip(plan.slots, aset.a, aset.b, plan.ranks):
             if a.dim() != 2 or a.shape[1] != K or b.dim() != 2 or b.shape != (N, r):
@@ -320,7 +334,6 @@ def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, de
             a_src.append(a if a.is_contiguous() else a.contiguous())
             b_src.append(b if b.is_contiguous() else b.contiguous())
         entry = aset.packs[key] = {"src": (a_src, b_src)}
-    want = ("a", "b", "bt", "at") if backward else ("a", "b")
     missing = [w for w in want if w not in entry]
     if missing:
         _fill_packs(entry, plan, dtype, K, N, device, missing)
@@ -361,7 +374,7 @@ def _fill_packs(entry, plan: _Plan, dtype, K, N, device, which) -> None:
         entry.setdefault("ptr_bufs", []).append((ptrs, ranks_dev))
 
 
-def _weight(base_weight: torch.Tensor, dtype, device) -> torch.Tensor:
+def _weight(base_weight: torch.Tensor, dtype, device, build=True) -> torch.Tensor:
     """Base weight as a contiguous tensor of the activation dtype (converted copies cached)."""
     if isinstance(base_weight, MX4Weight):
         raise ValueError("this call takes a dense base_weight (MX4Weight.dequantize)")
@@ -375,6 +388,8 @@ def _weight(base_weight: torch.Tensor, dtype, device) -> torch.Tensor:
         ref, ptr, ver, conv = hit
         if ref() is base_weight and ptr == base_weight.data_ptr() and ver == base_weight._version:
             return conv
+    if not build:
+        raise _not_captured("a copy of base_weight")
     conv = base_weight.to(dtype).contiguous()
     if len(_WEIGHT_CACHE) >= _CACHE_MAX:
         _WEIGHT_CACHE.clear()
@@ -408,11 +423,11 @@ def _problem(code, T, K, N, x, w, packs) -> nat.Problem:
     return p
 
 
-def _base(base_weight, x: torch.Tensor):
+def _base(base_weight, x: torch.Tensor, build=True):
     """(tensor that holds the base weight, whether it is the data of one in 4 bits).  A problem the tensor-core path
     cannot address takes a dense copy of a weight in 4 bits, made within the call."""
     if not isinstance(base_weight, MX4Weight):
-        return _weight(base_weight, x.dtype, x.device), False
+        return _weight(base_weight, x.dtype, x.device, build), False
     if base_weight.dtype is not x.dtype:
         raise ValueError(f"x ({x.dtype}) must have the dtype of the weight in 4 bits ({base_weight.dtype})")
     if base_weight.device != x.device:
@@ -442,10 +457,12 @@ class _Drop:
     def scales(self, scales):
         return tuple(s * (65536.0 / (65536 - t)) for s, t in zip(scales, self.thresholds))
 
-    def args(self, plan: _Plan, prob, backward: bool, device):
+    def args(self, plan: _Plan, prob, backward: bool, device, build=True):
         """lf_dropout, and what it points at."""
         table = plan.thresholds.get(self.thresholds)
         if table is None:
+            if not build:
+                raise _not_captured("the table of dropout thresholds")
             while len(plan.thresholds) >= 8:
                 plan.thresholds.pop(next(iter(plan.thresholds)))
             host = torch.tensor([self.thresholds[i] for i, _, _ in plan.vslots] or [0], dtype=torch.int32)
@@ -483,8 +500,9 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
 
     Two things have no counterpart in the reference.  ``base_weight`` may be a ``quant.MX4Weight`` of x's dtype
     and device.  ``dropout`` (keyword only) puts a mask in front of the adapters: ``y = x W^T + s_i / (1 - p_i) (m x)
-    A_i^T B_i^T``, a dropped element being zero whatever it was.  A call captured into a CUDA graph repeats its mask
-    in every replay.
+    A_i^T B_i^T``, a dropped element being zero whatever it was.  A call with either can be captured into a CUDA graph
+    once the same call has run (``RuntimeError`` before): replays read x and the base weight as they are then, repeat
+    the mask, and keep the adapters' values of the capture.
     """
     global _last_launches
     rts = _routes(routing, x.shape[0])
@@ -498,11 +516,13 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     code = _DTYPE_CODE[dtype]
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    w, mx4 = _base(base_weight, x)
+    # the capture into a CUDA graph that the call is part of, 0 for none
+    captured = nat.glue().capture_id(device.index) if drop is not None or isinstance(base_weight, MX4Weight) else 0
+    w, mx4 = _base(base_weight, x, not captured)
     if mx4 and x.data_ptr() % 16:
         x = x.detach().clone()
-    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
-    packs = _pack(plan, aset, dtype, K, N, device, backward=False)
+    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None, not captured)
+    packs = _pack(plan, aset, dtype, K, N, device, False, not captured)
     y = torch.empty((T, N), dtype=dtype, device=device)
     if T == 0 or N == 0:
         return y
@@ -518,7 +538,9 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     prob = _problem(code, T, K, N, x, w, packs)
     stream = nat.raw_stream(device.index)
     planes = ctypes.c_int32(0)
-    opt, keep = _options(mx4, drop, plan, prob, False, device)
+    opt, keep = _options(mx4, drop, plan, prob, False, device, not captured)
+    if captured:
+        _CAPTURED.append((plan, packs, w))
     with nat.on_device(device.index):
         rc = L.lf_forward_opt(ctypes.byref(prob), info, plan.table_dev.data_ptr(), opt, y.data_ptr(), ws.data_ptr(),
                               ws.numel(), tail.data_ptr(), tail.numel(), ctypes.byref(planes), stream)
@@ -528,23 +550,23 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     if drop is not None:
         _last_launches += planes.value == 0  # the masked copy on CUDA cores
     elif planes.value > 0 and plan.info.n_segtiles > 0:
-        _save_sf(x_in, rts, plan, aset, ws, planes.value)
+        _save_sf(x_in, rts, plan, aset, ws, planes.value, captured)
     return y
 
 
-def _options(mx4: bool, drop: _Drop | None, plan: _Plan, prob, backward: bool, device):
+def _options(mx4: bool, drop: _Drop | None, plan: _Plan, prob, backward: bool, device, build=True):
     """lf_options of a call (None for a plain one), and what must live until it is enqueued."""
     if not mx4 and drop is None:
         return None, None
     opt = nat.Options(nat.LF_WEIGHT_MX4 if mx4 else nat.LF_WEIGHT_DENSE, 0, None)
     keep = None
     if drop is not None:
-        args, keep = drop.args(plan, prob, backward, device)
+        args, keep = drop.args(plan, prob, backward, device, build)
         opt.dropout = ctypes.pointer(args)
     return ctypes.byref(opt), (opt, keep)
 
 
-def _save_sf(x, rts, plan, aset, ws, planes: int) -> None:
+def _save_sf(x, rts, plan, aset, ws, planes: int, captured: int = 0) -> None:
     """Remember this forward's S_f (the fixed part of its workspace: S_ext planes and flags, not
     the K-split tail's scratch) for a backward on the same inputs."""
     dead = [k for k, v in _SAVED_SF.items() if v[0]() is None]
@@ -554,20 +576,21 @@ def _save_sf(x, rts, plan, aset, ws, planes: int) -> None:
         _SAVED_SF.popitem(last=False)
     try:
         key = (id(x), id(rts), id(aset))
-        _SAVED_SF[key] = (weakref.ref(x), x._version, rts, plan, aset, ws, planes)
+        _SAVED_SF[key] = (weakref.ref(x), x._version, rts, plan, aset, ws, planes, captured)
         _SAVED_SF.move_to_end(key)
     except TypeError:  # pragma: no cover - objects without weakref support
         pass
 
 
-def _saved_sf(x, rts, plan, aset):
+def _saved_sf(x, rts, plan, aset, captured: int = 0):
     """(workspace, planes) of a forward on this very x (unchanged since), with the same validated
-    routes, plan and adapter record (every A and B tensor unchanged since), or None."""
+    routes, plan and adapter record (every A and B tensor unchanged since), or None.  A captured
+    backward takes that of a forward of the same capture alone: replays find another x."""
     hit = _SAVED_SF.get((id(x), id(rts), id(aset)))
     if hit is None:
         return None
-    xref, ver, r0, p0, a0, ws, planes = hit
-    if xref() is not x or x._version != ver or r0 is not rts or p0 is not plan or a0 is not aset:
+    xref, ver, r0, p0, a0, ws, planes, c0 = hit
+    if c0 != captured or xref() is not x or x._version != ver or r0 is not rts or p0 is not plan or a0 is not aset:
         return None
     return ws, planes
 
@@ -655,11 +678,13 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
         raise ValueError(f"grad_dtype must be None, x.dtype or torch.float32, got {grad_dtype}")
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    w, mx4 = _base(base_weight, x)
+    # the capture into a CUDA graph that the call is part of, 0 for none
+    captured = nat.glue().capture_id(device.index) if drop is not None or isinstance(base_weight, MX4Weight) else 0
+    w, mx4 = _base(base_weight, x, not captured)
     if mx4:
         x, g = (t.detach().clone() if t.data_ptr() % 16 else t for t in (x, g))
-    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
-    packs = _pack(plan, aset, dtype, K, N, device, backward=True)
+    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None, not captured)
+    packs = _pack(plan, aset, dtype, K, N, device, True, not captured)
     info = plan.info
     rtot = info.rank_total
     ext = _peer_layout(plan, peer, device) if peer is not None else None
@@ -673,7 +698,7 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=device)
     prob = _problem(code, T, K, N, x, w, packs)
     stream = nat.raw_stream(device.index)
-    saved = _saved_sf(x_in, rts, plan, aset) if dtype != torch.float32 and drop is None else None
+    saved = _saved_sf(x_in, rts, plan, aset, captured) if dtype != torch.float32 and drop is None else None
     sf_ptr, sf_planes = (saved[0].data_ptr(), saved[1]) if saved is not None else (None, 0)
     # S_f from the forward on these inputs, when there was one: no second s x A^T shrink
     pr = None
@@ -685,7 +710,9 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
             pr.exchange[r] = ptr
         pr.slot_span_dev = ext.slot_span.data_ptr()
         pr.span_info_dev = ext.span_info.data_ptr()
-    opt, keep = _options(mx4, drop, plan, prob, True, device)
+    opt, keep = _options(mx4, drop, plan, prob, True, device, not captured)
+    if captured:
+        _CAPTURED.append((plan, packs, w))
     with nat.on_device(device.index):
         rc = L.lf_backward_opt(ctypes.byref(prob), ctypes.byref(info), plan.table_dev.data_ptr(), opt, g.data_ptr(),
                                sf_ptr, sf_planes, _DTYPE_CODE[gdt], grad_x.data_ptr(), ga_flat.data_ptr(),

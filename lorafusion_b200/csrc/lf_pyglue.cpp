@@ -208,6 +208,24 @@ PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(w));
 }
 
+// capture_id(device index): the id of the capture into a CUDA graph that the device's current stream is in, 0 for none.
+PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1) {
+    PyErr_SetString(PyExc_TypeError, "capture_id takes 1 argument");
+    return nullptr;
+  }
+  const long dev = PyLong_AsLong(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(), &status,
+                               &id) != cudaSuccess) {
+    (void)cudaGetLastError();  // the legacy stream beside another one's capture: not captured itself
+    status = cudaStreamCaptureStatusNone;
+  }
+  return PyLong_FromUnsignedLongLong(status == cudaStreamCaptureStatusActive ? id : 0);
+}
+
 // bank_load(bank_a, bank_b, ranks, scales, slot, lora_a, lora_b, scaling): an adapter into its slot.  None unless its
 // tensors have the bank's dtype and device and dense rows; shapes were checked by the caller.
 PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -485,6 +503,7 @@ PyMethodDef methods[] = {
     {"mx4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_linear>)), METH_FASTCALL, nullptr},
     {"mx4_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_quantize>)), METH_FASTCALL, nullptr},
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_dequantize>)), METH_FASTCALL, nullptr},
+    {"capture_id", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<capture_id>)), METH_FASTCALL, nullptr},
     {"bank_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<bank_load>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},
     {"gather_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<gather_step>)), METH_FASTCALL, nullptr},

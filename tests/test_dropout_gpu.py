@@ -2,8 +2,8 @@
 
 Tolerances.  A result is off by at most half a step of its type, plus: ``n 2^-24`` of the sum of magnitudes for a float32
 sum of n products; the rank product S, which the forward on tensor cores rounds to the type (half a step, of S or of its
-two halves along K, which share out the reduction) and the backward keeps to 2^-15 (two 16-bit halves; the lower of float16 no finer than 2^-25); in float32 everything is summed in
-64 bits and only the factor s / (1 - p) and the result are rounded.
+two halves along K, which share out the reduction) and the backward keeps to 2^-15 (two 16-bit halves; the lower of float16
+no finer than 2^-25); in float32 everything is summed in 64 bits and only the factor s / (1 - p) and the result are rounded.
 """
 
 import numpy as np
@@ -362,6 +362,61 @@ def test_captured_graphs_and_streams():
         assert torch.equal(out[0], y) and torch.equal(out[1][0], back[0])
         assert all(torch.equal(out[1][1][i], back[1][i]) and torch.equal(out[1][2][i], back[2][i]) for i in back[1])
     assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("mx4,drop", [(True, True), (True, False), (False, True)])
+def test_a_captured_call_keeps_what_its_replays_read(mx4, drop):
+    """Other routings, rates and adapters push its tables out of the caches; a captured backward does not take what an
+    eager forward left."""
+    p = Problem(300, 256, 192, [16, 8], [100], [0.2, 0.1], BF16, mx4=mx4)
+    kw = {} if drop else {"dropout": None}
+    a0, b0 = dict(p.a), dict(p.b)
+    p.forward(**kw), p.backward(**kw)
+    graphs = []
+    for call in (p.forward, p.backward):
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = call(**kw)
+        graphs.append((gr, out))
+    p.x.copy_(rand(300, 256, seed=90))
+    y = p.forward(**kw)
+    b200_ops._SAVED_SF.clear()
+    gx, ga, gb = p.backward(**kw)
+    for n in range(300):
+        q = Problem(8 + n, 64, 64, [4], [], [n / 1000 + 0.1], BF16)
+        q.forward()
+        p.a[0], p.b[0] = a0[0] + n, b0[0] + n
+        p.forward(**kw)
+    (fw, y1), (bw, (gx1, ga1, gb1)) = graphs
+    bw.replay()
+    fw.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y1, y) and torch.equal(gx1, gx)
+    assert all(torch.equal(ga1[i], ga[i]) and torch.equal(gb1[i], gb[i]) for i in b0)
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("mx4", [False, True])
+def test_nothing_is_built_within_a_capture(mx4):
+    p = Problem(64, 64, 64, [8], [], [0.5], BF16, mx4=mx4)
+    for before, call in ((None, p.forward), (p.forward, p.backward)):
+        if before is not None:
+            before()
+        with pytest.raises(RuntimeError, match="once before"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+    torch.cuda.synchronize()
+    check_all(p)
+
+
+@pytest.mark.filterwarnings("ignore::lorafusion_b200.b200_ops.CudaCorePathWarning")
+def test_a_weight_at_an_odd_address():
+    """CUDA cores, sixteen-bit types: the mask is applied to a copy of x, by vectors and element by element."""
+    for K, shift in ((64, 1), (68, 0), (33, 0)):
+        p = Problem(70, K, 40, [8, 5], [30], [0.3, 0.0], BF16)
+        store = torch.zeros(p.w.numel() + 1, dtype=BF16, device=DEV)
+        p.w = p.base = store[shift:shift + p.w.numel()].view_as(p.w).copy_(p.w)
+        check_all(p)
 
 
 def test_empty_batches_and_refusals():
