@@ -1487,6 +1487,18 @@ constexpr int kPartLd = kBM + 1;             // column-major partial sums, odd s
 constexpr int kMaxShrCluster = 4;             // K split across at most 4 CTAs (all resident at once)
 static_assert(64 * kPartLd * 4 <= kShrStages * (kShrABytes + kShrBBytes), "partials must fit the stage area");
 
+// Eight sums of one row of S times the segment's factor, into both planes; zeros in another segment's rows.
+template <typename OutT>
+__device__ __forceinline__ void store_s(OutT* at, int64_t plane_elems, const float* f, bool in, float scale) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = in ? scale * f[i] : 0.f;
+  uint4 hi, lo;
+  pack8_hi_lo<OutT>(v, hi, lo);
+  *reinterpret_cast<uint4*>(at) = hi;
+  *reinterpret_cast<uint4*>(at + plane_elems) = lo;
+}
+
 // kDrop: sixteen more warps mask each tile of P between its copy and its MMAs, and with store_masked one more stores the
 // masked tile (map_m; by the first unit of a row tile, the others have the same).  The generator needs four warps a
 // scheduler to be issued back to back.
@@ -1520,6 +1532,7 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
   const int tile = tb.unit_tile(unit), st0 = tb.unit_st0(unit), nst = tb.unit_nst(unit);
   const int r_pad = prm.r_pad;
   const int N = nst * r_pad;
+  OutT* out = reinterpret_cast<OutT*>(prm.s_ext);
   const int nkb = (prm.Kred + kBK - 1) / kBK;
   const int kb0 = static_cast<int>(crank) * prm.kb_per_split;
   const int kb1 = min(nkb, kb0 + prm.kb_per_split);
@@ -1654,82 +1667,90 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
       bulk_wait_all();
     }
     __syncwarp();
-  } else if (kDrop && warp >= kThreads / 32) {
-    const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, quarter = w >> 2;
-    const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
-    const bool any = __any_sync(0xffffffffu, high != 0);
-    int stage = 0;
-    uint32_t phase = 0;
-    for (int kb = kb0; kb < kb1; ++kb) {
-      if (!warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) break;
-      if (any) {
-        mask_granules<2>(sA + stage * kShrABytes, row, 2 * quarter, kb, static_cast<uint32_t>(tile * kBM + row), high, prm.drop);
-        fence_proxy_async_smem();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&masked[stage]);
-      if (++stage == kShrStages) {
-        stage = 0;
-        phase ^= 1;
+  } else {
+    if (kDrop && warp >= kThreads / 32) {
+      const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, quarter = w >> 2;
+      const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
+      const bool any = __any_sync(0xffffffffu, high != 0);
+      int stage = 0;
+      uint32_t phase = 0;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        if (!warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) break;
+        if (any) {
+          mask_granules<2>(sA + stage * kShrABytes, row, 2 * quarter, kb, static_cast<uint32_t>(tile * kBM + row), high,
+                           prm.drop);
+          fence_proxy_async_smem();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&masked[stage]);
+        if (++stage == kShrStages) {
+          stage = 0;
+          phase ^= 1;
+        }
       }
     }
-  } else {
+    // the sums: 16 columns at a time, shared out over the warps of a lane quarter
+    constexpr int kBatch = kDrop ? 2 : 4;  // chains read at once; a CTA has four or eight of them
     const int q = warp & 3;
     const int row = q * 32 + lane;
-    bool ok = true;
-    if (has_k) ok = warp_wait(tfull, 0, abort_flag, prm.tb.err, kErrTimeoutAcc);
-    if (ok && has_k) {
-      tc_fence_after();
-      const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
-      const int n_ch = min(kShrChains, 4 * (kb1 - kb0));
-      for (int c = 0; c < N; c += 16) {
-        float f[16];
+    const bool ok = has_k && warp_wait(tfull, 0, abort_flag, prm.tb.err, kErrTimeoutAcc);
+    if (ok) tc_fence_after();
+    const uint32_t tbase = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+    const int n_ch = ok ? min(kShrChains, 4 * (kb1 - kb0)) : 0;
+    for (int c = (warp - 2) / 4 * 16; c < N; c += (kDrop ? 1 + kShrMaskWarps / 4 : 1) * 16) {
+      float f[16];
 #pragma unroll
-        for (int jj = 0; jj < 16; ++jj) f[jj] = 0.f;
-        for (int ch = 0; ch < n_ch; ++ch) {  // chains added in fixed order
-          uint32_t v[16];
-          tmem_ld16(tbase + ch * 64 + c, v);
-          tmem_wait_ld();
+      for (int jj = 0; jj < 16; ++jj) f[jj] = 0.f;
+      for (int ch = 0; ch < n_ch; ch += kBatch) {  // chains added in fixed order
+        uint32_t v[kBatch][16];
 #pragma unroll
-          for (int jj = 0; jj < 16; ++jj) f[jj] += __uint_as_float(v[jj]);
-        }
+        for (int i = 0; i < kBatch; ++i) tmem_ld16(tbase + (ch + i) * 64 + c, v[i]);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+#pragma unroll
+          for (int jj = 0; jj < 16; ++jj) f[jj] += __uint_as_float(v[i][jj]);
+      }
+      if (prm.cluster == 1) {
+        const int j = c / r_pad;
+        const bool in = row >= seg_lo[j] && row < seg_hi[j];
+        OutT* at = out + (static_cast<int64_t>(st0 + j) * kBM + row) * r_pad + (c - j * r_pad);
+        store_s<OutT>(at, prm.plane_elems, f, in, seg_scale[j]);
+        store_s<OutT>(at + 8, prm.plane_elems, f + 8, in, seg_scale[j]);
+      } else {
 #pragma unroll
         for (int jj = 0; jj < 16; ++jj) partial[(c + jj) * kPartLd + row] = f[jj];
       }
-    } else {
-      for (int c = 0; c < N; ++c) partial[c * kPartLd + row] = 0.f;
     }
   }
 
-  // all partial sums of the cluster are visible after this barrier
   tc_fence_before();
-  cluster_sync_all();
-
-  {
+  if (prm.cluster > 1) {
+    cluster_sync_all();  // all partial sums of the cluster are visible
     const int rows_per = kBM / prm.cluster;
     const int r0 = static_cast<int>(crank) * rows_per;
-    const int total = rows_per * N;
     const uint32_t part_base = smem_u32(partial);
-    OutT* out = reinterpret_cast<OutT*>(prm.s_ext);
-    for (int e = threadIdx.x; e < total; e += blockDim.x) {
-      const int row = r0 + e / N, col = e % N;
-      const uint32_t off = static_cast<uint32_t>((col * kPartLd + row) * 4);
-      float part[kMaxShrCluster];
+    for (int e = threadIdx.x; e < rows_per * (N / 8); e += blockDim.x) {
+      const int row = r0 + e % rows_per, col = e / rows_per * 8;
+      float part[kMaxShrCluster][8];
 #pragma unroll
       for (int qr = 0; qr < kMaxShrCluster; ++qr)  // issue every peer load before summing
-        part[qr] = qr < prm.cluster ? ld_cluster_f32(map_to_cta(part_base + off, qr)) : 0.f;
-      float sum = 0.f;
+        if (qr < prm.cluster) {
+          const uint32_t peer = map_to_cta(part_base + static_cast<uint32_t>((col * kPartLd + row) * 4), qr);
 #pragma unroll
-      for (int qr = 0; qr < kMaxShrCluster; ++qr) sum += part[qr];
-      const int j = col / r_pad, jj = col - j * r_pad;
-      const int st = st0 + j;
-      const bool in = row >= seg_lo[j] && row < seg_hi[j];
-      const float v = in ? seg_scale[j] * sum : 0.f;
-      OutT hi, lo;
-      split_hi_lo<OutT>(v, hi, lo);
-      const int64_t idx = (static_cast<int64_t>(st) * kBM + row) * r_pad + jj;
-      out[idx] = hi;
-      out[prm.plane_elems + idx] = lo;
+          for (int i = 0; i < 8; ++i) part[qr][i] = ld_cluster_f32(peer + i * kPartLd * 4);
+        }
+      float f[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        f[i] = part[0][i];
+#pragma unroll
+        for (int qr = 1; qr < kMaxShrCluster; ++qr)
+          if (qr < prm.cluster) f[i] += part[qr][i];
+      }
+      const int j = col / r_pad;
+      store_s<OutT>(out + (static_cast<int64_t>(st0 + j) * kBM + row) * r_pad + (col - j * r_pad), prm.plane_elems, f,
+                    row >= seg_lo[j] && row < seg_hi[j], seg_scale[j]);
     }
   }
 
