@@ -55,25 +55,26 @@ __device__ __forceinline__ uint32_t row_threshold(const Tables& tb, const DropAr
   return 0;
 }
 
-// N granules of eight elements, first .. first + N - 1 of the eight of row `row` of an x tile in shared memory (128 rows of
-// 128 bytes, 128-byte swizzle), K block kb, masked in place.  `t` is the row's number in the batch, `high` as in keep2.
-template <int N>
-__device__ __forceinline__ void mask_granules(uint8_t* tile, int row, int first, int kb, uint32_t t, uint32_t high,
-                                              const DropArgs& d) {
-  uint32_t c[N];
-  uint4 r[N], v[N];
+// Masks tiles of 128 rows of 128 bytes (128-byte swizzle) in shared memory in place, a lane a row and four of its granules
+// of eight elements at a time.  The numbers of the first four do not wait for the tile.
+struct RowMask {
+  uint32_t row, t, high;  // row of the tile, its number in the batch, `high` as in keep2
+  __device__ __forceinline__ void numbers(int kb, int first, const DropArgs& d, uint4 (&r)[4]) const {
+    uint32_t c[4];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    c[j] = static_cast<uint32_t>(kb * 8 + first + j);
-    v[j] = *reinterpret_cast<const uint4*>(tile + row * 128 + (((first + j) ^ (row & 7)) << 4));
+    for (int j = 0; j < 4; ++j) c[j] = static_cast<uint32_t>(kb * 8 + first + j);  // kb: the block of K
+    philox<4>(c, t, d, r);
   }
-  philox<N>(c, t, d, r);
+  __device__ __forceinline__ void keep(uint8_t* tile, int first, const uint4 (&r)[4]) const {
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    v[j].x = keep2(v[j].x, r[j].x, high), v[j].y = keep2(v[j].y, r[j].y, high);
-    v[j].z = keep2(v[j].z, r[j].z, high), v[j].w = keep2(v[j].w, r[j].w, high);
-    *reinterpret_cast<uint4*>(tile + row * 128 + (((first + j) ^ (row & 7)) << 4)) = v[j];
+    for (int j = 0; j < 4; ++j) {
+      uint4* p = reinterpret_cast<uint4*>(tile + row * 128 + (((first + j) ^ (row & 7)) << 4));
+      uint4 v = *p;
+      v.x = keep2(v.x, r[j].x, high), v.y = keep2(v.y, r[j].y, high);
+      v.z = keep2(v.z, r[j].z, high), v.w = keep2(v.w, r[j].w, high);
+      *p = v;
+    }
   }
-}
+};
 
 }  // namespace lf

@@ -696,7 +696,8 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
     }
     __syncwarp();
   } else if (kDrop && warp >= kThreads / 32 && warp < kThreads / 32 + kMaskWarps) {
-    const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, half = w >> 2;
+    const int w = warp - kThreads / 32, half = w >> 2;
+    const uint32_t row = (w & 3) * 32 + lane;
     int stage = 0;
     uint32_t phase = 0;
     bool ok = true;
@@ -705,14 +706,16 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
       const int nkb = job_nkb(item_job(item)), nkb_half = (nkb + parts - 1) / parts;
       const int tile = tb.unit_tile(u);
       const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
+      const RowMask mask{row, static_cast<uint32_t>(tile * kBM) + row, high};
       const bool any = __any_sync(0xffffffffu, high != 0);
       const int kb_end = min(nkb, (h + 1) * nkb_half);
       for (int kb = h * nkb_half; kb < kb_end; ++kb) {
+        uint4 r[4];
+        if (any) mask.numbers(kb, 4 * half, prm.drop, r);
         ok = warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull);
         if (!ok) break;
         if (any) {
-          mask_granules<4>(sA + stage * kRoleStageBytes, row, 4 * half, kb, static_cast<uint32_t>(tile * kBM + row), high,
-                           prm.drop);
+          mask.keep(sA + stage * kRoleStageBytes, 4 * half, r);
           fence_proxy_async_smem();
         }
         __syncwarp();
@@ -1500,9 +1503,12 @@ __device__ __forceinline__ void store_s(OutT* at, int64_t plane_elems, const flo
 }
 
 // kDrop: sixteen more warps mask each tile of P between its copy and its MMAs, and with store_masked one more stores the
-// masked tile (map_m; by the first unit of a row tile, the others have the same).  The generator needs four warps a
-// scheduler to be issued back to back.
-constexpr int kShrMaskWarps = 16;
+// masked tile (map_m; by the first unit of a row tile, the others have the same).  Four groups of four warps take the
+// stages in turn: beside the multiplies of some the others wait, load and store.  Of 8192 x 4096 in 91 units a stage takes
+// 0.66 us, 0.75 where all warps shared each stage, 0.33 without masks.
+constexpr int kShrMaskGroups = 4, kShrMaskWarps = 4 * kShrMaskGroups;
+// A stage's waits are all one group's, or their parity could be another use's.
+static_assert(kShrStages % kShrMaskGroups == 0, "groups keep their stages");
 constexpr int kShrDropThreads = kThreads + 32 * (kShrMaskWarps + 1);
 template <typename OutT, bool kDrop>
 __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
@@ -1542,7 +1548,7 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
     for (int s = 0; s < kShrStages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], kDrop && prm.store_masked ? 2 : 1);
-      if (kDrop) mbar_init(&masked[s], kShrMaskWarps);
+      if (kDrop) mbar_init(&masked[s], 4);
     }
     mbar_init(tfull, kDrop && prm.store_masked ? 2 : 1);
     mbar_init(drain, 1);
@@ -1669,22 +1675,28 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
     __syncwarp();
   } else {
     if (kDrop && warp >= kThreads / 32) {
-      const int w = warp - kThreads / 32, row = (w & 3) * 32 + lane, quarter = w >> 2;
-      const uint32_t high = row_threshold(tb, prm.drop, tile, row) << 16;
+      const int w = warp - kThreads / 32, group = w >> 2;
+      const uint32_t row = (w & 3) * 32 + lane, high = row_threshold(tb, prm.drop, tile, row) << 16;
+      const RowMask mask{row, static_cast<uint32_t>(tile * kBM) + row, high};
       const bool any = __any_sync(0xffffffffu, high != 0);
-      int stage = 0;
+      int stage = group;
       uint32_t phase = 0;
-      for (int kb = kb0; kb < kb1; ++kb) {
+      for (int kb = kb0 + group; kb < kb1; kb += kShrMaskGroups) {
+        uint8_t* at = sA + stage * kShrABytes;
+        uint4 r[4];
+        if (any) mask.numbers(kb, 0, prm.drop, r);
         if (!warp_wait_stage(&full[stage], phase, abort_flag, tb.err, kErrTimeoutFull)) break;
         if (any) {
-          mask_granules<2>(sA + stage * kShrABytes, row, 2 * quarter, kb, static_cast<uint32_t>(tile * kBM + row), high,
-                           prm.drop);
+          mask.keep(at, 0, r);
+          mask.numbers(kb, 4, prm.drop, r);
+          mask.keep(at, 4, r);
           fence_proxy_async_smem();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(&masked[stage]);
-        if (++stage == kShrStages) {
-          stage = 0;
+        stage += kShrMaskGroups;
+        if (stage >= kShrStages) {
+          stage -= kShrStages;
           phase ^= 1;
         }
       }
