@@ -419,11 +419,13 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       if (single) {
         e = tc_gemm(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st);
       } else {
+        const bool behind = do_shrink && lora;
         e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr,
-                         cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p);
+                         cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p, behind);
         if (e != cudaSuccess && cosched_allowed(ds)) {  // cooperative launch refused: nothing ran
           refuse_cosched(ds, e);
-          e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p);
+          e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p,
+                           behind);
         }
       }
     }
@@ -821,11 +823,13 @@ int backward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_
       dx.s = dx.l = p_g;
     }
     if (!gemm_done) {
+      const bool behind = lora && do_shrink;
       e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, nullptr,
-                       cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p);
+                       cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p, behind);
       if (e != cudaSuccess && cosched_allowed(ds)) {  // cooperative launch refused: nothing ran
         refuse_cosched(ds, e);
-        e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p);
+        e = tc_gemm_pair(dt, true, dx, T, K, N, lora, tb, grad_x_dev, K, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p,
+                         behind);
       }
       if (e != cudaSuccess) return LF_ERR_CUDA;
     }

@@ -1154,7 +1154,8 @@ __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
       }
       __syncwarp();
       if (lane == 0) {
-        if ((prm.n_shrink_pairs > 0 || prm.shrink_prologue) && pe > pb) {  // S_ext of both row tiles (and the zero block) published?
+        pdl_wait();  // S_ext of a shrink ahead of this launch (everything else was there before that one)
+        if ((prm.n_shrink_pairs > 0 || prm.shrink_prologue) && pe > pb) {  // S_ext of both row tiles (and the zero block)?
           bool seen = it1 - it0 <= 8;
 #pragma unroll
           for (int q = 0; q < 9; ++q) seen = seen && fl[q] == prm.ready_gen;
@@ -2535,7 +2536,8 @@ int pair_spare_pairs(int T, int Nout, int num_sms, int n_units) {
 
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
-                         const PairShrink* shrink, const PairTail* tail, const PairDelta* delta, const PairMx4* mx4) {
+                         const PairShrink* shrink, const PairTail* tail, const PairDelta* delta, const PairMx4* mx4,
+                         bool behind_shrink) {
   PairParams p{};
   if (mx4 != nullptr) p.mx4 = *mx4;
   p.out = out;
@@ -2638,6 +2640,11 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   attr[1].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.n_shrink_pairs > 0 || p.shrink_prologue || p.tail_parts > 1 ? 2 : 1;
+  if (behind_shrink && cfg.numAttrs == 1) {
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.numAttrs = 2;
+  }
   cudaError_t e;
 #define LF_LAUNCH_PAIR(QMN, OT, DELTA, MX4, DROP)                                                                        \
   {                                                                                                                      \
