@@ -2708,9 +2708,10 @@ cudaError_t tc_shrink(int dtype, const CUtensorMap& p_map, const CUtensorMap& a_
   // and each keeps at least four k-blocks
   int cluster = 1;
   while (cluster < kMaxShrCluster && tb.n_units * cluster * 2 <= num_sms && nkb >= 4 * cluster * 2) cluster *= 2;
-  // Two shrinks in flight fill the SMs that one leaves, and finer pieces pack better (8192 rows, 90 units each: with them
-  // side by side and the launch behind them started early a backward took 431 us, else 457).
-  if (two && cluster == 1 && nkb >= 8) cluster = 2;
+  // Two shrinks in flight, the masked one ahead, fill the SMs that one leaves.  The masked one, the longer, packs better in
+  // halves of K (8192 rows, 90 units each: a backward took 399 us so, 412 with both in halves, 415 with neither, 417 with
+  // the masked one in quarters; other shapes the same within their noise).  Alone it is not cut: 273 us a forward, else 278.
+  if (two && !beside && cluster == 1 && nkb >= 8) cluster = 2;
   ShrinkParams p{};
   p.s_ext = s_ext;
   p.plane_elems = static_cast<int64_t>(tb.n_segtiles + 1) * kBM * tb.r_pad;
