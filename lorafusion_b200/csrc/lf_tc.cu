@@ -1505,8 +1505,9 @@ __device__ __forceinline__ void store_s(OutT* at, int64_t plane_elems, const flo
 
 // kDrop: sixteen more warps mask each tile of P between its copy and its MMAs, and with store_masked one more stores the
 // masked tile (map_m; by the first unit of a row tile, the others have the same).  Four groups of four warps take the
-// stages in turn: beside the multiplies of some the others wait, load and store.  Of 8192 x 4096 in 91 units a stage takes
-// 0.66 us, 0.75 where all warps shared each stage, 0.33 without masks.
+// stages in turn: beside the multiplies of some the others wait, load and store.  8192 x 4096 in 91 units take 57 us (64
+// where all warps share each stage, 30 without masks; profiler, cold caches), 42 % of the issue slots: what bounds it is
+// the generator's chain of dependent multiplies, 20 of them a number of 128 bits.
 constexpr int kShrMaskGroups = 4, kShrMaskWarps = 4 * kShrMaskGroups;
 // A stage's waits are all one group's, or their parity could be another use's.
 static_assert(kShrStages % kShrMaskGroups == 0, "groups keep their stages");
