@@ -396,6 +396,44 @@ def test_a_captured_call_keeps_what_its_replays_read(mx4, drop):
     assert nat.device_error() == 0
 
 
+@pytest.mark.parametrize("mx4,drop", [(True, True), (True, False), (False, True), (False, False)])
+def test_a_gemm_that_starts_beside_its_shrink(mx4, drop):
+    """As many tiles as CTA pairs, so that none is left for the shrink: eager, on two streams at once and captured."""
+    p = Problem(18944, 512, 256, [16, 8, 64, 33], [37, 5000, 5003, 12800], [0.1, 0.0, 0.3, 0.05], BF16, mx4=mx4)
+    kw = {} if drop else {"dropout": None}
+    if drop:
+        check_all(p)
+
+    def step():
+        y = p.forward(**kw)
+        gx, ga, gb = p.backward(**kw)
+        return [y, gx, *ga.values(), *gb.values()]
+
+    b200_ops._SAVED_SF.clear()
+    want = step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for st in streams:
+            with torch.cuda.stream(st):
+                got.append(step())
+    torch.cuda.synchronize()
+    if mx4 or drop:
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            out = step()
+        for _ in range(3):
+            for t in out:
+                t.zero_()
+            gr.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+    for res in got:
+        assert all(torch.equal(a, b) for a, b in zip(res, want))
+    assert nat.device_error() == 0
+
+
 @pytest.mark.parametrize("mx4", [False, True])
 def test_nothing_is_built_within_a_capture(mx4):
     p = Problem(64, 64, 64, [8], [], [0.5], BF16, mx4=mx4)
