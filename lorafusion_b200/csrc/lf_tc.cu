@@ -2641,6 +2641,8 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   attr[1].val.cooperative = 1;
   cfg.attrs = attr;
   cfg.numAttrs = p.n_shrink_pairs > 0 || p.shrink_prologue || p.tail_parts > 1 ? 2 : 1;
+  // Beside the shrink's last CTAs the tiles of SMs that are done start: 8 us of 255 at 8192 rows 4096 -> 4096 over a weight in
+  // 4 bits, 7 of 787 at 32768 rows over a dense one; 32768 rows 8192 -> 8192 (3.2 ms) the same to 0.6 %.
   if (behind_shrink && cfg.numAttrs == 1) {
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
