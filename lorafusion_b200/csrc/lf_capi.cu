@@ -152,8 +152,9 @@ size_t segtile_elems(const lf_plan_info* info) {
 // the tensor-core path.  A tensor-core shrink writes each value v as hi = round(v) in plane h and
 // lo = round(v - hi) in plane kh + h, where kh (1 or 2) counts its K-half partial products (two
 // when it runs inside the GEMM launch): planes [hi of each K half..., lo of each K half...].  The
-// LoRA expand reads the hi planes; the dA/dB grams read all 2*kh planes, so S enters the
-// gradient sums with about 16 significant bits instead of 8.
+// expand of a forward without dropout reads the hi planes, S rounded once as an activation is; the dA/dB grams and the
+// expand of a forward with dropout read all 2*kh planes, so S enters their sums with about 16 significant bits
+// instead of 8.
 size_t sext_bytes(const lf_plan_info* info) { return (segtile_elems(info) * 8 + 255) & ~size_t(255); }
 
 constexpr int kSextPlanes = 4;  // planes one tensor-core S_ext buffer holds
@@ -401,7 +402,7 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       sh.n_pairs = spare;
       sh.prologue = cosched_prologue();
       sh.drop = opt.drop;
-      e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, &sh, &tail, nullptr, mx4p);
+      e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, &sh, &tail, nullptr, mx4p, false, drop);
       if (e == cudaSuccess) {
         if (sf_planes) *sf_planes = 2;
         return LF_OK;
@@ -421,11 +422,11 @@ int forward_impl(const lf_problem* prob, const lf_plan_info* info, const int32_t
       } else {
         const bool behind = do_shrink && lora;
         e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr,
-                         cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p, behind);
+                         cosched_allowed(ds) ? &tail : nullptr, nullptr, mx4p, behind, drop);
         if (e != cudaSuccess && cosched_allowed(ds)) {  // cooperative launch refused: nothing ran
           refuse_cosched(ds, e);
           e = tc_gemm_pair(dt, false, maps, T, N, K, lora, tb, y_dev, N, ds->num_sms, st, nullptr, nullptr, nullptr, mx4p,
-                           behind);
+                           behind, drop);
         }
       }
     }

@@ -129,11 +129,13 @@ struct PairMx4 {
 // CTA pairs the pair GEMM can leave to a co-scheduled shrink without adding a round (0: none).
 int pair_spare_pairs(int T, int Nout, int num_sms, int n_units);
 // `tail` (optional) enables the K-split tail; the launch is then cooperative.  `behind_shrink`: the launch ahead of this one
-// is the tc_shrink that writes S; where the launch is not cooperative its tiles start beside it.
+// is the tc_shrink that writes S; where the launch is not cooperative its tiles start beside it.  `s_lo`: S enters with its
+// low halves (of a shrink with dropout, which leaves their zero tile too).
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
                          const PairShrink* shrink = nullptr, const PairTail* tail = nullptr,
-                         const PairDelta* delta = nullptr, const PairMx4* mx4 = nullptr, bool behind_shrink = false);
+                         const PairDelta* delta = nullptr, const PairMx4* mx4 = nullptr, bool behind_shrink = false,
+                         bool s_lo = false);
 // Forward workspace without the tail scratch (the least lf_forward accepts).
 size_t forward_min_workspace_bytes(const lf_plan_info* info);
 // Gram load balance: slots (slot_order positions) the kernel can split into parts, and the

@@ -57,8 +57,8 @@ __device__ __forceinline__ __half cvt_out<__half>(float v) {
 __device__ __forceinline__ float cvt_in(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float cvt_in(__half v) { return __half2float(v); }
 
-// S values enter the dA/dB sums as hi + lo (both in the input type): hi = round(v) is what the
-// LoRA expand reads, lo = round(v - hi) restores the bits hi dropped.
+// S is kept as hi + lo (both in the input type): hi = round(v) is what the expand of a forward without dropout
+// reads, lo = round(v - hi) restores the bits hi dropped, for dA and dB and for the forward with dropout.
 template <typename OutT>
 __device__ __forceinline__ void split_hi_lo(float v, OutT& hi, OutT& lo) {
   hi = cvt_out<OutT>(v);
@@ -440,7 +440,8 @@ struct PairParams {
   uint64_t gen;
   uint64_t ready_gen;    // value GEMM CTAs wait for on unit_ready: gen (a test hook may change it)
   // S_ext planes the LoRA stages sum: 1 = the full product; 2 = two K-half partial products
-  // (written by the co-scheduled shrink), plane p starting at S map row p * s_plane_rows
+  // (written by the co-scheduled shrink), plane p starting at S map row p * s_plane_rows.  With the low halves twice
+  // as many: they follow the high ones.
   int s_planes, s_plane_rows;
   // optional second shrink job (own activations/slab/K), items after the first job's; job2_only: no first job, whole K
   // ranges (S_ext of one product, nobody waits for it), and the masked activations are stored (kDrop)
@@ -767,11 +768,10 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
     const int q = warp & 3;
     const int row = q * 32 + lane;
     OutT* s_ext = reinterpret_cast<OutT*>(prm.s_ext);
-    if (me == 0 && !only2)  // the all-zero segment tile of both planes, published with item 0
-      for (int e = threadIdx.x - 64; e < kBM * r_pad; e += 128) {
-        s_ext[static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad + e] = cvt_out<OutT>(0.f);
-        s_ext[plane_elems + static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad + e] = cvt_out<OutT>(0.f);
-      }
+    if (me == 0 && !only2)  // the all-zero segment tile of every plane that the expand reads, published with item 0
+      for (int p = 0; p < (kDrop ? 4 : 2); ++p)
+        for (int e = threadIdx.x - 64; e < kBM * r_pad; e += 128)
+          s_ext[p * plane_elems + static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad + e] = cvt_out<OutT>(0.f);
     int it = 0;
     for (int item = me; item < n_items; item += n_me, ++it) {
       const int job = item_job(item), u = item_unit(item), h = item_part(item);
@@ -1770,7 +1770,10 @@ __global__ void __launch_bounds__(kDrop ? kShrDropThreads : kThreads, 1)
 
   if (blockIdx.x == 0) {  // the all-zero segment tile the pair GEMM pads odd row tiles with
     OutT* zero = reinterpret_cast<OutT*>(prm.s_ext) + static_cast<int64_t>(tb.n_segtiles) * kBM * r_pad;
-    for (int e = threadIdx.x; e < kBM * r_pad; e += blockDim.x) zero[e] = cvt_out<OutT>(0.f);
+    for (int e = threadIdx.x; e < kBM * r_pad; e += blockDim.x) {
+      zero[e] = cvt_out<OutT>(0.f);
+      if (kDrop) zero[prm.plane_elems + e] = cvt_out<OutT>(0.f);  // and of the low halves
+    }
   }
 
   pdl_wait();  // launched beside another shrink: done when both are
@@ -2538,7 +2541,7 @@ int pair_spare_pairs(int T, int Nout, int num_sms, int n_units) {
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
                          const PairShrink* shrink, const PairTail* tail, const PairDelta* delta, const PairMx4* mx4,
-                         bool behind_shrink) {
+                         bool behind_shrink, bool s_lo) {
   PairParams p{};
   if (mx4 != nullptr) p.mx4 = *mx4;
   p.out = out;
@@ -2559,7 +2562,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   p.r_pad = tb.r_pad;
   const int fmt = dtype == LF_BF16 ? 1 : 0;
   p.ab_fmt = fmt;
-  p.s_planes = 1;
+  p.s_planes = s_lo ? 2 : 1;
   p.s_plane_rows = (tb.n_segtiles + 1) * kBM;
   p.idesc_main = umma_idesc_f16(256, 256, fmt, 0, q_mn_major ? 1 : 0);
   p.idesc_lora = umma_idesc_f16(256, 256, fmt, 0, 0);
@@ -2581,7 +2584,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
     if (!shrink->job2_only) p.group_m = 4;
     p.shrink_prologue = shrink->prologue ? 1 : 0;
     p.n_shrink_pairs = shrink->prologue ? 0 : shrink->n_pairs;
-    p.s_planes = shrink->job2_only ? 1 : 2;
+    if (!shrink->job2_only) p.s_planes *= 2;
     p.s_ext = shrink->s_ext;
     p.unit_ready = shrink->unit_ready;
     p.gen = shrink->gen;

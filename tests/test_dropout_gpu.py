@@ -466,3 +466,43 @@ def test_empty_batches_and_refusals():
         p.forward(dropout=AdapterDropout({1: 0.5}, 0))
     with pytest.raises(ValueError, match="AdapterDropout"):
         p.forward(dropout=0.5)
+
+
+@pytest.mark.parametrize("mx4", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("mode", [0, 1])
+@pytest.mark.parametrize("T,K,N,ranks,cuts", [
+    (300, 256, 192, [16, 8], [100]), (1030, 200, 1024, [64, 33, 100], [3, 140, 400, 401]),
+    (18944, 128, 256, [16, 8], [37, 5000, 12800])])
+def test_the_rank_product_enters_the_forward_in_two_halves(T, K, N, ranks, cuts, dtype, mode, mx4):
+    """Over a weight of zeros y is S B^T alone.  S is held as hi + lo, each of the type: |S - hi| is at most half a step,
+    eps / 2 |S|, and that rounded again leaves (eps / 2)^2 |S| (float16's low half ends at 2^-25), of S or of its two halves
+    along K.  Freed memory is full of NaN, so that a zero tile which nothing wrote shows."""
+    try:
+        nat.check(nat.lib().lf_set_co_scheduling(mode), "mode")
+        p = Problem(T, K, N, ranks, cuts, [0.1, 0.0, 0.3][:len(ranks)], dtype)
+        p.base = torch.zeros_like(p.w)
+        if mx4:
+            p.base = quantize_weight(p.base)
+        p.forward()
+        torch.cuda.empty_cache()
+        torch.full((64 << 20,), float("nan"), dtype=dtype, device=DEV)
+        y = p.forward()
+    finally:
+        nat.lib().lf_set_co_scheduling(1)
+    one, half = 2.0 ** -24, torch.finfo(dtype).eps / 2
+    xm = torch.where(p.mask(), p.x.double(), 0.0)
+    ref, bound = torch.zeros(T, N, dtype=torch.float64, device=DEV), torch.zeros(T, N, dtype=torch.float64, device=DEV)
+    for r in p.routing.routes:
+        i, s = r.adapter_id, slice(r.row_start, r.row_end)
+        f = p.specs[i].scaling / (1 - round(p.dropout.rates[i] * 65536) / 65536)
+        a, b = p.a[i].double(), p.b[i].double()
+        k = (-(-K // 64) + 1) // 2 * 64
+        S0, S1 = f * xm[s, :k] @ a[:, :k].t(), f * xm[s, k:] @ a[:, k:].t()
+        mag = f * xm[s].abs() @ a.abs().t()
+        eS = half * half * (S0.abs() + S1.abs()) + (K + 2) * one * mag + 2 * 2.0 ** -25
+        ref[s] = (S0 + S1) @ b.t()
+        # (two products a half and rank, summed in float32)
+        bound[s] = eS @ b.abs().t() + 4 * a.shape[0] * one * ((S0.abs() + S1.abs()) @ b.abs().t())
+    check(y, (ref, bound), "y")
+    assert nat.device_error() == 0
