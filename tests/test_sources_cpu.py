@@ -1,0 +1,21 @@
+"""What the kernels' sources must hold to, read from the files (no GPU)."""
+
+import os
+import re
+
+from lorafusion_b200.csrc import build
+
+
+def sources():
+    names = [s for s in build.SOURCES if s.endswith(".cu")] + [h for h in build.HEADERS if h.endswith(".cuh")]
+    return {n: open(os.path.join(build.HERE, n)).read() for n in names}
+
+
+def test_arrivals_at_another_cta_are_released_at_cluster_scope():
+    """A release at CTA scope orders nothing for a thread of another CTA that waits on the barrier."""
+    found = 0
+    for name, text in sources().items():
+        for m in re.finditer(r'"[^"\n]*mbarrier\.arrive[\w.:]*shared::cluster[^"\n]*"', text):
+            found += 1
+            assert ".release.cluster." in m.group(), f"{name}: {m.group()}"
+    assert found
