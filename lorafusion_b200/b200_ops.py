@@ -275,11 +275,19 @@ def _adapters(rts: _Routes, lora_a, lora_b, adapters) -> _AdapterSet:
     return rec
 
 
-def _not_captured(what: str) -> RuntimeError:
-    return RuntimeError(f"{what} would be made within a CUDA graph capture: make the same call once before it")
+def _capture(device) -> int:
+    """The capture into a CUDA graph that the device's current stream is in, 0 for none."""
+    return nat.glue().capture_id(device.index)
 
 
-def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, scales=None, build=True) -> _Plan:
+def _building(what: str, device) -> None:
+    """Refuses to fill a cache within a capture: nothing runs there, so later calls would find it empty, and replays would
+    fill it again from host memory that is gone by then."""
+    if _capture(device):
+        raise RuntimeError(f"{what} would be made within a CUDA graph capture: make the same call once before it")
+
+
+def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, scales=None) -> _Plan:
     ranks, scales = aset.ranks, aset.scales if scales is None else scales
     for pr, ps, pd, plan in rts.plans:
         if pd == device and pr == ranks and ps == scales:
@@ -292,8 +300,7 @@ def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device
                ranks, scales)
     plan = _PLAN_BY_CONTENT.get(content)
     if plan is None:
-        if not build:
-            raise _not_captured("the routing's tables")
+        _building("the routing's tables", device)
         plan = _build_plan(rts, ranks, scales, total_rows, device)
         if len(_PLAN_BY_CONTENT) >= _CACHE_MAX:
             _PLAN_BY_CONTENT.clear()
@@ -309,14 +316,13 @@ def _build_plan(rts: _Routes, ranks, scales, total_rows: int, device) -> _Plan:
     return _Plan(info, table_dev, rts.slots, ranks)
 
 
-def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, backward: bool,
-          build=True) -> dict:
+def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, backward: bool) -> dict:
     """Zero-padded adapter slabs in the layouts the kernels read (cached in the adapter record)."""
     key = (dtype, K, N, device, plan.info.r_pad)
     entry = aset.packs.get(key)
     want = ("a", "b", "bt", "at") if backward else ("a", "b")
-    if not build and (entry is None or any(w not in entry for w in want)):
-        raise _not_captured("the adapters' slabs")
+    if entry is None or any(w not in entry for w in want):
+        _building("the adapters' slabs", device)
     if entry is None:
         for aid, a, b, r in zip(plan.slots, aset.a, aset.b, plan.ranks):
             if a.dim() != 2 or a.shape[1] != K or b.dim() != 2 or b.shape != (N, r):
@@ -374,7 +380,7 @@ def _fill_packs(entry, plan: _Plan, dtype, K, N, device, which) -> None:
         entry.setdefault("ptr_bufs", []).append((ptrs, ranks_dev))
 
 
-def _weight(base_weight: torch.Tensor, dtype, device, build=True) -> torch.Tensor:
+def _weight(base_weight: torch.Tensor, dtype, device) -> torch.Tensor:
     """Base weight as a contiguous tensor of the activation dtype (converted copies cached)."""
     if isinstance(base_weight, MX4Weight):
         raise ValueError("this call takes a dense base_weight (MX4Weight.dequantize)")
@@ -388,8 +394,7 @@ def _weight(base_weight: torch.Tensor, dtype, device, build=True) -> torch.Tenso
         ref, ptr, ver, conv = hit
         if ref() is base_weight and ptr == base_weight.data_ptr() and ver == base_weight._version:
             return conv
-    if not build:
-        raise _not_captured("a copy of base_weight")
+    _building("a copy of base_weight", device)
     conv = base_weight.to(dtype).contiguous()
     if len(_WEIGHT_CACHE) >= _CACHE_MAX:
         _WEIGHT_CACHE.clear()
@@ -423,11 +428,11 @@ def _problem(code, T, K, N, x, w, packs) -> nat.Problem:
     return p
 
 
-def _base(base_weight, x: torch.Tensor, build=True):
+def _base(base_weight, x: torch.Tensor):
     """(tensor that holds the base weight, whether it is the data of one in 4 bits).  A problem the tensor-core path
     cannot address takes a dense copy of a weight in 4 bits, made within the call."""
     if not isinstance(base_weight, MX4Weight):
-        return _weight(base_weight, x.dtype, x.device, build), False
+        return _weight(base_weight, x.dtype, x.device), False
     if base_weight.dtype is not x.dtype:
         raise ValueError(f"x ({x.dtype}) must have the dtype of the weight in 4 bits ({base_weight.dtype})")
     if base_weight.device != x.device:
@@ -457,12 +462,11 @@ class _Drop:
     def scales(self, scales):
         return tuple(s * (65536.0 / (65536 - t)) for s, t in zip(scales, self.thresholds))
 
-    def args(self, plan: _Plan, prob, backward: bool, device, build=True):
+    def args(self, plan: _Plan, prob, backward: bool, device):
         """lf_dropout, and what it points at."""
         table = plan.thresholds.get(self.thresholds)
         if table is None:
-            if not build:
-                raise _not_captured("the table of dropout thresholds")
+            _building("the table of dropout thresholds", device)
             while len(plan.thresholds) >= 8:
                 plan.thresholds.pop(next(iter(plan.thresholds)))
             host = torch.tensor([self.thresholds[i] for i, _, _ in plan.vslots] or [0], dtype=torch.int32)
@@ -500,9 +504,10 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
 
     Two things have no counterpart in the reference.  ``base_weight`` may be a ``quant.MX4Weight`` of x's dtype
     and device.  ``dropout`` (keyword only) puts a mask in front of the adapters: ``y = x W^T + s_i / (1 - p_i) (m x)
-    A_i^T B_i^T``, a dropped element being zero whatever it was.  A call with either can be captured into a CUDA graph
-    once the same call has run (``RuntimeError`` before): replays read x and the base weight as they are then, repeat
-    the mask, and keep the adapters' values of the capture.
+    A_i^T B_i^T``, a dropped element being zero whatever it was.
+
+    A call can be captured into a CUDA graph once the same call has run (``RuntimeError`` before): replays read x and the
+    base weight as they are then, repeat the mask, and keep the adapters' values of the capture.
     """
     global _last_launches
     rts = _routes(routing, x.shape[0])
@@ -516,13 +521,12 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     code = _DTYPE_CODE[dtype]
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    # the capture into a CUDA graph that the call is part of, 0 for none
-    captured = nat.glue().capture_id(device.index) if drop is not None or isinstance(base_weight, MX4Weight) else 0
-    w, mx4 = _base(base_weight, x, not captured)
+    captured = _capture(device)
+    w, mx4 = _base(base_weight, x)
     if mx4 and x.data_ptr() % 16:
         x = x.detach().clone()
-    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None, not captured)
-    packs = _pack(plan, aset, dtype, K, N, device, False, not captured)
+    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
+    packs = _pack(plan, aset, dtype, K, N, device, backward=False)
     y = torch.empty((T, N), dtype=dtype, device=device)
     if T == 0 or N == 0:
         return y
@@ -538,7 +542,7 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     prob = _problem(code, T, K, N, x, w, packs)
     stream = nat.raw_stream(device.index)
     planes = ctypes.c_int32(0)
-    opt, keep = _options(mx4, drop, plan, prob, False, device, not captured)
+    opt, keep = _options(mx4, drop, plan, prob, False, device)
     if captured:
         _CAPTURED.append((plan, packs, w))
     with nat.on_device(device.index):
@@ -554,14 +558,14 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     return y
 
 
-def _options(mx4: bool, drop: _Drop | None, plan: _Plan, prob, backward: bool, device, build=True):
+def _options(mx4: bool, drop: _Drop | None, plan: _Plan, prob, backward: bool, device):
     """lf_options of a call (None for a plain one), and what must live until it is enqueued."""
     if not mx4 and drop is None:
         return None, None
     opt = nat.Options(nat.LF_WEIGHT_MX4 if mx4 else nat.LF_WEIGHT_DENSE, 0, None)
     keep = None
     if drop is not None:
-        args, keep = drop.args(plan, prob, backward, device, build)
+        args, keep = drop.args(plan, prob, backward, device)
         opt.dropout = ctypes.pointer(args)
     return ctypes.byref(opt), (opt, keep)
 
@@ -678,13 +682,14 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
         raise ValueError(f"grad_dtype must be None, x.dtype or torch.float32, got {grad_dtype}")
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    # the capture into a CUDA graph that the call is part of, 0 for none
-    captured = nat.glue().capture_id(device.index) if drop is not None or isinstance(base_weight, MX4Weight) else 0
-    w, mx4 = _base(base_weight, x, not captured)
+    captured = _capture(device)
+    if captured and peer is not None:  # every call numbers its blocks; replays would repeat the number
+        raise RuntimeError("a call with peer cannot be captured into a CUDA graph")
+    w, mx4 = _base(base_weight, x)
     if mx4:
         x, g = (t.detach().clone() if t.data_ptr() % 16 else t for t in (x, g))
-    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None, not captured)
-    packs = _pack(plan, aset, dtype, K, N, device, True, not captured)
+    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
+    packs = _pack(plan, aset, dtype, K, N, device, backward=True)
     info = plan.info
     rtot = info.rank_total
     ext = _peer_layout(plan, peer, device) if peer is not None else None
@@ -710,7 +715,7 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
             pr.exchange[r] = ptr
         pr.slot_span_dev = ext.slot_span.data_ptr()
         pr.span_info_dev = ext.span_info.data_ptr()
-    opt, keep = _options(mx4, drop, plan, prob, True, device, not captured)
+    opt, keep = _options(mx4, drop, plan, prob, True, device)
     if captured:
         _CAPTURED.append((plan, packs, w))
     with nat.on_device(device.index):

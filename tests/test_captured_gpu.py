@@ -1,0 +1,144 @@
+"""Calls captured into CUDA graphs: what they may take from eager calls, and eager calls from them."""
+
+import pytest
+import torch
+
+from lorafusion_b200 import _native as nat
+from lorafusion_b200 import b200_ops as ops
+from lorafusion_b200.config import AdapterDropout, AdapterSpec, TileRoute, TileRoutingConfig
+from lorafusion_b200.quant import quantize_weight
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+def rand(*shape, seed=0, scale=1.0, dtype=BF16):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=gen, device=DEV) * scale).to(dtype)
+
+
+class Problem:
+    def __init__(self, mx4=False, rate=0.0, T=300, K=256, N=192, seed=0, alpha=16.0):
+        self.x, self.g = rand(T, K, seed=seed + 1), rand(T, N, seed=seed + 2)
+        w = rand(N, K, seed=seed + 3, scale=K ** -0.5)
+        self.w = quantize_weight(w) if mx4 else w
+        self.a = {i: rand(r, K, seed=seed + 4 + i, scale=K ** -0.5) for i, r in enumerate((16, 8))}
+        self.b = {i: rand(N, r, seed=seed + 6 + i, scale=0.2) for i, r in enumerate((16, 8))}
+        self.specs = {i: AdapterSpec(i, r, alpha if i == 0 else 16.0, K, N) for i, r in enumerate((16, 8))}
+        self.routing = TileRoutingConfig(128, [TileRoute(0, 100, 0), TileRoute(100, T, 1)])
+        self.kw = {"dropout": AdapterDropout(rate, 5, 7)} if rate else {}
+
+    def forward(self, **kw):
+        return ops.fused_lora_forward(self.x, self.w, self.a, self.b, self.specs, self.routing, **{**self.kw, **kw})
+
+    def backward(self, **kw):
+        return ops.fused_lora_backward(self.g, self.x, self.w, self.a, self.b, self.specs, self.routing, **{**self.kw, **kw})
+
+    def fresh(self):
+        """The backward on its own, no forward's S at hand."""
+        ops._SAVED_SF.clear()
+        return self.backward()
+
+
+def captured(call):
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    return graph, out
+
+
+def same(got, want):
+    for x, y in zip(got, want):
+        if isinstance(x, dict):
+            assert x.keys() == y.keys() and all(torch.equal(x[i], y[i]) for i in y)
+        else:
+            assert torch.equal(x, y)
+
+
+ALL = [(False, 0.0), (False, 0.3), (True, 0.0), (True, 0.3)]
+
+
+@pytest.mark.parametrize("mx4,rate", ALL)
+def test_a_captured_backward_takes_nothing_from_an_eager_forward(mx4, rate):
+    """Its replays find another x than that forward did."""
+    p = Problem(mx4, rate)
+    p.forward(), p.backward()
+    graph, out = captured(p.backward)
+    for n in range(2):
+        p.x.copy_(rand(*p.x.shape, seed=20 + n))
+        want = p.fresh()
+        graph.replay()
+        torch.cuda.synchronize()
+        same(out, want)
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("mx4,rate", ALL)
+def test_an_eager_backward_takes_nothing_from_a_captured_forward(mx4, rate):
+    """A capture runs nothing, and replays run whenever they are launched."""
+    p = Problem(mx4, rate)
+    p.forward(), p.backward()
+    want = p.fresh()
+    captured(p.forward)
+    same(p.backward(), want)
+    # nor does another capture
+    one, _ = captured(p.forward)
+    two, out = captured(p.backward)
+    two.replay()
+    torch.cuda.synchronize()
+    same(out, want)
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("mx4,rate", ALL)
+def test_forward_and_backward_of_one_capture(mx4, rate):
+    p = Problem(mx4, rate)
+    p.forward(), p.backward()
+    graph, (y, back) = captured(lambda: (p.forward(), p.backward()))
+    for n in range(2):
+        p.x.copy_(rand(*p.x.shape, seed=30 + n))
+        wy, want = p.forward(), p.backward()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, wy)
+        same(back, want)
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("mx4,rate", ALL)
+def test_nothing_is_built_within_a_capture(mx4, rate):
+    """What a capture would build no later call could use: tables, slabs, a converted weight."""
+    p = Problem(mx4, rate, seed=50)
+    ops.clear_weight_cache()
+    for before, call in ((None, p.forward), (p.forward, p.backward)):
+        if before is not None:
+            before()
+        with pytest.raises(RuntimeError, match="once before"):
+            captured(call)
+    torch.cuda.synchronize()
+    want = p.fresh()
+    y = p.forward()
+    same(p.backward(), want)
+    if not mx4 and not rate:
+        wide = p.w.float()
+        with pytest.raises(RuntimeError, match="copy of base_weight"):
+            captured(lambda: ops.fused_lora_forward(p.x, wide, p.a, p.b, p.specs, p.routing))
+        torch.cuda.synchronize()
+        assert torch.equal(ops.fused_lora_forward(p.x, wide, p.a, p.b, p.specs, p.routing), y)
+        for prepare in (lambda: ops.prepare_forward(p.x, p.w, p.a, p.b, p.specs, TileRoutingConfig(128, [TileRoute(0, 300, 1)])),):
+            with pytest.raises(RuntimeError, match="once before"):
+                captured(prepare)
+    assert nat.device_error() == 0
+
+
+def test_a_call_with_peer_is_not_captured():
+    p = Problem()
+    p.forward(), p.backward()
+
+    class Peer:
+        """Never reached."""
+
+    with pytest.raises(RuntimeError, match="peer"):
+        captured(lambda: p.backward(peer=Peer()))
+    torch.cuda.synchronize()
