@@ -211,16 +211,44 @@ def _plan_tables(starts, ends, route_slot, total_rows, ranks, scales, n_slots):
     raise RuntimeError("lf_plan_tables: table size did not converge")
 
 
-class _Plan:
-    __slots__ = ("info", "table_dev", "slots", "ranks", "vslots", "thresholds")
+class _Made:
+    """Cached device memory and the stream that fills it.  A call on another stream comes after that, and the memory is
+    used for nothing else before that call has run, whatever the caches drop meanwhile; the host waits for nothing (but
+    within a capture)."""
 
-    def __init__(self, info, table_dev, slots, ranks):
+    __slots__ = ("tensors", "stream", "event", "others")
+
+    def __init__(self, device, *tensors):
+        stream = torch.cuda.current_stream(device)
+        self.tensors = tensors
+        self.stream = stream.cuda_stream
+        self.event = torch.cuda.Event()
+        self.event.record(stream)
+        self.others: set = set()  # streams that have waited
+
+    def use(self, device, captured: int) -> None:
+        raw = nat.raw_stream(device.index)
+        if captured:  # replays may run on any stream
+            nat.glue().wait_event(self.event.cuda_event)
+        elif raw != self.stream and raw not in self.others:
+            stream = torch.cuda.current_stream(device)
+            stream.wait_event(self.event)
+            for t in self.tensors:
+                t.record_stream(stream)
+            self.others.add(raw)
+
+
+class _Plan:
+    __slots__ = ("info", "table_dev", "slots", "ranks", "vslots", "thresholds", "made")
+
+    def __init__(self, info, table_dev, slots, ranks, thresholds=0):
         self.info = info
         self.table_dev = table_dev
         self.slots = slots
         self.ranks = ranks
         self.vslots = _virtual_slots(ranks)
-        self.thresholds: dict = {}  # dropout thresholds of the slots -> those of the virtual slots on the device
+        self.thresholds = thresholds  # address of the virtual slots' dropout thresholds, behind the table's words
+        self.made = _Made(table_dev.device, table_dev)
 
 
 class _AdapterSet:
@@ -287,36 +315,52 @@ def _building(what: str, device) -> None:
         raise RuntimeError(f"{what} would be made within a CUDA graph capture: make the same call once before it")
 
 
-def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, scales=None) -> _Plan:
-    ranks, scales = aset.ranks, aset.scales if scales is None else scales
-    for pr, ps, pd, plan in rts.plans:
-        if pd == device and pr == ranks and ps == scales:
+def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, captured: int,
+          drop=None) -> _Plan:
+    """The routing's tables for this adapter set and, with ``drop``, its factors and thresholds."""
+    ranks, scales, thresholds = aset.ranks, aset.scales, None
+    if drop is not None:
+        scales, thresholds = drop.scales(scales), drop.thresholds
+    for pr, ps, pt, pd, plan in rts.plans:
+        if pd == device and pr == ranks and ps == scales and pt == thresholds:
+            plan.made.use(device, captured)
             return plan
     if any(r <= 0 for r in ranks):
         bad = rts.slots[next(i for i, r in enumerate(ranks) if r <= 0)]
         raise ValueError(f"adapter {bad}: lora_a must be a non-empty [rank, in_features] matrix")
     # a new routing object with the same routes (a runtime that re-packs every batch) reuses the plan
     content = (rts.starts.tobytes(), rts.ends.tobytes(), rts.route_slot.tobytes(), rts.slots, total_rows, device,
-               ranks, scales)
+               ranks, scales, thresholds)
     plan = _PLAN_BY_CONTENT.get(content)
     if plan is None:
         _building("the routing's tables", device)
-        plan = _build_plan(rts, ranks, scales, total_rows, device)
+        plan = _build_plan(rts, ranks, scales, thresholds, total_rows, device)
         if len(_PLAN_BY_CONTENT) >= _CACHE_MAX:
             _PLAN_BY_CONTENT.clear()
         _PLAN_BY_CONTENT[content] = plan
-    rts.plans.insert(0, (ranks, scales, device, plan))
+    else:
+        plan.made.use(device, captured)
+    rts.plans.insert(0, (ranks, scales, thresholds, device, plan))
     del rts.plans[4:]
     return plan
 
 
-def _build_plan(rts: _Routes, ranks, scales, total_rows: int, device) -> _Plan:
+def _build_plan(rts: _Routes, ranks, scales, thresholds, total_rows: int, device) -> _Plan:
     info, table = _plan_tables(rts.starts, rts.ends, rts.route_slot, total_rows, ranks, scales, len(rts.slots))
-    table_dev = table[: max(info.table_words, 1)].to(device, non_blocking=True)
-    return _Plan(info, table_dev, rts.slots, ranks)
+    words = max(info.table_words, 1)
+    table = table[:words]
+    if thresholds is not None:  # behind them, in the same copy
+        more = [thresholds[i] for i, _, _ in _virtual_slots(ranks)]
+        both = torch.empty(words + len(more), dtype=torch.int32, pin_memory=True)
+        both[:words] = table
+        both[words:] = torch.tensor(more, dtype=torch.int32)
+        table = both
+    table_dev = table.to(device, non_blocking=True)
+    return _Plan(info, table_dev, rts.slots, ranks, table_dev.data_ptr() + 4 * words)
 
 
-def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, backward: bool) -> dict:
+def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, captured: int,
+          backward: bool) -> dict:
     """Zero-padded adapter slabs in the layouts the kernels read (cached in the adapter record)."""
     key = (dtype, K, N, device, plan.info.r_pad)
     entry = aset.packs.get(key)
@@ -340,9 +384,12 @@ def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, de
             a_src.append(a if a.is_contiguous() else a.contiguous())
             b_src.append(b if b.is_contiguous() else b.contiguous())
         entry = aset.packs[key] = {"src": (a_src, b_src)}
+    for made in entry.get("made", ()):
+        made.use(device, captured)
     missing = [w for w in want if w not in entry]
     if missing:
         _fill_packs(entry, plan, dtype, K, N, device, missing)
+        entry.setdefault("made", []).append(_Made(device, *(entry[w] for w in missing)))
     return entry
 
 
@@ -380,7 +427,7 @@ def _fill_packs(entry, plan: _Plan, dtype, K, N, device, which) -> None:
         entry.setdefault("ptr_bufs", []).append((ptrs, ranks_dev))
 
 
-def _weight(base_weight: torch.Tensor, dtype, device) -> torch.Tensor:
+def _weight(base_weight: torch.Tensor, dtype, device, captured: int) -> torch.Tensor:
     """Base weight as a contiguous tensor of the activation dtype (converted copies cached)."""
     if isinstance(base_weight, MX4Weight):
         raise ValueError("this call takes a dense base_weight (MX4Weight.dequantize)")
@@ -391,15 +438,17 @@ def _weight(base_weight: torch.Tensor, dtype, device) -> torch.Tensor:
     key = (id(base_weight), dtype)
     hit = _WEIGHT_CACHE.get(key)
     if hit is not None:
-        ref, ptr, ver, conv = hit
+        ref, ptr, ver, conv, made = hit
         if ref() is base_weight and ptr == base_weight.data_ptr() and ver == base_weight._version:
+            made.use(device, captured)
             return conv
     _building("a copy of base_weight", device)
     conv = base_weight.to(dtype).contiguous()
     if len(_WEIGHT_CACHE) >= _CACHE_MAX:
         _WEIGHT_CACHE.clear()
     try:
-        _WEIGHT_CACHE[key] = (weakref.ref(base_weight), base_weight.data_ptr(), base_weight._version, conv)
+        _WEIGHT_CACHE[key] = (weakref.ref(base_weight), base_weight.data_ptr(), base_weight._version, conv,
+                              _Made(device, conv))
     except TypeError:  # pragma: no cover
         pass
     return conv
@@ -428,11 +477,11 @@ def _problem(code, T, K, N, x, w, packs) -> nat.Problem:
     return p
 
 
-def _base(base_weight, x: torch.Tensor):
+def _base(base_weight, x: torch.Tensor, captured: int):
     """(tensor that holds the base weight, whether it is the data of one in 4 bits).  A problem the tensor-core path
     cannot address takes a dense copy of a weight in 4 bits, made within the call."""
     if not isinstance(base_weight, MX4Weight):
-        return _weight(base_weight, x.dtype, x.device), False
+        return _weight(base_weight, x.dtype, x.device, captured), False
     if base_weight.dtype is not x.dtype:
         raise ValueError(f"x ({x.dtype}) must have the dtype of the weight in 4 bits ({base_weight.dtype})")
     if base_weight.device != x.device:
@@ -463,18 +512,10 @@ class _Drop:
         return tuple(s * (65536.0 / (65536 - t)) for s, t in zip(scales, self.thresholds))
 
     def args(self, plan: _Plan, prob, backward: bool, device):
-        """lf_dropout, and what it points at."""
-        table = plan.thresholds.get(self.thresholds)
-        if table is None:
-            _building("the table of dropout thresholds", device)
-            while len(plan.thresholds) >= 8:
-                plan.thresholds.pop(next(iter(plan.thresholds)))
-            host = torch.tensor([self.thresholds[i] for i, _, _ in plan.vslots] or [0], dtype=torch.int32)
-            table = plan.thresholds[self.thresholds] = host.to(device)
-            torch.cuda.current_stream(device).synchronize()  # calls on other streams find it there
+        """lf_dropout, and the scratch that it points at."""
         n = int(nat.lib().lf_dropout_scratch_bytes(ctypes.byref(prob), int(backward)))
         scratch = torch.empty(n, dtype=torch.uint8, device=device) if n else None
-        return nat.Dropout(self.seed, self.offset, table.data_ptr(), scratch.data_ptr() if n else None, n), scratch
+        return nat.Dropout(self.seed, self.offset, plan.thresholds, scratch.data_ptr() if n else None, n), scratch
 
 
 # A float16 rank product s / (1 - p) x A^T must stay below 65504: factors beyond this one, which float16 training would
@@ -522,11 +563,11 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
     captured = _capture(device)
-    w, mx4 = _base(base_weight, x)
+    w, mx4 = _base(base_weight, x, captured)
     if mx4 and x.data_ptr() % 16:
         x = x.detach().clone()
-    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
-    packs = _pack(plan, aset, dtype, K, N, device, backward=False)
+    plan = _plan(rts, aset, T, device, captured, drop)
+    packs = _pack(plan, aset, dtype, K, N, device, captured, backward=False)
     y = torch.empty((T, N), dtype=dtype, device=device)
     if T == 0 or N == 0:
         return y
@@ -617,9 +658,10 @@ class PreparedForward:
         dtype = self.x.dtype
         self.dtype = dtype
         aset = _adapters(rts, lora_a, lora_b, adapters)
-        self.w = _weight(base_weight, dtype, self.device)
-        self.plan = _plan(rts, aset, self.T, self.device)
-        self.packs = _pack(self.plan, aset, dtype, self.K, self.N, self.device, backward=False)
+        captured = _capture(self.device)
+        self.w = _weight(base_weight, dtype, self.device, captured)
+        self.plan = _plan(rts, aset, self.T, self.device, captured)
+        self.packs = _pack(self.plan, aset, dtype, self.K, self.N, self.device, captured, backward=False)
         code = _DTYPE_CODE[dtype]
         L = nat.lib()
         ws_bytes = L.lf_forward_workspace_bytes(ctypes.byref(self.plan.info), code)
@@ -685,11 +727,11 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     captured = _capture(device)
     if captured and peer is not None:  # every call numbers its blocks; replays would repeat the number
         raise RuntimeError("a call with peer cannot be captured into a CUDA graph")
-    w, mx4 = _base(base_weight, x)
+    w, mx4 = _base(base_weight, x, captured)
     if mx4:
         x, g = (t.detach().clone() if t.data_ptr() % 16 else t for t in (x, g))
-    plan = _plan(rts, aset, T, device, drop.scales(aset.scales) if drop else None)
-    packs = _pack(plan, aset, dtype, K, N, device, backward=True)
+    plan = _plan(rts, aset, T, device, captured, drop)
+    packs = _pack(plan, aset, dtype, K, N, device, captured, backward=True)
     info = plan.info
     rtot = info.rank_total
     ext = _peer_layout(plan, peer, device) if peer is not None else None
@@ -814,9 +856,10 @@ class PreparedBackward:
         if gdt not in (dtype, torch.float32):
             raise ValueError(f"grad_dtype must be None, x.dtype or torch.float32, got {grad_dtype}")
         aset = _adapters(rts, lora_a, lora_b, adapters)
-        self.w = _weight(base_weight, dtype, self.device)
-        self.plan = _plan(rts, aset, T, self.device)
-        self.packs = _pack(self.plan, aset, dtype, K, N, self.device, backward=True)
+        captured = _capture(self.device)
+        self.w = _weight(base_weight, dtype, self.device, captured)
+        self.plan = _plan(rts, aset, T, self.device, captured)
+        self.packs = _pack(self.plan, aset, dtype, K, N, self.device, captured, backward=True)
         code = _DTYPE_CODE[dtype]
         self.gcode = _DTYPE_CODE[gdt]
         rtot = self.plan.info.rank_total
@@ -885,7 +928,7 @@ class _ChunkPlans:
     """Row chunks of one routing for the host-streamed forward: per chunk, tables of its routes
     (rebased to the chunk) over the whole batch's slots, as the C ABI's chunk array."""
 
-    __slots__ = ("array", "n", "infos", "tables", "ws_bytes", "launches")
+    __slots__ = ("array", "n", "infos", "tables", "ws_bytes", "launches", "made")
 
     def __init__(self, rts: _Routes, ranks, scales, total_rows: int, chunk_rows: int, device, code: int):
         L = nat.lib()
@@ -910,6 +953,7 @@ class _ChunkPlans:
             self.array[i].info = ctypes.pointer(info)
             self.array[i].table_dev = table_dev.data_ptr()
             self.ws_bytes = max(self.ws_bytes, int(L.lf_forward_workspace_bytes(ctypes.byref(info), code)))
+        self.made = _Made(device, *self.tables)
 
 
 EDGE_CHUNK_ROWS = 256
@@ -933,11 +977,14 @@ def _chunk_bounds(total_rows: int, chunk_rows: int) -> list[int]:
     return bounds
 
 
-def _chunk_plans(rts: _Routes, aset: _AdapterSet, total_rows: int, chunk_rows: int, device, code: int) -> _ChunkPlans:
+def _chunk_plans(rts: _Routes, aset: _AdapterSet, total_rows: int, chunk_rows: int, device, code: int,
+                 captured: int) -> _ChunkPlans:
     key = (chunk_rows, total_rows, aset.ranks, aset.scales, device, code)
     for k, v in rts.chunk_plans:
         if k == key:
+            v.made.use(device, captured)
             return v
+    _building("the chunks' tables", device)
     plans = _ChunkPlans(rts, aset.ranks, aset.scales, total_rows, chunk_rows, device, code)
     rts.chunk_plans.insert(0, (key, plans))
     del rts.chunk_plans[4:]
@@ -987,10 +1034,11 @@ def fused_lora_forward_host(x_host, base_weight, lora_a, lora_b, adapters, routi
         x_host = x_host.contiguous()
     code = _DTYPE_CODE[dtype]
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    w = _weight(base_weight, dtype, device)
-    plan = _plan(rts, aset, T, device)
-    packs = _pack(plan, aset, dtype, K, N, device, backward=False)
-    chunks = _chunk_plans(rts, aset, T, chunk_rows, device, code)
+    captured = _capture(device)
+    w = _weight(base_weight, dtype, device, captured)
+    plan = _plan(rts, aset, T, device, captured)
+    packs = _pack(plan, aset, dtype, K, N, device, captured, backward=False)
+    chunks = _chunk_plans(rts, aset, T, chunk_rows, device, code, captured)
     x_dev = torch.empty((T, K), dtype=dtype, device=device)
     y_dev = torch.empty((T, N), dtype=dtype, device=device)
     ws = torch.empty(chunks.ws_bytes, dtype=torch.uint8, device=device)

@@ -226,6 +226,29 @@ PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return PyLong_FromUnsignedLongLong(status == cudaStreamCaptureStatusActive ? id : 0);
 }
 
+// wait_event(cudaEvent_t): the host waits for an event recorded outside the capture that this thread may be in.
+PyObject* wait_event(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1) {
+    PyErr_SetString(PyExc_TypeError, "wait_event takes 1 argument");
+    return nullptr;
+  }
+  void* event = PyLong_AsVoidPtr(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // a wait here is none of the captured work
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) {
+    Py_BEGIN_ALLOW_THREADS
+    e = cudaEventSynchronize(static_cast<cudaEvent_t>(event));
+    Py_END_ALLOW_THREADS
+    cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+  if (e != cudaSuccess) {
+    PyErr_Format(PyExc_RuntimeError, "wait_event: %s", cudaGetErrorString(e));
+    return nullptr;
+  }
+  Py_RETURN_NONE;
+}
+
 // bank_load(bank_a, bank_b, ranks, scales, slot, lora_a, lora_b, scaling): an adapter into its slot.  None unless its
 // tensors have the bank's dtype and device and dense rows; shapes were checked by the caller.
 PyObject* bank_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -504,6 +527,7 @@ PyMethodDef methods[] = {
     {"mx4_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_quantize>)), METH_FASTCALL, nullptr},
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_dequantize>)), METH_FASTCALL, nullptr},
     {"capture_id", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<capture_id>)), METH_FASTCALL, nullptr},
+    {"wait_event", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<wait_event>)), METH_FASTCALL, nullptr},
     {"bank_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<bank_load>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},
     {"gather_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<gather_step>)), METH_FASTCALL, nullptr},

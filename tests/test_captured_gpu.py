@@ -142,3 +142,85 @@ def test_a_call_with_peer_is_not_captured():
     with pytest.raises(RuntimeError, match="peer"):
         captured(lambda: p.backward(peer=Peer()))
     torch.cuda.synchronize()
+
+
+def test_nine_rates_of_an_adapter_whose_factor_stays_zero():
+    """With alpha = 0 its factor is 0 whatever its rate: calls of other rates share all but the thresholds, and push
+    nothing out that a captured call reads."""
+    p = Problem(alpha=0.0)
+
+    def drop(n):
+        return AdapterDropout({0: n / 16, 1: 0.25}, 11, 3)
+
+    p.forward(dropout=drop(1)), p.backward(dropout=drop(1))
+    fw, y = captured(lambda: p.forward(dropout=drop(1)))
+    bw, back = captured(lambda: p.backward(dropout=drop(1)))
+    for n in range(2, 16):
+        p.forward(dropout=drop(n)), p.backward(dropout=drop(n))
+        torch.full((4096,), -1, dtype=torch.int32, device=DEV)
+    filler = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in (1, 2, 64, 128, 500, 512, 1024) for _ in range(64)]
+    want_y, want = p.forward(dropout=drop(1)), p.backward(dropout=drop(1))
+    fw.replay()
+    bw.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want_y)
+    same(back, want)
+    del filler
+    # adapter 1's rate is 1/4 whatever adapter 0's is
+    for n in (1, 9):
+        assert torch.equal(p.forward(dropout=drop(n))[100:], want_y[100:])
+    assert nat.device_error() == 0
+
+
+def busy(stream, ms=200):
+    """Work of some length on the stream; an event behind it."""
+    with torch.cuda.stream(stream):
+        torch.cuda._sleep(int(ms * 1e6 * 1.9))
+        event = torch.cuda.Event()
+        event.record(stream)
+    return event
+
+
+@pytest.mark.parametrize("mx4", [False, True])
+def test_a_new_routing_does_not_wait_for_the_gpu(mx4):
+    """A trainer packs other rows every step: its calls enqueue behind what is queued."""
+    p = Problem(mx4, 0.3)
+    p.forward(), p.backward()
+    for n in range(4):  # what the first new routing allocates is cached from here on
+        p.routing = TileRoutingConfig(128, [TileRoute(0, 110 + n, 0), TileRoute(110 + n, 300, 1)])
+        p.forward(), p.backward()
+    torch.cuda.synchronize()
+    done = busy(torch.cuda.current_stream())
+    for n in range(2):
+        p.routing = TileRoutingConfig(128, [TileRoute(0, 120 + n, 0), TileRoute(120 + n, 300, 1)])
+        y, back = p.forward(), p.backward()
+    assert not done.query()
+    torch.cuda.synchronize()
+    want_y, want = p.forward(), p.fresh()
+    assert torch.equal(y, want_y)
+    same(back, want)
+
+
+@pytest.mark.parametrize("mx4,rate", ALL)
+def test_tables_and_slabs_made_on_a_stream_that_is_behind(mx4, rate):
+    """The first call's tables and slabs are still to be written when a call on another stream takes them from the caches,
+    and the caches drop them before that has run."""
+    p = Problem(mx4, rate, seed=60)
+    want_y, want = p.forward(), p.fresh()
+    torch.cuda.synchronize()
+    ops.clear_weight_cache()
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    done = busy(first)
+    with torch.cuda.stream(first):
+        p.forward(), p.fresh()
+    with torch.cuda.stream(second):
+        y, back = p.forward(), p.fresh()
+    ops.clear_weight_cache()
+    with torch.cuda.stream(first):
+        filler = [torch.full((n,), -1, dtype=torch.int32, device=DEV) for n in (64, 128, 500, 512, 4096, 1 << 16) for _ in range(16)]
+    assert not done.query()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want_y)
+    same(back, want)
+    del filler
+    assert nat.device_error() == 0
