@@ -86,8 +86,9 @@ _last_launches = 0
 # x has died are dropped on the next insertion
 _SAVED_SF: "OrderedDict[tuple, tuple]" = OrderedDict()
 _SAVED_MAX = 1024
-# (plan, packed slabs, base weight) of calls captured into CUDA graphs: the replays read them, whatever the caches drop
-_CAPTURED: list = []
+# per capture into a CUDA graph: plans, packed slabs and base weights by id, which its replays read whatever the caches
+# drop, for as long as the graph (or one instantiated from it) lives
+_CAPTURED: dict[int, dict] = {}
 _VERSION = torch.Tensor._version.__get__
 _DATA_PTR = torch.Tensor.data_ptr
 
@@ -107,14 +108,14 @@ def use_cooperative_launch(enabled: bool, shrink_prologue: bool = False) -> None
 
 
 def clear_weight_cache() -> None:
-    """Drop every cached table, packed adapter slab and converted weight, those of captured calls too (their graphs must
-    not be replayed any more)."""
+    """Drop every cached table, packed adapter slab and converted weight.  What captured calls read stays for as long as
+    their graphs live."""
     _ROUTE_CACHE.clear()
     _ADAPTER_CACHE.clear()
     _PLAN_BY_CONTENT.clear()
     _SAVED_SF.clear()
     _WEIGHT_CACHE.clear()
-    _CAPTURED.clear()
+    _drop_ended()
 
 
 def release() -> None:
@@ -303,9 +304,27 @@ def _adapters(rts: _Routes, lora_a, lora_b, adapters) -> _AdapterSet:
     return rec
 
 
+def _drop_ended() -> None:
+    """Lets go of what captures held whose graphs are gone."""
+    if _CAPTURED:
+        for capture in nat.glue().ended():
+            _CAPTURED.pop(capture, None)
+            for k in [k for k, v in _SAVED_SF.items() if v[-1] == capture]:
+                del _SAVED_SF[k]
+
+
 def _capture(device) -> int:
     """The capture into a CUDA graph that the device's current stream is in, 0 for none."""
+    _drop_ended()
     return nat.glue().capture_id(device.index)
+
+
+def _hold(captured: int, device, *read) -> None:
+    """Keeps what a captured call reads for as long as its graph lives."""
+    held = _CAPTURED.get(captured)
+    if held is None:
+        held = _CAPTURED[nat.glue().hold_capture(device.index)] = {}
+    held.update((id(o), o) for o in read)
 
 
 def _building(what: str, device) -> None:
@@ -584,12 +603,12 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     stream = nat.raw_stream(device.index)
     planes = ctypes.c_int32(0)
     opt, keep = _options(mx4, drop, plan, prob, False, device)
-    if captured:
-        _CAPTURED.append((plan, packs, w))
     with nat.on_device(device.index):
         rc = L.lf_forward_opt(ctypes.byref(prob), info, plan.table_dev.data_ptr(), opt, y.data_ptr(), ws.data_ptr(),
                               ws.numel(), tail.data_ptr(), tail.numel(), ctypes.byref(planes), stream)
     nat.check(rc, "lf_forward_opt")
+    if captured:
+        _hold(captured, device, plan, packs, base_weight.data if isinstance(base_weight, MX4Weight) else w)
     # 2 K-half planes: shrink inside the GEMM launch (1 launch); 1: shrink launched on its own
     _last_launches = {2: 1, 1: 2}.get(planes.value) or int(L.lf_forward_launch_count(ctypes.byref(prob), info))
     if drop is not None:
@@ -758,8 +777,6 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
         pr.slot_span_dev = ext.slot_span.data_ptr()
         pr.span_info_dev = ext.span_info.data_ptr()
     opt, keep = _options(mx4, drop, plan, prob, True, device)
-    if captured:
-        _CAPTURED.append((plan, packs, w))
     with nat.on_device(device.index):
         rc = L.lf_backward_opt(ctypes.byref(prob), ctypes.byref(info), plan.table_dev.data_ptr(), opt, g.data_ptr(),
                                sf_ptr, sf_planes, _DTYPE_CODE[gdt], grad_x.data_ptr(), ga_flat.data_ptr(),
@@ -767,6 +784,8 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     if saved is not None:
         saved[0].record_stream(torch.cuda.current_stream(device))
     nat.check(rc, "lf_backward_opt")
+    if captured:
+        _hold(captured, device, plan, packs, base_weight.data if isinstance(base_weight, MX4Weight) else w)
     n_launch = max(0, int(L.lf_backward_launch_count(ctypes.byref(prob), ctypes.byref(info))))
     _last_launches = n_launch - 1 if saved is not None and n_launch == 4 else n_launch
     if drop is not None:

@@ -15,6 +15,8 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cstring>
+#include <memory>
+#include <mutex>
 #include <vector>
 
 #include "../../include/lorafusion_b200.h"
@@ -224,6 +226,86 @@ PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
     status = cudaStreamCaptureStatusNone;
   }
   return PyLong_FromUnsignedLongLong(status == cudaStreamCaptureStatusActive ? id : 0);
+}
+
+// Captures whose graphs are gone, until ended() takes them.  Never destroyed: graphs may outlive the module.
+struct Ended {
+  std::mutex lock;
+  std::vector<unsigned long long> ids;
+};
+Ended& ended_captures() {
+  static Ended* e = new Ended;
+  return *e;
+}
+struct Token {
+  unsigned long long id;
+};
+void CUDART_CB capture_ended(void* p) {  // on a thread of CUDA's, which must make no CUDA call
+  Token* token = static_cast<Token*>(p);
+  Ended& e = ended_captures();
+  try {
+    const std::lock_guard<std::mutex> hold(e.lock);
+    e.ids.push_back(token->id);
+  } catch (...) {  // what the capture held stays held
+  }
+  delete token;
+}
+
+// hold_capture(device index): the id of the capture that the device's current stream is in, for ended() to return once its
+// graph, every graph instantiated from it and their launches are over.
+PyObject* hold_capture(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  if (n != 1) {
+    PyErr_SetString(PyExc_TypeError, "hold_capture takes 1 argument");
+    return nullptr;
+  }
+  const long dev = PyLong_AsLong(a[0]);
+  if (PyErr_Occurred()) return nullptr;
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  cudaGraph_t graph = nullptr;
+  cudaError_t e = cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(),
+                                           &status, &id, &graph);
+  if (e == cudaSuccess && status != cudaStreamCaptureStatusActive) e = cudaErrorIllegalState;
+  if (e == cudaSuccess) {
+    std::unique_ptr<Token> token(new Token{id});
+    cudaUserObject_t object = nullptr;
+    e = cudaUserObjectCreate(&object, token.get(), capture_ended, 1, cudaUserObjectNoDestructorSync);
+    if (e == cudaSuccess) {
+      token.release();  // the object's
+      e = cudaGraphRetainUserObject(graph, object, 1, cudaGraphUserObjectMove);
+      if (e != cudaSuccess) cudaUserObjectRelease(object, 1);
+    }
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    PyErr_Format(PyExc_RuntimeError, "hold_capture: %s", cudaGetErrorString(e));
+    return nullptr;
+  }
+  return PyLong_FromUnsignedLongLong(id);
+}
+
+// ended(): ids of captures that are over since the last call.
+PyObject* ended(PyObject*, PyObject* const*, Py_ssize_t n) {
+  if (n != 0) {
+    PyErr_SetString(PyExc_TypeError, "ended takes no arguments");
+    return nullptr;
+  }
+  std::vector<unsigned long long> ids;
+  {
+    Ended& e = ended_captures();
+    const std::lock_guard<std::mutex> hold(e.lock);
+    ids.swap(e.ids);
+  }
+  PyObject* out = PyTuple_New(static_cast<Py_ssize_t>(ids.size()));
+  for (size_t i = 0; out && i < ids.size(); ++i) {
+    PyObject* id = PyLong_FromUnsignedLongLong(ids[i]);
+    if (!id) {
+      Py_DECREF(out);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(out, static_cast<Py_ssize_t>(i), id);
+  }
+  return out;
 }
 
 // wait_event(cudaEvent_t): the host waits for an event recorded outside the capture that this thread may be in.
@@ -527,6 +609,8 @@ PyMethodDef methods[] = {
     {"mx4_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_quantize>)), METH_FASTCALL, nullptr},
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_dequantize>)), METH_FASTCALL, nullptr},
     {"capture_id", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<capture_id>)), METH_FASTCALL, nullptr},
+    {"hold_capture", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<hold_capture>)), METH_FASTCALL, nullptr},
+    {"ended", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<ended>)), METH_FASTCALL, nullptr},
     {"wait_event", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<wait_event>)), METH_FASTCALL, nullptr},
     {"bank_load", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<bank_load>)), METH_FASTCALL, nullptr},
     {"clip", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<clip>)), METH_FASTCALL, nullptr},

@@ -1,5 +1,9 @@
 """Calls captured into CUDA graphs: what they may take from eager calls, and eager calls from them."""
 
+import gc
+import time
+import weakref
+
 import pytest
 import torch
 
@@ -224,3 +228,63 @@ def test_tables_and_slabs_made_on_a_stream_that_is_behind(mx4, rate):
     same(back, want)
     del filler
     assert nat.device_error() == 0
+
+
+def gone(count=0, seconds=20.0):
+    """Waits until captures are let go of (CUDA tells from a thread of its own)."""
+    end = time.monotonic() + seconds
+    while len(ops._CAPTURED) > count and time.monotonic() < end:
+        time.sleep(0.01)
+        ops._drop_ended()
+    return len(ops._CAPTURED)
+
+
+@pytest.mark.parametrize("mx4", [False, True])
+def test_a_capture_holds_what_it_reads_as_long_as_its_graph_lives(mx4):
+    """Once for the graph, however many calls are in it, and nothing of a graph that is gone."""
+    gc.collect()
+    torch.cuda.synchronize()
+    before = gone()
+    assert before == 0
+    p = Problem(mx4, 0.3, seed=70)
+    p.forward(), p.backward()
+    want_y, want = p.forward(), p.fresh()
+    graph, (y, back) = captured(lambda: [(p.forward(), p.backward()) for _ in range(6)][-1])
+    held, = ops._CAPTURED.values()
+    # one plan, one entry of slabs, one weight
+    assert len(held) == 3
+    ref = weakref.ref(next(v for v in held.values() if isinstance(v, torch.Tensor)))
+    # dropped caches, and other calls over the same memory, do not touch what it reads
+    ops.clear_weight_cache()
+    p.w = quantize_weight(rand(192, 256, seed=99)) if mx4 else rand(192, 256, seed=99)
+    p.a, p.b = {i: t * 2 for i, t in p.a.items()}, {i: t * 2 for i, t in p.b.items()}
+    for n in range(20):
+        Problem(mx4, 0.2, T=140 + n, seed=100 + n).forward()
+    assert ref() is not None
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want_y)
+    same(back, want)
+    del held, y, back
+    graph.replay()
+    graph.reset()
+    assert gone() == 0 and ref() is None
+    assert not any(v[-1] for v in ops._SAVED_SF.values())
+    assert nat.device_error() == 0
+
+
+def test_many_captures_leave_nothing_behind():
+    p = Problem(True, 0.3, seed=80)
+    p.forward(), p.backward()
+    for _ in range(12):
+        captured(lambda: (p.forward(), p.backward()))
+    gc.collect()
+    torch.cuda.synchronize()
+    assert gone() == 0
+    # a capture that fails is let go of as well
+    other = Problem(True, 0.3, T=140, seed=81)
+    with pytest.raises(RuntimeError, match="once before"):
+        captured(lambda: (p.forward(), other.forward()))
+    gc.collect()
+    torch.cuda.synchronize()
+    assert gone() == 0
