@@ -558,12 +558,15 @@ typedef struct lf_mx4_problem {
   const void* mx4_dev;  /* lf_mx4_bytes(N, K) */
 } lf_mx4_problem;
 
-/* Workspace bytes of lf_mx4_linear (16-byte aligned buffer).  Where K and N are multiples of 8 it is optional: with less,
- * or null, the last round of tiles is not split.  Elsewhere it takes a dense copy of the weight. */
+/* Workspace bytes of lf_mx4_linear (16-byte aligned buffer) where ld is a multiple of 8 and in and out are 16-byte aligned.
+ * With K and N multiples of 8 it is optional then: with less, or null, the last round of tiles is not split.  On CUDA
+ * cores (below) the call takes a dense copy of the weight, 2 K N bytes, whatever K and N are: LF_ERR_CAPACITY with
+ * less. */
 LF_API size_t lf_mx4_linear_workspace_bytes(int32_t K, int32_t N);
 
-/* A product with a weight in 4 bits; out is dense and shares no memory with the operands.  With K, N and ld multiples of
- * 8 and 16-byte aligned buffers it runs on the tensor cores in one launch, otherwise in two on CUDA cores. */
+/* A product with a weight in 4 bits; out is dense; out and the workspace share no memory with the operands or each other.
+ * With K, N and ld multiples of 8 and 16-byte aligned buffers it runs on the tensor cores in one launch, otherwise in two
+ * on CUDA cores. */
 LF_API int lf_mx4_linear(const lf_mx4_problem* prob, void* out_dev, void* workspace_dev, size_t workspace_bytes,
                          lf_stream_t stream);
 

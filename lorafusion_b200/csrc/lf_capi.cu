@@ -1245,14 +1245,18 @@ extern "C" int lf_mx4_linear(const lf_mx4_problem* p, void* out_dev, void* works
   if (meet(out_dev, out_bytes, p->in_dev, (static_cast<size_t>(T - 1) * p->ld + in) * 2) ||
       meet(out_dev, out_bytes, p->mx4_dev, mx4_bytes(N, K)))
     return LF_ERR_INVALID_ARG;
+  const bool cores = K % 8 || N % 8 || p->ld % 8 || !aligned16(p->in_dev) || !aligned16(out_dev);
+  const size_t dense = static_cast<size_t>(N) * K * 2;
+  if (cores && (!workspace_dev || workspace_bytes < dense)) return LF_ERR_CAPACITY;
+  const size_t used = cores ? dense : workspace_bytes < tail_scratch_bytes() ? workspace_bytes : tail_scratch_bytes();
+  if (workspace_dev && (meet(workspace_dev, used, p->in_dev, (static_cast<size_t>(T - 1) * p->ld + in) * 2) ||
+                        meet(workspace_dev, used, p->mx4_dev, mx4_bytes(N, K)) ||
+                        meet(workspace_dev, used, out_dev, out_bytes)))
+    return LF_ERR_INVALID_ARG;
   DeviceState* ds = nullptr;
   if (device_state(&ds) != cudaSuccess) return LF_ERR_CUDA;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (K % 8 || N % 8 || p->ld % 8 || !aligned16(p->in_dev) || !aligned16(out_dev)) {
-    const size_t dense = static_cast<size_t>(N) * K * 2;
-    if (!workspace_dev || workspace_bytes < dense) return LF_ERR_CAPACITY;
-    if (meet(workspace_dev, dense, p->mx4_dev, mx4_bytes(N, K)) || meet(workspace_dev, dense, out_dev, out_bytes))
-      return LF_ERR_INVALID_ARG;
+  if (cores) {
     cudaError_t e = mx4_dequantize(dt, p->mx4_dev, N, K, workspace_dev, ds->num_sms, st);
     const int64_t qsn = p->transpose ? 1 : K, qsk = p->transpose ? K : 1;
     if (e == cudaSuccess)

@@ -1,0 +1,49 @@
+"""lf_mx4_linear by the C ABI and at sizes its tests leave out, against 64-bit arithmetic.  A 16-bit result is off by at most
+half a step and ``n 2^-24`` of its sum of n magnitudes; the values of the weight are exact."""
+
+import pytest
+import torch
+
+from lorafusion_b200 import _native as nat
+from lorafusion_b200.quant import quantize_weight
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF16 = torch.bfloat16
+
+
+def rand(*shape, seed=0, scale=1.0, dtype=BF16):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=gen, device=DEV) * scale).to(dtype)
+
+
+def check(got, left, right):
+    ref, mag = left.double() @ right, left.double().abs() @ right.abs()
+    half = torch.finfo(got.dtype).eps / 2
+    bound = half * ref.abs() + (left.shape[1] * 2.0 ** -24) * mag * (1 + half)
+    assert torch.isfinite(got).all() and ((got.double() - ref).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("transpose", [0, 1])
+def test_a_pitch_that_only_cuda_cores_take(transpose):
+    """K and N are multiples of 8, the rows' pitch is not: the workspace is a dense copy's."""
+    T, K, N = 30, 256, 320
+    q = quantize_weight(rand(N, K, seed=1, scale=1 / 16))
+    v = q.dequantize().double()
+    width, out = (N, K) if transpose else (K, N)
+    x = rand(T, width + 3, seed=2)[:, :width]
+    y = torch.empty(T, out, dtype=BF16, device=DEV)
+    p = nat.Mx4Problem(nat.LF_BF16, T, K, N, transpose, 0, x.stride(0), x.data_ptr(), q.data.data_ptr())
+    ws = torch.empty(2 * K * N, dtype=torch.uint8, device=DEV)
+    stream = nat.raw_stream(0)
+    assert nat.lib().lf_mx4_linear(p, y.data_ptr(), ws.data_ptr(), ws.numel() - 1, stream) == nat.LF_ERR_CAPACITY
+    nat.check(nat.lib().lf_mx4_linear(p, y.data_ptr(), ws.data_ptr(), ws.numel(), stream), "lf_mx4_linear")
+    torch.cuda.synchronize()
+    check(y, x, v if transpose else v.t())
+    # operands of the tensor cores need none
+    x = x.contiguous()
+    p.ld, p.in_dev = width, x.data_ptr()
+    nat.check(nat.lib().lf_mx4_linear(p, y.data_ptr(), None, 0, stream), "lf_mx4_linear")
+    torch.cuda.synchronize()
+    check(y, x, v if transpose else v.t())
+    assert nat.device_error() == 0
