@@ -1756,7 +1756,7 @@ bool rows_use_pairs(int T, int K, int N, int num_sms) {
 // 1000 -> 1048 16 us against 26, 512 rows 4096 -> 4096 28 against 36, 1024 rows 41 against 42), the pairs beyond that (700 rows
 // 8192 -> 8192 96 against 121, 4096 rows 4096 -> 4096 119 against 141).
 bool mx4_use_pairs(int T, int N, int num_sms) {
-  return T > 256 && static_cast<int64_t>((T + 255) / 256) * ((N + kWRows - 1) / kWRows) > num_sms;
+  return T > 256 && (static_cast<int64_t>(T) + 255) / 256 * ((N + kWRows - 1) / kWRows) > num_sms;
 }
 
 cudaError_t bank_load(const BankLoad& p, int dtype, int num_sms, cudaStream_t st) {

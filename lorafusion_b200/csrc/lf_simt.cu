@@ -94,7 +94,10 @@ __global__ void __launch_bounds__(SG_T) simt_gemm_kernel(const T* __restrict__ P
   constexpr int kLoads = kB * kK / SG_T;
   __shared__ double ps[kK][kB + 1];
   __shared__ double qs[kK][kB + 1];
-  const int m0 = blockIdx.y * kB, n0 = blockIdx.x * kB;
+  // row tiles run along y, and along z where a grid's y (65535) is not enough
+  const int64_t tile_m = (static_cast<int64_t>(blockIdx.z) * gridDim.y + blockIdx.y) * kB;
+  if (tile_m >= Trows) return;
+  const int m0 = static_cast<int>(tile_m), n0 = blockIdx.x * kB;
   const int tid = threadIdx.x;
   const int tr = tid / kSide, tc = tid % kSide;
   double acc[kT][kT] = {};
@@ -276,9 +279,11 @@ cudaError_t simt_gemm(int dtype, const void* P, int64_t ldp, const void* Q, int6
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e != cudaSuccess) return e;
-  const bool large = static_cast<int64_t>((Nout + 63) / 64) * ((T + 63) / 64) >= sms;
+  const bool large = static_cast<int64_t>((Nout + 63) / 64) * ((static_cast<int64_t>(T) + 63) / 64) >= sms;
   const int side = large ? 64 : 16;
-  const dim3 grid((Nout + side - 1) / side, (T + side - 1) / side);
+  const int64_t tiles = (static_cast<int64_t>(T) + side - 1) / side;
+  const unsigned rows = static_cast<unsigned>(tiles < 65535 ? tiles : 65535);
+  const dim3 grid((Nout + side - 1) / side, rows, static_cast<unsigned>((tiles + rows - 1) / rows));
   auto run = [&](auto zero) {
     using E = decltype(zero);
     auto* k = large ? simt_gemm_kernel<E, 64, 4, 16> : simt_gemm_kernel<E, 16, 1, 32>;

@@ -2603,7 +2603,7 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
   p.T = T;
   p.Nout = Nout;
   p.Kred = Kred;
-  const int n_mtiles = (T + kBM - 1) / kBM;
+  const int n_mtiles = T / kBM + (T % kBM != 0);
   p.n_mpairs = (n_mtiles + 1) / 2;
   p.n_ntiles = (Nout + 255) / 256;
   // Raster groups of row pairs (tiles of a group go column block by column block, the row pairs

@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from lorafusion_b200 import _native as nat
-from lorafusion_b200.quant import quantize_weight
+from lorafusion_b200.quant import mx4_linear, mx4_linear_backward, quantize_weight
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -45,5 +45,17 @@ def test_a_pitch_that_only_cuda_cores_take(transpose):
     p.ld, p.in_dev = width, x.data_ptr()
     nat.check(nat.lib().lf_mx4_linear(p, y.data_ptr(), None, 0, stream), "lf_mx4_linear")
     torch.cuda.synchronize()
+    check(y, x, v if transpose else v.t())
+    assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("transpose", [False, True])
+def test_more_rows_than_one_dimension_of_a_grid(transpose):
+    """4,194,240 rows are 65,535 tiles of 64 on CUDA cores."""
+    T, K, N = 4_194_240 + 150, 9, 10
+    q = quantize_weight(rand(N, K, seed=3))
+    v = q.dequantize().double()
+    x = rand(T, N if transpose else K, seed=4)
+    y = (mx4_linear_backward if transpose else mx4_linear)(x, q)
     check(y, x, v if transpose else v.t())
     assert nat.device_error() == 0
