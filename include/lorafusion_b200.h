@@ -570,6 +570,10 @@ LF_API size_t lf_mx4_linear_workspace_bytes(int32_t K, int32_t N);
 LF_API int lf_mx4_linear(const lf_mx4_problem* prob, void* out_dev, void* workspace_dev, size_t workspace_bytes,
                          lf_stream_t stream);
 
+/* Parts along the reduction that lf_mx4_linear, with all of its workspace, cuts the tiles of its last round into on a GPU of
+ * num_sms SMs: 1 to 3, or 0 where the call takes another kernel than the CTA pairs' (host only). */
+LF_API int lf_mx4_linear_tail_parts(int32_t T, int32_t K, int32_t N, int32_t transpose, int32_t num_sms);
+
 /*
  * Dropout of the adapters' input: y = x W^T + s_i (m x) A_i^T B_i^T, and in the backward grad_x = g W + m (s_i g B_i A_i),
  * grad_A_i from m x, grad_B_i from s_i (m x) A_i^T.  The factor 1 / (1 - p_i) belongs into s_i (lf_plan_tables' scales).

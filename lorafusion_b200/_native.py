@@ -219,6 +219,8 @@ def _declare(L: ctypes.CDLL) -> None:
     L.lf_mx4_linear_workspace_bytes.restype = ctypes.c_size_t
     L.lf_mx4_linear.argtypes = [P(Mx4Problem), _c_p, _c_p, ctypes.c_size_t, _c_p]
     L.lf_mx4_linear.restype = ctypes.c_int
+    L.lf_mx4_linear_tail_parts.argtypes = [_c_i32, _c_i32, _c_i32, _c_i32, _c_i32]
+    L.lf_mx4_linear_tail_parts.restype = ctypes.c_int
     L.lf_dropout_scratch_bytes.argtypes = [P(Problem), _c_i32]
     L.lf_dropout_scratch_bytes.restype = ctypes.c_size_t
     L.lf_forward_opt.argtypes = [P(Problem), P(PlanInfo), _c_p, P(Options), _c_p, _c_p, ctypes.c_size_t, _c_p,

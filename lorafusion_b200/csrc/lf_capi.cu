@@ -1231,6 +1231,12 @@ extern "C" size_t lf_mx4_linear_workspace_bytes(int32_t K, int32_t N) {
   return K % 8 || N % 8 ? align256(static_cast<size_t>(N) * static_cast<size_t>(K) * 2) : tail_scratch_bytes();
 }
 
+extern "C" int lf_mx4_linear_tail_parts(int32_t T, int32_t K, int32_t N, int32_t transpose, int32_t num_sms) {
+  if (T <= 0 || K <= 0 || N <= 0 || K % 8 || N % 8 || num_sms < 2) return 0;
+  if (!transpose && !mx4_use_pairs(T, N, num_sms)) return 0;
+  return transpose ? pair_tail_parts(T, K, N, num_sms, true) : pair_tail_parts(T, N, K, num_sms, true);
+}
+
 extern "C" int lf_mx4_linear(const lf_mx4_problem* p, void* out_dev, void* workspace_dev, size_t workspace_bytes,
                              lf_stream_t stream) {
   if (!p || p->T < 0 || (p->transpose != 0 && p->transpose != 1)) return LF_ERR_INVALID_ARG;

@@ -128,6 +128,8 @@ struct PairMx4 {
 };
 // CTA pairs the pair GEMM can leave to a co-scheduled shrink without adding a round (0: none).
 int pair_spare_pairs(int T, int Nout, int num_sms, int n_units);
+// Parts along K of each tile of the last round, 1 where it is not cut: without a shrink, with all of the tail's scratch.
+int pair_tail_parts(int T, int Nout, int Kred, int num_sms, bool mx4);
 // `tail` (optional) enables the K-split tail; the launch is then cooperative.  `behind_shrink`: the launch ahead of this one
 // is the tc_shrink that writes S; where the launch is not cooperative its tiles start beside it.  `s_lo`: S enters with its
 // low halves (of a shrink with dropout, which leaves their zero tile too).

@@ -2592,6 +2592,32 @@ int pair_spare_pairs(int T, int Nout, int num_sms, int n_units) {
   return spare >= 4 ? spare : 0;  // below 8 SMs the shrink would hold up the first round
 }
 
+namespace {
+// The tail tiles are cut along K when the last round is at most half full (or there are fewer tiles than pairs), into
+// as many parts (each >= 2 k-blocks) as the idle pairs and the partial slots allow: at most four, three over a weight in
+// 4 bits, whose ring has no room for a fourth part's buffers.
+struct TailCut {
+  int parts;
+  bool few;  // fewer tiles than pairs: all of them are tail tiles
+};
+TailCut tail_cut(int total, int all_pairs, int gemm_pairs, int shrink_pairs, int nkb, int slots, bool mx4) {
+  const bool few = total < gemm_pairs || (shrink_pairs == 0 && total < all_pairs);
+  const int avail = few && shrink_pairs == 0 ? all_pairs : gemm_pairs;
+  const int rem = few ? total : total - (total / gemm_pairs) * gemm_pairs;
+  int parts = rem > 0 && 2 * rem <= avail ? avail / rem : 1;
+  const int most = mx4 ? 3 : 4;
+  if (parts > most) parts = most;
+  while (parts > 1 && (rem * (parts - 1) > slots || nkb < 2 * parts)) --parts;
+  return {parts, few};
+}
+}  // namespace
+
+int pair_tail_parts(int T, int Nout, int Kred, int num_sms, bool mx4) {
+  const int m = T / kBM + (T % kBM != 0), total = (m + 1) / 2 * ((Nout + 255) / 256), pairs = num_sms / 2;
+  if (total == 0 || pairs == 0) return 1;
+  return tail_cut(total, pairs, total < pairs ? total : pairs, 0, (Kred + kBK - 1) / kBK, kTailSlots, mx4).parts;
+}
+
 cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, int Nout, int Kred, bool lora,
                          const Tables& tb, void* out, int64_t ldo, int num_sms, cudaStream_t st,
                          const PairShrink* shrink, const PairTail* tail, const PairDelta* delta, const PairMx4* mx4,
@@ -2657,19 +2683,10 @@ cudaError_t tc_gemm_pair(int dtype, bool q_mn_major, const TcMaps& maps, int T, 
     }
   }
   if (tail != nullptr && tail->slots > 0) {
-    // Cut the tail tiles along K when the last round is at most half full (or there are fewer
-    // tiles than pairs), into as many parts (<= 4, each >= 2 k-blocks) as the idle pairs and the
-    // partial slots allow.
-    const bool few = total < gemm_pairs || (p.n_shrink_pairs == 0 && total < all_pairs);
-    const int avail = few && p.n_shrink_pairs == 0 ? all_pairs : gemm_pairs;
-    const int rem = few ? total : total - (total / gemm_pairs) * gemm_pairs;
-    int parts = rem > 0 && 2 * rem <= avail ? avail / rem : 1;
-    const int most = mx4 != nullptr ? 3 : 4;
-    if (parts > most) parts = most;
-    while (parts > 1 && (rem * (parts - 1) > tail->slots || nkb < 2 * parts)) --parts;
-    if (parts > 1) {
-      if (few) gemm_pairs = total * parts;  // every tile is a tail tile, one part per pair
-      p.tail_parts = parts;
+    const TailCut cut = tail_cut(total, all_pairs, gemm_pairs, p.n_shrink_pairs, nkb, tail->slots, mx4 != nullptr);
+    if (cut.parts > 1) {
+      if (cut.few) gemm_pairs = total * cut.parts;  // every tile is a tail tile, one part per pair
+      p.tail_parts = cut.parts;
       p.tail_partial = tail->partial;
       p.tail_flag = tail->flags;
       if (p.n_shrink_pairs == 0 && !p.shrink_prologue) p.gen = tail->gen;  // else the shrink's serves both

@@ -59,3 +59,27 @@ def test_more_rows_than_one_dimension_of_a_grid(transpose):
     y = (mx4_linear_backward if transpose else mx4_linear)(x, q)
     check(y, x, v if transpose else v.t())
     assert nat.device_error() == 0
+
+
+@pytest.mark.parametrize("T,red,out,parts,transpose", [
+    (1792, 384, 3584, 3, 0), (2048, 1000, 3328, 2, 0), (2300, 640, 2552, 3, 0), (2304, 256, 2560, 2, 0), (2304, 192, 2560, 1, 0),
+    (1792, 384, 3584, 3, 1), (2048, 1000, 3328, 2, 1), (2300, 640, 2552, 3, 1), (2304, 256, 2560, 2, 1),
+    (1024, 512, 1536, 3, 1), (1280, 2048, 1536, 2, 1), (3, 4096, 1000, 3, 1)])
+def test_a_last_round_cut_along_the_reduction(T, red, out, parts, transpose):
+    """Two and three parts in either direction, and the same sizes without the scratch for it."""
+    K, N = (out, red) if transpose else (red, out)
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert nat.lib().lf_mx4_linear_tail_parts(T, K, N, transpose, sms) == parts
+    q = quantize_weight(rand(N, K, seed=5, scale=red ** -0.5))
+    v = q.dequantize().double()
+    x = rand(T, red, seed=6)
+    call = mx4_linear_backward if transpose else mx4_linear
+    y = call(x, q)
+    check(y, x, v if transpose else v.t())
+    assert torch.equal(call(x, q), y)
+    whole = torch.empty_like(y)
+    p = nat.Mx4Problem(nat.LF_BF16, T, K, N, transpose, 0, red, x.data_ptr(), q.data.data_ptr())
+    nat.check(nat.lib().lf_mx4_linear(p, whole.data_ptr(), None, 0, nat.raw_stream(0)), "lf_mx4_linear")
+    torch.cuda.synchronize()
+    check(whole, x, v if transpose else v.t())
+    assert nat.device_error() == 0
