@@ -90,8 +90,9 @@ class AdapterDropout:
     ``0 <= rate < 1``, taken to the nearest multiple of 1/65536 (and then below 1; float16 calls take rates up to
     63/64).  ``seed`` and ``offset``, ``0 .. 2**64 - 1``, choose the mask: element ``(t, k)`` of ``x`` is dropped by a
     number that depends on seed, offset, ``t`` and ``k`` alone (Philox 4x32-10), so the forward and the backward that
-    get the same object agree on it and nothing of it is stored.  Take another offset for every step and every
-    projection whose mask should be its own.
+    get the same object agree on it and nothing of it is stored.  ``t`` is the row's number in the call.  Take another
+    offset for every step and every projection whose mask should be its own (:meth:`at`), and on every GPU that has
+    rows of the batch (``sharding.local_dropout``).
     """
 
     rates: float | Mapping[int, float]
@@ -106,6 +107,13 @@ class AdapterDropout:
         many = isinstance(self.rates, Mapping)
         thresholds = {a: self._threshold(r) for a, r in self.rates.items()} if many else self._threshold(self.rates)
         object.__setattr__(self, "_thresholds", thresholds)  # the rates as they are now
+
+    def at(self, offset: int) -> "AdapterDropout":
+        """The same rates and seed with another offset."""
+        out = AdapterDropout(0.0, self.seed, offset)
+        object.__setattr__(out, "rates", self.rates)
+        object.__setattr__(out, "_thresholds", self._thresholds)
+        return out
 
     @staticmethod
     def _threshold(rate: float) -> int:

@@ -15,6 +15,8 @@ the op needs to run one process per GPU:
   assignment without communicating.
 * :func:`local_layout` turns a rank's row ranges into its own fused rows and a
   rebased :class:`TileRoutingConfig`.
+* Dropout in front of the adapters takes :func:`local_dropout` on each rank, so that
+  no two ranks' rows share a mask.
 * The forward needs no communication (base weight replicated, adapters
   resident on every rank).  In the backward, the gradients of adapters whose
   routes land on more than one rank are summed over the ranks: inside the
@@ -32,7 +34,7 @@ from dataclasses import dataclass
 import numpy as np
 import torch
 
-from lorafusion_b200.config import TileRoute, TileRoutingConfig
+from lorafusion_b200.config import AdapterDropout, TileRoute, TileRoutingConfig
 
 TILE_PAIR_ROWS = 256  # rows of one CTA-pair tile of the fused GEMM
 
@@ -136,6 +138,18 @@ def local_layout(plan: ShardPlan, bins: list[list[tuple[int, int]]], rank: int, 
                 routes.append(TileRoute(cur + lo - s0, cur + hi - s0, a))
         cur += e0 - s0
     return rows, TileRoutingConfig(tile_size=tile_size, routes=routes)
+
+
+def local_dropout(dropout: AdapterDropout, plan: ShardPlan, rank: int) -> AdapterDropout:
+    """``dropout`` for one rank's rows of a batch: the same rates and seed, an offset of the rank's own.
+
+    A mask goes by the row's number in its call, which starts at 0 on every rank: with one offset the ranks would drop
+    the same elements of their rows.  The offsets ``offset * world_size + rank`` of different ranks, and of
+    different offsets, never meet; forward and backward of a rank take the same result.
+    """
+    if not 0 <= rank < plan.world_size:
+        raise ValueError(f"rank must be 0 .. {plan.world_size - 1}, got {rank}")
+    return dropout.at(dropout.offset * plan.world_size + rank)
 
 
 def allreduce_spanning_grads(plan: ShardPlan, grad_a: dict[int, torch.Tensor], grad_b: dict[int, torch.Tensor],
