@@ -1267,7 +1267,7 @@ __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
         if (prm.lora && un.last)
           n_lora = (ld_early(tb.base + tb.off_pair_lora + mp + 1) - ld_early(tb.base + tb.off_pair_lora + mp)) *
                    prm.s_planes;
-        if (!mbar_wait(&tempty[buf], ((it >> 1) & 1) ^ 1, abort_flag, tb.err, kErrTimeoutAcc)) {
+        if (!mbar_wait<true>(&tempty[buf], ((it >> 1) & 1) ^ 1, abort_flag, tb.err, kErrTimeoutAcc)) {
           ok = false;
           break;
         }

@@ -19,3 +19,12 @@ def test_arrivals_at_another_cta_are_released_at_cluster_scope():
             found += 1
             assert ".release.cluster." in m.group(), f"{name}: {m.group()}"
     assert found
+
+
+def test_barriers_that_another_cta_arrives_at_are_acquired_at_cluster_scope():
+    """In the CTA-pair kernel: `full` where the odd CTA's decoded tiles are reported, `tempty` of both CTAs' epilogues."""
+    text = sources()["lf_tc.cu"]
+    text = text[text.index("tc_gemm_pair_kernel(const __grid_constant__"):]
+    text = text[:text.index("\n}\n")]
+    waits = re.findall(r"mbar_wait\w*(<\w+>)?\(&(full|tempty)\[", text)
+    assert sorted(waits) == [("<kMx4>", "full"), ("<kMx4>", "full"), ("<true>", "tempty")]
