@@ -402,6 +402,15 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar_cluster) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster) : "memory");
 }
 
+// The same where all that the other CTA's thread has to see is in this CTA's shared memory: a release at cluster scope that
+// orders nothing else, and so does not wait for what is on its way to memory (about 0.8 us).
+__device__ __forceinline__ void mbar_arrive_cluster_smem(uint32_t bar_cluster) {
+  asm volatile(
+      "fence.release.sync_restrict::shared::cta.cluster;\n\t"
+      "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar_cluster)
+      : "memory");
+}
+
 // ---------------------------------------------------------------- clusters
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

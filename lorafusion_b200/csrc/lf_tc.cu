@@ -402,12 +402,7 @@ constexpr int kMx4CodeBytes = kMx4Slots * kMx4Block;
 // A decoding group waits on a slot only once the slot's use before, another group's, is over: the stage that the group
 // filled two uses ago was free by then, so everything kMx4PairStages before that has been used.
 static_assert(kMx4Slots >= kMx4PairStages + 2, "a slot's parity is unambiguous");
-constexpr int kMx4Reporters = 3;
-constexpr int kMx4Reports = 6;
-// A reporter waits on a report only once the one before in the same place, its own, has been passed on; and a place
-// is used again only after the stage that it stood for has been consumed.
-static_assert(kMx4Reports % kMx4Reporters == 0 && kMx4Reports >= kMx4PairStages, "a report's parity is unambiguous");
-constexpr int kMx4BarBytes = (2 * kMx4Slots + kMx4Reports) * 8;
+constexpr int kMx4BarBytes = 2 * kMx4Slots * 8;
 constexpr int kMx4PairSmem = 1024 + kMx4PairStages * (kPairABytes + kPairBBytes) + kPairOutBytes + kMx4CodeBytes +
                              kPairBarBytes + kPairEntBytes + kMx4BarBytes;
 static_assert(kMx4PairSmem <= 227 * 1024, "pair kernel shared memory");
@@ -865,23 +860,21 @@ __device__ __forceinline__ void pair_shrink_role(const PairParams& prm, const CU
 // for x V^T, for g V (kQMN) two panels of 64 columns by 64 rows.  The codes of a stage are two pieces that one more warp
 // copies into a ring of their own, kMx4Slots stages ahead.  (Loaded by the decoding warps themselves they were waited for
 // at every fence: 0.8 us a stage.)  Two groups of four warps take the stages in turn, so that one decodes while the
-// other waits or stores.  A warp decodes its rows, waits for the stage to be free, stores the values and reports: in the
-// even CTA to the `full` barrier, whose phase also counts the P tiles' bytes.  The odd CTA's warps report to a barrier of
-// their own CTA; a reporter, a thread with nothing else in flight, acquires that and arrives once on the even CTA's
-// `full` for all of them, released at cluster scope, as the MMA thread acquires it.  Such a release takes about 0.8 us, twice
-// a stage's time, so three reporters take the stages in turn: 4096 x 4096 -> 4096 takes 201 us with one of them, 136
-// with two, 132 with three or four; 144 with one that releases at once whatever has been reported.  LoRA stages are filled by
-// copies alone; the warps report them unseen.  The dense kernel takes 100 us.  (When the warps arrived across at CTA scope,
-// which orders nothing for a thread of another CTA, it was 125, alone 119, and of that 101 without storing values and 109
-// storing the codes as they are.)
+// other waits or stores.  A warp decodes its rows, waits for the stage to be free, stores the values and reports to the
+// even CTA's `full` barrier, whose phase also counts the P tiles' bytes.  The report is a release at cluster scope, as the
+// MMA thread acquires it, restricted to shared memory: an unrestricted one waits about 0.8 us for what is on its way to
+// memory, twice a stage's time (4096 x 4096 -> 4096 took 201 us with one thread of the odd CTA that reports for its
+// warps, 132 with three that take turns; 127 now.  Arrivals at CTA scope, which order nothing for a thread of
+// another CTA, took 125).  LoRA stages are filled by copies alone; the warps report them unseen.
+// The dense kernel takes 100 us.  Of the 119 that a call alone took at CTA scope, 101 were left without storing values, 109
+// when codes were stored as they are.
 constexpr int kMx4Warps = 8;
 constexpr int kMx4CodeWarp = kThreads / 32 + kMx4Warps;
-constexpr int kMx4Threads = 32 * (kMx4CodeWarp + 1 + kMx4Reporters - 1);  // (warp 1 is a reporter too)
+constexpr int kMx4Threads = 32 * (kMx4CodeWarp + 1);
 
 struct Mx4Ring {
   uint8_t* slots;
   uint64_t *full, *empty;
-  uint64_t* decoded;  // kMx4Reports of the odd CTA: the values of a stage, one after another, are written
 };
 
 template <bool kQMN>
@@ -930,23 +923,22 @@ __device__ __forceinline__ void pair_codes_role(const PairParams& prm, const Pai
 
 template <int kStages, typename OutT>
 __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const PairSched& sched, int pair, int n_pairs,
-                                                 int n_units, int nkb, int crank, uint8_t* sB, uint64_t* full,
-                                                 uint64_t* empty, const Mx4Ring& ring, volatile int* abort_flag) {
+                                                 int n_units, int nkb, uint8_t* sB, uint32_t full_lead, uint64_t* empty,
+                                                 const Mx4Ring& ring, volatile int* abort_flag) {
   const int w = (threadIdx.x >> 5) - kThreads / 32, lane = threadIdx.x & 31;
   const Tables& tb = prm.tb;
   const int group = w >> 2;
   const int row = (w & 3) * 32 + lane;  // of the stage: rows 0..63 of the first piece, then of the second
   uint8_t* dst = sB + row * 128;
-  int stage = 0, slot = 0, turn = 0, place = 0;
+  int stage = 0, slot = 0, turn = 0;
   uint32_t phase = 0, slot_phase = 0;
   bool ok = true;
   auto report = [&]() {
     __syncwarp();
-    if (lane == 0) mbar_arrive(crank ? &ring.decoded[place] : &full[stage]);
+    if (lane == 0) mbar_arrive_cluster_smem(full_lead + static_cast<uint32_t>(stage * 8));
   };
   auto next_stage = [&]() {
     turn ^= 1;
-    if (++place == kMx4Reports) place = 0;
     if (++stage == kStages) {
       stage = 0;
       phase ^= 1;
@@ -990,37 +982,6 @@ __device__ __forceinline__ void pair_decode_role(const PairParams& prm, const Pa
   }
 }
 
-// One of the odd CTA's reporters: every kMx4Reporters-th report of its decoding warps, to the even CTA.
-template <int kStages>
-__device__ __forceinline__ void pair_report_role(const PairParams& prm, const PairSched& sched, int pair, int n_pairs,
-                                                 int n_units, int nkb, int mine, uint32_t full_lead, const Mx4Ring& ring,
-                                                 volatile int* abort_flag) {
-  const Tables& tb = prm.tb;
-  int64_t total = 0;
-  for (int k = 0; k < n_units; ++k) {
-    const PairUnit un = pair_unit(prm, sched, pair, n_pairs, k, nkb);
-    total += un.kb1 - un.kb0;
-    if (prm.lora && un.last) {
-      const int n_lora = (tb.pair_lora(un.mp + 1) - tb.pair_lora(un.mp)) * prm.s_planes;
-      total += (n_lora + prm.lora_per_stage - 1) / prm.lora_per_stage;
-    }
-  }
-  int stage = mine, at = mine;
-  uint32_t phase = 0;
-  static_assert(kMx4Reporters <= kStages, "one step back");
-  for (int64_t i = mine; i < total; i += kMx4Reporters) {
-    if (!mbar_wait_stage(&ring.decoded[at], phase, abort_flag, tb.err, kErrTimeoutFull)) return;
-    mbar_arrive_cluster(full_lead + static_cast<uint32_t>(stage * 8));
-    stage += kMx4Reporters;
-    if (stage >= kStages) stage -= kStages;
-    at += kMx4Reporters;
-    if (at >= kMx4Reports) {
-      at -= kMx4Reports;
-      phase ^= 1;
-    }
-  }
-}
-
 // kDelta: a float32 matrix is added to the product (prm.delta).
 // kMx4: Q is held in 4 bits (prm.mx4) and decoded on the way into shared memory; map_q is not used.
 // kDrop: the co-scheduled shrink's input is masked (prm.drop), by warps that a kMx4 kernel has and others get for it.
@@ -1058,9 +1019,8 @@ __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
   uint64_t* rpub = rdrain + 1;
   uint64_t* tail_bar = reinterpret_cast<uint64_t*>(bars + kPairTailBarOff);
   int* pair_ent = reinterpret_cast<int*>(bars + kPairBarBytes);
-  Mx4Ring codes{sOut + kPairOutBytes, reinterpret_cast<uint64_t*>(bars + kPairBarBytes + kPairEntBytes), nullptr, nullptr};
+  Mx4Ring codes{sOut + kPairOutBytes, reinterpret_cast<uint64_t*>(bars + kPairBarBytes + kPairEntBytes), nullptr};
   codes.empty = codes.full + kMx4Slots;
-  codes.decoded = codes.empty + kMx4Slots;
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (static_cast<int>(blockIdx.x) < 2 * prm.n_shrink_pairs) {
@@ -1081,8 +1041,7 @@ __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      // half of a CTA's warps decode a stage; the odd CTA's are one arrival
-      mbar_init(&full[s], kMx4 ? 1 + kMx4Warps / 2 + 1 : 1);
+      mbar_init(&full[s], kMx4 ? 1 + kMx4Warps : 1);  // half of the warps of each CTA decode a stage
       mbar_init(&empty[s], 1);
     }
     for (int b = 0; b < 2; ++b) {
@@ -1095,8 +1054,6 @@ __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
         mbar_init(&codes.full[i], 1);
         mbar_init(&codes.empty[i], kMx4Warps / 2);
       }
-    if (kMx4)
-      for (int i = 0; i < kMx4Reports; ++i) mbar_init(&codes.decoded[i], kMx4Warps / 2);
     mbar_init(drain, 1);
     *abort_flag = 0;
     fence_mbar_init();
@@ -1328,21 +1285,14 @@ __global__ void __launch_bounds__(pair_threads(kMx4, kDrop), 1)
         drain_wait(drain, 0, tb.err);
       }
     }
-    if (kMx4 && lane == 0 && crank == 1)
-      pair_report_role<kStages>(prm, sched, pair, n_pairs, n_units, nkb, 0, full_lead, codes, abort_flag);
     __syncwarp();
   } else if (!kMx4 && kDrop && warp >= kThreads / 32) {
     // nothing to mask in a GEMM pair
   } else if (kMx4 && warp >= kThreads / 32) {
-    if (warp > kMx4CodeWarp) {
-      if (lane == 0 && crank == 1)
-        pair_report_role<kStages>(prm, sched, pair, n_pairs, n_units, nkb, warp - kMx4CodeWarp, full_lead, codes, abort_flag);
-      __syncwarp();
-    } else if (warp == kMx4CodeWarp)
+    if (warp == kMx4CodeWarp)
       pair_codes_role<kQMN>(prm, sched, pair, n_pairs, n_units, nkb, static_cast<int>(crank), codes, abort_flag);
     else
-      pair_decode_role<kStages, OutT>(prm, sched, pair, n_pairs, n_units, nkb, static_cast<int>(crank), sB, full, empty, codes,
-                                      abort_flag);
+      pair_decode_role<kStages, OutT>(prm, sched, pair, n_pairs, n_units, nkb, sB, full_lead, empty, codes, abort_flag);
   } else {
     const int q = warp & 3;
     int it = 0;
