@@ -32,7 +32,8 @@ class MX4Weight:
     ``data`` is its only tensor: uint8, in an order of its own that goes with ``dtype``, to be saved and restored as it is
     (``MX4Weight(data, out_features, in_features, dtype)``).  ``dtype`` (bfloat16 or float16) is that of the weight it was
     made from and of the activations it is multiplied with.  Its products read ``data`` on their stream: keep it
-    unchanged until they have run.
+    unchanged until they have run.  Another tensor of the same bytes may be put in its place (``weight.data = saved``);
+    the sizes and the dtype are fixed.
     """
 
     def __init__(self, data: torch.Tensor, out_features: int, in_features: int, dtype: torch.dtype):
@@ -40,15 +41,22 @@ class MX4Weight:
             raise ValueError(f"a weight in 4 bits serves bfloat16 or float16, not {dtype}")
         if not (0 < out_features <= _MAX and 0 < in_features <= _MAX):
             raise ValueError(f"out_features and in_features must be 1 .. {_MAX}, got {out_features}, {in_features}")
-        if data.device.type != "cuda":
-            raise ValueError("data must be a CUDA tensor: lorafusion_b200 has no CPU path")
-        need = nat.lib().lf_mx4_bytes(out_features, in_features)
-        if data.dtype is not torch.uint8 or data.shape != (need,) or not data.is_contiguous() or data.data_ptr() % 16:
-            raise ValueError(f"data must be a contiguous, 16-byte aligned uint8 tensor of shape ({need},), got "
-                             f"{data.dtype} {tuple(data.shape)}")
-        self.data = data
         self.out_features, self.in_features = out_features, in_features
         self.dtype = dtype
+        self.data = data
+
+    def __setattr__(self, name: str, value) -> None:
+        # the kernels go by the sizes: what they read has to hold them
+        if name == "data":
+            if value.device.type != "cuda":
+                raise ValueError("data must be a CUDA tensor: lorafusion_b200 has no CPU path")
+            need = nat.lib().lf_mx4_bytes(self.out_features, self.in_features)
+            if value.dtype is not torch.uint8 or value.shape != (need,) or not value.is_contiguous() or value.data_ptr() % 16:
+                raise ValueError(f"data must be a contiguous, 16-byte aligned uint8 tensor of shape ({need},), got "
+                                 f"{value.dtype} {tuple(value.shape)}")
+        elif name in ("out_features", "in_features", "dtype") and name in self.__dict__:
+            raise AttributeError(f"the {name} of a weight in 4 bits is fixed")
+        object.__setattr__(self, name, value)
 
     @property
     def shape(self) -> torch.Size:
@@ -88,7 +96,8 @@ def quantize_weight(weight: torch.Tensor) -> MX4Weight:
                              "first)")
         data = nat.glue().mx4_quantize(weight.detach().contiguous(), code)
     out = MX4Weight.__new__(MX4Weight)
-    out.data, (out.out_features, out.in_features), out.dtype = data, weight.shape, weight.dtype
+    N, K = weight.shape
+    out.__dict__.update(data=data, out_features=N, in_features=K, dtype=weight.dtype)
     return out
 
 
