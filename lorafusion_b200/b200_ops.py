@@ -28,6 +28,7 @@ of adapters stay ahead of the GPU.
 from __future__ import annotations
 
 import ctypes
+import threading
 import warnings
 import weakref
 from collections import OrderedDict
@@ -53,7 +54,7 @@ class CudaCorePathWarning(UserWarning):
 _WARNED_SHAPES: set = set()
 
 
-def _warn_if_cuda_core(dtype, K: int, N: int, tensors) -> None:
+def _warn_if_cuda_core(dtype, K: int, N: int, tensors, stacklevel: int = 3) -> None:
     """Warn once per (dtype, K, N) when a bf16/f16 call must run on CUDA cores: TMA needs K and N
     multiples of 8 and every buffer 16-byte aligned (the same test the library makes)."""
     if dtype == torch.float32:
@@ -66,10 +67,13 @@ def _warn_if_cuda_core(dtype, K: int, N: int, tensors) -> None:
         _WARNED_SHAPES.add(key)
         warnings.warn(f"{dtype} problem with in_features={K}, out_features={N} runs on the CUDA-core path: the "
                       "tensor-core path needs both to be multiples of 8 and 16-byte aligned buffers",
-                      CudaCorePathWarning, stacklevel=3)
+                      CudaCorePathWarning, stacklevel=stacklevel)
 
 
 # --------------------------------------------------------------------------- caches
+# Held by every call while it looks things up in the caches, fills them and enqueues its launches: calls of several threads
+# take turns on the host.
+_LOCK = threading.RLock()
 _ROUTE_CACHE: dict[int, "_Routes"] = {}
 # adapter records by (slots, id of the first A, id of the first B), least recently used first; a
 # model calls the op with one routing and many adapter sets (layers x projections), so every set
@@ -110,20 +114,22 @@ def use_cooperative_launch(enabled: bool, shrink_prologue: bool = False) -> None
 def clear_weight_cache() -> None:
     """Drop every cached table, packed adapter slab and converted weight.  What captured calls read stays for as long as
     their graphs live."""
-    _ROUTE_CACHE.clear()
-    _ADAPTER_CACHE.clear()
-    _PLAN_BY_CONTENT.clear()
-    _SAVED_SF.clear()
-    _WEIGHT_CACHE.clear()
-    _drop_ended()
+    with _LOCK:
+        _ROUTE_CACHE.clear()
+        _ADAPTER_CACHE.clear()
+        _PLAN_BY_CONTENT.clear()
+        _SAVED_SF.clear()
+        _WEIGHT_CACHE.clear()
+        _drop_ended()
 
 
 def release() -> None:
     """Drop every host cache (``clear_weight_cache``) and what the library holds on the devices
     (``lf_release``: the host-streamed forward's events); later calls rebuild what they need."""
-    clear_weight_cache()
-    _SIDE_STREAMS.clear()
-    nat.check(nat.lib().lf_release(), "lf_release")
+    with _LOCK:
+        clear_weight_cache()
+        _SIDE_STREAMS.clear()
+        nat.check(nat.lib().lf_release(), "lf_release")
 
 
 def last_launch_count() -> int:
@@ -227,8 +233,8 @@ class _Made:
         self.event.record(stream)
         self.others: set = set()  # streams that have waited
 
-    def use(self, device, captured: int) -> None:
-        raw = nat.raw_stream(device.index)
+    def use(self, device, at) -> None:
+        raw, captured = at
         if captured:  # replays may run on any stream
             nat.glue().wait_event(self.event.cuda_event)
         elif raw != self.stream and raw not in self.others:
@@ -313,10 +319,10 @@ def _drop_ended() -> None:
                 del _SAVED_SF[k]
 
 
-def _capture(device) -> int:
-    """The capture into a CUDA graph that the device's current stream is in, 0 for none."""
+def _at(device) -> tuple[int, int]:
+    """The device's current stream, and the capture into a CUDA graph that it is in (0: none)."""
     _drop_ended()
-    return nat.glue().capture_id(device.index)
+    return nat.glue().at(device.index)
 
 
 def _hold(captured: int, device, *read) -> None:
@@ -330,19 +336,18 @@ def _hold(captured: int, device, *read) -> None:
 def _building(what: str, device) -> None:
     """Refuses to fill a cache within a capture: nothing runs there, so later calls would find it empty, and replays would
     fill it again from host memory that is gone by then."""
-    if _capture(device):
+    if nat.glue().at(device.index)[1]:
         raise RuntimeError(f"{what} would be made within a CUDA graph capture: make the same call once before it")
 
 
-def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, captured: int,
-          drop=None) -> _Plan:
-    """The routing's tables for this adapter set and, with ``drop``, its factors and thresholds."""
+def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device, at, drop=None) -> _Plan:
+    """The routing's tables for this adapter set and, with ``drop``, its factors and thresholds (``at``: ``_at(device)``)."""
     ranks, scales, thresholds = aset.ranks, aset.scales, None
     if drop is not None:
         scales, thresholds = drop.scales(scales), drop.thresholds
     for pr, ps, pt, pd, plan in rts.plans:
         if pd == device and pr == ranks and ps == scales and pt == thresholds:
-            plan.made.use(device, captured)
+            plan.made.use(device, at)
             return plan
     if any(r <= 0 for r in ranks):
         bad = rts.slots[next(i for i, r in enumerate(ranks) if r <= 0)]
@@ -358,7 +363,7 @@ def _plan(rts: _Routes, aset: _AdapterSet, total_rows: int, device: torch.device
             _PLAN_BY_CONTENT.clear()
         _PLAN_BY_CONTENT[content] = plan
     else:
-        plan.made.use(device, captured)
+        plan.made.use(device, at)
     rts.plans.insert(0, (ranks, scales, thresholds, device, plan))
     del rts.plans[4:]
     return plan
@@ -378,8 +383,7 @@ def _build_plan(rts: _Routes, ranks, scales, thresholds, total_rows: int, device
     return _Plan(info, table_dev, rts.slots, ranks, table_dev.data_ptr() + 4 * words)
 
 
-def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, captured: int,
-          backward: bool) -> dict:
+def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, device, at, backward: bool) -> dict:
     """Zero-padded adapter slabs in the layouts the kernels read (cached in the adapter record)."""
     key = (dtype, K, N, device, plan.info.r_pad)
     entry = aset.packs.get(key)
@@ -404,7 +408,7 @@ def _pack(plan: _Plan, aset: _AdapterSet, dtype: torch.dtype, K: int, N: int, de
             b_src.append(b if b.is_contiguous() else b.contiguous())
         entry = aset.packs[key] = {"src": (a_src, b_src)}
     for made in entry.get("made", ()):
-        made.use(device, captured)
+        made.use(device, at)
     missing = [w for w in want if w not in entry]
     if missing:
         _fill_packs(entry, plan, dtype, K, N, device, missing)
@@ -446,7 +450,7 @@ def _fill_packs(entry, plan: _Plan, dtype, K, N, device, which) -> None:
         entry.setdefault("ptr_bufs", []).append((ptrs, ranks_dev))
 
 
-def _weight(base_weight: torch.Tensor, dtype, device, captured: int) -> torch.Tensor:
+def _weight(base_weight: torch.Tensor, dtype, device, at) -> torch.Tensor:
     """Base weight as a contiguous tensor of the activation dtype (converted copies cached)."""
     if isinstance(base_weight, MX4Weight):
         raise ValueError("this call takes a dense base_weight (MX4Weight.dequantize)")
@@ -459,7 +463,7 @@ def _weight(base_weight: torch.Tensor, dtype, device, captured: int) -> torch.Te
     if hit is not None:
         ref, ptr, ver, conv, made = hit
         if ref() is base_weight and ptr == base_weight.data_ptr() and ver == base_weight._version:
-            made.use(device, captured)
+            made.use(device, at)
             return conv
     _building("a copy of base_weight", device)
     conv = base_weight.to(dtype).contiguous()
@@ -496,11 +500,11 @@ def _problem(code, T, K, N, x, w, packs) -> nat.Problem:
     return p
 
 
-def _base(base_weight, x: torch.Tensor, captured: int):
+def _base(base_weight, x: torch.Tensor, at):
     """(tensor that holds the base weight, whether it is the data of one in 4 bits).  A problem the tensor-core path
     cannot address takes a dense copy of a weight in 4 bits, made within the call."""
     if not isinstance(base_weight, MX4Weight):
-        return _weight(base_weight, x.dtype, x.device, captured), False
+        return _weight(base_weight, x.dtype, x.device, at), False
     if base_weight.dtype is not x.dtype:
         raise ValueError(f"x ({x.dtype}) must have the dtype of the weight in 4 bits ({base_weight.dtype})")
     if base_weight.device != x.device:
@@ -569,6 +573,11 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     A call can be captured into a CUDA graph once the same call has run (``RuntimeError`` before): replays read x and the
     base weight as they are then, repeat the mask, and keep the adapters' values of the capture.
     """
+    with _LOCK:
+        return _forward(x, base_weight, lora_a, lora_b, adapters, routing, dropout)
+
+
+def _forward(x, base_weight, lora_a, lora_b, adapters, routing, dropout) -> torch.Tensor:
     global _last_launches
     rts = _routes(routing, x.shape[0])
     _last_launches = 0
@@ -581,16 +590,16 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     code = _DTYPE_CODE[dtype]
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    captured = _capture(device)
-    w, mx4 = _base(base_weight, x, captured)
+    at = stream, captured = _at(device)
+    w, mx4 = _base(base_weight, x, at)
     if mx4 and x.data_ptr() % 16:
         x = x.detach().clone()
-    plan = _plan(rts, aset, T, device, captured, drop)
-    packs = _pack(plan, aset, dtype, K, N, device, captured, backward=False)
+    plan = _plan(rts, aset, T, device, at, drop)
+    packs = _pack(plan, aset, dtype, K, N, device, at, backward=False)
     y = torch.empty((T, N), dtype=dtype, device=device)
     if T == 0 or N == 0:
         return y
-    _warn_if_cuda_core(dtype, K, N, (x, w, y))
+    _warn_if_cuda_core(dtype, K, N, (x, w, y), 4)
     L = nat.lib()
     info = ctypes.byref(plan.info)
     # S_ext and flags in one buffer (kept for the backward), the K-split tail's scratch in another
@@ -600,7 +609,6 @@ def fused_lora_forward(x, base_weight, lora_a, lora_b, adapters, routing, *,
     tail = torch.empty(max(int(L.lf_forward_workspace_bytes(info, code)) - fixed, 256), dtype=torch.uint8,
                        device=device)
     prob = _problem(code, T, K, N, x, w, packs)
-    stream = nat.raw_stream(device.index)
     planes = ctypes.c_int32(0)
     opt, keep = _options(mx4, drop, plan, prob, False, device)
     with nat.on_device(device.index):
@@ -677,10 +685,10 @@ class PreparedForward:
         dtype = self.x.dtype
         self.dtype = dtype
         aset = _adapters(rts, lora_a, lora_b, adapters)
-        captured = _capture(self.device)
-        self.w = _weight(base_weight, dtype, self.device, captured)
-        self.plan = _plan(rts, aset, self.T, self.device, captured)
-        self.packs = _pack(self.plan, aset, dtype, self.K, self.N, self.device, captured, backward=False)
+        at = _at(self.device)
+        self.w = _weight(base_weight, dtype, self.device, at)
+        self.plan = _plan(rts, aset, self.T, self.device, at)
+        self.packs = _pack(self.plan, aset, dtype, self.K, self.N, self.device, at, backward=False)
         code = _DTYPE_CODE[dtype]
         L = nat.lib()
         ws_bytes = L.lf_forward_workspace_bytes(ctypes.byref(self.plan.info), code)
@@ -704,7 +712,8 @@ class PreparedForward:
 
 def prepare_forward(x, base_weight, lora_a, lora_b, adapters, routing) -> PreparedForward:
     """Resolve a forward call once (see :class:`PreparedForward`)."""
-    return PreparedForward(x, base_weight, lora_a, lora_b, adapters, routing)
+    with _LOCK:
+        return PreparedForward(x, base_weight, lora_a, lora_b, adapters, routing)
 
 
 def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, *, grad_dtype=None,
@@ -723,6 +732,11 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     ``base_weight`` and ``dropout`` as in :func:`fused_lora_forward`: with the forward's ``dropout`` these are the
     gradients of its result, ``grad_x = g W + m (s_i / (1 - p_i) g B_i A_i)``.
     """
+    with _LOCK:
+        return _backward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, grad_dtype, peer, dropout)
+
+
+def _backward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, grad_dtype, peer, dropout):
     global _last_launches
     rts = _routes(routing, x.shape[0])
     _last_launches = 0
@@ -743,14 +757,14 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
         raise ValueError(f"grad_dtype must be None, x.dtype or torch.float32, got {grad_dtype}")
     drop = _drop(dropout, rts, dtype)
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    captured = _capture(device)
+    at = stream, captured = _at(device)
     if captured and peer is not None:  # every call numbers its blocks; replays would repeat the number
         raise RuntimeError("a call with peer cannot be captured into a CUDA graph")
-    w, mx4 = _base(base_weight, x, captured)
+    w, mx4 = _base(base_weight, x, at)
     if mx4:
         x, g = (t.detach().clone() if t.data_ptr() % 16 else t for t in (x, g))
-    plan = _plan(rts, aset, T, device, captured, drop)
-    packs = _pack(plan, aset, dtype, K, N, device, captured, backward=True)
+    plan = _plan(rts, aset, T, device, at, drop)
+    packs = _pack(plan, aset, dtype, K, N, device, at, backward=True)
     info = plan.info
     rtot = info.rank_total
     ext = _peer_layout(plan, peer, device) if peer is not None else None
@@ -758,12 +772,11 @@ def fused_lora_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, rout
     grad_x = torch.empty((T, K), dtype=dtype, device=device)
     ga_flat = torch.empty(max(rows * K, 1), dtype=gdt, device=device)
     gb_flat = torch.empty(max(rows * N, 1), dtype=gdt, device=device)
-    _warn_if_cuda_core(dtype, K, N, (x, w, g, grad_x))
+    _warn_if_cuda_core(dtype, K, N, (x, w, g, grad_x), 4)
     L = nat.lib()
     ws_bytes = L.lf_backward_workspace_bytes(ctypes.byref(info), code)
     ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=device)
     prob = _problem(code, T, K, N, x, w, packs)
-    stream = nat.raw_stream(device.index)
     saved = _saved_sf(x_in, rts, plan, aset, captured) if dtype != torch.float32 and drop is None else None
     sf_ptr, sf_planes = (saved[0].data_ptr(), saved[1]) if saved is not None else (None, 0)
     # S_f from the forward on these inputs, when there was one: no second s x A^T shrink
@@ -875,10 +888,10 @@ class PreparedBackward:
         if gdt not in (dtype, torch.float32):
             raise ValueError(f"grad_dtype must be None, x.dtype or torch.float32, got {grad_dtype}")
         aset = _adapters(rts, lora_a, lora_b, adapters)
-        captured = _capture(self.device)
-        self.w = _weight(base_weight, dtype, self.device, captured)
-        self.plan = _plan(rts, aset, T, self.device, captured)
-        self.packs = _pack(self.plan, aset, dtype, K, N, self.device, captured, backward=True)
+        at = _at(self.device)
+        self.w = _weight(base_weight, dtype, self.device, at)
+        self.plan = _plan(rts, aset, T, self.device, at)
+        self.packs = _pack(self.plan, aset, dtype, K, N, self.device, at, backward=True)
         code = _DTYPE_CODE[dtype]
         self.gcode = _DTYPE_CODE[gdt]
         rtot = self.plan.info.rank_total
@@ -903,7 +916,8 @@ class PreparedBackward:
 
 def prepare_backward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, grad_dtype=None) -> PreparedBackward:
     """Resolve a backward call once (see :class:`PreparedBackward`)."""
-    return PreparedBackward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, grad_dtype)
+    with _LOCK:
+        return PreparedBackward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, grad_dtype)
 
 
 def _grad_dicts(plan: _Plan, ga_flat, gb_flat, K: int, N: int):
@@ -997,11 +1011,11 @@ def _chunk_bounds(total_rows: int, chunk_rows: int) -> list[int]:
 
 
 def _chunk_plans(rts: _Routes, aset: _AdapterSet, total_rows: int, chunk_rows: int, device, code: int,
-                 captured: int) -> _ChunkPlans:
+                 at) -> _ChunkPlans:
     key = (chunk_rows, total_rows, aset.ranks, aset.scales, device, code)
     for k, v in rts.chunk_plans:
         if k == key:
-            v.made.use(device, captured)
+            v.made.use(device, at)
             return v
     _building("the chunks' tables", device)
     plans = _ChunkPlans(rts, aset.ranks, aset.scales, total_rows, chunk_rows, device, code)
@@ -1026,6 +1040,11 @@ def fused_lora_forward_host(x_host, base_weight, lora_a, lora_b, adapters, routi
     for: synchronize the current stream before reading the result.  No counterpart in the
     reference (its ops take device tensors).
     """
+    with _LOCK:
+        return _forward_host(x_host, base_weight, lora_a, lora_b, adapters, routing, out, chunk_rows)
+
+
+def _forward_host(x_host, base_weight, lora_a, lora_b, adapters, routing, out, chunk_rows):
     global _last_launches
     rts = _routes(routing, x_host.shape[0])
     if isinstance(base_weight, MX4Weight):
@@ -1053,11 +1072,11 @@ def fused_lora_forward_host(x_host, base_weight, lora_a, lora_b, adapters, routi
         x_host = x_host.contiguous()
     code = _DTYPE_CODE[dtype]
     aset = _adapters(rts, lora_a, lora_b, adapters)
-    captured = _capture(device)
-    w = _weight(base_weight, dtype, device, captured)
-    plan = _plan(rts, aset, T, device, captured)
-    packs = _pack(plan, aset, dtype, K, N, device, captured, backward=False)
-    chunks = _chunk_plans(rts, aset, T, chunk_rows, device, code, captured)
+    at = _at(device)
+    w = _weight(base_weight, dtype, device, at)
+    plan = _plan(rts, aset, T, device, at)
+    packs = _pack(plan, aset, dtype, K, N, device, at, backward=False)
+    chunks = _chunk_plans(rts, aset, T, chunk_rows, device, code, at)
     x_dev = torch.empty((T, K), dtype=dtype, device=device)
     y_dev = torch.empty((T, N), dtype=dtype, device=device)
     ws = torch.empty(chunks.ws_bytes, dtype=torch.uint8, device=device)

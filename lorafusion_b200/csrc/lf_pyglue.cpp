@@ -210,22 +210,27 @@ PyObject* mx4_dequantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return THPVariable_Wrap(std::move(w));
 }
 
-// capture_id(device index): the id of the capture into a CUDA graph that the device's current stream is in, 0 for none.
-PyObject* capture_id(PyObject*, PyObject* const* a, Py_ssize_t n) {
+// The capture into a CUDA graph that a stream is in, 0 for none.
+unsigned long long capture_of(cudaStream_t stream) {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (cudaStreamGetCaptureInfo(stream, &status, &id) != cudaSuccess) {
+    (void)cudaGetLastError();  // the legacy stream beside another one's capture: not captured itself
+    status = cudaStreamCaptureStatusNone;
+  }
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
+// at(device index): the device's current stream, and the id of the capture into a CUDA graph that it is in (0: none).
+PyObject* at_stream(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 1) {
-    PyErr_SetString(PyExc_TypeError, "capture_id takes 1 argument");
+    PyErr_SetString(PyExc_TypeError, "at takes 1 argument");
     return nullptr;
   }
   const long dev = PyLong_AsLong(a[0]);
   if (PyErr_Occurred()) return nullptr;
-  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
-  unsigned long long id = 0;
-  if (cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream(), &status,
-                               &id) != cudaSuccess) {
-    (void)cudaGetLastError();  // the legacy stream beside another one's capture: not captured itself
-    status = cudaStreamCaptureStatusNone;
-  }
-  return PyLong_FromUnsignedLongLong(status == cudaStreamCaptureStatusActive ? id : 0);
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(dev)).stream();
+  return Py_BuildValue("(KK)", static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)), capture_of(stream));
 }
 
 // Captures whose graphs are gone, until ended() takes them.  Never destroyed: graphs may outlive the module.
@@ -608,7 +613,7 @@ PyMethodDef methods[] = {
     {"mx4_linear", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_linear>)), METH_FASTCALL, nullptr},
     {"mx4_quantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_quantize>)), METH_FASTCALL, nullptr},
     {"mx4_dequantize", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<mx4_dequantize>)), METH_FASTCALL, nullptr},
-    {"capture_id", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<capture_id>)), METH_FASTCALL, nullptr},
+    {"at", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<at_stream>)), METH_FASTCALL, nullptr},
     {"hold_capture", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<hold_capture>)), METH_FASTCALL, nullptr},
     {"ended", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<ended>)), METH_FASTCALL, nullptr},
     {"wait_event", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(guarded<wait_event>)), METH_FASTCALL, nullptr},

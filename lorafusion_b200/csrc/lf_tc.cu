@@ -17,6 +17,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <mutex>
+
 #include "lf_drop.cuh"
 #include "lf_internal.cuh"
 #include "lf_launch.cuh"
@@ -2469,6 +2471,7 @@ struct SmemOptIn {
 };
 SmemOptIn g_smem_optin[64];
 int g_smem_optin_n = 0;
+std::mutex g_smem_mu;
 
 template <typename K>
 cudaError_t ensure_smem(K kernel, int bytes) {
@@ -2476,6 +2479,7 @@ cudaError_t ensure_smem(K kernel, int bytes) {
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   const void* fn = reinterpret_cast<const void*>(kernel);
+  const std::lock_guard<std::mutex> lk(g_smem_mu);
   for (int i = 0; i < g_smem_optin_n; ++i)
     if (g_smem_optin[i].fn == fn && g_smem_optin[i].dev == dev) return cudaSuccess;
   e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
