@@ -322,10 +322,21 @@ def raw_stream(device_index: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device_index)
 
 
+_current_device = None
+_HERE_ALREADY = nullcontext()
+
+
 def on_device(device_index: int):
-    """Context that makes a device current; nothing to do where it already is."""
+    """Context that makes a device current; nothing to do where it already is.  (CUDA has been initialised: the caller
+    has a tensor there.)"""
+    global _current_device
+    if _current_device is None:
+        import torch
+        _current_device = torch._C._cuda_getDevice
+    if _current_device() == device_index:
+        return _HERE_ALREADY
     import torch
-    return nullcontext() if torch.cuda.current_device() == device_index else torch.cuda.device(device_index)
+    return torch.cuda.device(device_index)
 
 
 def co_scheduling() -> tuple[int, int]:

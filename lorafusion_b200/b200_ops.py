@@ -246,7 +246,7 @@ class _Made:
 
 
 class _Plan:
-    __slots__ = ("info", "table_dev", "slots", "ranks", "vslots", "thresholds", "made")
+    __slots__ = ("info", "table_dev", "slots", "ranks", "vslots", "thresholds", "made", "sizes")
 
     def __init__(self, info, table_dev, slots, ranks, thresholds=0):
         self.info = info
@@ -256,6 +256,16 @@ class _Plan:
         self.vslots = _virtual_slots(ranks)
         self.thresholds = thresholds  # address of the virtual slots' dropout thresholds, behind the table's words
         self.made = _Made(table_dev.device, table_dev)
+        self.sizes: dict = {}  # dtype code -> bytes of a forward's fixed workspace, of its tail's, of a backward's
+
+    def workspace(self, code: int) -> tuple[int, int, int]:
+        sizes = self.sizes.get(code)
+        if sizes is None:
+            L, info = nat.lib(), ctypes.byref(self.info)
+            fixed = int(L.lf_forward_fixed_workspace_bytes(info, code))
+            sizes = self.sizes[code] = (max(fixed, 256), max(int(L.lf_forward_workspace_bytes(info, code)) - fixed, 256),
+                                        max(int(L.lf_backward_workspace_bytes(info, code)), 256))
+        return sizes
 
 
 class _AdapterSet:
@@ -604,10 +614,9 @@ def _forward(x, base_weight, lora_a, lora_b, adapters, routing, dropout) -> torc
     info = ctypes.byref(plan.info)
     # S_ext and flags in one buffer (kept for the backward), the K-split tail's scratch in another
     # (back to the allocator's cache once the launch is enqueued)
-    fixed = int(L.lf_forward_fixed_workspace_bytes(info, code))
-    ws = torch.empty(max(fixed, 256), dtype=torch.uint8, device=device)
-    tail = torch.empty(max(int(L.lf_forward_workspace_bytes(info, code)) - fixed, 256), dtype=torch.uint8,
-                       device=device)
+    fixed, rest, _ = plan.workspace(code)
+    ws = torch.empty(fixed, dtype=torch.uint8, device=device)
+    tail = torch.empty(rest, dtype=torch.uint8, device=device)
     prob = _problem(code, T, K, N, x, w, packs)
     planes = ctypes.c_int32(0)
     opt, keep = _options(mx4, drop, plan, prob, False, device)
@@ -774,8 +783,7 @@ def _backward(grad_out, x, base_weight, lora_a, lora_b, adapters, routing, grad_
     gb_flat = torch.empty(max(rows * N, 1), dtype=gdt, device=device)
     _warn_if_cuda_core(dtype, K, N, (x, w, g, grad_x), 4)
     L = nat.lib()
-    ws_bytes = L.lf_backward_workspace_bytes(ctypes.byref(info), code)
-    ws = torch.empty(max(ws_bytes, 256), dtype=torch.uint8, device=device)
+    ws = torch.empty(plan.workspace(code)[2], dtype=torch.uint8, device=device)
     prob = _problem(code, T, K, N, x, w, packs)
     saved = _saved_sf(x_in, rts, plan, aset, captured) if dtype != torch.float32 and drop is None else None
     sf_ptr, sf_planes = (saved[0].data_ptr(), saved[1]) if saved is not None else (None, 0)
